@@ -1,4 +1,4 @@
-"""ctypes binding of ``libssm_b200.so`` (declarations mirror ``include/ssm_b200.h``).
+"""ctypes binding of ``libssm_b200.so`` (declarations mirror ``include/ssm_b200.h`` and ``include/ssm_b200_lm.h``).
 
 There is no fallback: if the shared library is missing or an entry point is absent the
 import of the operators fails with a clear error, and every call that the library rejects
@@ -141,7 +141,61 @@ class SsdBwdArgs(C.Structure):
     ]
 
 
-# entry point -> (restype, argtypes); every name here is declared in include/ssm_b200.h
+# ---- include/ssm_b200_lm.h -----------------------------------------------------------------
+
+LM_ABI_VERSION = 1  # SSM_B200_LM_ABI_VERSION
+
+
+def _strides(names: str, axes: str) -> list:
+    return [(f"{n}_s{a}", i64) for n in names.split() for a in axes]
+
+
+class GatedDeltaArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("len", i32), ("heads", i32), ("key_heads", i32), ("kdim", i32), ("vdim", i32), ("io_dtype", i32), ("g_dtype", i32),
+        ("beta_dtype", i32), ("final_dtype", i32), ("num_seqs", i32), ("cu_is_64", i32), ("scale", C.c_float), ("reserved0", i32),
+        ("q", vp), ("k", vp), ("v", vp), ("g", vp), ("beta", vp), *_strides("q k v g beta", "bth"),
+        ("cu_seqlens", vp), ("initial_state", fp), ("o", vp), ("final_state", vp), ("table", vp), ("rest", fp), ("states", fp),
+    ]
+
+
+class GatedDeltaBwdArgs(C.Structure):
+    _fields_ = [("fwd", GatedDeltaArgs), ("dout", vp), ("dfinal", fp), ("dq", vp), ("dk", vp), ("dv", vp), ("dg", fp), ("dbeta", fp), ("dinitial", fp),
+                ("dv32", fp), ("dstates", fp), ("dqk", fp)]
+
+
+class GatedDeltaStepArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("heads", i32), ("key_heads", i32), ("kdim", i32), ("vdim", i32), ("io_dtype", i32), ("g_dtype", i32), ("beta_dtype", i32),
+        ("scale", C.c_float), ("reserved0", i32), ("state", fp), ("q", vp), ("k", vp), ("v", vp), ("g", vp), ("beta", vp), *_strides("q k v g beta", "bh"),
+        ("o", vp),
+    ]
+
+
+class TokenLogpArgs(C.Structure):
+    _fields_ = [
+        ("rows", i64), ("row_stride", i64), ("vocab", i32), ("io_dtype", i32), ("top_k", i32), ("reserved0", i32), ("ignore_index", i64),
+        ("temperature", C.c_float), ("reserved1", i32),
+        ("logits", vp), ("targets", vp), ("logp", fp), ("entropy", fp), ("top_logp", fp), ("top_ids", vp), ("stats", fp),
+    ]
+
+
+class TokenLogpBwdArgs(C.Structure):
+    _fields_ = [("fwd", TokenLogpArgs), ("dlogp", fp), ("dentropy", fp), ("dtop_logp", fp), ("dlogits", vp)]
+
+
+class TopkDistillArgs(C.Structure):
+    _fields_ = [
+        ("rows", i64), ("row_stride", i64), ("vocab", i32), ("io_dtype", i32), ("top_k", i32), ("teacher_dtype", i32), ("temperature", C.c_float), ("reserved0", i32),
+        ("logits", vp), ("teacher", vp), ("ids", vp), ("loss", fp), ("stats", fp),
+    ]
+
+
+class TopkDistillBwdArgs(C.Structure):
+    _fields_ = [("fwd", TopkDistillArgs), ("dloss", fp), ("dlogits", vp)]
+
+
+# entry point -> (restype, argtypes); every name here is declared in include/ssm_b200.h or include/ssm_b200_lm.h
 ENTRY_POINTS = {
     "ssm_b200_abi_version": (C.c_int, []),
     "ssm_b200_last_error": (C.c_char_p, []),
@@ -183,6 +237,16 @@ ENTRY_POINTS = {
     "ssm_ssd_fwd": (C.c_int, [C.POINTER(SsdArgs), vp]),
     "ssm_ssd_shard_summary_floats": (C.c_int64, [i32, i32]),
     "ssm_ssd_fold_shards": (C.c_int, [vp, i32, i32, i32, i32, vp, vp, vp]),
+    "ssm_b200_lm_abi_version": (C.c_int, []),
+    "ssm_gated_delta_chunks": (C.c_int64, [i32, i32, i32]),
+    "ssm_gated_delta_table_ints": (C.c_int64, [i32, i32, i32]),
+    "ssm_gated_delta_fwd": (C.c_int, [C.POINTER(GatedDeltaArgs), vp]),
+    "ssm_gated_delta_bwd": (C.c_int, [C.POINTER(GatedDeltaBwdArgs), vp]),
+    "ssm_gated_delta_step": (C.c_int, [C.POINTER(GatedDeltaStepArgs), vp]),
+    "ssm_token_logp": (C.c_int, [C.POINTER(TokenLogpArgs), vp]),
+    "ssm_token_logp_bwd": (C.c_int, [C.POINTER(TokenLogpBwdArgs), vp]),
+    "ssm_topk_distill": (C.c_int, [C.POINTER(TopkDistillArgs), vp]),
+    "ssm_topk_distill_bwd": (C.c_int, [C.POINTER(TopkDistillBwdArgs), vp]),
 }
 
 _lib = None
@@ -205,7 +269,7 @@ def load() -> C.CDLL:
         except AttributeError as exc:
             raise RuntimeError(f"{LIB_PATH} does not export {name}; rebuild the library") from exc
         fn.restype, fn.argtypes = res, args
-    if lib.ssm_b200_abi_version() != ABI_VERSION:
+    if lib.ssm_b200_abi_version() != ABI_VERSION or lib.ssm_b200_lm_abi_version() != LM_ABI_VERSION:
         raise RuntimeError("libssm_b200.so has an unexpected ABI version; rebuild the library")
     _lib = lib
     return lib

@@ -7,7 +7,7 @@ Objects are rebuilt only when a source or header is newer than they are.
 
 It then builds ``ssm_b200/lib/ssm_b200_ext.so``, the PyTorch extension (``csrc/torch_ext/*.cpp``, plain C++ compiled with
 g++ against the torch headers): the library under the ten names of upstream's compiled backend (``ssm_b200_ext.cpp``) and
-the operator surface of ``ssm_b200.ops`` with its autograd nodes (``operators.cpp``).
+the operator surface of ``ssm_b200.ops`` with its autograd nodes (``operators.cpp``, ``lm_operators.cpp``).
 """
 
 from __future__ import annotations
@@ -88,7 +88,7 @@ def build_extension(force: bool = False, verbose: bool = False) -> Path:
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
-    headers = [PKG.parent / "include" / "ssm_b200.h", *EXT_SRC.glob("*.h"), *CSRC.glob("*.h")]
+    headers = [*(PKG.parent / "include").glob("*.h"), *EXT_SRC.glob("*.h"), *CSRC.glob("*.h")]
     srcs = sorted(EXT_SRC.glob("*.cpp"))
     if not (force or _stale(EXT, [*srcs, *headers, LIB])):
         return EXT

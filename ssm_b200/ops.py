@@ -773,6 +773,88 @@ def ssd_scan(
     return out[0] if len(out) == 1 else tuple(out)
 
 
+# =========================================================================================
+# gated delta rule
+# =========================================================================================
+
+
+def gated_delta_scan(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    g: Optional[Tensor],
+    beta: Tensor,
+    scale: Optional[float] = None,
+    initial_state: Optional[Tensor] = None,
+    return_final_state: bool = False,
+    keep_state_fp32: bool = False,
+    cu_seqlens: Optional[Tensor] = None,
+):
+    """Extension: the gated delta rule over whole sequences.  Per value head, with the state ``S (V, K)`` from ``initial_state`` or zero::
+
+        S' = exp(g_t) S;   r_t = v_t - S' k_t;   S = S' + beta_t r_t k_t^T;   o_t = scale S q_t
+
+    ``q, k (B, L, Hk, K)``, ``v (B, L, H, V)``, ``g, beta (B, L, H)``; value head ``h`` reads key head ``h // (H / Hk)``; ``g`` is the natural
+    logarithm of the decay (``None``: no decay; ``-inf``: the state starts anew); ``scale`` defaults to ``K ** -0.5``.  Keys are taken as
+    they are (normalise them before).  ``K`` up to 256.  ``q`` and ``k`` are read in ``v``'s type, ``g`` and ``beta`` in their own; a
+    gradient has its input's type.  Returns ``o (B, L, H, V)``, and with ``return_final_state`` the state ``(B, H, V, K)`` in ``v``'s type, or
+    fp32 with ``keep_state_fp32`` (what :func:`gated_delta_step` continues from).
+
+    ``cu_seqlens (S + 1,)`` marks ``S`` sequences packed along ``L`` of a batch of one, each from its own state (``(S, H, V, K)``).  It rises from
+    0 to at most ``L``; rows behind the last sequence give zeros, and no gradient.  On the host it is checked; on the device it is
+    used where it lies without a synchronisation, entries that break the rule being clamped.
+
+    Everything is differentiable but ``cu_seqlens``; gradients are recorded once (no second derivative).
+    """
+    return _run("gated_delta_scan", q, k, v, g, beta, scale, initial_state, bool(return_final_state), bool(keep_state_fp32),
+                None if cu_seqlens is None else torch.as_tensor(cu_seqlens))
+
+
+def gated_delta_step(state: Tensor, q: Tensor, k: Tensor, v: Tensor, g: Optional[Tensor], beta: Tensor, scale: Optional[float] = None) -> Tensor:
+    """Extension: one decode token of the gated delta rule.  ``state (B, H, V, K)`` fp32 is overwritten in place; ``q, k (B, Hk, K)``,
+    ``v (B, H, V)``, ``g, beta (B, H)``; returns ``(B, H, V)``.  Where gradients are wanted the token goes through :func:`gated_delta_scan`
+    and the state receives the values of the new one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (state, q, k, v, g, beta)):
+        if state.ndim != 4 or state.dtype != torch.float32:
+            raise ValueError("state must be float32 of shape (B, H, V, K).")
+        if not (q.ndim == k.ndim == v.ndim == 3 and beta.ndim == 2 and (g is None or g.ndim == 2)):
+            raise ValueError("q and k must have shape (B, Hk, K), v (B, H, V), g and beta (B, H).")
+        o, new = gated_delta_scan(q[:, None], k[:, None], v[:, None], None if g is None else g[:, None], beta[:, None], scale, state.clone(), True, True)
+        with torch.no_grad():
+            state.copy_(new)
+        return o[:, 0]
+    return _native().gated_delta_step(state, q, k, v, g, beta, scale)
+
+
+# =========================================================================================
+# what is done with a head's logits
+# =========================================================================================
+
+
+def token_log_probs(logits: Tensor, targets: Tensor, temperature: float = 1.0, top_k: int = 0, return_entropy: bool = False,
+                    ignore_index: int = -100):
+    """Extension: log probabilities of given tokens.  ``logits (..., V)``, ``targets (...)`` integers; ``x = logits / temperature``,
+    ``p = softmax(x)``.  Returns ``log p[target]`` (fp32, ``(...)``; 0 where the target is ``ignore_index``), followed by the entropy of ``p``
+    with ``return_entropy`` and by the ``top_k`` largest log probabilities and their ids (``(..., top_k)``, falling; equal logits by rising
+    id; at most 128) with ``top_k > 0``.  All but the ids are differentiable with respect to ``logits``.
+
+    A row of ``-inf`` alone has no distribution: log probabilities ``-inf``, entropy 0, gradient 0.  A NaN or ``+inf`` in a row, or a target
+    outside of the vocabulary, makes the row's results NaN (for such a target: its log probability, and the row's gradient)."""
+    return _run("token_log_probs", logits, targets, float(temperature), int(top_k), bool(return_entropy), int(ignore_index))
+
+
+def topk_distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0) -> Tensor:
+    """Extension: distillation from a teacher's top logits.  ``logits (..., V)`` of the student, ``teacher_logits (..., k)`` with their
+    vocabulary ids ``teacher_ids (..., k)`` (``k`` up to 1024; a negative id leaves its entry out).  With ``t = softmax(teacher_logits /
+    temperature)`` over a row's entries returns ``sum_j t_j (log t_j - log softmax(logits / temperature)[id_j])``, fp32 ``(...)``: the
+    divergence of the student from the teacher restricted to its top tokens.  Differentiable with respect to ``logits`` (an id that occurs
+    twice counts twice); no gradient flows to the teacher, whose logits must not require one.
+
+    A row without entries (or with entries of ``-inf`` alone) gives 0 and no gradient, a student row of ``-inf`` alone ``inf`` and no gradient,
+    an id of ``V`` or above NaN."""
+    return _run("topk_distill_loss", logits, teacher_logits, teacher_ids, float(temperature))
+
+
 __all__ = [
     "selective_scan",
     "selective_state_step",
@@ -787,4 +869,8 @@ __all__ = [
     "ssd_check_status",
     "ssd_wait_selftest",
     "ssd_tensor_core_supported",
+    "gated_delta_scan",
+    "gated_delta_step",
+    "token_log_probs",
+    "topk_distill_loss",
 ]
