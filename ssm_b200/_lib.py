@@ -242,6 +242,9 @@ ENTRY_POINTS = {
     "ssm_gated_delta_table_ints": (C.c_int64, [i32, i32, i32]),
     "ssm_gated_delta_fwd": (C.c_int, [C.POINTER(GatedDeltaArgs), vp]),
     "ssm_gated_delta_bwd": (C.c_int, [C.POINTER(GatedDeltaBwdArgs), vp]),
+    "ssm_gated_delta_chunked_supported": (C.c_int, [C.POINTER(GatedDeltaArgs)]),
+    "ssm_gated_delta_chunked_scratch_bytes": (C.c_int64, [i32] * 7),
+    "ssm_gated_delta_chunked_fwd": (C.c_int, [C.POINTER(GatedDeltaArgs), vp, i32, vp, vp]),
     "ssm_gated_delta_step": (C.c_int, [C.POINTER(GatedDeltaStepArgs), vp]),
     "ssm_token_logp": (C.c_int, [C.POINTER(TokenLogpArgs), vp]),
     "ssm_token_logp_bwd": (C.c_int, [C.POINTER(TokenLogpBwdArgs), vp]),

@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/graph_task.h>
 
+#include <mutex>
 #include <utility>
 
 #include "operands.h"
@@ -116,5 +117,25 @@ inline variable_list invoke_call(const c10::intrusive_ptr<Call>& call) {
 }
 
 inline Tensor cast(const Tensor& grad, at::ScalarType t) { return grad.scalar_type() == t ? grad : grad.to(t); }
+
+// The word a kernel sets when one of its bounded waits runs out, one per device, in pinned host memory that the kernels write
+// directly: a failure is visible to the next call without a copy, an event or a synchronisation per launch.
+inline Tensor ssd_status(int64_t device) {
+  static std::mutex lock;
+  static std::vector<Tensor> words(64);
+  TORCH_CHECK(device >= 0 && device < (int64_t)words.size(), "ssd_scan: device index out of range");
+  std::lock_guard<std::mutex> hold(lock);
+  Tensor& w = words[device];
+  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().dtype(at::kInt)).pin_memory();
+  return w;
+}
+// Raise if a launch since the last report ran out of a wait.
+inline void ssd_poll(int64_t device) {
+  volatile int32_t* word = ssd_status(device).data_ptr<int32_t>();
+  const int32_t code = *word;
+  if (code == 0) return;
+  *word = 0;
+  TORCH_CHECK(false, std::string() + (code < 4 ? "ssd_scan" : "gated_delta_scan") + ": a bounded device-side wait ran out in an earlier launch (status " + std::to_string(code) + "); its outputs are invalid");
+}
 
 }  // namespace ssm_ext

@@ -23,12 +23,19 @@ Tensor lead(const Tensor& t, at::ScalarType type) { return strided(t.scalar_type
 // ---------------------------------------------------------------------------------------------
 // gated delta rule
 // ---------------------------------------------------------------------------------------------
+// An operand that the tensor-core kernels can copy: rows on 16-byte boundaries, no broadcast axis
+Tensor copyable(const Tensor& t) {
+  bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 struct DeltaCall final : Call {
   Tensor q, k, v, g, beta, init, cu, table, rest, states;  // g, init, cu may be undefined
   int64_t nb, nl, nh, nk, kd, vd, seqs;
   at::ScalarType t_q, t_k, t_v, t_g{}, t_beta, t_init{};
   double scale;
-  bool want_final, fp32_state, init_grad = false;
+  bool want_final, fp32_state, init_grad = false, chunked = false;
 
   DeltaCall(const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& g_, const Tensor& beta_, const c10::optional<double>& scale_, const OptTensor& init_,
             bool want_final_, bool fp32_state_, const OptTensor& cu_)
@@ -74,6 +81,10 @@ struct DeltaCall final : Call {
     input(g_), input(beta_), input(init_);
     q = lead(q_, t_v), k = lead(k_, t_v), v = strided(v_), beta = coefficient(beta_, "gated_delta_scan beta");
     if (g_.has_value()) g = coefficient(*g_, "gated_delta_scan g"), t_g = g_->scalar_type();
+    if (v.scalar_type() != at::kFloat && kd % 8 == 0 && kd <= 128 && vd % 8 == 0 && nl > 0 && nb > 0) {
+      chunked = true;
+      q = copyable(q), k = copyable(k), v = copyable(v);
+    }
     if (init_.has_value()) init = f32c(*init_), t_init = init_->scalar_type(), init_grad = init_->requires_grad();
   }
 
@@ -95,6 +106,7 @@ struct DeltaCall final : Call {
     c10::cuda::CUDAGuard guard(v.device());
     Tensor o = at::empty({nb, nl, nh, vd}, v.options()), fin;
     if (cu.defined()) table = at::empty({ssm_gated_delta_table_ints((int)nb, (int)nl, (int)seqs)}, v.options().dtype(at::kInt));
+    if (train) chunked = false;
     if (train) {
       rest = at::empty({nb, nl, nh, vd}, f32());
       states = at::empty({ssm_gated_delta_chunks((int)nb, (int)nl, (int)seqs * cu.defined()), nh, vd, kd}, f32());
@@ -103,7 +115,14 @@ struct DeltaCall final : Call {
     fill(a);
     a.o = o.data_ptr();
     if (want_final) fin = at::empty({seqs, nh, vd, kd}, fp32_state ? f32() : v.options()), a.final_state = fin.data_ptr(), a.final_dtype = dtype_code(fin, "gated_delta_scan");
-    run(ssm_gated_delta_fwd(&a, stream_of(v)));
+    if (chunked && init.defined() && reinterpret_cast<uintptr_t>(init.data_ptr()) % 16 != 0) init = init.clone(), a.initial_state = init.data_ptr<float>();
+    if (chunked && ssm_gated_delta_chunked_supported(&a)) {
+      ssd_poll(v.get_device());  // a wait that ran out in an earlier launch surfaces here, without a synchronisation
+      Tensor scratch = at::empty({ssm_gated_delta_chunked_scratch_bytes((int)nb, (int)nl, a.num_seqs, (int)nh, (int)kd, (int)vd, 0)}, v.options().dtype(at::kByte));
+      run(ssm_gated_delta_chunked_fwd(&a, scratch.data_ptr(), 0, ssd_status(v.get_device()).data_ptr<int32_t>(), stream_of(v)));
+    } else {
+      run(ssm_gated_delta_fwd(&a, stream_of(v)));
+    }
     if (want_final) return {o, fin};
     return {o};
   }

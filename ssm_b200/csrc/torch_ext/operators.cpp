@@ -442,9 +442,6 @@ py::object fused_layer_norm(const Tensor& x, const Tensor& weight, const OptTens
 // ---------------------------------------------------------------------------------------------
 // one decode token through a whole mixer (no gradients)
 // ---------------------------------------------------------------------------------------------
-Tensor ssd_status(int64_t device);
-void ssd_poll(int64_t device);
-
 bool plain(const Tensor& t, at::ScalarType type) {
   return t.scalar_type() == type && t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
@@ -700,26 +697,6 @@ Tensor mamba2_step(const Tensor& tok, const Tensor& conv_x, const Tensor& conv_B
 // ---------------------------------------------------------------------------------------------
 // state-space-dual scan, forward on the tensor cores
 // ---------------------------------------------------------------------------------------------
-// The word a kernel sets when one of its bounded waits runs out, one per device, in pinned host memory that the kernels write
-// directly: a failure is visible to the next call without a copy, an event or a synchronisation per launch.
-Tensor ssd_status(int64_t device) {
-  static std::mutex lock;
-  static std::vector<Tensor> words(64);
-  TORCH_CHECK(device >= 0 && device < (int64_t)words.size(), "ssd_scan: device index out of range");
-  std::lock_guard<std::mutex> hold(lock);
-  Tensor& w = words[device];
-  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().dtype(at::kInt)).pin_memory();
-  return w;
-}
-// Raise if a launch since the last report ran out of a wait.
-void ssd_poll(int64_t device) {
-  volatile int32_t* word = ssd_status(device).data_ptr<int32_t>();
-  const int32_t code = *word;
-  if (code == 0) return;
-  *word = 0;
-  TORCH_CHECK(false, std::string() + "ssd_scan: a bounded device-side wait ran out in an earlier launch (status " + std::to_string(code) + "); its outputs are invalid");
-}
-
 struct SsdShape {
   int64_t nb, nl, nh, np, ng, nn;
 };

@@ -80,6 +80,10 @@ def test_forward_and_every_gradient(nb, nl, nk, nh, kd, vd, dtype):
     assert got_o.dtype == dtype and got_s.dtype == F32
     near(got_o, o, tolerance(dtype, nl, kd, vd), "o")
     near(got_s, s, tolerance(dtype, nl, kd, vd), "state")
+    with torch.no_grad():  # nothing is kept for a backward pass
+        again = ops.gated_delta_scan(*leaves[:5], initial_state=leaves[5], return_final_state=True, keep_state_fp32=True)
+    near(again[0], o, tolerance(dtype, nl, kd, vd), "o without gradients")
+    near(again[1], s, tolerance(dtype, nl, kd, vd), "state without gradients")
     got = torch.autograd.grad([got_o, got_s], leaves, [do.to(dtype).cuda(), ds.float().cuda()])
     for name, x, y, leaf in zip(("q", "k", "v", "g", "beta", "initial"), got, want, leaves):
         assert x.dtype == leaf.dtype
@@ -109,6 +113,11 @@ def test_packed_sequences(dtype, kd, vd, cuts, where):
     near(got_o, o, tolerance(dtype, longest, kd, vd), "o")
     near(got_s, s, tolerance(dtype, longest, kd, vd), "state")
     assert not got_o[:, cuts[-1]:].any()
+    with torch.no_grad():
+        again = ops.gated_delta_scan(*leaves[:5], initial_state=leaves[5], return_final_state=True, keep_state_fp32=True, cu_seqlens=cu)
+    near(again[0], o, tolerance(dtype, longest, kd, vd), "o without gradients")
+    near(again[1], s, tolerance(dtype, longest, kd, vd), "state without gradients")
+    assert not again[0][:, cuts[-1]:].any()
     got = torch.autograd.grad([got_o, got_s], leaves, [do.to(dtype).cuda(), ds.float().cuda()])
     for name, x, y in zip(("q", "k", "v", "g", "beta", "initial"), got, want):
         near(x, y, tolerance(dtype, longest, kd, vd, True), "gradient of " + name)
