@@ -243,8 +243,9 @@ ENTRY_POINTS = {
     "ssm_gated_delta_fwd": (C.c_int, [C.POINTER(GatedDeltaArgs), vp]),
     "ssm_gated_delta_bwd": (C.c_int, [C.POINTER(GatedDeltaBwdArgs), vp]),
     "ssm_gated_delta_chunked_supported": (C.c_int, [C.POINTER(GatedDeltaArgs)]),
-    "ssm_gated_delta_chunked_scratch_bytes": (C.c_int64, [i32] * 7),
-    "ssm_gated_delta_chunked_fwd": (C.c_int, [C.POINTER(GatedDeltaArgs), vp, i32, vp, vp]),
+    "ssm_gated_delta_chunked_scratch_bytes": (C.c_int64, [i32] * 5),
+    "ssm_gated_delta_chunked_kept_bytes": (C.c_int64, [i32] * 7),
+    "ssm_gated_delta_chunked_fwd": (C.c_int, [C.POINTER(GatedDeltaArgs), vp, vp, i32, vp, vp]),
     "ssm_gated_delta_step": (C.c_int, [C.POINTER(GatedDeltaStepArgs), vp]),
     "ssm_token_logp": (C.c_int, [C.POINTER(TokenLogpArgs), vp]),
     "ssm_token_logp_bwd": (C.c_int, [C.POINTER(TokenLogpBwdArgs), vp]),

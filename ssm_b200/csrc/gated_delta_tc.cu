@@ -1,23 +1,23 @@
 // Gated delta rule on the tensor cores: 16-bit operands, kdim and vdim multiples of 8, kdim <= 128.
 //
-// A sequence is cut into chunks of 64 tokens.  With a = e^g, gam_i = a_1 .. a_i, suf_i = a_{i+1} .. a_64, G_ij = a_{j+1} .. a_i, S0 the state
-// before the chunk, the rows r_i = v_i - S'_i k_i solve a unit lower triangular system:
-//   (I + A) r = V - diag(gam) K S0^T,  A_ij = beta_j G_ij k_i.k_j (j < i);   X = (I + A)^-1;   P_ij = scale beta_j G_ij q_i.k_j (j <= i)
-//   r = X V - X diag(gam) K S0^T;   o = scale diag(gam) Q S0^T + P r;   S = gam_64 S0 + r^T diag(beta suf) K
-// and the adjoint state, from the end, with D the gradient of the state behind the chunk and Y = P X:
-//   w = dv = Y^T do + X^T diag(beta suf) K D^T;   D0 = gam_64 D + do^T diag(scale gam) Q - w^T diag(gam) K
+// A sequence is cut into chunks of 64 tokens.  With a = e^g, gam_i = a_1 .. a_i, suf_i = a_{i+1} .. a_64, G_ij = a_{j+1} .. a_i, S0 (vdim x kdim)
+// the state before the chunk, the rows r_i = v_i - S'_i k_i solve a unit lower triangular system:
+//   (I + A) r = V - diag(gam) K S0^T,  A_ij = beta_j G_ij k_i.k_j (j < i);   X = (I + A)^-1,  W = X diag(gam) K;   r = X V - W S0^T
+//   S = gam_64 S0 + r^T diag(beta suf) K
+//   o = scale diag(gam) Q S0^T + P r = Y V + Z S0^T,  P_ij = scale beta_j G_ij q_i.k_j (j <= i),  Y = P X,  Z = scale diag(gam) Q - P W
+// and the adjoint state, from the end, with D the gradient of the state behind the chunk and Wb = X^T diag(beta suf) K:
+//   w = dv = Y^T do + Wb D^T;   D0 = gam_64 D + do^T diag(scale gam) Q - w^T diag(gam) K
 //
-//   pairs_kernel   one CTA per (chunk, key head): X, P (and Y) of its value heads.  The two 64 x 64 x kdim products are mma.sync; the inverse is
-//                  fp32, blocks of 16 by substitution, then two rounds of block products.
+//   pairs_kernel   one CTA per (chunk, value head): X, Y, W, Z (and Wb), which depend on no state: all chunks at once.  Products by
+//                  mma.sync on 16 rows a warp; the inverse is fp32: blocks of 16 by substitution, then two rounds of block products.
 //   chunks_kernel  one CTA per (sequence, value head, 128 rows of the state): the walk over the chunks, forward or back (BACK).
 //
-// The walk is bound by its chain: the state of a chunk depends on the one before through three products and the conversions between
-// them.  So the state lies transposed, (vdim, kdim) with vdim on the 128 lanes of tensor memory, and every product of the chain takes its A
-// operand from tensor memory, written there by the threads that hold the rows: no shared memory round trip, no transposes.
-//   S (bf16, A) x K^T -> times -gam -> (A) x X^T, added to V^T X^T -> r -> times beta suf (A) x K -> added to the state in registers
-// What does not depend on the state (V X^T; do Y; do Q) or is not on the chain (o) is issued beside it.
-// Roundings to 16 bits: the operands above (S, gam K S, r and its weighted copy, X, P, Y, gam q), each half a step of the type; sums and the
-// state between chunks are fp32.  For bf16 the outputs and gradients of random inputs are 0.3 % off in norm (0.17 of it their own rounding).
+// The walk is bound by its chain, the state of a chunk depending on the one before through two products and the conversions between
+// them.  So the state lies transposed, with vdim on the 128 lanes of tensor memory, and both products take their A operand from tensor memory,
+// written there by the threads that hold the rows: S (16 bits) x W^T, added to V^T X^T -> r -> times beta suf x K -> added to the state,
+// which stays in registers.  o needs neither r nor a product of its own: Y and Z are 64 more rows of the operands X and W.
+// Roundings to 16 bits: S, W, Z, X, Y (from rounded P) and the weighted r, each half a step of the type; sums and the state between chunks are
+// fp32.  For bf16 the outputs and gradients of random inputs are 0.25 to 0.3 % off in norm before their own rounding (0.17 %).
 #include <algorithm>
 
 #include "gated_delta.cuh"
@@ -31,10 +31,14 @@ constexpr int C = 64;  // tokens of a chunk
 constexpr int kTileBytes = C * 128;  // 64 rows of 128 bytes
 constexpr float kReset = -150.f;     // base-2 logarithm of a decay that is zero in fp32
 
-struct Chunks {  // what pairs_kernel leaves per (chunk, value head)
-  unsigned char* pairs;  // X, P and (train) Y: tiles of 64 rows of 128 bytes in the 128-byte swizzle
-  float* vec;            // gam, beta, beta suf, scale gam: 64 each
-  int tiles;             // 2, or 3 with Y
+// What pairs_kernel leaves per (chunk, value head), matrices as tiles of 64 rows of 128 bytes in the 128-byte swizzle
+struct Chunks {
+  unsigned char* x;   // X
+  unsigned char* wz;  // per 64 columns of kdim: -W, Z
+  unsigned char* y;   // Y
+  unsigned char* wb;  // Wb; NULL without a backward pass to follow
+  float* vec;         // gam, beta, beta suf, scale gam: 64 each
+  int32_t* status;
 };
 
 __device__ __forceinline__ uint32_t swz(int row, int unit) { return (uint32_t)(row * 128 + ((unit ^ (row & 7)) << 4)); }  // 16-byte unit of a row
@@ -92,17 +96,6 @@ __device__ __forceinline__ void load_bt(uint32_t (&f)[4], uint32_t tile, int n0,
   ldsm4t(f, tile + (unit >> 3) * kTileBytes + swz(row, unit & 7));
 }
 
-// rows of an operand into a tile of KD columns; rows from n on and columns from kd on are zeros.  kd is a multiple of 8, rows lie on 16 bytes
-template <typename T, int KD>
-__device__ __forceinline__ void fill_tile(unsigned char* tile, const T* from, int64_t st, int n, int kd, int tid, int threads) {
-  constexpr int U = KD / 8;
-  for (int i = tid; i < C * U; i += threads) {
-    const int row = i / U, unit = i % U;
-    const uint4 v = row < n && unit * 8 < kd ? __ldg(reinterpret_cast<const uint4*>(from + (int64_t)row * st + unit * 8)) : make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(tile + (unit >> 3) * kTileBytes + swz(row, unit & 7)) = v;
-  }
-}
-
 // ---------------------------------------------------------------------------------------------
 // pairs of tokens
 // ---------------------------------------------------------------------------------------------
@@ -110,10 +103,12 @@ constexpr int kPairThreads = 128, kAS = 68, kTS = 36;  // row strides of the fp3
 
 template <int KD>
 struct PairSmem {
-  static constexpr int QK = (KD / 64) * kTileBytes;
-  static constexpr int TILES = 2 * QK > 3 * kTileBytes ? 2 * QK : 3 * kTileBytes;  // k and q rows; later X, P, Y on their way out
-  static constexpr int TOTAL = TILES + (C * kAS + 32 * kTS + 5 * C) * 4;
-  static constexpr int ALLOC = TOTAL + 128;
+  static constexpr int KT = (KD / 64) * kTileBytes;
+  static constexpr int QT = KT > 2 * kTileBytes ? KT : 2 * kTileBytes;
+  static constexpr int AT = C * kAS * 4 > KT ? C * kAS * 4 : KT;
+  // k's rows, later Z; q's rows, later X and P (then Y); A, then X in fp32, later W (then Wb)
+  static constexpr int K = 0, X = KT, P = X + kTileBytes, A = KT + QT, TMP = A + (AT + 1023) / 1024 * 1024, VEC = TMP + 32 * kTS * 4, TOTAL = VEC + 5 * C * 4;
+  static constexpr int ALLOC = TOTAL + 1024;
 };
 
 // cumulative base-2 logarithms of the decays of a chunk's tokens, by one warp; tokens from n on decay nothing
@@ -134,190 +129,327 @@ __device__ __forceinline__ void decay_logs(const Args& a, const Span& s, int n, 
   c[2 * lane + 1] = sum, c[2 * lane] = sum - x[1];
 }
 
-// acc[i][j] of `rows` x 64 with A rows r0.. of `ta` and B rows of `tb`, over KD columns: 8 blocks of 8 columns
+// k.k and q.k of this warp's 16 rows with all up to them, and the rows of q, which stay in the registers
 template <typename T, int KD>
-__device__ __forceinline__ void rows_product(float (&acc)[8][4], uint32_t ta, uint32_t tb, int r0, int lane) {
+__device__ __forceinline__ void rows_products(float (&kk)[8][4], float (&qk)[8][4], uint32_t (&q)[KD / 16][4], uint32_t tk, uint32_t tq, int r0, int lane) {
 #pragma unroll
   for (int nb = 0; nb < 8; ++nb)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[nb][e] = 0.f;
+    for (int e = 0; e < 4; ++e) kk[nb][e] = qk[nb][e] = 0.f;
 #pragma unroll
   for (int k0 = 0; k0 < KD; k0 += 16) {
-    uint32_t fa[4];
-    load_a(fa, ta, r0, k0, lane);
+    uint32_t fk[4];
+    load_a(fk, tk, r0, k0, lane);
+    load_a(q[k0 / 16], tq, r0, k0, lane);
 #pragma unroll
     for (int n0 = 0; n0 < C; n0 += 16) {
-      if (n0 > r0) continue;  // only pairs j <= i are looked at
+      if (n0 > r0) continue;
       uint32_t fb[4];
-      load_b(fb, tb, n0, k0, lane);
-      mma16816<T>(acc[n0 / 8], fa, fb[0], fb[1]);
-      mma16816<T>(acc[n0 / 8 + 1], fa, fb[2], fb[3]);
+      load_b(fb, tk, n0, k0, lane);
+      mma16816<T>(kk[n0 / 8], fk, fb[0], fb[1]);
+      mma16816<T>(kk[n0 / 8 + 1], fk, fb[2], fb[3]);
+      mma16816<T>(qk[n0 / 8], q[k0 / 16], fb[0], fb[1]);
+      mma16816<T>(qk[n0 / 8 + 1], q[k0 / 16], fb[2], fb[3]);
     }
   }
 }
 
-template <typename T, int KD, bool TRAIN>
-__global__ void __launch_bounds__(kPairThreads) pairs_kernel(const Args a, const Chunks out) {
-  using M = PairSmem<KD>;
-  extern __shared__ unsigned char smdyn[];
-  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 127) & ~(uintptr_t)127);
-  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const Span s = chunk_of(a.where, blockIdx.x, C);
-  const int n = s.t1 - s.t0;
-  if (n <= 0 || s.seq < 0) return;
-  float* A = reinterpret_cast<float*>(sm + M::TILES);  // A, then X, in place
-  float *tmp = A + C * kAS, *c = tmp + 32 * kTS, *beta = c + C;
-  const int kh = blockIdx.y;
-  fill_tile<T, KD>(sm, reinterpret_cast<const T*>(a.k.p) + s.b * a.k.sb + s.t0 * a.k.st + kh * a.k.sh, a.k.st, n, a.kd, tid, kPairThreads);
-  fill_tile<T, KD>(sm + M::QK, reinterpret_cast<const T*>(a.q.p) + s.b * a.q.sb + s.t0 * a.q.st + kh * a.q.sh, a.q.st, n, a.kd, tid, kPairThreads);
-  __syncthreads();
-  const int r0 = warp * 16;
-  float kk[8][4], qk[8][4];
-  rows_product<T, KD>(kk, tc::smem_u32(sm), tc::smem_u32(sm), r0, lane);
-  rows_product<T, KD>(qk, tc::smem_u32(sm + M::QK), tc::smem_u32(sm), r0, lane);
-  unsigned char *tX = sm, *tP = sm + kTileBytes, *tY = sm + 2 * kTileBytes;
-  for (int hh = 0; hh < a.group; ++hh) {
-    const int h = kh * a.group + hh;
-    __syncthreads();  // the rows of k and q, or the tiles of the head before, have been read
-    if (warp == 0) decay_logs(a, s, n, h, c, beta, lane);
-    __syncthreads();
-    uint32_t pa[TRAIN ? 8 : 1][2], pl[TRAIN ? 8 : 1][2];  // P as an A operand, and what its rounding leaves
+// contiguous shared -> global; both addresses 16-byte aligned, size a multiple of 16
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+// rows 16 r, columns 16 c of a 32 x 32 product of fp32 blocks in shared memory, by one warp; each factor in two 16-bit pieces, three products
+template <typename T>
+__device__ __forceinline__ void product32(float (&d)[2][4], const float* left, int ls, const float* right, int rs, int r0, int n0, int lane) {
 #pragma unroll
-    for (int nb = 0; nb < 8; ++nb) {
-      const int j = nb * 8 + (lane & 3) * 2;
-      float x[4], p[4];
+  for (int e = 0; e < 4; ++e) d[0][e] = d[1][e] = 0.f;
+  auto split = [](float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = pack2<T>(x, y);
+    const float2 z = unpack2<T>(hi);
+    lo = pack2<T>(x - z.x, y - z.y);
+  };
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = r0 + (lane >> 2) + (e >> 1) * 8, jj = j + (e & 1);
-        const float G = jj <= i ? ex2_approx(c[i] - c[jj]) * beta[jj] : 0.f;
-        x[e] = jj < i ? G * kk[nb][e] : 0.f;
-        p[e] = jj <= i ? G * qk[nb][e] * a.scale : 0.f;
-      }
-      const int i = r0 + (lane >> 2);
-      *reinterpret_cast<float2*>(&A[i * kAS + j]) = make_float2(x[0], x[1]);
-      *reinterpret_cast<float2*>(&A[(i + 8) * kAS + j]) = make_float2(x[2], x[3]);
-      const uint32_t w0 = pack2<T>(p[0], p[1]), w1 = pack2<T>(p[2], p[3]);
-      *reinterpret_cast<uint32_t*>(tP + swz(i, nb) + (lane & 3) * 4) = w0;
-      *reinterpret_cast<uint32_t*>(tP + swz(i + 8, nb) + (lane & 3) * 4) = w1;
-      if constexpr (TRAIN) {
-        const float2 u0 = unpack2<T>(w0), u1 = unpack2<T>(w1);
-        pa[nb][0] = w0, pa[nb][1] = w1, pl[nb][0] = pack2<T>(p[0] - u0.x, p[1] - u0.y), pl[nb][1] = pack2<T>(p[2] - u1.x, p[3] - u1.y);
-      }
+  for (int k0 = 0; k0 < 32; k0 += 16) {
+    uint32_t ah[4], al[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = *reinterpret_cast<const float2*>(&left[(r0 + (lane >> 2) + (e & 1) * 8) * ls + k0 + (lane & 3) * 2 + (e >> 1) * 8]);
+      split(x.x, x.y, ah[e], al[e]);
     }
-    __syncthreads();
-    {  // the diagonal blocks, one a warp, a column a lane (both halves of the warp the same ones)
-      const float* D = A + r0 * kAS + r0;
-      float x[16];
-      const int col = lane & 15;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float v = i == col ? 1.f : 0.f;
+    for (int nb = 0; nb < 2; ++nb) {
+      uint32_t bh[2], bl[2];
 #pragma unroll
-        for (int j = 0; j < i; ++j) v = fmaf(-D[i * kAS + j], x[j], v);
-        x[i] = v;
+      for (int e = 0; e < 2; ++e) {
+        const float* at = &right[(k0 + (lane & 3) * 2 + e * 8) * rs + n0 + nb * 8 + (lane >> 2)];
+        split(at[0], at[rs], bh[e], bl[e]);
       }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if ((i & 1) == lane >> 4) A[(r0 + i) * kAS + r0 + col] = x[i];
-    }
-    __syncthreads();
-    {  // pairs of blocks: X10 = -X11 (A10 X00); a thread has a row and four columns of one of the two
-      const int b = tid >> 6, row = (tid & 63) >> 2, c4 = (tid & 3) * 4;
-      const float* A10 = A + (b * 32 + 16) * kAS + b * 32;
-      const float* X00 = A + (b * 32) * kAS + b * 32;
-      const float* X11 = A + (b * 32 + 16) * kAS + b * 32 + 16;
-      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float m = A10[row * kAS + k];
-        const float4 y = *reinterpret_cast<const float4*>(&X00[k * kAS + c4]);
-        t.x = fmaf(m, y.x, t.x), t.y = fmaf(m, y.y, t.y), t.z = fmaf(m, y.z, t.z), t.w = fmaf(m, y.w, t.w);
-      }
-      *reinterpret_cast<float4*>(&tmp[(b * 16 + row) * kTS + c4]) = t;
-      __syncthreads();
-      t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float m = -X11[row * kAS + k];
-        const float4 y = *reinterpret_cast<const float4*>(&tmp[(b * 16 + k) * kTS + c4]);
-        t.x = fmaf(m, y.x, t.x), t.y = fmaf(m, y.y, t.y), t.z = fmaf(m, y.z, t.z), t.w = fmaf(m, y.w, t.w);
-      }
-      *reinterpret_cast<float4*>(&A[(b * 32 + 16 + row) * kAS + b * 32 + c4]) = t;
-    }
-    __syncthreads();
-    {  // the same for the halves: two rows and four columns a thread
-      const int row = (tid >> 3) * 2, c4 = (tid & 7) * 4;
-      const float* A10 = A + 32 * kAS;
-      float4 t[2];
-      auto product = [&](const float* left, int ls, const float* right, int rs, float sign) {
-        t[0] = t[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int k = 0; k < 32; ++k) {
-          const float m0 = sign * left[row * ls + k], m1 = sign * left[(row + 1) * ls + k];
-          const float4 y = *reinterpret_cast<const float4*>(&right[k * rs + c4]);
-          t[0].x = fmaf(m0, y.x, t[0].x), t[0].y = fmaf(m0, y.y, t[0].y), t[0].z = fmaf(m0, y.z, t[0].z), t[0].w = fmaf(m0, y.w, t[0].w);
-          t[1].x = fmaf(m1, y.x, t[1].x), t[1].y = fmaf(m1, y.y, t[1].y), t[1].z = fmaf(m1, y.z, t[1].z), t[1].w = fmaf(m1, y.w, t[1].w);
-        }
-      };
-      product(A10, kAS, A, kAS, 1.f);
-      *reinterpret_cast<float4*>(&tmp[row * kTS + c4]) = t[0];
-      *reinterpret_cast<float4*>(&tmp[(row + 1) * kTS + c4]) = t[1];
-      __syncthreads();
-      product(A + 32 * kAS + 32, kAS, tmp, kTS, -1.f);
-      __syncthreads();
-      *reinterpret_cast<float4*>(&A[(32 + row) * kAS + c4]) = t[0];
-      *reinterpret_cast<float4*>(&A[(33 + row) * kAS + c4]) = t[1];
-    }
-    __syncthreads();
-    for (int i = tid; i < C * 8; i += kPairThreads) {  // X in 16 bits
-      const int row = i >> 3, unit = i & 7;
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = unit * 8 + e * 2;
-        const float2 v = *reinterpret_cast<const float2*>(&A[row * kAS + j]);
-        w[e] = pack2<T>(j <= row ? v.x : 0.f, j + 1 <= row ? v.y : 0.f);
-      }
-      *reinterpret_cast<uint4*>(tX + swz(row, unit)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __syncthreads();
-    if constexpr (TRAIN) {  // Y = P X, columns up to the rows' own; P in two pieces
-      const uint32_t bX = tc::smem_u32(tX);
-#pragma unroll
-      for (int n0 = 0; n0 < C; n0 += 16) {
-        float y[2][4] = {};
-#pragma unroll
-        for (int k0 = 0; k0 < C; k0 += 16) {
-          if (k0 < n0 || k0 > r0) continue;
-          uint32_t fb[4];
-          load_bt(fb, bX, n0, k0, lane);
-          const uint32_t hi[4] = {pa[k0 / 8][0], pa[k0 / 8][1], pa[k0 / 8 + 1][0], pa[k0 / 8 + 1][1]};
-          const uint32_t lo[4] = {pl[k0 / 8][0], pl[k0 / 8][1], pl[k0 / 8 + 1][0], pl[k0 / 8 + 1][1]};
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            mma16816<T>(y[e], hi, fb[2 * e], fb[2 * e + 1]);
-            mma16816<T>(y[e], lo, fb[2 * e], fb[2 * e + 1]);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = r0 + (lane >> 2);
-          *reinterpret_cast<uint32_t*>(tY + swz(i, n0 / 8 + e) + (lane & 3) * 4) = pack2<T>(y[e][0], y[e][1]);
-          *reinterpret_cast<uint32_t*>(tY + swz(i + 8, n0 / 8 + e) + (lane & 3) * 4) = pack2<T>(y[e][2], y[e][3]);
-        }
-      }
-      __syncthreads();
-    }
-    const int64_t at = (int64_t)s.chunk * a.heads + h;
-    uint4* to = reinterpret_cast<uint4*>(out.pairs + at * (out.tiles * kTileBytes));
-    for (int i = tid; i < (TRAIN ? 3 : 2) * (kTileBytes / 16); i += kPairThreads) to[i] = reinterpret_cast<const uint4*>(sm)[i];
-    if (tid < C) {
-      float* v = out.vec + at * (4 * C);
-      const float gam = ex2_approx(c[tid]);
-      v[tid] = gam, v[C + tid] = beta[tid], v[2 * C + tid] = beta[tid] * ex2_approx(c[C - 1] - c[tid]), v[3 * C + tid] = gam * a.scale;
+      mma16816<T>(d[nb], ah, bh[0], bh[1]);
+      mma16816<T>(d[nb], al, bh[0], bh[1]);
+      mma16816<T>(d[nb], ah, bl[0], bl[1]);
     }
   }
+}
+
+struct PairMaps {
+  CUtensorMap q, k;
+};
+
+template <typename T, int KD, bool TRAIN>
+__global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, const Chunks out, const __grid_constant__ PairMaps maps) {
+  using M = PairSmem<KD>;
+  extern __shared__ unsigned char smdyn[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t mbar;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const Span s = chunk_of(a.where, blockIdx.x, C);
+  const int n = s.t1 - s.t0, h = blockIdx.y, kh = h / a.group;
+  if (n <= 0 || s.seq < 0) return;
+  const int64_t at = (int64_t)s.chunk * a.heads + h;
+  unsigned char *tK = sm + M::K, *tQ = sm + M::X, *tX = sm + M::X, *tP = sm + M::P, *tW = sm + M::A;
+  float* A = reinterpret_cast<float*>(sm + M::A);
+  float *tmp = reinterpret_cast<float*>(sm + M::TMP), *c = reinterpret_cast<float*>(sm + M::VEC), *beta = c + C, *gam = beta + C, *bsuf = gam + C, *sgam = bsuf + C;
+  const uint32_t landed = tc::smem_u32(&mbar);
+  if (tid == 0) {
+    tc::mbar_init(landed, 1);
+    tc::mbar_expect_tx(landed, 2 * M::KT);
+    for (int b = 0; b < KD / 64; ++b) {
+      tc::tma_load_4d(tc::smem_u32(tK + b * kTileBytes), &maps.k, landed, b * 64, kh, s.t0, s.b);
+      tc::tma_load_4d(tc::smem_u32(tQ + b * kTileBytes), &maps.q, landed, b * 64, kh, s.t0, s.b);
+    }
+  }
+  if (warp == 0) {  // beside the copies
+    decay_logs(a, s, n, h, c, beta, lane);
+    __syncwarp();
+    float* v = out.vec + at * (4 * C);
+    for (int i = lane; i < C; i += 32) {
+      const float x = ex2_approx(c[i]), y = beta[i] * ex2_approx(c[C - 1] - c[i]);
+      gam[i] = x, bsuf[i] = y, sgam[i] = x * a.scale;
+      v[i] = x, v[C + i] = beta[i], v[2 * C + i] = y, v[3 * C + i] = x * a.scale;
+    }
+  }
+  __syncthreads();
+  if (!__syncthreads_and(tc::mbar_wait(landed, 0))) {
+    if (tid == 0 && out.status) *(volatile int32_t*)out.status = 6;
+    return;
+  }
+  if (a.where.table && n < C) {  // rows of the next sequence: nothing of them may enter a product, not even times zero
+    constexpr int U = KD / 8;
+    for (int i = tid; i < (C - n) * U; i += kPairThreads)
+      *reinterpret_cast<uint4*>(tK + (i % U >> 3) * kTileBytes + swz(n + i / U, i % U & 7)) = *reinterpret_cast<uint4*>(tQ + (i % U >> 3) * kTileBytes + swz(n + i / U, i % U & 7)) =
+          make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  const int r0 = warp * 16, gi = lane >> 2, gj = (lane & 3) * 2;
+  const uint32_t bK = tc::smem_u32(tK);
+  float kk[8][4], qk[8][4];
+  uint32_t fq[KD / 16][4];
+  rows_products<T, KD>(kk, qk, fq, bK, tc::smem_u32(tQ), r0, lane);
+  __syncthreads();  // the rows of q have been read
+  {
+    const float ci[2] = {c[r0 + gi], c[r0 + gi + 8]};
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) {
+      float x[4] = {}, p[4] = {};
+      if (nb * 8 <= r0 + 8) {
+        const float2 cj = *reinterpret_cast<const float2*>(&c[nb * 8 + gj]), bj = *reinterpret_cast<const float2*>(&beta[nb * 8 + gj]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = r0 + gi + (e >> 1) * 8 - (nb * 8 + gj + (e & 1));
+          const float G = ex2_approx(ci[e >> 1] - (e & 1 ? cj.y : cj.x)) * (e & 1 ? bj.y : bj.x);
+          x[e] = d > 0 ? G * kk[nb][e] : 0.f;
+          p[e] = d >= 0 ? G * a.scale * qk[nb][e] : 0.f;
+        }
+      }
+      const int i = r0 + gi;
+      *reinterpret_cast<float2*>(&A[i * kAS + nb * 8 + gj]) = make_float2(x[0], x[1]);
+      *reinterpret_cast<float2*>(&A[(i + 8) * kAS + nb * 8 + gj]) = make_float2(x[2], x[3]);
+      *reinterpret_cast<uint32_t*>(tP + swz(i, nb) + gj * 2) = pack2<T>(p[0], p[1]);
+      *reinterpret_cast<uint32_t*>(tP + swz(i + 8, nb) + gj * 2) = pack2<T>(p[2], p[3]);
+    }
+  }
+  __syncwarp();  // the diagonal block is this warp's own
+  {              // its inverse, a column a lane (both halves of the warp the same ones)
+    const float* D = A + r0 * kAS + r0;
+    float x[16];
+    const int col = lane & 15;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = i == col ? 1.f : 0.f, v1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < i; j += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(&D[i * kAS + j]);  // zeros from the diagonal on
+        v = fmaf(-m.x, x[j], v);
+        if (j + 1 < i) v1 = fmaf(-m.y, x[j + 1], v1);
+        if (j + 2 < i) v = fmaf(-m.z, x[j + 2], v);
+        if (j + 3 < i) v1 = fmaf(-m.w, x[j + 3], v1);
+      }
+      x[i] = v + v1;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((i & 1) == lane >> 4) A[(r0 + i) * kAS + r0 + col] = x[i];
+  }
+  __syncthreads();
+  {  // pairs of blocks: X10 = -X11 (A10 X00); a thread has a row and four columns of one of the two
+    const int b = tid >> 6, row = (tid & 63) >> 2, c4 = (tid & 3) * 4;
+    const float* A10 = A + (b * 32 + 16) * kAS + b * 32;
+    const float* X00 = A + (b * 32) * kAS + b * 32;
+    const float* X11 = A + (b * 32 + 16) * kAS + b * 32 + 16;
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto product = [&](const float* left, const float* right, int rs) {
+      t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(&left[row * kAS + k]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = e == 0 ? m.x : e == 1 ? m.y : e == 2 ? m.z : m.w;
+          const float4 y = *reinterpret_cast<const float4*>(&right[(k + e) * rs + c4]);
+          t.x = fmaf(x, y.x, t.x), t.y = fmaf(x, y.y, t.y), t.z = fmaf(x, y.z, t.z), t.w = fmaf(x, y.w, t.w);
+        }
+      }
+    };
+    product(A10, X00, kAS);
+    *reinterpret_cast<float4*>(&tmp[(b * 16 + row) * kTS + c4]) = t;
+    __syncthreads();
+    product(X11, tmp + b * 16 * kTS, kTS);
+    *reinterpret_cast<float4*>(&A[(b * 32 + 16 + row) * kAS + b * 32 + c4]) = make_float4(-t.x, -t.y, -t.z, -t.w);
+  }
+  __syncthreads();
+  {  // the same for the halves, 16 x 16 of it a warp
+    const int br = (warp >> 1) * 16, bc = (warp & 1) * 16;
+    float d[2][4];
+    product32<T>(d, A + 32 * kAS, kAS, A, kAS, br, bc, lane);
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      *reinterpret_cast<float2*>(&tmp[(br + gi) * kTS + bc + nb * 8 + gj]) = make_float2(d[nb][0], d[nb][1]);
+      *reinterpret_cast<float2*>(&tmp[(br + gi + 8) * kTS + bc + nb * 8 + gj]) = make_float2(d[nb][2], d[nb][3]);
+    }
+    __syncthreads();
+    product32<T>(d, A + 32 * kAS + 32, kAS, tmp, kTS, br, bc, lane);
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      *reinterpret_cast<float2*>(&A[(32 + br + gi) * kAS + bc + nb * 8 + gj]) = make_float2(-d[nb][0], -d[nb][1]);
+      *reinterpret_cast<float2*>(&A[(32 + br + gi + 8) * kAS + bc + nb * 8 + gj]) = make_float2(-d[nb][2], -d[nb][3]);
+    }
+  }
+  __syncthreads();
+  // X in 16 bits, and the operands of W (X with columns times -gam) and Wb (X^T with columns times beta suf)
+  uint32_t fw[4][4], fb[TRAIN ? 4 : 1][4];
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = r0 + gi + (e & 1) * 8, j = kb * 16 + gj + (e >> 1) * 8;
+      float2 x = make_float2(0.f, 0.f);
+      if (kb <= warp) {
+        x = *reinterpret_cast<const float2*>(&A[i * kAS + j]);
+        const float2 m = *reinterpret_cast<const float2*>(&gam[j]);
+        fw[kb][e] = pack2<T>(-x.x * m.x, -x.y * m.y);
+      }
+      *reinterpret_cast<uint32_t*>(tX + swz(i, j >> 3) + gj * 2) = pack2<T>(x.x, x.y);
+      if constexpr (TRAIN) {
+        if (kb >= warp) {
+          const float2 m = *reinterpret_cast<const float2*>(&bsuf[j]);
+          fb[kb][e] = pack2<T>(A[j * kAS + i] * m.x, A[(j + 1) * kAS + i] * m.y);
+        }
+      }
+    }
+  }
+  __syncthreads();  // A has been read, X is written
+  // 64 columns of rows x a tile, from the accumulator given
+  auto times = [&](float (&d)[8][4], const uint32_t (&fa)[4][4], uint32_t tile, int from, int to) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      if (kb < from || kb > to) continue;
+#pragma unroll
+      for (int n0 = 0; n0 < 64; n0 += 16) {
+        uint32_t b[4];
+        load_bt(b, tile, n0, kb * 16, lane);
+        mma16816<T>(d[n0 / 8], fa[kb], b[0], b[1]);
+        mma16816<T>(d[n0 / 8 + 1], fa[kb], b[2], b[3]);
+      }
+    }
+  };
+  auto put = [&](unsigned char* tile, const float (&d)[8][4]) {  // this warp's rows
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) {
+      *reinterpret_cast<uint32_t*>(tile + swz(r0 + gi, nb) + gj * 2) = pack2<T>(d[nb][0], d[nb][1]);
+      *reinterpret_cast<uint32_t*>(tile + swz(r0 + gi + 8, nb) + gj * 2) = pack2<T>(d[nb][2], d[nb][3]);
+    }
+  };
+  // Wb waits in the registers for W's place; k's rows are not needed after it
+  uint32_t wb[TRAIN ? KD / 64 : 1][8][2];
+#pragma unroll
+  for (int half = 0; half < KD / 64; ++half) {
+    float d[8][4] = {};
+    times(d, fw, bK + half * kTileBytes, 0, warp);
+    put(tW + half * kTileBytes, d);
+    if constexpr (TRAIN) {
+      float e[8][4] = {};
+      times(e, fb, bK + half * kTileBytes, warp, 3);
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) wb[half][nb][0] = pack2<T>(e[nb][0], e[nb][1]), wb[half][nb][1] = pack2<T>(e[nb][2], e[nb][3]);
+    }
+  }
+  uint32_t fp[4][4];
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb)
+    if (kb <= warp) load_a(fp[kb], tc::smem_u32(tP), r0, kb * 16, lane);
+  {
+    float d[8][4] = {};
+    times(d, fp, tc::smem_u32(tX), 0, warp);
+    __syncwarp();
+    put(tP, d);
+  }
+  __syncthreads();  // W is written, the rows of k have been read
+  const float s0 = sgam[r0 + gi], s1 = sgam[r0 + gi + 8];
+#pragma unroll
+  for (int half = 0; half < KD / 64; ++half) {
+    float d[8][4];
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) {
+      const uint32_t* q = &fq[half * 4 + nb / 2][(nb & 1) * 2];
+      const float2 x = unpack2<T>(q[0]), y = unpack2<T>(q[1]);
+      d[nb][0] = s0 * x.x, d[nb][1] = s0 * x.y, d[nb][2] = s1 * y.x, d[nb][3] = s1 * y.y;
+    }
+    times(d, fp, tc::smem_u32(tW) + half * kTileBytes, 0, warp);
+    put(tK + half * kTileBytes, d);
+  }
+  tc::fence_async_smem();
+  __syncthreads();
+  if (tid == 0) {
+    bulk_store(out.x + at * kTileBytes, tc::smem_u32(tX), kTileBytes);
+    bulk_store(out.y + at * kTileBytes, tc::smem_u32(tP), kTileBytes);
+    unsigned char* to = out.wz + at * (2 * M::KT);
+#pragma unroll
+    for (int half = 0; half < KD / 64; ++half) {
+      bulk_store(to + 2 * half * kTileBytes, tc::smem_u32(tW) + half * kTileBytes, kTileBytes);
+      bulk_store(to + (2 * half + 1) * kTileBytes, bK + half * kTileBytes, kTileBytes);
+    }
+    tc::bulk_commit();
+    if constexpr (TRAIN) tc::bulk_wait_read();
+  }
+  if constexpr (TRAIN) {
+    __syncthreads();  // W has left
+#pragma unroll
+    for (int half = 0; half < KD / 64; ++half)
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) {
+        *reinterpret_cast<uint32_t*>(tW + half * kTileBytes + swz(r0 + gi, nb) + gj * 2) = wb[half][nb][0];
+        *reinterpret_cast<uint32_t*>(tW + half * kTileBytes + swz(r0 + gi + 8, nb) + gj * 2) = wb[half][nb][1];
+      }
+    tc::fence_async_smem();
+    __syncthreads();
+    if (tid == 0) {
+      bulk_store(out.wb + at * M::KT, tc::smem_u32(tW), M::KT);
+      tc::bulk_commit();
+    }
+  }
+  if (tid == 0) tc::bulk_wait_all();  // shared memory outlives the copies that read it
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -335,35 +467,67 @@ struct ChunkWalk {
   int last_dtype;
   void* rest;    // 16-bit r for the backward pass, [token / 8][vdim][8] per (chunk, head); nullable
   void* states;  // 16-bit state before every chunk (BACK: adjoint state behind it), [kdim / 8][vdim][8]; nullable
-  int32_t* status;
 };
 
-constexpr int kCompute = 256, kWalkThreads = kCompute + 128;  // eight warps of rows; one each for copies, products, stores (and an idle one)
-template <int KD>
+// Warps 0-7 hold the rows of the state (a lane a row, two warps share the columns of 32 rows; with four of them 2240 cycles a chunk instead of 1940), 8-11
+// prepare operands and store what leaves, 12 copies, 13 issues the products.  Launched with 128 registers a thread (512 x 128 = 65536), of which
+// the groups of four warps keep 168, 168, 104 and 40.
+constexpr int kParts = 2, kCompute = 128 * kParts, kHelp = 128, kWalkThreads = kCompute + kHelp + 128;
+constexpr int kComputeRegs = 168, kHelpRegs = 104, kIssueRegs = 40;
+static_assert(kCompute * kComputeRegs + kHelp * kHelpRegs + 128 * kIssueRegs <= kWalkThreads * 128, "the split draws on what the block was launched with");
+// Operands in two rings: what the first product reads is free again a third into its chunk, the rest at its end.  (One ring of two stages of 81 KB:
+// 4200 cycles a chunk, of which 1800 waiting for copies.)
+template <int KD, bool BACK>
 struct WalkSmem {
-  static constexpr int K_BYTES = (KD / 64) * kTileBytes;
-  static constexpr int V_BYTES = 2 * kTileBytes;
-  static constexpr int VEC_BYTES = 4 * C * 4;
-  static constexpr int K = 0, Q = K_BYTES, V = Q + K_BYTES, X = V + V_BYTES, P = X + kTileBytes, VEC = P + kTileBytes;  // BACK: Y in P's place
-  static constexpr int STAGE = VEC + VEC_BYTES;
-  static constexpr int STAGES = 3;
-  static constexpr int OUT = 2 * kTileBytes;
-  static constexpr int ALLOC = STAGES * STAGE + OUT + 1024;
-  static constexpr uint32_t BYTES = 2 * K_BYTES + V_BYTES + 2 * kTileBytes + VEC_BYTES;
+  static constexpr int KB = (KD / 64) * kTileBytes, VB = 2 * kTileBytes, VEC_BYTES = 4 * C * 4;
+  static constexpr int WB = BACK ? KB : 2 * KB, XB = BACK ? kTileBytes : 2 * kTileBytes;
+  static constexpr int V = 0, X = VB, W = X + XB, EARLY = W + WB;                       // v, X and Y, W and Z; BACK: do, Y, Wb
+  static constexpr int K = 0, Q = KB, VEC = Q + (BACK ? KB : 0), LATE = VEC + VEC_BYTES;  // k, vectors; BACK: q too
+  static constexpr int NE = 2, NL = 3;
+  static constexpr int OUT = NE * EARLY + NL * LATE, ALLOC = OUT + 2 * VB + 1024;
 };
+static_assert(WalkSmem<128, false>::ALLOC <= 227 * 1024 && WalkSmem<128, true>::ALLOC <= 227 * 1024, "shared memory of an SM");
 
-// tensor memory, in columns: the state as an operand, the scaled product (then r), the weighted r; accumulators
-template <int KD>
+// tensor memory, in columns: operands (the state; the weighted r) and accumulators: r and o side by side, twice; the state's increment
 struct Cols {
-  static constexpr int S = 0, A2 = 64, U = 96, KS = 128, R = 192, O = 256, DS = 384;  // O: two of 64
+  static constexpr int S = 0, U = 64, RO = 128, DS = 384;
 };
 
-enum Bar { kFull = 0, kFree = 3, kPrep = 6, kState = 7, kKS = 8, kA2 = 9, kR = 10, kU = 11, kDS = 12, kO = 13, kOut = 14, kOutFree = 15, kEnd = 16, kBars = 17 };
+// A wait by parity must not fall two completions behind: each barrier's next completion but one needs what its waiter does after this one (two of
+// kPrep for that)
+enum Bar { kFullE = 0, kFreeE = 2, kFullL = 4, kFreeL = 7, kPrep = 10, kState = 12, kR, kU, kDS, kO, kOut, kEnd, kBars };
+
+// a load from tensor memory that is under way until `landed`
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// ... and its registers hang on the wait, so that no use of them moves in front of it
+__device__ __forceinline__ void landed(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+// One probe that returns at once, then the suspending ones, which take 300 cycles even where the phase is complete.  (Polling instead costs the warps
+// that work more than the ones that wait gain: 2170 to 2300 cycles a chunk against 1940.)
+__device__ __forceinline__ bool phase_done(uint32_t mbar, uint32_t parity) { return tc::mbar_test(mbar, parity) || tc::mbar_wait(mbar, parity); }
+__device__ __forceinline__ void put16(uint32_t saddr, uint16_t x) { asm volatile("st.shared.u16 [%0], %1;\n" ::"r"(saddr), "h"(x) : "memory"); }
+__device__ __forceinline__ float f(uint32_t x) { return __uint_as_float(x); }
 
 template <typename T, int KD, bool BACK>
 __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk w, const __grid_constant__ WalkMaps maps) {
-  using M = WalkSmem<KD>;
-  using TC = Cols<KD>;
+  using M = WalkSmem<KD, BACK>;
+  using TC = Cols;
   extern __shared__ unsigned char smdyn[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t mbar[kBars];
@@ -382,299 +546,314 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
   const int nchunks = (s.t1 - s.t0 + C - 1) / C;
   const bool packed = a.where.table != nullptr;
   auto bar = [&](int i) { return tc::smem_u32(&mbar[i]); };
-  auto wait = [&](int i, int n) { return (bool)__all_sync(0xffffffffu, tc::mbar_test(bar(i), n & 1) || tc::mbar_wait(bar(i), n & 1)); };  // the n-th completion
+  auto wait = [&](int i, int n) { return (bool)__all_sync(0xffffffffu, phase_done(bar(i), n & 1)); };  // for the n-th completion
   if (warp == 0) tc::tmem_alloc(tc::smem_u32(&tmem_slot), 512);
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const bool all = i == kPrep || i == kState || i == kA2 || i == kU || i == kOut;
-      tc::mbar_init(bar(i), i >= kFree && i < kFree + M::STAGES ? 1 + kCompute / 32 : all ? kCompute / 32 : 1);
+      const bool rows = i == kState || i == kU, help = i == kPrep || i == kPrep + 1 || i == kOut;
+      tc::mbar_init(bar(i), i >= kFreeL && i < kFreeL + M::NL ? 1 + (kCompute + kHelp) / 32 : rows ? kCompute / 32 : help ? kHelp / 32 : 1);
     }
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  // position p in the walk -> chunk of the sequence
-  auto chunk_at = [&](int p) { return BACK ? nchunks - 1 - p : p; };
-  unsigned char* out = sm + M::STAGES * M::STAGE;
+  auto chunk_at = [&](int p) { return BACK ? nchunks - 1 - p : p; };  // position in the walk -> chunk of the sequence
+  auto done = [&](int i) {                                            // this warp's part of a phase
+    tc::fence_before_sync();
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(bar(i));
+  };
+  auto together = [](bool mine) {  // the helping warps meet, with one verdict
+    uint32_t all;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.aligned.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}\n"
+        : "=r"(all)
+        : "r"((uint32_t)mine), "n"(kHelp)
+        : "memory");
+    return all != 0;
+  };
+  const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+  const int row = (warp & 3) * 32 + lane, v = v0 + row;  // rows of the state: a warp reaches the lanes of its quarter
+  const bool live = v < a.vd;
   bool ok = true;
 
-  if (warp == kCompute / 32) {  // ---- copies
-    int sent = 0;
-    for (int p = 0; p < nchunks && ok; ++p) {
-      const int st = p % M::STAGES;
-      if (p >= M::STAGES) ok = wait(kFree + st, p / M::STAGES - 1);
-      if (!ok) break;
-      if (lane == 0) {
-        const int c = chunk_at(p), t = s.t0 + c * C;
-        unsigned char* d = sm + st * M::STAGE;
-        const uint32_t full = bar(kFull + st);
-        tc::mbar_expect_tx(full, M::BYTES);
-        for (int b = 0; b < KD / 64; ++b) {
-          tc::tma_load_4d(tc::smem_u32(d + M::K + b * kTileBytes), &maps.k, full, b * 64, kh, t, s.b);
-          tc::tma_load_4d(tc::smem_u32(d + M::Q + b * kTileBytes), &maps.q, full, b * 64, kh, t, s.b);
-        }
-        for (int b = 0; b < 2; ++b) tc::tma_load_4d(tc::smem_u32(d + M::V + b * kTileBytes), &maps.v, full, v0 + b * 64, h, t, s.b);
-        const int64_t at = (int64_t)(s.chunk + c) * a.heads + h;
-        const unsigned char* pairs = w.in.pairs + at * (w.in.tiles * kTileBytes);
-        tc::bulk_load(tc::smem_u32(d + M::X), pairs, kTileBytes, full);
-        tc::bulk_load(tc::smem_u32(d + M::P), pairs + (BACK ? 2 : 1) * kTileBytes, kTileBytes, full);
-        tc::bulk_load(tc::smem_u32(d + M::VEC), w.in.vec + at * (4 * C), M::VEC_BYTES, full);
-      }
-      __syncwarp();
-      sent = p + 1;
-    }
-    for (int p = max(0, sent - M::STAGES); p < sent; ++p) ok = wait(kFull + p % M::STAGES, p / M::STAGES) && ok;  // nothing is under way when the block ends
-  } else if (warp == kCompute / 32 + 1) {  // ---- products
-    constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-    constexpr uint32_t id_row = tc::instr_desc(128, C, fmt, 0, BACK ? 1 : 0);       // rows (tensor memory) x X or, transposed, X^T
-    constexpr uint32_t id_kt = tc::instr_desc(128, C, fmt, 0, 0);                   // state x K^T, Q^T; r x P^T
-    constexpr uint32_t id_vx = tc::instr_desc(128, C, fmt, 1, BACK ? 1 : 0);        // V^T X^T; do^T Y
-    constexpr uint32_t id_k = tc::instr_desc(128, KD, fmt, 0, 1);                   // weighted rows x K
-    constexpr uint32_t id_doq = tc::instr_desc(128, KD, fmt, 1, 1);                 // do^T Q
-    for (int p = 0; p < nchunks && ok; ++p) {
-      const int st = p % M::STAGES;
-      ok = wait(kFull + st, p / M::STAGES) && wait(kPrep, p);  // rows of another sequence cut, q scaled
-      if (!ok) break;
-      tc::fence_after_sync();
-      const uint32_t base = tc::smem_u32(sm + st * M::STAGE);
-      const uint64_t k_rows = tc::smem_desc_sw128(base + M::K, 16, 1024), q_rows = tc::smem_desc_sw128(base + M::Q, 16, 1024);
-      const uint64_t k_cols = tc::smem_desc_sw128(base + M::K, kTileBytes, 1024), q_cols = tc::smem_desc_sw128(base + M::Q, kTileBytes, 1024);
-      const uint64_t v_cols = tc::smem_desc_sw128(base + M::V, kTileBytes, 1024);
-      const uint64_t x_rows = tc::smem_desc_sw128(base + M::X, 16, 1024), p_rows = tc::smem_desc_sw128(base + M::P, 16, 1024);
-      const uint64_t x_cols = tc::smem_desc_sw128(base + M::X, kTileBytes, 1024), y_cols = tc::smem_desc_sw128(base + M::P, kTileBytes, 1024);
-      auto along = [](int kk) { return (uint64_t)(((kk >> 2) * kTileBytes + (kk & 3) * 32) >> 4); };  // 16 columns further
-      auto down = [](int kk) { return (uint64_t)(kk * (2048 >> 4)); };                                // 16 rows further
-      if (tc::elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < C / 16; ++kk)
-          tc::mma_ss(tmem + TC::R, v_cols + down(kk), BACK ? y_cols + down(kk) : x_rows + along(kk), id_vx, kk > 0);
-      }
-      __syncwarp();
-      ok = wait(kState, p);
-      if (!ok) break;
-      tc::fence_after_sync();
-      const uint32_t dO = tmem + TC::O + (p & 1) * 64;
-      if (tc::elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < KD / 16; ++kk) tc::mma_ts(tmem + TC::KS, tmem + TC::S + kk * 8, k_rows + along(kk), id_kt, kk > 0);
-        tc::commit(bar(kKS));
-        if constexpr (BACK) {
-#pragma unroll
-          for (int kk = 0; kk < C / 16; ++kk) tc::mma_ss(tmem + TC::DS, v_cols + down(kk), q_cols + down(kk), id_doq, kk > 0);
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < KD / 16; ++kk) tc::mma_ts(dO, tmem + TC::S + kk * 8, q_rows + along(kk), id_kt, kk > 0);
-        }
-      }
-      __syncwarp();
-      ok = wait(kA2, p);
-      if (!ok) break;
-      tc::fence_after_sync();
-      if (tc::elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < C / 16; ++kk) tc::mma_ts(tmem + TC::R, tmem + TC::A2 + kk * 8, BACK ? x_cols + down(kk) : x_rows + along(kk), id_row, true);
-        tc::commit(bar(kR));
-      }
-      __syncwarp();
-      ok = wait(kU, p);
-      if (!ok) break;
-      tc::fence_after_sync();
-      if (tc::elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < C / 16; ++kk) tc::mma_ts(tmem + TC::DS, tmem + TC::U + kk * 8, k_cols + down(kk), id_k, BACK || kk > 0);
-        tc::commit(bar(kDS));
-        if constexpr (!BACK) {
-#pragma unroll
-          for (int kk = 0; kk < C / 16; ++kk) tc::mma_ts(dO, tmem + TC::A2 + kk * 8, p_rows + along(kk), id_kt, true);
-          tc::commit(bar(kO));
-        }
-        tc::commit(bar(kFree + st));
-      }
-      __syncwarp();
-    }
-    if (tc::elect_one()) tc::commit(bar(kEnd));  // nothing is under way when the block ends, nor where a wait ran out
-    __syncwarp();
-    ok = wait(kEnd, 0) && ok;
-  } else if (warp == kCompute / 32 + 2) {  // ---- stores of o (BACK: dv)
-    for (int p = 0; p < nchunks && ok; ++p) {
-      ok = wait(kOut, p);
-      if (!ok) break;
-      const int t = s.t0 + chunk_at(p) * C, n = min(C, s.t1 - t);
-      if (!packed || n == C) {  // TMA cuts at the tensor's end
+  if (warp >= (kCompute + kHelp) / 32) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegs));
+    if (warp == (kCompute + kHelp) / 32) {  // ---- copies
+      auto pair_at = [&](int p) { return (int64_t)(s.chunk + chunk_at(p)) * a.heads + h; };
+      const unsigned char* wide = BACK ? w.in.wb : w.in.wz;
+      auto early = [&](int p) {
         if (lane == 0) {
-          tc::tma_store_4d(&maps.o, tc::smem_u32(out), v0, h, t, s.b);
-          if (v0 + 64 < a.vd) tc::tma_store_4d(&maps.o, tc::smem_u32(out + kTileBytes), v0 + 64, h, t, s.b);
-          tc::bulk_commit();
-          tc::bulk_wait_read();
+          const uint32_t full = bar(kFullE + p % M::NE), d = tc::smem_u32(sm + p % M::NE * M::EARLY);
+          tc::mbar_expect_tx(full, M::EARLY);
+          for (int b = 0; b < 2; ++b) tc::tma_load_4d(d + M::V + b * kTileBytes, &maps.v, full, v0 + b * 64, h, s.t0 + chunk_at(p) * C, s.b);
+          if constexpr (!BACK) tc::bulk_load(d + M::X, w.in.x + pair_at(p) * kTileBytes, kTileBytes, full);
+          tc::bulk_load(d + M::X + M::XB - kTileBytes, w.in.y + pair_at(p) * kTileBytes, kTileBytes, full);
+          tc::bulk_load(d + M::W, wide + pair_at(p) * M::WB, M::WB, full);
         }
         __syncwarp();
+      };
+      auto late = [&](int p) {
+        if (lane == 0) {
+          const int t = s.t0 + chunk_at(p) * C;
+          const uint32_t full = bar(kFullL + p % M::NL), d = tc::smem_u32(sm + M::NE * M::EARLY + p % M::NL * M::LATE);
+          tc::mbar_expect_tx(full, M::LATE);
+          for (int b = 0; b < KD / 64; ++b) {
+            tc::tma_load_4d(d + M::K + b * kTileBytes, &maps.k, full, b * 64, kh, t, s.b);
+            if constexpr (BACK) tc::tma_load_4d(d + M::Q + b * kTileBytes, &maps.q, full, b * 64, kh, t, s.b);
+          }
+          tc::bulk_load(d + M::VEC, w.in.vec + pair_at(p) * (4 * C), M::VEC_BYTES, full);
+        }
+        __syncwarp();
+      };
+      int ne = 0, nl = 0;
+      while (ne < min(M::NE, nchunks)) early(ne++);
+      while (nl < min(M::NL, nchunks)) late(nl++);
+      for (int p = 0; p < nchunks && ok; ++p) {
+        if (ne < nchunks && (ok = wait(kFreeE + p % M::NE, p / M::NE))) {
+          if (ne + 1 < nchunks && lane == 0) {  // the next one's on their way into the L2
+            for (int b = 0; b < 2 && v0 + b * 64 < a.vd; ++b) tc::tma_prefetch_4d(&maps.v, v0 + b * 64, h, s.t0 + chunk_at(ne + 1) * C, s.b);
+            tc::bulk_prefetch(wide + pair_at(ne + 1) * M::WB, M::WB);
+            tc::bulk_prefetch(w.in.y + pair_at(ne + 1) * kTileBytes, kTileBytes);
+            if constexpr (!BACK) tc::bulk_prefetch(w.in.x + pair_at(ne + 1) * kTileBytes, kTileBytes);
+          }
+          early(ne++);
+        }
+        if (ok && nl < nchunks && (ok = wait(kFreeL + p % M::NL, p / M::NL))) late(nl++);
+      }
+      // nothing is under way when the block ends
+      for (int p = max(0, ne - M::NE); p < ne; ++p) ok = wait(kFullE + p % M::NE, p / M::NE) && ok;
+      for (int p = max(0, nl - M::NL); p < nl; ++p) ok = wait(kFullL + p % M::NL, p / M::NL) && ok;
+    } else if (warp == (kCompute + kHelp) / 32 + 1) {  // ---- products
+      constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      constexpr int N1 = BACK ? C : 2 * C;  // r, and forward o beside it
+      constexpr uint32_t id_s = tc::instr_desc(128, C, fmt, 0, 0);               // state x W^T, Z^T; Wb^T
+      constexpr uint32_t id_v = tc::instr_desc(128, N1, fmt, 1, BACK ? 1 : 0);   // V^T x X^T, Y^T; do^T x Y
+      constexpr uint32_t id_k = tc::instr_desc(128, KD, fmt, 0, 1);              // weighted rows x K
+      constexpr uint32_t id_doq = tc::instr_desc(128, KD, fmt, 1, 1);            // do^T Q
+      for (int p = 0; p < nchunks; ++p) {
+        const int se = p % M::NE, sl = p % M::NL;
+        if (!(ok = wait(kFullE + se, p / M::NE) && wait(kFullL + sl, p / M::NL) && wait(kPrep + (p & 1), p >> 1))) break;  // rows of another sequence cut; BACK: q scaled
+        tc::fence_after_sync();
+        const uint32_t e = tc::smem_u32(sm + se * M::EARLY), l = tc::smem_u32(sm + M::NE * M::EARLY + sl * M::LATE), R = tmem + TC::RO + (p & 1) * 128;
+        const uint64_t w_rows = tc::smem_desc_sw128(e + M::W, 16, 1024), v_cols = tc::smem_desc_sw128(e + M::V, kTileBytes, 1024);
+        const uint64_t x_rows = tc::smem_desc_sw128(e + M::X, 16, 1024), y_cols = tc::smem_desc_sw128(e + M::X, kTileBytes, 1024);
+        const uint64_t k_cols = tc::smem_desc_sw128(l + M::K, kTileBytes, 1024), q_cols = tc::smem_desc_sw128(l + M::Q, kTileBytes, 1024);
+        auto along = [](int kk) { return (uint64_t)(((kk >> 2) * (N1 * 128) + (kk & 3) * 32) >> 4); };  // 16 columns further in a tile of N1 rows
+        auto down = [](int kk) { return (uint64_t)(kk * (2048 >> 4)); };                                // 16 rows further
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < C / 16; ++kk) tc::mma_ss(R, v_cols + down(kk), BACK ? y_cols + down(kk) : x_rows + along(kk), id_v, kk > 0);
+        }
+        __syncwarp();
+        if (BACK && p > 0 && !(ok = wait(kOut, p - 1))) break;  // the results before these have been read: kR is not two ahead of the helping warps
+        if (!(ok = wait(kState, p))) break;
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < KD / 16; ++kk) tc::mma_ts(R, tmem + TC::S + kk * 8, w_rows + along(kk), id_s, true);
+          tc::commit(bar(kR));
+        }
+        __syncwarp();
+        // beside the rows' step
+        if (!BACK && p > 0 && !(ok = wait(kOut, p - 1))) break;
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+          if constexpr (BACK) {
+#pragma unroll
+            for (int kk = 0; kk < C / 16; ++kk) tc::mma_ss(tmem + TC::DS, v_cols + down(kk), q_cols + down(kk), id_doq, kk > 0);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < KD / 16; ++kk) tc::mma_ts(R + C, tmem + TC::S + kk * 8, w_rows + (uint64_t)(kTileBytes >> 4) + along(kk), id_s, true);
+            tc::commit(bar(kO));
+          }
+          tc::commit(bar(kFreeE + se));
+        }
+        __syncwarp();
+        if (!(ok = wait(kU, p))) break;
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < C / 16; ++kk) tc::mma_ts(tmem + TC::DS, tmem + TC::U + kk * 8, k_cols + down(kk), id_k, BACK || kk > 0);
+          tc::commit(bar(kDS));
+          tc::commit(bar(kFreeL + sl));
+        }
+        __syncwarp();
+      }
+      if (tc::elect_one()) tc::commit(bar(kEnd));  // nothing is under way when the block ends, nor where a wait ran out
+      __syncwarp();
+      ok = wait(kEnd, 0) && ok;
+    }
+  } else if (warp >= kCompute / 32) {  // ---- operands prepared, results stored
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kHelpRegs));
+    const int me = tid - kCompute;
+    auto tokens_of = [&](int p) { return min(C, s.t1 - (s.t0 + chunk_at(p) * C)); };
+    // rows of another sequence cut from the products over tokens; BACK: q times scale gam
+    auto late_at = [&](int p) { return sm + M::NE * M::EARLY + p % M::NL * M::LATE; };
+    auto prepare = [&](int p) {
+      const int n = tokens_of(p);
+      const bool cut = packed && n < C;
+      if (!wait(kFullL + p % M::NL, p / M::NL) || (cut && !wait(kFullE + p % M::NE, p / M::NE))) return false;
+      unsigned char *d = late_at(p), *e = sm + p % M::NE * M::EARLY;
+      constexpr int U = KD / 8;
+      if constexpr (BACK) {
+        const float* sg = reinterpret_cast<const float*>(d + M::VEC) + 3 * C;
+#pragma unroll 4
+        for (int i = me; i < C * U; i += kHelp) {
+          const int r = i / U, u = i % U;
+          uint4* at = reinterpret_cast<uint4*>(d + M::Q + (u >> 3) * kTileBytes + swz(r, u & 7));
+          const float m = sg[r];
+          const uint4 x = *at;
+          const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+          uint32_t y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 z = unpack2<T>(in[e]);
+            y[e] = r < n ? pack2<T>(z.x * m, z.y * m) : 0u;
+          }
+          *at = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+      }
+      if (cut) {
+        for (int i = me; i < (C - n) * U; i += kHelp) *reinterpret_cast<uint4*>(d + M::K + (i % U >> 3) * kTileBytes + swz(n + i / U, i % U & 7)) = make_uint4(0, 0, 0, 0);
+        for (int i = me; i < (C - n) * 16; i += kHelp) *reinterpret_cast<uint4*>(e + M::V + (i % 16 >> 3) * kTileBytes + swz(n + i / 16, i % 16 & 7)) = make_uint4(0, 0, 0, 0);
+      }
+      if (BACK || cut) tc::fence_async_smem();
+      done(kPrep + (p & 1));
+      return true;
+    };
+    unsigned char* out = sm + M::OUT;  // rows of tokens on their way out, two blocks of 64 columns
+    uint32_t unit[8];                  // where this thread's column lies in them, by the row's place in the swizzle
+#pragma unroll
+    for (int e = 0; e < 8; ++e) unit[e] = tc::smem_u32(out) + (row >> 6) * kTileBytes + swz(e, (row & 63) >> 3) + (row & 7) * 2;
+    if (nchunks > 0) ok = prepare(0);
+    for (int p = 0; p < nchunks; ++p) {
+      ok = ok && (p + 1 >= nchunks || prepare(p + 1)) && wait(BACK ? kR : kO, p);
+      if (!(ok = together(ok))) break;  // all four warps or none
+      tc::fence_after_sync();
+      const int n = tokens_of(p), t = s.t0 + chunk_at(p) * C, buf = (p & 1) * M::VB;
+      uint32_t x[2][32];  // 64 tokens of this thread's row
+#pragma unroll
+      for (int q = 0; q < 2; ++q) ld32(tmem + lanes + TC::RO + (p & 1) * 128 + (BACK ? 0 : C) + q * 32, x[q]);
+      landed(x[0]), landed(x[1]);
+      done(kOut);
+      if (me == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");  // the tile of the chunk before the last has left
+      together(true);
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const uint32_t z = pack2<T>(f(x[q][e]), f(x[q][e + 1]));
+          put16(unit[e & 7] + buf + (q * 32 + (e & ~7)) * 128, (uint16_t)z);
+          put16(unit[(e + 1) & 7] + buf + (q * 32 + (e & ~7)) * 128, (uint16_t)(z >> 16));
+        }
+      tc::fence_async_smem();
+      together(true);
+      if (!packed || n == C) {  // TMA cuts at the tensor's end
+        if (me == 0) {
+          tc::tma_store_4d(&maps.o, tc::smem_u32(out + buf), v0, h, t, s.b);
+          if (v0 + 64 < a.vd) tc::tma_store_4d(&maps.o, tc::smem_u32(out + buf + kTileBytes), v0 + 64, h, t, s.b);
+          tc::bulk_commit();
+        }
       } else {  // what follows belongs to the next sequence
         T* o = reinterpret_cast<T*>(w.o);
         const int units = min(128, a.vd - v0) / 8;
-        for (int i = lane; i < n * units; i += 32) {
-          const int row = i / units, u = i % units;
-          *reinterpret_cast<uint4*>(o + ((int64_t)(t + row) * a.heads + h) * a.vd + v0 + u * 8) =
-              *reinterpret_cast<const uint4*>(out + (u >> 3) * kTileBytes + swz(row, u & 7));
-        }
-        __syncwarp();
+        for (int i = me; i < n * units; i += kHelp)
+          *reinterpret_cast<uint4*>(o + ((int64_t)(t + i / units) * a.heads + h) * a.vd + v0 + i % units * 8) =
+              *reinterpret_cast<const uint4*>(out + buf + (i % units >> 3) * kTileBytes + swz(i / units, i % units & 7));
       }
-      if (lane == 0) tc::mbar_arrive(bar(kOutFree));
       __syncwarp();
+      if (lane == 0) tc::mbar_arrive(bar(kFreeL + p % M::NL));
     }
-    if (lane == 0) tc::bulk_wait_all();
-  } else if (warp < kCompute / 32) {  // ---- rows of the state: lane = row, the warps of a lane quarter have half of the columns each
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, v = v0 + row;
-    const bool live = v < a.vd;
-    constexpr int NS = KD / 2;  // columns of the state a thread holds
+    if (me == 0) tc::bulk_wait_all();
+  } else {  // ---- rows of the state: lane = row, the warps of a lane quarter share the columns
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kComputeRegs));
+    const int part = warp >> 2;
+    constexpr int NS = KD / kParts, NT = C / kParts;  // columns of the state and tokens of a thread
     float S[NS];
-    const int64_t state_at = (((int64_t)s.seq * a.heads + h) * a.vd + v) * a.kd + half * NS;
+    const int64_t state_at = (((int64_t)s.seq * a.heads + h) * a.vd + v) * a.kd + part * NS;
 #pragma unroll
     for (int e = 0; e < NS; e += 4) {
-      const bool in = w.initial && live && half * NS + e < a.kd;  // kdim is a multiple of 8
+      const bool in = w.initial && live && part * NS + e < a.kd;  // kdim is a multiple of 8
       const float4 x = in ? __ldg(reinterpret_cast<const float4*>(w.initial + state_at + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
       S[e] = x.x, S[e + 1] = x.y, S[e + 2] = x.z, S[e + 3] = x.w;
     }
-    auto done = [&](int i) {  // this warp's part of a phase
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(bar(i));
-    };
     // the state as an operand, and for a backward pass to follow
     auto publish = [&](int p) {
-      uint4* keep = w.states && p < nchunks && live
-                        ? reinterpret_cast<uint4*>(w.states) + (((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (KD / 8) + half * (NS / 8)) * a.vd + v
-                        : nullptr;
+      uint32_t x[NS / 2];
 #pragma unroll
-      for (int q = 0; q < NS / 32; ++q) {
-        uint32_t x[16];
+      for (int e = 0; e < NS / 2; ++e) x[e] = pack2<T>(S[2 * e], S[2 * e + 1]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = pack2<T>(S[q * 32 + 2 * e], S[q * 32 + 2 * e + 1]);
-        tc::tmem_st16(tmem + lanes + TC::S + half * (NS / 2) + q * 16, x);
-        if (keep)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) keep[(int64_t)(q * 4 + u) * a.vd] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
-      }
+      for (int q = 0; q < NS / 32; ++q) tc::tmem_st16(tmem + lanes + TC::S + part * (NS / 2) + q * 16, reinterpret_cast<const uint32_t(&)[16]>(x[q * 16]));
       tc::tmem_wait_st();
       done(kState);
-    };
-    // rows of another sequence cut from the products over tokens; q times scale gam
-    auto prepare = [&](int p) {
-      const int st = p % M::STAGES;
-      if (!wait(kFull + st, p / M::STAGES)) return false;
-      unsigned char* d = sm + st * M::STAGE;
-      const float* sg = reinterpret_cast<const float*>(d + M::VEC) + 3 * C;
-      const int n = min(C, s.t1 - (s.t0 + chunk_at(p) * C));
-      constexpr int U = KD / 8;
-      for (int i = tid; i < C * U; i += kCompute) {
-        const int r = i / U, u = i % U;
-        uint4* at = reinterpret_cast<uint4*>(d + M::Q + (u >> 3) * kTileBytes + swz(r, u & 7));
-        const float m = sg[r];
-        const uint4 x = *at;
-        const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-        uint32_t y[4];
+      if (w.states && live) {
+        uint4* keep = reinterpret_cast<uint4*>(w.states) + (((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (KD / 8) + part * (NS / 8)) * a.vd + v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack2<T>(in[e]);
-          y[e] = r < n ? pack2<T>(f.x * m, f.y * m) : 0u;
-        }
-        *at = make_uint4(y[0], y[1], y[2], y[3]);
+        for (int u = 0; u < NS / 8; ++u) keep[(int64_t)u * a.vd] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
       }
-      if (packed && n < C) {
-        for (int i = tid; i < (C - n) * U; i += kCompute) *reinterpret_cast<uint4*>(d + M::K + (i % U >> 3) * kTileBytes + swz(n + i / U, i % U & 7)) = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i < (C - n) * 16; i += kCompute) *reinterpret_cast<uint4*>(d + M::V + (i % 16 >> 3) * kTileBytes + swz(n + i / 16, i % 16 & 7)) = make_uint4(0, 0, 0, 0);
-      }
-      tc::fence_async_smem();
-      done(kPrep);
-      return true;
     };
-    // 32 values of this thread's row (tokens 32 half ..) into the tile of rows of tokens that leaves by TMA
-    auto stage_out = [&](const float (&x)[32]) {
-      unsigned char* at = out + (row >> 6) * kTileBytes + (row & 7) * 2;
+    if (nchunks > 0) publish(0);
+    for (int p = 0; p < nchunks; ++p) {
+      const int sl = p % M::NL;
+      if (!(ok = wait(kFullL + sl, p / M::NL))) break;
+      const float* vec = reinterpret_cast<const float*>(sm + M::NE * M::EARLY + sl * M::LATE + M::VEC);
+      const float* weight = vec + (BACK ? 0 : 2 * C) + part * NT;  // beta suf; BACK: gam
+      const float whole = vec[C - 1];
+      float4 m[NT / 4];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) *reinterpret_cast<T*>(at + swz(half * 32 + e, (row & 63) >> 3)) = from_f<T>(x[e]);
-      tc::fence_async_smem();
-      done(kOut);
-    };
-    if (nchunks > 0) ok = prepare(0);
-    publish(0);
-    for (int p = 0; p < nchunks && ok; ++p) {
-      const int st = p % M::STAGES;
-      const float* vec = reinterpret_cast<const float*>(sm + st * M::STAGE + M::VEC);
-      const float* first = vec + (BACK ? 2 * C : 0) + half * 32;   // gam; BACK: beta suf
-      const float* second = vec + (BACK ? 0 : 2 * C) + half * 32;  // beta suf; BACK: gam
-      float x[32];
-      if (!(ok = wait(kKS, p))) break;
-      tc::fence_after_sync();
-      tc::tmem_ld32(tmem + lanes + TC::KS + half * 32, x);
-      {
-        uint32_t y[16];
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float4 m = *reinterpret_cast<const float4*>(first + 2 * e);
-          if constexpr (BACK) y[e] = pack2<T>(x[2 * e] * m.x, x[2 * e + 1] * m.y), y[e + 1] = pack2<T>(x[2 * e + 2] * m.z, x[2 * e + 3] * m.w);
-          else y[e] = pack2<T>(-x[2 * e] * m.x, -x[2 * e + 1] * m.y), y[e + 1] = pack2<T>(-x[2 * e + 2] * m.z, -x[2 * e + 3] * m.w);
-        }
-        tc::tmem_st16(tmem + lanes + TC::A2 + half * 16, y);
-        tc::tmem_wait_st();
-      }
-      done(kA2);
+      for (int e = 0; e < NT / 4; ++e) m[e] = *reinterpret_cast<const float4*>(weight + 4 * e);
+      uint32_t x[NT];
       if (!(ok = wait(kR, p))) break;
       tc::fence_after_sync();
-      tc::tmem_ld32(tmem + lanes + TC::R + half * 32, x);
+      ld32(tmem + lanes + TC::RO + (p & 1) * 128 + part * NT, x);
+      landed(x);
       {
-        uint32_t y[16], u[16];
+        uint32_t y[NT / 2];
+        constexpr float sign = BACK ? -1.f : 1.f;
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float4 m = *reinterpret_cast<const float4*>(second + 2 * e);
-          if constexpr (BACK) u[e] = pack2<T>(-x[2 * e] * m.x, -x[2 * e + 1] * m.y), u[e + 1] = pack2<T>(-x[2 * e + 2] * m.z, -x[2 * e + 3] * m.w);
-          else u[e] = pack2<T>(x[2 * e] * m.x, x[2 * e + 1] * m.y), u[e + 1] = pack2<T>(x[2 * e + 2] * m.z, x[2 * e + 3] * m.w);
-          if constexpr (!BACK) y[e] = pack2<T>(x[2 * e], x[2 * e + 1]), y[e + 1] = pack2<T>(x[2 * e + 2], x[2 * e + 3]);
-        }
-        tc::tmem_st16(tmem + lanes + TC::U + half * 16, u);
-        if constexpr (!BACK) tc::tmem_st16(tmem + lanes + TC::A2 + half * 16, y);
+        for (int e = 0; e < NT / 4; ++e)
+          y[2 * e] = pack2<T>(sign * f(x[4 * e]) * m[e].x, sign * f(x[4 * e + 1]) * m[e].y), y[2 * e + 1] = pack2<T>(sign * f(x[4 * e + 2]) * m[e].z, sign * f(x[4 * e + 3]) * m[e].w);
+        tc::tmem_st16(tmem + lanes + TC::U + part * (NT / 2), y);
         tc::tmem_wait_st();
         done(kU);
         if constexpr (!BACK)
           if (w.rest && live) {
-            uint4* to = reinterpret_cast<uint4*>(w.rest) + (((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (C / 8) + half * 4) * a.vd + v;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) to[(int64_t)q * a.vd] = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+            for (int e = 0; e < NT / 2; ++e) y[e] = pack2<T>(f(x[2 * e]), f(x[2 * e + 1]));
+            uint4* to = reinterpret_cast<uint4*>(w.rest) + (((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (C / 8) + part * (NT / 8)) * a.vd + v;
+#pragma unroll
+            for (int q = 0; q < NT / 8; ++q) to[(int64_t)q * a.vd] = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
           }
       }
-      if constexpr (BACK) {
-        if (p > 0 && !(ok = wait(kOutFree, p - 1))) break;
-        stage_out(x);
-      }
-      const float whole = vec[C - 1];
-      if (p + 1 < nchunks && !(ok = prepare(p + 1))) break;
       if (!(ok = wait(kDS, p))) break;
       tc::fence_after_sync();
+      uint32_t z[NS / 32][32];
+#pragma unroll
+      for (int q = 0; q < NS / 32; ++q) ld32(tmem + lanes + TC::DS + part * NS + q * 32, z[q]);
 #pragma unroll
       for (int q = 0; q < NS / 32; ++q) {
-        tc::tmem_ld32(tmem + lanes + TC::DS + half * NS + q * 32, x);
+        landed(z[q]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) S[q * 32 + e] = fmaf(whole, S[q * 32 + e], x[e]);
+        for (int e = 0; e < 32; ++e) S[q * 32 + e] = fmaf(whole, S[q * 32 + e], f(z[q][e]));
       }
+      if (p + 1 < nchunks) publish(p + 1);
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(bar(kFree + st));
-      publish(p + 1);
-      if constexpr (!BACK) {
-        if (!(ok = wait(kO, p))) break;
-        tc::fence_after_sync();
-        tc::tmem_ld32(tmem + lanes + TC::O + (p & 1) * 64 + half * 32, x);
-        if (p > 0 && !(ok = wait(kOutFree, p - 1))) break;
-        stage_out(x);
-      }
+      if (lane == 0) tc::mbar_arrive(bar(kFreeL + sl));
     }
     if (ok && live && w.last) {
 #pragma unroll
       for (int e = 0; e < NS; ++e)
-        if (half * NS + e < a.kd) store_dyn(w.last, state_at + e, w.last_dtype, S[e]);
+        if (part * NS + e < a.kd) store_dyn(w.last, state_at + e, w.last_dtype, S[e]);
     }
   }
-  if (!ok && lane == 0 && w.status) *(volatile int32_t*)w.status = BACK ? 5 : 4;
+  if (!ok && lane == 0 && w.in.status) *(volatile int32_t*)w.in.status = BACK ? 5 : 4;
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem_slot, 512);
@@ -702,15 +881,15 @@ bool lies(const void* p, int heads, int len, int batch, int64_t sh, int64_t st, 
 }
 
 template <typename T, int KD, bool TRAIN>
-int launch_pairs(const Args& a, const Chunks& c, int64_t chunks, cudaStream_t st) {
+int launch_pairs(const Args& a, const Chunks& c, const PairMaps& maps, int64_t chunks, cudaStream_t st) {
   const int smem = PairSmem<KD>::ALLOC;
   if (const cudaError_t e = cudaFuncSetAttribute(pairs_kernel<T, KD, TRAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return set_error("pairs_kernel: %s", cudaGetErrorString(e)), (int)e;
-  pairs_kernel<T, KD, TRAIN><<<dim3((unsigned)chunks, a.heads / a.group), kPairThreads, smem, st>>>(a, c);
+  pairs_kernel<T, KD, TRAIN><<<dim3((unsigned)chunks, a.heads), kPairThreads, smem, st>>>(a, c, maps);
   return launch_status("pairs_kernel");
 }
 template <typename T, int KD, bool BACK>
 int launch_chunks(const ChunkWalk& w, const WalkMaps& maps, cudaStream_t st) {
-  const int smem = WalkSmem<KD>::ALLOC;
+  const int smem = WalkSmem<KD, BACK>::ALLOC;
   if (const cudaError_t e = cudaFuncSetAttribute(chunks_kernel<T, KD, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return set_error("chunks_kernel: %s", cudaGetErrorString(e)), (int)e;
   chunks_kernel<T, KD, BACK><<<dim3((w.a.vd + 127) / 128, w.a.heads, w.a.seqs + (w.a.where.table ? 1 : 0)), kWalkThreads, smem, st>>>(w, maps);
   return launch_status("chunks_kernel");
@@ -719,22 +898,22 @@ int launch_chunks(const ChunkWalk& w, const WalkMaps& maps, cudaStream_t st) {
 int64_t chunks_of(const ssm_gated_delta_args& a) { return chunk_bound(a.batch, a.len, a.num_seqs, C); }
 int width(int kd) { return kd <= 64 ? 64 : 128; }
 
-// scratch of a call, in this order: tiles of pairs, vectors, and for a backward pass the rests and the states
+// what a call leaves for its backward pass, in this order; without one the vectors and Y alone
 struct Layout {
-  int64_t pairs, vec, rest, states, total;
-  int tiles;
+  int64_t vec, y, wb, rest, states, total;
 };
+int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 Layout layout_of(int64_t chunks, int heads, int kd, int vd, bool train) {
   Layout l{};
-  l.tiles = train ? 3 : 2;
-  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  l.pairs = 0;
-  l.vec = up(chunks * heads * l.tiles * kTileBytes);
-  l.rest = l.vec + up(chunks * heads * 4 * C * 4);
-  l.states = l.rest + (train ? up(chunks * heads * C * vd * 2) : 0);
-  l.total = l.states + (train ? up(chunks * heads * (int64_t)width(kd) * vd * 2) : 0);
+  const int64_t n = chunks * heads;
+  l.y = up(n * 4 * C * 4);
+  l.wb = l.y + up(n * kTileBytes);
+  l.rest = l.wb + (train ? up(n * (width(kd) / 64) * kTileBytes) : 0);
+  l.states = l.rest + (train ? up(n * C * vd * 2) : 0);
+  l.total = l.states + (train ? up(n * (int64_t)width(kd) * vd * 2) : 0);
   return l;
 }
+int64_t fwd_bytes(int64_t chunks, int heads, int kd) { return up(chunks * heads * (1 + 2 * (width(kd) / 64)) * kTileBytes); }
 
 }  // namespace
 
@@ -749,26 +928,30 @@ extern "C" int ssm_gated_delta_chunked_supported(const ssm_gated_delta_args* a) 
          gd::lies(a->k, a->key_heads, a->len, a->batch, a->k_sh, a->k_st, a->k_sb) && gd::lies(a->v, a->heads, a->len, a->batch, a->v_sh, a->v_st, a->v_sb) &&
          aligned_to(a->o, 16) && aligned_to(a->initial_state, 16);
 }
-extern "C" int64_t ssm_gated_delta_chunked_scratch_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim, int32_t vdim, int32_t train) {
+extern "C" int64_t ssm_gated_delta_chunked_scratch_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim) {
+  return gd::fwd_bytes(gd::chunk_bound(batch, len, num_seqs, gd::C), heads, kdim);
+}
+extern "C" int64_t ssm_gated_delta_chunked_kept_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim, int32_t vdim, int32_t train) {
   return gd::layout_of(gd::chunk_bound(batch, len, num_seqs, gd::C), heads, kdim, vdim, train != 0).total;
 }
 
-extern "C" int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, void* scratch, int32_t train, int32_t* status, ssm_stream_t stream) {
+extern "C" int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, void* scratch, void* kept, int32_t train, int32_t* status, ssm_stream_t stream) {
   SSM_REQUIRE(args, SSM_ERR_NULL, "gated_delta: NULL arguments");
   const ssm_gated_delta_args& f = *args;
   gd::ChunkWalk w{};
   if (const int rc = gd::check(f, w.a)) return rc;
   SSM_REQUIRE(ssm_gated_delta_chunked_supported(args), SSM_ERR_UNSUPPORTED, "gated_delta: these operands do not go to the tensor cores");
   if (w.a.seqs == 0) return SSM_OK;
-  SSM_REQUIRE(f.o && scratch && aligned_to(scratch, 256), SSM_ERR_NULL, "gated_delta: NULL output or scratch");
+  SSM_REQUIRE(f.o && scratch && kept && aligned_to(scratch, 256) && aligned_to(kept, 256), SSM_ERR_NULL, "gated_delta: NULL output or scratch");
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   w.a.where.per = (f.len + gd::C - 1) / gd::C;
   const int64_t chunks = gd::chunks_of(f);
-  SSM_REQUIRE(chunks < 0x7fffffff && f.key_heads <= 65535, SSM_ERR_TOO_LARGE, "gated_delta: too many chunks");
+  SSM_REQUIRE(chunks < 0x7fffffff, SSM_ERR_TOO_LARGE, "gated_delta: too many chunks");
   const gd::Layout l = gd::layout_of(chunks, f.heads, f.kdim, f.vdim, train != 0);
-  unsigned char* base = reinterpret_cast<unsigned char*>(scratch);
-  w.in = {base + l.pairs, reinterpret_cast<float*>(base + l.vec), l.tiles};
-  w.initial = f.initial_state, w.o = f.o, w.last = f.final_state, w.last_dtype = f.final_dtype, w.status = status;
+  unsigned char* base = reinterpret_cast<unsigned char*>(kept);
+  unsigned char* wz = reinterpret_cast<unsigned char*>(scratch);
+  w.in = {wz + chunks * f.heads * (2 * (gd::width(f.kdim) / 64)) * gd::kTileBytes, wz, base + l.y, train ? base + l.wb : nullptr, reinterpret_cast<float*>(base + l.vec), status};
+  w.initial = f.initial_state, w.o = f.o, w.last = f.final_state, w.last_dtype = f.final_dtype;
   if (train) w.rest = base + l.rest, w.states = base + l.states;
   gd::WalkMaps maps;
   if (const int rc = gd::encode_map(&maps.q, f.q, f.kdim, f.key_heads, f.len, f.batch, f.q_sh, f.q_st, f.q_sb, f.io_dtype)) return rc;
@@ -776,11 +959,12 @@ extern "C" int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, voi
   if (const int rc = gd::encode_map(&maps.v, f.v, f.vdim, f.heads, f.len, f.batch, f.v_sh, f.v_st, f.v_sb, f.io_dtype)) return rc;
   const int64_t row = (int64_t)f.heads * f.vdim;
   if (const int rc = gd::encode_map(&maps.o, f.o, f.vdim, f.heads, f.len, f.batch, f.vdim, row, row * f.len, f.io_dtype)) return rc;
+  const gd::PairMaps pm{maps.q, maps.k};
   if (const int rc = gd::make_table(f, gd::C, st)) return rc;
   auto go = [&](auto type, auto kd) {
     using T = decltype(type);
     constexpr int KD = decltype(kd)::value;
-    const int rc = train ? gd::launch_pairs<T, KD, true>(w.a, w.in, chunks, st) : gd::launch_pairs<T, KD, false>(w.a, w.in, chunks, st);
+    const int rc = train ? gd::launch_pairs<T, KD, true>(w.a, w.in, pm, chunks, st) : gd::launch_pairs<T, KD, false>(w.a, w.in, pm, chunks, st);
     return rc ? rc : gd::launch_chunks<T, KD, false>(w, maps, st);
   };
   const bool wide = f.kdim > 64;

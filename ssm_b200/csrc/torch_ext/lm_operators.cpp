@@ -31,7 +31,7 @@ Tensor copyable(const Tensor& t) {
 }
 
 struct DeltaCall final : Call {
-  Tensor q, k, v, g, beta, init, cu, table, rest, states;  // g, init, cu may be undefined
+  Tensor q, k, v, g, beta, init, cu, table, rest, states, kept;  // g, init, cu may be undefined
   int64_t nb, nl, nh, nk, kd, vd, seqs;
   at::ScalarType t_q, t_k, t_v, t_g{}, t_beta, t_init{};
   double scale;
@@ -118,8 +118,10 @@ struct DeltaCall final : Call {
     if (chunked && init.defined() && reinterpret_cast<uintptr_t>(init.data_ptr()) % 16 != 0) init = init.clone(), a.initial_state = init.data_ptr<float>();
     if (chunked && ssm_gated_delta_chunked_supported(&a)) {
       ssd_poll(v.get_device());  // a wait that ran out in an earlier launch surfaces here, without a synchronisation
-      Tensor scratch = at::empty({ssm_gated_delta_chunked_scratch_bytes((int)nb, (int)nl, a.num_seqs, (int)nh, (int)kd, (int)vd, 0)}, v.options().dtype(at::kByte));
-      run(ssm_gated_delta_chunked_fwd(&a, scratch.data_ptr(), 0, ssd_status(v.get_device()).data_ptr<int32_t>(), stream_of(v)));
+      const auto bytes = v.options().dtype(at::kByte);
+      Tensor scratch = at::empty({ssm_gated_delta_chunked_scratch_bytes((int)nb, (int)nl, a.num_seqs, (int)nh, (int)kd)}, bytes);
+      kept = at::empty({ssm_gated_delta_chunked_kept_bytes((int)nb, (int)nl, a.num_seqs, (int)nh, (int)kd, (int)vd, train)}, bytes);
+      run(ssm_gated_delta_chunked_fwd(&a, scratch.data_ptr(), kept.data_ptr(), train, ssd_status(v.get_device()).data_ptr<int32_t>(), stream_of(v)));
     } else {
       run(ssm_gated_delta_fwd(&a, stream_of(v)));
     }
