@@ -97,6 +97,9 @@ int ssm_gated_delta_chunked_supported(const ssm_gated_delta_args* args);
 int64_t ssm_gated_delta_chunked_scratch_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim);
 int64_t ssm_gated_delta_chunked_kept_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim, int32_t vdim, int32_t train);
 int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, void* scratch, void* kept, int32_t train, int32_t* status, ssm_stream_t stream);
+/* Its backward: dv32 and dstates of the arguments are not used (scratch takes their place); dout, dq, dk, dv, dfinal, dqk 16-byte aligned. */
+int64_t ssm_gated_delta_chunked_bwd_scratch_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim, int32_t vdim);
+int ssm_gated_delta_chunked_bwd(const ssm_gated_delta_bwd_args* args, void* kept, void* scratch, int32_t* status, ssm_stream_t stream);
 
 /* One token: state (batch, heads, vdim, kdim) fp32, 16-byte aligned, updated in place; q, k (batch, key_heads, kdim), v (batch, heads,
  * vdim), g, beta (batch, heads) at strides; o (batch, heads, vdim) dense. */

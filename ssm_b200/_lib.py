@@ -246,6 +246,8 @@ ENTRY_POINTS = {
     "ssm_gated_delta_chunked_scratch_bytes": (C.c_int64, [i32] * 5),
     "ssm_gated_delta_chunked_kept_bytes": (C.c_int64, [i32] * 7),
     "ssm_gated_delta_chunked_fwd": (C.c_int, [C.POINTER(GatedDeltaArgs), vp, vp, i32, vp, vp]),
+    "ssm_gated_delta_chunked_bwd_scratch_bytes": (C.c_int64, [i32] * 6),
+    "ssm_gated_delta_chunked_bwd": (C.c_int, [C.POINTER(GatedDeltaBwdArgs), vp, vp, vp, vp]),
     "ssm_gated_delta_step": (C.c_int, [C.POINTER(GatedDeltaStepArgs), vp]),
     "ssm_token_logp": (C.c_int, [C.POINTER(TokenLogpArgs), vp]),
     "ssm_token_logp_bwd": (C.c_int, [C.POINTER(TokenLogpBwdArgs), vp]),

@@ -8,6 +8,8 @@
 // Backward: the adjoint state walks the same way from the end (dS' = dS + scale do q^T; w = beta dS' k = dv; dS <- a (dS' - w k^T)),
 // and needs nothing of the states.  What the other gradients need of them is the state before and the adjoint state behind each
 // chunk; within a chunk they are sums over pairs of tokens (see grad_kernel), all chunks at once.
+#include <algorithm>
+
 #include "gated_delta.cuh"
 
 namespace ssmb {
@@ -528,6 +530,18 @@ __global__ void __launch_bounds__(256) fold_heads_kernel(const float* dqk, T* dq
     dq[i] = from_f<T>(x), dk[i] = from_f<T>(y);
   }
 }
+int fold_heads(const float* dqk, void* dq, void* dk, int64_t tokens, int kd, int key_heads, int group, int dtype, cudaStream_t st) {
+  const int64_t n = tokens * key_heads * kd, half = n * group;
+  const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 8 * sm_count());
+  auto go = [&](auto type) {
+    using T = decltype(type);
+    fold_heads_kernel<T><<<grid, 256, 0, st>>>(dqk, reinterpret_cast<T*>(dq), reinterpret_cast<T*>(dk), n, kd, key_heads, group, half);
+  };
+  if (dtype == SSM_F32) go(float());
+  else if (dtype == SSM_BF16) go(__nv_bfloat16());
+  else go(__half());
+  return launch_status("fold_heads_kernel");
+}
 template <typename T>
 int launch_grad(const GradArgs& g, int64_t chunks, cudaStream_t st) {
   const size_t smem = grad_smem(g.a.kd, kVTile) + sizeof(float) * 24 * kThreads;
@@ -539,12 +553,7 @@ int launch_grad(const GradArgs& g, int64_t chunks, cudaStream_t st) {
   }
   grad_kernel<T><<<dim3((unsigned)chunks, g.a.heads), kThreads, smem, st>>>(g);
   if (const int rc = launch_status("grad_kernel")) return rc;
-  if (!g.dqk) return SSM_OK;
-  const int key_heads = g.a.heads / g.a.group;
-  const int64_t n = g.tokens * key_heads * g.a.kd;
-  fold_heads_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 8 * sm_count()), 256, 0, st>>>(g.dqk, reinterpret_cast<T*>(g.dq), reinterpret_cast<T*>(g.dk), n, g.a.kd,
-                                                                                                  key_heads, g.a.group, g.tokens * g.a.heads * g.a.kd);
-  return launch_status("fold_heads_kernel");
+  return g.dqk ? fold_heads(g.dqk, g.dq, g.dk, g.tokens, g.a.kd, g.a.heads / g.a.group, g.a.group, g.a.io, st) : (int)SSM_OK;
 }
 
 // ---------------------------------------------------------------------------------------------

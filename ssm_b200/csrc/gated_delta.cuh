@@ -58,6 +58,8 @@ __device__ __forceinline__ float beta_of(const Args& a, int b, int t, int h) {
 }
 
 int check(const ssm_gated_delta_args& a, Args& d);
+// sums the fp32 gradients of a key head's value heads (dq, then dk of all tokens) into dq and dk
+int fold_heads(const float* dqk, void* dq, void* dk, int64_t tokens, int kd, int key_heads, int group, int dtype, cudaStream_t st);
 // forms the table on the device; a no-op without packed sequences
 int make_table(const ssm_gated_delta_args& a, int chunk, cudaStream_t st);
 

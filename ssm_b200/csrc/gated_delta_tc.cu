@@ -11,6 +11,7 @@
 //   pairs_kernel   one CTA per (chunk, value head): X, Y, W, Z (and Wb), which depend on no state: all chunks at once.  Products by
 //                  mma.sync on 16 rows a warp; the inverse is fp32: blocks of 16 by substitution, then two rounds of block products.
 //   chunks_kernel  one CTA per (sequence, value head, 128 rows of the state): the walk over the chunks, forward or back (BACK).
+//   grads_kernel   one CTA per (chunk, value head): the other gradients from what both walks left (the formulas stand there).
 //
 // The walk is bound by its chain, the state of a chunk depending on the one before through two products and the conversions between
 // them.  So the state lies transposed, with vdim on the 128 lanes of tensor memory, and both products take their A operand from tensor memory,
@@ -860,8 +861,356 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
 }
 
 // ---------------------------------------------------------------------------------------------
+// gradients of a chunk's tokens
+// ---------------------------------------------------------------------------------------------
+// With N1_ij = do_i.r_j, N2_ij = w_i.r_j, S0 the state before and D the adjoint state behind the chunk:
+//   dq_i = scale gam_i S0^T do_i + sum_{j<=i} scale G_ij N1_ij beta_j k_j
+//   y_i = suf_i D^T r_i + scale sum_{j>=i} G_ji N1_ji q_j - sum_{j>i} G_ji N2_ji k_j;   dbeta_i = k_i.y_i
+//   dk_i = beta_i y_i - gam_i S0^T w_i - sum_{j<i} G_ij N2_ij beta_j k_j
+//   dg_t = gam_64 <S0, D> + sum_{i<t} beta_i suf_i k_i.(D^T r_i) + sum_{i>=t} gam_i (scale q_i.(S0^T do_i) - k_i.(S0^T w_i)) + sum_{j<t<=i} M_ij,
+//   M_ij = G_ij beta_j (scale N1_ij q_i.k_j - N2_ij k_i.k_j): every path from before t to t or behind it
+// Eight warps, each 16 tokens x half of the columns, products by mma.sync (15 Mflop a chunk).  Bound: 145 KB read and 32 KB written a chunk, and
+// that one CTA fills an SM's shared memory, so that its copies and its products take turns.
+struct GradMaps {
+  CUtensorMap q, k, d, w;
+};
+struct ChunkGrads {
+  Args a;
+  const void* rest;     // [token / 8][vdim][8]
+  const void* states;   // [kdim / 8][vdim][8]
+  const void* dstates;
+  void* dq;
+  void* dk;
+  float* dqk;  // fp32, per value head: dq then dk; NULL where heads do not share keys
+  float* dg;
+  float* dbeta;
+  int64_t tokens;
+  int32_t* status;
+};
+constexpr int kGradThreads = 256, kSlice = 128;  // columns of v at a time
+template <int KD>
+struct GradSmem {
+  static constexpr int KT = (KD / 64) * kTileBytes, VT = 2 * kTileBytes, RT = (C / 8) * kSlice * 16, ST = (KD / 8) * kSlice * 16;
+  static constexpr int Q = 0, K = KT, D = 2 * KT, W = D + VT, R = W + VT, S = R + RT, DS = S + ST, Y1 = DS + ST, Y2 = Y1 + kTileBytes, A1 = Y2 + kTileBytes, A2 = A1 + kTileBytes,
+                       VEC = A2 + kTileBytes, TOTAL = VEC + 24 * C * 4;
+  static constexpr int ALLOC = TOTAL + 1024;
+};
+static_assert(GradSmem<128>::ALLOC <= 227 * 1024, "shared memory of an SM");
+
+// Units of 16 bytes (8 elements along the first axis of a matrix, one place v): unit (c, v) at (c kSlice + v) 16.
+// B[k = v][n]: two neighbouring blocks of eight columns n0 .., depth v0 ..
+__device__ __forceinline__ void units_b(uint32_t (&f)[4], uint32_t base, int n0, int v0, int lane) { ldsm4t(f, base + (((n0 >> 3) + (lane >> 4)) * kSlice + v0 + (lane & 15)) * 16); }
+// A[m][k = v]: rows m0 .. + 15
+__device__ __forceinline__ void units_a(uint32_t (&f)[4], uint32_t base, int m0, int v0, int lane) {
+  ldsm4t(f, base + (((m0 >> 3) + ((lane >> 3) & 1)) * kSlice + v0 + (lane & 7) + ((lane >> 4) << 3)) * 16);
+}
+// A[m][k] = tile[k][m]
+__device__ __forceinline__ void load_at(uint32_t (&f)[4], uint32_t tile, int m0, int k0, int lane) {
+  const int row = k0 + (lane & 7) + ((lane >> 4) << 3), unit = m0 / 8 + ((lane >> 3) & 1);
+  ldsm4t(f, tile + (unit >> 3) * kTileBytes + swz(row, unit & 7));
+}
+
+template <typename T, int KD>
+__global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads g, const __grid_constant__ GradMaps maps) {
+  using M = GradSmem<KD>;
+  constexpr int NB = KD / 16;  // blocks of eight columns of a warp: half of kdim
+  extern __shared__ unsigned char smdyn[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t mbar;
+  const Args& a = g.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const Span s = chunk_of(a.where, blockIdx.x, C);
+  const int n = s.t1 - s.t0, h = blockIdx.y, kh = h / a.group;
+  if (n <= 0) return;
+  const int64_t tok = (int64_t)s.b * a.len + s.t0;
+  T* dq = reinterpret_cast<T*>(g.dq);
+  T* dk = reinterpret_cast<T*>(g.dk);
+  if (s.seq < 0) {  // rows of no sequence
+    for (int at = tid; at < n * a.kd; at += kGradThreads) {
+      const int64_t to = ((tok + at / a.kd) * a.heads + h) * a.kd + at % a.kd;
+      if (g.dqk) g.dqk[to] = 0.f, g.dqk[g.tokens * a.heads * a.kd + to] = 0.f;
+      else dq[to] = from_f<T>(0.f), dk[to] = from_f<T>(0.f);
+    }
+    for (int i = tid; i < n; i += kGradThreads) g.dg[(tok + i) * a.heads + h] = 0.f, g.dbeta[(tok + i) * a.heads + h] = 0.f;
+    return;
+  }
+  const uint32_t base = tc::smem_u32(sm), landed_bar = tc::smem_u32(&mbar);
+  float* c = reinterpret_cast<float*>(sm + M::VEC);
+  float *beta = c + C, *gam = beta + C, *suf = gam + C, *rows = suf + C, *cols = rows + 2 * C;  // rows [2][C], cols [4][C]: sums of M
+  float *into = cols + 4 * C, *outof = into + 2 * C, *db = outof + 2 * C, *part = db + 2 * C;   // [2][C] each; 8 partial sums
+  const int64_t pair = (int64_t)s.chunk * a.heads + h;
+  const unsigned char* rest = reinterpret_cast<const unsigned char*>(g.rest) + pair * (C / 8) * a.vd * 16;
+  const unsigned char* states = reinterpret_cast<const unsigned char*>(g.states) + pair * (KD / 8) * a.vd * 16;
+  const unsigned char* dstates = reinterpret_cast<const unsigned char*>(g.dstates) + pair * (KD / 8) * a.vd * 16;
+  auto request = [&](int v0) {  // by warp 0
+    const int nv = min(kSlice, a.vd - v0);
+    if (lane == 0) {
+      tc::mbar_expect_tx(landed_bar, 2 * M::VT + (C / 8 + 2 * (KD / 8)) * nv * 16 + (v0 ? 0 : 2 * M::KT));
+      for (int b = 0; b < KD / 64 && v0 == 0; ++b) {
+        tc::tma_load_4d(base + M::Q + b * kTileBytes, &maps.q, landed_bar, b * 64, kh, s.t0, s.b);
+        tc::tma_load_4d(base + M::K + b * kTileBytes, &maps.k, landed_bar, b * 64, kh, s.t0, s.b);
+      }
+      for (int b = 0; b < 2; ++b) {
+        tc::tma_load_4d(base + M::D + b * kTileBytes, &maps.d, landed_bar, v0 + b * 64, h, s.t0, s.b);
+        tc::tma_load_4d(base + M::W + b * kTileBytes, &maps.w, landed_bar, v0 + b * 64, h, s.t0, s.b);
+      }
+    }
+    __syncwarp();
+    for (int u = lane; u < C / 8 + 2 * (KD / 8); u += 32) {
+      const int i = u < C / 8 ? u : (u - C / 8) % (KD / 8);
+      const unsigned char* from = u < C / 8 ? rest : u < C / 8 + KD / 8 ? states : dstates;
+      const int to = u < C / 8 ? M::R : u < C / 8 + KD / 8 ? M::S : M::DS;
+      tc::bulk_load(base + to + i * (kSlice * 16), from + ((int64_t)i * a.vd + v0) * 16, nv * 16, landed_bar);
+    }
+  };
+  if (tid == 0) tc::mbar_init(landed_bar, 1);
+  __syncthreads();
+  if (warp == 0) {
+    request(0);
+    decay_logs(a, s, n, h, c, beta, lane);
+    __syncwarp();
+    for (int i = lane; i < C; i += 32) gam[i] = ex2_approx(c[i]), suf[i] = ex2_approx(c[C - 1] - c[i]);
+  }
+  const int r0 = (warp >> 1) * 16, half = warp & 1, c0 = half * 32, k_cols = half * (KD / 2), gi = lane >> 2, gj = (lane & 3) * 2;
+  float N1[4][4] = {}, N2[4][4] = {}, dQ[NB][4] = {}, dK[NB][4] = {}, y[NB][4] = {}, whole = 0.f;
+  for (int v0 = 0, turn = 0; v0 < a.vd; v0 += kSlice, ++turn) {
+    const int nv = min(kSlice, a.vd - v0);
+    if (!__syncthreads_and(phase_done(landed_bar, turn & 1))) {
+      if (tid == 0 && g.status) *(volatile int32_t*)g.status = 7;
+      return;
+    }
+    if (a.where.table && n < C) {  // rows of the next sequence: nothing of them may enter a product, not even times zero
+      constexpr int U = KD / 8;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i < (C - n) * U; i += kGradThreads) {
+        const int at = (i % U >> 3) * kTileBytes + swz(n + i / U, i % U & 7);
+        *reinterpret_cast<uint4*>(sm + M::Q + at) = zero, *reinterpret_cast<uint4*>(sm + M::K + at) = zero;
+      }
+      for (int i = tid; i < (C - n) * 16; i += kGradThreads) {
+        const int at = (i % 16 >> 3) * kTileBytes + swz(n + i / 16, i % 16 & 7);
+        *reinterpret_cast<uint4*>(sm + M::D + at) = zero, *reinterpret_cast<uint4*>(sm + M::W + at) = zero;
+      }
+    }
+    if (nv % 16) {  // products take 16 columns of v at a time
+      for (int i = tid; i < (C / 8 + 2 * (KD / 8)) * 8; i += kGradThreads) {
+        const int u = i / 8, at = u < C / 8 ? M::R + u * (kSlice * 16) : M::S + (u - C / 8) * (kSlice * 16);  // the adjoint state follows the state
+        *reinterpret_cast<uint4*>(sm + at + (nv + i % 8) * 16) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    __syncthreads();
+    for (int k0 = 0; k0 < nv; k0 += 16) {
+      uint32_t fd[4], fw[4], fr[4], b[4];
+      load_a(fd, base + M::D, r0, k0, lane);
+      load_a(fw, base + M::W, r0, k0, lane);
+      units_a(fr, base + M::R, r0, k0, lane);
+#pragma unroll
+      for (int n0 = 0; n0 < 32; n0 += 16) {
+        if (c0 + n0 > r0) continue;
+        units_b(b, base + M::R, c0 + n0, k0, lane);
+        mma16816<T>(N1[n0 / 8], fd, b[0], b[1]), mma16816<T>(N1[n0 / 8 + 1], fd, b[2], b[3]);
+        mma16816<T>(N2[n0 / 8], fw, b[0], b[1]), mma16816<T>(N2[n0 / 8 + 1], fw, b[2], b[3]);
+      }
+#pragma unroll
+      for (int n0 = 0; n0 < NB * 8; n0 += 16) {
+        units_b(b, base + M::S, k_cols + n0, k0, lane);
+        mma16816<T>(dQ[n0 / 8], fd, b[0], b[1]), mma16816<T>(dQ[n0 / 8 + 1], fd, b[2], b[3]);
+        mma16816<T>(dK[n0 / 8], fw, b[0], b[1]), mma16816<T>(dK[n0 / 8 + 1], fw, b[2], b[3]);
+        units_b(b, base + M::DS, k_cols + n0, k0, lane);
+        mma16816<T>(y[n0 / 8], fr, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fr, b[2], b[3]);
+      }
+    }
+    for (int i = tid; i < (KD / 8) * nv; i += kGradThreads) {
+      const int at = ((i / nv) * kSlice + i % nv) * 16;
+      const uint4 x = *reinterpret_cast<const uint4*>(sm + M::S + at), z = *reinterpret_cast<const uint4*>(sm + M::DS + at);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 p = unpack2<T>(xs[e]), q = unpack2<T>(zs[e]);
+        whole = fmaf(p.x, q.x, fmaf(p.y, q.y, whole));
+      }
+    }
+    if (v0 + kSlice < a.vd) {
+      tc::fence_async_smem();  // what was read and written here, before the next copies
+      __syncthreads();
+      if (warp == 0) request(v0 + kSlice);
+    }
+  }
+  whole = warp_sum(whole);
+  if (lane == 0) part[warp] = whole;
+  {  // pairs of tokens: this warp's 16 x 32
+    float QK[4][4] = {}, KK[4][4] = {};
+#pragma unroll
+    for (int k0 = 0; k0 < KD; k0 += 16) {
+      uint32_t fq[4], fk[4], b[4];
+      load_a(fq, base + M::Q, r0, k0, lane);
+      load_a(fk, base + M::K, r0, k0, lane);
+#pragma unroll
+      for (int n0 = 0; n0 < 32; n0 += 16) {
+        if (c0 + n0 > r0) continue;
+        load_b(b, base + M::K, c0 + n0, k0, lane);
+        mma16816<T>(QK[n0 / 8], fq, b[0], b[1]), mma16816<T>(QK[n0 / 8 + 1], fq, b[2], b[3]);
+        mma16816<T>(KK[n0 / 8], fk, b[0], b[1]), mma16816<T>(KK[n0 / 8 + 1], fk, b[2], b[3]);
+      }
+    }
+    float row[2] = {0.f, 0.f};
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) {
+      const int j0 = c0 + nb * 8 + gj;
+      float y1[4], y2[4], a1[4], a2[4], col[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = r0 + gi + (e >> 1) * 8, j = j0 + (e & 1);
+        const float G = ex2_approx(c[i] - c[j]), b = beta[j];
+        y1[e] = j <= i ? G * a.scale * N1[nb][e] : 0.f;
+        y2[e] = j < i ? -G * N2[nb][e] : 0.f;
+        a1[e] = b * y1[e], a2[e] = b * y2[e];
+        const float m = j < i ? a1[e] * QK[nb][e] + a2[e] * KK[nb][e] : 0.f;
+        row[e >> 1] += m, col[e & 1] += m;
+      }
+#pragma unroll
+      for (int off = 4; off <= 16; off *= 2) col[0] += __shfl_xor_sync(0xffffffffu, col[0], off), col[1] += __shfl_xor_sync(0xffffffffu, col[1], off);
+      if (gi == 0) cols[(warp >> 1) * C + j0] = col[0], cols[(warp >> 1) * C + j0 + 1] = col[1];
+      const int lo = swz(r0 + gi, j0 >> 3) + gj * 2, hi = swz(r0 + gi + 8, j0 >> 3) + gj * 2;
+      *reinterpret_cast<uint32_t*>(sm + M::Y1 + lo) = pack2<T>(y1[0], y1[1]), *reinterpret_cast<uint32_t*>(sm + M::Y1 + hi) = pack2<T>(y1[2], y1[3]);
+      *reinterpret_cast<uint32_t*>(sm + M::Y2 + lo) = pack2<T>(y2[0], y2[1]), *reinterpret_cast<uint32_t*>(sm + M::Y2 + hi) = pack2<T>(y2[2], y2[3]);
+      *reinterpret_cast<uint32_t*>(sm + M::A1 + lo) = pack2<T>(a1[0], a1[1]), *reinterpret_cast<uint32_t*>(sm + M::A1 + hi) = pack2<T>(a1[2], a1[3]);
+      *reinterpret_cast<uint32_t*>(sm + M::A2 + lo) = pack2<T>(a2[0], a2[1]), *reinterpret_cast<uint32_t*>(sm + M::A2 + hi) = pack2<T>(a2[2], a2[3]);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      row[e] += __shfl_xor_sync(0xffffffffu, row[e], 1), row[e] += __shfl_xor_sync(0xffffffffu, row[e], 2);
+      if ((lane & 3) == 0) rows[half * C + r0 + gi + e * 8] = row[e];
+    }
+  }
+  // the states' parts, scaled, and what dg takes of them
+  const float gm[2] = {gam[r0 + gi], gam[r0 + gi + 8]}, sf[2] = {suf[r0 + gi], suf[r0 + gi + 8]}, bt[2] = {beta[r0 + gi], beta[r0 + gi + 8]};
+  auto row_sums = [&](float (&x)[2], float* to) {  // over the four lanes of a row, to this half's place
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      x[e] += __shfl_xor_sync(0xffffffffu, x[e], 1), x[e] += __shfl_xor_sync(0xffffffffu, x[e], 2);
+      if ((lane & 3) == 0) to[half * C + r0 + gi + e * 8] = x[e];
+    }
+  };
+  auto pair_at = [&](int tile, int e, int nb) {  // two neighbouring elements of q or k
+    const int col = k_cols + nb * 8;
+    return unpack2<T>(*reinterpret_cast<const uint32_t*>(sm + tile + (col >> 6) * kTileBytes + swz(r0 + gi + e * 8, (col & 63) >> 3) + gj * 2));
+  };
+  {
+    float in[2] = {0.f, 0.f}, outp[2] = {0.f, 0.f};
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 q = pair_at(M::Q, e, nb), k = pair_at(M::K, e, nb);
+        dQ[nb][2 * e] *= gm[e] * a.scale, dQ[nb][2 * e + 1] *= gm[e] * a.scale;
+        dK[nb][2 * e] *= -gm[e], dK[nb][2 * e + 1] *= -gm[e];
+        y[nb][2 * e] *= sf[e], y[nb][2 * e + 1] *= sf[e];
+        in[e] += dQ[nb][2 * e] * q.x + dQ[nb][2 * e + 1] * q.y + dK[nb][2 * e] * k.x + dK[nb][2 * e + 1] * k.y;
+        outp[e] += bt[e] * (y[nb][2 * e] * k.x + y[nb][2 * e + 1] * k.y);
+      }
+    row_sums(in, into), row_sums(outp, outof);
+  }
+  __syncthreads();  // the pair matrices are written, the states have been read
+#pragma unroll
+  for (int k0 = 0; k0 < C; k0 += 16) {
+    uint32_t fa[4], fb[4], b[4];
+    if (k0 <= r0) {  // pairs with tokens before
+      load_a(fa, base + M::A1, r0, k0, lane);
+      load_a(fb, base + M::A2, r0, k0, lane);
+#pragma unroll
+      for (int n0 = 0; n0 < NB * 8; n0 += 16) {
+        const int col = k_cols + n0;
+        load_bt(b, base + M::K + (col >> 6) * kTileBytes, col & 63, k0, lane);
+        mma16816<T>(dQ[n0 / 8], fa, b[0], b[1]), mma16816<T>(dQ[n0 / 8 + 1], fa, b[2], b[3]);
+        mma16816<T>(dK[n0 / 8], fb, b[0], b[1]), mma16816<T>(dK[n0 / 8 + 1], fb, b[2], b[3]);
+      }
+    }
+    if (k0 >= r0) {  // and with those behind
+      load_at(fa, base + M::Y1, r0, k0, lane);
+      load_at(fb, base + M::Y2, r0, k0, lane);
+#pragma unroll
+      for (int n0 = 0; n0 < NB * 8; n0 += 16) {
+        const int col = k_cols + n0;
+        load_bt(b, base + M::Q + (col >> 6) * kTileBytes, col & 63, k0, lane);
+        mma16816<T>(y[n0 / 8], fa, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fa, b[2], b[3]);
+        load_bt(b, base + M::K + (col >> 6) * kTileBytes, col & 63, k0, lane);
+        mma16816<T>(y[n0 / 8], fb, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fb, b[2], b[3]);
+      }
+    }
+  }
+  {
+    float sum[2] = {0.f, 0.f};
+    float* wide = g.dqk ? g.dqk + ((tok + r0 + gi) * a.heads + h) * a.kd : nullptr;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int col = k_cols + nb * 8 + gj;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 k = pair_at(M::K, e, nb);
+        sum[e] += y[nb][2 * e] * k.x + y[nb][2 * e + 1] * k.y;
+        const float k0 = fmaf(bt[e], y[nb][2 * e], dK[nb][2 * e]), k1 = fmaf(bt[e], y[nb][2 * e + 1], dK[nb][2 * e + 1]);
+        if (wide) {
+          if (r0 + gi + e * 8 < n && col < a.kd) {
+            float* to = wide + (int64_t)e * 8 * a.heads * a.kd + col;
+            *reinterpret_cast<float2*>(to) = make_float2(dQ[nb][2 * e], dQ[nb][2 * e + 1]);
+            *reinterpret_cast<float2*>(to + g.tokens * a.heads * a.kd) = make_float2(k0, k1);
+          }
+        } else {  // over the states, to leave in whole pieces
+          const int at = (col >> 6) * kTileBytes + swz(r0 + gi + e * 8, (col & 63) >> 3) + gj * 2;
+          *reinterpret_cast<uint32_t*>(sm + M::S + at) = pack2<T>(dQ[nb][2 * e], dQ[nb][2 * e + 1]);
+          *reinterpret_cast<uint32_t*>(sm + M::DS + at) = pack2<T>(k0, k1);
+        }
+      }
+    }
+    row_sums(sum, db);
+  }
+  __syncthreads();
+  if (!g.dqk)
+    for (int i = tid; i < n * (a.kd / 8); i += kGradThreads) {
+      const int r = i / (a.kd / 8), u = i % (a.kd / 8), at = (u >> 3) * kTileBytes + swz(r, u & 7);
+      const int64_t to = ((tok + r) * a.heads + h) * a.kd + u * 8;
+      *reinterpret_cast<uint4*>(dq + to) = *reinterpret_cast<const uint4*>(sm + M::S + at);
+      *reinterpret_cast<uint4*>(dk + to) = *reinterpret_cast<const uint4*>(sm + M::DS + at);
+    }
+  if (warp == 0) {
+    float all = 0.f;
+    for (int i = 0; i < kGradThreads / 32; ++i) all += part[i];
+    float x[2], z[2];  // of tokens 2 lane, 2 lane + 1: into them, out of them
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * lane + e;
+      float col = 0.f;
+      for (int b = 0; b < 4; ++b) col += (b * 16 + 15 > i ? cols[b * C + i] : 0.f);
+      x[e] = into[i] + into[C + i] + rows[i] + rows[C + i] - col;
+      z[e] = outof[i] + outof[C + i];
+    }
+    float behind = x[0] + x[1], before = z[0] + z[1];  // inclusive sums from the end, and from the start
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const float u = __shfl_down_sync(0xffffffffu, behind, off), v = __shfl_up_sync(0xffffffffu, before, off);
+      if (lane + off < 32) behind += u;
+      if (lane >= off) before += v;
+    }
+    const float total = gam[C - 1] * all;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * lane + e;
+      if (i < n) {
+        g.dg[(tok + i) * a.heads + h] = total + (e ? behind - x[0] : behind) + (e ? before - z[1] : before - z[0] - z[1]);
+        g.dbeta[(tok + i) * a.heads + h] = db[i] + db[C + i];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------
+// The driver's call below wants a context, which a thread that has launched nothing yet (autograd's, on its first call) does not have.
+void bind_context() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
+}
 // (batch, len, heads, inner) at strides, as rank 4 (inner, head, token, batch); boxes of 64 columns of one head x 64 tokens
 int encode_map(CUtensorMap* m, const void* base, int inner, int heads, int len, int batch, int64_t sh, int64_t st, int64_t sb, int dtype) {
   EncodeTiledFn fn = encode_tiled_fn();
@@ -953,6 +1302,7 @@ extern "C" int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, voi
   w.in = {wz + chunks * f.heads * (2 * (gd::width(f.kdim) / 64)) * gd::kTileBytes, wz, base + l.y, train ? base + l.wb : nullptr, reinterpret_cast<float*>(base + l.vec), status};
   w.initial = f.initial_state, w.o = f.o, w.last = f.final_state, w.last_dtype = f.final_dtype;
   if (train) w.rest = base + l.rest, w.states = base + l.states;
+  gd::bind_context();
   gd::WalkMaps maps;
   if (const int rc = gd::encode_map(&maps.q, f.q, f.kdim, f.key_heads, f.len, f.batch, f.q_sh, f.q_st, f.q_sb, f.io_dtype)) return rc;
   if (const int rc = gd::encode_map(&maps.k, f.k, f.kdim, f.key_heads, f.len, f.batch, f.k_sh, f.k_st, f.k_sb, f.io_dtype)) return rc;
@@ -966,6 +1316,55 @@ extern "C" int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, voi
     constexpr int KD = decltype(kd)::value;
     const int rc = train ? gd::launch_pairs<T, KD, true>(w.a, w.in, pm, chunks, st) : gd::launch_pairs<T, KD, false>(w.a, w.in, pm, chunks, st);
     return rc ? rc : gd::launch_chunks<T, KD, false>(w, maps, st);
+  };
+  const bool wide = f.kdim > 64;
+  if (f.io_dtype == SSM_BF16) return wide ? go(__nv_bfloat16(), std::integral_constant<int, 128>()) : go(__nv_bfloat16(), std::integral_constant<int, 64>());
+  return wide ? go(__half(), std::integral_constant<int, 128>()) : go(__half(), std::integral_constant<int, 64>());
+}
+
+extern "C" int64_t ssm_gated_delta_chunked_bwd_scratch_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim, int32_t vdim) {
+  return gd::up(gd::chunk_bound(batch, len, num_seqs, gd::C) * heads * (int64_t)gd::width(kdim) * vdim * 2);
+}
+
+extern "C" int ssm_gated_delta_chunked_bwd(const ssm_gated_delta_bwd_args* args, void* kept, void* scratch, int32_t* status, ssm_stream_t stream) {
+  SSM_REQUIRE(args, SSM_ERR_NULL, "gated_delta: NULL arguments");
+  const ssm_gated_delta_args& f = args->fwd;
+  gd::ChunkWalk w{};
+  if (const int rc = gd::check(f, w.a)) return rc;
+  SSM_REQUIRE(ssm_gated_delta_chunked_supported(&f), SSM_ERR_UNSUPPORTED, "gated_delta: these operands do not go to the tensor cores");
+  if (w.a.seqs == 0) return SSM_OK;
+  SSM_REQUIRE(args->dout && args->dq && args->dk && args->dv && args->dg && args->dbeta && kept && scratch, SSM_ERR_NULL, "gated_delta backward: NULL pointer");
+  SSM_REQUIRE(w.a.group == 1 || args->dqk, SSM_ERR_NULL, "gated_delta backward: shared keys need the dqk scratch");
+  SSM_REQUIRE(aligned_to(args->dout, 16) && aligned_to(args->dv, 16) && aligned_to(args->dq, 16) && aligned_to(args->dk, 16) && aligned_to(args->dfinal, 16) && aligned_to(args->dqk, 16) &&
+                  aligned_to(kept, 256) && aligned_to(scratch, 256),
+              SSM_ERR_ALIGN, "gated_delta backward: misaligned pointer");
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  w.a.where.per = (f.len + gd::C - 1) / gd::C;
+  const int64_t chunks = gd::chunks_of(f);
+  const gd::Layout l = gd::layout_of(chunks, f.heads, f.kdim, f.vdim, true);
+  unsigned char* base = reinterpret_cast<unsigned char*>(kept);
+  w.in = {nullptr, nullptr, base + l.y, base + l.wb, reinterpret_cast<float*>(base + l.vec), status};
+  w.initial = args->dfinal, w.o = args->dv, w.last = args->dinitial, w.last_dtype = SSM_F32, w.states = scratch;
+  const int64_t row = (int64_t)f.heads * f.vdim;
+  gd::bind_context();
+  gd::WalkMaps maps;
+  if (const int rc = gd::encode_map(&maps.q, f.q, f.kdim, f.key_heads, f.len, f.batch, f.q_sh, f.q_st, f.q_sb, f.io_dtype)) return rc;
+  if (const int rc = gd::encode_map(&maps.k, f.k, f.kdim, f.key_heads, f.len, f.batch, f.k_sh, f.k_st, f.k_sb, f.io_dtype)) return rc;
+  if (const int rc = gd::encode_map(&maps.v, args->dout, f.vdim, f.heads, f.len, f.batch, f.vdim, row, row * f.len, f.io_dtype)) return rc;
+  if (const int rc = gd::encode_map(&maps.o, args->dv, f.vdim, f.heads, f.len, f.batch, f.vdim, row, row * f.len, f.io_dtype)) return rc;
+  const gd::GradMaps gm{maps.q, maps.k, maps.v, maps.o};
+  gd::ChunkGrads g{};
+  g.a = w.a, g.rest = base + l.rest, g.states = base + l.states, g.dstates = scratch, g.dq = args->dq, g.dk = args->dk, g.dqk = w.a.group > 1 ? args->dqk : nullptr;
+  g.dg = args->dg, g.dbeta = args->dbeta, g.tokens = (int64_t)f.batch * f.len, g.status = status;
+  auto go = [&](auto type, auto kd) {
+    using T = decltype(type);
+    constexpr int KD = decltype(kd)::value;
+    if (const int rc = gd::launch_chunks<T, KD, true>(w, maps, st)) return rc;
+    const int smem = gd::GradSmem<KD>::ALLOC;
+    if (const cudaError_t e = cudaFuncSetAttribute(gd::grads_kernel<T, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return set_error("grads_kernel: %s", cudaGetErrorString(e)), (int)e;
+    gd::grads_kernel<T, KD><<<dim3((unsigned)chunks, f.heads), gd::kGradThreads, smem, st>>>(g, gm);
+    if (const int rc = launch_status("grads_kernel")) return rc;
+    return g.dqk ? gd::fold_heads(g.dqk, g.dq, g.dk, g.tokens, f.kdim, f.key_heads, w.a.group, f.io_dtype, st) : (int)SSM_OK;
   };
   const bool wide = f.kdim > 64;
   if (f.io_dtype == SSM_BF16) return wide ? go(__nv_bfloat16(), std::integral_constant<int, 128>()) : go(__nv_bfloat16(), std::integral_constant<int, 64>());

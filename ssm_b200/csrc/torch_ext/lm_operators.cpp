@@ -106,8 +106,8 @@ struct DeltaCall final : Call {
     c10::cuda::CUDAGuard guard(v.device());
     Tensor o = at::empty({nb, nl, nh, vd}, v.options()), fin;
     if (cu.defined()) table = at::empty({ssm_gated_delta_table_ints((int)nb, (int)nl, (int)seqs)}, v.options().dtype(at::kInt));
-    if (train) chunked = false;
-    if (train) {
+    if (chunked && init.defined() && reinterpret_cast<uintptr_t>(init.data_ptr()) % 16 != 0) init = init.clone();
+    if (train && !chunked) {
       rest = at::empty({nb, nl, nh, vd}, f32());
       states = at::empty({ssm_gated_delta_chunks((int)nb, (int)nl, (int)seqs * cu.defined()), nh, vd, kd}, f32());
     }
@@ -115,8 +115,7 @@ struct DeltaCall final : Call {
     fill(a);
     a.o = o.data_ptr();
     if (want_final) fin = at::empty({seqs, nh, vd, kd}, fp32_state ? f32() : v.options()), a.final_state = fin.data_ptr(), a.final_dtype = dtype_code(fin, "gated_delta_scan");
-    if (chunked && init.defined() && reinterpret_cast<uintptr_t>(init.data_ptr()) % 16 != 0) init = init.clone(), a.initial_state = init.data_ptr<float>();
-    if (chunked && ssm_gated_delta_chunked_supported(&a)) {
+    if (chunked) {
       ssd_poll(v.get_device());  // a wait that ran out in an earlier launch surfaces here, without a synchronisation
       const auto bytes = v.options().dtype(at::kByte);
       Tensor scratch = at::empty({ssm_gated_delta_chunked_scratch_bytes((int)nb, (int)nl, a.num_seqs, (int)nh, (int)kd)}, bytes);
@@ -134,16 +133,26 @@ struct DeltaCall final : Call {
     Tensor go = grads[0].defined() ? like(grads[0], v) : at::zeros({nb, nl, nh, vd}, v.options()), gfin, dinit, dqk;
     if (grads.size() > 1 && grads[1].defined()) gfin = f32c(grads[1]);
     Tensor dq = at::empty({nb, nl, nk, kd}, v.options()), dk = at::empty_like(dq), dv = at::empty({nb, nl, nh, vd}, v.options());
-    Tensor dg = at::empty({nb, nl, nh}, f32()), db = at::empty_like(dg), dv32 = v.scalar_type() == at::kFloat ? dv : at::empty({nb, nl, nh, vd}, f32()), dstates = at::empty_like(states);
+    Tensor dg = at::empty({nb, nl, nh}, f32()), db = at::empty_like(dg), dv32, dstates;
     if (nh != nk) dqk = at::empty({2, nb, nl, nh, kd}, f32());
     if (init_grad) dinit = at::empty({seqs, nh, vd, kd}, f32());
     ssm_gated_delta_bwd_args a{};
     fill(a.fwd);
+    auto aligned = [&](Tensor& t) {
+      if (t.defined() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) t = t.clone();
+    };
+    if (chunked) aligned(go), aligned(gfin);
     a.dout = go.data_ptr(), a.dfinal = gfin.defined() ? gfin.data_ptr<float>() : nullptr;
     a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv = dv.data_ptr(), a.dg = dg.data_ptr<float>(), a.dbeta = db.data_ptr<float>();
-    a.dinitial = dinit.defined() ? dinit.data_ptr<float>() : nullptr, a.dv32 = dv32.data_ptr<float>(), a.dstates = dstates.data_ptr<float>();
-    a.dqk = dqk.defined() ? dqk.data_ptr<float>() : nullptr;
-    run(ssm_gated_delta_bwd(&a, stream_of(v)));
+    a.dinitial = dinit.defined() ? dinit.data_ptr<float>() : nullptr, a.dqk = dqk.defined() ? dqk.data_ptr<float>() : nullptr;
+    if (chunked) {
+      Tensor scratch = at::empty({ssm_gated_delta_chunked_bwd_scratch_bytes((int)nb, (int)nl, a.fwd.num_seqs, (int)nh, (int)kd, (int)vd)}, v.options().dtype(at::kByte));
+      run(ssm_gated_delta_chunked_bwd(&a, kept.data_ptr(), scratch.data_ptr(), ssd_status(v.get_device()).data_ptr<int32_t>(), stream_of(v)));
+    } else {
+      dv32 = v.scalar_type() == at::kFloat ? dv : at::empty({nb, nl, nh, vd}, f32()), dstates = at::empty_like(states);
+      a.dv32 = dv32.data_ptr<float>(), a.dstates = dstates.data_ptr<float>();
+      run(ssm_gated_delta_bwd(&a, stream_of(v)));
+    }
     variable_list res = {cast(dq, t_q), cast(dk, t_k), cast(dv, t_v)};
     if (g.defined()) res.push_back(cast(dg, t_g));
     res.push_back(cast(db, t_beta));
