@@ -1,11 +1,12 @@
 // Log probabilities of given tokens (with entropy and top alternatives) and distillation from a teacher's top logits.
 //
-// Both are one pass over a row of logits with a running maximum m, s = sum e^{(x - m)/T} and, for the entropy,
-// w = sum (x - m)/T e^{(x - m)/T}: log p_i = (x_i - m)/T - ln s and H = ln s - w / s.  The backward pass is one more read of the row and
-// one write of its gradient.  Bound: HBM (two or four bytes an element each way).  A row goes to one CTA, or to a cluster of up to
-// eight that join their sums through distributed shared memory where the rows alone would not fill the GPU.
+// Both are one pass over a row of logits.  With c = log2(e) / T and a running reference M (c times the largest logit so far), d = c x - M:
+// s = sum 2^d and, for the entropy, w = sum d 2^d; then log2 p_i = d_i - log2 s and H = (log2 s - w / s) ln 2.  M is rounded, but the same in every
+// term, so that it drops out.  The backward pass is one more read of the row and one write of its gradient.  Bound: HBM (two or four bytes an element
+// each way), beside 16 exponentials a cycle and SM: 91 us of them where 8192 x 50280 bf16 logits take 126 us to read.  A row goes to one CTA, or to a
+// cluster of up to eight that join their sums through distributed shared memory where the rows alone would not fill the GPU.
 //
-// Top alternatives: the k-th largest of the threads' own maxima bounds the k-th largest logit from below, so a second
+// Top alternatives: the k-th largest of the maxima of groups of threads bounds the k-th largest logit from below, so a second
 // pass over the row (which then lies in the L2) keeps the few elements at or above it, and ranks them by (value, lowest id).
 #include <cooperative_groups.h>
 
@@ -19,8 +20,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kUnroll = 4;       // 16-byte pieces a thread has in flight
-constexpr int kCandidates = 1024;  // kept elements of a slice; more (many equal logits) go through rounds of one maximum each
+constexpr int kCandidates = 1024;  // kept elements of a slice above the bound, and at it
 constexpr int kMaxTop = 128;
+constexpr int kGroups = kThreads / 2;  // groups of threads whose maxima are looked at, at most
 constexpr int kMaxTeacher = 1024;
 
 enum Flags { kEntropy = 1, kTop = 2 };
@@ -34,8 +36,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 // larger key: larger value, among equal ones the lower id
 __device__ __forceinline__ uint64_t key_of(float x, int id) { return ((uint64_t)order_of(x) << 32) | (uint32_t)~id; }
 
-// f(x, id) for the elements [lo, hi) of a row: 16-byte pieces between a ragged head and tail.  `lanes` threads share the work; this one is `me`.
-// P pieces are requested before the first is used.
+// one(x, id) for the elements [lo, hi) of a row in a ragged head and tail, piece(raw, ids) for the 16-byte pieces between, P of them requested before
+// the first is used.  `lanes` threads share the work; this one is `me`.
 template <typename T, int P, typename F, typename G>
 __device__ __forceinline__ void walk(const T* row, int lo, int hi, int me, int lanes, F&& one, G&& piece) {
   constexpr int V = Vec16<T>::N;
@@ -47,38 +49,84 @@ __device__ __forceinline__ void walk(const T* row, int lo, int hi, int me, int l
   int i = me;
   for (; i + (P - 1) * lanes < body; i += P * lanes) {
     Vec16<T> r[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) r[p].raw = src[i + p * lanes];
-    float f[P][V];
-#pragma unroll
-    for (int p = 0; p < P; ++p) r[p].unpack(f[p]);
     int ids[P];
 #pragma unroll
-    for (int p = 0; p < P; ++p) ids[p] = at + (i + p * lanes) * V;
-    piece(f, ids, std::integral_constant<int, P>{});
+    for (int p = 0; p < P; ++p) r[p].raw = src[i + p * lanes], ids[p] = at + (i + p * lanes) * V;
+    piece(r, ids);
   }
   for (; i < body; i += lanes) {
-    Vec16<T> r;
-    r.raw = src[i];
-    float f[1][V];
-    r.unpack(f[0]);
+    Vec16<T> r[1];
+    r[0].raw = src[i];
     const int ids[1] = {at + i * V};
-    piece(f, ids, std::integral_constant<int, 1>{});
+    piece(r, ids);
   }
   const int tail = at + body * V;
   if (me < hi - tail) one(to_f<T>(row[tail + me]), tail + me);
 }
 
+// two fp32 values in a register pair: one instruction for both
+typedef unsigned long long pair_t;
+__device__ __forceinline__ pair_t pair_of(float x, float y) {
+  pair_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void parts_of(pair_t p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+  pair_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+  pair_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// the largest (BIG) or smallest value of 16-byte pieces; a NaN makes the result NaN (NAN_COUNTS), or is passed over
+template <bool BIG, bool NAN_COUNTS, typename T, int P>
+__device__ __forceinline__ float extreme(const Vec16<T> (&r)[P]) {
+  if constexpr (std::is_same<T, float>::value) {
+    float top = BIG ? -INFINITY : INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      float f[4];
+      r[p].unpack(f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = BIG ? fmaxf(top, f[e]) : fminf(top, f[e]), bad = bad || f[e] != f[e];
+    }
+    return NAN_COUNTS && bad ? __uint_as_float(0x7fc00000u) : top;
+  } else {
+    using V2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+    auto of2 = [](V2 a, V2 b) { return !BIG ? __hmin2(a, b) : NAN_COUNTS ? __hmax2_nan(a, b) : __hmax2(a, b); };
+    V2 top;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const uint32_t w[4] = {r[p].raw.x, r[p].raw.y, r[p].raw.z, r[p].raw.w};
+      const V2 a = of2(*reinterpret_cast<const V2*>(&w[0]), *reinterpret_cast<const V2*>(&w[1])), b = of2(*reinterpret_cast<const V2*>(&w[2]), *reinterpret_cast<const V2*>(&w[3]));
+      top = p ? of2(top, of2(a, b)) : of2(a, b);
+    }
+    const float lo = to_f<T>(top.x), hi = to_f<T>(top.y);
+    if constexpr (NAN_COUNTS) return lo != lo ? lo : hi != hi ? hi : fmaxf(lo, hi);
+    else return BIG ? fmaxf(lo, hi) : fminf(lo, hi);
+  }
+}
+
+// m: the largest logit seen, M: c m, the reference of s and w.  Logits below kFloor count for nothing here, whose c x might overflow: beside any other they
+// do not, and rows without any other are looked at again.  A NaN in s stays
+constexpr float kFloor = -1e37f;
 struct Sums {
-  float m, s, w;
+  float m, M, s, w;
 };
-// c: log2(e) / T.  w in units of base-2 exponents
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, 0.f};  // NaN sums stay NaN
-  const float da = fmaxf((a.m - m) * c, -1e30f), db = fmaxf((b.m - m) * c, -1e30f);
-  const float ea = ex2_approx(da), eb = ex2_approx(db);
-  return {m, a.s * ea + b.s * eb, ea * fmaf(a.s, da, a.w) + eb * fmaf(b.s, db, b.w)};
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+  const bool first = a.m >= b.m;
+  const Sums &hi = first ? a : b, &lo = first ? b : a;
+  const float d = lo.m == kFloor ? 0.f : lo.M - hi.M, e = lo.m == kFloor ? 1.f : ex2_approx(d);  // nothing in lo: s is 0 or NaN
+  return {hi.m, hi.M, hi.s + lo.s * e, hi.w + e * fmaf(lo.s, fmaxf(d, -1e30f), lo.w)};
+}
+__device__ __forceinline__ Sums exchanged(const Sums& a, int off) {
+  return {__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.M, off), __shfl_xor_sync(0xffffffffu, a.s, off), __shfl_xor_sync(0xffffffffu, a.w, off)};
 }
 
 struct StatsArgs {
@@ -93,7 +141,7 @@ struct StatsArgs {
   float* entropy;
   float* top_logp;
   int64_t* top_ids;
-  float4* stats;  // m, log2 s, entropy, unused
+  float4* stats;  // M, log2 s, entropy, 0; m in M's place and 2 where all logits lie below kFloor; 1 for a row of -inf
 };
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -130,11 +178,11 @@ template <typename T, int FLAGS, bool DISTILL>
 __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, const int cluster) {
   __shared__ Sums part[kThreads / 32];
   __shared__ Sums mine;
-  __shared__ __align__(16) float maxima[kThreads];
-  __shared__ uint64_t cand[kCandidates];
+  __shared__ __align__(16) float maxima[kGroups];
+  __shared__ uint64_t cand[(FLAGS & kTop) ? 2 * kCandidates : 1];  // above the bound; at it
   __shared__ uint64_t best[kMaxTop];
   __shared__ uint64_t round_best[kThreads / 32];
-  __shared__ int count;
+  __shared__ int count, equals;
   __shared__ float bound_s;
   __shared__ float teach[DISTILL ? kMaxTeacher : 1];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -145,66 +193,86 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
   const int per = ((a.vocab + cluster - 1) / cluster + 63) / 64 * 64;
   const int lo = min(a.vocab, part_of * per), hi = part_of == cluster - 1 ? a.vocab : min(a.vocab, lo + per);
 
-  Sums me{-INFINITY, 0.f, 0.f};
   const float c = a.c;
-  auto raise = [&](float top) {
-    if (top > me.m) {
-      const float d = fmaxf((me.m - top) * c, -1e30f), e = ex2_approx(d);
-      if constexpr ((FLAGS & kEntropy) != 0) me.w = e * fmaf(me.s, d, me.w);
-      me.s *= e, me.m = top;
-    }
-  };
-  auto add = [&](float x, float base) {
-    const float d = (x - base) * c, e = ex2_approx(d);
-    me.s += e;
-    if constexpr ((FLAGS & kEntropy) != 0) me.w = fmaf(e, fmaxf(d, -1e30f), me.w);
-  };
-  walk<T, kUnroll>(
-      row, lo, hi, tid, kThreads,
-      [&](float x, int) {
-        raise(x);
-        add(x, me.m == -INFINITY ? 0.f : me.m);
-      },
-      [&](const auto& f, const int*, auto pieces) {
-        constexpr int V = Vec16<T>::N;
-        float top = f[0][0];
+  const pair_t c2 = pair_of(c, c);
+  Sums me{kFloor, 0.f, 0.f, 0.f};
+  {
+    pair_t s2 = pair_of(0.f, 0.f), w2 = s2, M2 = s2;
+    auto raise = [&](float top) {
+      if (top > me.m) {
+        const float M = top * c, d = me.M - M, e = me.m == kFloor ? 0.f : ex2_approx(d);
+        const pair_t e2 = pair_of(e, e), none = pair_of(0.f, 0.f);
+        if constexpr ((FLAGS & kEntropy) != 0) w2 = fma2(e2, fma2(s2, pair_of(d, d), w2), none);
+        s2 = fma2(e2, s2, none);
+        me.m = top, me.M = M, M2 = pair_of(-M, -M);
+      }
+    };
+    walk<T, kUnroll>(
+        row, lo, hi, tid, kThreads,
+        [&](float x, int) {
+          raise(x);
+          const float d = fmaf(x, c, -me.M), e = ex2_approx(d);
+          s2 = add2(s2, pair_of(e, 0.f));
+          if constexpr ((FLAGS & kEntropy) != 0) w2 = add2(w2, pair_of(e * fmaxf(d, -1e30f), 0.f));
+        },
+        [&](const auto& r, const int*) {
+          constexpr int V = Vec16<T>::N, P = sizeof(r) / sizeof(r[0]);
+          raise(extreme<true, false>(r));
+          auto add = [&](auto masked) {
 #pragma unroll
-        for (int p = 0; p < decltype(pieces)::value; ++p)
+            for (int p = 0; p < P; ++p) {
+              float f[V];
+              r[p].unpack(f);
 #pragma unroll
-          for (int j = 0; j < V; ++j) top = fmaxf(top, f[p][j]);
-        raise(top);
-        const float base = me.m == -INFINITY ? 0.f : me.m;
-#pragma unroll
-        for (int p = 0; p < decltype(pieces)::value; ++p)
-#pragma unroll
-          for (int j = 0; j < V; ++j) add(f[p][j], base);
-      });
+              for (int j = 0; j < V; j += 2) {
+                const pair_t d2 = fma2(pair_of(f[j], f[j + 1]), c2, M2);
+                float d0, d1;
+                parts_of(d2, d0, d1);
+                const pair_t e2 = pair_of(ex2_approx(d0), ex2_approx(d1));
+                s2 = add2(s2, e2);
+                if constexpr ((FLAGS & kEntropy) != 0) w2 = fma2(e2, decltype(masked)::value ? pair_of(fmaxf(d0, -1e30f), fmaxf(d1, -1e30f)) : d2, w2);
+              }
+            }
+          };
+          if ((FLAGS & kEntropy) != 0 && extreme<false, false>(r) < -1e30f) add(std::true_type());  // 0 times -inf
+          else add(std::false_type());
+        });
+    float x, y;
+    parts_of(s2, x, y), me.s = x + y;
+    parts_of(w2, x, y), me.w = x + y;
+  }
 
-  if constexpr ((FLAGS & kTop) != 0) maxima[tid] = me.m;
+  if constexpr ((FLAGS & kTop) != 0) {  // maxima of groups of threads, at least twice as many as alternatives where that is possible
+    const int size = a.top_k <= kGroups / 8 ? 8 : a.top_k <= kGroups / 4 ? 4 : 2;
+    float top = me.m == kFloor ? -INFINITY : me.m;
+    for (int off = 1; off < size; off *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (tid % size == 0) maxima[tid / size] = top;
+  }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) {
-    const Sums o{__shfl_xor_sync(0xffffffffu, me.m, off), __shfl_xor_sync(0xffffffffu, me.s, off), __shfl_xor_sync(0xffffffffu, me.w, off)};
-    me = lane & off ? join(o, me, c) : join(me, o, c);  // the same order on both sides
+    const Sums o = exchanged(me, off);
+    me = lane & off ? join(o, me) : join(me, o);  // the same order on both sides
   }
   if (lane == 0) part[warp] = me;
-  if (tid == 0) count = 0, bound_s = -INFINITY;
+  if (tid == 0) count = equals = 0, bound_s = -INFINITY;
   __syncthreads();
   if (warp == 0) {
-    me = lane < kThreads / 32 ? part[lane] : Sums{-INFINITY, 0.f, 0.f};
+    me = lane < kThreads / 32 ? part[lane] : Sums{kFloor, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) {
-      const Sums o{__shfl_xor_sync(0xffffffffu, me.m, off), __shfl_xor_sync(0xffffffffu, me.s, off), __shfl_xor_sync(0xffffffffu, me.w, off)};
-      me = lane & off ? join(o, me, c) : join(me, o, c);
+      const Sums o = exchanged(me, off);
+      me = lane & off ? join(o, me) : join(me, o);
     }
     if (lane == 0) mine = me;
   }
 
   if constexpr ((FLAGS & kTop) != 0) {
     const int k = a.top_k;
-    {  // the k-th largest of the threads' maxima
+    const int groups = kThreads / (k <= kGroups / 8 ? 8 : k <= kGroups / 4 ? 4 : 2);
+    if (tid < groups) {  // the k-th largest of the groups' maxima
       const float own = maxima[tid];
       int above = 0;
-      for (int i = 0; i < kThreads; i += 4) {
+      for (int i = 0; i < groups; i += 4) {
         const float4 v = *reinterpret_cast<const float4*>(&maxima[i]);
         above += (v.x > own || (v.x == own && i < tid)) + (v.y > own || (v.y == own && i + 1 < tid)) + (v.z > own || (v.z == own && i + 2 < tid)) +
                  (v.w > own || (v.w == own && i + 3 < tid));
@@ -212,31 +280,55 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
       if (above == k - 1) bound_s = own;
     }
     __syncthreads();
-    const uint32_t bound = order_of(bound_s);
+    const float bound = bound_s;
     auto keep = [&](float x, int id) {
-      if (order_of(x) >= bound) {
+      if (x == bound) {
+        const int at = atomicAdd(&equals, 1);
+        if (at < kCandidates) cand[kCandidates + at] = key_of(x, id);
+      } else if (!(x < bound)) {  // NaN counts as the largest
         const int at = atomicAdd(&count, 1);
         if (at < kCandidates) cand[at] = key_of(x, id);
       }
     };
-    walk<T, 2>(row, lo, hi, tid, kThreads, keep, [&](const auto& f, const int* ids, auto pieces) {
-      constexpr int V = Vec16<T>::N;
+    walk<T, kUnroll>(row, lo, hi, tid, kThreads, keep, [&](const auto& r, const int* ids) {
+      constexpr int V = Vec16<T>::N, P = sizeof(r) / sizeof(r[0]);
+      if (extreme<true, true>(r) < bound) return;
 #pragma unroll
-      for (int p = 0; p < decltype(pieces)::value; ++p)
+      for (int p = 0; p < P; ++p) {
+        float f[V];
+        r[p].unpack(f);
 #pragma unroll
-        for (int j = 0; j < V; ++j) keep(f[p][j], ids[p] + j);
+        for (int j = 0; j < V; ++j) keep(f[j], ids[p] + j);
+      }
     });
     if (tid < kMaxTop) best[tid] = 0;  // below every key
     __syncthreads();
     const int n = count;
+    int m = equals;
+    if (m > kCandidates) {  // many at the bound: the first of them in the row's order
+      if (warp == 0) {
+        int found = 0;
+        for (int id = lo; id < hi && found < k; id += 32) {
+          const bool is = id + lane < hi && to_f<T>(row[id + lane]) == bound;
+          const uint32_t votes = __ballot_sync(0xffffffffu, is);
+          const int at = found + __popc(votes & ((1u << lane) - 1));
+          if (is && at < k) cand[kCandidates + at] = key_of(bound, id + lane);
+          found += __popc(votes);
+        }
+      }
+      m = k;
+      __syncthreads();
+    }
     if (n <= kCandidates) {
-      for (int i = tid; i < n; i += kThreads) {  // keys differ (ids do), so ranks do
-        const uint64_t own = cand[i];
+      for (int i = tid; i < n + m; i += kThreads) {  // keys differ (ids do), so ranks do
+        const uint64_t own = cand[i < n ? i : kCandidates + i - n];
         int above = 0;
         for (int j = 0; j < n; ++j) above += cand[j] > own;
+        if (i >= n && above < k)
+          for (int j = 0; j < m; ++j) above += cand[kCandidates + j] > own;
         if (above < k) best[above] = own;
       }
-    } else {  // more equal logits than fit: one maximum at a time
+    } else {  // a few threads hold most of the largest: one maximum at a time
       uint64_t last = ~0ull;
       for (int j = 0; j < k; ++j) {
         uint64_t top = 0;
@@ -244,12 +336,12 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
           const uint64_t key = key_of(x, id);
           if (key < last && key > top) top = key;
         };
-        walk<T, 2>(row, lo, hi, tid, kThreads, look, [&](const auto& f, const int* ids, auto pieces) {
+        walk<T, 1>(row, lo, hi, tid, kThreads, look, [&](const auto& r, const int* ids) {
           constexpr int V = Vec16<T>::N;
+          float f[V];
+          r[0].unpack(f);
 #pragma unroll
-          for (int p = 0; p < decltype(pieces)::value; ++p)
-#pragma unroll
-            for (int e = 0; e < V; ++e) look(f[p][e], ids[p] + e);
+          for (int e = 0; e < V; ++e) look(f[e], ids[0] + e);
         });
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) {
@@ -273,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
     cl.sync();
     if (part_of == 0) {
       all = *cl.map_shared_rank(&mine, 0);
-      for (int i = 1; i < cluster; ++i) all = join(all, *cl.map_shared_rank(&mine, i), c);
+      for (int i = 1; i < cluster; ++i) all = join(all, *cl.map_shared_rank(&mine, i));
       if constexpr ((FLAGS & kTop) != 0) {  // the slices' best, joined
         const int k = a.top_k, n = cluster * k;
         for (int i = tid; i < n; i += kThreads) cand[i] = cl.map_shared_rank(&best[0], i / k)[i % k];
@@ -296,12 +388,39 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
     all = mine;
   }
 
-  const bool none = all.m == -INFINITY && all.s == 0.f;  // a row of -inf
-  const float log2s = none ? 0.f : log2f(all.s), lns = log2s * kLn2;
-  const float entropy = none ? 0.f : lns - kLn2 * all.w / all.s;
-  auto logp_of = [&](float x) { return none ? -INFINITY : fmaf(x - all.m, a.inv_t, -lns); };
+  float kind = 0.f;
+  if (all.s == 0.f) {  // nothing above kFloor: the whole row once more, by this CTA, with differences before products
+    __syncthreads();
+    auto over = [&](float v, auto f) {  // over the threads
+      for (int off = 16; off >= 1; off >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, off));
+      if (lane == 0) part[warp].m = v;
+      __syncthreads();
+      v = part[0].m;
+      for (int i = 1; i < kThreads / 32; ++i) v = f(v, part[i].m);
+      __syncthreads();
+      return v;
+    };
+    auto sum = [](float x, float y) { return x + y; };
+    float m = -INFINITY, s = 0.f, w = 0.f;
+    for (int id = tid; id < a.vocab; id += kThreads) m = fmaxf(m, to_f<T>(row[id]));
+    m = over(m, [](float x, float y) { return fmaxf(x, y); });
+    if (m != -INFINITY)
+      for (int id = tid; id < a.vocab; id += kThreads) {
+        const float d = (to_f<T>(row[id]) - m) * c, e = ex2_approx(d);
+        s += e, w = fmaf(e, fmaxf(d, -1e30f), w);
+      }
+    s = over(s, sum), w = over(w, sum);
+    all = {m, m, s, w};
+    kind = m == -INFINITY ? 1.f : 2.f;
+  }
+  const bool none = kind == 1.f;
+  const float log2s = none ? 0.f : log2f(all.s), entropy = none ? 0.f : kLn2 * (log2s - all.w / all.s);
+  auto logp_of = [&](float x) {
+    if (none) return -INFINITY;
+    return x < kFloor ? fmaf(x - all.m, a.inv_t, -kLn2 * log2s) : kLn2 * (fmaf(x, c, -all.M) - log2s);
+  };
   if (tid == 0) {
-    if (a.stats) a.stats[r] = make_float4(all.s != all.s ? all.s : all.m, log2s, entropy, 0.f);
+    if (a.stats) a.stats[r] = make_float4(all.M, log2s, entropy, kind);
     if constexpr (!DISTILL) {
       const int64_t t = a.targets[r];
       a.logp[r] = t == a.ignore ? 0.f : t < 0 || t >= a.vocab ? __uint_as_float(0x7fc00000u) : logp_of(to_f<T>(row[t]));
@@ -347,12 +466,9 @@ struct GradArgs {
 
 // d logits = (sum_e coef_e 1[id_e] - p (sum_e coef_e + dH (log p + H))) / T for the log probabilities (an entry e per given token and per
 // alternative); dloss (q - sum_j t_j 1[id_j]) / T for the distillation.
-template <typename T, bool DISTILL>
-__global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradArgs g) {
+template <typename T, bool DISTILL, bool PLAIN>
+__device__ __forceinline__ void row_grad(const GradArgs& g, const float4 st, int* col, float* coef) {
   constexpr int V = Vec16<T>::N;
-  constexpr int kEntries = DISTILL ? kMaxTeacher : kMaxTop + 1;
-  __shared__ int col[kEntries];
-  __shared__ float coef[kEntries];
   const StatsArgs& a = g.f;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x / g.splits;
@@ -361,8 +477,7 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradArgs g) {
   T* out = reinterpret_cast<T*>(g.out) + r * (int64_t)a.vocab;
   const int per = ((a.vocab + g.splits - 1) / g.splits + 63) / 64 * 64;
   const int lo = min(a.vocab, part_of * per), hi = part_of == g.splits - 1 ? a.vocab : min(a.vocab, lo + per);
-  const float4 st = a.stats[r];
-  const bool none = st.x == -INFINITY;
+  const bool none = st.w == 1.f;
   const float dl = g.dlogp ? g.dlogp[r] : 0.f, dh = !DISTILL && g.dentropy ? g.dentropy[r] : 0.f;
   int n;
   float on_p;  // gradient = p (on_p + on_plogp log2 p) + entries
@@ -399,28 +514,30 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradArgs g) {
     }
   }
   const float on_plogp = -dh * kLn2 * a.inv_t, c = a.c;
-  const float base = none ? 0.f : st.x;
   auto grad = [&](float x) {
-    const float e = fmaf(x - base, c, -st.y);
+    const float e = (PLAIN ? fmaf(x, c, -st.x) : (x - st.x) * c) - st.y;
     const float p = ex2_approx(e);
-    return none ? 0.f : p * fmaf(on_plogp, fmaxf(e, -1e30f), on_p);
+    if constexpr (DISTILL) return none ? 0.f : p * on_p;
+    else return none ? 0.f : p * fmaf(on_plogp, fmaxf(e, -1e30f), on_p);
   };
   // the rows of the gradient are dense, those of the logits need not be: whole pieces where both lie alike
   const bool alike = (reinterpret_cast<uintptr_t>(row + lo) % 16) == (reinterpret_cast<uintptr_t>(out + lo) % 16);
   auto one = [&](float x, int id) { out[id] = from_f<T>(grad(x)); };
-  auto piece = [&](const auto& f, const int* ids, auto pieces) {
+  auto piece = [&](const auto& r, const int* ids) {
+    constexpr int P = sizeof(r) / sizeof(r[0]);
 #pragma unroll
-    for (int p = 0; p < decltype(pieces)::value; ++p) {
-      float d[V];
+    for (int p = 0; p < P; ++p) {
+      float f[V];
+      r[p].unpack(f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = grad(f[p][j]);
+      for (int j = 0; j < V; ++j) f[j] = grad(f[j]);
       if (alike) {
         Vec16<T> o;
-        o.pack(d);
+        o.pack(f);
         o.store_stream(out + ids[p]);
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) out[ids[p] + j] = from_f<T>(d[j]);
+        for (int j = 0; j < V; ++j) out[ids[p] + j] = from_f<T>(f[j]);
       }
     }
   };
@@ -439,6 +556,16 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradArgs g) {
     }
     if (first) out[id] = from_f<T>(grad(to_f<T>(row[id])) + add);
   }
+}
+
+template <typename T, bool DISTILL>
+__global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradArgs g) {
+  constexpr int kEntries = DISTILL ? kMaxTeacher : kMaxTop + 1;
+  __shared__ int col[kEntries];
+  __shared__ float coef[kEntries];
+  const float4 st = g.f.stats[blockIdx.x / g.splits];
+  if (st.w == 2.f) row_grad<T, DISTILL, false>(g, st, col, coef);  // all logits of the row below kFloor
+  else row_grad<T, DISTILL, true>(g, st, col, coef);
 }
 
 // CTAs a row: as many as keep about two waves of CTAs busy, each with at least 4096 elements

@@ -125,6 +125,29 @@ def test_masked_logits(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [700, 40000])
+def test_few_live_logits_among_masked_ones(dtype, vocab):
+    """Fewer live logits than alternatives: the rest of the alternatives are the first masked ones.  One thread holding most of the largest."""
+    from ssm_b200 import ops
+
+    x = torch.full((6, vocab), -INF, dtype=torch.float64)
+    x[0, [3, 5, vocab - 1]] = torch.tensor([1.0, 2.0, 1.0], dtype=torch.float64)
+    x[1] = torch.finfo(dtype).min
+    x[1, [8, vocab // 2]] = torch.tensor([-1.0, 4.0], dtype=torch.float64)
+    x[2, ::2] = torch.finfo(dtype).min
+    x[3, vocab - 40:] = 1.0
+    x[4] = 0.5 * torch.arange(vocab).remainder(8)
+    x[5] = torch.finfo(dtype).min
+    targets = torch.tensor([5, 8, 0, vocab - 1, 7, 3])
+    want = lm_oracle.token_log_probs(x, targets, 1.0, 30)
+    got = ops.token_log_probs(x.to(dtype).cuda(), targets.cuda(), top_k=30, return_entropy=True)
+    near(got[0], want[0], bar(vocab, 4))
+    near(got[1], want[1], 20 * bar(vocab, 4))
+    near(got[2], want[2], bar(vocab, 4), 4 * 2.0 ** -24)
+    assert torch.equal(got[3].cpu(), want[3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_nan_inf_and_targets_outside(dtype):
     from ssm_b200 import ops
 
