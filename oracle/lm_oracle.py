@@ -40,7 +40,7 @@ def token_log_probs(logits, targets, temperature=1.0, top_k=0, ignore_index=-100
     at = torch.where(kept, targets, torch.zeros_like(targets))
     got = torch.where(kept, torch.gather(logp, -1, at[..., None])[..., 0], torch.zeros((), dtype=logits.dtype))
     p = torch.exp(logp)
-    entropy = -torch.where(p > 0, p * logp.clamp_min(-1e300), torch.zeros((), dtype=logits.dtype)).sum(-1)
+    entropy = -torch.where(p > 0, p * logp.clamp_min(torch.finfo(logp.dtype).min), torch.zeros((), dtype=logits.dtype)).sum(-1)
     _, ids = torch.sort(logits.detach(), dim=-1, descending=True, stable=True)
     ids = ids[..., :top_k]
     return got, entropy, torch.gather(logp, -1, ids), ids
@@ -54,5 +54,30 @@ def topk_distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0):
     empty = (t == -float("inf")).all(-1, keepdim=True)
     logt = torch.log_softmax(torch.where(empty, torch.zeros_like(t), t), -1)
     pt = torch.where(empty, torch.zeros_like(t), torch.exp(logt))
-    term = pt * (logt.clamp_min(-1e300) - torch.gather(logq, -1, teacher_ids.clamp_min(0)))
+    term = pt * (logt.clamp_min(torch.finfo(logt.dtype).min) - torch.gather(logq, -1, teacher_ids.clamp_min(0)))
     return torch.where(pt > 0, term, torch.zeros_like(term)).sum(-1)
+
+
+def namespace():
+    """The state-space oracle's operators with these beside them, under the names and signatures of ``ssm_b200.ops``."""
+    from types import SimpleNamespace
+
+    from . import ssm_oracle
+
+    def gated_delta_scan(q, k, v, g, beta, scale=None, initial_state=None, return_final_state=False, keep_state_fp32=False, cu_seqlens=None):
+        o, s = gated_delta(q, k, v, g, beta, scale, initial_state, cu_seqlens)
+        return (o, s) if return_final_state else o
+
+    def gated_delta_step(state, q, k, v, g, beta, scale=None):
+        o, s = gated_delta(q[:, None], k[:, None], v[:, None], None if g is None else g[:, None], beta[:, None], scale, state.clone())
+        with torch.no_grad():
+            state.copy_(s)
+        return o[:, 0]
+
+    def log_probs(logits, targets, temperature=1.0, top_k=0, return_entropy=False, ignore_index=-100):
+        got = token_log_probs(logits, targets, temperature, top_k, ignore_index)
+        out = got[:1] + (got[1:2] if return_entropy else ()) + (got[2:] if top_k else ())
+        return out if len(out) > 1 else out[0]
+
+    return SimpleNamespace(**{n: f for n, f in vars(ssm_oracle).items() if not n.startswith("_")}, gated_delta_scan=gated_delta_scan,
+                           gated_delta_step=gated_delta_step, token_log_probs=log_probs, topk_distill_loss=topk_distill_loss)

@@ -6,11 +6,13 @@ Every layer is upstream's fused-add-norm block (src/ssm/modules/block.py:109-131
 and ``hidden = norm(residual)`` are ONE call of ``fused_layer_norm(..., return_residual=True)`` (upstream routes that
 to an external Triton kernel), followed by the mixer; the final norm folds the last residual add the same way
 (lm.py:378-387).  The residual stream is kept in fp32 when ``residual_in_fp32``.  Mixers: ``ssm_cfg["layer"]`` selects
-``"Mamba1"`` (selective scan) or ``"Mamba2"`` (state-space-dual scan with a d_state axis, upstream Mamba-2 layout).
+``"Mamba1"`` (selective scan) or ``"Mamba2"`` (state-space-dual scan with a d_state axis, upstream Mamba-2 layout); beyond upstream ``"GatedDelta"``
+(the gated delta rule).
 Attention layers and the gated MLP of upstream's hybrid configurations are outside the operator hot path and are
 rejected.  Beyond upstream: ``forward(..., sharded=True, group=pg)`` runs a Mamba-2 stack on one contiguous shard of a
 sequence split over ranks (`ssm_b200.seqpar`), and ``step`` decodes one token against caches allocated by
-``allocate_inference_cache``.
+``allocate_inference_cache``; ``MambaLMHeadModel.score`` gives the log probabilities of given tokens and ``distill_loss`` the divergence from a
+teacher's top logits, both differentiable.
 """
 
 from __future__ import annotations
@@ -22,7 +24,7 @@ from typing import Any, Optional
 import torch
 from torch import Tensor, nn
 
-from .mixer import Mamba1Block, Mamba2Block
+from .mixer import GatedDeltaBlock, Mamba1Block, Mamba2Block
 
 CausalLMOutput = namedtuple("CausalLMOutput", ["logits"])
 
@@ -71,10 +73,10 @@ class MixerModel(nn.Module):
         cfg = dict(ssm_cfg or {})
         kind = cfg.pop("layer", "Mamba1")
         cfg.pop("dt_init", None)
-        if kind == "Mamba2":
-            cfg.pop("dt_rank", None)  # Mamba-2 has one step size per head, projected straight from the input
-        if kind not in ("Mamba1", "Mamba2"):
-            raise ValueError("ssm_cfg['layer'] must be either 'Mamba1' or 'Mamba2'")
+        if kind in ("Mamba2", "GatedDelta"):
+            cfg.pop("dt_rank", None)  # one step size per head, projected straight from the input
+        if kind not in ("Mamba1", "Mamba2", "GatedDelta"):
+            raise ValueError("ssm_cfg['layer'] must be 'Mamba1', 'Mamba2' or 'GatedDelta'")
         self.kind, self.rms_norm, self.eps, self.residual_in_fp32 = kind, bool(rms_norm), norm_epsilon, bool(residual_in_fp32)
         self.d_model = d_model
         self._ops = ops
@@ -82,7 +84,7 @@ class MixerModel(nn.Module):
         self.embedding = nn.Embedding(vocab_size, d_model, **kw)
         std = (initializer_cfg or {}).get("initializer_range", 0.02)
         nn.init.normal_(self.embedding.weight, std=std)
-        block = Mamba1Block if kind == "Mamba1" else Mamba2Block
+        block = {"Mamba1": Mamba1Block, "Mamba2": Mamba2Block, "GatedDelta": GatedDeltaBlock}[kind]
         # a block's own norm weight (`norm_w` / `pre_norm_w`) serves as the pre-norm of its layer
         self.layers = nn.ModuleList([block(d_model, eps=norm_epsilon, ops=ops, **cfg, **kw) for _ in range(n_layer)])
         self.norm_f_weight = nn.Parameter(torch.ones(d_model, **kw))
@@ -169,6 +171,24 @@ class MambaLMHeadModel(nn.Module):
         if num_last_tokens > 0:
             hidden = hidden[:, -num_last_tokens:, :]
         return CausalLMOutput(logits=self.lm_head(hidden))
+
+    def score(self, input_ids: Tensor, labels: Optional[Tensor] = None, temperature: float = 1.0, top_k: int = 0, return_entropy: bool = False,
+              ignore_index: int = -100, **mixer_kwargs):
+        """Log probabilities of a sequence's own tokens, each given those before it: ``input_ids (B, L)`` -> ``(B, L - 1)`` fp32, with the entropies and
+        the ``top_k`` alternatives behind them as in ``ops.token_log_probs``.  ``labels (B, L)`` in the place of the tokens; those equal to
+        ``ignore_index`` give 0."""
+        logits = self.forward(input_ids, **mixer_kwargs).logits
+        targets = input_ids if labels is None else labels
+        # the logits as they lie, their last row with nothing to predict
+        targets = torch.cat([targets[:, 1:], torch.full_like(targets[:, :1], ignore_index)], 1)
+        got = self.backbone._namespace().token_log_probs(logits, targets, temperature, top_k, return_entropy, ignore_index)
+        return tuple(t[:, :-1] for t in got) if isinstance(got, tuple) else got[:, :-1]
+
+    def distill_loss(self, input_ids: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0, **mixer_kwargs) -> Tensor:
+        """Divergence of this model's distributions from a teacher's top logits ``(B, L, k)`` with their ids, per position: ``(B, L)`` fp32
+        (``ops.topk_distill_loss``)."""
+        logits = self.forward(input_ids, **mixer_kwargs).logits
+        return self.backbone._namespace().topk_distill_loss(logits, teacher_logits, teacher_ids, temperature)
 
     @torch.no_grad()
     def generate(self, input_ids: Tensor, max_length: int, cuda_graph: bool = False) -> Tensor:

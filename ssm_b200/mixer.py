@@ -350,3 +350,127 @@ class Mamba2Block(nn.Module):
     def mixer_step(self, tok: Tensor, cache) -> Tensor:
         """The mixer alone on one normed token: tok (B, d_model) -> (B, d_model); ``cache`` from `allocate_inference_cache`."""
         return mamba2_mixer_step(self._namespace(), self._parameters, self._cfg(), tok, cache[0], cache[1])
+
+
+def _unit(ops: Any, x: Tensor, weight: Tensor) -> Tensor:
+    """Rows over the last axis scaled to norm one: RMSNorm with the weight ``K ** -0.5``."""
+    return ops.fused_layer_norm(x.reshape(x.shape[0], -1, x.shape[-1]), weight, None, is_rms=True, eps=1e-6 / x.shape[-1]).view(x.shape)
+
+
+def gated_delta_mixer_forward(ops: Any, w: dict, cfg: dict, u: Tensor) -> Tensor:
+    """The gated delta mixer alone on normed activations u (B, L, d_model) -> (B, L, d_model).
+
+    Projections of u to q, k (key heads), v (value heads), a step size and a write strength per value head and the gate z; depthwise causal conv + SiLU
+    on q, k and v (channels-last); keys and queries to norm one; log decay ``-exp(A_log) softplus(step + dt_bias)``; the gated delta rule;
+    RMSNorm per head, times SiLU(z); out projection.  ``cfg``: heads, key_heads, headdim, d_state, eps."""
+    nb, nl, dm = u.shape
+    nh, nk, vd, kd = cfg["heads"], cfg["key_heads"], cfg["headdim"], cfg["d_state"]
+    u2 = u.reshape(nb * nl, dm)
+
+    def proj(name):
+        return torch.matmul(u2, w[name].t()).view(nb, nl, -1)
+
+    def conv(name):
+        t = proj("in_" + name)
+        if nl == t.shape[2]:  # as many steps as channels: (B, L, C) would be taken for (B, C, L)
+            return ops.dw_causal_conv(t.transpose(1, 2), w["conv_" + name], w["conv_" + name + "_b"], "silu").transpose(1, 2).contiguous()
+        return ops.dw_causal_conv(t, w["conv_" + name], w["conv_" + name + "_b"], "silu")
+
+    q, k = (_unit(ops, conv(n).reshape(nb, nl, nk, kd), w["unit"]) for n in "qk")
+    v = conv("v").reshape(nb, nl, nh, vd)
+    g = -torch.exp(w["A_log"]) * nn.functional.softplus(proj("in_a").float() + w["dt_bias"])
+    o = ops.gated_delta_scan(q, k, v, g, torch.sigmoid(proj("in_b")))
+    o = ops.fused_layer_norm(o.reshape(nb, nl * nh, vd), w["norm_w"], None, is_rms=True, eps=cfg.get("eps", 1e-5)).view(nb, nl, nh * vd)
+    return torch.matmul((o * nn.functional.silu(proj("in_z"))).view(nb * nl, nh * vd), w["out_proj"].t()).view(nb, nl, dm)
+
+
+def gated_delta_mixer_step(ops: Any, w: dict, cfg: dict, tok: Tensor, conv_states: tuple, state: Tensor) -> Tensor:
+    """One decode token through the gated delta mixer: tok (B, d_model), normed -> (B, d_model).  ``conv_states``: the rolling windows of the q, k and
+    v convolutions ((B, C_i, K) fp32 each); ``state (B, H, V, K)`` fp32; all updated in place."""
+    nb = tok.shape[0]
+    nh, nk, vd, kd = cfg["heads"], cfg["key_heads"], cfg["headdim"], cfg["d_state"]
+    q, k, v = (ops.dw_causal_conv_update(st, tok @ w["in_" + n].t(), w["conv_" + n], w["conv_" + n + "_b"], "silu") for n, st in zip("qkv", conv_states))
+    q, k = (_unit(ops, t.view(nb, 1, nk, kd), w["unit"]).view(nb, nk, kd) for t in (q, k))
+    g = -torch.exp(w["A_log"]) * nn.functional.softplus((tok @ w["in_a"].t()).float() + w["dt_bias"])
+    o = ops.gated_delta_step(state, q, k, v.view(nb, nh, vd), g, torch.sigmoid(tok @ w["in_b"].t()))
+    o = ops.fused_layer_norm(o, w["norm_w"], None, is_rms=True, eps=cfg.get("eps", 1e-5)).view(nb, nh * vd)
+    return (o * nn.functional.silu(tok @ w["in_z"].t())) @ w["out_proj"].t()
+
+
+class GatedDeltaBlock(nn.Module):
+    """Pre-norm block around the gated delta rule: ``forward(hidden, residual) -> (mixer output, residual stream)``, as :class:`Mamba2Block`.
+    ``expand * d_model`` channels in value heads of ``headdim``; ``key_heads`` (a divisor of their number, all of them by default) with keys of
+    ``d_state``."""
+
+    def __init__(self, d_model: int, d_state: int = 128, d_conv: int = 4, expand: int = 2, headdim: int = 128, key_heads: Optional[int] = None,
+                 dt_min: float = 1e-3, dt_max: float = 1e-1, dt_init_floor: float = 1e-4, eps: float = 1e-5, device=None, dtype=None, ops: Any = None) -> None:
+        super().__init__()
+        d_inner = expand * d_model
+        if d_inner % headdim:
+            raise ValueError("expand * d_model must be a multiple of headdim.")
+        heads = d_inner // headdim
+        key_heads = heads if key_heads is None else int(key_heads)
+        if key_heads <= 0 or heads % key_heads:
+            raise ValueError("key_heads must divide the heads.")
+        self.d_model, self.d_inner, self.d_state, self.d_conv = d_model, d_inner, d_state, d_conv
+        self.heads, self.key_heads, self.headdim, self.eps = heads, key_heads, headdim, eps
+        self._ops = ops
+        kw = dict(device=device, dtype=dtype)
+        f32 = dict(device=device, dtype=torch.float32)
+        dk = key_heads * d_state
+
+        def lin(o, i):
+            return nn.Parameter(torch.randn(o, i, **kw) / i ** 0.5)
+
+        def conv_w(c):
+            return nn.Parameter((torch.rand(c, d_conv, **kw) - 0.5) * (2.0 / d_conv ** 0.5))
+
+        self.pre_norm_w = nn.Parameter(torch.ones(d_model, **kw))
+        self.in_q, self.in_k, self.in_v, self.in_z = lin(dk, d_model), lin(dk, d_model), lin(d_inner, d_model), lin(d_inner, d_model)
+        self.in_a, self.in_b = lin(heads, d_model), lin(heads, d_model)
+        self.conv_q, self.conv_k, self.conv_v = conv_w(dk), conv_w(dk), conv_w(d_inner)
+        self.conv_q_b, self.conv_k_b, self.conv_v_b = (nn.Parameter(torch.zeros(c, **kw)) for c in (dk, dk, d_inner))
+        dt = torch.exp(torch.rand(heads, **f32) * (math.log(dt_max) - math.log(dt_min)) + math.log(dt_min)).clamp(min=dt_init_floor)
+        self.dt_bias = nn.Parameter(dt + torch.log(-torch.expm1(-dt)))
+        self.A_log = nn.Parameter(torch.log(torch.empty(heads, **f32).uniform_(1.0, 16.0)))
+        self.norm_w = nn.Parameter(torch.ones(headdim, **kw))
+        self.out_proj = lin(d_model, d_inner)
+        self.register_buffer("unit", torch.full((d_state,), d_state ** -0.5, **f32), persistent=False)
+
+    def _namespace(self):
+        if self._ops is not None:
+            return self._ops
+        from . import ops  # the CUDA operators; raises if the library has not been built
+
+        return ops
+
+    _WEIGHTS = ("in_q", "in_k", "in_v", "in_z", "in_a", "in_b", "conv_q", "conv_k", "conv_v", "conv_q_b", "conv_k_b", "conv_v_b", "dt_bias", "A_log", "norm_w",
+                "out_proj", "unit")
+
+    def _weights(self) -> dict:
+        return {n: getattr(self, n) for n in self._WEIGHTS}
+
+    def _cfg(self) -> dict:
+        return dict(heads=self.heads, key_heads=self.key_heads, headdim=self.headdim, d_state=self.d_state, eps=self.eps)
+
+    def forward(self, hidden: Tensor, residual: Optional[Tensor] = None):
+        if hidden.ndim != 3 or hidden.shape[-1] != self.d_model:
+            raise ValueError("hidden_states must have shape (B, L, d_model).")
+        u, residual = self._namespace().fused_layer_norm(hidden, self.pre_norm_w, None, residual=residual, is_rms=True, eps=self.eps, prenorm=True,
+                                                         residual_in_fp32=True, return_residual=True)
+        return self.mixer_forward(u), residual
+
+    def mixer_forward(self, u: Tensor) -> Tensor:
+        """The mixer alone on normed activations: u (B, L, d_model) -> (B, L, d_model)."""
+        return gated_delta_mixer_forward(self._namespace(), self._weights(), self._cfg(), u)
+
+    def allocate_inference_cache(self, batch_size: int, dtype: Optional[torch.dtype] = None):
+        """((conv windows of q, k, v: (B, C_i, K)), state (B, H, V, K)), all fp32 and zero-filled."""
+        del dtype
+        z = lambda *s: torch.zeros(batch_size, *s, device=self.in_q.device, dtype=torch.float32)  # noqa: E731
+        dk = self.key_heads * self.d_state
+        return (z(dk, self.d_conv), z(dk, self.d_conv), z(self.d_inner, self.d_conv)), z(self.heads, self.headdim, self.d_state)
+
+    def mixer_step(self, tok: Tensor, cache) -> Tensor:
+        """The mixer alone on one normed token: tok (B, d_model) -> (B, d_model); ``cache`` from `allocate_inference_cache`."""
+        return gated_delta_mixer_step(self._namespace(), self._weights(), self._cfg(), tok, cache[0], cache[1])
