@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
 //   dk_i = beta_i y_i - gam_i S0^T w_i - sum_{j<i} G_ij N2_ij beta_j k_j
 //   dg_t = gam_64 <S0, D> + sum_{i<t} beta_i suf_i k_i.(D^T r_i) + sum_{i>=t} gam_i (scale q_i.(S0^T do_i) - k_i.(S0^T w_i)) + sum_{j<t<=i} M_ij,
 //   M_ij = G_ij beta_j (scale N1_ij q_i.k_j - N2_ij k_i.k_j): every path from before t to t or behind it
-// Eight warps, each 16 tokens x half of the columns, products by mma.sync (15 Mflop a chunk).  Bound: 145 KB read and 32 KB written a chunk, and
+// Sixteen warps, each 16 tokens x a quarter of the columns, products by mma.sync (15 Mflop a chunk).  Bound: 145 KB read and 32 KB written a chunk, and
 // that one CTA fills an SM's shared memory, so that its copies and its products take turns.
 struct GradMaps {
   CUtensorMap q, k, d, w;
@@ -887,12 +887,12 @@ struct ChunkGrads {
   int64_t tokens;
   int32_t* status;
 };
-constexpr int kGradThreads = 256, kSlice = 128;  // columns of v at a time
+constexpr int kGradThreads = 512, kSlice = 128;  // columns of v at a time
 template <int KD>
 struct GradSmem {
   static constexpr int KT = (KD / 64) * kTileBytes, VT = 2 * kTileBytes, RT = (C / 8) * kSlice * 16, ST = (KD / 8) * kSlice * 16;
   static constexpr int Q = 0, K = KT, D = 2 * KT, W = D + VT, R = W + VT, S = R + RT, DS = S + ST, Y1 = DS + ST, Y2 = Y1 + kTileBytes, A1 = Y2 + kTileBytes, A2 = A1 + kTileBytes,
-                       VEC = A2 + kTileBytes, TOTAL = VEC + 24 * C * 4;
+                       VEC = A2 + kTileBytes, TOTAL = VEC + (24 * C + kGradThreads / 32) * 4;
   static constexpr int ALLOC = TOTAL + 1024;
 };
 static_assert(GradSmem<128>::ALLOC <= 227 * 1024, "shared memory of an SM");
@@ -913,7 +913,7 @@ __device__ __forceinline__ void load_at(uint32_t (&f)[4], uint32_t tile, int m0,
 template <typename T, int KD>
 __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads g, const __grid_constant__ GradMaps maps) {
   using M = GradSmem<KD>;
-  constexpr int NB = KD / 16;  // blocks of eight columns of a warp: half of kdim
+  constexpr int NB = KD / 32;  // blocks of eight columns of a warp: a quarter of kdim
   extern __shared__ unsigned char smdyn[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t mbar;
@@ -936,8 +936,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
   }
   const uint32_t base = tc::smem_u32(sm), landed_bar = tc::smem_u32(&mbar);
   float* c = reinterpret_cast<float*>(sm + M::VEC);
-  float *beta = c + C, *gam = beta + C, *suf = gam + C, *rows = suf + C, *cols = rows + 2 * C;  // rows [2][C], cols [4][C]: sums of M
-  float *into = cols + 4 * C, *outof = into + 2 * C, *db = outof + 2 * C, *part = db + 2 * C;   // [2][C] each; 8 partial sums
+  float *beta = c + C, *gam = beta + C, *suf = gam + C, *rows = suf + C, *cols = rows + 4 * C;  // [4][C] each: sums of M
+  float *into = cols + 4 * C, *outof = into + 4 * C, *db = outof + 4 * C, *part = db + 4 * C;   // [4][C] each; a partial sum of every warp
   const int64_t pair = (int64_t)s.chunk * a.heads + h;
   const unsigned char* rest = reinterpret_cast<const unsigned char*>(g.rest) + pair * (C / 8) * a.vd * 16;
   const unsigned char* states = reinterpret_cast<const unsigned char*>(g.states) + pair * (KD / 8) * a.vd * 16;
@@ -971,8 +971,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
     __syncwarp();
     for (int i = lane; i < C; i += 32) gam[i] = ex2_approx(c[i]), suf[i] = ex2_approx(c[C - 1] - c[i]);
   }
-  const int r0 = (warp >> 1) * 16, half = warp & 1, c0 = half * 32, k_cols = half * (KD / 2), gi = lane >> 2, gj = (lane & 3) * 2;
-  float N1[4][4] = {}, N2[4][4] = {}, dQ[NB][4] = {}, dK[NB][4] = {}, y[NB][4] = {}, whole = 0.f;
+  const int r0 = (warp >> 2) * 16, quarter = (warp + (warp >> 2)) & 3, c0 = quarter * 16, k_cols = quarter * (KD / 4), gi = lane >> 2, gj = (lane & 3) * 2;
+  float N1[2][4] = {}, N2[2][4] = {}, dQ[NB][4] = {}, dK[NB][4] = {}, y[NB][4] = {}, whole = 0.f;
   for (int v0 = 0, turn = 0; v0 < a.vd; v0 += kSlice, ++turn) {
     const int nv = min(kSlice, a.vd - v0);
     if (!__syncthreads_and(phase_done(landed_bar, turn & 1))) {
@@ -1003,12 +1003,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
       load_a(fd, base + M::D, r0, k0, lane);
       load_a(fw, base + M::W, r0, k0, lane);
       units_a(fr, base + M::R, r0, k0, lane);
-#pragma unroll
-      for (int n0 = 0; n0 < 32; n0 += 16) {
-        if (c0 + n0 > r0) continue;
-        units_b(b, base + M::R, c0 + n0, k0, lane);
-        mma16816<T>(N1[n0 / 8], fd, b[0], b[1]), mma16816<T>(N1[n0 / 8 + 1], fd, b[2], b[3]);
-        mma16816<T>(N2[n0 / 8], fw, b[0], b[1]), mma16816<T>(N2[n0 / 8 + 1], fw, b[2], b[3]);
+      if (c0 <= r0) {
+        units_b(b, base + M::R, c0, k0, lane);
+        mma16816<T>(N1[0], fd, b[0], b[1]), mma16816<T>(N1[1], fd, b[2], b[3]);
+        mma16816<T>(N2[0], fw, b[0], b[1]), mma16816<T>(N2[1], fw, b[2], b[3]);
       }
 #pragma unroll
       for (int n0 = 0; n0 < NB * 8; n0 += 16) {
@@ -1037,24 +1035,22 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
   }
   whole = warp_sum(whole);
   if (lane == 0) part[warp] = whole;
-  {  // pairs of tokens: this warp's 16 x 32
-    float QK[4][4] = {}, KK[4][4] = {};
+  {  // pairs of tokens: this warp's 16 x 16
+    float QK[2][4] = {}, KK[2][4] = {};
+    if (c0 <= r0) {
 #pragma unroll
-    for (int k0 = 0; k0 < KD; k0 += 16) {
-      uint32_t fq[4], fk[4], b[4];
-      load_a(fq, base + M::Q, r0, k0, lane);
-      load_a(fk, base + M::K, r0, k0, lane);
-#pragma unroll
-      for (int n0 = 0; n0 < 32; n0 += 16) {
-        if (c0 + n0 > r0) continue;
-        load_b(b, base + M::K, c0 + n0, k0, lane);
-        mma16816<T>(QK[n0 / 8], fq, b[0], b[1]), mma16816<T>(QK[n0 / 8 + 1], fq, b[2], b[3]);
-        mma16816<T>(KK[n0 / 8], fk, b[0], b[1]), mma16816<T>(KK[n0 / 8 + 1], fk, b[2], b[3]);
+      for (int k0 = 0; k0 < KD; k0 += 16) {
+        uint32_t fq[4], fk[4], b[4];
+        load_a(fq, base + M::Q, r0, k0, lane);
+        load_a(fk, base + M::K, r0, k0, lane);
+        load_b(b, base + M::K, c0, k0, lane);
+        mma16816<T>(QK[0], fq, b[0], b[1]), mma16816<T>(QK[1], fq, b[2], b[3]);
+        mma16816<T>(KK[0], fk, b[0], b[1]), mma16816<T>(KK[1], fk, b[2], b[3]);
       }
     }
     float row[2] = {0.f, 0.f};
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
+    for (int nb = 0; nb < 2; ++nb) {
       const int j0 = c0 + nb * 8 + gj;
       float y1[4], y2[4], a1[4], a2[4], col[2] = {0.f, 0.f};
 #pragma unroll
@@ -1069,7 +1065,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
       }
 #pragma unroll
       for (int off = 4; off <= 16; off *= 2) col[0] += __shfl_xor_sync(0xffffffffu, col[0], off), col[1] += __shfl_xor_sync(0xffffffffu, col[1], off);
-      if (gi == 0) cols[(warp >> 1) * C + j0] = col[0], cols[(warp >> 1) * C + j0 + 1] = col[1];
+      if (gi == 0) cols[(warp >> 2) * C + j0] = col[0], cols[(warp >> 2) * C + j0 + 1] = col[1];
       const int lo = swz(r0 + gi, j0 >> 3) + gj * 2, hi = swz(r0 + gi + 8, j0 >> 3) + gj * 2;
       *reinterpret_cast<uint32_t*>(sm + M::Y1 + lo) = pack2<T>(y1[0], y1[1]), *reinterpret_cast<uint32_t*>(sm + M::Y1 + hi) = pack2<T>(y1[2], y1[3]);
       *reinterpret_cast<uint32_t*>(sm + M::Y2 + lo) = pack2<T>(y2[0], y2[1]), *reinterpret_cast<uint32_t*>(sm + M::Y2 + hi) = pack2<T>(y2[2], y2[3]);
@@ -1079,16 +1075,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       row[e] += __shfl_xor_sync(0xffffffffu, row[e], 1), row[e] += __shfl_xor_sync(0xffffffffu, row[e], 2);
-      if ((lane & 3) == 0) rows[half * C + r0 + gi + e * 8] = row[e];
+      if ((lane & 3) == 0) rows[quarter * C + r0 + gi + e * 8] = row[e];
     }
   }
   // the states' parts, scaled, and what dg takes of them
   const float gm[2] = {gam[r0 + gi], gam[r0 + gi + 8]}, sf[2] = {suf[r0 + gi], suf[r0 + gi + 8]}, bt[2] = {beta[r0 + gi], beta[r0 + gi + 8]};
-  auto row_sums = [&](float (&x)[2], float* to) {  // over the four lanes of a row, to this half's place
+  auto row_sums = [&](float (&x)[2], float* to) {  // over the four lanes of a row, to this quarter's place
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       x[e] += __shfl_xor_sync(0xffffffffu, x[e], 1), x[e] += __shfl_xor_sync(0xffffffffu, x[e], 2);
-      if ((lane & 3) == 0) to[half * C + r0 + gi + e * 8] = x[e];
+      if ((lane & 3) == 0) to[quarter * C + r0 + gi + e * 8] = x[e];
     }
   };
   auto pair_at = [&](int tile, int e, int nb) {  // two neighbouring elements of q or k
@@ -1179,10 +1175,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = 2 * lane + e;
-      float col = 0.f;
-      for (int b = 0; b < 4; ++b) col += (b * 16 + 15 > i ? cols[b * C + i] : 0.f);
-      x[e] = into[i] + into[C + i] + rows[i] + rows[C + i] - col;
-      z[e] = outof[i] + outof[C + i];
+      x[e] = z[e] = 0.f;
+      for (int b = 0; b < 4; ++b) x[e] += into[b * C + i] + rows[b * C + i] - (b * 16 + 15 > i ? cols[b * C + i] : 0.f), z[e] += outof[b * C + i];
     }
     float behind = x[0] + x[1], before = z[0] + z[1];  // inclusive sums from the end, and from the start
 #pragma unroll
@@ -1197,7 +1191,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
       const int i = 2 * lane + e;
       if (i < n) {
         g.dg[(tok + i) * a.heads + h] = total + (e ? behind - x[0] : behind) + (e ? before - z[1] : before - z[0] - z[1]);
-        g.dbeta[(tok + i) * a.heads + h] = db[i] + db[C + i];
+        g.dbeta[(tok + i) * a.heads + h] = db[i] + db[C + i] + db[2 * C + i] + db[3 * C + i];
       }
     }
   }
