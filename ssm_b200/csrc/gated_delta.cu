@@ -91,11 +91,11 @@ struct WalkArgs {
   float* states;  // forward: the state before every chunk; backward: the adjoint state behind it
 };
 
-template <typename T, int E, bool BACK>
-__global__ void __launch_bounds__(kThreads) walk_kernel(const WalkArgs w) {
-  constexpr int KP = kLanes * E, kTile = E > 16 ? 8 : 16;  // two buffers within 48 KB
+template <typename T, int kLanes, int E, bool BACK>
+__global__ void __launch_bounds__(kLanes* kRows) walk_kernel(const WalkArgs w) {
+  constexpr int KP = kLanes * E, kThreads = kLanes * kRows, kTile = KP > 128 ? 8 : 16, kOuts = BACK ? 1 : 2;  // two buffers within 48 KB
   __shared__ __align__(16) float ks[2][kTile][KP], qs[2][kTile][KP];
-  __shared__ float vs[2][kTile][kRows], decay[2][kTile], beta[2][kTile], kq[2][kTile], out_s[2][kTile][kRows];
+  __shared__ float vs[2][kTile][kRows], decay[2][kTile], beta[2][kTile], out_s[2][kOuts][kTile][kRows];
   const Args& a = w.a;
   const int tid = threadIdx.x, lane = tid % kLanes, row = tid / kLanes, h = blockIdx.y, v0 = blockIdx.x * kRows, kh = h / a.group;
   T* o = reinterpret_cast<T*>(w.o);
@@ -120,18 +120,18 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const WalkArgs w) {
   const int64_t v_st = BACK ? (int64_t)a.heads * vd : a.v.st;
   const int64_t state_at = (((int64_t)s.seq * a.heads + h) * vd + v) * a.kd;
 
-  float S[E];
+  float2 S[E / 2];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = (e / 4) * (4 * kLanes) + lane * 4 + e % 4;
-    S[e] = w.initial && live && c < a.kd ? w.initial[state_at + c] : 0.f;
+    (e % 2 ? S[e / 2].y : S[e / 2].x) = w.initial && live && c < a.kd ? w.initial[state_at + c] : 0.f;
   }
   auto keep = [&](int chunk) {
     float* to = w.states + (((int64_t)chunk * a.heads + h) * vd + v) * a.kd;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (e / 4) * (4 * kLanes) + lane * 4 + e % 4;
-      if (live && c < a.kd) to[c] = S[e];
+      if (live && c < a.kd) to[c] = e % 2 ? S[e / 2].y : S[e / 2].x;
     }
   };
 
@@ -148,7 +148,14 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const WalkArgs w) {
     }
   };
   constexpr int NK = kTile * KP / kThreads, NV = kTile * kRows / kThreads;
-  float kr[NK], qr[NK], vr[NV], gr = 1.f, br = 0.f;
+  // As they lie in memory: a conversion here would wait for them.
+  T kr[NK], qr[NK], vr[NV];
+  uint32_t raw = 0;
+  auto raw_at = [&](const Rows& x, int dtype, int t) -> uint32_t {
+    const int64_t at = s.b * x.sb + t * x.st + h * x.sh;
+    return dtype == SSM_F32 ? __ldg(reinterpret_cast<const uint32_t*>(x.p) + at) : __ldg(reinterpret_cast<const uint16_t*>(x.p) + at);
+  };
+  auto value = [&](int dtype) { return dtype == SSM_F32 ? __uint_as_float(raw) : dtype == SSM_BF16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half((uint16_t)raw)); };
   auto request = [&](int i) {
     int from, count;
     tile_at(i, from, count);
@@ -156,57 +163,46 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const WalkArgs w) {
     for (int j = 0; j < NK; ++j) {
       const int at = tid + j * kThreads, t = at / KP, c = at % KP;
       const bool in = t < count && c < a.kd;
-      kr[j] = in ? to_f<T>(kp[(int64_t)(from + t) * a.k.st + c]) : 0.f;
-      qr[j] = in ? to_f<T>(qp[(int64_t)(from + t) * a.q.st + c]) * a.scale : 0.f;
+      kr[j] = in ? kp[(int64_t)(from + t) * a.k.st + c] : from_f<T>(0.f);
+      qr[j] = in ? qp[(int64_t)(from + t) * a.q.st + c] : from_f<T>(0.f);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = tid + j * kThreads, t = at / kRows, c = v0 + at % kRows;
-      vr[j] = t < count && c < a.vd ? to_f<T>(vp[(int64_t)(from + t) * v_st + c]) : 0.f;
+      vr[j] = t < count && c < a.vd ? vp[(int64_t)(from + t) * v_st + c] : from_f<T>(0.f);
     }
-    if (tid < kTile) gr = tid < count ? decay_of(a, s.b, from + tid, h) : 1.f;
-    else if (tid < 2 * kTile) br = tid - kTile < count ? beta_of(a, s.b, from + tid - kTile, h) : 0.f;
+    if (tid < kTile) raw = tid < count && a.g.p ? raw_at(a.g, a.g_dtype, from + tid) : 0;
+    else if (tid < 2 * kTile) raw = tid - kTile < count ? raw_at(a.beta, a.beta_dtype, from + tid - kTile) : 0;
   };
   auto place = [&](int buf) {
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
       const int at = tid + j * kThreads;
-      ks[buf][at / KP][at % KP] = kr[j], qs[buf][at / KP][at % KP] = qr[j];
+      ks[buf][at / KP][at % KP] = to_f<T>(kr[j]), qs[buf][at / KP][at % KP] = to_f<T>(qr[j]) * a.scale;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = tid + j * kThreads;
-      vs[buf][at / kRows][at % kRows] = vr[j];
+      vs[buf][at / kRows][at % kRows] = to_f<T>(vr[j]);
     }
-    if (tid < kTile) decay[buf][tid] = gr;
-    else if (tid < 2 * kTile) beta[buf][tid - kTile] = br;
+    if (tid < kTile) decay[buf][tid] = expf(value(a.g_dtype));  // without decays e^0
+    else if (tid < 2 * kTile) beta[buf][tid - kTile] = value(a.beta_dtype);
   };
-  auto dots = [&](int buf) {  // k.q of the tile's tokens, two a warp
-    const int wp = tid / 32, ln = tid % 32;
-    for (int t = wp; t < kTile; t += kThreads / 32) {
-      float d = 0.f;
-      for (int c = ln; c < KP; c += 32) d = fmaf(ks[buf][t][c], qs[buf][t][c], d);
-      d = warp_sum(d);
-      if (ln == 0) kq[buf][t] = d;
-    }
-  };
-  auto flush = [&](int i, int buf) {  // out_s[0]: o or w for the output; out_s[1]: r or w in fp32
+  auto flush = [&](int i, int buf) {  // forward o and r, back w
     int from, count;
     tile_at(i, from, count);
     for (int at = tid; at < count * kRows; at += kThreads) {
       const int t = at / kRows, c = v0 + at % kRows;
       if (c >= a.vd) continue;
       const int64_t to = (((int64_t)s.b * a.len + from + t) * a.heads + h) * vd + c;
-      if (o) o[to] = from_f<T>(out_s[0][t][at % kRows]);
-      if (w.rest) w.rest[to] = out_s[BACK ? 0 : 1][t][at % kRows];
+      if (o) o[to] = from_f<T>(out_s[buf][0][t][at % kRows]);
+      if (w.rest) w.rest[to] = out_s[buf][kOuts - 1][t][at % kRows];
     }
   };
   if (tiles > 0) {
     request(0);
     place(0);
   }
-  __syncthreads();
-  if (tiles > 0) dots(0);
   __syncthreads();
   for (int i = 0; i < tiles; ++i) {
     const int buf = i & 1;
@@ -218,54 +214,53 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const WalkArgs w) {
       if (!BACK && local % kChunk == 0) keep(s.chunk + local / kChunk);
       if (BACK && ((local + count) % kChunk == 0 || i == 0)) keep(s.chunk + (local + count - 1) / kChunk);
     }
-    for (int j = 0; j < count; ++j) {
-      const int t = BACK ? count - 1 - j : j;
-      const float al = decay[buf][t], be = beta[buf][t], x = vs[buf][t][row], c0 = kq[buf][t];
-      float kk[E], dk0 = 0.f, dk1 = 0.f, dq0 = 0.f, dq1 = 0.f;
-      if constexpr (!BACK) {
+    auto row_of = [&](const float(&from)[kTile][KP], int t, float2(&x)[E / 2]) {
 #pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(&ks[buf][t][e * kLanes + lane * 4]);
-          const float4 q4 = *reinterpret_cast<const float4*>(&qs[buf][t][e * kLanes + lane * 4]);
-          kk[e] = k4.x, kk[e + 1] = k4.y, kk[e + 2] = k4.z, kk[e + 3] = k4.w;
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) S[e + i4] *= al;
-          dk0 = fmaf(S[e], k4.x, dk0), dk1 = fmaf(S[e + 1], k4.y, dk1), dk0 = fmaf(S[e + 2], k4.z, dk0), dk1 = fmaf(S[e + 3], k4.w, dk1);
-          dq0 = fmaf(S[e], q4.x, dq0), dq1 = fmaf(S[e + 1], q4.y, dq1), dq0 = fmaf(S[e + 2], q4.z, dq0), dq1 = fmaf(S[e + 3], q4.w, dq1);
-        }
-        const float sk = group_sum<kLanes, 1>(dk0 + dk1), sq = group_sum<kLanes, 1>(dq0 + dq1);
-        const float r = x - sk, u = be * r;
-#pragma unroll
-        for (int e = 0; e < E; ++e) S[e] = fmaf(u, kk[e], S[e]);
-        if (lane == 0) out_s[0][t][row] = fmaf(c0, u, sq);
-        if (lane == 1 && w.rest) out_s[1][t][row] = r;
-      } else {
-        float qq[E];
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(&ks[buf][t][e * kLanes + lane * 4]);
-          const float4 q4 = *reinterpret_cast<const float4*>(&qs[buf][t][e * kLanes + lane * 4]);
-          kk[e] = k4.x, kk[e + 1] = k4.y, kk[e + 2] = k4.z, kk[e + 3] = k4.w;
-          qq[e] = q4.x, qq[e + 1] = q4.y, qq[e + 2] = q4.z, qq[e + 3] = q4.w;
-          dk0 = fmaf(S[e], k4.x, dk0), dk1 = fmaf(S[e + 1], k4.y, dk1), dk0 = fmaf(S[e + 2], k4.z, dk0), dk1 = fmaf(S[e + 3], k4.w, dk1);
-        }
-        const float du = fmaf(c0, x, group_sum<kLanes, 1>(dk0 + dk1)), ww = be * du;
-#pragma unroll
-        for (int e = 0; e < E; ++e) S[e] = al * fmaf(-ww, kk[e], fmaf(x, qq[e], S[e]));
-        if (lane == 0) out_s[0][t][row] = ww;
+      for (int e = 0; e < E; e += 4) {
+        const float4 z = *reinterpret_cast<const float4*>(&from[t][e * kLanes + lane * 4]);
+        x[e / 2] = make_float2(z.x, z.y), x[e / 2 + 1] = make_float2(z.z, z.w);
       }
+    };
+    auto dot = [&](const float2(&x)[E / 2]) {
+      float2 d[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) d[e % 2] = __ffma2_rn(S[e], x[e], d[e % 2]);
+      return group_sum<kLanes, 1>((d[0].x + d[1].x) + (d[0].y + d[1].y));
+    };
+    auto token = [&](int t) {
+      const float al = decay[buf][t], be = beta[buf][t], x = vs[buf][t][row];
+      float2 kk[E / 2], qq[E / 2];
+      row_of(ks[buf], t, kk), row_of(qs[buf], t, qq);
+      if constexpr (!BACK) {
+        const float r = fmaf(-al, dot(kk), x), u = be * r;
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) S[e] = __ffma2_rn(make_float2(u, u), kk[e], __fmul2_rn(make_float2(al, al), S[e]));
+        const float y = dot(qq);
+        out_s[buf][lane & 1][t][row] = lane & 1 ? r : y;  // lanes agree; no branch
+      } else {
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) S[e] = __ffma2_rn(make_float2(x, x), qq[e], S[e]);
+        const float ww = be * dot(kk), aw = -al * ww;
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) S[e] = __ffma2_rn(make_float2(aw, aw), kk[e], __fmul2_rn(make_float2(al, al), S[e]));
+        out_s[buf][0][t][row] = ww;
+      }
+    };
+    if (count == kTile) {  // tokens side by side in the instruction stream: only the state runs from one to the next
+#pragma unroll 4
+      for (int j = 0; j < kTile; ++j) token(BACK ? kTile - 1 - j : j);
+    } else {
+      for (int j = 0; j < count; ++j) token(BACK ? count - 1 - j : j);
     }
     if (i + 1 < tiles) place(buf ^ 1);
     __syncthreads();
-    if (i + 1 < tiles) dots(buf ^ 1);
-    flush(i, buf);
-    __syncthreads();
+    flush(i, buf);  // its place is written again after the next barrier
   }
   if (w.last && live) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (e / 4) * (4 * kLanes) + lane * 4 + e % 4;
-      if (c < a.kd) store_dyn(w.last, state_at + c, w.last_dtype, S[e]);
+      if (c < a.kd) store_dyn(w.last, state_at + c, w.last_dtype, e % 2 ? S[e / 2].y : S[e / 2].x);
     }
   }
 }
@@ -273,10 +268,10 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const WalkArgs w) {
 template <typename T, bool BACK>
 int launch_walk(const WalkArgs& w, cudaStream_t st) {
   const dim3 grid((w.a.vd + kRows - 1) / kRows, w.a.heads, w.a.seqs + (w.a.where.table ? 1 : 0));
-  if (w.a.kd <= 32) walk_kernel<T, 4, BACK><<<grid, kThreads, 0, st>>>(w);
-  else if (w.a.kd <= 64) walk_kernel<T, 8, BACK><<<grid, kThreads, 0, st>>>(w);
-  else if (w.a.kd <= 128) walk_kernel<T, 16, BACK><<<grid, kThreads, 0, st>>>(w);
-  else walk_kernel<T, 32, BACK><<<grid, kThreads, 0, st>>>(w);
+  if (w.a.kd <= 32) walk_kernel<T, 4, 8, BACK><<<grid, 4 * kRows, 0, st>>>(w);
+  else if (w.a.kd <= 64) walk_kernel<T, 4, 16, BACK><<<grid, 4 * kRows, 0, st>>>(w);
+  else if (w.a.kd <= 128) walk_kernel<T, 4, 32, BACK><<<grid, 4 * kRows, 0, st>>>(w);
+  else walk_kernel<T, 8, 32, BACK><<<grid, 8 * kRows, 0, st>>>(w);
   return launch_status(BACK ? "walk_kernel (backward)" : "walk_kernel");
 }
 template <bool BACK>
@@ -318,6 +313,9 @@ __host__ __device__ inline int padded(int n) { return (n + 3) / 4 * 4 + 4; }
 inline size_t grad_smem(int kd, int vd_tile) { return sizeof(float) * (2 * kChunk * padded(kd) + 3 * kChunk * padded(vd_tile) + 5 * kChunk * (kChunk + 1) + 16 * kChunk); }
 constexpr int kVTile = 128;  // columns of v at a time
 
+__device__ __forceinline__ float4 at4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float dot4(float4 a, float4 b, float sum) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, sum)))); }
+
 // A thread owns one element of kdim (rounds of kThreads of them where there are more) and all tokens of the chunk.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) grad_kernel(const GradArgs g) {
@@ -350,10 +348,11 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const GradArgs g) {
   float *al = KK + C * MP, *be = al + C, *gam = be + C, *suf = gam + C, *into = suf + C, *outof = into + C, *db = outof + C, *inner = db + C;
   const T* qp = reinterpret_cast<const T*>(a.q.p) + s.b * a.q.sb + kh * a.q.sh;
   const T* kp = reinterpret_cast<const T*>(a.k.p) + s.b * a.k.sb + kh * a.k.sh;
-  for (int at = tid; at < C * a.kd; at += kThreads) {
-    const int i = at / a.kd, c = at % a.kd;
-    q[i * KS + c] = i < n ? to_f<T>(qp[(int64_t)(s.t0 + i) * a.q.st + c]) * a.scale : 0.f;  // scale rides on q
-    k[i * KS + c] = i < n ? to_f<T>(kp[(int64_t)(s.t0 + i) * a.k.st + c]) : 0.f;
+  for (int at = tid; at < C * (KS - 4); at += kThreads) {
+    const int i = at / (KS - 4), c = at % (KS - 4);
+    const bool in = i < n && c < a.kd;
+    q[i * KS + c] = in ? to_f<T>(qp[(int64_t)(s.t0 + i) * a.q.st + c]) * a.scale : 0.f;  // scale rides on q
+    k[i * KS + c] = in ? to_f<T>(kp[(int64_t)(s.t0 + i) * a.k.st + c]) : 0.f;
   }
   if (tid < C) {
     al[tid] = tid < n ? decay_of(a, s.b, s.t0 + tid, h) : 1.f;
@@ -378,7 +377,10 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const GradArgs g) {
     const int i = at / C, j = at % C;
     float x = 0.f, y = 0.f;
     if (j <= i)
-      for (int c = 0; c < a.kd; ++c) x = fmaf(q[i * KS + c], k[j * KS + c], x), y = fmaf(k[i * KS + c], k[j * KS + c], y);
+      for (int c = 0; c < a.kd; c += 4) {  // rows are padded with zeros to whole vectors
+        const float4 kj = at4(&k[j * KS + c]);
+        x = dot4(at4(&q[i * KS + c]), kj, x), y = dot4(at4(&k[i * KS + c]), kj, y);
+      }
     QK[i * MP + j] = x, KK[i * MP + j] = y;
   }
   const float* S0 = g.states + ((int64_t)s.chunk * a.heads + h) * vd * a.kd;
@@ -400,12 +402,14 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const GradArgs g) {
         const bool loaded = a.vd <= kVTile && (c0 > 0 || i0 > 0);
         if (!loaded) {
           __syncthreads();
-          for (int at = tid; at < C * nv; at += kThreads) {
-            const int i = at / nv, x = at % nv;
+          const int whole_v = (nv + 3) / 4 * 4;
+          for (int at = tid; at < C * whole_v; at += kThreads) {
+            const int i = at / whole_v, x = at % whole_v;
             const int64_t from = ((tok + i) * a.heads + h) * vd + v0 + x;
-            r[i * VS + x] = i < n ? g.rest[from] : 0.f;
-            w[i * VS + x] = i < n ? g.w[from] : 0.f;
-            d[i * VS + x] = i < n ? to_f<T>(reinterpret_cast<const T*>(g.dout)[from]) : 0.f;
+            const bool in = i < n && x < nv;
+            r[i * VS + x] = in ? g.rest[from] : 0.f;
+            w[i * VS + x] = in ? g.w[from] : 0.f;
+            d[i * VS + x] = in ? to_f<T>(reinterpret_cast<const T*>(g.dout)[from]) : 0.f;
           }
           __syncthreads();
           if (c0 == 0 && i0 == 0)  // N1, N2 once over all of v
@@ -413,69 +417,59 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const GradArgs g) {
               const int i = at / C, j = at % C;
               if (j > i) continue;
               float x = N1[i * MP + j], y = N2[i * MP + j];
-              for (int v = 0; v < nv; ++v) x = fmaf(d[i * VS + v], r[j * VS + v], x), y = fmaf(w[i * VS + v], r[j * VS + v], y);
+              for (int v = 0; v < nv; v += 4) {
+                const float4 rj = at4(&r[j * VS + v]);
+                x = dot4(at4(&d[i * VS + v]), rj, x), y = dot4(at4(&w[i * VS + v]), rj, y);
+              }
               N1[i * MP + j] = x, N2[i * MP + j] = y;
             }
         }
         if (on)
-          for (int v = part; v < nv; v += parts) {
-            const float s0 = S0[(int64_t)(v0 + v) * a.kd + c], ds = dS[(int64_t)(v0 + v) * a.kd + c];
-            if (i0 == 0) whole = fmaf(s0, ds, whole);
+          for (int v = 4 * part; v < nv; v += 4 * parts) {
+            float s0[4], ds[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s0[e] = v + e < nv ? S0[(int64_t)(v0 + v + e) * a.kd + c] : 0.f, ds[e] = v + e < nv ? dS[(int64_t)(v0 + v + e) * a.kd + c] : 0.f;
+            const float4 s4 = make_float4(s0[0], s0[1], s0[2], s0[3]), d4 = make_float4(ds[0], ds[1], ds[2], ds[3]);
+            if (i0 == 0) whole = dot4(s4, d4, whole);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              D1[i] = fmaf(s0, d[(i0 + i) * VS + v], D1[i]);
-              D2[i] = fmaf(s0, w[(i0 + i) * VS + v], D2[i]);
-              Z[i] = fmaf(ds, r[(i0 + i) * VS + v], Z[i]);
+              D1[i] = dot4(s4, at4(&d[(i0 + i) * VS + v]), D1[i]);
+              D2[i] = dot4(s4, at4(&w[(i0 + i) * VS + v]), D2[i]);
+              Z[i] = dot4(d4, at4(&r[(i0 + i) * VS + v]), Z[i]);
             }
           }
       }
       __syncthreads();
-      // the parts of v meet in shared memory (a buffer of its own behind the arrays)
+      if (c0 == 0 && i0 == 0)  // the decays between the tokens of a pair
+        for (int at = tid; at < C * C; at += kThreads) N1[at / C * MP + at % C] *= G[at / C * MP + at % C], N2[at / C * MP + at % C] *= G[at / C * MP + at % C];
+      // the parts of v meet in shared memory (a buffer of its own behind the arrays); the tokens are dealt out to the parts
       float* meet = sm + 2 * C * KS + 3 * C * VS + 5 * C * MP + 16 * C;
-      if (parts > 1) {
-        if (on)
+      if (on)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) meet[(i * 3 + 0) * kThreads + tid] = D1[i], meet[(i * 3 + 1) * kThreads + tid] = D2[i], meet[(i * 3 + 2) * kThreads + tid] = Z[i];
-        __syncthreads();
-        if (on && part == 0)
-          for (int p = 1; p < parts; ++p)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              D1[i] += meet[(i * 3 + 0) * kThreads + tid + p * cols];
-              D2[i] += meet[(i * 3 + 1) * kThreads + tid + p * cols];
-              Z[i] += meet[(i * 3 + 2) * kThreads + tid + p * cols];
-            }
-      }
-      float xq[8], xk[8], xb[8], xi[8], xo[8];
-      const bool own = on && part == 0;
+        for (int i = 0; i < 8; ++i) meet[(i * 3 + 0) * kThreads + tid] = D1[i], meet[(i * 3 + 1) * kThreads + tid] = D2[i], meet[(i * 3 + 2) * kThreads + tid] = Z[i];
+      __syncthreads();
+      float xb[8], xi[8], xo[8];
 #pragma unroll
       for (int ii = 0; ii < 8; ++ii) {
         const int i = i0 + ii;
-        float sq = 0.f, sk = 0.f, y = 0.f;
-        if (own) {
-          for (int j = 0; j <= i; ++j) {
-            const float m = G[i * MP + j] * be[j] * k[j * KS + c];
-            sq = fmaf(m, N1[i * MP + j], sq);
-            if (j < i) sk = fmaf(m, N2[i * MP + j], sk);
-          }
-          for (int j = i; j < n; ++j) {
-            const float m = G[j * MP + i];
-            y = fmaf(m * N1[j * MP + i], q[j * KS + c], y);
-            if (j > i) y = fmaf(-m * N2[j * MP + i], k[j * KS + c], y);
-          }
-          y = fmaf(suf[i], Z[ii], y);
+        xb[ii] = xi[ii] = xo[ii] = 0.f;
+        if (!on || ii % parts != part || i >= n) continue;
+        float d1 = 0.f, d2 = 0.f, z = 0.f, sq = 0.f, sk = 0.f, y = 0.f;
+        for (int p = tid % cols; p < parts * cols; p += cols) d1 += meet[(ii * 3 + 0) * kThreads + p], d2 += meet[(ii * 3 + 1) * kThreads + p], z += meet[(ii * 3 + 2) * kThreads + p];
+        for (int j = 0; j < i; ++j) {
+          const float m = be[j] * k[j * KS + c];
+          sq = fmaf(m, N1[i * MP + j], sq), sk = fmaf(m, N2[i * MP + j], sk);
         }
-        const float kc = own ? k[i * KS + c] : 0.f, qc = own ? q[i * KS + c] : 0.f;
-        xq[ii] = a.scale * fmaf(gam[i], D1[ii], sq);
-        xk[ii] = be[i] * y - fmaf(gam[i], D2[ii], sk);
+        const float kc = k[i * KS + c], qc = q[i * KS + c];
+        sq = fmaf(be[i] * kc, N1[i * MP + i], sq);
+        y = N1[i * MP + i] * qc;
+        for (int j = i + 1; j < n; ++j) y = fmaf(N1[j * MP + i], q[j * KS + c], y), y = fmaf(-N2[j * MP + i], k[j * KS + c], y);
+        y = fmaf(suf[i], z, y);
+        put(i, c, a.scale * fmaf(gam[i], d1, sq), be[i] * y - fmaf(gam[i], d2, sk));
         xb[ii] = kc * y;
-        xi[ii] = own ? gam[i] * (qc * D1[ii] - kc * D2[ii]) : 0.f;  // S0 into token i
-        xo[ii] = own ? be[i] * suf[i] * kc * Z[ii] : 0.f;           // token i into dS
+        xi[ii] = gam[i] * (qc * d1 - kc * d2);  // S0 into token i
+        xo[ii] = be[i] * suf[i] * kc * z;       // token i into dS
       }
-      if (own)
-#pragma unroll
-        for (int ii = 0; ii < 8; ++ii)
-          if (i0 + ii < n) put(i0 + ii, c, xq[ii], xk[ii]);
       __syncthreads();
       // sums over kdim: warps in order, no atomics
 #pragma unroll
@@ -499,7 +493,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const GradArgs g) {
   // M over N1's place
   for (int at = tid; at < C * C; at += kThreads) {
     const int i = at / C, j = at % C;
-    if (j < i) N1[i * MP + j] = G[i * MP + j] * be[j] * (N1[i * MP + j] * QK[i * MP + j] - N2[i * MP + j] * KK[i * MP + j]);
+    if (j < i) N1[i * MP + j] = be[j] * (N1[i * MP + j] * QK[i * MP + j] - N2[i * MP + j] * KK[i * MP + j]);
   }
   __syncthreads();
   for (int t = tid / 32; t < n; t += per) {
