@@ -112,15 +112,25 @@ struct PairSmem {
   static constexpr int ALLOC = TOTAL + 1024;
 };
 
-// cumulative base-2 logarithms of the decays of a chunk's tokens, by one warp; tokens from n on decay nothing
-__device__ __forceinline__ void decay_logs(const Args& a, const Span& s, int n, int h, float* c, float* beta, int lane) {
-  float x[2];
+// log decays and strengths of tokens 2 lane, 2 lane + 1 of a chunk, by one warp; tokens from n on decay nothing
+struct TokenPair {
+  float g[2], beta[2];
+};
+__device__ __forceinline__ TokenPair token_pair(const Args& a, const Span& s, int n, int h, int lane) {
+  TokenPair x;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int t = 2 * lane + i;
-    x[i] = t < n && a.g.p ? fmaxf(load_dyn(a.g.p, s.b * a.g.sb + (s.t0 + t) * a.g.st + h * a.g.sh, a.g_dtype) * kLog2e, kReset) : 0.f;
-    beta[t] = t < n ? beta_of(a, s.b, s.t0 + t, h) : 0.f;
+    x.g[i] = t < n && a.g.p ? load_dyn(a.g.p, s.b * a.g.sb + (s.t0 + t) * a.g.st + h * a.g.sh, a.g_dtype) : 0.f;
+    x.beta[i] = t < n ? beta_of(a, s.b, s.t0 + t, h) : 0.f;
   }
+  return x;
+}
+// their cumulative base-2 logarithms
+__device__ __forceinline__ void decay_logs(const TokenPair& p, float* c, float* beta, int lane) {
+  float x[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) x[i] = fmaxf(p.g[i] * kLog2e, kReset), beta[2 * lane + i] = p.beta[i];
   float sum = x[0] + x[1];
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -221,7 +231,7 @@ __global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, co
     }
   }
   if (warp == 0) {  // beside the copies
-    decay_logs(a, s, n, h, c, beta, lane);
+    decay_logs(token_pair(a, s, n, h, lane), c, beta, lane);
     __syncwarp();
     float* v = out.vec + at * (4 * C);
     for (int i = lane; i < C; i += 32) {
@@ -456,6 +466,7 @@ __global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, co
 // ---------------------------------------------------------------------------------------------
 // the walk over the chunks
 // ---------------------------------------------------------------------------------------------
+constexpr int kSlice = 64;  // columns of v that the gradients take at a time
 struct WalkMaps {
   CUtensorMap q, k, v, o;  // boxes of 64 columns of one head x 64 tokens; BACK: v is do, o is dv
 };
@@ -466,7 +477,7 @@ struct ChunkWalk {
   void* o;               // BACK: dv
   void* last;            // final state; BACK: gradient of the initial one, fp32
   int last_dtype;
-  void* rest;    // 16-bit r for the backward pass, [token / 8][vdim][8] per (chunk, head); nullable
+  void* rest;    // 16-bit r for the backward pass, [slice of vdim][token / 8][column][8] per (chunk, head); nullable
   void* states;  // 16-bit state before every chunk (BACK: adjoint state behind it), [kdim / 8][vdim][8]; nullable
 };
 
@@ -785,6 +796,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       const float4 x = in ? __ldg(reinterpret_cast<const float4*>(w.initial + state_at + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
       S[e] = x.x, S[e + 1] = x.y, S[e + 2] = x.z, S[e + 3] = x.w;
     }
+    // kept for a backward pass: slices of 64 columns v (`width` in the last one), of each its units of eight elements, of each its columns
+    const int width = min(kSlice, a.vd - v / kSlice * kSlice);
+    auto unit_at = [&](int units, int u) { return v / kSlice * kSlice * units + u * width + v % kSlice; };
     // the state as an operand, and for a backward pass to follow
     auto publish = [&](int p) {
       uint32_t x[NS / 2];
@@ -795,9 +809,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       tc::tmem_wait_st();
       done(kState);
       if (w.states && live) {
-        uint4* keep = reinterpret_cast<uint4*>(w.states) + (((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (KD / 8) + part * (NS / 8)) * a.vd + v;
+        uint4* keep = reinterpret_cast<uint4*>(w.states) + ((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (KD / 8) * a.vd + unit_at(KD / 8, part * (NS / 8));
 #pragma unroll
-        for (int u = 0; u < NS / 8; ++u) keep[(int64_t)u * a.vd] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+        for (int u = 0; u < NS / 8; ++u) keep[u * width] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
       }
     };
     if (nchunks > 0) publish(0);
@@ -828,9 +842,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
           if (w.rest && live) {
 #pragma unroll
             for (int e = 0; e < NT / 2; ++e) y[e] = pack2<T>(f(x[2 * e]), f(x[2 * e + 1]));
-            uint4* to = reinterpret_cast<uint4*>(w.rest) + (((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (C / 8) + part * (NT / 8)) * a.vd + v;
+            uint4* to = reinterpret_cast<uint4*>(w.rest) + ((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (C / 8) * a.vd + unit_at(C / 8, part * (NT / 8));
 #pragma unroll
-            for (int q = 0; q < NT / 8; ++q) to[(int64_t)q * a.vd] = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+            for (int q = 0; q < NT / 8; ++q) to[q * width] = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
           }
       }
       if (!(ok = wait(kDS, p))) break;
@@ -869,15 +883,17 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
 //   dk_i = beta_i y_i - gam_i S0^T w_i - sum_{j<i} G_ij N2_ij beta_j k_j
 //   dg_t = gam_64 <S0, D> + sum_{i<t} beta_i suf_i k_i.(D^T r_i) + sum_{i>=t} gam_i (scale q_i.(S0^T do_i) - k_i.(S0^T w_i)) + sum_{j<t<=i} M_ij,
 //   M_ij = G_ij beta_j (scale N1_ij q_i.k_j - N2_ij k_i.k_j): every path from before t to t or behind it
-// Sixteen warps, each 16 tokens x a quarter of the columns, products by mma.sync (15 Mflop a chunk).  Bound: 145 KB read and 32 KB written a chunk, and
-// that one CTA fills an SM's shared memory, so that its copies and its products take turns.
+// Sixteen warps, each 16 tokens x a quarter of the columns, products by mma.sync (15 Mflop a chunk); one block an SM that walks over its
+// chunks, 64 columns of v at a time, with the next two slices' copies under way (145 KB read and 32 KB written a chunk).  A slice of the states
+// lies in one piece, since copies of a kilobyte each cost their warp more than its products (187 -> 164 us).  Bound: instructions, some 2100 a
+// warp and chunk at 1.7 a cycle, of which 200 are products.  2 x 4096 tokens x 16 heads: 164 us, 2.2 TB/s; with eight warps and a block a chunk 204.
 struct GradMaps {
   CUtensorMap q, k, d, w;
 };
 struct ChunkGrads {
   Args a;
-  const void* rest;     // [token / 8][vdim][8]
-  const void* states;   // [kdim / 8][vdim][8]
+  const void* rest;     // [slice of vdim][token / 8][column][8]
+  const void* states;   // [slice of vdim][kdim / 8][column][8]
   const void* dstates;
   void* dq;
   void* dk;
@@ -885,14 +901,16 @@ struct ChunkGrads {
   float* dg;
   float* dbeta;
   int64_t tokens;
+  int chunks;
   int32_t* status;
 };
-constexpr int kGradThreads = 512, kSlice = 128;  // columns of v at a time
+constexpr int kGradThreads = 512;
 template <int KD>
 struct GradSmem {
-  static constexpr int KT = (KD / 64) * kTileBytes, VT = 2 * kTileBytes, RT = (C / 8) * kSlice * 16, ST = (KD / 8) * kSlice * 16;
-  static constexpr int Q = 0, K = KT, D = 2 * KT, W = D + VT, R = W + VT, S = R + RT, DS = S + ST, Y1 = DS + ST, Y2 = Y1 + kTileBytes, A1 = Y2 + kTileBytes, A2 = A1 + kTileBytes,
-                       VEC = A2 + kTileBytes, TOTAL = VEC + (24 * C + kGradThreads / 32) * 4;
+  static constexpr int KT = (KD / 64) * kTileBytes, RT = (C / 8) * kSlice * 16, ST = (KD / 8) * kSlice * 16;
+  // a slice of the columns of v (two of them), q and k (two of them), the matrices of pairs, later dq and dk
+  static constexpr int D = 0, W = kTileBytes, R = 2 * kTileBytes, S = R + RT, DS = S + ST, SLICE = DS + ST, Q = 0, K = KT, QK = 2 * SLICE, Y1 = QK + 4 * KT, Y2 = Y1 + kTileBytes,
+                       A1 = Y2 + kTileBytes, A2 = A1 + kTileBytes, VEC = A2 + kTileBytes, TOTAL = VEC + (24 * C + kGradThreads / 32) * 4;
   static constexpr int ALLOC = TOTAL + 1024;
 };
 static_assert(GradSmem<128>::ALLOC <= 227 * 1024, "shared memory of an SM");
@@ -916,284 +934,331 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
   constexpr int NB = KD / 32;  // blocks of eight columns of a warp: a quarter of kdim
   extern __shared__ unsigned char smdyn[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t mbar;
+  __shared__ __align__(8) uint64_t mbar[2];
   const Args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const Span s = chunk_of(a.where, blockIdx.x, C);
-  const int n = s.t1 - s.t0, h = blockIdx.y, kh = h / a.group;
-  if (n <= 0) return;
-  const int64_t tok = (int64_t)s.b * a.len + s.t0;
   T* dq = reinterpret_cast<T*>(g.dq);
   T* dk = reinterpret_cast<T*>(g.dk);
-  if (s.seq < 0) {  // rows of no sequence
-    for (int at = tid; at < n * a.kd; at += kGradThreads) {
-      const int64_t to = ((tok + at / a.kd) * a.heads + h) * a.kd + at % a.kd;
-      if (g.dqk) g.dqk[to] = 0.f, g.dqk[g.tokens * a.heads * a.kd + to] = 0.f;
-      else dq[to] = from_f<T>(0.f), dk[to] = from_f<T>(0.f);
+  const int items = g.chunks * a.heads, slices = (a.vd + kSlice - 1) / kSlice;
+  if (a.where.table)  // rows of no sequence
+    for (int it = blockIdx.x; it < items; it += gridDim.x) {
+      const Span s = chunk_of(a.where, it % g.chunks, C);
+      const int n = s.t1 - s.t0, h = it / g.chunks;
+      if (n <= 0 || s.seq >= 0) continue;
+      const int64_t tok = (int64_t)s.b * a.len + s.t0;
+      for (int at = tid; at < n * a.kd; at += kGradThreads) {
+        const int64_t to = ((tok + at / a.kd) * a.heads + h) * a.kd + at % a.kd;
+        if (g.dqk) g.dqk[to] = 0.f, g.dqk[g.tokens * a.heads * a.kd + to] = 0.f;
+        else dq[to] = from_f<T>(0.f), dk[to] = from_f<T>(0.f);
+      }
+      for (int i = tid; i < n; i += kGradThreads) g.dg[(tok + i) * a.heads + h] = 0.f, g.dbeta[(tok + i) * a.heads + h] = 0.f;
     }
-    for (int i = tid; i < n; i += kGradThreads) g.dg[(tok + i) * a.heads + h] = 0.f, g.dbeta[(tok + i) * a.heads + h] = 0.f;
-    return;
-  }
-  const uint32_t base = tc::smem_u32(sm), landed_bar = tc::smem_u32(&mbar);
+  // the others, in this block's order
+  auto from_on = [&](int it) {
+    for (; it < items; it += gridDim.x) {
+      const Span s = chunk_of(a.where, it % g.chunks, C);
+      if (s.t1 > s.t0 && s.seq >= 0) break;
+    }
+    return it;
+  };
+  const uint32_t base = tc::smem_u32(sm), bars = tc::smem_u32(mbar);
   float* c = reinterpret_cast<float*>(sm + M::VEC);
   float *beta = c + C, *gam = beta + C, *suf = gam + C, *rows = suf + C, *cols = rows + 4 * C;  // [4][C] each: sums of M
   float *into = cols + 4 * C, *outof = into + 4 * C, *db = outof + 4 * C, *part = db + 4 * C;   // [4][C] each; a partial sum of every warp
-  const int64_t pair = (int64_t)s.chunk * a.heads + h;
-  const unsigned char* rest = reinterpret_cast<const unsigned char*>(g.rest) + pair * (C / 8) * a.vd * 16;
-  const unsigned char* states = reinterpret_cast<const unsigned char*>(g.states) + pair * (KD / 8) * a.vd * 16;
-  const unsigned char* dstates = reinterpret_cast<const unsigned char*>(g.dstates) + pair * (KD / 8) * a.vd * 16;
-  auto request = [&](int v0) {  // by warp 0
-    const int nv = min(kSlice, a.vd - v0);
+  // a slice's copies, by warp 0: what follows is on its way while a chunk is worked on
+  auto request = [&](int it, int slice, int to_slice, int to_qk) {
+    const Span s = chunk_of(a.where, it % g.chunks, C);
+    const int h = it / g.chunks, kh = h / a.group, v0 = slice * kSlice, nv = min(kSlice, a.vd - v0);
+    const int64_t pair = (int64_t)s.chunk * a.heads + h;
+    const uint32_t bar = bars + to_slice * 8, to = base + to_slice * M::SLICE, qk = base + M::QK + to_qk * 2 * M::KT;
     if (lane == 0) {
-      tc::mbar_expect_tx(landed_bar, 2 * M::VT + (C / 8 + 2 * (KD / 8)) * nv * 16 + (v0 ? 0 : 2 * M::KT));
+      tc::mbar_expect_tx(bar, 2 * kTileBytes + (C / 8 + 2 * (KD / 8)) * nv * 16 + (v0 ? 0 : 2 * M::KT));
       for (int b = 0; b < KD / 64 && v0 == 0; ++b) {
-        tc::tma_load_4d(base + M::Q + b * kTileBytes, &maps.q, landed_bar, b * 64, kh, s.t0, s.b);
-        tc::tma_load_4d(base + M::K + b * kTileBytes, &maps.k, landed_bar, b * 64, kh, s.t0, s.b);
+        tc::tma_load_4d(qk + M::Q + b * kTileBytes, &maps.q, bar, b * 64, kh, s.t0, s.b);
+        tc::tma_load_4d(qk + M::K + b * kTileBytes, &maps.k, bar, b * 64, kh, s.t0, s.b);
       }
-      for (int b = 0; b < 2; ++b) {
-        tc::tma_load_4d(base + M::D + b * kTileBytes, &maps.d, landed_bar, v0 + b * 64, h, s.t0, s.b);
-        tc::tma_load_4d(base + M::W + b * kTileBytes, &maps.w, landed_bar, v0 + b * 64, h, s.t0, s.b);
-      }
+      tc::tma_load_4d(to + M::D, &maps.d, bar, v0, h, s.t0, s.b);
+      tc::tma_load_4d(to + M::W, &maps.w, bar, v0, h, s.t0, s.b);
     }
     __syncwarp();
-    for (int u = lane; u < C / 8 + 2 * (KD / 8); u += 32) {
-      const int i = u < C / 8 ? u : (u - C / 8) % (KD / 8);
-      const unsigned char* from = u < C / 8 ? rest : u < C / 8 + KD / 8 ? states : dstates;
-      const int to = u < C / 8 ? M::R : u < C / 8 + KD / 8 ? M::S : M::DS;
-      tc::bulk_load(base + to + i * (kSlice * 16), from + ((int64_t)i * a.vd + v0) * 16, nv * 16, landed_bar);
-    }
-  };
-  if (tid == 0) tc::mbar_init(landed_bar, 1);
-  __syncthreads();
-  if (warp == 0) {
-    request(0);
-    decay_logs(a, s, n, h, c, beta, lane);
-    __syncwarp();
-    for (int i = lane; i < C; i += 32) gam[i] = ex2_approx(c[i]), suf[i] = ex2_approx(c[C - 1] - c[i]);
-  }
-  const int r0 = (warp >> 2) * 16, quarter = (warp + (warp >> 2)) & 3, c0 = quarter * 16, k_cols = quarter * (KD / 4), gi = lane >> 2, gj = (lane & 3) * 2;
-  float N1[2][4] = {}, N2[2][4] = {}, dQ[NB][4] = {}, dK[NB][4] = {}, y[NB][4] = {}, whole = 0.f;
-  for (int v0 = 0, turn = 0; v0 < a.vd; v0 += kSlice, ++turn) {
-    const int nv = min(kSlice, a.vd - v0);
-    if (!__syncthreads_and(phase_done(landed_bar, turn & 1))) {
-      if (tid == 0 && g.status) *(volatile int32_t*)g.status = 7;
+    if (nv == kSlice) {  // in one piece
+      if (lane == 0) {
+        const int64_t from = (pair * a.vd + v0) * 16;
+        auto piece = [&](int at, const void* p, int units) { tc::bulk_load(to + at, reinterpret_cast<const unsigned char*>(p) + from * units, units * (kSlice * 16), bar); };
+        piece(M::R, g.rest, C / 8), piece(M::S, g.states, KD / 8), piece(M::DS, g.dstates, KD / 8);
+      }
+      __syncwarp();
       return;
     }
-    if (a.where.table && n < C) {  // rows of the next sequence: nothing of them may enter a product, not even times zero
-      constexpr int U = KD / 8;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (int i = tid; i < (C - n) * U; i += kGradThreads) {
-        const int at = (i % U >> 3) * kTileBytes + swz(n + i / U, i % U & 7);
-        *reinterpret_cast<uint4*>(sm + M::Q + at) = zero, *reinterpret_cast<uint4*>(sm + M::K + at) = zero;
-      }
-      for (int i = tid; i < (C - n) * 16; i += kGradThreads) {
-        const int at = (i % 16 >> 3) * kTileBytes + swz(n + i / 16, i % 16 & 7);
-        *reinterpret_cast<uint4*>(sm + M::D + at) = zero, *reinterpret_cast<uint4*>(sm + M::W + at) = zero;
-      }
+    for (int u = lane; u < C / 8 + 2 * (KD / 8); u += 32) {
+      const int i = u < C / 8 ? u : (u - C / 8) % (KD / 8), units = u < C / 8 ? C / 8 : KD / 8;
+      const void* from = u < C / 8 ? g.rest : u < C / 8 + KD / 8 ? g.states : g.dstates;
+      const int at = u < C / 8 ? M::R : u < C / 8 + KD / 8 ? M::S : M::DS;
+      tc::bulk_load(to + at + i * (kSlice * 16), reinterpret_cast<const unsigned char*>(from) + ((pair * a.vd + v0) * units + i * nv) * 16, nv * 16, bar);
     }
-    if (nv % 16) {  // products take 16 columns of v at a time
-      for (int i = tid; i < (C / 8 + 2 * (KD / 8)) * 8; i += kGradThreads) {
-        const int u = i / 8, at = u < C / 8 ? M::R + u * (kSlice * 16) : M::S + (u - C / 8) * (kSlice * 16);  // the adjoint state follows the state
-        *reinterpret_cast<uint4*>(sm + at + (nv + i % 8) * 16) = make_uint4(0, 0, 0, 0);
+  };
+  if (tid == 0) tc::mbar_init(bars, 1), tc::mbar_init(bars + 8, 1);
+  __syncthreads();
+  int it = from_on(blockIdx.x);
+  int used = 0, asked = 0, ahead = 0, ahead_slice = 0;  // slices worked on and asked for; the next to ask for, `ahead` chunks from the current one
+  const int r0 = (warp >> 2) * 16, quarter = (warp + (warp >> 2)) & 3, c0 = quarter * 16, k_cols = quarter * (KD / 4), gi = lane >> 2, gj = (lane & 3) * 2;
+  TokenPair token{};
+  auto tokens_of = [&](int i) {
+    if (i >= items) return;
+    const Span s = chunk_of(a.where, i % g.chunks, C);
+    token = token_pair(a, s, s.t1 - s.t0, i / g.chunks, lane);
+  };
+  constexpr int kDecays = 5, kSums = 10;  // warps that do more than their share, each with another scheduler; warp 0 asks for the copies
+  if (warp == kDecays) tokens_of(it);
+  for (int order = 0; it < items; ++order) {
+    const Span s = chunk_of(a.where, it % g.chunks, C);
+    const int n = s.t1 - s.t0, h = it / g.chunks, next = from_on(it + gridDim.x);
+    const int64_t tok = (int64_t)s.b * a.len + s.t0;
+    unsigned char* qk = sm + M::QK + (order & 1) * 2 * M::KT;
+    const uint32_t qk_base = tc::smem_u32(qk);
+    auto feed = [&] {  // as far as there are buffers: two of slices, and for q and k this chunk's and the next one's
+      for (; asked - used < 2 && ahead < 2 && (ahead ? next : it) < items; ++asked) {
+        if (warp == 0) request(ahead ? next : it, ahead_slice, asked & 1, (order + ahead) & 1);
+        if (++ahead_slice == slices) ahead_slice = 0, ++ahead;
       }
+    };
+    feed();
+    if (warp == kDecays) {
+      decay_logs(token, c, beta, lane);
+      __syncwarp();
+      for (int i = lane; i < C; i += 32) gam[i] = ex2_approx(c[i]), suf[i] = ex2_approx(c[C - 1] - c[i]);
     }
-    __syncthreads();
-    for (int k0 = 0; k0 < nv; k0 += 16) {
-      uint32_t fd[4], fw[4], fr[4], b[4];
-      load_a(fd, base + M::D, r0, k0, lane);
-      load_a(fw, base + M::W, r0, k0, lane);
-      units_a(fr, base + M::R, r0, k0, lane);
-      if (c0 <= r0) {
-        units_b(b, base + M::R, c0, k0, lane);
-        mma16816<T>(N1[0], fd, b[0], b[1]), mma16816<T>(N1[1], fd, b[2], b[3]);
-        mma16816<T>(N2[0], fw, b[0], b[1]), mma16816<T>(N2[1], fw, b[2], b[3]);
+    float N1[2][4] = {}, N2[2][4] = {}, dQ[NB][4] = {}, dK[NB][4] = {}, y[NB][4] = {}, whole = 0.f;
+    for (int v0 = 0; v0 < a.vd; v0 += kSlice) {
+      const int nv = min(kSlice, a.vd - v0);
+      unsigned char* sl = sm + (used & 1) * M::SLICE;
+      const uint32_t slice = tc::smem_u32(sl);
+      if (!__syncthreads_and(phase_done(bars + (used & 1) * 8, used >> 1 & 1))) {
+        if (tid == 0 && g.status) *(volatile int32_t*)g.status = 7;
+        for (; used < asked; ++used) phase_done(bars + (used & 1) * 8, used >> 1 & 1);  // nothing is under way when the block ends
+        return;
+      }
+      if (a.where.table && n < C) {  // rows of the next sequence: nothing of them may enter a product, not even times zero
+        constexpr int U = KD / 8;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < (C - n) * U; i += kGradThreads) {
+          const int at = (i % U >> 3) * kTileBytes + swz(n + i / U, i % U & 7);
+          *reinterpret_cast<uint4*>(qk + M::Q + at) = zero, *reinterpret_cast<uint4*>(qk + M::K + at) = zero;
+        }
+        for (int i = tid; i < (C - n) * 8; i += kGradThreads) {
+          const int at = swz(n + i / 8, i % 8);
+          *reinterpret_cast<uint4*>(sl + M::D + at) = zero, *reinterpret_cast<uint4*>(sl + M::W + at) = zero;
+        }
+      }
+      if (nv % 16) {  // products take 16 columns of v at a time
+        for (int i = tid; i < (C / 8 + 2 * (KD / 8)) * 8; i += kGradThreads) {
+          const int u = i / 8, at = u < C / 8 ? M::R + u * (kSlice * 16) : M::S + (u - C / 8) * (kSlice * 16);  // the adjoint state follows the state
+          *reinterpret_cast<uint4*>(sl + at + (nv + i % 8) * 16) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (nv % 16 || (a.where.table && n < C)) __syncthreads();
+      for (int k0 = 0; k0 < nv; k0 += 16) {
+        uint32_t fd[4], fw[4], fr[4], b[4];
+        load_a(fd, slice + M::D, r0, k0, lane);
+        load_a(fw, slice + M::W, r0, k0, lane);
+        units_a(fr, slice + M::R, r0, k0, lane);
+        if (c0 <= r0) {
+          units_b(b, slice + M::R, c0, k0, lane);
+          mma16816<T>(N1[0], fd, b[0], b[1]), mma16816<T>(N1[1], fd, b[2], b[3]);
+          mma16816<T>(N2[0], fw, b[0], b[1]), mma16816<T>(N2[1], fw, b[2], b[3]);
+        }
+#pragma unroll
+        for (int n0 = 0; n0 < NB * 8; n0 += 16) {
+          units_b(b, slice + M::S, k_cols + n0, k0, lane);
+          mma16816<T>(dQ[n0 / 8], fd, b[0], b[1]), mma16816<T>(dQ[n0 / 8 + 1], fd, b[2], b[3]);
+          mma16816<T>(dK[n0 / 8], fw, b[0], b[1]), mma16816<T>(dK[n0 / 8 + 1], fw, b[2], b[3]);
+          units_b(b, slice + M::DS, k_cols + n0, k0, lane);
+          mma16816<T>(y[n0 / 8], fr, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fr, b[2], b[3]);
+        }
       }
 #pragma unroll
-      for (int n0 = 0; n0 < NB * 8; n0 += 16) {
-        units_b(b, base + M::S, k_cols + n0, k0, lane);
-        mma16816<T>(dQ[n0 / 8], fd, b[0], b[1]), mma16816<T>(dQ[n0 / 8 + 1], fd, b[2], b[3]);
-        mma16816<T>(dK[n0 / 8], fw, b[0], b[1]), mma16816<T>(dK[n0 / 8 + 1], fw, b[2], b[3]);
-        units_b(b, base + M::DS, k_cols + n0, k0, lane);
-        mma16816<T>(y[n0 / 8], fr, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fr, b[2], b[3]);
-      }
-    }
-    for (int i = tid; i < (KD / 8) * nv; i += kGradThreads) {
-      const int at = ((i / nv) * kSlice + i % nv) * 16;
-      const uint4 x = *reinterpret_cast<const uint4*>(sm + M::S + at), z = *reinterpret_cast<const uint4*>(sm + M::DS + at);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, zs[4] = {z.x, z.y, z.z, z.w};
+      for (int i = tid; i < (KD / 8) * kSlice; i += kGradThreads) {
+        const int at = i * 16;
+        if (i % kSlice >= nv) continue;
+        const uint4 x = *reinterpret_cast<const uint4*>(sl + M::S + at), z = *reinterpret_cast<const uint4*>(sl + M::DS + at);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 p = unpack2<T>(xs[e]), q = unpack2<T>(zs[e]);
-        whole = fmaf(p.x, q.x, fmaf(p.y, q.y, whole));
+        for (int e = 0; e < 4; ++e) {
+          const float2 p = unpack2<T>(xs[e]), q = unpack2<T>(zs[e]);
+          whole = fmaf(p.x, q.x, fmaf(p.y, q.y, whole));
+        }
       }
-    }
-    if (v0 + kSlice < a.vd) {
       tc::fence_async_smem();  // what was read and written here, before the next copies
       __syncthreads();
-      if (warp == 0) request(v0 + kSlice);
+      ++used;
+      feed();
     }
-  }
-  whole = warp_sum(whole);
-  if (lane == 0) part[warp] = whole;
-  {  // pairs of tokens: this warp's 16 x 16
-    float QK[2][4] = {}, KK[2][4] = {};
-    if (c0 <= r0) {
+    if (warp == kDecays) tokens_of(next);
+    whole = warp_sum(whole);
+    if (lane == 0) part[warp] = gam[C - 1] * whole;  // here: the next chunk's decays may be written during the last sums
+    {  // pairs of tokens: this warp's 16 x 16
+      float QK[2][4] = {}, KK[2][4] = {};
+      if (c0 <= r0) {
 #pragma unroll
-      for (int k0 = 0; k0 < KD; k0 += 16) {
-        uint32_t fq[4], fk[4], b[4];
-        load_a(fq, base + M::Q, r0, k0, lane);
-        load_a(fk, base + M::K, r0, k0, lane);
-        load_b(b, base + M::K, c0, k0, lane);
-        mma16816<T>(QK[0], fq, b[0], b[1]), mma16816<T>(QK[1], fq, b[2], b[3]);
-        mma16816<T>(KK[0], fk, b[0], b[1]), mma16816<T>(KK[1], fk, b[2], b[3]);
+        for (int k0 = 0; k0 < KD; k0 += 16) {
+          uint32_t fq[4], fk[4], b[4];
+          load_a(fq, qk_base + M::Q, r0, k0, lane);
+          load_a(fk, qk_base + M::K, r0, k0, lane);
+          load_b(b, qk_base + M::K, c0, k0, lane);
+          mma16816<T>(QK[0], fq, b[0], b[1]), mma16816<T>(QK[1], fq, b[2], b[3]);
+          mma16816<T>(KK[0], fk, b[0], b[1]), mma16816<T>(KK[1], fk, b[2], b[3]);
+        }
       }
-    }
-    float row[2] = {0.f, 0.f};
+      float row[2] = {0.f, 0.f};
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      const int j0 = c0 + nb * 8 + gj;
-      float y1[4], y2[4], a1[4], a2[4], col[2] = {0.f, 0.f};
+      for (int nb = 0; nb < 2; ++nb) {
+        const int j0 = c0 + nb * 8 + gj;
+        float y1[4], y2[4], a1[4], a2[4], col[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = r0 + gi + (e >> 1) * 8, j = j0 + (e & 1);
-        const float G = ex2_approx(c[i] - c[j]), b = beta[j];
-        y1[e] = j <= i ? G * a.scale * N1[nb][e] : 0.f;
-        y2[e] = j < i ? -G * N2[nb][e] : 0.f;
-        a1[e] = b * y1[e], a2[e] = b * y2[e];
-        const float m = j < i ? a1[e] * QK[nb][e] + a2[e] * KK[nb][e] : 0.f;
-        row[e >> 1] += m, col[e & 1] += m;
+        for (int e = 0; e < 4; ++e) {
+          const int i = r0 + gi + (e >> 1) * 8, j = j0 + (e & 1);
+          const float G = ex2_approx(c[i] - c[j]), b = beta[j];
+          y1[e] = j <= i ? G * a.scale * N1[nb][e] : 0.f;
+          y2[e] = j < i ? -G * N2[nb][e] : 0.f;
+          a1[e] = b * y1[e], a2[e] = b * y2[e];
+          const float m = j < i ? a1[e] * QK[nb][e] + a2[e] * KK[nb][e] : 0.f;
+          row[e >> 1] += m, col[e & 1] += m;
+        }
+#pragma unroll
+        for (int off = 4; off <= 16; off *= 2) col[0] += __shfl_xor_sync(0xffffffffu, col[0], off), col[1] += __shfl_xor_sync(0xffffffffu, col[1], off);
+        if (gi == 0) cols[(warp >> 2) * C + j0] = col[0], cols[(warp >> 2) * C + j0 + 1] = col[1];
+        const int lo = swz(r0 + gi, j0 >> 3) + gj * 2, hi = swz(r0 + gi + 8, j0 >> 3) + gj * 2;
+        *reinterpret_cast<uint32_t*>(sm + M::Y1 + lo) = pack2<T>(y1[0], y1[1]), *reinterpret_cast<uint32_t*>(sm + M::Y1 + hi) = pack2<T>(y1[2], y1[3]);
+        *reinterpret_cast<uint32_t*>(sm + M::Y2 + lo) = pack2<T>(y2[0], y2[1]), *reinterpret_cast<uint32_t*>(sm + M::Y2 + hi) = pack2<T>(y2[2], y2[3]);
+        *reinterpret_cast<uint32_t*>(sm + M::A1 + lo) = pack2<T>(a1[0], a1[1]), *reinterpret_cast<uint32_t*>(sm + M::A1 + hi) = pack2<T>(a1[2], a1[3]);
+        *reinterpret_cast<uint32_t*>(sm + M::A2 + lo) = pack2<T>(a2[0], a2[1]), *reinterpret_cast<uint32_t*>(sm + M::A2 + hi) = pack2<T>(a2[2], a2[3]);
       }
-#pragma unroll
-      for (int off = 4; off <= 16; off *= 2) col[0] += __shfl_xor_sync(0xffffffffu, col[0], off), col[1] += __shfl_xor_sync(0xffffffffu, col[1], off);
-      if (gi == 0) cols[(warp >> 2) * C + j0] = col[0], cols[(warp >> 2) * C + j0 + 1] = col[1];
-      const int lo = swz(r0 + gi, j0 >> 3) + gj * 2, hi = swz(r0 + gi + 8, j0 >> 3) + gj * 2;
-      *reinterpret_cast<uint32_t*>(sm + M::Y1 + lo) = pack2<T>(y1[0], y1[1]), *reinterpret_cast<uint32_t*>(sm + M::Y1 + hi) = pack2<T>(y1[2], y1[3]);
-      *reinterpret_cast<uint32_t*>(sm + M::Y2 + lo) = pack2<T>(y2[0], y2[1]), *reinterpret_cast<uint32_t*>(sm + M::Y2 + hi) = pack2<T>(y2[2], y2[3]);
-      *reinterpret_cast<uint32_t*>(sm + M::A1 + lo) = pack2<T>(a1[0], a1[1]), *reinterpret_cast<uint32_t*>(sm + M::A1 + hi) = pack2<T>(a1[2], a1[3]);
-      *reinterpret_cast<uint32_t*>(sm + M::A2 + lo) = pack2<T>(a2[0], a2[1]), *reinterpret_cast<uint32_t*>(sm + M::A2 + hi) = pack2<T>(a2[2], a2[3]);
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      row[e] += __shfl_xor_sync(0xffffffffu, row[e], 1), row[e] += __shfl_xor_sync(0xffffffffu, row[e], 2);
-      if ((lane & 3) == 0) rows[quarter * C + r0 + gi + e * 8] = row[e];
-    }
-  }
-  // the states' parts, scaled, and what dg takes of them
-  const float gm[2] = {gam[r0 + gi], gam[r0 + gi + 8]}, sf[2] = {suf[r0 + gi], suf[r0 + gi + 8]}, bt[2] = {beta[r0 + gi], beta[r0 + gi + 8]};
-  auto row_sums = [&](float (&x)[2], float* to) {  // over the four lanes of a row, to this quarter's place
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      x[e] += __shfl_xor_sync(0xffffffffu, x[e], 1), x[e] += __shfl_xor_sync(0xffffffffu, x[e], 2);
-      if ((lane & 3) == 0) to[quarter * C + r0 + gi + e * 8] = x[e];
-    }
-  };
-  auto pair_at = [&](int tile, int e, int nb) {  // two neighbouring elements of q or k
-    const int col = k_cols + nb * 8;
-    return unpack2<T>(*reinterpret_cast<const uint32_t*>(sm + tile + (col >> 6) * kTileBytes + swz(r0 + gi + e * 8, (col & 63) >> 3) + gj * 2));
-  };
-  {
-    float in[2] = {0.f, 0.f}, outp[2] = {0.f, 0.f};
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float2 q = pair_at(M::Q, e, nb), k = pair_at(M::K, e, nb);
-        dQ[nb][2 * e] *= gm[e] * a.scale, dQ[nb][2 * e + 1] *= gm[e] * a.scale;
-        dK[nb][2 * e] *= -gm[e], dK[nb][2 * e + 1] *= -gm[e];
-        y[nb][2 * e] *= sf[e], y[nb][2 * e + 1] *= sf[e];
-        in[e] += dQ[nb][2 * e] * q.x + dQ[nb][2 * e + 1] * q.y + dK[nb][2 * e] * k.x + dK[nb][2 * e + 1] * k.y;
-        outp[e] += bt[e] * (y[nb][2 * e] * k.x + y[nb][2 * e + 1] * k.y);
-      }
-    row_sums(in, into), row_sums(outp, outof);
-  }
-  __syncthreads();  // the pair matrices are written, the states have been read
-#pragma unroll
-  for (int k0 = 0; k0 < C; k0 += 16) {
-    uint32_t fa[4], fb[4], b[4];
-    if (k0 <= r0) {  // pairs with tokens before
-      load_a(fa, base + M::A1, r0, k0, lane);
-      load_a(fb, base + M::A2, r0, k0, lane);
-#pragma unroll
-      for (int n0 = 0; n0 < NB * 8; n0 += 16) {
-        const int col = k_cols + n0;
-        load_bt(b, base + M::K + (col >> 6) * kTileBytes, col & 63, k0, lane);
-        mma16816<T>(dQ[n0 / 8], fa, b[0], b[1]), mma16816<T>(dQ[n0 / 8 + 1], fa, b[2], b[3]);
-        mma16816<T>(dK[n0 / 8], fb, b[0], b[1]), mma16816<T>(dK[n0 / 8 + 1], fb, b[2], b[3]);
+        row[e] += __shfl_xor_sync(0xffffffffu, row[e], 1), row[e] += __shfl_xor_sync(0xffffffffu, row[e], 2);
+        if ((lane & 3) == 0) rows[quarter * C + r0 + gi + e * 8] = row[e];
       }
     }
-    if (k0 >= r0) {  // and with those behind
-      load_at(fa, base + M::Y1, r0, k0, lane);
-      load_at(fb, base + M::Y2, r0, k0, lane);
-#pragma unroll
-      for (int n0 = 0; n0 < NB * 8; n0 += 16) {
-        const int col = k_cols + n0;
-        load_bt(b, base + M::Q + (col >> 6) * kTileBytes, col & 63, k0, lane);
-        mma16816<T>(y[n0 / 8], fa, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fa, b[2], b[3]);
-        load_bt(b, base + M::K + (col >> 6) * kTileBytes, col & 63, k0, lane);
-        mma16816<T>(y[n0 / 8], fb, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fb, b[2], b[3]);
-      }
-    }
-  }
-  {
-    float sum[2] = {0.f, 0.f};
-    float* wide = g.dqk ? g.dqk + ((tok + r0 + gi) * a.heads + h) * a.kd : nullptr;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int col = k_cols + nb * 8 + gj;
+    // the states' parts, scaled, and what dg takes of them
+    const float gm[2] = {gam[r0 + gi], gam[r0 + gi + 8]}, sf[2] = {suf[r0 + gi], suf[r0 + gi + 8]}, bt[2] = {beta[r0 + gi], beta[r0 + gi + 8]};
+    auto row_sums = [&](float (&x)[2], float* to) {  // over the four lanes of a row, to this quarter's place
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float2 k = pair_at(M::K, e, nb);
-        sum[e] += y[nb][2 * e] * k.x + y[nb][2 * e + 1] * k.y;
-        const float k0 = fmaf(bt[e], y[nb][2 * e], dK[nb][2 * e]), k1 = fmaf(bt[e], y[nb][2 * e + 1], dK[nb][2 * e + 1]);
-        if (wide) {
-          if (r0 + gi + e * 8 < n && col < a.kd) {
-            float* to = wide + (int64_t)e * 8 * a.heads * a.kd + col;
-            *reinterpret_cast<float2*>(to) = make_float2(dQ[nb][2 * e], dQ[nb][2 * e + 1]);
-            *reinterpret_cast<float2*>(to + g.tokens * a.heads * a.kd) = make_float2(k0, k1);
-          }
-        } else {  // over the states, to leave in whole pieces
-          const int at = (col >> 6) * kTileBytes + swz(r0 + gi + e * 8, (col & 63) >> 3) + gj * 2;
-          *reinterpret_cast<uint32_t*>(sm + M::S + at) = pack2<T>(dQ[nb][2 * e], dQ[nb][2 * e + 1]);
-          *reinterpret_cast<uint32_t*>(sm + M::DS + at) = pack2<T>(k0, k1);
+        x[e] += __shfl_xor_sync(0xffffffffu, x[e], 1), x[e] += __shfl_xor_sync(0xffffffffu, x[e], 2);
+        if ((lane & 3) == 0) to[quarter * C + r0 + gi + e * 8] = x[e];
+      }
+    };
+    auto pair_at = [&](int tile, int e, int nb) {  // two neighbouring elements of q or k
+      const int col = k_cols + nb * 8;
+      return unpack2<T>(*reinterpret_cast<const uint32_t*>(qk + tile + (col >> 6) * kTileBytes + swz(r0 + gi + e * 8, (col & 63) >> 3) + gj * 2));
+    };
+    {
+      float in[2] = {0.f, 0.f}, outp[2] = {0.f, 0.f};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 q = pair_at(M::Q, e, nb), k = pair_at(M::K, e, nb);
+          dQ[nb][2 * e] *= gm[e] * a.scale, dQ[nb][2 * e + 1] *= gm[e] * a.scale;
+          dK[nb][2 * e] *= -gm[e], dK[nb][2 * e + 1] *= -gm[e];
+          y[nb][2 * e] *= sf[e], y[nb][2 * e + 1] *= sf[e];
+          in[e] += dQ[nb][2 * e] * q.x + dQ[nb][2 * e + 1] * q.y + dK[nb][2 * e] * k.x + dK[nb][2 * e + 1] * k.y;
+          outp[e] += bt[e] * (y[nb][2 * e] * k.x + y[nb][2 * e + 1] * k.y);
+        }
+      row_sums(in, into), row_sums(outp, outof);
+    }
+    __syncthreads();  // the pair matrices are written, the states have been read
+#pragma unroll
+    for (int k0 = 0; k0 < C; k0 += 16) {
+      uint32_t fa[4], fb[4], b[4];
+      if (k0 <= r0) {  // pairs with tokens before
+        load_a(fa, base + M::A1, r0, k0, lane);
+        load_a(fb, base + M::A2, r0, k0, lane);
+#pragma unroll
+        for (int n0 = 0; n0 < NB * 8; n0 += 16) {
+          const int col = k_cols + n0;
+          load_bt(b, qk_base + M::K + (col >> 6) * kTileBytes, col & 63, k0, lane);
+          mma16816<T>(dQ[n0 / 8], fa, b[0], b[1]), mma16816<T>(dQ[n0 / 8 + 1], fa, b[2], b[3]);
+          mma16816<T>(dK[n0 / 8], fb, b[0], b[1]), mma16816<T>(dK[n0 / 8 + 1], fb, b[2], b[3]);
+        }
+      }
+      if (k0 >= r0) {  // and with those behind
+        load_at(fa, base + M::Y1, r0, k0, lane);
+        load_at(fb, base + M::Y2, r0, k0, lane);
+#pragma unroll
+        for (int n0 = 0; n0 < NB * 8; n0 += 16) {
+          const int col = k_cols + n0;
+          load_bt(b, qk_base + M::Q + (col >> 6) * kTileBytes, col & 63, k0, lane);
+          mma16816<T>(y[n0 / 8], fa, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fa, b[2], b[3]);
+          load_bt(b, qk_base + M::K + (col >> 6) * kTileBytes, col & 63, k0, lane);
+          mma16816<T>(y[n0 / 8], fb, b[0], b[1]), mma16816<T>(y[n0 / 8 + 1], fb, b[2], b[3]);
         }
       }
     }
-    row_sums(sum, db);
-  }
-  __syncthreads();
-  if (!g.dqk)
-    for (int i = tid; i < n * (a.kd / 8); i += kGradThreads) {
-      const int r = i / (a.kd / 8), u = i % (a.kd / 8), at = (u >> 3) * kTileBytes + swz(r, u & 7);
-      const int64_t to = ((tok + r) * a.heads + h) * a.kd + u * 8;
-      *reinterpret_cast<uint4*>(dq + to) = *reinterpret_cast<const uint4*>(sm + M::S + at);
-      *reinterpret_cast<uint4*>(dk + to) = *reinterpret_cast<const uint4*>(sm + M::DS + at);
-    }
-  if (warp == 0) {
-    float all = 0.f;
-    for (int i = 0; i < kGradThreads / 32; ++i) all += part[i];
-    float x[2], z[2];  // of tokens 2 lane, 2 lane + 1: into them, out of them
+    __syncthreads();  // and the pair matrices
+    {
+      float sum[2] = {0.f, 0.f};
+      float* wide = g.dqk ? g.dqk + ((tok + r0 + gi) * a.heads + h) * a.kd : nullptr;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * lane + e;
-      x[e] = z[e] = 0.f;
-      for (int b = 0; b < 4; ++b) x[e] += into[b * C + i] + rows[b * C + i] - (b * 16 + 15 > i ? cols[b * C + i] : 0.f), z[e] += outof[b * C + i];
-    }
-    float behind = x[0] + x[1], before = z[0] + z[1];  // inclusive sums from the end, and from the start
+      for (int nb = 0; nb < NB; ++nb) {
+        const int col = k_cols + nb * 8 + gj;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const float u = __shfl_down_sync(0xffffffffu, behind, off), v = __shfl_up_sync(0xffffffffu, before, off);
-      if (lane + off < 32) behind += u;
-      if (lane >= off) before += v;
+        for (int e = 0; e < 2; ++e) {
+          const float2 k = pair_at(M::K, e, nb);
+          sum[e] += y[nb][2 * e] * k.x + y[nb][2 * e + 1] * k.y;
+          const float k0 = fmaf(bt[e], y[nb][2 * e], dK[nb][2 * e]), k1 = fmaf(bt[e], y[nb][2 * e + 1], dK[nb][2 * e + 1]);
+          if (wide) {
+            if (r0 + gi + e * 8 < n && col < a.kd) {
+              float* to = wide + (int64_t)e * 8 * a.heads * a.kd + col;
+              *reinterpret_cast<float2*>(to) = make_float2(dQ[nb][2 * e], dQ[nb][2 * e + 1]);
+              *reinterpret_cast<float2*>(to + g.tokens * a.heads * a.kd) = make_float2(k0, k1);
+            }
+          } else {  // over the pair matrices, to leave in whole pieces
+            const int at = (col >> 6) * kTileBytes + swz(r0 + gi + e * 8, (col & 63) >> 3) + gj * 2;
+            *reinterpret_cast<uint32_t*>(sm + M::Y1 + at) = pack2<T>(dQ[nb][2 * e], dQ[nb][2 * e + 1]);
+            *reinterpret_cast<uint32_t*>(sm + M::A1 + at) = pack2<T>(k0, k1);
+          }
+        }
+      }
+      row_sums(sum, db);
     }
-    const float total = gam[C - 1] * all;
+    __syncthreads();
+    if (!g.dqk)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * lane + e;
-      if (i < n) {
-        g.dg[(tok + i) * a.heads + h] = total + (e ? behind - x[0] : behind) + (e ? before - z[1] : before - z[0] - z[1]);
-        g.dbeta[(tok + i) * a.heads + h] = db[i] + db[C + i] + db[2 * C + i] + db[3 * C + i];
+      for (int i = tid; i < C * (KD / 8); i += kGradThreads) {
+        const int r = i / (KD / 8), u = i % (KD / 8), at = (u >> 3) * kTileBytes + swz(r, u & 7);
+        if (r >= n || u * 8 >= a.kd) continue;
+        const int64_t to = ((tok + r) * a.heads + h) * a.kd + u * 8;
+        *reinterpret_cast<uint4*>(dq + to) = *reinterpret_cast<const uint4*>(sm + M::Y1 + at);
+        *reinterpret_cast<uint4*>(dk + to) = *reinterpret_cast<const uint4*>(sm + M::A1 + at);
+      }
+    if (warp == kSums) {
+      float all = 0.f;
+      for (int i = 0; i < kGradThreads / 32; ++i) all += part[i];
+      float x[2], z[2];  // of tokens 2 lane, 2 lane + 1: into them, out of them
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * lane + e;
+        x[e] = z[e] = 0.f;
+        for (int b = 0; b < 4; ++b) x[e] += into[b * C + i] + rows[b * C + i] - (b * 16 + 15 > i ? cols[b * C + i] : 0.f), z[e] += outof[b * C + i];
+      }
+      float behind = x[0] + x[1], before = z[0] + z[1];  // inclusive sums from the end, and from the start
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const float u = __shfl_down_sync(0xffffffffu, behind, off), v = __shfl_up_sync(0xffffffffu, before, off);
+        if (lane + off < 32) behind += u;
+        if (lane >= off) before += v;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * lane + e;
+        if (i < n) {
+          g.dg[(tok + i) * a.heads + h] = all + (e ? behind - x[0] : behind) + (e ? before - z[1] : before - z[0] - z[1]);
+          g.dbeta[(tok + i) * a.heads + h] = db[i] + db[C + i] + db[2 * C + i] + db[3 * C + i];
+        }
       }
     }
+    it = next, --ahead;  // all of this chunk's slices have been asked for
   }
 }
 
@@ -1289,7 +1354,7 @@ extern "C" int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, voi
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   w.a.where.per = (f.len + gd::C - 1) / gd::C;
   const int64_t chunks = gd::chunks_of(f);
-  SSM_REQUIRE(chunks < 0x7fffffff, SSM_ERR_TOO_LARGE, "gated_delta: too many chunks");
+  SSM_REQUIRE(chunks * f.heads < 0x7f000000, SSM_ERR_TOO_LARGE, "gated_delta: too many chunks");
   const gd::Layout l = gd::layout_of(chunks, f.heads, f.kdim, f.vdim, train != 0);
   unsigned char* base = reinterpret_cast<unsigned char*>(kept);
   unsigned char* wz = reinterpret_cast<unsigned char*>(scratch);
@@ -1335,6 +1400,7 @@ extern "C" int ssm_gated_delta_chunked_bwd(const ssm_gated_delta_bwd_args* args,
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   w.a.where.per = (f.len + gd::C - 1) / gd::C;
   const int64_t chunks = gd::chunks_of(f);
+  SSM_REQUIRE(chunks * f.heads < 0x7f000000, SSM_ERR_TOO_LARGE, "gated_delta: too many chunks");
   const gd::Layout l = gd::layout_of(chunks, f.heads, f.kdim, f.vdim, true);
   unsigned char* base = reinterpret_cast<unsigned char*>(kept);
   w.in = {nullptr, nullptr, base + l.y, base + l.wb, reinterpret_cast<float*>(base + l.vec), status};
@@ -1349,14 +1415,14 @@ extern "C" int ssm_gated_delta_chunked_bwd(const ssm_gated_delta_bwd_args* args,
   const gd::GradMaps gm{maps.q, maps.k, maps.v, maps.o};
   gd::ChunkGrads g{};
   g.a = w.a, g.rest = base + l.rest, g.states = base + l.states, g.dstates = scratch, g.dq = args->dq, g.dk = args->dk, g.dqk = w.a.group > 1 ? args->dqk : nullptr;
-  g.dg = args->dg, g.dbeta = args->dbeta, g.tokens = (int64_t)f.batch * f.len, g.status = status;
+  g.dg = args->dg, g.dbeta = args->dbeta, g.tokens = (int64_t)f.batch * f.len, g.chunks = (int)chunks, g.status = status;
   auto go = [&](auto type, auto kd) {
     using T = decltype(type);
     constexpr int KD = decltype(kd)::value;
     if (const int rc = gd::launch_chunks<T, KD, true>(w, maps, st)) return rc;
     const int smem = gd::GradSmem<KD>::ALLOC;
     if (const cudaError_t e = cudaFuncSetAttribute(gd::grads_kernel<T, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return set_error("grads_kernel: %s", cudaGetErrorString(e)), (int)e;
-    gd::grads_kernel<T, KD><<<dim3((unsigned)chunks, f.heads), gd::kGradThreads, smem, st>>>(g, gm);
+    gd::grads_kernel<T, KD><<<(unsigned)std::min<int64_t>(chunks * f.heads, sm_count()), gd::kGradThreads, smem, st>>>(g, gm);
     if (const int rc = launch_status("grads_kernel")) return rc;
     return g.dqk ? gd::fold_heads(g.dqk, g.dq, g.dk, g.tokens, f.kdim, f.key_heads, w.a.group, f.io_dtype, st) : (int)SSM_OK;
   };
