@@ -81,7 +81,11 @@ struct DeltaCall final : Call {
     input(g_), input(beta_), input(init_);
     q = lead(q_, t_v), k = lead(k_, t_v), v = strided(v_), beta = coefficient(beta_, "gated_delta_scan beta");
     if (g_.has_value()) g = coefficient(*g_, "gated_delta_scan g"), t_g = g_->scalar_type();
-    if (v.scalar_type() != at::kFloat && kd % 8 == 0 && kd <= 128 && vd % 8 == 0 && nl > 0 && nb > 0) {
+    // A few tokens without gradients walk one by one: a chunk costs the same whatever its tokens.  Measured (K = V = 128, bf16, us, chunks | tokens):
+    // 16 heads, 8 tokens 14.2 | 5.4, 16 tokens 14.3 | 7.6; 128 heads, 8 tokens 15.1 | 12.3, 16 tokens 15.2 | 18.2; 1024 heads, 4 tokens 56 | 54,
+    // 8 tokens 56 | 74; 8192 heads, 4 tokens 416 | 414.  With gradients chunks win from one token on (16 heads 33 | 48, 1024 heads 185 | 439).
+    const bool few = nl <= (nb * nh <= 128 ? 8 : 4) && !needs_grad();
+    if (v.scalar_type() != at::kFloat && kd % 8 == 0 && kd <= 128 && vd % 8 == 0 && nl > 0 && nb > 0 && !few) {
       chunked = true;
       q = copyable(q), k = copyable(k), v = copyable(v);
     }

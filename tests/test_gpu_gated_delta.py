@@ -125,6 +125,46 @@ def test_packed_sequences(dtype, kd, vd, cuts, where):
             assert not x[:, cuts[-1]:].any(), name
 
 
+@pytest.mark.parametrize("nb,nl,nk,nh,kd,vd,cuts", [
+    (3, 500, 4, 8, 128, 64, None), (4, 330, 4, 8, 64, 128, None), (5, 260, 4, 8, 128, 192, None), (2, 410, 16, 16, 72, 88, None),
+    (1, 1500, 6, 12, 128, 72, [0, 3, 70, 71, 200, 200, 520, 1111, 1400]), (1, 1500, 12, 12, 64, 128, [0, 640, 641, 1300]),
+])
+def test_more_chunks_than_blocks_side_by_side(nb, nl, nk, nh, kd, vd, cuts):
+    """The gradients' blocks take several chunks each: slices of 64 columns, one to three of them, whole and ragged, and chunks of no sequence."""
+    from ssm_b200 import ops
+
+    ts = inputs(nb, nl, nk, nh, kd, vd, BF16, seed=nl)
+    gen = torch.Generator().manual_seed(11)
+    do = torch.randn(nb, nl, nh, vd, generator=gen).to(BF16).double()
+    ref = [t.clone().requires_grad_(True) for t in ts]
+    o, _ = lm_oracle.gated_delta(*ref, cu_seqlens=cuts)
+    want = torch.autograd.grad(o, ref, do)
+    leaves = on_gpu(ts, BF16, True)
+    got_o = ops.gated_delta_scan(*leaves, cu_seqlens=None if cuts is None else torch.tensor(cuts).cuda())
+    longest = nl if cuts is None else max(b - a for a, b in zip(cuts, cuts[1:]))
+    near(got_o, o, tolerance(BF16, longest, kd, vd), "o")
+    got = torch.autograd.grad(got_o, leaves, do.to(BF16).cuda())
+    for name, x, y in zip(("q", "k", "v", "g", "beta"), got, want):
+        near(x, y, tolerance(BF16, longest, kd, vd, True), "gradient of " + name)
+        if cuts is not None:
+            assert not x[:, cuts[-1]:].any(), name
+
+
+@pytest.mark.parametrize("nb,nl,nk,nh", [(1, 8, 8, 16), (1, 9, 8, 16), (40, 4, 2, 4), (40, 5, 4, 4), (2, 1, 1, 1)])
+def test_a_few_tokens_without_gradients(nb, nl, nk, nh):
+    """On both sides of the choice between chunks and single tokens, a state carried on in place of a longer call."""
+    from ssm_b200 import ops
+
+    kd = vd = 128
+    ts = inputs(nb, 2 * nl, nk, nh, kd, vd, BF16, seed=nb + nl)
+    o, s = lm_oracle.gated_delta(*ts)
+    x = on_gpu(ts, BF16)
+    first = ops.gated_delta_scan(*[t[:, :nl] for t in x], return_final_state=True, keep_state_fp32=True)
+    second = ops.gated_delta_scan(*[t[:, nl:] for t in x], initial_state=first[1], return_final_state=True, keep_state_fp32=True)
+    near(torch.cat([first[0], second[0]], 1), o, tolerance(BF16, 2 * nl, kd, vd), "o")
+    near(second[1], s, tolerance(BF16, 2 * nl, kd, vd), "state")
+
+
 @pytest.mark.parametrize("cuts", [[0, 90, 40, 120], [5, -3, 500, 60], [0, 1 << 40, 0, 0], [100, 100, 100, 100]])
 def test_boundaries_on_the_device_that_break_the_rule_stay_inside(cuts):
     """Entries are clamped to rise from 0 to at most L: the call answers as for the clamped ones."""
