@@ -9,14 +9,18 @@
 //   w = dv = Y^T do + Wb D^T;   D0 = gam_64 D + do^T diag(scale gam) Q - w^T diag(gam) K
 //
 //   pairs_kernel   one CTA per (chunk, value head): X, Y, W, Z (and Wb), which depend on no state: all chunks at once.  Products by
-//                  mma.sync on 16 rows a warp; the inverse is fp32: blocks of 16 by substitution, then two rounds of block products.
+//                  mma.sync on 16 rows a warp; the inverse is kept in fp32: blocks of 16 by substitution, then two rounds of products of
+//                  blocks whose factors are split into two 16-bit pieces.  Bound: shared memory, 70 % of its cycles: 24 ns a chunk and head
+//                  on the whole GPU (192 us for 8192 at K = 128), 41 with Wb, whose registers spill.
 //   chunks_kernel  one CTA per (sequence, value head, 128 rows of the state): the walk over the chunks, forward or back (BACK).
-//   grads_kernel   one CTA per (chunk, value head): the other gradients from what both walks left (the formulas stand there).
+//   grads_kernel   a CTA per SM over all (chunk, value head): the other gradients from what both walks left (the formulas stand there).
 //
 // The walk is bound by its chain, the state of a chunk depending on the one before through two products and the conversions between
 // them.  So the state lies transposed, with vdim on the 128 lanes of tensor memory, and both products take their A operand from tensor memory,
 // written there by the threads that hold the rows: S (16 bits) x W^T, added to V^T X^T -> r -> times beta suf x K -> added to the state,
 // which stays in registers.  o needs neither r nor a product of its own: Y and Z are 64 more rows of the operands X and W.
+// Measured, K = V = 128: 1.2 us a chunk with 32 walks side by side (tensor pipe 48 % busy on the SMs that have one), 1.9 forward and 2.2 back of
+// which a training call's kept states and rest are a third; 128 walks move 796 MB in 141 us, 5.6 TB/s.
 // Roundings to 16 bits: S, W, Z, X, Y (from rounded P) and the weighted r, each half a step of the type; sums and the state between chunks are
 // fp32.  For bf16 the outputs and gradients of random inputs are 0.25 to 0.3 % off in norm before their own rounding (0.17 %).
 #include <algorithm>
@@ -170,30 +174,31 @@ __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t byt
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
 }
 
-// rows 16 r, columns 16 c of a 32 x 32 product of fp32 blocks in shared memory, by one warp; each factor in two 16-bit pieces, three products
-template <typename T>
-__device__ __forceinline__ void product32(float (&d)[2][4], const float* left, int ls, const float* right, int rs, int r0, int n0, int lane) {
+// 16 x 8 NB of a product of fp32 blocks in shared memory with an inner extent of K, by one warp: `left` points to its rows, `right` to its columns.
+// Each factor in two 16-bit pieces, three products
+template <typename T, int K, int NB>
+__device__ __forceinline__ void block_product(float (&d)[NB][4], const float* left, int ls, const float* right, int rs, int lane) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) d[0][e] = d[1][e] = 0.f;
+  for (int nb = 0; nb < NB; ++nb) d[nb][0] = d[nb][1] = d[nb][2] = d[nb][3] = 0.f;
   auto split = [](float x, float y, uint32_t& hi, uint32_t& lo) {
     hi = pack2<T>(x, y);
     const float2 z = unpack2<T>(hi);
     lo = pack2<T>(x - z.x, y - z.y);
   };
 #pragma unroll
-  for (int k0 = 0; k0 < 32; k0 += 16) {
+  for (int k0 = 0; k0 < K; k0 += 16) {
     uint32_t ah[4], al[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 x = *reinterpret_cast<const float2*>(&left[(r0 + (lane >> 2) + (e & 1) * 8) * ls + k0 + (lane & 3) * 2 + (e >> 1) * 8]);
+      const float2 x = *reinterpret_cast<const float2*>(&left[((lane >> 2) + (e & 1) * 8) * ls + k0 + (lane & 3) * 2 + (e >> 1) * 8]);
       split(x.x, x.y, ah[e], al[e]);
     }
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
+    for (int nb = 0; nb < NB; ++nb) {
       uint32_t bh[2], bl[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float* at = &right[(k0 + (lane & 3) * 2 + e * 8) * rs + n0 + nb * 8 + (lane >> 2)];
+        const float* at = &right[(k0 + (lane & 3) * 2 + e * 8) * rs + nb * 8 + (lane >> 2)];
         split(at[0], at[rs], bh[e], bl[e]);
       }
       mma16816<T>(d[nb], ah, bh[0], bh[1]);
@@ -304,48 +309,31 @@ __global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, co
       if ((i & 1) == lane >> 4) A[(r0 + i) * kAS + r0 + col] = x[i];
   }
   __syncthreads();
-  {  // pairs of blocks: X10 = -X11 (A10 X00); a thread has a row and four columns of one of the two
-    const int b = tid >> 6, row = (tid & 63) >> 2, c4 = (tid & 3) * 4;
-    const float* A10 = A + (b * 32 + 16) * kAS + b * 32;
-    const float* X00 = A + (b * 32) * kAS + b * 32;
-    const float* X11 = A + (b * 32 + 16) * kAS + b * 32 + 16;
-    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto product = [&](const float* left, const float* right, int rs) {
-      t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < 16; k += 4) {
-        const float4 m = *reinterpret_cast<const float4*>(&left[row * kAS + k]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = e == 0 ? m.x : e == 1 ? m.y : e == 2 ? m.z : m.w;
-          const float4 y = *reinterpret_cast<const float4*>(&right[(k + e) * rs + c4]);
-          t.x = fmaf(x, y.x, t.x), t.y = fmaf(x, y.y, t.y), t.z = fmaf(x, y.z, t.z), t.w = fmaf(x, y.w, t.w);
-        }
-      }
-    };
-    product(A10, X00, kAS);
-    *reinterpret_cast<float4*>(&tmp[(b * 16 + row) * kTS + c4]) = t;
+  auto put_rows = [&](float* to, int stride, const float (&d)[4], float sign) {  // 16 x 8 of a block
+    *reinterpret_cast<float2*>(&to[gi * stride + gj]) = make_float2(sign * d[0], sign * d[1]);
+    *reinterpret_cast<float2*>(&to[(gi + 8) * stride + gj]) = make_float2(sign * d[2], sign * d[3]);
+  };
+  {  // pairs of blocks: X10 = -X11 (A10 X00), two warps each
+    const int n0 = (warp & 1) * 8;
+    float* block = A + (warp >> 1) * 32 * (kAS + 1);
+    float *half = tmp + (warp >> 1) * 16 * kTS + n0, d[1][4];
+    block_product<T, 16>(d, block + 16 * kAS, kAS, block + n0, kAS, lane);
+    put_rows(half, kTS, d[0], 1.f);
     __syncthreads();
-    product(X11, tmp + b * 16 * kTS, kTS);
-    *reinterpret_cast<float4*>(&A[(b * 32 + 16 + row) * kAS + b * 32 + c4]) = make_float4(-t.x, -t.y, -t.z, -t.w);
+    block_product<T, 16>(d, block + 16 * kAS + 16, kAS, half, kTS, lane);
+    put_rows(block + 16 * kAS + n0, kAS, d[0], -1.f);
   }
   __syncthreads();
   {  // the same for the halves, 16 x 16 of it a warp
     const int br = (warp >> 1) * 16, bc = (warp & 1) * 16;
     float d[2][4];
-    product32<T>(d, A + 32 * kAS, kAS, A, kAS, br, bc, lane);
+    block_product<T, 32>(d, A + (32 + br) * kAS, kAS, A + bc, kAS, lane);
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      *reinterpret_cast<float2*>(&tmp[(br + gi) * kTS + bc + nb * 8 + gj]) = make_float2(d[nb][0], d[nb][1]);
-      *reinterpret_cast<float2*>(&tmp[(br + gi + 8) * kTS + bc + nb * 8 + gj]) = make_float2(d[nb][2], d[nb][3]);
-    }
+    for (int nb = 0; nb < 2; ++nb) put_rows(tmp + br * kTS + bc + nb * 8, kTS, d[nb], 1.f);
     __syncthreads();
-    product32<T>(d, A + 32 * kAS + 32, kAS, tmp, kTS, br, bc, lane);
+    block_product<T, 32>(d, A + (32 + br) * kAS + 32, kAS, tmp + bc, kTS, lane);
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      *reinterpret_cast<float2*>(&A[(32 + br + gi) * kAS + bc + nb * 8 + gj]) = make_float2(-d[nb][0], -d[nb][1]);
-      *reinterpret_cast<float2*>(&A[(32 + br + gi + 8) * kAS + bc + nb * 8 + gj]) = make_float2(-d[nb][2], -d[nb][3]);
-    }
+    for (int nb = 0; nb < 2; ++nb) put_rows(A + (32 + br) * kAS + bc + nb * 8, kAS, d[nb], -1.f);
   }
   __syncthreads();
   // X in 16 bits, and the operands of W (X with columns times -gam) and Wb (X^T with columns times beta suf)
