@@ -129,7 +129,7 @@ int ssm_gated_delta_step(const ssm_gated_delta_step_args* args, ssm_stream_t str
  * p = softmax(x).  logp[r] = log p[targets[r]]; 0 where targets[r] == ignore_index; NaN for any other target outside of the vocabulary.
  * entropy[r] = -sum p log p.  top_ids / top_logp (rows, top_k): the top_k largest logits in falling order, equal ones by rising id.
  * stats (rows, 4) fp32: what the backward pass needs.  A row of -inf alone has no distribution: log probabilities -inf, entropy 0,
- * gradients 0; a NaN or +inf in a row makes its results NaN.  vocab < 2^31, top_k <= min(vocab, 128).
+ * gradients 0; a NaN or +inf in a row makes its results NaN.  vocab <= 2^30, top_k <= min(vocab, 128).
  *
  * Backward: dlogits (rows, vocab) dense, from dlogp, dentropy, dtop_logp (each nullable).
  * ------------------------------------------------------------------------------------- */

@@ -614,10 +614,10 @@ int grad_of(GradArgs& g, int dtype, cudaStream_t st) {
 
 int check_rows(int64_t rows, int64_t stride, int vocab, int dtype, float temperature) {
   SSM_REQUIRE(rows >= 0 && vocab >= 1, SSM_ERR_SHAPE, "logits must have at least one column");
-  SSM_REQUIRE(rows <= (1 << 28) && vocab <= 0x7fffff00, SSM_ERR_TOO_LARGE, "logits: more than 2^28 rows or 2^31 columns");
+  SSM_REQUIRE(rows <= (1 << 28) && vocab <= (1 << 30), SSM_ERR_TOO_LARGE, "logits: more than 2^28 rows or 2^30 columns");
   SSM_REQUIRE(stride >= 0, SSM_ERR_SHAPE, "logits: negative row stride");
   SSM_REQUIRE(valid_dtype(dtype), SSM_ERR_DTYPE, "logits: unknown dtype");
-  SSM_REQUIRE(temperature > 0.f && temperature <= 3e38f, SSM_ERR_SHAPE, "temperature must be positive and finite");
+  SSM_REQUIRE(temperature >= 1e-37f && temperature <= 3e38f, SSM_ERR_SHAPE, "temperature must be positive and finite, and so its inverse");
   return SSM_OK;
 }
 int fill(const ssm_token_logp_args& a, StatsArgs& s) {

@@ -45,6 +45,7 @@ struct DeltaCall final : Call {
     SSM_ARG(k_.size(0) == nb && k_.size(1) == nl && q_.sizes() == k_.sizes(), "q and k must have shape (B, L, Hk, K) with v's B and L.");
     SSM_ARG(nk > 0 && nh > 0 && nh % nk == 0, "The key heads must divide the value heads.");
     SSM_ARG(kd > 0 && vd > 0, "K and V must be positive.");
+    SSM_ARG(kd <= 256 && vd <= 65536 && nh <= 65535, "gated_delta_scan: K is at most 256, V at most 65536, the heads at most 65535.");
     auto per_head = [&](const Tensor& t) { return t.dim() == 3 && t.size(0) == nb && t.size(1) == nl && t.size(2) == nh; };
     SSM_ARG(per_head(beta_) && (!g_.has_value() || per_head(*g_)), "g and beta must have shape (B, L, H).");
     scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)kd);
@@ -183,6 +184,7 @@ Tensor gated_delta_step(const Tensor& state, const Tensor& q_, const Tensor& k_,
   const int64_t nk = k_.size(1);
   SSM_ARG(nk > 0 && nh > 0 && nh % nk == 0, "The key heads must divide the value heads.");
   SSM_ARG(kd > 0 && vd > 0, "K and V must be positive.");
+  SSM_ARG(kd <= 256 && vd <= 65536 && nh <= 65535, "gated_delta_step: K is at most 256, V at most 65536, the heads at most 65535.");
   auto per_head = [&](const Tensor& t) { return t.dim() == 2 && t.size(0) == nb && t.size(1) == nh; };
   SSM_ARG(per_head(beta_) && (!g_.has_value() || per_head(*g_)), "g and beta must have shape (B, H).");
   same_device(state, {&q_, &k_, &v_, &beta_});
@@ -208,6 +210,7 @@ Tensor gated_delta_step(const Tensor& state, const Tensor& q_, const Tensor& k_,
   }
   run(ssm_gated_delta_step(&a, stream_of(state)));
   if (!state.is_contiguous()) state.detach().copy_(work);
+  else if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();  // a graph that keeps this state for its backward pass notices
   return o;
 }
 
@@ -228,6 +231,7 @@ std::vector<int64_t> without_last(const Tensor& t) {
 }
 void logits_check(const Tensor& logits, double temperature, const char* what) {
   SSM_ARG(logits.dim() >= 1 && logits.size(-1) >= 1, "logits must have shape (..., V) with V of at least one.");
+  SSM_ARG(logits.size(-1) <= (1 << 30), "logits: more than 2^30 columns.");
   SSM_ARG(temperature > 0 && std::isfinite(temperature), "temperature must be positive and finite.");
   TORCH_CHECK(logits.is_cuda(), "ssm_b200 operators run on CUDA tensors only; there is no CPU fallback");
   dtype_code(logits, what);

@@ -441,3 +441,52 @@ def test_a_long_chain_in_16_bits():
     got = ops.gated_delta_scan(*on_gpu(ts, BF16, g_dtype=F32), return_final_state=True, keep_state_fp32=True)
     near(got[0], o, tolerance(BF16, 1, 128, 128))
     near(got[1], s, tolerance(BF16, 1, 128, 128))
+
+
+@pytest.mark.parametrize("dtype,kd,vd", [(F32, 24, 40), (BF16, 128, 128), (F16, 64, 72)])
+def test_nan_and_inf_stay_in_their_sequence(dtype, kd, vd):
+    """A sequence of NaN and infinities between others, in the same chunks of rows, and rows of NaN behind the last one."""
+    from ssm_b200 import ops
+
+    cuts, nl, nh = [0, 40, 75, 170, 171], 200, 2
+    ts = inputs(1, nl, 1, nh, kd, vd, dtype)
+    do = torch.randn(1, nl, nh, vd, generator=torch.Generator().manual_seed(3)).to(dtype).double()
+    cu = torch.tensor(cuts).cuda()
+
+    def call(spoil):
+        leaves = on_gpu(ts, dtype)
+        go = do.to(dtype).cuda()
+        if spoil:
+            for t in (*leaves, go):
+                t[:, 40:75] = float("nan")
+                t[:, 60] = float("inf")
+                t[:, 171:] = float("nan")
+        leaves = [t.requires_grad_(True) for t in leaves]
+        o, s = ops.gated_delta_scan(*leaves, return_final_state=True, keep_state_fp32=True, cu_seqlens=cu)
+        with torch.no_grad():
+            again = ops.gated_delta_scan(*leaves, return_final_state=True, keep_state_fp32=True, cu_seqlens=cu)
+        return [o, s, *again, *torch.autograd.grad(o, leaves, go)]
+
+    clean, spoilt = call(False), call(True)
+    keep = torch.tensor([i for i in range(nl) if not 40 <= i < 75], device="cuda")
+    for i, (x, y) in enumerate(zip(clean, spoilt)):
+        if i in (1, 3):  # states
+            assert torch.equal(x[[0, 2, 3]], y[[0, 2, 3]]) and not torch.isfinite(y[1]).all()
+        else:
+            assert torch.equal(x[:, keep], y[:, keep]), i
+
+
+def test_a_step_on_a_state_that_a_graph_keeps_is_noticed():
+    from ssm_b200 import ops
+
+    x = on_gpu(inputs(1, 70, 1, 2, 64, 64, BF16), BF16, True)
+    state = torch.randn(1, 2, 64, 64, device="cuda")
+    o = ops.gated_delta_scan(*x, initial_state=state)
+    with torch.no_grad():
+        ops.gated_delta_step(state, *[t[:, 0] for t in x])
+    with pytest.raises(RuntimeError, match="modified in place"):
+        o.sum().backward()
+    with torch.inference_mode():  # no version counter there
+        held = torch.zeros(1, 2, 64, 64, device="cuda")
+        ops.gated_delta_step(held, *[t[:, 0] for t in x])
+        assert held.any()

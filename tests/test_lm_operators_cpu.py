@@ -164,6 +164,62 @@ def test_topk_distill_refuses_without_a_gpu(code, kw):
     assert lib.ssm_topk_distill(ctypes.byref(a), None) == code
 
 
+@pytest.mark.parametrize("code,kw", [
+    (-1, {}), (-2, {"heads": 3, "key_heads": 2}), (-2, {"kdim": 0}), (-3, {"io_dtype": 9}), (-2, {"batch": 2, "num_seqs": 1})])
+def test_chunked_gated_delta_refuses_without_a_gpu(code, kw):
+    from ssm_b200 import _lib
+
+    lib = _lib.load()
+    g = _lib.GatedDeltaBwdArgs()
+    g.fwd = _delta_args(io_dtype=1, **{k: x for k, x in kw.items() if k != "io_dtype"})
+    if "io_dtype" in kw:
+        g.fwd.io_dtype = kw["io_dtype"]
+    assert lib.ssm_gated_delta_chunked_fwd(ctypes.byref(g.fwd), None, None, 0, None, None) == code
+    assert lib.ssm_gated_delta_chunked_bwd(ctypes.byref(g), None, None, None, None) == code
+    assert lib.ssm_gated_delta_chunked_fwd(None, None, None, 0, None, None) == lib.ssm_gated_delta_chunked_bwd(None, None, None, None, None) == -1
+
+
+def test_what_goes_to_the_tensor_cores():
+    """Pointers are looked at for their alignment alone here."""
+    from ssm_b200 import _lib
+
+    lib = _lib.load()
+
+    def supported(**kw):
+        a = _delta_args(io_dtype=1)
+        a.q = a.k = a.v = a.o = 4096
+        a.q_sh = a.k_sh = a.v_sh = 8
+        a.q_st = a.k_st = a.v_st = 16
+        a.q_sb = a.k_sb = a.v_sb = 64
+        for name, value in kw.items():
+            setattr(a, name, value)
+        return lib.ssm_gated_delta_chunked_supported(ctypes.byref(a))
+
+    assert supported() == supported(io_dtype=2) == supported(kdim=128) == supported(vdim=1024) == 1
+    for kw in ({"io_dtype": 0}, {"kdim": 12}, {"kdim": 136}, {"kdim": 0}, {"vdim": 4}, {"vdim": 100}, {"len": 0}, {"q": 4098}, {"k": 4104}, {"v": 4100}, {"o": 4104},
+               {"initial_state": 4100}, {"q_st": 12}, {"k_st": 0}, {"v_st": -16}, {"v_sh": 4}, {"heads": 0}, {"key_heads": 0}):
+        assert supported(**kw) == 0, kw
+    assert lib.ssm_gated_delta_chunked_supported(None) == 0
+
+
+def test_sizes_beyond_32_bits_are_refused_before_they_are_cut():
+    from ssm_b200 import ops
+
+    wide = torch.zeros(1).expand(2, (1 << 32) + 5)
+    with pytest.raises(ValueError, match="columns"):
+        ops.token_log_probs(wide, torch.zeros(2, dtype=torch.long))
+    with pytest.raises(ValueError, match="columns"):
+        ops.topk_distill_loss(wide, torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.long))
+    one = torch.zeros(1)
+    big = (1 << 32) + 8
+    for kd, vd, nh in ((big, 8, 2), (8, big, 2), (8, 8, 1 << 17)):
+        q, v, b = one.expand(1, 3, 1, kd), one.expand(1, 3, nh, vd), one.expand(1, 3, nh)
+        with pytest.raises(ValueError, match="at most"):
+            ops.gated_delta_scan(q, q, v, b, b)
+        with pytest.raises(ValueError, match="at most"):
+            ops.gated_delta_step(one.expand(1, nh, vd, kd), q[:, 0], q[:, 0], v[:, 0], b[:, 0], b[:, 0])
+
+
 def test_operators_refuse_wrong_shapes_and_cpu_tensors():
     from ssm_b200 import ops
 
