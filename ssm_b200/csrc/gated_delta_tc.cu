@@ -788,19 +788,22 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
     const int width = min(kSlice, a.vd - v / kSlice * kSlice);
     auto unit_at = [&](int units, int u) { return v / kSlice * kSlice * units + u * width + v % kSlice; };
     // the state as an operand, and for a backward pass to follow
+    uint32_t x16[NS / 2];
+    auto keep_units = [&](int p, int from, int to) {
+      uint4* keep = reinterpret_cast<uint4*>(w.states) + ((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (KD / 8) * a.vd + unit_at(KD / 8, part * (NS / 8));
+#pragma unroll
+      for (int u = 0; u < NS / 8; ++u)
+        if (u >= from && u < to) keep[u * width] = make_uint4(x16[4 * u], x16[4 * u + 1], x16[4 * u + 2], x16[4 * u + 3]);
+    };
     auto publish = [&](int p) {
-      uint32_t x[NS / 2];
+      auto& x = x16;
 #pragma unroll
       for (int e = 0; e < NS / 2; ++e) x[e] = pack2<T>(S[2 * e], S[2 * e + 1]);
 #pragma unroll
       for (int q = 0; q < NS / 32; ++q) tc::tmem_st16(tmem + lanes + TC::S + part * (NS / 2) + q * 16, reinterpret_cast<const uint32_t(&)[16]>(x[q * 16]));
       tc::tmem_wait_st();
       done(kState);
-      if (w.states && live) {
-        uint4* keep = reinterpret_cast<uint4*>(w.states) + ((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (KD / 8) * a.vd + unit_at(KD / 8, part * (NS / 8));
-#pragma unroll
-        for (int u = 0; u < NS / 8; ++u) keep[u * width] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
-      }
+      if (w.states && live) keep_units(p, 0, BACK ? NS / 16 : NS / 8);
     };
     if (nchunks > 0) publish(0);
     for (int p = 0; p < nchunks; ++p) {
@@ -826,6 +829,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
         tc::tmem_st16(tmem + lanes + TC::U + part * (NT / 2), y);
         tc::tmem_wait_st();
         done(kU);
+        if constexpr (BACK)  // the rest of the state here, where the rows wait again: 126 us, 141 in one piece
+          if (w.states && live) keep_units(p, NS / 16, NS / 8);
         if constexpr (!BACK)
           if (w.rest && live) {
 #pragma unroll
