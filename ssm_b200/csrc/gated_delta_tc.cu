@@ -19,8 +19,8 @@
 // them.  So the state lies transposed, with vdim on the 128 lanes of tensor memory, and both products take their A operand from tensor memory,
 // written there by the threads that hold the rows: S (16 bits) x W^T, added to V^T X^T -> r -> times beta suf x K -> added to the state,
 // which stays in registers.  o needs neither r nor a product of its own: Y and Z are 64 more rows of the operands X and W.
-// Measured, K = V = 128: 1.2 us a chunk with 32 walks side by side (tensor pipe 48 % busy on the SMs that have one), 1.9 forward and 2.2 back of
-// which a training call's kept states and rest are a third; 128 walks move 796 MB in 141 us, 5.6 TB/s.
+// Measured, K = V = 128: 1.2 us a chunk with 32 walks side by side (tensor pipe 48 % busy on the SMs that have one), 1.9 where a training call's
+// states and rest are stored, forward and back; 128 walks move 796 MB in 141 us, 5.6 TB/s.
 // Roundings to 16 bits: S, W, Z, X, Y (from rounded P) and the weighted r, each half a step of the type; sums and the state between chunks are
 // fp32.  For bf16 the outputs and gradients of random inputs are 0.25 to 0.3 % off in norm before their own rounding (0.17 %).
 #include <algorithm>
@@ -829,7 +829,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
         tc::tmem_st16(tmem + lanes + TC::U + part * (NT / 2), y);
         tc::tmem_wait_st();
         done(kU);
-        if constexpr (BACK)  // the rest of the state here, where the rows wait again: 126 us, 141 in one piece
+        if constexpr (BACK)  // the rest of the state here, where the rows wait again: 124 us, 141 in one piece
           if (w.states && live) keep_units(p, NS / 16, NS / 8);
         if constexpr (!BACK)
           if (w.rest && live) {
@@ -879,7 +879,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
 // Sixteen warps, each 16 tokens x a quarter of the columns, products by mma.sync (15 Mflop a chunk); one block an SM that walks over its
 // chunks, 64 columns of v at a time, with the next two slices' copies under way (145 KB read and 32 KB written a chunk).  A slice of the states
 // lies in one piece, since copies of a kilobyte each cost their warp more than its products (187 -> 164 us).  Bound: instructions, some 2100 a
-// warp and chunk at 1.7 a cycle, of which 200 are products.  2 x 4096 tokens x 16 heads: 164 us, 2.2 TB/s; with eight warps and a block a chunk 204.
+// warp and chunk at 1.7 a cycle, of which 200 are products.  2 x 4096 tokens x 16 heads: 160 us, 2.2 TB/s; with eight warps and a block a chunk 204.
 struct GradMaps {
   CUtensorMap q, k, d, w;
 };
@@ -947,21 +947,26 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
       for (int i = tid; i < n; i += kGradThreads) g.dg[(tok + i) * a.heads + h] = 0.f, g.dbeta[(tok + i) * a.heads + h] = 0.f;
     }
   // the others, in this block's order
+  struct Item {
+    int it, h;
+    Span s;
+  };
   auto from_on = [&](int it) {
-    for (; it < items; it += gridDim.x) {
-      const Span s = chunk_of(a.where, it % g.chunks, C);
-      if (s.t1 > s.t0 && s.seq >= 0) break;
+    Item x{it, 0, {}};
+    for (; x.it < items; x.it += gridDim.x) {
+      x.h = x.it / g.chunks, x.s = chunk_of(a.where, x.it - x.h * g.chunks, C);
+      if (x.s.t1 > x.s.t0 && x.s.seq >= 0) break;
     }
-    return it;
+    return x;
   };
   const uint32_t base = tc::smem_u32(sm), bars = tc::smem_u32(mbar);
   float* c = reinterpret_cast<float*>(sm + M::VEC);
   float *beta = c + C, *gam = beta + C, *suf = gam + C, *rows = suf + C, *cols = rows + 4 * C;  // [4][C] each: sums of M
   float *into = cols + 4 * C, *outof = into + 4 * C, *db = outof + 4 * C, *part = db + 4 * C;   // [4][C] each; a partial sum of every warp
   // a slice's copies, by warp 0: what follows is on its way while a chunk is worked on
-  auto request = [&](int it, int slice, int to_slice, int to_qk) {
-    const Span s = chunk_of(a.where, it % g.chunks, C);
-    const int h = it / g.chunks, kh = h / a.group, v0 = slice * kSlice, nv = min(kSlice, a.vd - v0);
+  auto request = [&](const Item& x, int slice, int to_slice, int to_qk) {
+    const Span& s = x.s;
+    const int h = x.h, kh = h / a.group, v0 = slice * kSlice, nv = min(kSlice, a.vd - v0);
     const int64_t pair = (int64_t)s.chunk * a.heads + h;
     const uint32_t bar = bars + to_slice * 8, to = base + to_slice * M::SLICE, qk = base + M::QK + to_qk * 2 * M::KT;
     if (lane == 0) {
@@ -992,26 +997,25 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
   };
   if (tid == 0) tc::mbar_init(bars, 1), tc::mbar_init(bars + 8, 1);
   __syncthreads();
-  int it = from_on(blockIdx.x);
+  Item now = from_on(blockIdx.x);
   int used = 0, asked = 0, ahead = 0, ahead_slice = 0;  // slices worked on and asked for; the next to ask for, `ahead` chunks from the current one
   const int r0 = (warp >> 2) * 16, quarter = (warp + (warp >> 2)) & 3, c0 = quarter * 16, k_cols = quarter * (KD / 4), gi = lane >> 2, gj = (lane & 3) * 2;
   TokenPair token{};
-  auto tokens_of = [&](int i) {
-    if (i >= items) return;
-    const Span s = chunk_of(a.where, i % g.chunks, C);
-    token = token_pair(a, s, s.t1 - s.t0, i / g.chunks, lane);
+  auto tokens_of = [&](const Item& x) {
+    if (x.it < items) token = token_pair(a, x.s, x.s.t1 - x.s.t0, x.h, lane);
   };
   constexpr int kDecays = 5, kSums = 10;  // warps that do more than their share, each with another scheduler; warp 0 asks for the copies
-  if (warp == kDecays) tokens_of(it);
-  for (int order = 0; it < items; ++order) {
-    const Span s = chunk_of(a.where, it % g.chunks, C);
-    const int n = s.t1 - s.t0, h = it / g.chunks, next = from_on(it + gridDim.x);
+  if (warp == kDecays) tokens_of(now);
+  for (int order = 0; now.it < items; ++order) {
+    const Item next = from_on(now.it + gridDim.x);
+    const Span s = now.s;
+    const int n = s.t1 - s.t0, h = now.h;
     const int64_t tok = (int64_t)s.b * a.len + s.t0;
     unsigned char* qk = sm + M::QK + (order & 1) * 2 * M::KT;
     const uint32_t qk_base = tc::smem_u32(qk);
     auto feed = [&] {  // as far as there are buffers: two of slices, and for q and k this chunk's and the next one's
-      for (; asked - used < 2 && ahead < 2 && (ahead ? next : it) < items; ++asked) {
-        if (warp == 0) request(ahead ? next : it, ahead_slice, asked & 1, (order + ahead) & 1);
+      for (; asked - used < 2 && ahead < 2 && (ahead ? next.it : now.it) < items; ++asked) {
+        if (warp == 0) request(ahead ? next : now, ahead_slice, asked & 1, (order + ahead) & 1);
         if (++ahead_slice == slices) ahead_slice = 0, ++ahead;
       }
     };
@@ -1251,7 +1255,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grads_kernel(const ChunkGrads
         }
       }
     }
-    it = next, --ahead;  // all of this chunk's slices have been asked for
+    now = next, --ahead;  // all of this chunk's slices have been asked for
   }
 }
 
