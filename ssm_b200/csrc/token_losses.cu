@@ -23,8 +23,12 @@ constexpr int kThreads = 256;  // 4096 rows of 50280 bf16 logits with 5 alternat
 constexpr int kUnroll = 4, kUnrollTop = 2;
 constexpr int kCandidates = 1024;  // kept elements of a slice above the bound, and at it
 constexpr int kMaxTop = 128;
-constexpr int kGroups = kThreads / 2;  // groups of threads whose maxima are looked at, at most
+constexpr int kGroups = kThreads;  // groups of threads whose maxima are looked at, at most
 constexpr int kMaxTeacher = 1024;
+
+// threads of a group: twice as many groups as alternatives
+__device__ __forceinline__ int group_size(int k) { return k <= kThreads / 16 ? 8 : k <= kThreads / 8 ? 4 : k <= kThreads / 4 ? 2 : 1; }
+static_assert(2 * kMaxTop <= kThreads, "a group has a thread");
 
 enum Flags { kEntropy = 1, kTop = 2 };
 
@@ -243,8 +247,8 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
     parts_of(w2, x, y), me.w = x + y;
   }
 
-  if constexpr ((FLAGS & kTop) != 0) {  // maxima of groups of threads, at least twice as many as alternatives where that is possible
-    const int size = a.top_k <= kGroups / 8 ? 8 : a.top_k <= kGroups / 4 ? 4 : 2;
+  if constexpr ((FLAGS & kTop) != 0) {  // maxima of groups of threads, at least twice as many as alternatives
+    const int size = group_size(a.top_k);
     float top = me.m == kFloor ? -INFINITY : me.m;
     for (int off = 1; off < size; off *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     if (tid % size == 0) maxima[tid / size] = top;
@@ -269,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
 
   if constexpr ((FLAGS & kTop) != 0) {
     const int k = a.top_k;
-    const int groups = kThreads / (k <= kGroups / 8 ? 8 : k <= kGroups / 4 ? 4 : 2);
+    const int groups = kThreads / group_size(k);
     if (tid < groups) {  // the k-th largest of the groups' maxima
       const float own = maxima[tid];
       int above = 0;
