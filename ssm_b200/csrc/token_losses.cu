@@ -88,6 +88,16 @@ __device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
   return r;
 }
 
+// one element of a piece, chosen at run time
+template <typename T>
+__device__ __forceinline__ float element(const Vec16<T>& v, int j) {
+  const int word = j * (int)sizeof(T) / 4;
+  const uint32_t w = word < 2 ? (word == 0 ? v.raw.x : v.raw.y) : word == 2 ? v.raw.z : v.raw.w;
+  if constexpr (std::is_same<T, float>::value) return __uint_as_float(w);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+  else return __half2float(__ushort_as_half((uint16_t)(j & 1 ? w >> 16 : w)));
+}
+
 // the largest (BIG) or smallest value of 16-byte pieces; a NaN makes the result NaN (NAN_COUNTS), or is passed over
 template <bool BIG, bool NAN_COUNTS, typename T, int P>
 __device__ __forceinline__ float extreme(const Vec16<T> (&r)[P]) {
@@ -302,8 +312,13 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
       for (int p = 0; p < P; ++p) {
         float f[V];
         r[p].unpack(f);
+        uint32_t reach = 0;  // a branch for each of the few, not for each element: 4096 rows, 20 alternatives: 137 us, 158
 #pragma unroll
-        for (int j = 0; j < V; ++j) keep(f[j], ids[p] + j);
+        for (int j = 0; j < V; ++j) reach |= f[j] < bound ? 0u : 1u << j;
+        for (; reach; reach &= reach - 1) {
+          const int j = __ffs(reach) - 1;
+          keep(element(r[p], j), ids[p] + j);
+        }
       }
     });
     if (tid < kMaxTop) best[tid] = 0;  // below every key
