@@ -18,9 +18,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;  // 4096 rows of 50280 bf16 logits with 5 alternatives: 154 us, 204 with 512; forward and backward of 8192 rows 436, 454
-// 16-byte pieces a thread has in flight.  Two where alternatives are kept, whose registers four would take from other rows: 136 us instead of 154
-constexpr int kUnroll = 4, kUnrollTop = 2;
+constexpr int kThreads = 256;  // forward and backward of 8192 rows of 50280 bf16 logits: 436 us, 442 with 128, 454 with 512
+constexpr int kUnroll = 4;  // 16-byte pieces a thread has in flight; with alternatives, 4096 rows and 5 of them: 107 us, 125 with two
 constexpr int kCandidates = 1024;  // kept elements of a slice above the bound, and at it
 constexpr int kMaxTop = 128;
 constexpr int kGroups = kThreads;  // groups of threads whose maxima are looked at, at most
@@ -222,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
         me.m = top, me.M = M, M2 = pair_of(-M, -M);
       }
     };
-    walk<T, (FLAGS & kTop) != 0 ? kUnrollTop : kUnroll>(
+    walk<T, kUnroll>(
         row, lo, hi, tid, kThreads,
         [&](float x, int) {
           raise(x);
@@ -305,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
         if (at < kCandidates) cand[at] = key_of(x, id);
       }
     };
-    walk<T, kUnrollTop>(row, lo, hi, tid, kThreads, keep, [&](const auto& r, const int* ids) {
+    walk<T, kUnroll>(row, lo, hi, tid, kThreads, keep, [&](const auto& r, const int* ids) {
       constexpr int V = Vec16<T>::N, P = sizeof(r) / sizeof(r[0]);
       if (extreme<true, true>(r) < bound) return;
 #pragma unroll
