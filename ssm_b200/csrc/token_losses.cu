@@ -1,14 +1,18 @@
 // Log probabilities of given tokens (with entropy and top alternatives) and distillation from a teacher's top logits.
 //
 // Both are one pass over a row of logits.  With c = log2(e) / T and a running reference M (c times the largest logit so far), d = c x - M:
-// s = sum 2^d and, for the entropy, w = sum d 2^d; then log2 p_i = d_i - log2 s and H = (log2 s - w / s) ln 2.  M is rounded, but the same in every
-// term, so that it drops out.  The backward pass is one more read of the row and one write of its gradient.  Bound: HBM (two or four bytes an element
-// each way), beside 16 exponentials a cycle and SM: 91 us of them where 8192 x 50280 bf16 logits take 126 us to read.  A row goes to one CTA, or to a
+// s = sum 2^d and, for the entropy, w = sum d 2^d; then log2 p_i = d_i - log2 s and H = (log2 s - w / s) ln 2.  M is rounded, by at most half a step of
+// its own size, but the same in every term, so that it drops out as long as 2 to that power is a number to reckon with: rows whose M is
+// beyond kFar are summed once more with differences before products.  The backward pass is one more read of the row and one write of its gradient.
+// Bound: HBM (two or four bytes an element each way), beside 16 exponentials a cycle and SM: 91 us of them where 8192 x 50280 bf16 logits take 126 us
+// to read.  A row goes to one CTA, or to a
 // cluster of up to eight that join their sums through distributed shared memory where the rows alone would not fill the GPU.
 //
 // Top alternatives: the k-th largest of the maxima of groups of threads bounds the k-th largest logit from below, so a second
 // pass over the row (which then lies in the L2) keeps the few elements at or above it, and ranks them by (value, lowest id).
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "../../include/ssm_b200_lm.h"
 #include "common.cuh"
@@ -127,16 +131,17 @@ __device__ __forceinline__ float extreme(const Vec16<T> (&r)[P]) {
   }
 }
 
-// m: the largest logit seen, M: c m, the reference of s and w.  Logits below kFloor count for nothing here, whose c x might overflow: beside any other they
-// do not, and rows without any other are looked at again.  A NaN in s stays
-constexpr float kFloor = -1e37f;
+// m: the largest logit seen, M: the reference of s and w, c m but no less than -kFar.  Against that one, logits far below count for nothing: beside any above it
+// they do not, and rows without one are looked at again, as those with c m beyond kFar are.  A NaN in s stays
+constexpr float kFar = 268435456.f;  // 2^28, rounded by 16 at most: s between 2^-16 and V 2^16, log2 s and d off by 2^-20 each
 struct Sums {
   float m, M, s, w;
 };
+__device__ __forceinline__ Sums nothing() { return {-INFINITY, -kFar, 0.f, 0.f}; }
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   const bool first = a.m >= b.m;
   const Sums &hi = first ? a : b, &lo = first ? b : a;
-  const float d = lo.m == kFloor ? 0.f : lo.M - hi.M, e = lo.m == kFloor ? 1.f : ex2_approx(d);  // nothing in lo: s is 0 or NaN
+  const float d = lo.M - hi.M, e = ex2_approx(d);
   return {hi.m, hi.M, hi.s + lo.s * e, hi.w + e * fmaf(lo.s, fmaxf(d, -1e30f), lo.w)};
 }
 __device__ __forceinline__ Sums exchanged(const Sums& a, int off) {
@@ -146,7 +151,7 @@ __device__ __forceinline__ Sums exchanged(const Sums& a, int off) {
 struct StatsArgs {
   int64_t rows, row_stride, ignore;
   int vocab, top_k, teacher_dtype;
-  float c, inv_t;
+  float c, inv_t, low;  // of logits from `low` on c x is a number
   const void* logits;
   const int64_t* targets;
   const void* teacher;
@@ -155,7 +160,7 @@ struct StatsArgs {
   float* entropy;
   float* top_logp;
   int64_t* top_ids;
-  float4* stats;  // M, log2 s, entropy, 0; m in M's place and 2 where all logits lie below kFloor; 1 for a row of -inf
+  float4* stats;  // M, log2 s, entropy, 0; m in M's place and 2 where the row was summed by differences; 1 for a row of -inf
 };
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -209,12 +214,12 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
 
   const float c = a.c;
   const pair_t c2 = pair_of(c, c);
-  Sums me{kFloor, 0.f, 0.f, 0.f};
+  Sums me = nothing();
   {
-    pair_t s2 = pair_of(0.f, 0.f), w2 = s2, M2 = s2;
+    pair_t s2 = pair_of(0.f, 0.f), w2 = s2, M2 = pair_of(kFar, kFar);
     auto raise = [&](float top) {
       if (top > me.m) {
-        const float M = top * c, d = me.M - M, e = me.m == kFloor ? 0.f : ex2_approx(d);
+        const float M = fmaxf(top * c, -kFar), d = me.M - M, e = ex2_approx(d);
         const pair_t e2 = pair_of(e, e), none = pair_of(0.f, 0.f);
         if constexpr ((FLAGS & kEntropy) != 0) w2 = fma2(e2, fma2(s2, pair_of(d, d), w2), none);
         s2 = fma2(e2, s2, none);
@@ -248,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
               }
             }
           };
-          if ((FLAGS & kEntropy) != 0 && extreme<false, false>(r) < -1e30f) add(std::true_type());  // 0 times -inf
+          if ((FLAGS & kEntropy) != 0 && extreme<false, false>(r) < a.low) add(std::true_type());  // 0 times -inf
           else add(std::false_type());
         });
     float x, y;
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
 
   if constexpr ((FLAGS & kTop) != 0) {  // maxima of groups of threads, at least twice as many as alternatives
     const int size = group_size(a.top_k);
-    float top = me.m == kFloor ? -INFINITY : me.m;
+    float top = me.m;
     for (int off = 1; off < size; off *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     if (tid % size == 0) maxima[tid / size] = top;
   }
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
   if (tid == 0) count = equals = 0, bound_s = -INFINITY;
   __syncthreads();
   if (warp == 0) {
-    me = lane < kThreads / 32 ? part[lane] : Sums{kFloor, 0.f, 0.f, 0.f};
+    me = lane < kThreads / 32 ? part[lane] : nothing();
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) {
       const Sums o = exchanged(me, off);
@@ -408,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
   }
 
   float kind = 0.f;
-  if (all.s == 0.f) {  // nothing above kFloor: the whole row once more, by this CTA, with differences before products
+  if (!(fabsf(all.M) < kFar)) {  // the whole row once more, by this CTA, with differences before products
     __syncthreads();
     auto over = [&](float v, auto f) {  // over the threads
       for (int off = 16; off >= 1; off >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, off));
@@ -419,24 +424,39 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
       __syncthreads();
       return v;
     };
+    auto each = [&](auto f) {
+      walk<T, 2>(row, 0, a.vocab, tid, kThreads, [&](float x, int) { f(x); }, [&](const auto& r, const int*) {
+        constexpr int V = Vec16<T>::N, P = sizeof(r) / sizeof(r[0]);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          float x[V];
+          r[p].unpack(x);
+#pragma unroll
+          for (int j = 0; j < V; ++j) f(x[j]);
+        }
+      });
+    };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
     auto sum = [](float x, float y) { return x + y; };
-    float m = -INFINITY, s = 0.f, w = 0.f;
-    for (int id = tid; id < a.vocab; id += kThreads) m = fmaxf(m, to_f<T>(row[id]));
-    m = over(m, [](float x, float y) { return fmaxf(x, y); });
+    float m = -INFINITY, bad = 0.f, s = 0.f, w = 0.f;
+    each([&](float x) { m = fmaxf(m, x), bad = x != x ? 1.f : bad; });
+    m = over(m, larger), bad = over(bad, larger);
     if (m != -INFINITY)
-      for (int id = tid; id < a.vocab; id += kThreads) {
-        const float d = (to_f<T>(row[id]) - m) * c, e = ex2_approx(d);
+      each([&](float x) {
+        const float d = (x - m) * c, e = ex2_approx(d);
         s += e, w = fmaf(e, fmaxf(d, -1e30f), w);
-      }
+      });
     s = over(s, sum), w = over(w, sum);
+    if (bad != 0.f) s = w = __uint_as_float(0x7fc00000u);  // beside -inf alone too
     all = {m, m, s, w};
-    kind = m == -INFINITY ? 1.f : 2.f;
+    kind = m == -INFINITY && bad == 0.f ? 1.f : 2.f;
   }
   const bool none = kind == 1.f;
   const float log2s = none ? 0.f : log2f(all.s), entropy = none ? 0.f : kLn2 * (log2s - all.w / all.s);
   auto logp_of = [&](float x) {
     if (none) return -INFINITY;
-    return x < kFloor ? fmaf(x - all.m, a.inv_t, -kLn2 * log2s) : kLn2 * (fmaf(x, c, -all.M) - log2s);
+    const float l = kLn2 * (fmaf(x, c, -all.M) - log2s);
+    return kind == 2.f || l == -INFINITY ? fmaf(x - all.m, a.inv_t, -kLn2 * log2s) : l;  // c x can be beyond the numbers where x / T is not
   };
   if (tid == 0) {
     if (a.stats) a.stats[r] = make_float4(all.M, log2s, entropy, kind);
@@ -532,12 +552,12 @@ __device__ __forceinline__ void row_grad(const GradArgs& g, const float4 st, int
       col[j] = j < k ? (int)a.top_ids[r * k + j] : in && t != a.ignore ? (int)t : -1;
     }
   }
-  const float on_plogp = -dh * kLn2 * a.inv_t, c = a.c;
+  const float on_plogp = -dh * kLn2 * a.inv_t, c = a.c, at_zero = on_p != on_p ? on_p : 0.f;
   auto grad = [&](float x) {
     const float e = (PLAIN ? fmaf(x, c, -st.x) : (x - st.x) * c) - st.y;
     const float p = ex2_approx(e);
     if constexpr (DISTILL) return none ? 0.f : p * on_p;
-    else return none ? 0.f : p * fmaf(on_plogp, fmaxf(e, -1e30f), on_p);
+    else return none ? 0.f : p == 0.f ? at_zero : p * fmaf(on_plogp, e, on_p);  // e of -inf, or so large that its product with 1 / T is no number
   };
   // the rows of the gradient are dense, those of the logits need not be: whole pieces where both lie alike
   const bool alike = (reinterpret_cast<uintptr_t>(row + lo) % 16) == (reinterpret_cast<uintptr_t>(out + lo) % 16);
@@ -583,7 +603,7 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradArgs g) {
   __shared__ int col[kEntries];
   __shared__ float coef[kEntries];
   const float4 st = g.f.stats[blockIdx.x / g.splits];
-  if (st.w == 2.f) row_grad<T, DISTILL, false>(g, st, col, coef);  // all logits of the row below kFloor
+  if (st.w == 2.f) row_grad<T, DISTILL, false>(g, st, col, coef);  // summed by differences
   else row_grad<T, DISTILL, true>(g, st, col, coef);
 }
 
@@ -638,6 +658,10 @@ int check_rows(int64_t rows, int64_t stride, int vocab, int dtype, float tempera
   SSM_REQUIRE(temperature >= 1e-37f && temperature <= 3e38f, SSM_ERR_SHAPE, "temperature must be positive and finite, and so its inverse");
   return SSM_OK;
 }
+void set_temperature(StatsArgs& s, float t) {
+  s.inv_t = 1.f / t, s.c = kLog2e / t;
+  s.low = std::max(-1e30f, -3.3e38f / s.c);
+}
 int fill(const ssm_token_logp_args& a, StatsArgs& s) {
   if (const int rc = check_rows(a.rows, a.row_stride, a.vocab, a.io_dtype, a.temperature)) return rc;
   SSM_REQUIRE(a.top_k >= 0 && a.top_k <= a.vocab, SSM_ERR_SHAPE, "token_log_probs: top_k must lie between 0 and the vocabulary's size");
@@ -645,7 +669,7 @@ int fill(const ssm_token_logp_args& a, StatsArgs& s) {
   SSM_REQUIRE(a.rows == 0 || (a.logits && a.targets), SSM_ERR_NULL, "token_log_probs: NULL pointer");
   SSM_REQUIRE(aligned_to(a.logits, dtype_size(a.io_dtype)) && aligned_to(a.stats, 16), SSM_ERR_ALIGN, "token_log_probs: misaligned pointer");
   s.rows = a.rows, s.row_stride = a.row_stride, s.ignore = a.ignore_index, s.vocab = a.vocab, s.top_k = a.top_k;
-  s.inv_t = 1.f / a.temperature, s.c = kLog2e / a.temperature;
+  set_temperature(s, a.temperature);
   s.logits = a.logits, s.targets = a.targets, s.logp = a.logp, s.entropy = a.entropy, s.top_logp = a.top_logp, s.top_ids = a.top_ids;
   s.stats = reinterpret_cast<float4*>(a.stats);
   return SSM_OK;
@@ -658,7 +682,7 @@ int fill(const ssm_topk_distill_args& a, StatsArgs& s) {
   SSM_REQUIRE(a.rows == 0 || (a.logits && a.teacher && a.ids), SSM_ERR_NULL, "topk_distill_loss: NULL pointer");
   SSM_REQUIRE(aligned_to(a.logits, dtype_size(a.io_dtype)) && aligned_to(a.stats, 16), SSM_ERR_ALIGN, "topk_distill_loss: misaligned pointer");
   s.rows = a.rows, s.row_stride = a.row_stride, s.vocab = a.vocab, s.top_k = a.top_k, s.teacher_dtype = a.teacher_dtype;
-  s.inv_t = 1.f / a.temperature, s.c = kLog2e / a.temperature;
+  set_temperature(s, a.temperature);
   s.logits = a.logits, s.teacher = a.teacher, s.ids = a.ids, s.logp = a.loss, s.stats = reinterpret_cast<float4*>(a.stats);
   return SSM_OK;
 }
