@@ -161,7 +161,8 @@ int ssm_token_logp_bwd(const ssm_token_logp_bwd_args* args, ssm_stream_t stream)
 
 /* ---------------------------------------------------------------------------------------
  * Distillation from a teacher's top logits: t = softmax(teacher / temperature) over a row's top_k entries (those with a negative id
- * left out), loss[r] = sum_j t_j (log t_j - log softmax(logits / temperature)[ids_j]).  An id of vocab or above makes a row's loss NaN.
+ * left out), loss[r] = sum_j t_j (log t_j - log softmax(logits / temperature)[ids_j]).  An id of vocab or above whose t_j is not 0 makes a row's loss
+ * and gradient NaN; with a teacher logit of -inf, or one so low that t_j is 0, it counts for nothing.
  * A row without entries, or with entries of -inf alone, has loss 0 and no gradient; a student row of -inf alone has loss inf and no gradient.
  * teacher, ids: (rows, top_k) dense.  top_k <= 1024.  Backward: dlogits (rows, vocab) dense from dloss; an id given twice counts twice.
  * ------------------------------------------------------------------------------------- */

@@ -529,14 +529,13 @@ __device__ __forceinline__ void row_grad(const GradArgs& g, const float4 st, int
     }
     any = __syncthreads_or(tid < 32 && any);
     on_p = any ? dl * a.inv_t : 0.f;
+    bool bad = false;  // an id outside of the vocabulary that has a weight made the loss NaN
     for (int j = tid; j < n; j += kThreads) {
       const int64_t id = a.ids[r * n + j];
+      bad = bad || (id >= a.vocab && coef[j] != 0.f);
       coef[j] = -coef[j] * dl * a.inv_t;
       col[j] = id < 0 || id >= a.vocab ? -1 : (int)id;
     }
-    // an id outside of the vocabulary made the loss NaN
-    bool bad = false;
-    for (int j = tid; j < n; j += kThreads) bad = bad || a.ids[r * n + j] >= a.vocab;
     if (__syncthreads_or(bad)) on_p = __uint_as_float(0x7fc00000u);
   } else {
     const int k = g.dtop ? a.top_k : 0;

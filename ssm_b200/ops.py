@@ -851,7 +851,7 @@ def topk_distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tenso
     twice counts twice); no gradient flows to the teacher, whose logits must not require one.
 
     A row without entries (or with entries of ``-inf`` alone) gives 0 and no gradient, a student row of ``-inf`` alone ``inf`` and no gradient,
-    an id of ``V`` or above NaN."""
+    an id of ``V`` or above NaN, loss and gradient, unless its weight ``t_j`` is 0 (a teacher logit of ``-inf``, or next to that)."""
     return _run("topk_distill_loss", logits, teacher_logits, teacher_ids, float(temperature))
 
 

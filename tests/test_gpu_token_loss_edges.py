@@ -1,0 +1,32 @@
+"""Token losses at the border of what their documents say: ids outside the vocabulary that carry no weight, rows of NaN, rows without a teacher."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_id_outside_the_vocabulary_counts_by_its_weight_in_both_directions(dtype):
+    """Lists padded with an id of V and a logit of -inf, or with one whose weight is nothing: as if left out; with any weight NaN, loss and gradient."""
+    from ssm_b200 import ops
+
+    vocab = 700
+    x = torch.randn(6, vocab, generator=torch.Generator().manual_seed(0)).to(dtype).cuda().requires_grad_(True)
+    ids = torch.tensor([[4, 5, vocab], [4, 5, vocab + 9], [vocab, vocab, vocab], [4, 5, -1], [4, 5, vocab], [vocab, -1, 4]]).cuda()
+    teacher = torch.tensor([[0.0, 1.0, -INF], [0.0, 1.0, -30000.0], [-INF, -INF, -INF], [0.0, 1.0, 7.0], [0.0, 1.0, 0.5], [-INF, 3.0, -INF]]).to(dtype).cuda()
+    loss = ops.topk_distill_loss(x, teacher, ids)
+    d, = torch.autograd.grad(loss.sum(), x)
+    left = ids.masked_fill(ids >= vocab, -1)
+    left[4, 2] = 6
+    want = ops.topk_distill_loss(x, teacher, left)
+    ref, = torch.autograd.grad(want.sum(), x)
+    for row in (0, 1, 2, 3, 5):
+        assert torch.equal(loss[row], want[row]) and torch.equal(d[row], ref[row]), row
+    assert torch.isnan(loss[4]) and torch.isnan(d[4]).all()
+    assert loss[2] == 0 and not d[2].any() and loss[5] == 0 and not d[5].any()
