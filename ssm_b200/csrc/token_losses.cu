@@ -516,7 +516,7 @@ __device__ __forceinline__ void row_grad(const GradArgs& g, const float4 st, int
   T* out = reinterpret_cast<T*>(g.out) + r * (int64_t)a.vocab;
   const int per = ((a.vocab + g.splits - 1) / g.splits + 63) / 64 * 64;
   const int lo = min(a.vocab, part_of * per), hi = part_of == g.splits - 1 ? a.vocab : min(a.vocab, lo + per);
-  const bool none = st.w == 1.f;
+  bool none = st.w == 1.f;
   const float dl = g.dlogp ? g.dlogp[r] : 0.f, dh = !DISTILL && g.dentropy ? g.dentropy[r] : 0.f;
   int n;
   float on_p;  // gradient = p (on_p + on_plogp log2 p) + entries
@@ -527,8 +527,8 @@ __device__ __forceinline__ void row_grad(const GradArgs& g, const float4 st, int
       float top, lns;
       teacher_softmax(a, r, tid, coef, top, lns, any);
     }
-    any = __syncthreads_or(tid < 32 && any);
-    on_p = any ? dl * a.inv_t : 0.f;
+    none = !__syncthreads_or(tid < 32 && any) || none;  // nothing asked of the row, whatever its logits are
+    on_p = dl * a.inv_t;
     bool bad = false;  // an id outside of the vocabulary that has a weight made the loss NaN
     for (int j = tid; j < n; j += kThreads) {
       const int64_t id = a.ids[r * n + j];

@@ -30,3 +30,17 @@ def test_an_id_outside_the_vocabulary_counts_by_its_weight_in_both_directions(dt
         assert torch.equal(loss[row], want[row]) and torch.equal(d[row], ref[row]), row
     assert torch.isnan(loss[4]) and torch.isnan(d[4]).all()
     assert loss[2] == 0 and not d[2].any() and loss[5] == 0 and not d[5].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_without_a_teacher_have_no_gradient_whatever_the_student_says(dtype):
+    from ssm_b200 import ops
+
+    x = torch.randn(3, 500, generator=torch.Generator().manual_seed(0)).to(dtype)
+    x[0, 7], x[1, 8] = NAN, INF
+    x = x.cuda().requires_grad_(True)
+    ids = torch.tensor([[-1, -1], [3, 4], [3, 4]]).cuda()
+    teacher = torch.tensor([[1.0, 2.0], [-INF, -INF], [0.0, 1.0]]).cuda()
+    loss = ops.topk_distill_loss(x, teacher, ids)
+    d, = torch.autograd.grad(loss.sum(), x)
+    assert loss[0] == 0 and loss[1] == 0 and not d[:2].any() and torch.isfinite(d[2]).all() and d[2].any()
