@@ -353,12 +353,12 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(const StatsArgs a, 
         if (above < k) best[above] = own;
       }
     } else {  // a few threads hold most of the largest: one maximum at a time
-      uint64_t last = ~0ull;
+      uint64_t last = 0;
       for (int j = 0; j < k; ++j) {
         uint64_t top = 0;
         auto look = [&](float x, int id) {
           const uint64_t key = key_of(x, id);
-          if (key < last && key > top) top = key;
+          if ((j == 0 || key < last) && key > top) top = key;  // NaN in the first column has the largest of keys
         };
         walk<T, 1>(row, lo, hi, tid, kThreads, look, [&](const auto& r, const int* ids) {
           constexpr int V = Vec16<T>::N;

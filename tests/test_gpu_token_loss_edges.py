@@ -44,3 +44,23 @@ def test_rows_without_a_teacher_have_no_gradient_whatever_the_student_says(dtype
     loss = ops.topk_distill_loss(x, teacher, ids)
     d, = torch.autograd.grad(loss.sum(), x)
     assert loss[0] == 0 and loss[1] == 0 and not d[:2].any() and torch.isfinite(d[2]).all() and d[2].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(1, 5000), (3, 40000), (400, 3000)])
+def test_alternatives_of_rows_of_nan_start_at_the_first(rows, vocab, dtype):
+    """More values of NaN than are kept as candidates, the first column among them; and one at the first column before thousands of ties."""
+    from ssm_b200 import ops
+
+    x = torch.zeros(rows, vocab)
+    x[0] = NAN
+    if rows > 1:
+        x[1, ::2] = NAN
+        x[2, 0] = NAN
+        x[2, 1:2500] = torch.arange(2499).remainder(3).float()
+    k = 20
+    ids = ops.token_log_probs(x.to(dtype).cuda(), torch.zeros(rows, dtype=torch.long).cuda(), top_k=k)[2].cpu()
+    assert torch.equal(ids[0], torch.arange(k))
+    if rows > 1:
+        assert torch.equal(ids[1], 2 * torch.arange(k))
+        assert torch.equal(ids[2], torch.cat([torch.tensor([0]), torch.arange(k - 1) * 3 + 3]))
