@@ -134,7 +134,10 @@ __device__ __forceinline__ TokenPair token_pair(const Args& a, const Span& s, in
 __device__ __forceinline__ void decay_logs(const TokenPair& p, float* c, float* beta, int lane) {
   float x[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) x[i] = fmaxf(p.g[i] * kLog2e, kReset), beta[2 * lane + i] = p.beta[i];
+  for (int i = 0; i < 2; ++i) {
+    x[i] = p.g[i] * kLog2e, beta[2 * lane + i] = p.beta[i];
+    if (x[i] < kReset) x[i] = kReset;  // NaN stays
+  }
   float sum = x[0] + x[1];
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {

@@ -1,0 +1,41 @@
+"""Values that are not finite in the gated delta rule: they reach what depends on them, in every kernel that a call can take, and nothing before."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_gpu_gated_delta import BF16, F16, F32, inputs, on_gpu
+
+pytestmark = pytest.mark.gpu
+
+NAN = float("nan")
+
+
+@pytest.mark.parametrize("dtype,kd,vd", [(F32, 64, 48), (BF16, 128, 128), (F16, 64, 64)])
+@pytest.mark.parametrize("at", [0, 70, 149])
+def test_a_decay_that_is_not_a_number_shows(dtype, kd, vd, at):
+    """In one head, at one token: that head's answers from there on and its state, the gradients; the other head and tokens as before."""
+    from ssm_b200 import ops
+
+    ts = inputs(1, 150, 1, 2, kd, vd, dtype)
+
+    def call(spoil):
+        leaves = on_gpu(ts, dtype)
+        if spoil:
+            leaves[3][0, at, 1] = NAN
+        with torch.no_grad():
+            first = ops.gated_delta_scan(*leaves, return_final_state=True, keep_state_fp32=True)
+        leaves = [t.requires_grad_(True) for t in leaves]
+        again = ops.gated_delta_scan(*leaves, return_final_state=True, keep_state_fp32=True)
+        return [*first, *again], torch.autograd.grad(again[0].float().sum(), leaves)
+
+    (clean, grads), (spoilt, bad) = call(False), call(True)
+    for i in (0, 2):
+        assert torch.equal(clean[i][:, :, 0], spoilt[i][:, :, 0])
+        assert torch.isnan(spoilt[i][:, at:, 1]).all()
+        whole = at // 64 * 64
+        assert torch.equal(clean[i][:, :whole, 1], spoilt[i][:, :whole, 1])
+    for i in (1, 3):
+        assert torch.equal(clean[i][:, 0], spoilt[i][:, 0]) and torch.isnan(spoilt[i][:, 1]).all()
+    assert torch.isnan(bad[3][:, at, 1]).all() and torch.equal(bad[3][:, :, 0], grads[3][:, :, 0])
