@@ -215,12 +215,34 @@ struct PairMaps {
   CUtensorMap q, k;
 };
 
+// Decays and strengths of a chunk's tokens, by one warp, here (c, beta, gam, beta suf, scale gam: 64 each) and for the kernels behind, there NaN from token
+// `gone` on
+__device__ __forceinline__ void leave_decays(const Args& a, const Chunks& out, int64_t at, const TokenPair& p, float* c, int gone, int lane) {
+  float *beta = c + C, *gam = beta + C, *bsuf = gam + C, *sgam = bsuf + C, *v = out.vec + at * (4 * C);
+  decay_logs(p, c, beta, lane);
+  __syncwarp();
+  for (int i = lane; i < C; i += 32) {
+    const float x = ex2_approx(c[i]), y = beta[i] * ex2_approx(c[C - 1] - c[i]), none = i >= gone ? __uint_as_float(0x7fc00000u) : 0.f;
+    gam[i] = x, bsuf[i] = y, sgam[i] = x * a.scale;
+    v[i] = x + none, v[C + i] = beta[i] + none, v[2 * C + i] = y + none, v[3 * C + i] = x * a.scale + none;
+  }
+}
+// A chunk without the tokens from `lost` on; not inline, and its products once more beside the first ones rather than in a loop: both would cost registers
+template <int KD>
+__device__ __noinline__ void cut_chunk(const Args& a, const Chunks& out, unsigned char* tK, float* c, int lost) {
+  const Span s = chunk_of(a.where, blockIdx.x, C);
+  constexpr int U = KD / 8;
+  for (int i = threadIdx.x; i < (C - lost) * U; i += kPairThreads) *reinterpret_cast<uint4*>(tK + (i % U >> 3) * kTileBytes + swz(lost + i / U, i % U & 7)) = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x < 32) leave_decays(a, out, (int64_t)s.chunk * a.heads + blockIdx.y, token_pair(a, s, min(s.t1 - s.t0, lost), blockIdx.y, threadIdx.x), c, lost, threadIdx.x);
+}
+
 template <typename T, int KD, bool TRAIN>
-__global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, const Chunks out, const __grid_constant__ PairMaps maps) {
+__global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const __grid_constant__ Args a, const __grid_constant__ Chunks out, const __grid_constant__ PairMaps maps) {
   using M = PairSmem<KD>;
   extern __shared__ unsigned char smdyn[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t mbar;
+  __shared__ int lost;  // the first token whose key, decay or strength is not finite
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const Span s = chunk_of(a.where, blockIdx.x, C);
   const int n = s.t1 - s.t0, h = blockIdx.y, kh = h / a.group;
@@ -239,14 +261,11 @@ __global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, co
     }
   }
   if (warp == 0) {  // beside the copies
-    decay_logs(token_pair(a, s, n, h, lane), c, beta, lane);
-    __syncwarp();
-    float* v = out.vec + at * (4 * C);
-    for (int i = lane; i < C; i += 32) {
-      const float x = ex2_approx(c[i]), y = beta[i] * ex2_approx(c[C - 1] - c[i]);
-      gam[i] = x, bsuf[i] = y, sgam[i] = x * a.scale;
-      v[i] = x, v[C + i] = beta[i], v[2 * C + i] = y, v[3 * C + i] = x * a.scale;
-    }
+    const TokenPair p = token_pair(a, s, n, h, lane);
+    leave_decays(a, out, at, p, c, C, lane);
+    const uint32_t even = __ballot_sync(0xffffffffu, !(p.g[0] * kLog2e < INFINITY && fabsf(p.beta[0]) < INFINITY)),
+                   odd = __ballot_sync(0xffffffffu, !(p.g[1] * kLog2e < INFINITY && fabsf(p.beta[1]) < INFINITY));
+    if (lane == 0) lost = min(even ? 2 * __ffs(even) - 2 : C, odd ? 2 * __ffs(odd) - 1 : C);
   }
   __syncthreads();
   if (!__syncthreads_and(tc::mbar_wait(landed, 0))) {
@@ -265,7 +284,20 @@ __global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, co
   float kk[8][4], qk[8][4];
   uint32_t fq[KD / 16][4];
   rows_products<T, KD>(kk, qk, fq, bK, tc::smem_u32(tQ), r0, lane);
-  __syncthreads();  // the rows of q have been read
+  // What is not finite would meet the zeros of the triangles below, and so reach tokens before it.  From the first such token on the chunk is formed
+  // without keys, strengths and decays; those rows of X and Y and the decay of the whole chunk are NaN when they leave.  A key shows in its product with itself
+  int own = C;
+#pragma unroll
+  for (int nb = 7; nb >= 0; --nb)
+    if (nb >> 1 == warp && (gi & ~1) == gj && !(fabsf(gi & 1 ? kk[nb][2 * (nb & 1) + 1] : kk[nb][2 * (nb & 1)]) < INFINITY)) own = r0 + gi + (nb & 1) * 8;
+  if (__syncthreads_or(own < C || lost < C)) {  // and the rows of q have been read
+    if (own < C) atomicMin(&lost, own);
+    __syncthreads();
+    cut_chunk<KD>(a, out, tK, c, lost);
+    __syncthreads();
+    rows_products<T, KD>(kk, qk, fq, bK, tc::smem_u32(tQ), r0, lane);
+    __syncthreads();
+  }
   {
     const float ci[2] = {c[r0 + gi], c[r0 + gi + 8]};
 #pragma unroll
@@ -421,6 +453,8 @@ __global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const Args a, co
     times(d, fp, tc::smem_u32(tW) + half * kTileBytes, 0, warp);
     put(tK + half * kTileBytes, d);
   }
+  for (int i = lost * 8 + tid; i < C * 8; i += kPairThreads)  // NaN in either type
+    *reinterpret_cast<uint4*>(tX + swz(i / 8, i % 8)) = *reinterpret_cast<uint4*>(tP + swz(i / 8, i % 8)) = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
   tc::fence_async_smem();
   __syncthreads();
   if (tid == 0) {

@@ -9,7 +9,7 @@ from tests.test_gpu_gated_delta import BF16, F16, F32, inputs, on_gpu
 
 pytestmark = pytest.mark.gpu
 
-NAN = float("nan")
+INF, NAN = float("inf"), float("nan")
 
 
 @pytest.mark.parametrize("dtype,kd,vd", [(F32, 64, 48), (BF16, 128, 128), (F16, 64, 64)])
@@ -39,3 +39,39 @@ def test_a_decay_that_is_not_a_number_shows(dtype, kd, vd, at):
     for i in (1, 3):
         assert torch.equal(clean[i][:, 0], spoilt[i][:, 0]) and torch.isnan(spoilt[i][:, 1]).all()
     assert torch.isnan(bad[3][:, at, 1]).all() and torch.equal(bad[3][:, :, 0], grads[3][:, :, 0])
+
+
+def _spoil(leaves, name, value, at, head=1):
+    q, k, v, g, beta = leaves
+    if name in "qk":
+        (q if name == "q" else k)[0, at, head, 5] = value
+    else:
+        (g if name == "g" else beta)[0, at, head] = value
+
+
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("dtype,kd,vd", [(F32, 64, 48), (BF16, 128, 128), (BF16, 64, 192), (F16, 128, 64), (F16, 72, 40)])
+@pytest.mark.parametrize("name,value", [("q", NAN), ("k", NAN), ("k", -INF), ("g", NAN), ("beta", NAN), ("beta", INF)])
+def test_nothing_before_a_value_that_is_not_finite_changes(name, value, dtype, kd, vd, train):
+    """Tokens before it give the same bits, its own head gives nothing finite behind it."""
+    from ssm_b200 import ops
+
+    nl = 200
+    ts = inputs(1, nl, 2, 2, kd, vd, dtype, seed=3)
+
+    def call(at):
+        leaves = on_gpu(ts, dtype)
+        if at is not None:
+            _spoil(leaves, name, value, at)
+        leaves = [t.requires_grad_(train) for t in leaves]
+        return [t.detach() for t in ops.gated_delta_scan(*leaves, return_final_state=True, keep_state_fp32=True)]
+
+    o, s = call(None)
+    for at in (0, 15, 17, 63, 64, 100, 199):
+        bo, bs = call(at)
+        assert torch.equal(o[:, :, 0], bo[:, :, 0]) and torch.equal(s[:, 0], bs[:, 0]), at
+        assert torch.equal(o[:, :at, 1], bo[:, :at, 1]), at
+        if name == "q":  # its own answer alone
+            assert not torch.isfinite(bo[:, at, 1]).any() and torch.equal(o[:, at + 1:], bo[:, at + 1:]) and torch.equal(s, bs), at
+        else:
+            assert not torch.isfinite(bo[:, at + 1:, 1]).any() and not torch.isfinite(bs[:, 1]).any(), at
