@@ -46,6 +46,12 @@ struct Chunks {
   int32_t* status;
 };
 
+// not 0 where one of a 16-byte unit's elements is not finite: an exponent of ones carries into the sign
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint4 x) {
+  constexpr uint32_t ones = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u, carry = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
+  return ((((x.x & ones) + carry) | ((x.y & ones) + carry) | ((x.z & ones) + carry) | ((x.w & ones) + carry)) & 0x80008000u);
+}
 __device__ __forceinline__ uint32_t swz(int row, int unit) { return (uint32_t)(row * 128 + ((unit ^ (row & 7)) << 4)); }  // 16-byte unit of a row
 
 template <typename T>
@@ -507,7 +513,7 @@ struct ChunkWalk {
 };
 
 // Warps 0-7 hold the rows of the state (a lane a row, two warps share the columns of 32 rows; with four of them 2240 cycles a chunk instead of 1940), 8-11
-// prepare operands and store what leaves, 12 copies, 13 issues the products.  Launched with 128 registers a thread (512 x 128 = 65536), of which
+// prepare operands and store what leaves, 12 copies, 13 issues the products, 14 and 15 look at v (forward).  Launched with 128 registers a thread (512 x 128 = 65536), of which
 // the groups of four warps keep 168, 168, 104 and 40.
 constexpr int kParts = 2, kCompute = 128 * kParts, kHelp = 128, kWalkThreads = kCompute + kHelp + 128;
 constexpr int kComputeRegs = 168, kHelpRegs = 104, kIssueRegs = 40;
@@ -531,8 +537,8 @@ struct Cols {
 };
 
 // A wait by parity must not fall two completions behind: each barrier's next completion but one needs what its waiter does after this one (two of
-// kPrep for that)
-enum Bar { kFullE = 0, kFreeE = 2, kFullL = 4, kFreeL = 7, kPrep = 10, kState = 12, kR, kU, kDS, kO, kOut, kEnd, kBars };
+// kPrep and kSeen for that)
+enum Bar { kFullE = 0, kFreeE = 2, kFullL = 4, kFreeL = 7, kPrep = 10, kSeen = 12, kFullV = 14, kState = 16, kR, kU, kDS, kO, kOut, kEnd, kBars };
 
 // a load from tensor memory that is under way until `landed`
 __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -569,6 +575,12 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smdyn) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t mbar[kBars];
   __shared__ uint32_t tmem_slot;
+  // Forward: what is not finite in v would meet the zeros of X and Y, and so reach tokens before it.  Two warps look at a chunk's v while the first products
+  // run.  Where they find something they put zeros in its place, the products are issued once more before they count, and answers, rest and state of
+  // such a column are NaN from its first such token on: `lost`, of halves of 64 columns that have any.  A chunk's place is used again four chunks later: its v
+  // is there only when the rows and the answers of the one three before it have been read.  v has a barrier of its own, as it lands before the rest.
+  // 1 x 16384 x 32 heads: 498 us, 493 without a look; 658 when v landed with the rest, 569 when the products waited for it, 568 with a look in pairs_kernel.
+  __shared__ int lost[BACK ? 1 : 4][BACK ? 1 : 128], any_lost[BACK ? 1 : 4][2];
   const Args& a = w.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int h = blockIdx.y, kh = h / a.group, v0 = blockIdx.x * 128;
@@ -587,8 +599,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
   if (warp == 0) tc::tmem_alloc(tc::smem_u32(&tmem_slot), 512);
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const bool rows = i == kState || i == kU, help = i == kPrep || i == kPrep + 1 || i == kOut;
-      tc::mbar_init(bar(i), i >= kFreeL && i < kFreeL + M::NL ? 1 + (kCompute + kHelp) / 32 : rows ? kCompute / 32 : help ? kHelp / 32 : 1);
+      const bool rows = i == kState || i == kU, help = i == kPrep || i == kPrep + 1 || i == kOut, seen = i == kSeen || i == kSeen + 1;
+      tc::mbar_init(bar(i), i >= kFreeL && i < kFreeL + M::NL ? 1 + (kCompute + kHelp) / 32 : rows ? kCompute / 32 : help ? kHelp / 32 : seen ? 2 : 1);
     }
   }
   tc::fence_before_sync();
@@ -627,9 +639,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       const unsigned char* wide = BACK ? w.in.wb : w.in.wz;
       auto early = [&](int p) {
         if (lane == 0) {
-          const uint32_t full = bar(kFullE + p % M::NE), d = tc::smem_u32(sm + p % M::NE * M::EARLY);
-          tc::mbar_expect_tx(full, M::EARLY);
-          for (int b = 0; b < 2; ++b) tc::tma_load_4d(d + M::V + b * kTileBytes, &maps.v, full, v0 + b * 64, h, s.t0 + chunk_at(p) * C, s.b);
+          const uint32_t full = bar(kFullE + p % M::NE), full_v = BACK ? full : bar(kFullV + p % M::NE), d = tc::smem_u32(sm + p % M::NE * M::EARLY);
+          if constexpr (!BACK) tc::mbar_expect_tx(full_v, M::VB);
+          tc::mbar_expect_tx(full, BACK ? M::EARLY : M::EARLY - M::VB);
+          for (int b = 0; b < 2; ++b) tc::tma_load_4d(d + M::V + b * kTileBytes, &maps.v, full_v, v0 + b * 64, h, s.t0 + chunk_at(p) * C, s.b);
           if constexpr (!BACK) tc::bulk_load(d + M::X, w.in.x + pair_at(p) * kTileBytes, kTileBytes, full);
           tc::bulk_load(d + M::X + M::XB - kTileBytes, w.in.y + pair_at(p) * kTileBytes, kTileBytes, full);
           tc::bulk_load(d + M::W, wide + pair_at(p) * M::WB, M::WB, full);
@@ -665,7 +678,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
         if (ok && nl < nchunks && (ok = wait(kFreeL + p % M::NL, p / M::NL))) late(nl++);
       }
       // nothing is under way when the block ends
-      for (int p = max(0, ne - M::NE); p < ne; ++p) ok = wait(kFullE + p % M::NE, p / M::NE) && ok;
+      for (int p = max(0, ne - M::NE); p < ne; ++p) ok = wait(kFullE + p % M::NE, p / M::NE) && (BACK || wait(kFullV + p % M::NE, p / M::NE)) && ok;
       for (int p = max(0, nl - M::NL); p < nl; ++p) ok = wait(kFullL + p % M::NL, p / M::NL) && ok;
     } else if (warp == (kCompute + kHelp) / 32 + 1) {  // ---- products
       constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
@@ -676,7 +689,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       constexpr uint32_t id_doq = tc::instr_desc(128, KD, fmt, 1, 1);            // do^T Q
       for (int p = 0; p < nchunks; ++p) {
         const int se = p % M::NE, sl = p % M::NL;
-        if (!(ok = wait(kFullE + se, p / M::NE) && wait(kFullL + sl, p / M::NL) && wait(kPrep + (p & 1), p >> 1))) break;  // rows of another sequence cut; BACK: q scaled
+        if (!(ok = wait(kFullE + se, p / M::NE) && (BACK || wait(kFullV + se, p / M::NE)) && wait(kFullL + sl, p / M::NL) && wait(kPrep + (p & 1), p >> 1))) break;  // rows of another sequence cut; BACK: q scaled
         tc::fence_after_sync();
         const uint32_t e = tc::smem_u32(sm + se * M::EARLY), l = tc::smem_u32(sm + M::NE * M::EARLY + sl * M::LATE), R = tmem + TC::RO + (p & 1) * 128;
         const uint64_t w_rows = tc::smem_desc_sw128(e + M::W, 16, 1024), v_cols = tc::smem_desc_sw128(e + M::V, kTileBytes, 1024);
@@ -684,20 +697,34 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
         const uint64_t k_cols = tc::smem_desc_sw128(l + M::K, kTileBytes, 1024), q_cols = tc::smem_desc_sw128(l + M::Q, kTileBytes, 1024);
         auto along = [](int kk) { return (uint64_t)(((kk >> 2) * (N1 * 128) + (kk & 3) * 32) >> 4); };  // 16 columns further in a tile of N1 rows
         auto down = [](int kk) { return (uint64_t)(kk * (2048 >> 4)); };                                // 16 rows further
-        if (tc::elect_one()) {
+        auto first = [&] {
 #pragma unroll
           for (int kk = 0; kk < C / 16; ++kk) tc::mma_ss(R, v_cols + down(kk), BACK ? y_cols + down(kk) : x_rows + along(kk), id_v, kk > 0);
-        }
+        };
+        auto second = [&] {
+#pragma unroll
+          for (int kk = 0; kk < KD / 16; ++kk) tc::mma_ts(R, tmem + TC::S + kk * 8, w_rows + along(kk), id_s, true);
+        };
+        if (tc::elect_one()) first();
         __syncwarp();
         if (BACK && p > 0 && !(ok = wait(kOut, p - 1))) break;  // the results before these have been read: kR is not two ahead of the helping warps
         if (!(ok = wait(kState, p))) break;
         tc::fence_after_sync();
         if (tc::elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < KD / 16; ++kk) tc::mma_ts(R, tmem + TC::S + kk * 8, w_rows + along(kk), id_s, true);
-          tc::commit(bar(kR));
+          second();
+          if constexpr (BACK) tc::commit(bar(kR));
         }
         __syncwarp();
+        if constexpr (!BACK) {
+          if (!(ok = wait(kSeen + (p & 1), p >> 1))) break;
+          const bool again = any_lost[p & 3][0] + any_lost[p & 3][1] != 0;
+          tc::fence_after_sync();
+          if (tc::elect_one()) {
+            if (again) first(), second();
+            tc::commit(bar(kR));
+          }
+          __syncwarp();
+        }
         // beside the rows' step
         if (!BACK && p > 0 && !(ok = wait(kOut, p - 1))) break;
         tc::fence_after_sync();
@@ -726,6 +753,33 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       if (tc::elect_one()) tc::commit(bar(kEnd));  // nothing is under way when the block ends, nor where a wait ran out
       __syncwarp();
       ok = wait(kEnd, 0) && ok;
+    } else if (!BACK) {  // ---- a look at 64 columns of v
+      const int half = warp & 1;
+      for (int p = 0; p < nchunks && (ok = wait(kFullV + p % M::NE, p / M::NE)); ++p) {
+        int* mine = &lost[BACK ? 0 : p & 3][BACK ? 0 : half * 64];
+        mine[lane] = mine[lane + 32] = C;
+        __syncwarp();
+        const int n = min(C, s.t1 - (s.t0 + p * C));  // what lies behind belongs to the next sequence
+        unsigned char* tile = sm + p % M::NE * M::EARLY + M::V + half * kTileBytes;
+        uint32_t hits = 0;
+#pragma unroll 4
+        for (int i = 0; i < C / 4; ++i) {
+          const int r = lane / 8 + i * 4;
+          const uint32_t hit = not_finite<T>(*reinterpret_cast<const uint4*>(tile + swz(r, lane & 7)));
+          hits |= r < n ? hit : 0u;
+        }
+        const bool found = __any_sync(0xffffffffu, hits != 0);
+        if (found) {
+          for (int i = lane; i < n * 64; i += 32) {
+            constexpr uint16_t ones = std::is_same<T, __nv_bfloat16>::value ? 0x7f80 : 0x7c00;
+            uint16_t* x = reinterpret_cast<uint16_t*>(tile + swz(i / 64, i % 64 / 8)) + i % 8;
+            if ((*x & ones) == ones) *x = 0, atomicMin(&mine[i % 64], i / 64);
+          }
+          tc::fence_async_smem();
+        }
+        if (lane == 0) any_lost[BACK ? 0 : p & 3][half] = found;
+        done(kSeen + (p & 1));
+      }
     }
   } else if (warp >= kCompute / 32) {  // ---- operands prepared, results stored
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kHelpRegs));
@@ -736,7 +790,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
     auto prepare = [&](int p) {
       const int n = tokens_of(p);
       const bool cut = packed && n < C;
-      if (!wait(kFullL + p % M::NL, p / M::NL) || (cut && !wait(kFullE + p % M::NE, p / M::NE))) return false;
+      if (!wait(kFullL + p % M::NL, p / M::NL) || (cut && !wait((BACK ? kFullE : kFullV) + p % M::NE, p / M::NE))) return false;
       unsigned char *d = late_at(p), *e = sm + p % M::NE * M::EARLY;
       constexpr int U = KD / 8;
       if constexpr (BACK) {
@@ -780,6 +834,14 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       for (int q = 0; q < 2; ++q) ld32(tmem + lanes + TC::RO + (p & 1) * 128 + (BACK ? 0 : C) + q * 32, x[q]);
       landed(x[0]), landed(x[1]);
       done(kOut);
+      if (!BACK && any_lost[BACK ? 0 : p & 3][row >> 6]) {
+        const int from = lost[BACK ? 0 : p & 3][BACK ? 0 : row];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (q * 32 + e >= from) x[q][e] = 0x7fc00000u;
+      }
       if (me == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");  // the tile of the chunk before the last has left
       together(true);
 #pragma unroll
@@ -855,6 +917,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       uint32_t x[NT];
       if (!(ok = wait(kR, p))) break;
       tc::fence_after_sync();
+      const bool spoilt = !BACK && any_lost[BACK ? 0 : p & 3][row >> 6];
       ld32(tmem + lanes + TC::RO + (p & 1) * 128 + part * NT, x);
       landed(x);
       {
@@ -870,6 +933,12 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
           if (w.states && live) keep_units(p, NS / 16, NS / 8);
         if constexpr (!BACK)
           if (w.rest && live) {
+            if (spoilt) {
+              const int from = lost[p & 3][row] - part * NT;
+#pragma unroll
+              for (int e = 0; e < NT; ++e)
+                if (e >= from) x[e] = 0x7fc00000u;
+            }
 #pragma unroll
             for (int e = 0; e < NT / 2; ++e) y[e] = pack2<T>(f(x[2 * e]), f(x[2 * e + 1]));
             uint4* to = reinterpret_cast<uint4*>(w.rest) + ((int64_t)(s.chunk + chunk_at(p)) * a.heads + h) * (C / 8) * a.vd + unit_at(C / 8, part * (NT / 8));
@@ -887,6 +956,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
         landed(z[q]);
 #pragma unroll
         for (int e = 0; e < 32; ++e) S[q * 32 + e] = fmaf(whole, S[q * 32 + e], f(z[q][e]));
+      }
+      if (spoilt && lost[BACK ? 0 : p & 3][BACK ? 0 : row] < C) {
+#pragma unroll
+        for (int e = 0; e < NS; ++e) S[e] = f(0x7fc00000u);
       }
       if (p + 1 < nchunks) publish(p + 1);
       __syncwarp();

@@ -804,6 +804,10 @@ def gated_delta_scan(
     0 to at most ``L``; rows behind the last sequence give zeros, and no gradient.  On the host it is checked; on the device it is
     used where it lies without a synchronisation, entries that break the rule being clamped.
 
+    A value that is not finite reaches the answers and states that depend on it and no token before it (what lies behind the sequences of a padded batch
+    does no harm); in chunks of 16-bit operands they are NaN where the recurrence may still say infinity, and a key whose square is beyond 32 bits
+    counts as such a value.  The gradients of its sequence and head are not defined then.
+
     Everything is differentiable but ``cu_seqlens``; gradients are recorded once (no second derivative).
     """
     return _run("gated_delta_scan", q, k, v, g, beta, scale, initial_state, bool(return_final_state), bool(keep_state_fp32),
