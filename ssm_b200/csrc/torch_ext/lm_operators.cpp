@@ -194,6 +194,19 @@ Tensor gated_delta_step(const Tensor& state, const Tensor& q_, const Tensor& k_,
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)kd);
   SSM_ARG(std::isfinite(s), "scale must be finite.");
   SSM_ARG(nb < 65536, "gated_delta_step: too many sequences.");
+  bool wanted = false;  // gradients
+  for (const Tensor* t : {&state, &q_, &k_, &v_, &beta_, g_.has_value() ? &*g_ : &beta_}) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "ssm_b200 operators have no forward-mode derivative");
+    wanted = wanted || (at::GradMode::is_enabled() && t->requires_grad());
+  }
+  if (wanted) {
+    const OptTensor g = g_.has_value() ? OptTensor(g_->unsqueeze(1)) : c10::nullopt;
+    const variable_list r = invoke_call(c10::make_intrusive<DeltaCall>(q_.unsqueeze(1), k_.unsqueeze(1), v_.unsqueeze(1), g, beta_.unsqueeze(1), s, OptTensor(state.clone()), true, true, c10::nullopt));
+    const Tensor o = r[0].select(1, 0);
+    at::NoGradGuard values;
+    state.copy_(r[1]);
+    return o;
+  }
   c10::cuda::CUDAGuard guard(state.device());
   const Tensor q = lead(q_, v_.scalar_type()), k = lead(k_, v_.scalar_type()), v = strided(v_), beta = coefficient(beta_, "gated_delta_step beta");
   const Tensor work = state.is_contiguous() ? state.detach() : state.detach().contiguous();

@@ -818,16 +818,7 @@ def gated_delta_step(state: Tensor, q: Tensor, k: Tensor, v: Tensor, g: Optional
     """Extension: one decode token of the gated delta rule.  ``state (B, H, V, K)`` fp32 is overwritten in place; ``q, k (B, Hk, K)``,
     ``v (B, H, V)``, ``g, beta (B, H)``; returns ``(B, H, V)``.  Where gradients are wanted the token goes through :func:`gated_delta_scan`
     and the state receives the values of the new one."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (state, q, k, v, g, beta)):
-        if state.ndim != 4 or state.dtype != torch.float32:
-            raise ValueError("state must be float32 of shape (B, H, V, K).")
-        if not (q.ndim == k.ndim == v.ndim == 3 and beta.ndim == 2 and (g is None or g.ndim == 2)):
-            raise ValueError("q and k must have shape (B, Hk, K), v (B, H, V), g and beta (B, H).")
-        o, new = gated_delta_scan(q[:, None], k[:, None], v[:, None], None if g is None else g[:, None], beta[:, None], scale, state.clone(), True, True)
-        with torch.no_grad():
-            state.copy_(new)
-        return o[:, 0]
-    return _native().gated_delta_step(state, q, k, v, g, beta, scale)
+    return _run("gated_delta_step", state, q, k, v, g, beta, scale)
 
 
 # =========================================================================================
