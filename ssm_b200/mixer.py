@@ -437,6 +437,11 @@ class GatedDeltaBlock(nn.Module):
         self.out_proj = lin(d_model, d_inner)
         self.register_buffer("unit", torch.full((d_state,), d_state ** -0.5, **f32), persistent=False)
 
+    def _apply(self, fn, recurse=True):  # a cast of the module rounds its parameters, but not this factor; nor does it come with memory that a module is given
+        super()._apply(fn, recurse)
+        self.unit = torch.full_like(self.unit, self.d_state ** -0.5, dtype=torch.float64 if self.unit.dtype == torch.float64 else torch.float32)
+        return self
+
     def _namespace(self):
         if self._ops is not None:
             return self._ops
