@@ -176,7 +176,11 @@ class MambaLMHeadModel(nn.Module):
               ignore_index: int = -100, **mixer_kwargs):
         """Log probabilities of a sequence's own tokens, each given those before it: ``input_ids (B, L)`` -> ``(B, L - 1)`` fp32, with the entropies and
         the ``top_k`` alternatives behind them as in ``ops.token_log_probs``.  ``labels (B, L)`` in the place of the tokens; those equal to
-        ``ignore_index`` give 0."""
+        ``ignore_index`` give 0.  A whole sequence at once: no shard of one, no cache; over all of the head's columns, padded ones too."""
+        if mixer_kwargs.get("sharded"):
+            raise ValueError("score: a shard of a sequence has neither the distribution before its first token nor the token behind its last one")
+        if mixer_kwargs.get("inference_params") is not None or mixer_kwargs.get("num_last_tokens"):
+            raise ValueError("score runs over the whole sequence: inference_params and num_last_tokens are not taken")
         logits = self.forward(input_ids, **mixer_kwargs).logits
         targets = input_ids if labels is None else labels
         # the logits as they lie, their last row with nothing to predict
