@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <cstdio>
+#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/ssm_b200.h"
@@ -80,6 +81,11 @@ inline int sm_count() {
 inline bool valid_dtype(int d) { return d == SSM_F32 || d == SSM_BF16 || d == SSM_F16; }
 inline int dtype_size(int d) { return d == SSM_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+inline bool aligned_to(std::initializer_list<const void*> ps, size_t a) {
+  for (const void* p : ps)
+    if (!aligned_to(p, a)) return false;
+  return true;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

@@ -661,11 +661,21 @@ int check(const ssm_gated_delta_args& a, Args& d) {
   SSM_REQUIRE(a.num_seqs == 0 || (a.cu_seqlens && a.table), SSM_ERR_NULL, "gated_delta: packed sequences need cu_seqlens and table");
   SSM_REQUIRE((int64_t)a.batch * a.len == 0 || (a.q && a.k && a.v && a.beta), SSM_ERR_NULL, "gated_delta: NULL pointer");
   SSM_REQUIRE(a.final_state == nullptr || valid_dtype(a.final_dtype), SSM_ERR_DTYPE, "gated_delta: unknown state dtype");
+  SSM_REQUIRE(aligned_to({a.q, a.k, a.v, a.o}, dtype_size(a.io_dtype)) && aligned_to(a.g, dtype_size(a.g_dtype)) && aligned_to(a.beta, dtype_size(a.beta_dtype)) &&
+                  (a.num_seqs == 0 || aligned_to(a.cu_seqlens, a.cu_is_64 ? 8 : 4)) && aligned_to({a.initial_state, a.table, a.rest, a.states}, 4) &&
+                  (a.final_state == nullptr || aligned_to(a.final_state, dtype_size(a.final_dtype))),
+              SSM_ERR_ALIGN, "gated_delta: misaligned pointer");
   d.q = {a.q, a.q_sb, a.q_st, a.q_sh}, d.k = {a.k, a.k_sb, a.k_st, a.k_sh}, d.v = {a.v, a.v_sb, a.v_st, a.v_sh};
   d.g = {a.g, a.g_sb, a.g_st, a.g_sh}, d.beta = {a.beta, a.beta_sb, a.beta_st, a.beta_sh};
   d.io = a.io_dtype, d.g_dtype = a.g_dtype, d.beta_dtype = a.beta_dtype, d.kd = a.kdim, d.vd = a.vdim, d.heads = a.heads, d.group = a.heads / a.key_heads;
   d.len = a.len, d.seqs = a.num_seqs > 0 ? a.num_seqs : a.batch, d.final_dtype = a.final_dtype, d.scale = a.scale;
   d.where = {a.num_seqs > 0 ? a.table : nullptr, a.len, d.seqs, (a.len + kChunk - 1) / kChunk};
+  return SSM_OK;
+}
+
+int check_gradients(const ssm_gated_delta_bwd_args& g) {
+  SSM_REQUIRE(aligned_to({g.dout, g.dq, g.dk, g.dv}, dtype_size(g.fwd.io_dtype)) && aligned_to({g.dfinal, g.dg, g.dbeta, g.dinitial, g.dv32, g.dstates, g.dqk}, 4), SSM_ERR_ALIGN,
+              "gated_delta backward: misaligned pointer");
   return SSM_OK;
 }
 
@@ -700,6 +710,7 @@ extern "C" int ssm_gated_delta_bwd(const ssm_gated_delta_bwd_args* args, ssm_str
   SSM_REQUIRE(!any || (args->dout && args->dq && args->dk && args->dv && args->dg && args->dbeta && args->dv32 && args->dstates && args->fwd.rest && args->fwd.states),
               SSM_ERR_NULL, "gated_delta backward: NULL pointer");
   SSM_REQUIRE(!any || w.a.group == 1 || args->dqk, SSM_ERR_NULL, "gated_delta backward: shared keys need the dqk scratch");
+  if (const int rc = gd::check_gradients(*args)) return rc;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   w.initial = args->dfinal, w.dout = args->dout, w.last = args->dinitial, w.last_dtype = SSM_F32;
   w.o = args->dv == (void*)args->dv32 ? nullptr : args->dv, w.rest = args->dv32, w.states = args->dstates;
@@ -726,7 +737,8 @@ extern "C" int ssm_gated_delta_step(const ssm_gated_delta_step_args* args, ssm_s
   SSM_REQUIRE(a.batch <= 65535, SSM_ERR_TOO_LARGE, "gated_delta_step: more than 65535 sequences");
   if (a.batch == 0) return SSM_OK;
   SSM_REQUIRE(a.state && a.q && a.k && a.v && a.beta && a.o, SSM_ERR_NULL, "gated_delta_step: NULL pointer");
-  SSM_REQUIRE(aligned_to(a.state, 4), SSM_ERR_ALIGN, "gated_delta_step: misaligned state");
+  SSM_REQUIRE(aligned_to(a.state, 4) && aligned_to({a.q, a.k, a.v, a.o}, dtype_size(a.io_dtype)) && aligned_to(a.g, dtype_size(a.g_dtype)) && aligned_to(a.beta, dtype_size(a.beta_dtype)),
+              SSM_ERR_ALIGN, "gated_delta_step: misaligned pointer");
   gd::StepArgs s{};
   s.q = {a.q, a.q_sb, 0, a.q_sh}, s.k = {a.k, a.k_sb, 0, a.k_sh}, s.v = {a.v, a.v_sb, 0, a.v_sh};
   s.g = {a.g, a.g_sb, 0, a.g_sh}, s.beta = {a.beta, a.beta_sb, 0, a.beta_sh};

@@ -58,6 +58,7 @@ __device__ __forceinline__ float beta_of(const Args& a, int b, int t, int h) {
 }
 
 int check(const ssm_gated_delta_args& a, Args& d);
+int check_gradients(const ssm_gated_delta_bwd_args& g);  // of the backward call's own pointers, their alignment
 // sums the fp32 gradients of a key head's value heads (dq, then dk of all tokens) into dq and dk
 int fold_heads(const float* dqk, void* dq, void* dk, int64_t tokens, int kd, int key_heads, int group, int dtype, cudaStream_t st);
 // forms the table on the device; a no-op without packed sequences

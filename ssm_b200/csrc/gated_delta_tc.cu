@@ -1457,7 +1457,8 @@ extern "C" int ssm_gated_delta_chunked_fwd(const ssm_gated_delta_args* args, voi
   if (const int rc = gd::check(f, w.a)) return rc;
   SSM_REQUIRE(ssm_gated_delta_chunked_supported(args), SSM_ERR_UNSUPPORTED, "gated_delta: these operands do not go to the tensor cores");
   if (w.a.seqs == 0) return SSM_OK;
-  SSM_REQUIRE(f.o && scratch && kept && aligned_to(scratch, 256) && aligned_to(kept, 256), SSM_ERR_NULL, "gated_delta: NULL output or scratch");
+  SSM_REQUIRE(f.o && scratch && kept, SSM_ERR_NULL, "gated_delta: NULL output or scratch");
+  SSM_REQUIRE(aligned_to({scratch, kept}, 256) && aligned_to(status, 4), SSM_ERR_ALIGN, "gated_delta: misaligned scratch");
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   w.a.where.per = (f.len + gd::C - 1) / gd::C;
   const int64_t chunks = gd::chunks_of(f);
@@ -1504,6 +1505,8 @@ extern "C" int ssm_gated_delta_chunked_bwd(const ssm_gated_delta_bwd_args* args,
   SSM_REQUIRE(aligned_to(args->dout, 16) && aligned_to(args->dv, 16) && aligned_to(args->dq, 16) && aligned_to(args->dk, 16) && aligned_to(args->dfinal, 16) && aligned_to(args->dqk, 16) &&
                   aligned_to(kept, 256) && aligned_to(scratch, 256),
               SSM_ERR_ALIGN, "gated_delta backward: misaligned pointer");
+  if (const int rc = gd::check_gradients(*args)) return rc;
+  SSM_REQUIRE(aligned_to(status, 4), SSM_ERR_ALIGN, "gated_delta backward: misaligned pointer");
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   w.a.where.per = (f.len + gd::C - 1) / gd::C;
   const int64_t chunks = gd::chunks_of(f);

@@ -666,7 +666,8 @@ int fill(const ssm_token_logp_args& a, StatsArgs& s) {
   SSM_REQUIRE(a.top_k >= 0 && a.top_k <= a.vocab, SSM_ERR_SHAPE, "token_log_probs: top_k must lie between 0 and the vocabulary's size");
   SSM_REQUIRE(a.top_k <= kMaxTop, SSM_ERR_TOO_LARGE, "token_log_probs: top_k is at most 128");
   SSM_REQUIRE(a.rows == 0 || (a.logits && a.targets), SSM_ERR_NULL, "token_log_probs: NULL pointer");
-  SSM_REQUIRE(aligned_to(a.logits, dtype_size(a.io_dtype)) && aligned_to(a.stats, 16), SSM_ERR_ALIGN, "token_log_probs: misaligned pointer");
+  SSM_REQUIRE(aligned_to(a.logits, dtype_size(a.io_dtype)) && aligned_to(a.stats, 16) && aligned_to({a.targets, a.top_ids}, 8) && aligned_to({a.logp, a.entropy, a.top_logp}, 4), SSM_ERR_ALIGN,
+              "token_log_probs: misaligned pointer");
   s.rows = a.rows, s.row_stride = a.row_stride, s.ignore = a.ignore_index, s.vocab = a.vocab, s.top_k = a.top_k;
   set_temperature(s, a.temperature);
   s.logits = a.logits, s.targets = a.targets, s.logp = a.logp, s.entropy = a.entropy, s.top_logp = a.top_logp, s.top_ids = a.top_ids;
@@ -679,7 +680,8 @@ int fill(const ssm_topk_distill_args& a, StatsArgs& s) {
   SSM_REQUIRE(a.top_k <= kMaxTeacher, SSM_ERR_TOO_LARGE, "topk_distill_loss: at most 1024 teacher entries a row");
   SSM_REQUIRE(valid_dtype(a.teacher_dtype), SSM_ERR_DTYPE, "topk_distill_loss: unknown teacher dtype");
   SSM_REQUIRE(a.rows == 0 || (a.logits && a.teacher && a.ids), SSM_ERR_NULL, "topk_distill_loss: NULL pointer");
-  SSM_REQUIRE(aligned_to(a.logits, dtype_size(a.io_dtype)) && aligned_to(a.stats, 16), SSM_ERR_ALIGN, "topk_distill_loss: misaligned pointer");
+  SSM_REQUIRE(aligned_to(a.logits, dtype_size(a.io_dtype)) && aligned_to(a.teacher, dtype_size(a.teacher_dtype)) && aligned_to(a.stats, 16) && aligned_to(a.ids, 8) && aligned_to(a.loss, 4),
+              SSM_ERR_ALIGN, "topk_distill_loss: misaligned pointer");
   s.rows = a.rows, s.row_stride = a.row_stride, s.vocab = a.vocab, s.top_k = a.top_k, s.teacher_dtype = a.teacher_dtype;
   set_temperature(s, a.temperature);
   s.logits = a.logits, s.teacher = a.teacher, s.ids = a.ids, s.logp = a.loss, s.stats = reinterpret_cast<float4*>(a.stats);
@@ -710,6 +712,8 @@ extern "C" int ssm_token_logp_bwd(const ssm_token_logp_bwd_args* args, ssm_strea
   if (const int rc = fill(args->fwd, g.f)) return rc;
   if (g.f.rows == 0) return SSM_OK;
   SSM_REQUIRE(args->dlogits && g.f.stats && (!args->dtop_logp || g.f.top_ids), SSM_ERR_NULL, "token_log_probs backward: NULL pointer");
+  SSM_REQUIRE(aligned_to({args->dlogp, args->dentropy, args->dtop_logp}, 4) && aligned_to(args->dlogits, dtype_size(args->fwd.io_dtype)), SSM_ERR_ALIGN,
+              "token_log_probs backward: misaligned pointer");
   g.dlogp = args->dlogp, g.dentropy = args->dentropy, g.dtop = g.f.top_k ? args->dtop_logp : nullptr, g.out = args->dlogits;
   return grad_of<false>(g, args->fwd.io_dtype, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -729,6 +733,7 @@ extern "C" int ssm_topk_distill_bwd(const ssm_topk_distill_bwd_args* args, ssm_s
   if (const int rc = fill(args->fwd, g.f)) return rc;
   if (g.f.rows == 0) return SSM_OK;
   SSM_REQUIRE(args->dlogits && g.f.stats && args->dloss, SSM_ERR_NULL, "topk_distill_loss backward: NULL pointer");
+  SSM_REQUIRE(aligned_to(args->dloss, 4) && aligned_to(args->dlogits, dtype_size(args->fwd.io_dtype)), SSM_ERR_ALIGN, "topk_distill_loss backward: misaligned pointer");
   g.dlogp = args->dloss, g.out = args->dlogits;
   return grad_of<true>(g, args->fwd.io_dtype, reinterpret_cast<cudaStream_t>(stream));
 }
