@@ -276,6 +276,7 @@ __global__ void __launch_bounds__(kPairThreads, 4) pairs_kernel(const __grid_con
   __syncthreads();
   if (!__syncthreads_and(tc::mbar_wait(landed, 0))) {
     if (tid == 0 && out.status) *(volatile int32_t*)out.status = 6;
+    tc::mbar_wait(landed, 0);  // nothing is under way when the block ends, as far as a second limit goes
     return;
   }
   if (a.where.table && n < C) {  // rows of the next sequence: nothing of them may enter a product, not even times zero
