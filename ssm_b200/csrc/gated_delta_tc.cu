@@ -21,8 +21,13 @@
 // which stays in registers.  o needs neither r nor a product of its own: Y and Z are 64 more rows of the operands X and W.
 // Measured, K = V = 128: 1.2 us a chunk with 32 walks side by side (tensor pipe 48 % busy on the SMs that have one), 1.9 where a training call's
 // states and rest are stored, forward and back; 128 walks move 796 MB in 141 us, 5.6 TB/s.
-// Roundings to 16 bits: S, W, Z, X, Y (from rounded P) and the weighted r, each half a step of the type; sums and the state between chunks are
-// fp32.  For bf16 the outputs and gradients of random inputs are 0.25 to 0.3 % off in norm before their own rounding (0.17 %).
+// Roundings to 16 bits, each half a step of the type, because the tensor cores take such operands; two pieces of each would double the walk's products and
+// bytes.  Forward: S as an operand, X, W (from X gam), P, Y (from rounded P and X), Z (from rounded P and W), the weighted r.  Backward: the kept S, D and r,
+// w as it is read again, gam w, the scaled q, Wb (from X^T beta suf) and the four matrices of pairs in grads_kernel.  The inverse's products split their factors
+// into two pieces each (16 bits of bf16, 22 of fp16).  Sums, the state and its adjoint from chunk to chunk are fp32.
+// Off 64 bits in norm, bf16 (fp16 an eighth of it), with the result's own rounding of 0.17 %: 0.31 % for keys in all directions, gradients 0.33 %.  Keys that
+// hardly differ make X and W large against r = X V - W S0: 0.8 % where they are 0.3 of their length apart and strengths come from a sigmoid, gradients
+// up to 1.3 %; 1.2 and 2.1 % at strength 1; 3.2 and 8 % at 1.9.  (The answers as Q S0 and P r of a rounded r: 1.3 % in place of 0.8.)
 #include <algorithm>
 
 #include "gated_delta.cuh"

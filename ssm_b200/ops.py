@@ -808,6 +808,10 @@ def gated_delta_scan(
     does no harm); in chunks of 16-bit operands they are NaN where the recurrence may still say infinity, and a key whose square is beyond 32 bits
     counts as such a value.  The gradients of its sequence and head are not defined then.
 
+    16-bit operands are multiplied on the tensor cores in chunks of 64 tokens, where the state and a chunk's matrices are rounded to their type: bf16 results
+    are 0.3 % off in norm for independent keys, about 1 % (gradients 1 to 2 %) where keys hardly differ, several per cent with strengths close to 2 on top; fp16
+    an eighth of that.  fp32 operands keep 32 bits throughout.
+
     Everything is differentiable but ``cu_seqlens``; gradients are recorded once (no second derivative).
     """
     return _run("gated_delta_scan", q, k, v, g, beta, scale, initial_state, bool(return_final_state), bool(keep_state_fp32),
