@@ -522,14 +522,14 @@ __device__ __forceinline__ void row_grad(const GradArgs& g, const float4 st, int
   float on_p;  // gradient = p (on_p + on_plogp log2 p) + entries
   if constexpr (DISTILL) {
     n = a.top_k;
-    bool any = true;
+    bool any = true, bad = false;  // the loss is NaN where a teacher's sum is, and by an id outside of the vocabulary that has a weight
     if (tid < 32) {
       float top, lns;
       teacher_softmax(a, r, tid, coef, top, lns, any);
+      bad = any && lns != lns;
     }
     none = !__syncthreads_or(tid < 32 && any) || none;  // nothing asked of the row, whatever its logits are
     on_p = dl * a.inv_t;
-    bool bad = false;  // an id outside of the vocabulary that has a weight made the loss NaN
     for (int j = tid; j < n; j += kThreads) {
       const int64_t id = a.ids[r * n + j];
       bad = bad || (id >= a.vocab && coef[j] != 0.f);

@@ -64,3 +64,17 @@ def test_alternatives_of_rows_of_nan_start_at_the_first(rows, vocab, dtype):
     if rows > 1:
         assert torch.equal(ids[1], 2 * torch.arange(k))
         assert torch.equal(ids[2], torch.cat([torch.tensor([0]), torch.arange(k - 1) * 3 + 3]))
+
+
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_a_teacher_that_is_not_finite_shows_in_loss_and_gradient(value):
+    """Its weights are NaN, and with them every column of the row's gradient; the other rows as without it."""
+    from ssm_b200 import ops
+
+    x = torch.randn(3, 700, generator=torch.Generator().manual_seed(0)).cuda().requires_grad_(True)
+    ids = torch.tensor([[1, 2, 3], [3, 4, 5], [5, 6, -1]]).cuda()
+    teacher = torch.tensor([[0.5, 0.0, 1.0], [0.0, value, 1.0], [0.0, 1.0, value]]).cuda()
+    loss = ops.topk_distill_loss(x, teacher, ids)
+    d, = torch.autograd.grad(loss.sum(), x)
+    assert torch.isnan(loss[1]) and torch.isnan(d[1]).all()
+    assert torch.isfinite(loss[[0, 2]]).all() and torch.isfinite(d[[0, 2]]).all()  # an entry left out counts for nothing
