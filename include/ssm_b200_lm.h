@@ -91,8 +91,11 @@ int ssm_gated_delta_bwd(const ssm_gated_delta_bwd_args* args, ssm_stream_t strea
 /* The same on the tensor cores, in chunks of 64 tokens: 16-bit operands, kdim and vdim multiples of 8, kdim <= 128, q, k, v with rows on
  * 16-byte boundaries (strides multiples of 8 elements, none of zero), o and initial_state 16-byte aligned: ..._supported() tells, without
  * looking at anything on the device.  rest and states of the arguments are not used.  scratch is free again when the call's work is done,
- * kept holds what a backward pass reads (`train` nonzero) and is needed without one too; both 256-byte aligned.  State, adjoint state and
- * operands of products are rounded to io_dtype once a chunk (results in bf16: 0.3 % off in norm for independent keys, more where keys hardly differ).  status: a 32-bit word in memory that the device can write, set if a bounded wait ran out. */
+ * kept holds what a backward pass reads (`train` nonzero) and is needed without one too; both 256-byte aligned.  They grow with the chunks, of
+ * which packed sequences have up to len / 64 + num_seqs + 1: for kdim above 64, 40 KiB of scratch and 9 KiB kept a chunk and head; with a backward
+ * pass to follow 25 KiB and 384 vdim bytes kept, and 256 vdim bytes of scratch in the backward call.  State, adjoint state and operands of products are
+ * rounded to io_dtype once a chunk (results in bf16: 0.3 % off in norm for independent keys, more where keys hardly differ).  status: a 32-bit
+ * word in memory that the device can write, set if a bounded wait ran out. */
 int ssm_gated_delta_chunked_supported(const ssm_gated_delta_args* args);
 int64_t ssm_gated_delta_chunked_scratch_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim);
 int64_t ssm_gated_delta_chunked_kept_bytes(int32_t batch, int32_t len, int32_t num_seqs, int32_t heads, int32_t kdim, int32_t vdim, int32_t train);

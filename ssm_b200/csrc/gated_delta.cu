@@ -3,9 +3,9 @@
 //
 // The columns of v are independent rows of the state, so a CTA walks a sequence with 32 of them: four lanes share a row (eight above kdim 128),
 // each with its part of kdim in registers, in pairs for packed fp32 instructions.  A token is one sum over the lanes, S k, behind which the
-// correction follows; o = S q after it does not hold up the next token.  Bound: that chain of products, shuffles and shared-memory loads, on as
-// few SMs as there are rows: 0.26 us a token forward and 0.22 back (777 tokens, kdim 64, 18 CTAs: 200 and 170 us; with eight lanes, a barrier more
-// and loads converted as they were asked for 285 and 244).
+// correction follows; o = S q after it does not hold up the next token.  Bound: one token after another, each some 110 instructions of a warp that has its
+// scheduler to itself (four warps an SM, 22 % of the issue slots): 0.26 us a token forward and 0.22 back on as few SMs as there are rows (777
+// tokens, kdim 64, 18 CTAs: 200 and 170 us; with eight lanes, a barrier more and loads converted as they were asked for 285 and 244).
 //
 // Backward: the adjoint state walks the same way from the end (dS' = dS + scale do q^T; w = beta dS' k = dv; dS <- a (dS' - w k^T)),
 // and needs nothing of the states.  What the other gradients need of them is the state before and the adjoint state behind each
