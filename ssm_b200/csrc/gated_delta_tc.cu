@@ -11,7 +11,7 @@
 //   pairs_kernel   one CTA per (chunk, value head): X, Y, W, Z (and Wb), which depend on no state: all chunks at once.  Products by
 //                  mma.sync on 16 rows a warp; the inverse is kept in fp32: blocks of 16 by substitution, then two rounds of products of
 //                  blocks whose factors are split into two 16-bit pieces.  Bound: shared memory, 70 % of its cycles: 24 ns a chunk and head
-//                  on the whole GPU (192 us for 8192 at K = 128), 41 with Wb, whose registers spill.
+//                  on the whole GPU (196 us for 8192 at K = 128), 42 with Wb, whose registers spill.
 //   chunks_kernel  one CTA per (sequence, value head, 128 rows of the state): the walk over the chunks, forward or back (BACK).
 //   grads_kernel   a CTA per SM over all (chunk, value head): the other gradients from what both walks left (the formulas stand there).
 //
@@ -20,7 +20,7 @@
 // written there by the threads that hold the rows: S (16 bits) x W^T, added to V^T X^T -> r -> times beta suf x K -> added to the state,
 // which stays in registers.  o needs neither r nor a product of its own: Y and Z are 64 more rows of the operands X and W.
 // Measured, K = V = 128: 1.2 us a chunk with 32 walks side by side (tensor pipe 48 % busy on the SMs that have one), 1.9 where a training call's
-// states and rest are stored, forward and back; 128 walks move 796 MB in 141 us, 5.6 TB/s.
+// states and rest are stored, forward and back; 128 walks move 796 MB in 144 us, 5.5 TB/s.
 // Roundings to 16 bits, each half a step of the type, because the tensor cores take such operands; two pieces of each would double the walk's products and
 // bytes.  Forward: S as an operand, X, W (from X gam), P, Y (from rounded P and X), Z (from rounded P and W), the weighted r.  Backward: the kept S, D and r,
 // w as it is read again, gam w, the scaled q, Wb (from X^T beta suf) and the four matrices of pairs in grads_kernel.  The inverse's products split their factors

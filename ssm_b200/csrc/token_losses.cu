@@ -23,7 +23,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256;  // forward and backward of 8192 rows of 50280 bf16 logits: 436 us, 442 with 128, 454 with 512
-constexpr int kUnroll = 4;  // 16-byte pieces a thread has in flight; with alternatives, 4096 rows and 5 of them: 107 us, 125 with two
+constexpr int kUnroll = 4;  // 16-byte pieces a thread has in flight; with entropy and alternatives, 4096 rows and 5 of them: 107 us, 125 with two
 constexpr int kCandidates = 1024;  // kept elements of a slice above the bound, and at it
 constexpr int kMaxTop = 128;
 constexpr int kGroups = kThreads;  // groups of threads whose maxima are looked at, at most
