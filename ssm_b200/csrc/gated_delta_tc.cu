@@ -519,8 +519,8 @@ struct ChunkWalk {
 };
 
 // Warps 0-7 hold the rows of the state (a lane a row, two warps share the columns of 32 rows; with four of them 2240 cycles a chunk instead of 1940), 8-11
-// prepare operands and store what leaves, 12 copies, 13 issues the products, 14 and 15 look at v (forward).  Launched with 128 registers a thread (512 x 128 = 65536), of which
-// the groups of four warps keep 168, 168, 104 and 40.
+// prepare operands and store what leaves, 12 copies, 13 issues the products, 14 and 15 look at v (forward).  Launched with 128 registers a thread
+// (512 x 128 = 65536), of which the groups of four warps keep 168, 168, 104 and 40.
 constexpr int kParts = 2, kCompute = 128 * kParts, kHelp = 128, kWalkThreads = kCompute + kHelp + 128;
 constexpr int kComputeRegs = 168, kHelpRegs = 104, kIssueRegs = 40;
 static_assert(kCompute * kComputeRegs + kHelp * kHelpRegs + 128 * kIssueRegs <= kWalkThreads * 128, "the split draws on what the block was launched with");
@@ -695,7 +695,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) chunks_kernel(const ChunkWalk
       constexpr uint32_t id_doq = tc::instr_desc(128, KD, fmt, 1, 1);            // do^T Q
       for (int p = 0; p < nchunks; ++p) {
         const int se = p % M::NE, sl = p % M::NL;
-        if (!(ok = wait(kFullE + se, p / M::NE) && (BACK || wait(kFullV + se, p / M::NE)) && wait(kFullL + sl, p / M::NL) && wait(kPrep + (p & 1), p >> 1))) break;  // rows of another sequence cut; BACK: q scaled
+        if (!(ok = wait(kFullE + se, p / M::NE) && (BACK || wait(kFullV + se, p / M::NE)) && wait(kFullL + sl, p / M::NL) && wait(kPrep + (p & 1), p >> 1)))
+          break;  // rows of another sequence cut; BACK: q scaled
         tc::fence_after_sync();
         const uint32_t e = tc::smem_u32(sm + se * M::EARLY), l = tc::smem_u32(sm + M::NE * M::EARLY + sl * M::LATE), R = tmem + TC::RO + (p & 1) * 128;
         const uint64_t w_rows = tc::smem_desc_sw128(e + M::W, 16, 1024), v_cols = tc::smem_desc_sw128(e + M::V, kTileBytes, 1024);
