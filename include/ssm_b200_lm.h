@@ -1,6 +1,7 @@
 /*
  * ssm_b200 — C ABI of the operators that stand beside the state-space operators of ssm_b200.h in a language model: the gated
- * delta rule (whole sequences and single tokens), log probabilities of given tokens, distillation from a teacher's top logits.
+ * delta rule (whole sequences and single tokens), log probabilities of given tokens, distillation from a teacher's top logits, the norms around
+ * a block, cross entropy from hidden states, the norm over many tensors with clipping.
  * Same conventions: plain argument structs of raw device pointers, sizes, element strides and SSM_* dtype codes; kernels are
  * enqueued on the given stream; nothing is allocated or synchronised; 0, a negative SSM_ERR_* or a positive cudaError_t is returned
  * and ssm_b200_last_error() describes the last failure.
@@ -15,7 +16,7 @@ extern "C" {
 #endif
 
 /* Raised with every change of a struct's layout, of an entry point's signature or of the set of entry points below. */
-#define SSM_B200_LM_ABI_VERSION 1
+#define SSM_B200_LM_ABI_VERSION 2
 int ssm_b200_lm_abi_version(void);
 
 /* ---------------------------------------------------------------------------------------
@@ -189,6 +190,68 @@ typedef struct {
 
 int ssm_topk_distill(const ssm_topk_distill_args* args, ssm_stream_t stream);
 int ssm_topk_distill_bwd(const ssm_topk_distill_bwd_args* args, ssm_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The norms after and before a block with its gate, residual scale and residual add:
+ *   n = norm(x) post_weight + post_bias;   residual_out = residual + scale gate n;   y = norm(residual_out) weight + bias
+ * norm(x) = (x - m) / sqrt(mean (x - m)^2 + eps), m the row's mean, or 0 with is_rms; post_eps and eps for the two.  All tensors dense: x, y (rows, dim) of io_dtype,
+ * residual (nullable: 0) of res_dtype, residual_out of resout_dtype (rounded there; y is formed from what it was before), parameters (dim) of param_dtype,
+ * both biases or neither.  gate of gate_dtype: gate_kind 0 none (1), 1 (dim), 2 (rows / len, dim), one row for `len` rows, 3 (rows, dim).
+ * stats (rows, 4) fp32, 16-byte aligned, for the backward pass; nullable.  dim <= 8192.
+ *
+ * Backward: from dy and dresidual_out (nullable) writes dx, dresidual (nullable; res_dtype), the parameters' gradients (param_dtype; biases' nullable) and dgate
+ * (gate's shape and type).  partial: ssm_block_norm_bwd_scratch_floats floats, 16-byte aligned.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  int64_t rows, len;
+  int32_t dim, io_dtype, res_dtype, resout_dtype;
+  int32_t param_dtype, gate_dtype, gate_kind, is_rms;
+  float eps, post_eps, scale;
+  int32_t reserved0;
+  const void* x;
+  const void* residual; /* nullable */
+  const void* post_weight;
+  const void* weight;
+  const void* post_bias; /* nullable */
+  const void* bias;      /* nullable */
+  const void* gate;      /* nullable */
+  void* y;
+  void* residual_out;
+  float* stats; /* nullable */
+} ssm_block_norm_args;
+
+typedef struct {
+  ssm_block_norm_args fwd; /* y and residual_out are not read */
+  const void* dy;
+  const void* dresidual_out; /* nullable */
+  void* dx;
+  void* dresidual; /* nullable */
+  void* dpost_weight;
+  void* dweight;
+  void* dpost_bias; /* nullable */
+  void* dbias;      /* nullable */
+  void* dgate;      /* nullable without a gate */
+  float* partial;
+} ssm_block_norm_bwd_args;
+
+int ssm_block_norm_fwd(const ssm_block_norm_args* args, ssm_stream_t stream);
+int64_t ssm_block_norm_bwd_scratch_floats(int64_t rows, int32_t dim);
+int ssm_block_norm_bwd(const ssm_block_norm_bwd_args* args, ssm_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The norm over all elements of many tensors: sqrt(sum x^2), or max |x| with is_max, into *norm (device, fp32); NaN once there is one.  Clipping multiplies
+ * every element in place by min(1, max_norm / (norm + 1e-6)) and leaves all as it is where that is 1 or max_norm infinite.  The list is read by the
+ * host during the call; every tensor is dense memory of its type.  scratch: ssm_global_norm_scratch_bytes(count) bytes, 8-byte aligned.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  const void* data;
+  int64_t numel;
+  int32_t dtype, reserved0;
+} ssm_tensor_ref;
+
+int64_t ssm_global_norm_scratch_bytes(int64_t count);
+int ssm_global_norm(const ssm_tensor_ref* tensors, int64_t count, int32_t is_max, void* scratch, float* norm, ssm_stream_t stream);
+int ssm_clip_global_norm(const ssm_tensor_ref* tensors, int64_t count, int32_t is_max, float max_norm, void* scratch, float* norm, ssm_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -143,7 +143,7 @@ class SsdBwdArgs(C.Structure):
 
 # ---- include/ssm_b200_lm.h -----------------------------------------------------------------
 
-LM_ABI_VERSION = 1  # SSM_B200_LM_ABI_VERSION
+LM_ABI_VERSION = 2  # SSM_B200_LM_ABI_VERSION
 
 
 def _strides(names: str, axes: str) -> list:
@@ -193,6 +193,23 @@ class TopkDistillArgs(C.Structure):
 
 class TopkDistillBwdArgs(C.Structure):
     _fields_ = [("fwd", TopkDistillArgs), ("dloss", fp), ("dlogits", vp)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [
+        ("rows", i64), ("len", i64), ("dim", i32), ("io_dtype", i32), ("res_dtype", i32), ("resout_dtype", i32), ("param_dtype", i32), ("gate_dtype", i32),
+        ("gate_kind", i32), ("is_rms", i32), ("eps", C.c_float), ("post_eps", C.c_float), ("scale", C.c_float), ("reserved0", i32),
+        ("x", vp), ("residual", vp), ("post_weight", vp), ("weight", vp), ("post_bias", vp), ("bias", vp), ("gate", vp), ("y", vp), ("residual_out", vp), ("stats", fp),
+    ]
+
+
+class BlockNormBwdArgs(C.Structure):
+    _fields_ = [("fwd", BlockNormArgs), *[(n, vp) for n in ("dy", "dresidual_out", "dx", "dresidual", "dpost_weight", "dweight", "dpost_bias", "dbias", "dgate")],
+                ("partial", fp)]
+
+
+class TensorRef(C.Structure):
+    _fields_ = [("data", vp), ("numel", i64), ("dtype", i32), ("reserved0", i32)]
 
 
 # entry point -> (restype, argtypes); every name here is declared in include/ssm_b200.h or include/ssm_b200_lm.h
@@ -253,6 +270,12 @@ ENTRY_POINTS = {
     "ssm_token_logp_bwd": (C.c_int, [C.POINTER(TokenLogpBwdArgs), vp]),
     "ssm_topk_distill": (C.c_int, [C.POINTER(TopkDistillArgs), vp]),
     "ssm_topk_distill_bwd": (C.c_int, [C.POINTER(TopkDistillBwdArgs), vp]),
+    "ssm_block_norm_fwd": (C.c_int, [C.POINTER(BlockNormArgs), vp]),
+    "ssm_block_norm_bwd_scratch_floats": (C.c_int64, [i64, i32]),
+    "ssm_block_norm_bwd": (C.c_int, [C.POINTER(BlockNormBwdArgs), vp]),
+    "ssm_global_norm_scratch_bytes": (C.c_int64, [i64]),
+    "ssm_global_norm": (C.c_int, [C.POINTER(TensorRef), i64, i32, vp, vp, vp]),
+    "ssm_clip_global_norm": (C.c_int, [C.POINTER(TensorRef), i64, i32, C.c_float, vp, vp, vp]),
 }
 
 _lib = None

@@ -16,6 +16,7 @@
 namespace ssm_ext {
 void bind_operators(pybind11::module& m);     // operators.cpp
 void bind_lm_operators(pybind11::module& m);  // lm_operators.cpp
+void bind_training_operators(pybind11::module& m);  // training_operators.cpp
 }
 
 using namespace ssm_ext;
@@ -280,6 +281,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "ssm.ops CUDA backend for B200 (sm_100a): the ten entry points of upstream's compiled extension, on libssm_b200";
   ssm_ext::bind_operators(m);
   ssm_ext::bind_lm_operators(m);
+  ssm_ext::bind_training_operators(m);
   m.def("abi_version", []() { return ssm_b200_abi_version(); });
   m.def("selective_scan", &selective_scan, py::arg("u"), py::arg("delta"), py::arg("A"), py::arg("B"), py::arg("C"), py::arg("D") = c10::nullopt,
         py::arg("z") = c10::nullopt, py::arg("dt_bias") = c10::nullopt, py::arg("softplus") = false, py::arg("return_last_state") = false);

@@ -1,0 +1,203 @@
+// The norms around a block and the norm over many tensors with clipping: the operator surface of ssm_b200.ops over
+// include/ssm_b200_lm.h.
+#include "../../../include/ssm_b200_lm.h"
+
+#include <algorithm>
+
+#include "call.h"
+
+namespace ssm_ext {
+namespace {
+
+namespace py = pybind11;
+
+// ---------------------------------------------------------------------------------------------
+// the norms after and before a block
+// ---------------------------------------------------------------------------------------------
+struct BlockNormCall final : Call {
+  Tensor x, pw, w, stats;
+  OptTensor res, pb, b, gate;
+  at::ScalarType t_r{}, t_pw, t_w, t_pb{}, t_b{}, out_type;
+  std::vector<int64_t> gate_shape;
+  int64_t rows, len, dim;
+  int gate_kind = 0;
+  bool is_rms, has_pb, has_b;
+  double scale, eps, post_eps;
+
+  BlockNormCall(const Tensor& x_, const OptTensor& res_, const Tensor& pw_, const Tensor& w_, const OptTensor& pb_, const OptTensor& b_, const OptTensor& gate_, double scale_,
+                bool is_rms_, double eps_, double post_eps_, bool in_fp32)
+      : t_pw(pw_.scalar_type()), t_w(w_.scalar_type()), out_type(in_fp32 ? at::kFloat : x_.scalar_type()), is_rms(is_rms_), scale(scale_), eps(eps_), post_eps(post_eps_) {
+    SSM_ARG(x_.dim() == 3, "x must have shape (B, L, D).");
+    dim = x_.size(2), len = x_.size(1), rows = x_.size(0) * x_.size(1);
+    SSM_ARG(dim >= 1 && dim <= 8192, "fused_block_norm: D lies between 1 and 8192.");
+    SSM_ARG(rows < ((int64_t)1 << 31), "fused_block_norm: too many rows.");
+    auto param = [&](const Tensor& t, const char* name) { SSM_ARG(t.dim() == 1 && t.size(0) == dim, name, " must have shape (D,)."); };
+    param(pw_, "post_weight"), param(w_, "weight");
+    if (pb_.has_value()) param(*pb_, "post_bias"), t_pb = pb_->scalar_type();
+    if (b_.has_value()) param(*b_, "bias"), t_b = b_->scalar_type();
+    if (res_.has_value()) {
+      SSM_ARG(res_->sizes() == x_.sizes(), "residual must match the shape of x.");
+      t_r = res_->scalar_type();
+    }
+    if (gate_.has_value()) {
+      const Tensor& g = *gate_;
+      if (g.dim() == 1 && g.size(0) == dim) gate_kind = 1;
+      else if ((g.dim() == 2 && g.size(0) == x_.size(0) && g.size(1) == dim) || (g.dim() == 3 && g.size(0) == x_.size(0) && g.size(1) == 1 && g.size(2) == dim)) gate_kind = 2;
+      else if (g.sizes() == x_.sizes()) gate_kind = 3;
+      else reject("gate must have shape (D,), (B, D), (B, 1, D) or (B, L, D).");
+      gate_shape = g.sizes().vec();
+    }
+    SSM_ARG(std::isfinite(scale) && std::abs(scale) < 3e38, "residual_scale must be finite, in fp32 too.");
+    SSM_ARG(eps >= 0 && post_eps >= 0 && std::isfinite(eps) && std::isfinite(post_eps), "eps must be finite and not negative.");
+    same_device(x_, {&pw_, &w_});
+    need_cuda(x_, {&res_, &pb_, &b_, &gate_});
+    dtype_code(x_, "fused_block_norm"), dtype_code(pw_, "fused_block_norm post_weight"), dtype_code(w_, "fused_block_norm weight");
+    if (res_.has_value()) dtype_code(*res_, "fused_block_norm residual");
+    if (pb_.has_value()) dtype_code(*pb_, "fused_block_norm post_bias");
+    if (b_.has_value()) dtype_code(*b_, "fused_block_norm bias");
+    if (gate_.has_value()) dtype_code(*gate_, "fused_block_norm gate");
+    input(x_), input(res_), input(pw_), input(w_), input(pb_), input(b_), input(gate_);
+    auto dense = [](const OptTensor& t) { return t.has_value() ? OptTensor(t->detach().contiguous()) : OptTensor(); };
+    x = x_.detach().contiguous(), res = dense(res_), gate = dense(gate_);
+    // the parameters go in as they are where they share a type
+    if (t_pw == t_w && (!pb_.has_value() || t_pb == t_w) && (!b_.has_value() || t_b == t_w)) pw = pw_.detach().contiguous(), w = w_.detach().contiguous(), pb = dense(pb_), b = dense(b_);
+    else pw = f32c(pw_), w = f32c(w_), pb = f32c(pb_), b = f32c(b_);
+    has_pb = pb.has_value(), has_b = b.has_value();
+    if (has_pb != has_b) (has_pb ? b : pb) = at::zeros(w.sizes(), w.options());  // the kernels take both or neither
+  }
+  void fill(ssm_block_norm_args& a) const {
+    a.rows = rows, a.len = std::max<int64_t>(len, 1), a.dim = (int)dim, a.io_dtype = dtype_code(x, "fused_block_norm");
+    a.res_dtype = res.has_value() ? dtype_code(*res, "fused_block_norm residual") : 0, a.resout_dtype = out_type == at::kFloat ? SSM_F32 : a.io_dtype;
+    a.param_dtype = dtype_code(w, "fused_block_norm weight"), a.gate_dtype = gate.has_value() ? dtype_code(*gate, "fused_block_norm gate") : 0;
+    a.gate_kind = gate_kind, a.is_rms = is_rms, a.eps = (float)eps, a.post_eps = (float)post_eps, a.scale = (float)scale;
+    a.x = x.data_ptr(), a.residual = ptr(res), a.post_weight = pw.data_ptr(), a.weight = w.data_ptr(), a.post_bias = ptr(pb), a.bias = ptr(b), a.gate = ptr(gate);
+    if (stats.defined()) a.stats = stats.data_ptr<float>();
+  }
+  variable_list forward(bool train) override {
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = at::empty(x.sizes(), x.options()), r = at::empty(x.sizes(), x.options().dtype(out_type));
+    if (train) stats = at::empty({rows, 4}, x.options().dtype(at::kFloat));
+    ssm_block_norm_args a{};
+    fill(a);
+    a.y = y.data_ptr(), a.residual_out = r.data_ptr();
+    run(ssm_block_norm_fwd(&a, stream_of(x)));
+    return {y, r};
+  }
+  variable_list backward(const variable_list& grads) override {
+    c10::cuda::CUDAGuard guard(x.device());
+    const auto like_empty = [&](const Tensor& t) { return rows ? at::empty(t.sizes(), t.options()) : at::zeros(t.sizes(), t.options()); };
+    Tensor dy = grads[0].defined() ? like(grads[0], x) : at::zeros(x.sizes(), x.options()), dr;
+    if (grads[1].defined()) dr = grads[1].detach().to(out_type).contiguous();
+    Tensor dx = like_empty(x), dpw = like_empty(pw), dw = like_empty(w), dres, dpb, db, dgate;
+    if (res.has_value()) dres = like_empty(*res);
+    if (has_pb) dpb = like_empty(w);
+    if (has_b) db = like_empty(w);
+    if (gate.has_value()) dgate = like_empty(*gate);
+    Tensor partial = at::empty({ssm_block_norm_bwd_scratch_floats(rows, (int)dim)}, x.options().dtype(at::kFloat));
+    ssm_block_norm_bwd_args g{};
+    fill(g.fwd);
+    auto p = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    g.dy = p(dy), g.dresidual_out = p(dr), g.dx = p(dx), g.dresidual = p(dres), g.dpost_weight = p(dpw), g.dweight = p(dw), g.dpost_bias = p(dpb), g.dbias = p(db), g.dgate = p(dgate);
+    g.partial = partial.data_ptr<float>();
+    run(ssm_block_norm_bwd(&g, stream_of(x)));
+    variable_list out = {dx};
+    if (res.has_value()) out.push_back(cast(dres, t_r));
+    out.push_back(cast(dpw, t_pw)), out.push_back(cast(dw, t_w));
+    if (has_pb) out.push_back(cast(dpb, t_pb));
+    if (has_b) out.push_back(cast(db, t_b));
+    if (gate.has_value()) out.push_back(dgate.view(gate_shape));
+    return out;
+  }
+};
+py::tuple fused_block_norm(const Tensor& x, const OptTensor& residual, const Tensor& post_weight, const Tensor& weight, const OptTensor& post_bias, const OptTensor& bias, const OptTensor& gate,
+                           double scale, bool is_rms, double eps, double post_eps, bool in_fp32) {
+  ValueErrors scope;
+  const variable_list r = invoke_call(c10::make_intrusive<BlockNormCall>(x, residual, post_weight, weight, post_bias, bias, gate, scale, is_rms, eps, post_eps, in_fp32));
+  return py::make_tuple(r[0], r[1]);
+}
+
+// ---------------------------------------------------------------------------------------------
+// the norm over many tensors, and clipping by it
+// ---------------------------------------------------------------------------------------------
+struct TensorList {
+  std::vector<ssm_tensor_ref> refs;
+  std::vector<Tensor> held;                             // dense copies
+  std::vector<std::pair<Tensor, Tensor>> strided;       // (given, copy) of those that do not fill their memory
+  c10::Device device = c10::Device(c10::kCUDA, 0);
+
+  TensorList(const std::vector<Tensor>& tensors, const char* what, bool in_place) {
+    device = tensors.empty() ? c10::Device(c10::kCUDA, at::cuda::current_device()) : tensors[0].device();
+    c10::cuda::OptionalCUDAGuard guard;
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    refs.reserve(tensors.size());
+    for (const Tensor& t : tensors) {
+      SSM_ARG(t.layout() == c10::kStrided, what, ": sparse tensors are not taken.");
+      same_device(tensors[0], {&t});
+      const int type = dtype_code(t, what);
+      SSM_ARG(!(at::GradMode::is_enabled() && t.requires_grad()), what, ": no gradient flows through it; detach the tensors.");
+      TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "ssm_b200 operators have no forward-mode derivative");
+      if (t.numel() == 0) continue;
+      Tensor d = t.detach();
+      if (in_place) {
+        int64_t reach = 0;
+        for (int64_t i = 0; i < d.dim(); ++i) {
+          SSM_ARG(d.size(i) <= 1 || d.stride(i) != 0, what, ": a broadcast tensor cannot be scaled in place.");
+          reach += (d.size(i) - 1) * d.stride(i);
+        }
+        const uintptr_t at = reinterpret_cast<uintptr_t>(d.data_ptr());
+        spans.emplace_back(at, at + (uintptr_t)(reach + 1) * d.element_size());
+      }
+      if (!d.is_non_overlapping_and_dense()) {
+        if (!guard.original_device().has_value()) guard.set_device(device);
+        Tensor copy = d.contiguous();
+        if (in_place) strided.emplace_back(d, copy);
+        d = copy;
+        held.push_back(d);
+      }
+      refs.push_back(ssm_tensor_ref{d.data_ptr(), d.numel(), type, 0});
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i) SSM_ARG(spans[i].first >= spans[i - 1].second, what, ": two of the tensors share memory (one given twice would be scaled twice).");
+  }
+};
+double max_of(double norm_type) {
+  SSM_ARG(norm_type == 2.0 || norm_type == HUGE_VAL, "norm_type must be 2 or inf.");
+  return norm_type == 2.0 ? 0 : 1;
+}
+Tensor global_norm(const std::vector<Tensor>& tensors, double norm_type) {
+  ValueErrors scope;
+  const int kind = (int)max_of(norm_type);
+  const TensorList list(tensors, "global_norm", false);
+  c10::cuda::CUDAGuard guard(list.device);
+  const auto bytes = at::TensorOptions().device(list.device).dtype(at::kByte);
+  const int64_t n = (int64_t)list.refs.size();
+  Tensor norm = at::empty({}, bytes.dtype(at::kFloat)), scratch = at::empty({ssm_global_norm_scratch_bytes(n)}, bytes);
+  run(ssm_global_norm(list.refs.data(), n, kind, scratch.data_ptr(), norm.data_ptr<float>(), stream_of(norm)));
+  return norm;
+}
+Tensor clip_global_norm_(const std::vector<Tensor>& tensors, double max_norm, double norm_type) {
+  ValueErrors scope;
+  const int kind = (int)max_of(norm_type);
+  SSM_ARG(max_norm >= 0, "max_norm must not be negative.");
+  TensorList list(tensors, "clip_global_norm_", true);
+  c10::cuda::CUDAGuard guard(list.device);
+  const auto bytes = at::TensorOptions().device(list.device).dtype(at::kByte);
+  const int64_t n = (int64_t)list.refs.size();
+  Tensor norm = at::empty({}, bytes.dtype(at::kFloat)), scratch = at::empty({ssm_global_norm_scratch_bytes(n)}, bytes);
+  run(ssm_clip_global_norm(list.refs.data(), n, kind, (float)max_norm, scratch.data_ptr(), norm.data_ptr<float>(), stream_of(norm)));
+  for (const auto& s : list.strided) s.first.copy_(s.second);
+  for (const Tensor& t : tensors)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // a graph that keeps one of them for its backward pass notices
+  return norm;
+}
+
+}  // namespace
+
+void bind_training_operators(py::module& m) {
+  auto ops = m.attr("operators").cast<py::module>();
+  ops.def("fused_block_norm", &fused_block_norm);
+  ops.def("global_norm", &global_norm);
+  ops.def("clip_global_norm_", &clip_global_norm_);
+}
+
+}  // namespace ssm_ext

@@ -854,6 +854,57 @@ def topk_distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tenso
     return _run("topk_distill_loss", logits, teacher_logits, teacher_ids, float(temperature))
 
 
+# =========================================================================================
+# a training step around the mixers
+# =========================================================================================
+
+
+def fused_block_norm(
+    x: Tensor,
+    residual: Optional[Tensor],
+    post_weight: Tensor,
+    weight: Tensor,
+    post_bias: Optional[Tensor] = None,
+    bias: Optional[Tensor] = None,
+    gate: Optional[Tensor] = None,
+    residual_scale: float = 1.0,
+    is_rms: bool = True,
+    eps: float = 1e-5,
+    post_eps: Optional[float] = None,
+    residual_in_fp32: bool = True,
+):
+    """Extension: the norm after a block and the one before the next, with the block's gate, its residual scale and the residual add in one call::
+
+        n = norm(x) post_weight + post_bias;   r = residual + residual_scale gate n;   y = norm(r) weight + bias
+
+    ``x (B, L, D)`` is the block's output, ``residual`` the stream (``None``: zero), ``norm`` RMSNorm or, with ``is_rms=False``, LayerNorm (``eps`` for
+    ``y``, ``post_eps`` for ``n``, ``eps`` where that is ``None``).  ``gate``: ``(D,)`` per channel, ``(B, D)`` or ``(B, 1, D)`` per sequence, ``(B, L, D)``
+    per token.  Returns ``(y, r)``, ``y`` in ``x``'s type, ``r`` in fp32 with ``residual_in_fp32``, else in ``x``'s type; ``y`` is formed from ``r`` before that
+    rounding.  ``D`` up to 8192.  All tensors are differentiable (once); a gradient has its input's type."""
+    return _run("fused_block_norm", x, residual, post_weight, weight, post_bias, bias, gate, float(residual_scale), bool(is_rms), float(eps),
+                float(eps if post_eps is None else post_eps), bool(residual_in_fp32))
+
+
+def _tensor_list(tensors, what: str) -> list:
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what} is not traced: it reads a list of tensors that a traced graph does not hold")
+    return [tensors] if isinstance(tensors, Tensor) else list(tensors)
+
+
+def global_norm(tensors, norm_type: float = 2.0) -> Tensor:
+    """Extension: the norm over all elements of many tensors (their mixed types as they are), as a 0-d fp32 tensor on their device: the root of the sum of
+    squares, or with ``norm_type=inf`` the largest absolute value.  Squares that 32 bits cannot hold are summed in 64.  NaN anywhere gives NaN.
+    No tensors: 0.  Not differentiable; tensors that require a gradient are refused while gradients are recorded."""
+    return _native().global_norm(_tensor_list(tensors, "global_norm"), float(norm_type))
+
+
+def clip_global_norm_(tensors, max_norm: float, norm_type: float = 2.0) -> Tensor:
+    """Extension: multiplies all tensors in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being :func:`global_norm` of them, which is
+    returned (its value before).  No synchronisation; where nothing is to be clipped, nothing is written.  A norm of infinity leaves 0 (NaN in place of
+    infinities), a NaN makes all NaN; ``max_norm=inf`` clips nothing.  Tensors that share memory, and broadcast ones, are refused."""
+    return _native().clip_global_norm_(_tensor_list(tensors, "clip_global_norm_"), float(max_norm), float(norm_type))
+
+
 __all__ = [
     "selective_scan",
     "selective_state_step",
@@ -872,4 +923,7 @@ __all__ = [
     "gated_delta_step",
     "token_log_probs",
     "topk_distill_loss",
+    "fused_block_norm",
+    "global_norm",
+    "clip_global_norm_",
 ]
