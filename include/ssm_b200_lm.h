@@ -239,6 +239,44 @@ int64_t ssm_block_norm_bwd_scratch_floats(int64_t rows, int32_t dim);
 int ssm_block_norm_bwd(const ssm_block_norm_bwd_args* args, ssm_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Cross entropy from hidden states: z = hidden weight^T, log_z[r] = ln sum_v exp z[r, v], loss[r] = log_z[r] - z[r, targets[r]], without a (rows, vocab) matrix.
+ * hidden (rows, dim), weight (vocab, dim) of io_dtype, rows at their strides.  A row whose target is ignore_index costs nothing, is not read and gives 0; any other target outside
+ * of the vocabulary gives a loss of NaN.  row_loss and log_z (rows) fp32; loss, with reduction 1 (sum) or 2 (mean over the rows that count, 0 without any), one float.
+ * stats (rows, 2) fp32 keeps what the backward pass needs (nullable).  status: a word in host memory that the device writes, set where a bounded wait ran out.
+ *
+ * Backward: from dloss (rows, or one float with a reduction) and dlog_z (rows, nullable) writes dhidden (rows, dim; io_dtype) and dweight (vocab, dim; dweight_dtype),
+ * dense, each nullable, via pieces of at most SSM_LINEAR_CE_PIECE_BYTES of the logits' gradient in 16 bits.
+ * scratch: ssm_linear_ce_scratch_bytes(args, backward) bytes, 256-byte aligned.
+ * ------------------------------------------------------------------------------------- */
+#define SSM_LINEAR_CE_PIECE_BYTES (512 << 20)
+typedef struct {
+  int64_t rows, hidden_stride, weight_stride, ignore_index;
+  int32_t dim, vocab, io_dtype, reduction;
+  const void* hidden;
+  const void* weight;
+  const int64_t* targets;
+  float* row_loss;
+  float* log_z;
+  float* loss;  /* nullable without a reduction */
+  float* stats; /* nullable */
+  void* scratch;
+  int32_t* status;
+} ssm_linear_ce_args;
+
+typedef struct {
+  ssm_linear_ce_args fwd; /* hidden, weight, targets and stats are read */
+  const float* dloss;
+  const float* dlog_z; /* nullable */
+  void* dhidden;       /* nullable */
+  void* dweight;       /* nullable */
+  int32_t dweight_dtype, reserved0;
+} ssm_linear_ce_bwd_args;
+
+int64_t ssm_linear_ce_scratch_bytes(const ssm_linear_ce_args* args, int32_t backward);
+int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t stream);
+int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * The norm over all elements of many tensors: sqrt(sum x^2), or max |x| with is_max, into *norm (device, fp32); NaN once there is one.  Clipping multiplies
  * every element in place by min(1, max_norm / (norm + 1e-6)) and leaves all as it is where that is 1 or max_norm infinite.  The list is read by the
  * host during the call; every tensor is dense memory of its type.  scratch: ssm_global_norm_scratch_bytes(count) bytes, 8-byte aligned.

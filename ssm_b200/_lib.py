@@ -208,6 +208,17 @@ class BlockNormBwdArgs(C.Structure):
                 ("partial", fp)]
 
 
+class LinearCeArgs(C.Structure):
+    _fields_ = [
+        ("rows", i64), ("hidden_stride", i64), ("weight_stride", i64), ("ignore_index", i64), ("dim", i32), ("vocab", i32), ("io_dtype", i32), ("reduction", i32),
+        ("hidden", vp), ("weight", vp), ("targets", vp), ("row_loss", fp), ("log_z", fp), ("loss", fp), ("stats", fp), ("scratch", vp), ("status", vp),
+    ]
+
+
+class LinearCeBwdArgs(C.Structure):
+    _fields_ = [("fwd", LinearCeArgs), ("dloss", fp), ("dlog_z", fp), ("dhidden", vp), ("dweight", vp), ("dweight_dtype", i32), ("reserved0", i32)]
+
+
 class TensorRef(C.Structure):
     _fields_ = [("data", vp), ("numel", i64), ("dtype", i32), ("reserved0", i32)]
 
@@ -273,6 +284,9 @@ ENTRY_POINTS = {
     "ssm_block_norm_fwd": (C.c_int, [C.POINTER(BlockNormArgs), vp]),
     "ssm_block_norm_bwd_scratch_floats": (C.c_int64, [i64, i32]),
     "ssm_block_norm_bwd": (C.c_int, [C.POINTER(BlockNormBwdArgs), vp]),
+    "ssm_linear_ce_scratch_bytes": (C.c_int64, [C.POINTER(LinearCeArgs), i32]),
+    "ssm_linear_ce_fwd": (C.c_int, [C.POINTER(LinearCeArgs), vp]),
+    "ssm_linear_ce_bwd": (C.c_int, [C.POINTER(LinearCeBwdArgs), vp]),
     "ssm_global_norm_scratch_bytes": (C.c_int64, [i64]),
     "ssm_global_norm": (C.c_int, [C.POINTER(TensorRef), i64, i32, vp, vp, vp]),
     "ssm_clip_global_norm": (C.c_int, [C.POINTER(TensorRef), i64, i32, C.c_float, vp, vp, vp]),

@@ -135,7 +135,7 @@ inline void ssd_poll(int64_t device) {
   const int32_t code = *word;
   if (code == 0) return;
   *word = 0;
-  TORCH_CHECK(false, std::string() + (code < 4 ? "ssd_scan" : "gated_delta_scan") + ": a bounded device-side wait ran out in an earlier launch (status " + std::to_string(code) + "); its outputs are invalid");
+  TORCH_CHECK(false, std::string() + (code < 4 ? "ssd_scan" : code < 128 ? "gated_delta_scan" : "linear_cross_entropy") + ": a bounded device-side wait ran out in an earlier launch (status " + std::to_string(code) + "); its outputs are invalid");
 }
 
 }  // namespace ssm_ext

@@ -1,5 +1,5 @@
-// The norms around a block and the norm over many tensors with clipping: the operator surface of ssm_b200.ops over
-// include/ssm_b200_lm.h.
+// The norms around a block, cross entropy from hidden states and the norm over many tensors with clipping: the operator surface of
+// ssm_b200.ops over include/ssm_b200_lm.h.
 #include "../../../include/ssm_b200_lm.h"
 
 #include <algorithm>
@@ -117,6 +117,96 @@ py::tuple fused_block_norm(const Tensor& x, const OptTensor& residual, const Ten
 }
 
 // ---------------------------------------------------------------------------------------------
+// cross entropy from hidden states
+// ---------------------------------------------------------------------------------------------
+// (..., D) as rows with a stride; copied where the axes before the last do not lie evenly, or lie on one another
+Tensor rows_of(const Tensor& t) {
+  Tensor d = t.detach();
+  int64_t rows = 1;
+  for (int64_t i = 0; i + 1 < d.dim(); ++i) rows *= d.size(i);
+  d = d.reshape({rows, d.size(-1)});
+  return (d.size(1) <= 1 || d.stride(1) == 1) && (d.size(0) <= 1 || d.stride(0) >= d.size(1)) ? d : d.contiguous();
+}
+struct LinearCeCall final : Call {
+  Tensor h, w, targets, stats;
+  std::vector<int64_t> shape, lead_shape;
+  at::ScalarType t_w;
+  int64_t ignore;
+  int reduction;
+  bool want_z, grad_h, grad_w;
+
+  LinearCeCall(const Tensor& hidden, const Tensor& weight, const Tensor& targets_, int64_t ignore_, const std::string& reduction_, bool want_z_)
+      : t_w(weight.scalar_type()), ignore(ignore_), want_z(want_z_), grad_h(hidden.requires_grad()), grad_w(weight.requires_grad()) {
+    SSM_ARG(hidden.dim() >= 1 && weight.dim() == 2 && hidden.size(-1) == weight.size(1), "hidden must have shape (..., D) and weight (V, D).");
+    SSM_ARG(weight.size(0) >= 1 && weight.size(1) >= 1, "weight must have at least one row and one column.");
+    SSM_ARG(weight.size(0) <= (1 << 28) && weight.size(1) <= (1 << 20), "linear_cross_entropy: V is at most 2^28, D at most 2^20.");
+    shape = hidden.sizes().vec(), lead_shape = shape;
+    lead_shape.pop_back();
+    SSM_ARG(targets_.sizes() == at::IntArrayRef(lead_shape), "targets must have the shape of hidden without the last axis.");
+    SSM_ARG(at::isIntegralType(targets_.scalar_type(), false), "targets must be integers.");
+    SSM_ARG(targets_.numel() <= (1 << 28), "linear_cross_entropy: more than 2^28 rows.");
+    SSM_ARG(reduction_ == "none" || reduction_ == "sum" || reduction_ == "mean", "reduction must be 'none', 'sum' or 'mean'.");
+    reduction = reduction_ == "none" ? 0 : reduction_ == "sum" ? 1 : 2;
+    same_device(hidden, {&weight, &targets_});
+    dtype_code(hidden, "linear_cross_entropy"), dtype_code(weight, "linear_cross_entropy weight");
+    input(hidden), input(weight), input(targets_);
+    h = rows_of(hidden), w = rows_of(weight.scalar_type() == hidden.scalar_type() ? weight : weight.detach().to(hidden.scalar_type()));
+    targets = targets_.detach().to(at::kLong).contiguous();
+  }
+  int64_t rows() const { return targets.numel(); }
+  at::TensorOptions f32() const { return h.options().dtype(at::kFloat).requires_grad(false); }
+  void fill(ssm_linear_ce_args& a) const {
+    a.rows = rows(), a.hidden_stride = rows() > 1 ? h.stride(0) : h.size(1), a.weight_stride = w.size(0) > 1 ? w.stride(0) : w.size(1), a.ignore_index = ignore;
+    a.dim = (int)w.size(1), a.vocab = (int)w.size(0), a.io_dtype = dtype_code(h, "linear_cross_entropy"), a.reduction = reduction;
+    a.hidden = h.data_ptr(), a.weight = w.data_ptr(), a.targets = targets.data_ptr<int64_t>();
+    if (stats.defined()) a.stats = stats.data_ptr<float>();
+    a.status = ssd_status(h.get_device()).data_ptr<int32_t>();
+  }
+  Tensor scratch(ssm_linear_ce_args& a, bool backward) const {
+    Tensor s = at::empty({std::max<int64_t>(ssm_linear_ce_scratch_bytes(&a, backward), 256)}, h.options().dtype(at::kByte));
+    a.scratch = s.data_ptr();
+    return s;
+  }
+  variable_list forward(bool train) override {
+    c10::cuda::CUDAGuard guard(h.device());
+    ssd_poll(h.get_device());  // a wait that ran out in an earlier launch surfaces here, without a synchronisation
+    Tensor row_loss = at::empty(lead_shape, f32()), log_z = at::empty(lead_shape, f32()), loss;
+    if (train) stats = at::empty({std::max<int64_t>(rows(), 1), 2}, f32());
+    ssm_linear_ce_args a{};
+    fill(a);
+    const Tensor s = scratch(a, false);
+    a.row_loss = row_loss.data_ptr<float>(), a.log_z = log_z.data_ptr<float>();
+    if (reduction) loss = at::empty({}, f32()), a.loss = loss.data_ptr<float>();
+    run(ssm_linear_ce_fwd(&a, stream_of(h)));
+    variable_list res = {reduction ? loss : row_loss};
+    if (want_z) res.push_back(log_z);
+    return res;
+  }
+  variable_list backward(const variable_list& grads) override {
+    c10::cuda::CUDAGuard guard(h.device());
+    ssd_poll(h.get_device());
+    Tensor gl = grads[0].defined() ? f32c(grads[0]) : reduction ? at::zeros({}, f32()) : at::zeros(lead_shape, f32()), gz, dh, dw;
+    if (want_z && grads[1].defined()) gz = f32c(grads[1]);
+    if (grad_h) dh = at::empty(shape, h.options());
+    if (grad_w) dw = at::empty(w.sizes(), w.options().dtype(t_w));
+    ssm_linear_ce_bwd_args b{};
+    fill(b.fwd);
+    const Tensor s = scratch(b.fwd, true);
+    b.dloss = gl.data_ptr<float>(), b.dlog_z = gz.defined() ? gz.data_ptr<float>() : nullptr;
+    if (grad_h) b.dhidden = dh.data_ptr();
+    if (grad_w) b.dweight = dw.data_ptr(), b.dweight_dtype = dtype_code(dw, "linear_cross_entropy weight");
+    run(ssm_linear_ce_bwd(&b, stream_of(h)));
+    return {dh, dw, Tensor()};
+  }
+};
+py::object linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore, const std::string& reduction, bool want_z) {
+  ValueErrors scope;
+  const variable_list r = invoke_call(c10::make_intrusive<LinearCeCall>(hidden, weight, targets, ignore, reduction, want_z));
+  if (want_z) return py::make_tuple(r[0], r[1]);
+  return py::cast(r[0]);
+}
+
+// ---------------------------------------------------------------------------------------------
 // the norm over many tensors, and clipping by it
 // ---------------------------------------------------------------------------------------------
 struct TensorList {
@@ -196,6 +286,7 @@ Tensor clip_global_norm_(const std::vector<Tensor>& tensors, double max_norm, do
 void bind_training_operators(py::module& m) {
   auto ops = m.attr("operators").cast<py::module>();
   ops.def("fused_block_norm", &fused_block_norm);
+  ops.def("linear_cross_entropy", &linear_cross_entropy);
   ops.def("global_norm", &global_norm);
   ops.def("clip_global_norm_", &clip_global_norm_);
 }

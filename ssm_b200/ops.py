@@ -885,6 +885,20 @@ def fused_block_norm(
                 float(eps if post_eps is None else post_eps), bool(residual_in_fp32))
 
 
+def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore_index: int = -100, reduction: str = "none", return_log_z: bool = False):
+    """Extension: softmax cross entropy of a linear head, without its logits: ``hidden (..., D)``, ``weight (V, D)``, ``targets (...)`` integers; with
+    ``z = hidden weight^T`` returns ``log sum exp z - z[target]`` in fp32, per position (``reduction="none"``), summed, or as the mean over the positions that
+    count (0 without any), followed by ``log sum exp z (...)`` with ``return_log_z``.  Differentiable (once) with respect to ``hidden`` and ``weight``, whose gradients
+    have their types; ``weight`` is read in ``hidden``'s type.  Neither pass holds the logits: the backward pass forms their gradient again, at most 512 MB of it at a time.
+
+    A position whose target is ``ignore_index`` gives 0 (``log_z`` too) and no gradient, is not computed, and may hold anything.  Any other target outside of the vocabulary
+    makes its loss and the gradients NaN, as a hidden state that is not finite does.
+
+    16-bit operands are multiplied as they are with sums in 32 bits; the gradient with respect to the logits is rounded to their type before its two products (relative
+    to its largest weight in fp16).  fp32 operands are taken as sums of three bf16 numbers each, products below ``2**-24`` left out."""
+    return _run("linear_cross_entropy", hidden, weight, targets, int(ignore_index), str(reduction), bool(return_log_z))
+
+
 def _tensor_list(tensors, what: str) -> list:
     if torch._C._get_tracing_state() is not None:
         raise RuntimeError(f"{what} is not traced: it reads a list of tensors that a traced graph does not hold")
@@ -924,6 +938,7 @@ __all__ = [
     "token_log_probs",
     "topk_distill_loss",
     "fused_block_norm",
+    "linear_cross_entropy",
     "global_norm",
     "clip_global_norm_",
 ]

@@ -1,0 +1,298 @@
+"""``ops.linear_cross_entropy`` against its definition in 64 bits.
+
+Tolerances.  A logit is a sum of D products, each exact to 2^-24 or better, added in fp32 a few at a time: off by at most (D / 4 + 8) 2^-23 of the sum of the products' sizes, `dz`.  log Z is off by
+no more than the largest of these, and by the exponentials' 2^-22 and the sums' 2^-18; the loss by twice that.  An element of the logits' gradient is then off by
+p (2 dz + 2^-18) |w| and by half a step of the type it is rounded to (fp16: at least 2^-25 of 2^-13 of the largest weight; fp32: 2^-24), and its products with W and h carry that as sums of
+sizes, with (terms / 4 + 8) 2^-23 of the sums for the additions; half a step of the result's type ends it (2^-25 at least in fp16, whose numbers below 2^-14 are 2^-24 apart)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import training_oracle as oracle
+from ssm_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def make(n, d, v, dtype, seed=0, left_out=0.1, spread=2.5):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    h, w = rn(n, d).to(dtype), (spread / math.sqrt(d) * rn(v, d)).to(dtype)
+    t = torch.randint(0, v, (n,), device="cuda", generator=gen)
+    t = torch.where(torch.rand(n, device="cuda", generator=gen) < left_out, torch.full_like(t, -100), t)
+    return h, w, t, torch.rand(n, device="cuda", generator=gen) + 0.1, 0.3 * rn(n)
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def bounds(h, w, t, wl, wz):
+    """Values in 64 bits with how far each may be off: loss, log_z, dh, dw."""
+    dtype = h.dtype
+    kept = t != -100
+    h, w = h.detach().double(), w.detach().double()
+    h = torch.where(kept[:, None], h, torch.zeros((), dtype=torch.float64, device="cuda"))
+    wl, wz = wl.double() * kept, wz.double() * kept
+    at = torch.where(kept, t, torch.zeros_like(t))[:, None]
+    z = h @ w.t()
+    log_z = torch.logsumexp(z, -1)
+    loss = (log_z - torch.gather(z, 1, at)[:, 0]) * kept
+    d = h.shape[1]
+    dz = (d / 4 + 8) * 2.0 ** -23 * (h.abs() @ w.abs().t())
+    far = dz.amax(-1)
+    e_z = far + 2.0 ** -18 + 2.0 ** -23 * log_z.abs()
+    p = torch.exp(z - log_z[:, None])
+    g = p * (wl + wz)[:, None]
+    e = g.abs() * (2 * far + 2.0 ** -18)[:, None]
+    g.scatter_add_(1, at, -wl[:, None])
+    step = 2.0 ** -24 if dtype == torch.float32 else half(dtype)
+    e = e + step * (g.abs() + e)
+    if dtype == torch.float16:
+        e = e + 2.0 ** -38 * float(torch.maximum(wl.abs(), (wl + wz).abs()).amax()) * kept[:, None]
+    v, n = w.shape[0], h.shape[0]
+    out = []
+    for a, ea, b, terms in ((g, e, w, v), (g.t(), e.t(), h, n)):
+        val = a @ b
+        out.append((val, (ea + (terms / 4 + 8) * 2.0 ** -23 * a.abs()) @ b.abs() + half(dtype) * val.abs() + 1e-30))
+    return (loss, 2 * e_z * kept), (log_z * kept, e_z * kept), *out
+
+
+def near(got, want, tol, what):
+    assert got.shape == want.shape, what
+    err = (got.double() - want).abs()
+    tol = tol + torch.finfo(got.dtype).smallest_normal * half(got.dtype)
+    beyond = (want.abs() + tol >= torch.finfo(got.dtype).max) & got.isinf() & (got.double().sign() == want.sign())  # the type holds no more
+    err = torch.where(beyond, torch.zeros_like(err), err)
+    assert (err <= tol).all(), f"{what}: {float((err / tol.clamp(min=1e-30)).max())} of the tolerance"
+
+
+def check(h, w, t, wl, wz, **kw):
+    h, w = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss, log_z = ops.linear_cross_entropy(h, w, t, return_log_z=True, **kw)
+    dh, dw = torch.autograd.grad([loss, log_z], [h, w], [wl, wz])
+    want = bounds(h, w, t, wl, wz)
+    for got, (val, tol), what in zip((loss.detach(), log_z.detach(), dh, dw), want, ("loss", "log_z", "dh", "dw")):
+        near(got, val, tol, what)
+    assert dh.dtype == h.dtype and dw.dtype == w.dtype and loss.dtype == log_z.dtype == torch.float32
+    assert not dh[t == -100].any() and not loss[t == -100].any() and not log_z[t == -100].any()
+    with torch.no_grad():
+        assert torch.equal(ops.linear_cross_entropy(h, w, t, **kw), loss)
+    return dh, dw
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,v", [(1, 64, 256), (300, 64, 256), (256, 128, 512), (128, 1, 1), (7, 3, 5), (130, 100, 1000), (257, 65, 257), (1000, 320, 5003), (1, 768, 50277), (513, 260, 2049)])
+def test_sizes(dtype, n, d, v):
+    check(*make(n, d, v, dtype, left_out=0.0 if n == 1 else 0.1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_several_pieces_of_the_backward_pass(dtype):
+    v = 151936  # 512 MB hold 1766 such rows in 16 bits
+    check(*make(2000 if dtype != torch.float32 else 600, 64, v, dtype))
+
+
+def test_more_rows_than_one_piece_of_the_forward_pass():
+    check(*make(16384 + 300, 32, 300, torch.bfloat16))
+
+
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_reductions(reduction, dtype):
+    h, w, t, _, wz = make(500, 96, 700, dtype)
+    share = 3.0 / (1 if reduction == "sum" else int((t != -100).sum()))
+    want = bounds(h, w, t, torch.full((500,), share, device="cuda"), wz)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    loss, log_z = ops.linear_cross_entropy(h, w, t, reduction=reduction, return_log_z=True)
+    dh, dw = torch.autograd.grad([loss, log_z], [h, w], [torch.full((), 3.0, device="cuda"), wz])
+    total, tol = want[0][0].sum() * share / 3, want[0][1].sum() * share / 3
+    near(loss.detach(), total, tol + 2.0 ** -24 * total.abs(), "loss")
+    # the row's weight is one fp32 division more
+    near(dh, want[2][0], want[2][1] + 2.0 ** -23 * want[2][0].abs(), "dh")
+    near(dw, want[3][0], want[3][1] + 2.0 ** -23 * want[3][0].abs(), "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_left_out_may_hold_anything(dtype):
+    h, w, t, wl, wz = make(400, 96, 600, dtype, left_out=0.5)
+    want = check(h, w, t, wl, wz)
+    h = torch.where((t == -100)[:, None], torch.full_like(h, math.nan), h)
+    h[(t == -100).nonzero()[0, 0]] = math.inf
+    got = check(h, w, t, wl, wz)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("rows", [0, 5, 300])
+def test_nothing_counts(rows):
+    h, w, t, _, _ = make(max(rows, 1), 64, 300, torch.bfloat16)
+    h, t = h[:rows].requires_grad_(True), torch.full((rows,), -100, device="cuda")
+    w.requires_grad_(True)
+    for reduction in ("none", "sum", "mean"):
+        loss = ops.linear_cross_entropy(h, w, t, reduction=reduction)
+        dh, dw = torch.autograd.grad(loss, [h, w], torch.ones_like(loss))
+        assert not loss.detach().any() and not dh.any() and not dw.any() and dh.shape == h.shape
+
+
+def test_the_first_and_last_row_and_column():
+    h, w, t, wl, wz = make(512, 64, 513, torch.bfloat16, left_out=0.0)
+    t[0], t[1], t[255], t[256], t[511] = 0, 512, 511, 256, 255
+    check(h, w, t, wl, wz)
+    t[1:] = -100
+    check(h, w, t, wl, wz)
+    t[:], t[511] = -100, 512
+    check(h, w, t, wl, wz)
+
+
+def test_other_ignore_index_and_integer_types():
+    h, w, t, wl, wz = make(100, 64, 300, torch.float16)
+    want = ops.linear_cross_entropy(h, w, t)
+    for kind in (torch.int32, torch.int16):
+        assert torch.equal(ops.linear_cross_entropy(h, w, t.to(kind)), want)
+    moved = torch.where(t == -100, torch.full_like(t, 7), torch.where(t == 7, torch.full_like(t, 8), t))
+    got = ops.linear_cross_entropy(h, w, moved, ignore_index=7)
+    assert not got[t == -100].any() and torch.equal(got[(t != -100) & (t != 7)], want[(t != -100) & (t != 7)])
+
+
+def test_targets_outside_and_values_that_are_not_finite():
+    h, w, t, wl, wz = make(300, 64, 400, torch.bfloat16, left_out=0.0)
+    clean = ops.linear_cross_entropy(h, w, t)
+    t2 = t.clone()
+    t2[5], t2[6], t2[7] = 400, -1, 2 ** 40
+    h2 = h.clone()
+    h2[9, 3], h2[10, 0] = math.nan, math.inf
+    hl = h2.requires_grad_(True)
+    loss = ops.linear_cross_entropy(hl, w, t2)
+    bad = torch.zeros(300, dtype=torch.bool, device="cuda")
+    bad[[5, 6, 7, 9, 10]] = True
+    assert loss[bad].isnan().all() and torch.equal(loss[~bad], clean[~bad])
+    dh = torch.autograd.grad(loss, hl, wl)[0]
+    assert dh[bad].isnan().all() and dh[~bad].isfinite().all()
+
+
+@pytest.mark.parametrize("spread", [0.0, 40.0, 3000.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_flat_and_steep_distributions(spread, dtype):
+    check(*make(200, 128, 900, dtype, spread=spread))
+
+
+@pytest.mark.parametrize("scale", [1e-4, 1.0, 65536.0])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_small_and_large_weights_of_rows(scale, dtype):
+    h, w, t, wl, wz = make(200, 64, 300, dtype)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    dh = torch.autograd.grad(ops.linear_cross_entropy(h, w, t), h, scale * wl)[0]
+    val, tol = bounds(h, w, t, scale * wl, 0 * wz)[2]
+    near(dh, val, tol + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps, "dh")
+
+
+def test_strides_and_shapes():
+    h, w, t, _, _ = make(60, 72, 500, torch.bfloat16)
+    want = ops.linear_cross_entropy(h, w, t)
+    assert torch.equal(ops.linear_cross_entropy(h.view(4, 15, 72), w, t.view(4, 15)), want.view(4, 15))
+    wide = torch.randn(60, 200, device="cuda").to(torch.bfloat16)
+    wide[:, 5:77] = h
+    assert torch.equal(ops.linear_cross_entropy(wide[:, 5:77], w, t), want)
+    odd = torch.empty(500, 75, device="cuda", dtype=torch.bfloat16)
+    odd[:, 1:73] = w
+    assert torch.equal(ops.linear_cross_entropy(h, odd[:, 1:73], t), want)
+    assert torch.equal(ops.linear_cross_entropy(h.t().contiguous().t(), w.t().contiguous().t(), t), want)
+    same = ops.linear_cross_entropy(h[:1].expand(60, 72), w, t)
+    assert torch.equal(same, ops.linear_cross_entropy(h[:1].repeat(60, 1), w, t))
+    one = ops.linear_cross_entropy(h[0], w, t[0])
+    assert one.shape == () and torch.equal(one, want[0])
+    for shape in ((3, 20), (2, 3, 10)):
+        hl = h.view(*shape, 72).requires_grad_(True)
+        g = torch.autograd.grad(ops.linear_cross_entropy(hl, w, t.view(shape), reduction="sum"), hl)[0]
+        assert g.shape == hl.shape
+
+
+@pytest.mark.parametrize("wt", TYPES)
+def test_a_weight_of_another_type(wt):
+    h, w, t, wl, wz = make(150, 64, 300, torch.bfloat16)
+    w = w.to(wt).requires_grad_(True)
+    h = h.requires_grad_(True)
+    dh, dw = torch.autograd.grad(ops.linear_cross_entropy(h, w, t), [h, w], wl)
+    assert dw.dtype == wt
+    val, tol = bounds(h, w.to(torch.bfloat16), t, wl, 0 * wz)[3]
+    near(dw, val, tol + half(wt) * val.abs(), "dw")
+
+
+def test_only_one_gradient_is_wanted():
+    h, w, t, wl, _ = make(150, 64, 300, torch.bfloat16)
+    both = torch.autograd.grad(ops.linear_cross_entropy(h.requires_grad_(True), w.requires_grad_(True), t), [h, w], wl)
+    only_h = torch.autograd.grad(ops.linear_cross_entropy(h, w.detach(), t), h, wl)[0]
+    only_w = torch.autograd.grad(ops.linear_cross_entropy(h.detach(), w, t), w, wl)[0]
+    assert torch.equal(only_h, both[0]) and torch.equal(only_w, both[1])
+    loss, log_z = ops.linear_cross_entropy(h, w, t, reduction="mean", return_log_z=True)
+    g = torch.autograd.grad(log_z, h, wl)[0]
+    want = bounds(h, w, t, 0 * wl, wl)[2]
+    near(g, *want, "dh of log_z alone")
+
+
+def test_gradients_against_differences():
+    """Central differences of the 64-bit definition, in random directions."""
+    h, w, t, wl, _ = make(20, 24, 50, torch.float32)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    dh, dw = torch.autograd.grad((ops.linear_cross_entropy(h, w, t) * wl).sum(), [h, w])
+    f = lambda a, b: (oracle.linear_cross_entropy(a, b, t) * wl.double()).sum()  # noqa: E731
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for i, g in ((0, dh), (1, dw)):
+        x = [h.detach().double(), w.detach().double()]
+        dir = torch.randn(x[i].shape, device="cuda", generator=gen, dtype=torch.float64)
+        up, down = list(x), list(x)
+        up[i], down[i] = x[i] + 1e-5 * dir, x[i] - 1e-5 * dir
+        want = float((f(*up) - f(*down)) / 2e-5)
+        assert abs(float((g.double() * dir).sum()) - want) < 1e-4 * (1 + abs(want))
+
+
+def test_repeats_streams_and_graphs_give_the_same_bits():
+    h, w, t, wl, _ = make(700, 128, 1500, torch.bfloat16)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+
+    def once():
+        loss = ops.linear_cross_entropy(h, w, t, reduction="mean")
+        return [loss.detach(), *torch.autograd.grad(loss, [h, w])]
+
+    want = once()
+    for a, b in zip(once(), want):
+        assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = once()
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for _ in range(2):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+    t.copy_(torch.where(torch.arange(700, device="cuda") < 400, torch.full_like(t, -100), t))  # other rows count now
+    graph.replay()
+    for a, b in zip(out, once()):
+        assert torch.equal(a, b)
+
+
+def test_an_edit_between_the_passes_and_second_derivatives_are_errors():
+    h, w, t, wl, _ = make(50, 64, 100, torch.bfloat16)
+    h.requires_grad_(True)
+    loss = ops.linear_cross_entropy(h, w, t)
+    w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified in place"):
+        loss.sum().backward()
+    g = torch.autograd.grad(ops.linear_cross_entropy(h, w, t).sum(), h, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.sum().backward()
