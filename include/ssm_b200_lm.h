@@ -242,11 +242,14 @@ int ssm_block_norm_bwd(const ssm_block_norm_bwd_args* args, ssm_stream_t stream)
  * Cross entropy from hidden states: z = hidden weight^T, log_z[r] = ln sum_v exp z[r, v], loss[r] = log_z[r] - z[r, targets[r]], without a (rows, vocab) matrix.
  * hidden (rows, dim), weight (vocab, dim) of io_dtype, rows at their strides.  A row whose target is ignore_index costs nothing, is not read and gives 0; any other target outside
  * of the vocabulary gives a loss of NaN.  row_loss and log_z (rows) fp32; loss, with reduction 1 (sum) or 2 (mean over the rows that count, 0 without any), one float.
- * stats (rows, 2) fp32 keeps what the backward pass needs (nullable).  status: a word in host memory that the device writes, set where a bounded wait ran out.
+ * stats (rows, 4) fp32, 16-byte aligned, keeps what the backward pass needs (nullable).  status: a word in host memory that the device writes, set where a bounded wait ran out.
  *
  * Backward: from dloss (rows, or one float with a reduction) and dlog_z (rows, nullable) writes dhidden (rows, dim; io_dtype) and dweight (vocab, dim; dweight_dtype),
  * dense, each nullable, via pieces of at most SSM_LINEAR_CE_PIECE_BYTES of the logits' gradient in 16 bits.
- * scratch: ssm_linear_ce_scratch_bytes(args, backward) bytes, 256-byte aligned.
+ * scratch: ssm_linear_ce_scratch_bytes(args, pass) bytes, 256-byte aligned; pass 0 forward, 1 backward, 2 both at once.
+ *
+ * ssm_linear_ce_train, for bf16 with a reduction: the forward pass and, for a dloss that is known later, dhidden (rows, dim) and dweight (vocab, dim rounded up to a multiple of
+ * 4) in fp32, 16-byte aligned, each nullable; kept: three words.  ssm_linear_ce_scale then multiplies either, (rows, dim) at the row stride ld, by dloss and what `kept` holds.
  * ------------------------------------------------------------------------------------- */
 #define SSM_LINEAR_CE_PIECE_BYTES (512 << 20)
 typedef struct {
@@ -272,9 +275,11 @@ typedef struct {
   int32_t dweight_dtype, reserved0;
 } ssm_linear_ce_bwd_args;
 
-int64_t ssm_linear_ce_scratch_bytes(const ssm_linear_ce_args* args, int32_t backward);
+int64_t ssm_linear_ce_scratch_bytes(const ssm_linear_ce_args* args, int32_t pass);
 int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t stream);
 int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_t stream);
+int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidden, float* dweight, float* kept, ssm_stream_t stream);
+int ssm_linear_ce_scale(const float* src, int64_t ld, int64_t rows, int32_t dim, const float* kept, const float* dloss, void* out, int32_t dtype, ssm_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * The norm over all elements of many tensors: sqrt(sum x^2), or max |x| with is_max, into *norm (device, fp32); NaN once there is one.  Clipping multiplies

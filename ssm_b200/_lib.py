@@ -287,6 +287,8 @@ ENTRY_POINTS = {
     "ssm_linear_ce_scratch_bytes": (C.c_int64, [C.POINTER(LinearCeArgs), i32]),
     "ssm_linear_ce_fwd": (C.c_int, [C.POINTER(LinearCeArgs), vp]),
     "ssm_linear_ce_bwd": (C.c_int, [C.POINTER(LinearCeBwdArgs), vp]),
+    "ssm_linear_ce_train": (C.c_int, [C.POINTER(LinearCeArgs), vp, vp, vp, vp]),
+    "ssm_linear_ce_scale": (C.c_int, [vp, i64, i64, i32, vp, vp, vp, i32, vp]),
     "ssm_global_norm_scratch_bytes": (C.c_int64, [i64]),
     "ssm_global_norm": (C.c_int, [C.POINTER(TensorRef), i64, i32, vp, vp, vp]),
     "ssm_clip_global_norm": (C.c_int, [C.POINTER(TensorRef), i64, i32, C.c_float, vp, vp, vp]),

@@ -1,8 +1,15 @@
 // Cross entropy from hidden states and the head's weight, without the logits: z = h W^T, log Z = ln sum exp z, loss = log Z - z_t.
 //
 // Forward: one product whose tiles end in a row's maximum and sum of exponentials (of powers of two, 2^(c z - M), c = log2 e, M the maximum rounded up to a whole number); a second
-// kernel joins the tiles.  Backward, from w = dloss and wz = dlog_z of a row: G = p (w + wz) - [v = t] w, dh = G W, dW = G^T h.  G is formed again by the same product, a piece of the rows at a
-// time, rounded to the operands' type (its sums are held in 32 bits), and read by the two others: 2 + 6 N D V operations where 6 are the least.
+// kernel joins the tiles.  Backward, from w = dloss and wz = dlog_z of a row: G = p (w + wz), q = p_t (w + wz) - w; dh = G' W + q W_t, dW = G'^T h + sum q h at the targets' rows, with
+// G' = G but 0 at the target.  G' is formed again by the same product, a piece of the rows at a time, rounded to the operands' type, and read by the two others:
+// 2 + 6 N D V operations where 6 are the least.  q, as a rule the largest number of its row by far, keeps 32 bits and goes to the results apart (rounded into G it gave
+// most of the gradients' error: 0.31e-3 in fp16 where the result's own rounding is 0.21e-3).
+//
+// Loss and gradient in one pass, for sums and means in bf16: what the loss is multiplied by is one number, known later, and 6 N D V do.  The first product leaves
+// 2^(c z - M) in bf16 with M from the target's logit: bf16 reaches as far as fp32, so that any M within 2^60 of the maximum will do, and it needs not be known before.  A row's factor
+// 1 / sum goes to h for dW, and to the result for dh.  Rows whose maximum is further away are noticed when their tiles are joined, and their tiles formed again.
+//
 // Bound: the tensor cores; for few rows, reading W.
 //
 // Rows that are left out are not computed: the others are packed first, behind one another (which also gives the copies their alignment), and how many
@@ -10,9 +17,11 @@
 //
 // Products: pairs of CTAs (cta_group::2) on tiles of 256 x 256 (x 128 for narrow outputs), a CTA holding 128 rows of the accumulator; operands by TMA in the 128-byte swizzle, blocks of 64 x 64, two to
 // an operand, with K innermost (h, W, G as stored) or M / N innermost (G^T, W and h as the second factor).  One thread copies, one multiplies, eight
-// warps read an accumulator while the next one is formed.  fp32 operands are taken as sums of three bf16 numbers (24 bits of mantissa in all) and
+// warps read an accumulator while the next one is formed.  Logits, and all results in fp32, leave the accumulator every 512 terms and are added up by the warps that read it: the tensor core
+// cuts its sums off (4096 rows of 2560: the losses were off by 1.0e-6, 2.4e-7 so).  fp32 operands are taken as sums of three bf16 numbers (24 bits of mantissa in all) and
 // multiplied in six products, the smallest first; what is left out is below 2^-24.
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/ssm_b200_lm.h"
 #include "ssd_common.cuh"
@@ -28,29 +37,36 @@ constexpr float kFar = 268435456.f;    // M of a tile is no less than minus this
 constexpr int kPairs = 6;
 __constant__ const signed char kPlaneA[kPairs] = {2, 0, 1, 1, 0, 0}, kPlaneB[kPairs] = {0, 2, 1, 0, 1, 0};
 
-enum Epilogue { kStats = 0, kGrad = 1, kOut = 2 };
+enum Epilogue { kStats = 0, kGrad = 1, kOut = 2, kKeep = 3 };
+constexpr int kSegment = 8;            // blocks of K between two readings of an accumulator, where its sums have to keep 32 bits
+constexpr float kReach = 60.f;         // how far a row's maximum may be from the M of the one-pass form
 
-struct GemmArgs {
-  int m_tiles, n_tiles, splits, k_blocks, bn, m_inner;
+// one product: M x N in tiles, K in blocks of 64, cut into `splits`
+struct Job {
+  int m_tiles, n_tiles, splits, k_blocks, m_inner;
   int a_mn, b_mn;              // innermost axis of an operand: its M / N instead of K
   int a_m0, a_k0, b_k0;        // where the operands' rows begin
-  int planes, fmt;             // 3 for fp32; 0 fp16, 1 bf16
-  int row0, rows, k_is_rows;   // the packed rows of this call: its M, or its K
-  const int* count;            // packed rows in all
-  int32_t* status;
-  // kStats, kGrad
-  int vocab;
-  const int* targets;          // of packed rows; -1: outside of the vocabulary
-  float2* part;                // [128 columns][rows of this call]: M, sum 2^(c z - M)
-  int part_ld;
-  float* z_target;
-  const float4* row;           // of packed rows: M, 1 / s, w, w + wz
-  uint16_t* g;                 // [plane][row][ldg]
-  int64_t ldg, g_plane;
-  // kOut
-  float* out;                  // [split][row][ld]
+  int k_is_rows;               // the packed rows of the call are its K, not its M
+  float* out;                  // kOut: [split][row][ld]
   int64_t ld, out_split;
   int out_rows, add;
+};
+struct GemmArgs {
+  Job job[2];                  // kOut takes two; no tiles: none
+  int bn, fmt;                 // columns of a tile; 0 fp16, 1 bf16
+  int row0, rows;              // the packed rows of this call
+  const int* count;            // packed rows in all
+  int32_t* status;
+  // kStats, kGrad, kKeep
+  int vocab;
+  const int* targets;          // of packed rows; -1: outside of the vocabulary
+  float2* part;                // [128 columns][rows of this call]: M, sum 2^(c z - M); kKeep: the maximum, the sum
+  int part_ld;
+  float* z_target;
+  const float4* row;           // of packed rows: M, 1 / s, w + wz, q; kKeep: M
+  uint16_t* g;                 // [plane][row][ldg]
+  int64_t ldg, g_plane;
+  const int* again;            // kKeep, nullable: the tiles of rows to be formed again
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -126,12 +142,12 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 }
 
 struct TileAt {
-  int m, n, split, kb0, kb1;
+  int job, m, n, split, kb0, kb1;  // job -1: no more
 };
 
 template <int EPI, typename T, int PLANES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ GemmArgs g) {
+    gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mb1, const __grid_constant__ GemmArgs g) {
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
   __shared__ uint32_t tmem_slot;
@@ -141,9 +157,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t ring = (tc::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t full = tc::smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16;
   const int live = min(g.rows, max(0, *g.count - g.row0));
-  const int m_tiles = g.k_is_rows ? g.m_tiles : (live + kTile - 1) / kTile, k_blocks = g.k_is_rows ? (live + kK - 1) / kK : g.k_blocks;
-  const int tiles = live > 0 ? m_tiles * g.n_tiles * g.splits : 0;
   constexpr int kProducts = PLANES == 1 ? 1 : kPairs;
+  constexpr bool kSegments = EPI != kOut || PLANES > 1;
+
+  // This pair's k-th tile.  The first job's tiles (long ones) go round the pairs; pairs that have one less of them take as many rounds of the second job's alone as fit into
+  // its time, then all take turns: the tiles that run at one time stay neighbours, and share operands in the L2.
+  const int m0 = (live + kTile - 1) / kTile, kb_rows = (live + kK - 1) / kK;
+  const int tiles0 = live > 0 ? (g.job[0].k_is_rows ? g.job[0].m_tiles : min(g.job[0].m_tiles, m0)) * g.job[0].n_tiles * g.job[0].splits : 0;
+  const int tiles1 = EPI == kOut && live > 0 ? (g.job[1].k_is_rows ? g.job[1].m_tiles : min(g.job[1].m_tiles, m0)) * g.job[1].n_tiles * g.job[1].splits : 0;
+  const int extra = tiles0 % pairs, mine0 = tiles0 / pairs + (pair < extra ? 1 : 0);
+  const int alone = EPI == kOut && extra ? g.job[0].k_blocks / g.job[0].splits / max(1, g.job[1].k_is_rows ? kb_rows : g.job[1].k_blocks) : 0;
+  auto place = [&](int k) {
+    TileAt p;
+    int t;
+    p.job = 0;
+    if (k < mine0) {
+      t = pair + k * pairs;
+    } else {
+      if (EPI != kOut) {
+        p.job = -1;
+        return p;
+      }
+      k -= mine0;
+      if (pair < extra) t = alone * (pairs - extra) + k * pairs + pair;
+      else if (k < alone) t = k * (pairs - extra) + pair - extra;
+      else t = alone * (pairs - extra) + (k - alone) * pairs + pair;
+      p.job = t < tiles1 ? 1 : -1;
+      if (p.job < 0) return p;
+    }
+    const Job& j = g.job[p.job];
+    const int m_tiles = j.k_is_rows ? j.m_tiles : min(j.m_tiles, m0), k_blocks = j.k_is_rows ? kb_rows : j.k_blocks, per = m_tiles * j.n_tiles;
+    p.split = t / per, t -= p.split * per;
+    if (j.m_inner) p.m = t % m_tiles, p.n = t / m_tiles;
+    else p.n = t % j.n_tiles, p.m = t / j.n_tiles;
+    p.kb0 = (int)((int64_t)k_blocks * p.split / j.splits), p.kb1 = (int)((int64_t)k_blocks * (p.split + 1) / j.splits);
+    if (EPI == kKeep && g.again != nullptr && !g.again[p.m]) p.kb1 = p.kb0;  // nothing to do
+    return p;
+  };
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) tc::mbar_init(full + 8 * s, 1), tc::mbar_init(empty + 8 * s, 1);
@@ -164,15 +214,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gave_up = 1;
     *reinterpret_cast<volatile int32_t*>(g.status) = kStatus;
   };
-  auto place = [&](int t) {
-    TileAt p;
-    const int per = m_tiles * g.n_tiles;
-    p.split = t / per, t -= p.split * per;
-    if (g.m_inner) p.m = t % m_tiles, p.n = t / m_tiles;
-    else p.n = t % g.n_tiles, p.m = t / g.n_tiles;
-    p.kb0 = (int)((int64_t)k_blocks * p.split / g.splits), p.kb1 = (int)((int64_t)k_blocks * (p.split + 1) / g.splits);
-    return p;
-  };
 
   if (warp == 0) {
     if (tc::elect_one()) {  // copies
@@ -180,24 +221,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t full0 = leader_address(full);
       int it = 0;
       bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        const TileAt p = place(t);
-        const int am = g.a_m0 + p.m * kTile + rank * 128, bn = p.n * g.bn + rank * half;
-        for (int q = 0; q < kProducts && ok; ++q) {
-          const int pa = PLANES == 1 ? 0 : kPlaneA[q], pb = PLANES == 1 ? 0 : kPlaneB[q];
-          for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
-            const int s = it % kStages, round = it / kStages;
-            if (round > 0 && !tc::mbar_wait(empty + 8 * s, (round - 1) & 1)) {
-              ran_out();
-              ok = false;
-              break;
-            }
-            if (rank == 0) tc::mbar_expect_tx(full + 8 * s, bytes);
-            const uint32_t at = ring + s * kStageBytes, bar = full0 + 8 * s;
-            const int ka = g.a_k0 + kb * kK, kb_at = g.b_k0 + kb * kK;
+      for (int k = 0; ok; ++k) {
+        const TileAt p = place(k);
+        if (p.job < 0) break;
+        const Job& j = g.job[p.job];
+        const CUtensorMap* const map_b = EPI == kOut && p.job ? &mb1 : &mb;
+        const int am = j.a_m0 + p.m * kTile + rank * 128, bn = p.n * g.bn + rank * half;
+        for (int seg = p.kb0; seg < p.kb1 && ok; seg += kSegment) {
+          const int end = min(seg + kSegment, p.kb1);
+          for (int q = 0; q < kProducts && ok; ++q) {
+            const int pa = PLANES == 1 ? 0 : kPlaneA[q], pb = PLANES == 1 ? 0 : kPlaneB[q];
+            for (int kb = seg; kb < end; ++kb, ++it) {
+              const int s = it % kStages, round = it / kStages;
+              if (round > 0 && !tc::mbar_wait(empty + 8 * s, (round - 1) & 1)) {
+                ran_out();
+                ok = false;
+                break;
+              }
+              if (rank == 0) tc::mbar_expect_tx(full + 8 * s, bytes);
+              const uint32_t at = ring + s * kStageBytes, bar = full0 + 8 * s;
+              const int ka = j.a_k0 + kb * kK, kb_at = j.b_k0 + kb * kK;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) load_box(at + j * kBoxBytes, &ma, bar, g.a_mn ? am + 64 * j : ka, g.a_mn ? ka : am + 64 * j, pa);
-            for (int j = 0; j < half / 64; ++j) load_box(at + (2 + j) * kBoxBytes, &mb, bar, g.b_mn ? bn + 64 * j : kb_at, g.b_mn ? kb_at : bn + 64 * j, pb);
+              for (int i = 0; i < 2; ++i) load_box(at + i * kBoxBytes, &ma, bar, j.a_mn ? am + 64 * i : ka, j.a_mn ? ka : am + 64 * i, pa);
+              for (int i = 0; i < half / 64; ++i) load_box(at + (2 + i) * kBoxBytes, map_b, bar, j.b_mn ? bn + 64 * i : kb_at, j.b_mn ? kb_at : bn + 64 * i, pb);
+            }
           }
         }
       }
@@ -210,36 +257,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && tc::elect_one()) {  // products
-      const uint32_t idesc = tc::instr_desc(kTile, g.bn, g.fmt, g.a_mn, g.b_mn);
-      const uint32_t a_lbo = g.a_mn ? kBoxBytes : 16, b_lbo = g.b_mn ? kBoxBytes : 16;
-      const int a_step = g.a_mn ? 128 : 2, b_step = g.b_mn ? 128 : 2;
       int it = 0, n = 0;
       bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs, ++n) {
-        const TileAt p = place(t);
-        const int b = n & 1;
-        if (n >= 2 && !tc::mbar_wait(tempty + 8 * b, ((n >> 1) - 1) & 1)) {
-          ran_out();
-          break;
-        }
-        tc::fence_after_sync();
-        const uint32_t d = tmem + b * 256;
-        const int steps = (p.kb1 - p.kb0) * kProducts;
-        for (int i = 0; i < steps; ++i, ++it) {
-          const int s = it % kStages;
-          if (!tc::mbar_wait(full + 8 * s, (it / kStages) & 1)) {
+      for (int k = 0; ok; ++k) {
+        const TileAt p = place(k);
+        if (p.job < 0) break;
+        const Job& j = g.job[p.job];
+        const uint32_t idesc = tc::instr_desc(kTile, g.bn, g.fmt, j.a_mn, j.b_mn);
+        const uint32_t a_lbo = j.a_mn ? kBoxBytes : 16, b_lbo = j.b_mn ? kBoxBytes : 16;
+        const int a_step = j.a_mn ? 128 : 2, b_step = j.b_mn ? 128 : 2;
+        const int length = kSegments ? kSegment : p.kb1 - p.kb0;
+        for (int seg = p.kb0; seg < p.kb1 && ok; seg += length, ++n) {
+          const int b = n & 1, steps = (min(seg + length, p.kb1) - seg) * kProducts;
+          if (n >= 2 && !tc::mbar_wait(tempty + 8 * b, ((n >> 1) - 1) & 1)) {
             ran_out();
             ok = false;
             break;
           }
           tc::fence_after_sync();
-          const uint32_t at = ring + s * kStageBytes;
-          const uint64_t da = tc::smem_desc_sw128(at, a_lbo, 1024), db = tc::smem_desc_sw128(at + 2 * kBoxBytes, b_lbo, 1024);
+          const uint32_t d = tmem + b * 256;
+          for (int i = 0; i < steps; ++i, ++it) {
+            const int s = it % kStages;
+            if (!tc::mbar_wait(full + 8 * s, (it / kStages) & 1)) {
+              ran_out();
+              ok = false;
+              break;
+            }
+            tc::fence_after_sync();
+            const uint32_t at = ring + s * kStageBytes;
+            const uint64_t da = tc::smem_desc_sw128(at, a_lbo, 1024), db = tc::smem_desc_sw128(at + 2 * kBoxBytes, b_lbo, 1024);
 #pragma unroll
-          for (int kk = 0; kk < kK / 16; ++kk) mma_pair(d, da + kk * a_step, db + kk * b_step, idesc, i > 0 || kk > 0);
-          commit_pair(empty + 8 * s);
+            for (int kk = 0; kk < kK / 16; ++kk) mma_pair(d, da + kk * a_step, db + kk * b_step, idesc, i > 0 || kk > 0);
+            commit_pair(empty + 8 * s);
+          }
+          if (ok) commit_pair(tfull + 8 * b);
         }
-        if (ok) commit_pair(tfull + 8 * b);
       }
     }
     __syncwarp();
@@ -248,114 +300,168 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int half = (warp - 4) >> 2, row_in = rank * 128 + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     int n = 0;
-    for (int t = pair; t < tiles; t += pairs, ++n) {
-      const TileAt p = place(t);
-      const int b = n & 1;
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(tfull + 8 * b, (n >> 1) & 1))) {
-        if (lane == 0) ran_out();
-        break;
-      }
+    bool ok = true;
+    auto arrived = [&](int b) {
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(tfull + 8 * b, (n >> 1) & 1));
+      if (!ok && lane == 0) ran_out();
       tc::fence_after_sync();
-      const uint32_t from = tmem + lanes + b * 256 + half * (g.bn / 2);
-      const int row = p.m * kTile + row_in;
-      if constexpr (EPI == kOut) {
-        float* out = g.out + p.split * g.out_split + row * g.ld + p.n * g.bn + half * (g.bn / 2);
-        const int cols = (int)min((int64_t)(g.bn / 2), g.ld - p.n * g.bn - half * (g.bn / 2));
-        for (int c = 0; c < g.bn / 2; c += 32) {
+      return ok;
+    };
+    auto release = [&](int b) {
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_at(tempty0 + 8 * b);
+    };
+    for (int k = 0; ok; ++k) {
+      const TileAt p = place(k);
+      if (p.job < 0) break;
+      if (p.kb0 == p.kb1 && EPI == kKeep) continue;
+      const Job& j = g.job[p.job];
+      const int row = p.m * kTile + row_in, width = g.bn / 2;
+      const int64_t out_col = p.n * g.bn + half * width;
+      if constexpr (!kSegments) {
+        const int b = n & 1;
+        if (!arrived(b)) break;
+        const uint32_t from = tmem + lanes + b * 256 + half * width;
+        float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
+        const int cols = (int)min((int64_t)width, j.ld - out_col);
+        for (int c = 0; c < width; c += 32) {
           uint32_t v[32];
           tmem_ld32_issue(from + c, v);
           tmem_wait_ld();
-          if (row < g.out_rows) {
+          if (row < j.out_rows) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              if (c + j < cols) {
-                if (g.add) asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"l"(out + c + j), "f"(__uint_as_float(v[j])), "f"(__uint_as_float(v[j + 1])),
-                                        "f"(__uint_as_float(v[j + 2])), "f"(__uint_as_float(v[j + 3]))
+            for (int i = 0; i < 32; i += 4) {
+              if (c + i < cols) {
+                if (j.add) asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"l"(out + c + i), "f"(__uint_as_float(v[i])), "f"(__uint_as_float(v[i + 1])),
+                                        "f"(__uint_as_float(v[i + 2])), "f"(__uint_as_float(v[i + 3]))
                                         : "memory");
-                else *reinterpret_cast<uint4*>(out + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                else *reinterpret_cast<uint4*>(out + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
               }
             }
           }
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) arrive_at(tempty0 + 8 * b);
+        release(b);
+        ++n;
       } else {
         uint32_t v[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_issue(from + 32 * c, v[c]);
-        tmem_wait_ld();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) arrive_at(tempty0 + 8 * b);
-        const int col0 = p.n * kTile + half * 128, left = g.vocab - col0;
-        const bool in = row < live;
-        const int at = in ? g.targets[g.row0 + row] - col0 : -1;  // the target's column here
-        if constexpr (EPI == kStats) {
-          float m = -INFINITY, s = 0.f;
-          if (left < 128) {
+        for (int seg = p.kb0; seg < p.kb1 && ok; seg += kSegment, ++n) {
+          const int b = n & 1;
+          if (!arrived(b)) break;
+          const uint32_t from = tmem + lanes + b * 256 + half * width;
+          if (seg == p.kb0) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
+              if (32 * c < width) tmem_ld32_issue(from + 32 * c, v[c]);
+            tmem_wait_ld();
+          } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (32 * c + j >= left) v[c][j] = 0xff800000u;
+            for (int c = 0; c < 8; ++c) {
+              if (16 * c < width) {
+                float w[16];
+                tc::tmem_ld16(from + 16 * c, w);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[c / 2][c % 2 * 16 + i] = __float_as_uint(__uint_as_float(v[c / 2][c % 2 * 16 + i]) + w[i]);
+              }
+            }
           }
+          release(b);
+        }
+        if (!ok) break;
+        if constexpr (EPI == kOut) {
+          float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
+          const int cols = (int)min((int64_t)width, j.ld - out_col);
+          if (row < j.out_rows) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) m = fmaxf(m, __uint_as_float(v[c][j]));
-          const float M = fmaxf(ceilf(m * kLog2e), -kFar);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s += ex2_approx(fmaf(__uint_as_float(v[c][j]), kLog2e, -M));
-          if (in) {
-            g.part[(int64_t)(p.n * 2 + half) * g.part_ld + row] = make_float2(M, s);
-            if (at >= 0 && at < 128) {
-              float z = 0.f;
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int j = 0; j < 32; ++j) z = 32 * c + j == at ? __uint_as_float(v[c][j]) : z;
-              g.z_target[g.row0 + row] = z;
+            for (int i = 0; i < 128; i += 4) {
+              if (i < cols) {
+                float4 w = make_float4(__uint_as_float(v[i / 32][i % 32]), __uint_as_float(v[i / 32][i % 32 + 1]), __uint_as_float(v[i / 32][i % 32 + 2]), __uint_as_float(v[i / 32][i % 32 + 3]));
+                float4* to = reinterpret_cast<float4*>(out + i);
+                if (j.add) {
+                  const float4 o = *to;
+                  w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
+                }
+                *to = w;
+              }
             }
           }
         } else {
-          float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (in) r = g.row[g.row0 + row];
-          uint16_t* to = g.g + row * g.ldg + col0;
-          const int room = (int)min((int64_t)128, g.ldg - col0);
+          const int col0 = p.n * kTile + half * 128, left = g.vocab - col0;
+          const bool in = row < live;
+          const int at = in ? g.targets[g.row0 + row] - col0 : -1;  // the target's column here
+          if constexpr (EPI == kStats) {
+            float m = -INFINITY, s = 0.f;
+            if (left < 128) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+              for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float e = ex2_approx(fmaf(__uint_as_float(v[c][j]), kLog2e, -r.x)) * r.y;
-              float x = e * r.w;
-              if (32 * c + j == at) x -= r.z;
-              v[c][j] = in && 32 * c + j < left ? __float_as_uint(x) : 0u;
+                for (int i = 0; i < 32; ++i)
+                  if (32 * c + i >= left) v[c][i] = 0xff800000u;
             }
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (32 * c + j < room) {
-                if constexpr (PLANES == 1) {
-                  uint32_t w[4];
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                  for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(v[c][j + 2 * k]), __uint_as_float(v[c][j + 2 * k + 1]));
-                  *reinterpret_cast<uint4*>(to + 32 * c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int i = 0; i < 32; ++i) m = fmaxf(m, __uint_as_float(v[c][i]));
+            const float M = fmaxf(ceilf(m * kLog2e), -kFar);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s += ex2_approx(fmaf(__uint_as_float(v[c][i]), kLog2e, -M));
+            if (in) {
+              g.part[(int64_t)(p.n * 2 + half) * g.part_ld + row] = make_float2(M, s);
+              if (at >= 0 && at < 128) {
+                float z = 0.f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) z = 32 * c + i == at ? __uint_as_float(v[c][i]) : z;
+                g.z_target[g.row0 + row] = z;
+              }
+            }
+          } else {
+            float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (in) r = g.row[g.row0 + row];
+            uint16_t* to = g.g + row * g.ldg + col0;
+            const int room = (int)min((int64_t)128, g.ldg - col0);
+            float m = -INFINITY, s = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float z = __uint_as_float(v[c][i]);
+                const bool is = in && 32 * c + i < left;
+                float e = ex2_approx(fmaf(z, kLog2e, -r.x));
+                if constexpr (EPI == kKeep) {
+                  if (is) m = fmaxf(m, z), s += e;
                 } else {
-                  __nv_bfloat16 e[8][3];
+                  e = e * r.y * r.z;
+                }
+                v[c][i] = is && 32 * c + i != at ? __float_as_uint(e) : 0u;
+              }
 #pragma unroll
-                  for (int k = 0; k < 8; ++k) split3(__uint_as_float(v[c][j + k]), e[k]);
-#pragma unroll
-                  for (int q = 0; q < 3; ++q) {
+              for (int i = 0; i < 32; i += 8) {
+                if (32 * c + i < room) {
+                  if constexpr (PLANES == 1) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__bfloat16_as_ushort(e[2 * k][q]) | (uint32_t)__bfloat16_as_ushort(e[2 * k + 1][q]) << 16;
-                    *reinterpret_cast<uint4*>(to + q * g.g_plane + 32 * c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int q = 0; q < 4; ++q) w[q] = pack2<T>(__uint_as_float(v[c][i + 2 * q]), __uint_as_float(v[c][i + 2 * q + 1]));
+                    *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                  } else {
+                    __nv_bfloat16 e[8][3];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) split3(__uint_as_float(v[c][i + q]), e[q]);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                      uint32_t w[4];
+#pragma unroll
+                      for (int h = 0; h < 4; ++h) w[h] = (uint32_t)__bfloat16_as_ushort(e[2 * h][q]) | (uint32_t)__bfloat16_as_ushort(e[2 * h + 1][q]) << 16;
+                      *reinterpret_cast<uint4*>(to + q * g.g_plane + 32 * c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                   }
                 }
               }
             }
+            if (EPI == kKeep && in) g.part[(int64_t)(p.n * 2 + half) * g.part_ld + row] = make_float2(m, s);
           }
         }
       }
@@ -465,7 +571,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
 
 // The tiles of a row joined: 32 rows of a call to a block, eight slices of the columns.
 __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
-                                                   const int* __restrict__ targets, const float* __restrict__ z_target, float2* __restrict__ stats, float* __restrict__ row_loss,
+                                                   const int* __restrict__ targets, const float* __restrict__ z_target, float4* __restrict__ stats, float* __restrict__ row_loss,
                                                    float* __restrict__ log_z) {
   __shared__ float2 slices[8][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
@@ -493,12 +599,96 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ pa
       M = top;
     }
     const int r = row0 + row, t = targets[r], out = idx[r];
-    stats[r] = make_float2(M, s);
-    const float ln_s = logf(s);
-    // log Z - z_t as differences from M, which take no bits from a small loss
-    const float z = z_target[r];
-    row_loss[out] = t < 0 ? NAN : ln_s - kLn2 * fmaf(z, kLog2e, -M);
+    const float ln_s = logf(s), z = t < 0 ? NAN : z_target[r];
+    stats[r] = make_float4(M, s, z, 0.f);
+    row_loss[out] = ln_s - kLn2 * fmaf(z, kLog2e, -M);  // log Z - z_t as differences from M, which take no bits from a small loss
     log_z[out] = fmaf(M, kLn2, ln_s);
+  }
+}
+
+// ---- loss and gradient in one pass: the target's logit of packed rows, which M comes from
+__global__ void __launch_bounds__(256) reference_kernel(const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w, int64_t ldh, int64_t ldw, int dim, const int* __restrict__ targets,
+                                                        const int* __restrict__ count, int row0, int rows, float* __restrict__ z_target, float4* __restrict__ row, int* __restrict__ again) {
+  const int i = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31, r = row0 + i;
+  if (i >= rows) return;
+  if (lane == 0 && i % kTile == 0) again[i / kTile] = 0;
+  if (r >= *count) return;
+  const int t = targets[r];
+  const __nv_bfloat16 *a = h + r * ldh, *b = w + (int64_t)max(t, 0) * ldw;
+  float z = 0.f;
+  for (int c = lane * 8; c < dim; c += 256) {
+    if (c + 8 <= dim) {
+      Vec16<__nv_bfloat16> x, y;
+      float f[8], e[8];
+      x.load(a + c), y.load(b + c);
+      x.unpack(f), y.unpack(e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z = fmaf(f[k], e[k], z);
+    } else {
+      for (int k = c; k < dim; ++k) z = fmaf(__bfloat162float(a[k]), __bfloat162float(b[k]), z);
+    }
+  }
+  z = warp_sum(z);
+  if (lane == 0) {
+    const float M = t < 0 || !(fabsf(z) < 1e30f) ? 0.f : ceilf(z * kLog2e);
+    z_target[r] = t < 0 ? NAN : z;
+    row[r] = make_float4(M, 0.f, 0.f, 0.f);
+  }
+}
+// Its tiles joined.  A row whose maximum is too far from M gets one from its maximum, and its tile of rows is formed again; the second call (`second`) then joins those.
+__global__ void __launch_bounds__(256) join_keep_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
+                                                        const float* __restrict__ z_target, float4* __restrict__ row, int* __restrict__ again, int second, float* __restrict__ row_loss,
+                                                        float* __restrict__ log_z) {
+  __shared__ float2 slices[8][32];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+  const int live = min(rows, *count - row0);
+  if ((int)blockIdx.x * 32 >= live || (second && !again[blockIdx.x * 32 / kTile])) return;
+  float m = -INFINITY, s = 0.f;
+  if (i < live) {
+#pragma unroll 4
+    for (int p = slice; p < parts; p += 8) {
+      const float2 v = part[(int64_t)p * ld + i];
+      m = fmaxf(m, v.x), s += v.y;
+    }
+  }
+  slices[slice][lane] = make_float2(m, s);
+  __syncthreads();
+  if (slice == 0 && i < live) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) m = fmaxf(m, slices[w][lane].x), s += slices[w][lane].y;
+    const int r = row0 + i, out = idx[r];
+    const float z = z_target[r], top = ceilf(m * kLog2e);
+    float4 v = row[r];
+    if (!second && fabsf(top) < 1e30f && fabsf(top - v.x) > kReach) {
+      again[i / kTile] = 1;
+      row[r] = make_float4(top, 0.f, 0.f, 0.f);
+      return;
+    }
+    const float d = fmaf(z, kLog2e, -v.x), inv = s < INFINITY ? 1.f / s : NAN, ln_s = s < INFINITY ? logf(s) : NAN;
+    const float bad = z != z ? NAN : 0.f;  // a target outside of the vocabulary, or a NaN
+    v.y = inv + bad, v.z = 1.f, v.w = ex2_approx(d) * inv - 1.f;
+    row[r] = v;
+    row_loss[out] = ln_s - kLn2 * d;
+    log_z[out] = fmaf(v.x, kLn2, ln_s);
+  }
+}
+// packed rows times their 1 / sum, zeros behind them to the end of their tile
+__global__ void __launch_bounds__(256) scaled_rows_kernel(const __nv_bfloat16* __restrict__ h, int64_t ld, int dim, const float4* __restrict__ row, const int* __restrict__ count, int64_t row0, int64_t rows,
+                                                          __nv_bfloat16* __restrict__ out) {
+  const int64_t r = row0 + (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x & 31, n = *count;
+  if (r >= row0 + rows || r >= (n + kTile - 1) / kTile * kTile) return;
+  const bool zero = r >= n;
+  const float f = zero ? 0.f : row[r].y;
+  for (int c = lane * 8; c < dim; c += 256) {  // rows have room for whole pieces
+    Vec16<__nv_bfloat16> v;
+    float e[8];
+    v.load(h + r * ld + c);
+    v.unpack(e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = zero ? 0.f : e[k] * f;
+    v.pack(e);
+    v.store(out + r * ld + c);
   }
 }
 
@@ -519,7 +709,7 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ 
 }
 
 // What the backward pass needs of a packed row, and the power of two that brings the largest weight to 2^13 .. 2^14 where the pieces are fp16 (products of small weights would vanish there).
-__global__ void __launch_bounds__(1024) weights_kernel(const float2* __restrict__ stats, const int* __restrict__ idx, const int* __restrict__ targets, const int* __restrict__ count, const float* __restrict__ dloss, int reduction,
+__global__ void __launch_bounds__(1024) weights_kernel(const float4* __restrict__ stats, const int* __restrict__ idx, const int* __restrict__ count, const float* __restrict__ dloss, int reduction,
                                                        const float* __restrict__ dlog_z, int has_z, int half, float4* __restrict__ row, float* __restrict__ scales) {
   __shared__ float tops[32];
   const int n = *count, tid = threadIdx.x;
@@ -527,7 +717,7 @@ __global__ void __launch_bounds__(1024) weights_kernel(const float2* __restrict_
   float top = 0.f;
   for (int i = tid; i < n; i += 1024) {
     const float w = reduction ? all : dloss[idx[i]], z = has_z ? dlog_z[idx[i]] : 0.f;
-    top = fmaxf(top, fmaxf(fabsf(w), fabsf(w + z)));
+    top = fmaxf(top, fabsf(w + z));
   }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -539,33 +729,124 @@ __global__ void __launch_bounds__(1024) weights_kernel(const float2* __restrict_
   if (tid == 0) scales[0] = scale, scales[1] = 1.f / scale;
   for (int i = tid; i < n; i += 1024) {
     const float w = reduction ? all : dloss[idx[i]], z = has_z ? dlog_z[idx[i]] : 0.f;
-    const float2 s = stats[i];
-    const float bad = targets[i] < 0 ? NAN : 0.f;  // a target outside of the vocabulary
-    row[i] = make_float4(s.x, 1.f / s.y, w * scale + bad, (w + z) * scale + bad);
+    const float4 s = stats[i];
+    const float inv = 1.f / s.y, d = fmaf(s.z, kLog2e, -s.x), bad = s.z != s.z ? NAN : 0.f;  // a target outside of the vocabulary, or a NaN
+    row[i] = make_float4(s.x, inv, (w + z) * scale + bad, ex2_approx(d) * inv * (w + z) - w);
   }
 }
 
-// dhidden: a packed row's partial sums joined, into its place; zeros for rows that are left out.  Rows [row0, row0 + rows) of idx.
-__global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ part, int splits, int64_t split, int64_t ld, int dim, const int* __restrict__ idx, const int* __restrict__ count, int row0,
-                                                      int rows, const float* __restrict__ scales, void* out, int dtype) {
-  const int n = *count;
-  const float inv = scales[1];
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * dim; i += (int64_t)gridDim.x * 256) {
-    const int r = (int)(i / dim), c = (int)(i - (int64_t)r * dim);
-    float v = 0.f;
-    if (row0 + r < n) {
-      for (int s = 0; s < splits; ++s) v += part[s * split + r * ld + c];
-      v *= inv;
+// dhidden: a packed row's partial sums joined, times its own factor (`by_row`) or all rows', and q W_t, into its place; zeros for rows that are left out.  Rows [row0, row0 + rows) of idx, a
+// warp each.  V columns at a time.
+template <int V>
+__global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ part, int splits, int64_t split, int64_t ld, int dim, const int* __restrict__ idx, const int* __restrict__ targets,
+                                                      const int* __restrict__ count, int row0, int rows, const float4* __restrict__ row, int by_row, const float* __restrict__ scales, const void* weight,
+                                                      int64_t weight_stride, int weight_dtype, void* out, int dtype) {
+  const int i = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31, r = row0 + i;
+  if (i >= rows) return;
+  const bool in = r < *count;
+  const int64_t to = (int64_t)idx[r] * dim;
+  const int t = in ? max(targets[r], 0) : 0;
+  const float4 w = in ? row[r] : make_float4(0.f, 0.f, 0.f, 0.f);
+  const float f = by_row ? w.y : scales[1];
+  for (int c = lane * V; c < dim; c += 32 * V) {
+    float v[V] = {}, e[V];
+    if (in) {
+      for (int s = 0; s < splits; ++s) {
+        const float* from = part + s * split + i * ld + c;
+        if constexpr (V == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(from);
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        } else {
+          v[0] += *from;
+        }
+      }
+      if constexpr (V == 4) load_param_vec<4>(weight, t * weight_stride + c, weight_dtype, e);
+      else e[0] = load_dyn(weight, t * weight_stride + c, weight_dtype);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = fmaf(w.w, e[k], v[k] * f);
     }
-    store_dyn(out, (int64_t)idx[row0 + r] * dim + c, dtype, v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) store_dyn(out, to + c + k, dtype, v[k]);
   }
 }
-__global__ void __launch_bounds__(256) dweight_kernel(const float* __restrict__ sums, int64_t ld, int vocab, int dim, const int* __restrict__ count, const float* __restrict__ scales, void* out, int dtype) {
+
+// Packed rows [8192 b, ..) in the order of their targets: keys (target, packed row), all ones behind them.  A block each.
+constexpr int kSort = 8192;
+__global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targets, const int* __restrict__ count, int size, uint64_t* __restrict__ keys) {
+  extern __shared__ uint64_t key[];
+  const int first = blockIdx.x * kSort, n = *count;
+  for (int i = threadIdx.x; i < size; i += 1024) {
+    const int r = first + i, t = r < n ? targets[r] : -1;
+    key[i] = t >= 0 ? (uint64_t)t << 32 | (uint32_t)r : ~0ull;
+  }
+  for (int k = 2; k <= size; k *= 2) {
+    for (int j = k / 2; j > 0; j /= 2) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < size; i += 1024) {
+        const int o = i ^ j;
+        if (o > i) {
+          const uint64_t a = key[i], b = key[o];
+          if ((a > b) == ((i & k) == 0)) key[i] = b, key[o] = a;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < size; i += 1024) keys[first + i] = key[i];
+}
+// dweight's row of a target += the sum of q h over the rows that have it, in their order: one block (of 512 columns) for each run of equal targets
+__global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* __restrict__ keys, int size, const float4* __restrict__ row, const int* __restrict__ idx, const void* hidden, int64_t stride, int dtype,
+                                                          int dim, const float* __restrict__ scales, float* __restrict__ out, int64_t ld) {
+  const int p = blockIdx.x;
+  const uint64_t key = keys[p];
+  if (key == ~0ull || (p > 0 && keys[p - 1] >> 32 == key >> 32)) return;
+  const int c0 = blockIdx.y * 512 + threadIdx.x;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int q = p; q < size && keys[q] >> 32 == key >> 32; ++q) {
+    const int r = (int)(uint32_t)keys[q];
+    const float w = row[r].w;
+    const int64_t at = idx[r] * stride;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c0 + 128 * k < dim) v[k] = fmaf(w, load_dyn(hidden, at + c0 + 128 * k, dtype), v[k]);
+  }
+  const float scale = scales[0];
+  float* to = out + (int64_t)(key >> 32) * ld;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (c0 + 128 * k < dim) to[c0 + 128 * k] += v[k] * scale;
+}
+
+// out = factor * src, the factor scales[1] (dloss NULL) or scales[1] dloss; zeros where no row counts.  V elements at a time.
+template <int V>
+__global__ void __launch_bounds__(256) scaled_copy_kernel(const float* __restrict__ src, int64_t ld, int64_t rows, int dim, const int* __restrict__ count, const float* __restrict__ scales,
+                                                          const float* __restrict__ dloss, int has_dloss, void* out, int dtype) {
   const bool none = *count == 0;
-  const float inv = scales[1];
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)vocab * dim; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / dim, c = i - r * dim;
-    store_dyn(out, i, dtype, none ? 0.f : sums[r * ld + c] * inv);
+  const float f = has_dloss ? scales[1] * dloss[0] : scales[1];
+  const int per = dim / V;
+  const int64_t all = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * V;
+    float v[V];
+    if constexpr (V == 4) {
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(src + r * ld + c));
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      v[0] = src[r * ld + c];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = none ? 0.f : v[k] * f;
+    if constexpr (V == 4) {
+      if (dtype == SSM_F32) {
+        __stcs(reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + r * dim + c), make_float4(v[0], v[1], v[2], v[3]));
+      } else {
+        const uint2 w = dtype == SSM_BF16 ? make_uint2(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3])) : make_uint2(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]));
+        __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + r * dim + c), w);
+      }
+    } else {
+      store_dyn(out, r * dim + c, dtype, v[0]);
+    }
   }
 }
 
@@ -584,39 +865,43 @@ int encode(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int p
   return rc == CUDA_SUCCESS ? SSM_OK : fail(SSM_ERR_DEVICE, "linear_cross_entropy: cuTensorMapEncodeTiled rejected the matrix");
 }
 
+enum Pass { kForward = 0, kBackward = 1, kBoth = 2 };
 // sizes and places of a call
 struct Plan {
-  int planes, fmt, pairs_at_once;
+  int planes, fmt, pairs;
   int64_t rows, dim, vocab, ldh, ldg, ldo;  // leading dimensions: packed h, pieces of G, fp32 outputs
   bool copy_w;
-  int64_t piece;      // rows of a piece, forward and backward
+  int64_t piece;      // rows of a piece
   int splits, bn;     // of dh = G W
-  int parts;
+  int parts, sort, sorts;
   // offsets into scratch
-  int64_t idx, packed, count, scales, h, w, part, z, row, g, dh, dw, bytes;
+  int64_t idx, packed, count, scales, h, w, part, z, row, g, dh, dw, keys, again, hs, bytes;
 };
 constexpr int64_t kForwardRows = 16384;
 
-Plan plan_of(const ssm_linear_ce_args& a, bool backward) {
+Plan plan_of(const ssm_linear_ce_args& a, int pass) {
   Plan p{};
-  p.splits = 1;
   p.planes = a.io_dtype == SSM_F32 ? 3 : 1, p.fmt = a.io_dtype != SSM_F16;
   p.rows = std::max<int64_t>(a.rows, 1), p.dim = a.dim, p.vocab = a.vocab;
   p.ldh = up(p.dim, 8), p.ldg = up(p.vocab, 64), p.ldo = up(p.dim, 4);
   p.copy_w = p.planes == 3 || a.weight_stride % 8 != 0 || a.weight_stride < a.dim || !aligned_to(a.weight, 16);
   p.parts = (int)((p.vocab + kTile - 1) / kTile) * 2;
-  p.pairs_at_once = sm_count() / 2;
+  p.pairs = std::max(1, sm_count() / 2);
   p.bn = p.dim <= 128 ? 128 : 256;
+  p.splits = 1, p.sort = 1;
+  while (p.sort < kSort && p.sort < p.rows) p.sort *= 2;
+  p.sorts = (int)((p.rows + kSort - 1) / kSort);
   p.piece = std::min<int64_t>(up(p.rows, kTile), kForwardRows);
-  if (backward) {
-    const int64_t fit = std::max<int64_t>(1, SSM_LINEAR_CE_PIECE_BYTES / (p.ldg * 2 * p.planes) / kTile) * kTile;
-    p.piece = up((p.rows + (p.rows + fit - 1) / fit - 1) / ((p.rows + fit - 1) / fit), kTile);  // pieces of one size
-    const int64_t tiles = p.piece / kTile * ((p.dim + p.bn - 1) / p.bn), kb = (p.vocab + kK - 1) / kK;
-    // as many splits of the vocabulary as leave the pairs least idle, each of at least 16 steps
+  if (pass != kForward) {
+    const int64_t fit = std::max<int64_t>(1, SSM_LINEAR_CE_PIECE_BYTES / (p.ldg * 2 * p.planes) / kTile) * kTile, n = (p.rows + fit - 1) / fit;
+    p.piece = up((p.rows + n - 1) / n, kTile);  // pieces of one size
+    // Splits of the vocabulary for dh: the pairs share its tiles and those of dW, which fill up where dh's do not come out even, as long as none of dh's takes longer than all of
+    // a pair's share.  A split costs its partial sums' way through memory, 0.3 blocks of K a tile.
+    const double t0 = (double)(p.piece / kTile) * (double)((p.dim + p.bn - 1) / p.bn), kb0 = (double)((p.vocab + kK - 1) / kK);
+    const double t1 = (double)((p.vocab + kTile - 1) / kTile) * (double)((p.dim + p.bn - 1) / p.bn), share = (t0 * kb0 + t1 * (double)(p.piece / kK)) / p.pairs;
     double least = 1e300;
-    for (int s = 1; s <= 32 && (s == 1 || kb / s >= 16); ++s) {
-      const double rounds = (double)((tiles * s + p.pairs_at_once - 1) / p.pairs_at_once);
-      const double cost = rounds * ((double)kb / s + 8.0) + 0.2 * (double)s * (double)tiles;
+    for (int s = 1; s <= 32 && (s == 1 || kb0 / s >= 16); ++s) {
+      const double cost = std::max(share, std::ceil(t0 * s / p.pairs) * (kb0 / s)) + 0.3 * s * t0;
       if (cost < least) least = cost, p.splits = s;
     }
   }
@@ -626,15 +911,14 @@ Plan plan_of(const ssm_linear_ce_args& a, bool backward) {
     at += up(bytes, 256);
     return here;
   };
-  p.idx = take(p.rows * 4), p.packed = take(p.rows * 4), p.count = take(4), p.scales = take(8);
+  p.idx = take(p.rows * 4), p.packed = take(p.rows * 4), p.count = take(4), p.scales = take(8), p.row = take(p.rows * 16);  // row: stats of a forward pass that keeps none
   p.h = take(p.planes * up(p.rows, kTile) * p.ldh * 2);
   p.w = take(p.copy_w ? p.planes * p.vocab * p.ldh * 2 : 0);
-  if (!backward) {
-    p.part = take((int64_t)p.parts * p.piece * 8), p.z = take(p.rows * 4);
-    p.row = take(p.rows * 8);  // stats of a call that keeps none
-  } else {
-    p.row = take(p.rows * 16), p.g = take(p.planes * p.piece * p.ldg * 2);
-    p.dh = take((int64_t)p.splits * p.piece * p.ldo * 4), p.dw = take(p.vocab * p.ldo * 4);
+  if (pass != kBackward) p.part = take((int64_t)p.parts * p.piece * 8), p.z = take(p.rows * 4);
+  if (pass != kForward) {
+    p.g = take(p.planes * p.piece * p.ldg * 2), p.dh = take((int64_t)p.splits * p.piece * p.ldo * 4), p.keys = take((int64_t)p.sorts * kSort * 8);
+    if (pass == kBackward) p.dw = take(p.vocab * p.ldo * 4);
+    else p.again = take(p.piece / kTile * 4), p.hs = take(up(p.rows, kTile) * p.ldh * 2);
   }
   p.bytes = at;
   return p;
@@ -646,62 +930,144 @@ int check(const ssm_linear_ce_args& a) {
   SSM_REQUIRE(valid_dtype(a.io_dtype), SSM_ERR_DTYPE, "linear_cross_entropy: unknown dtype");
   SSM_REQUIRE(a.reduction >= 0 && a.reduction <= 2, SSM_ERR_SHAPE, "linear_cross_entropy: unknown reduction");
   SSM_REQUIRE(a.weight && (a.rows == 0 || (a.hidden && a.targets)) && a.scratch && a.status, SSM_ERR_NULL, "linear_cross_entropy: NULL pointer");
-  SSM_REQUIRE(aligned_to({a.hidden, a.weight}, dtype_size(a.io_dtype)) && aligned_to({a.targets, a.stats}, 8) && aligned_to({a.row_loss, a.log_z, a.loss, a.status}, 4) && aligned_to(a.scratch, 256),
+  SSM_REQUIRE(aligned_to({a.hidden, a.weight}, dtype_size(a.io_dtype)) && aligned_to(a.targets, 8) && aligned_to(a.stats, 16) && aligned_to({a.row_loss, a.log_z, a.loss, a.status}, 4) && aligned_to(a.scratch, 256),
               SSM_ERR_ALIGN, "linear_cross_entropy: misaligned pointer");
   return SSM_OK;
 }
 
 template <int EPI, typename T, int PLANES>
-int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g, int pairs_at_once, cudaStream_t st) {
+int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb1, const GemmArgs& g, int pairs, cudaStream_t st) {
   auto kern = gemm_kernel<EPI, T, PLANES>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-  const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles * g.splits;
-  kern<<<(unsigned)(2 * std::min<int64_t>(tiles, pairs_at_once)), kThreads, kSmem, st>>>(ma, mb, g);
+  int64_t tiles = 0;
+  for (const Job& j : g.job) tiles += (int64_t)j.m_tiles * j.n_tiles * j.splits;
+  kern<<<(unsigned)(2 * std::max<int64_t>(1, std::min<int64_t>(tiles, pairs))), kThreads, kSmem, st>>>(ma, mb, mb1, g);
   return launch_status("linear_ce gemm_kernel");
 }
 template <int EPI>
-int gemm_of(const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g, cudaStream_t st) {
-  if (p.planes == 3) return launch_gemm<EPI, __nv_bfloat16, 3>(ma, mb, g, p.pairs_at_once, st);
-  if (EPI == kGrad && p.fmt == 0) return launch_gemm<EPI, __half, 1>(ma, mb, g, p.pairs_at_once, st);
-  return launch_gemm<EPI, __nv_bfloat16, 1>(ma, mb, g, p.pairs_at_once, st);
+int gemm_of(const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb1, const GemmArgs& g, cudaStream_t st) {
+  if constexpr (EPI == kKeep) {
+    return launch_gemm<EPI, __nv_bfloat16, 1>(ma, mb, mb1, g, p.pairs, st);
+  } else {
+    if (p.planes == 3) return launch_gemm<EPI, __nv_bfloat16, 3>(ma, mb, mb1, g, p.pairs, st);
+    if (EPI == kGrad && p.fmt == 0) return launch_gemm<EPI, __half, 1>(ma, mb, mb1, g, p.pairs, st);
+    return launch_gemm<EPI, __nv_bfloat16, 1>(ma, mb, mb1, g, p.pairs, st);
+  }
 }
 
 struct Run {
   const ssm_linear_ce_args& a;
   Plan p;
   char* base;
-  CUtensorMap mh, mw;
+  cudaStream_t st;
+  CUtensorMap mh, mw, mg;
   template <typename U>
   U* at(int64_t off) const { return reinterpret_cast<U*>(base + off); }
+  int* idx() const { return at<int>(p.idx); }
+  int* packed() const { return at<int>(p.packed); }
+  int* count() const { return at<int>(p.count); }
+  float4* row() const { return at<float4>(p.row); }
+  const void* w() const { return p.copy_w ? at<void>(p.w) : a.weight; }
+  int64_t ldw() const { return p.copy_w ? p.ldh : a.weight_stride; }
 };
 // packs the rows (and the weight, where it cannot be copied from its place) and describes them to the copies
-int prepare(Run& r, bool write, cudaStream_t st) {
+int prepare(Run& r, bool write) {
   const ssm_linear_ce_args& a = r.a;
   const Plan& p = r.p;
-  int *idx = r.at<int>(p.idx), *count = r.at<int>(p.count);
-  rows_kernel<<<1, 1024, 0, st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, idx, r.at<int>(p.packed), count, a.row_loss, a.log_z, write);
+  rows_kernel<<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z, write);
   if (const int rc = launch_status("linear_ce rows_kernel")) return rc;
-  const int64_t plane_h = up(p.rows, kTile) * p.ldh, plane_w = p.vocab * p.ldh;
+  const int64_t plane_h = up(p.rows, kTile) * p.ldh, plane_w = p.copy_w ? p.vocab * p.ldh : p.vocab * a.weight_stride;
   auto pack = [&](const void* src, int64_t stride, int64_t rows, const int* map, uint16_t* dst, int64_t plane) {
     const unsigned grid = (unsigned)((rows + 7) / 8);
-    if (p.planes == 3) pack_kernel<float, 3><<<grid, 256, 0, st>>>(src, stride, rows, (int)p.dim, map, count, dst, p.ldh, plane);
-    else pack_kernel<uint16_t, 1><<<grid, 256, 0, st>>>(src, stride, rows, (int)p.dim, map, count, dst, p.ldh, plane);
+    if (p.planes == 3) pack_kernel<float, 3><<<grid, 256, 0, r.st>>>(src, stride, rows, (int)p.dim, map, r.count(), dst, p.ldh, plane);
+    else pack_kernel<uint16_t, 1><<<grid, 256, 0, r.st>>>(src, stride, rows, (int)p.dim, map, r.count(), dst, p.ldh, plane);
     return launch_status("linear_ce pack_kernel");
   };
-  if (const int rc = pack(a.hidden, a.hidden_stride, p.rows, idx, r.at<uint16_t>(p.h), plane_h)) return rc;
+  if (const int rc = pack(a.hidden, a.hidden_stride, p.rows, r.idx(), r.at<uint16_t>(p.h), plane_h)) return rc;
   if (p.copy_w)
     if (const int rc = pack(a.weight, a.weight_stride, p.vocab, nullptr, r.at<uint16_t>(p.w), plane_w)) return rc;
   if (const int rc = encode(&r.mh, r.at<void>(p.h), p.dim, p.rows, p.planes, p.ldh, plane_h, p.fmt)) return rc;
-  return encode(&r.mw, p.copy_w ? r.at<void>(p.w) : a.weight, p.dim, p.vocab, p.planes, p.copy_w ? p.ldh : a.weight_stride, p.copy_w ? plane_w : p.vocab * a.weight_stride, p.fmt);
+  if (const int rc = encode(&r.mw, r.w(), p.dim, p.vocab, p.planes, r.ldw(), plane_w, p.fmt)) return rc;
+  return p.g ? encode(&r.mg, r.at<void>(p.g), p.vocab, p.piece, p.planes, p.ldg, p.piece * p.ldg, p.fmt) : SSM_OK;
 }
 // z = h W^T for the packed rows [row0, row0 + rows)
 GemmArgs logits_args(const Run& r, int64_t row0, int64_t rows) {
   const Plan& p = r.p;
   GemmArgs g{};
-  g.m_tiles = (int)((rows + kTile - 1) / kTile), g.n_tiles = (int)((p.vocab + kTile - 1) / kTile), g.splits = 1, g.k_blocks = (int)((p.dim + kK - 1) / kK), g.bn = kTile, g.m_inner = 1;
-  g.a_m0 = (int)row0, g.planes = p.planes, g.fmt = p.fmt, g.row0 = (int)row0, g.rows = (int)rows, g.count = r.at<int>(p.count), g.status = r.a.status;
-  g.vocab = (int)p.vocab, g.targets = r.at<int>(p.packed);
+  Job& j = g.job[0];
+  j.m_tiles = (int)((rows + kTile - 1) / kTile), j.n_tiles = (int)((p.vocab + kTile - 1) / kTile), j.splits = 1, j.k_blocks = (int)((p.dim + kK - 1) / kK), j.m_inner = 1, j.a_m0 = (int)row0;
+  g.job[1].splits = 1;
+  g.bn = kTile, g.fmt = p.fmt, g.row0 = (int)row0, g.rows = (int)rows, g.count = r.count(), g.status = r.a.status;
+  g.vocab = (int)p.vocab, g.targets = r.packed(), g.row = r.row();
+  g.part = r.at<float2>(p.part), g.part_ld = (int)p.piece, g.z_target = r.at<float>(p.z);
+  g.g = r.at<uint16_t>(p.g), g.ldg = p.ldg, g.g_plane = p.piece * p.ldg;
   return g;
+}
+// dh = G W and dW += G^T h of a piece, `h2` for h, and dh's way to its rows; each nullable
+int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, bool by_row, void* dh, int dh_dtype, float* dw) {
+  const Plan& p = r.p;
+  GemmArgs g{};
+  g.bn = p.bn, g.fmt = p.fmt, g.row0 = (int)row0, g.rows = (int)rows, g.count = r.count(), g.status = r.a.status;
+  const int d_tiles = (int)((p.dim + p.bn - 1) / p.bn);
+  Job &a = g.job[0], &b = g.job[1];
+  a.splits = b.splits = 1;
+  if (dh) {
+    a.m_tiles = (int)((rows + kTile - 1) / kTile), a.n_tiles = d_tiles, a.splits = p.splits, a.k_blocks = (int)((p.vocab + kK - 1) / kK), a.b_mn = 1;
+    a.out = r.at<float>(p.dh), a.ld = p.ldo, a.out_split = p.piece * p.ldo, a.out_rows = (int)rows;
+  }
+  if (dw) {
+    b.m_tiles = (int)((p.vocab + kTile - 1) / kTile), b.n_tiles = d_tiles, b.a_mn = b.b_mn = 1, b.k_is_rows = 1, b.b_k0 = (int)row0;
+    b.out = dw, b.ld = p.ldo, b.out_rows = (int)p.vocab, b.add = row0 > 0;
+  }
+  if (const int rc = gemm_of<kOut>(p, r.mg, r.mw, h2, g, r.st)) return rc;
+  if (!dh) return SSM_OK;
+  const unsigned grid = (unsigned)((rows + 7) / 8);
+  const bool wide = p.dim % 4 == 0 && r.a.weight_stride % 4 == 0 && aligned_to(r.a.weight, 16);
+  auto kern = wide ? dhidden_kernel<4> : dhidden_kernel<1>;
+  kern<<<grid, 256, 0, r.st>>>(a.out, a.splits, a.out_split, p.ldo, (int)p.dim, r.idx(), r.packed(), r.count(), (int)row0, (int)rows, r.row(), by_row, r.at<float>(p.scales), r.a.weight, r.a.weight_stride,
+                               r.a.io_dtype, dh, dh_dtype);
+  return launch_status("linear_ce dhidden_kernel");
+}
+// the targets' part of dW
+int target_rows(const Run& r, float* dw) {
+  const Plan& p = r.p;
+  uint64_t* keys = r.at<uint64_t>(p.keys);
+  cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
+  sort_kernel<<<p.sorts, 1024, p.sort * 8, r.st>>>(r.packed(), r.count(), p.sort, keys);
+  if (const int rc = launch_status("linear_ce sort_kernel")) return rc;
+  for (int i = 0; i < p.sorts; ++i) {
+    target_rows_kernel<<<dim3((unsigned)p.sort, (unsigned)((p.dim + 511) / 512)), 128, 0, r.st>>>(keys + (int64_t)i * kSort, p.sort, r.row(), r.idx(), r.a.hidden, r.a.hidden_stride, r.a.io_dtype, (int)p.dim,
+                                                                                                  r.at<float>(p.scales), dw, p.ldo);
+    if (const int rc = launch_status("linear_ce target_rows_kernel")) return rc;
+  }
+  return SSM_OK;
+}
+int scaled_copy(const float* src, int64_t ld, int64_t rows, int64_t dim, const int* count, const float* scales, const float* dloss, void* out, int dtype, cudaStream_t st) {
+  const bool wide = dim % 4 == 0 && ld % 4 == 0 && aligned_to({src, out}, 16);
+  const int64_t all = rows * (wide ? dim / 4 : dim);
+  const unsigned grid = (unsigned)std::min<int64_t>((all + 255) / 256, 148 * 32);
+  auto kern = wide ? scaled_copy_kernel<4> : scaled_copy_kernel<1>;
+  kern<<<grid, 256, 0, st>>>(src, ld, rows, (int)dim, count, scales, dloss ? dloss : scales, dloss != nullptr, out, dtype);
+  return launch_status("linear_ce scaled_copy_kernel");
+}
+int zero(void* p, size_t bytes, cudaStream_t st) {
+  const cudaError_t e = cudaMemsetAsync(p, 0, bytes, st);
+  if (e == cudaSuccess) return SSM_OK;
+  set_error("linear_cross_entropy: %s", cudaGetErrorString(e));
+  return (int)e;
+}
+int reduce(const Run& r) {
+  if (r.a.reduction == 0) return SSM_OK;
+  if (r.a.rows == 0) return zero(r.a.loss, 4, r.st);
+  reduce_kernel<<<1, 1024, 0, r.st>>>(r.a.row_loss, (int)r.a.rows, r.count(), r.a.reduction == 2, r.a.loss);
+  return launch_status("linear_ce reduce_kernel");
+}
+// what the one-pass form's gradients are multiplied by: kept[0] 1 / rows that count for a mean, kept[1] how many count (as an integer); scales of this call
+__global__ void share_kernel(const int* count, int mean, float* kept, float* scales) {
+  kept[0] = scales[0] = 1.f;
+  scales[1] = 1.f;
+  kept[1] = mean ? 1.f / (float)max(1, *count) : 1.f;
+  reinterpret_cast<int*>(kept)[2] = *count;
 }
 
 }  // namespace
@@ -709,9 +1075,9 @@ GemmArgs logits_args(const Run& r, int64_t row0, int64_t rows) {
 
 using namespace ssmb;
 
-extern "C" int64_t ssm_linear_ce_scratch_bytes(const ssm_linear_ce_args* args, int32_t backward) {
+extern "C" int64_t ssm_linear_ce_scratch_bytes(const ssm_linear_ce_args* args, int32_t pass) {
   if (!args || args->rows < 0 || args->dim < 1 || args->vocab < 1) return 0;
-  return plan_of(*args, backward != 0).bytes;
+  return plan_of(*args, pass).bytes;
 }
 
 extern "C" int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t stream) {
@@ -719,28 +1085,20 @@ extern "C" int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t st
   if (const int rc = check(*args)) return rc;
   const ssm_linear_ce_args& a = *args;
   SSM_REQUIRE((a.rows == 0 || (a.row_loss && a.log_z)) && (a.reduction == 0 || a.loss), SSM_ERR_NULL, "linear_cross_entropy: NULL output");
-  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  Run r{a, plan_of(a, false), static_cast<char*>(a.scratch)};
+  Run r{a, plan_of(a, kForward), static_cast<char*>(a.scratch), reinterpret_cast<cudaStream_t>(stream)};
   const Plan& p = r.p;
   if (a.rows) {
-    if (const int rc = prepare(r, true, st)) return rc;
-    float2* stats = a.stats ? reinterpret_cast<float2*>(a.stats) : r.at<float2>(p.row);
+    if (const int rc = prepare(r, true)) return rc;
+    float4* stats = a.stats ? reinterpret_cast<float4*>(a.stats) : r.row();
     for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
       const int64_t rows = std::min(p.piece, p.rows - row0);
-      GemmArgs g = logits_args(r, row0, rows);
-      g.part = r.at<float2>(p.part), g.part_ld = (int)p.piece, g.z_target = r.at<float>(p.z);
-      if (const int rc = gemm_of<kStats>(p, r.mh, r.mw, g, st)) return rc;
-      join_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.at<int>(p.idx), r.at<int>(p.packed), g.z_target, stats, a.row_loss, a.log_z);
+      const GemmArgs g = logits_args(r, row0, rows);
+      if (const int rc = gemm_of<kStats>(p, r.mh, r.mw, r.mw, g, r.st)) return rc;
+      join_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z);
       if (const int rc = launch_status("linear_ce join_kernel")) return rc;
     }
   }
-  if (a.reduction == 0) return SSM_OK;
-  if (a.rows == 0) {
-    const cudaError_t e = cudaMemsetAsync(a.loss, 0, 4, st);
-    return e == cudaSuccess ? SSM_OK : (set_error("linear_cross_entropy: %s", cudaGetErrorString(e)), (int)e);
-  }
-  reduce_kernel<<<1, 1024, 0, st>>>(a.row_loss, (int)a.rows, r.at<int>(p.count), a.reduction == 2, a.loss);
-  return launch_status("linear_ce reduce_kernel");
+  return reduce(r);
 }
 
 extern "C" int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_t stream) {
@@ -751,47 +1109,69 @@ extern "C" int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_
   SSM_REQUIRE(a.rows == 0 || (a.stats && args->dloss), SSM_ERR_NULL, "linear_cross_entropy backward: NULL pointer");
   SSM_REQUIRE(aligned_to({args->dloss, args->dlog_z}, 4) && aligned_to(args->dhidden, dtype_size(a.io_dtype)) && aligned_to(args->dweight, dtype_size(args->dweight_dtype)), SSM_ERR_ALIGN,
               "linear_cross_entropy backward: misaligned pointer");
-  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (a.rows == 0) {
-    if (!args->dweight) return SSM_OK;
-    const cudaError_t e = cudaMemsetAsync(args->dweight, 0, (size_t)a.vocab * a.dim * dtype_size(args->dweight_dtype), st);
-    return e == cudaSuccess ? SSM_OK : (set_error("linear_cross_entropy: %s", cudaGetErrorString(e)), (int)e);
-  }
-  Run r{a, plan_of(a, true), static_cast<char*>(a.scratch)};
+  Run r{a, plan_of(a, kBackward), static_cast<char*>(a.scratch), reinterpret_cast<cudaStream_t>(stream)};
   const Plan& p = r.p;
-  if (const int rc = prepare(r, false, st)) return rc;
-  int *idx = r.at<int>(p.idx), *count = r.at<int>(p.count);
-  float* scales = r.at<float>(p.scales);
-  weights_kernel<<<1, 1024, 0, st>>>(reinterpret_cast<const float2*>(a.stats), idx, r.at<int>(p.packed), count, args->dloss, a.reduction, args->dlog_z ? args->dlog_z : args->dloss, args->dlog_z != nullptr,
-                                     a.io_dtype == SSM_F16, r.at<float4>(p.row), scales);
+  if (a.rows == 0) return args->dweight ? zero(args->dweight, (size_t)a.vocab * a.dim * dtype_size(args->dweight_dtype), r.st) : SSM_OK;
+  if (const int rc = prepare(r, false)) return rc;
+  float *scales = r.at<float>(p.scales), *dw = args->dweight ? r.at<float>(p.dw) : nullptr;
+  weights_kernel<<<1, 1024, 0, r.st>>>(reinterpret_cast<const float4*>(a.stats), r.idx(), r.count(), args->dloss, a.reduction, args->dlog_z ? args->dlog_z : args->dloss, args->dlog_z != nullptr,
+                                       a.io_dtype == SSM_F16, r.row(), scales);
   if (const int rc = launch_status("linear_ce weights_kernel")) return rc;
-  CUtensorMap mg;
-  if (const int rc = encode(&mg, r.at<void>(p.g), p.vocab, p.piece, p.planes, p.ldg, p.piece * p.ldg, p.fmt)) return rc;
-  const int d_tiles = (int)((p.dim + p.bn - 1) / p.bn);
   for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
     const int64_t rows = std::min(p.piece, p.rows - row0);
-    GemmArgs z = logits_args(r, row0, rows);
-    z.row = r.at<float4>(p.row), z.g = r.at<uint16_t>(p.g), z.ldg = p.ldg, z.g_plane = p.piece * p.ldg;
-    if (const int rc = gemm_of<kGrad>(p, r.mh, r.mw, z, st)) return rc;
-    GemmArgs g{};
-    g.bn = p.bn, g.n_tiles = d_tiles, g.b_mn = 1, g.planes = p.planes, g.fmt = p.fmt, g.row0 = (int)row0, g.rows = (int)rows, g.count = count, g.status = a.status, g.ld = p.ldo;
-    if (args->dhidden) {  // dh = G W
-      GemmArgs d = g;
-      d.m_tiles = z.m_tiles, d.splits = p.splits, d.k_blocks = (int)((p.vocab + kK - 1) / kK);
-      d.out = r.at<float>(p.dh), d.out_split = p.piece * p.ldo, d.out_rows = (int)rows;
-      if (const int rc = gemm_of<kOut>(p, mg, r.mw, d, st)) return rc;
-      dhidden_kernel<<<(unsigned)std::min<int64_t>((rows * p.dim + 255) / 256, 148 * 8), 256, 0, st>>>(d.out, d.splits, d.out_split, p.ldo, (int)p.dim, idx, count, (int)row0, (int)rows, scales,
-                                                                                                       args->dhidden, a.io_dtype);
-      if (const int rc = launch_status("linear_ce dhidden_kernel")) return rc;
-    }
-    if (args->dweight) {  // dW += G^T h
-      GemmArgs d = g;
-      d.m_tiles = (int)((p.vocab + kTile - 1) / kTile), d.splits = 1, d.a_mn = 1, d.k_is_rows = 1, d.b_k0 = (int)row0;
-      d.out = r.at<float>(p.dw), d.out_rows = (int)p.vocab, d.add = row0 > 0;
-      if (const int rc = gemm_of<kOut>(p, mg, r.mh, d, st)) return rc;
-    }
+    if (const int rc = gemm_of<kGrad>(p, r.mh, r.mw, r.mw, logits_args(r, row0, rows), r.st)) return rc;
+    if (const int rc = gradients(r, row0, rows, r.mh, false, args->dhidden, a.io_dtype, dw)) return rc;
   }
-  if (!args->dweight) return SSM_OK;
-  dweight_kernel<<<(unsigned)std::min<int64_t>((p.vocab * p.dim + 255) / 256, 148 * 16), 256, 0, st>>>(r.at<float>(p.dw), p.ldo, (int)p.vocab, (int)p.dim, count, scales, args->dweight, args->dweight_dtype);
-  return launch_status("linear_ce dweight_kernel");
+  if (!dw) return SSM_OK;
+  if (const int rc = target_rows(r, dw)) return rc;
+  return scaled_copy(dw, p.ldo, p.vocab, p.dim, r.count(), scales, nullptr, args->dweight, args->dweight_dtype, r.st);
+}
+
+extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidden, float* dweight, float* kept, ssm_stream_t stream) {
+  SSM_REQUIRE(args, SSM_ERR_NULL, "linear_cross_entropy: NULL arguments");
+  if (const int rc = check(*args)) return rc;
+  const ssm_linear_ce_args& a = *args;
+  SSM_REQUIRE(a.io_dtype == SSM_BF16 && a.reduction != 0 && a.rows > 0, SSM_ERR_UNSUPPORTED, "linear_cross_entropy: loss and gradient in one pass are built for sums and means of bf16");
+  SSM_REQUIRE(a.row_loss && a.log_z && a.loss && kept, SSM_ERR_NULL, "linear_cross_entropy: NULL output");
+  SSM_REQUIRE(aligned_to({dhidden, dweight}, 16) && aligned_to(kept, 4), SSM_ERR_ALIGN, "linear_cross_entropy: misaligned pointer");
+  Run r{a, plan_of(a, kBoth), static_cast<char*>(a.scratch), reinterpret_cast<cudaStream_t>(stream)};
+  const Plan& p = r.p;
+  if (const int rc = prepare(r, true)) return rc;
+  share_kernel<<<1, 1, 0, r.st>>>(r.count(), a.reduction == 2, kept, r.at<float>(p.scales));
+  if (const int rc = launch_status("linear_ce share_kernel")) return rc;
+  const __nv_bfloat16* h = r.at<__nv_bfloat16>(p.h);
+  __nv_bfloat16* hs = r.at<__nv_bfloat16>(p.hs);
+  CUtensorMap mhs;
+  if (const int rc = encode(&mhs, hs, p.dim, p.rows, 1, p.ldh, up(p.rows, kTile) * p.ldh, p.fmt)) return rc;
+  int* again = r.at<int>(p.again);
+  for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
+    const int64_t rows = std::min(p.piece, p.rows - row0);
+    const unsigned warps = (unsigned)((rows + 7) / 8);
+    GemmArgs g = logits_args(r, row0, rows);
+    reference_kernel<<<warps, 256, 0, r.st>>>(h, static_cast<const __nv_bfloat16*>(r.w()), p.ldh, r.ldw(), (int)p.dim, r.packed(), r.count(), (int)row0, (int)rows, g.z_target, r.row(), again);
+    if (const int rc = launch_status("linear_ce reference_kernel")) return rc;
+    for (int second = 0; second < 2; ++second) {
+      g.again = second ? again : nullptr;
+      if (const int rc = gemm_of<kKeep>(p, r.mh, r.mw, r.mw, g, r.st)) return rc;
+      join_keep_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), g.z_target, r.row(), again, second, a.row_loss, a.log_z);
+      if (const int rc = launch_status("linear_ce join_keep_kernel")) return rc;
+    }
+    if (dweight) {
+      scaled_rows_kernel<<<warps, 256, 0, r.st>>>(h, p.ldh, (int)p.dim, r.row(), r.count(), row0, rows, hs);
+      if (const int rc = launch_status("linear_ce scaled_rows_kernel")) return rc;
+    }
+    if (const int rc = gradients(r, row0, rows, mhs, true, dhidden, SSM_F32, dweight)) return rc;
+  }
+  if (dweight)
+    if (const int rc = target_rows(r, dweight)) return rc;
+  return reduce(r);
+}
+
+extern "C" int ssm_linear_ce_scale(const float* src, int64_t ld, int64_t rows, int32_t dim, const float* kept, const float* dloss, void* out, int32_t dtype, ssm_stream_t stream) {
+  SSM_REQUIRE(rows >= 0 && dim >= 1 && ld >= dim, SSM_ERR_SHAPE, "linear_cross_entropy: bad shape");
+  SSM_REQUIRE(valid_dtype(dtype), SSM_ERR_DTYPE, "linear_cross_entropy: unknown dtype");
+  SSM_REQUIRE(rows == 0 || (src && kept && dloss && out), SSM_ERR_NULL, "linear_cross_entropy: NULL pointer");
+  SSM_REQUIRE(aligned_to({src, kept, dloss}, 4) && aligned_to(out, dtype_size(dtype)), SSM_ERR_ALIGN, "linear_cross_entropy: misaligned pointer");
+  if (rows == 0) return SSM_OK;
+  return scaled_copy(src, ld, rows, dim, reinterpret_cast<const int*>(kept) + 2, kept, dloss, out, dtype, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -128,7 +128,7 @@ Tensor rows_of(const Tensor& t) {
   return (d.size(1) <= 1 || d.stride(1) == 1) && (d.size(0) <= 1 || d.stride(0) >= d.size(1)) ? d : d.contiguous();
 }
 struct LinearCeCall final : Call {
-  Tensor h, w, targets, stats;
+  Tensor h, w, targets, stats, dh32, dw32, kept;  // stats: for a second pass; the others: of a pass that formed the gradients too
   std::vector<int64_t> shape, lead_shape;
   at::ScalarType t_w;
   int64_t ignore;
@@ -162,8 +162,8 @@ struct LinearCeCall final : Call {
     if (stats.defined()) a.stats = stats.data_ptr<float>();
     a.status = ssd_status(h.get_device()).data_ptr<int32_t>();
   }
-  Tensor scratch(ssm_linear_ce_args& a, bool backward) const {
-    Tensor s = at::empty({std::max<int64_t>(ssm_linear_ce_scratch_bytes(&a, backward), 256)}, h.options().dtype(at::kByte));
+  Tensor scratch(ssm_linear_ce_args& a, int pass) const {
+    Tensor s = at::empty({std::max<int64_t>(ssm_linear_ce_scratch_bytes(&a, pass), 256)}, h.options().dtype(at::kByte));
     a.scratch = s.data_ptr();
     return s;
   }
@@ -171,13 +171,22 @@ struct LinearCeCall final : Call {
     c10::cuda::CUDAGuard guard(h.device());
     ssd_poll(h.get_device());  // a wait that ran out in an earlier launch surfaces here, without a synchronisation
     Tensor row_loss = at::empty(lead_shape, f32()), log_z = at::empty(lead_shape, f32()), loss;
-    if (train) stats = at::empty({std::max<int64_t>(rows(), 1), 2}, f32());
+    // A sum or mean is multiplied by one number, which may come later: in bf16 loss and gradients are formed in one pass, 6 N D V operations instead of 8
+    const bool both = train && reduction && !want_z && h.scalar_type() == at::kBFloat16 && rows() > 0 && (grad_h || grad_w);
+    if (train && !both) stats = at::empty({std::max<int64_t>(rows(), 1), 4}, f32());
     ssm_linear_ce_args a{};
     fill(a);
-    const Tensor s = scratch(a, false);
+    const Tensor s = scratch(a, both ? 2 : 0);
     a.row_loss = row_loss.data_ptr<float>(), a.log_z = log_z.data_ptr<float>();
     if (reduction) loss = at::empty({}, f32()), a.loss = loss.data_ptr<float>();
-    run(ssm_linear_ce_fwd(&a, stream_of(h)));
+    if (both) {
+      kept = at::empty({4}, f32());
+      if (grad_h) dh32 = at::empty(shape, f32());
+      if (grad_w) dw32 = at::empty({w.size(0), (w.size(1) + 3) / 4 * 4}, f32());
+      run(ssm_linear_ce_train(&a, grad_h ? dh32.data_ptr<float>() : nullptr, grad_w ? dw32.data_ptr<float>() : nullptr, kept.data_ptr<float>(), stream_of(h)));
+    } else {
+      run(ssm_linear_ce_fwd(&a, stream_of(h)));
+    }
     variable_list res = {reduction ? loss : row_loss};
     if (want_z) res.push_back(log_z);
     return res;
@@ -189,9 +198,16 @@ struct LinearCeCall final : Call {
     if (want_z && grads[1].defined()) gz = f32c(grads[1]);
     if (grad_h) dh = at::empty(shape, h.options());
     if (grad_w) dw = at::empty(w.sizes(), w.options().dtype(t_w));
+    if (kept.defined()) {
+      const ssm_stream_t st = stream_of(h);
+      if (grad_h) run(ssm_linear_ce_scale(dh32.data_ptr<float>(), w.size(1), rows(), (int)w.size(1), kept.data_ptr<float>(), gl.data_ptr<float>(), dh.data_ptr(), dtype_code(dh, "linear_cross_entropy"), st));
+      if (grad_w)
+        run(ssm_linear_ce_scale(dw32.data_ptr<float>(), dw32.size(1), w.size(0), (int)w.size(1), kept.data_ptr<float>(), gl.data_ptr<float>(), dw.data_ptr(), dtype_code(dw, "linear_cross_entropy weight"), st));
+      return {dh, dw, Tensor()};
+    }
     ssm_linear_ce_bwd_args b{};
     fill(b.fwd);
-    const Tensor s = scratch(b.fwd, true);
+    const Tensor s = scratch(b.fwd, 1);
     b.dloss = gl.data_ptr<float>(), b.dlog_z = gz.defined() ? gz.data_ptr<float>() : nullptr;
     if (grad_h) b.dhidden = dh.data_ptr();
     if (grad_w) b.dweight = dw.data_ptr(), b.dweight_dtype = dtype_code(dw, "linear_cross_entropy weight");

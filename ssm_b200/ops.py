@@ -889,13 +889,16 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore
     """Extension: softmax cross entropy of a linear head, without its logits: ``hidden (..., D)``, ``weight (V, D)``, ``targets (...)`` integers; with
     ``z = hidden weight^T`` returns ``log sum exp z - z[target]`` in fp32, per position (``reduction="none"``), summed, or as the mean over the positions that
     count (0 without any), followed by ``log sum exp z (...)`` with ``return_log_z``.  Differentiable (once) with respect to ``hidden`` and ``weight``, whose gradients
-    have their types; ``weight`` is read in ``hidden``'s type.  Neither pass holds the logits: the backward pass forms their gradient again, at most 512 MB of it at a time.
+    have their types; ``weight`` is read in ``hidden``'s type.
 
     A position whose target is ``ignore_index`` gives 0 (``log_z`` too) and no gradient, is not computed, and may hold anything.  Any other target outside of the vocabulary
     makes its loss and the gradients NaN, as a hidden state that is not finite does.
 
-    16-bit operands are multiplied as they are with sums in 32 bits; the gradient with respect to the logits is rounded to their type before its two products (relative
-    to its largest weight in fp16).  fp32 operands are taken as sums of three bf16 numbers each, products below ``2**-24`` left out."""
+    Neither pass holds the logits; in 16 bits at most 512 MB of their gradient at a time.  For a sum or mean in bf16 without ``return_log_z`` the gradients are formed along with the
+    loss, and held in fp32 until the backward pass scales them (``torch.no_grad()`` forms the loss alone); otherwise the backward pass forms the logits again.
+
+    16-bit operands are multiplied as they are; the gradient with respect to the logits is rounded to their type before its two products, but for the targets' own, which keep 32 bits.
+    fp32 operands are taken as sums of three bf16 numbers each, products below ``2**-24`` left out."""
     return _run("linear_cross_entropy", hidden, weight, targets, int(ignore_index), str(reduction), bool(return_log_z))
 
 

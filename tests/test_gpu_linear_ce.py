@@ -119,6 +119,85 @@ def test_reductions(reduction, dtype):
     near(dw, want[3][0], want[3][1] + 2.0 ** -23 * want[3][0].abs(), "dw")
 
 
+def one_pass(h, w, t, reduction="mean", scale=3.0):
+    """bf16 sums and means form the gradients with the loss: values against the definition.  There the rows' 1 / sum is rounded into h once more (2^-9) for dw, and z_t comes from a
+    sum of its own."""
+    n = h.shape[0]
+    share = scale / (1 if reduction == "sum" else max(1, int((t != -100).sum())))
+    want = bounds(h, w, t, torch.full((n,), share, device="cuda"), torch.zeros(n, device="cuda"))
+    h, w = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = ops.linear_cross_entropy(h, w, t, reduction=reduction)
+    dh, dw = torch.autograd.grad(loss, [h, w], torch.full((), scale, device="cuda"))
+    total, tol = want[0][0].sum() * share / scale, want[0][1].sum() * share / scale
+    near(loss.detach(), total, tol + 2.0 ** -24 * total.abs(), "loss")
+    near(dh, want[2][0], want[2][1] + 2.0 ** -23 * want[2][0].abs(), "dh")
+    hd, wd = h.detach().double(), w.detach().double()
+    kept = (t != -100).double()[:, None]
+    p = torch.softmax(hd @ wd.t(), -1) * share * kept
+    near(dw, want[3][0], want[3][1] + 2.0 ** -9 * (p.t() @ hd.abs()) * 1.01 + 2.0 ** -23 * want[3][0].abs(), "dw")
+    return dh, dw
+
+
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("n,d,v", [(1, 64, 256), (300, 64, 256), (7, 3, 5), (130, 100, 1000), (257, 65, 257), (1000, 320, 5003), (1, 768, 50277), (2000, 64, 151936), (9000, 40, 300)])
+def test_loss_and_gradient_in_one_pass(n, d, v, reduction):
+    one_pass(*make(n, d, v, torch.bfloat16, left_out=0.0 if n == 1 else 0.1)[:3], reduction)
+
+
+@pytest.mark.parametrize("spread", [0.0, 40.0, 3000.0])
+def test_one_pass_with_targets_far_below_the_maximum(spread):
+    h, w, t, _, _ = make(700, 128, 900, torch.bfloat16, spread=spread)
+    one_pass(h, w, t)
+    one_pass(h, w, (h @ w.t()).float().argmax(-1))
+    one_pass(h, w, (h @ w.t()).float().argmin(-1))
+
+
+def test_one_pass_where_one_tile_of_rows_is_formed_again():
+    h, w, t, _, _ = make(1000, 64, 700, torch.bfloat16, left_out=0.0)
+    h[300] *= 100
+    t[300] = (h[300] @ w.t()).float().argmin()
+    one_pass(h, w, t)
+
+
+def test_one_pass_with_common_targets():
+    h, w, t, _, _ = make(3000, 64, 700, torch.bfloat16)
+    one_pass(h, w, torch.where(torch.arange(3000, device="cuda") % 3 == 0, torch.full_like(t, 17), t))
+    one_pass(h, w, torch.full_like(t, 699))
+
+
+def test_one_pass_with_values_that_are_not_finite():
+    h, w, t, _, _ = make(600, 64, 400, torch.bfloat16)
+    want = one_pass(h, w, t)
+    h2 = torch.where((t == -100)[:, None], torch.full_like(h, math.nan), h)
+    for a, b in zip(torch.autograd.grad(ops.linear_cross_entropy(h2.requires_grad_(True), w.requires_grad_(True), t, reduction="mean"), [h2, w], torch.full((), 3.0, device="cuda")), want):
+        assert torch.equal(a, b)
+    for kind in ("target", math.nan, math.inf):
+        h3, t3 = h.detach().clone(), t.clone()
+        if kind == "target":
+            t3[5] = 400
+        else:
+            h3[5, 7], t3[5] = kind, 3
+        h3.requires_grad_(True)
+        loss = ops.linear_cross_entropy(h3, w, t3, reduction="sum")
+        dh, dw = torch.autograd.grad(loss, [h3, w])
+        assert loss.isnan() and dh[5].isnan().all() and dw.isnan().all()
+        assert dh[torch.arange(600, device="cuda") != 5].isfinite().all()
+
+
+def test_one_pass_may_be_walked_twice():
+    h, w, t, _, _ = make(300, 64, 400, torch.bfloat16)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    loss = ops.linear_cross_entropy(h, w, t, reduction="mean")
+    a = torch.autograd.grad(loss, [h, w], retain_graph=True)
+    a[0].zero_()
+    b = torch.autograd.grad(2 * loss, [h, w])
+    assert b[0].any() and torch.equal(b[1], 2 * a[1])
+    only = torch.autograd.grad(ops.linear_cross_entropy(h, w.detach(), t, reduction="mean"), h)[0]
+    assert torch.equal(2 * only, b[0])
+    only = torch.autograd.grad(ops.linear_cross_entropy(h.detach(), w, t, reduction="mean"), w)[0]
+    assert torch.equal(only, a[1])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_left_out_may_hold_anything(dtype):
     h, w, t, wl, wz = make(400, 96, 600, dtype, left_out=0.5)
