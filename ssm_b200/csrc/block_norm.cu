@@ -21,6 +21,7 @@ namespace ssmb {
 namespace {
 
 constexpr int kMaxRuns = 148 * 8;  // backward blocks
+constexpr int kMaxDim = 8192;
 
 template <int V>
 __device__ __forceinline__ void load_vec(const void* base, int64_t i, int dtype, float (&f)[V]) {
@@ -97,17 +98,19 @@ __device__ __forceinline__ void convert(const Raw<V>& r, int dtype, float (&f)[V
   }
 }
 
-// sums of two values over the G threads of a block
-template <int G>
+// sums of two values over a block
 __device__ __forceinline__ void allsum2(float& a, float& b, float2 (*scratch)[16], int& turn) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off), b += __shfl_xor_sync(0xffffffffu, b, off);
-  if constexpr (G > 32) {  // two rows of scratch in turn: a barrier a sum
+  const int warps = blockDim.x / 32;
+  if (warps > 1) {  // two rows of scratch in turn: a barrier a sum
     if (threadIdx.x % 32 == 0) scratch[turn][threadIdx.x / 32] = make_float2(a, b);
     __syncthreads();
     a = b = 0.f;
-#pragma unroll
-    for (int w = 0; w < G / 32; ++w) a += scratch[turn][w].x, b += scratch[turn][w].y;
+    for (int w = 0; w < warps; ++w) {
+      const float2 v = scratch[turn][w];
+      a += v.x, b += v.y;
+    }
     turn ^= 1;
   }
 }
@@ -117,8 +120,18 @@ enum Gate { kNone = 0, kChannel = 1, kSequence = 2, kToken = 3 };
 // No load of these kernels depends on a condition for its address: what a call does not have (a residual, an incoming gradient) points at what it has, with a flag to leave it
 // out, and in the forward pass a thread beyond the row's end reads the row's last piece.
 
-// Mean and 1 / std of a row; V elements to a piece, MC pieces to a thread: piece c of thread t is c G + t, and there are n of them
-template <int V, int G, int MC>
+// Types known at compile time: 0 none; 1 bf16, 2 fp16, 3 fp32 activations, gate and parameters, with a residual stream of fp32, in and out
+template <int TYPES>
+__device__ __forceinline__ int io_type(int dtype) {
+  return TYPES == 1 ? SSM_BF16 : TYPES == 2 ? SSM_F16 : TYPES == 3 ? SSM_F32 : dtype;
+}
+template <int TYPES>
+__device__ __forceinline__ int stream_type(int dtype) {
+  return TYPES ? SSM_F32 : dtype;
+}
+
+// Mean and 1 / std of a row; V elements to a piece, MC pieces to a thread: piece c of thread t is c blockDim + t, and there are n of them
+template <int V, int MC>
 __device__ __forceinline__ void row_stats(const float (&f)[MC][V], int n, float inv, bool rms, float eps, float2 (*scratch)[16], int& turn, float& mean, float& rstd) {
   float t = 0.f, q = 0.f;
   mean = 0.f;
@@ -126,37 +139,23 @@ __device__ __forceinline__ void row_stats(const float (&f)[MC][V], int n, float 
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) t += c * G + (int)threadIdx.x < n ? f[c][k] : 0.f;
+      for (int k = 0; k < V; ++k) t += (int)(c * blockDim.x + threadIdx.x) < n ? f[c][k] : 0.f;
     }
-    allsum2<G>(t, q, scratch, turn);
+    allsum2(t, q, scratch, turn);
     mean = t * inv, q = 0.f;
   }
 #pragma unroll
   for (int c = 0; c < MC; ++c) {
+    const bool live = (int)(c * blockDim.x + threadIdx.x) < n;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float d = c * G + (int)threadIdx.x < n ? f[c][k] - mean : 0.f;
+      const float d = live ? f[c][k] - mean : 0.f;
       q = fmaf(d, d, q);
     }
   }
   t = 0.f;
-  allsum2<G>(q, t, scratch, turn);
+  allsum2(q, t, scratch, turn);
   rstd = rsqrtf(q * inv + eps);
-}
-
-// h, n and the factor of n in r, for a row's piece; w is left as post_weight
-template <int V, bool BIAS, bool GATE>
-__device__ __forceinline__ void branch(const ssm_block_norm_args& a, int col, int64_t gate_at, float m1, float s1, const float (&x)[V], float (&h)[V], float (&n)[V], float (&ga)[V],
-                                       float (&w)[V]) {
-  load_vec<V>(a.post_weight, col, a.param_dtype, w);
-  if (BIAS) load_vec<V>(a.post_bias, col, a.param_dtype, n);
-  if (GATE) load_vec<V>(a.gate, gate_at + col, a.gate_dtype, ga);
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    h[k] = (x[k] - m1) * s1;
-    n[k] = BIAS ? fmaf(h[k], w[k], n[k]) : h[k] * w[k];
-    ga[k] = GATE ? a.scale * ga[k] : a.scale;
-  }
 }
 
 struct FwdArgs {
@@ -164,47 +163,55 @@ struct FwdArgs {
   int len, has_r;  // rows of a sequence; the residual is one
 };
 
-template <int V, int G, int MC, bool BIAS, bool GATE>
-__global__ void __launch_bounds__(G) block_norm_kernel(const __grid_constant__ FwdArgs args) {
+template <int V, int MC, bool BIAS, bool GATE, int TYPES>
+__global__ void __launch_bounds__(512) block_norm_kernel(const __grid_constant__ FwdArgs args) {
   const ssm_block_norm_args& a = args.a;
   __shared__ float2 scratch[2][16];
   int turn = 0;
-  const int tid = threadIdx.x, dim = a.dim, n = dim / V, row = blockIdx.x;
+  const int io = io_type<TYPES>(a.io_dtype), rt = stream_type<TYPES>(a.res_dtype), ot = stream_type<TYPES>(a.resout_dtype), pt = io_type<TYPES>(a.param_dtype), gt = io_type<TYPES>(a.gate_dtype);
+  const bool has_r = TYPES || args.has_r;
+  const int tid = threadIdx.x, threads = blockDim.x, dim = a.dim, n = dim / V, row = blockIdx.x;
   const float inv = 1.f / (float)dim;
   const int64_t at = (int64_t)row * dim, gate_at = a.gate_kind == kToken ? at : a.gate_kind == kSequence ? (int64_t)(row / args.len) * dim : 0;
   float v[MC][V];
   Raw<V> rx[MC], rr[MC];
+  int col[MC];
 #pragma unroll
-  for (int c = 0; c < MC; ++c) issue<V>(a.x, at + min(c * G + tid, n - 1) * V, a.io_dtype, rx[c]);
+  for (int c = 0; c < MC; ++c) col[c] = min(c * threads + tid, n - 1) * V;
 #pragma unroll
-  for (int c = 0; c < MC; ++c) issue<V>(a.residual, at + min(c * G + tid, n - 1) * V, a.res_dtype, rr[c]);
+  for (int c = 0; c < MC; ++c) issue<V>(a.x, at + col[c], io, rx[c]);
 #pragma unroll
-  for (int c = 0; c < MC; ++c) convert<V>(rx[c], a.io_dtype, v[c]);
+  for (int c = 0; c < MC; ++c) issue<V>(a.residual, at + col[c], rt, rr[c]);
+#pragma unroll
+  for (int c = 0; c < MC; ++c) convert<V>(rx[c], io, v[c]);
   float m1, s1, m2, s2;
-  row_stats<V, G, MC>(v, n, inv, a.is_rms, a.post_eps, scratch, turn, m1, s1);
+  row_stats<V, MC>(v, n, inv, a.is_rms, a.post_eps, scratch, turn, m1, s1);
 #pragma unroll
   for (int c = 0; c < MC; ++c) {
-    const int col = min(c * G + tid, n - 1) * V;
-    float h[V], b[V], ga[V], w[V], r[V];
-    branch<V, BIAS, GATE>(a, col, gate_at, m1, s1, v[c], h, b, ga, w);
-    convert<V>(rr[c], a.res_dtype, r);
+    float b[V], ga[V], w[V], r[V];
+    load_vec<V>(a.post_weight, col[c], pt, w);
+    if (BIAS) load_vec<V>(a.post_bias, col[c], pt, b);
+    if (GATE) load_vec<V>(a.gate, gate_at + col[c], gt, ga);
+    convert<V>(rr[c], rt, r);
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[c][k] = args.has_r ? fmaf(ga[k], b[k], r[k]) : ga[k] * b[k];
-    if (c * G + tid < n) store_vec<V>(a.residual_out, at + col, a.resout_dtype, v[c]);
+    for (int k = 0; k < V; ++k) {
+      const float h = (v[c][k] - m1) * s1, y = BIAS ? fmaf(h, w[k], b[k]) : h * w[k], f = GATE ? a.scale * ga[k] : a.scale;
+      v[c][k] = has_r ? fmaf(f, y, r[k]) : f * y;
+    }
+    if (c * threads + tid < n) store_vec<V>(a.residual_out, at + col[c], ot, v[c]);
   }
-  row_stats<V, G, MC>(v, n, inv, a.is_rms, a.eps, scratch, turn, m2, s2);
+  row_stats<V, MC>(v, n, inv, a.is_rms, a.eps, scratch, turn, m2, s2);
 #pragma unroll
   for (int c = 0; c < MC; ++c) {
-    const int col = min(c * G + tid, n - 1) * V;
     float w[V], b[V], y[V];
-    load_vec<V>(a.weight, col, a.param_dtype, w);
-    if (BIAS) load_vec<V>(a.bias, col, a.param_dtype, b);
+    load_vec<V>(a.weight, col[c], pt, w);
+    if (BIAS) load_vec<V>(a.bias, col[c], pt, b);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const float h = (v[c][k] - m2) * s2;
       y[k] = BIAS ? fmaf(h, w[k], b[k]) : h * w[k];
     }
-    if (c * G + tid < n) store_vec<V>(a.y, at + col, a.io_dtype, y);
+    if (c * threads + tid < n) store_vec<V>(a.y, at + col[c], io, y);
   }
   if (a.stats && tid == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(m1, s1, m2, s2);
 }
@@ -212,13 +219,9 @@ __global__ void __launch_bounds__(G) block_norm_kernel(const __grid_constant__ F
 // where a run of rows leaves its sums: [run][which][dim]; which: dpost_weight, dweight, dpost_bias, dbias, dgate (of its first sequence, of its last)
 constexpr int kSlots = 6;
 
-// The backward pass of a run of rows.  V elements to a piece, piece c of thread t is c G + t.  A row's chain is long (loads, two rounds of sums, stores), so the next row is on its way
+// The backward pass of a run of rows.  V elements to a piece, piece c of thread t is c blockDim + t.  A row's chain is long (loads, two rounds of sums, stores), so the next row is on its way
 // into shared memory while this one is worked on: each thread copies its own pieces (asynchronous copies, no barrier) and reads them there again where it needs them,
-// which leaves the registers to the sums of its columns.
-template <int V, int G, int MC>
-struct RowRing {
-  static constexpr int kBytes = MC * G * V * 4;  // of one tensor, 32-bit elements
-};
+// which leaves the registers to the sums of its columns.  The parameters, and a gate per channel or sequence, lie beside them in fp32, loaded once (a sequence).
 template <int V>
 __device__ __forceinline__ void copy_piece(uint32_t dst, const void* base, int64_t i, int dtype) {
   if constexpr (V == 4) {
@@ -229,9 +232,13 @@ __device__ __forceinline__ void copy_piece(uint32_t dst, const void* base, int64
       const uint16_t* src = reinterpret_cast<const uint16_t*>(base) + i;
       asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
     }
-  } else {  // element by element, through the registers
-    if (dtype == SSM_F32) asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(dst), "r"(reinterpret_cast<const uint32_t*>(base)[i]) : "memory");
-    else asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(dst), "r"((uint32_t) reinterpret_cast<const uint16_t*>(base)[i]) : "memory");
+  } else {
+    if (dtype == SSM_F32) {
+      const float* src = reinterpret_cast<const float*>(base) + i;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
+    } else {  // through a register
+      asm volatile("st.shared.b16 [%0], %1;\n" ::"r"(dst), "h"(reinterpret_cast<const uint16_t*>(base)[i]) : "memory");
+    }
   }
 }
 template <int V>
@@ -245,10 +252,9 @@ __device__ __forceinline__ void read_piece(const unsigned char* at, int dtype, f
       halves(v.x, dtype, f[0], f[1]), halves(v.y, dtype, f[2], f[3]);
     }
   } else {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(at);
     float hi;
-    if (dtype == SSM_F32) f[0] = __uint_as_float(v);
-    else halves(v, dtype, f[0], hi);
+    if (dtype == SSM_F32) f[0] = *reinterpret_cast<const float*>(at);
+    else halves(*reinterpret_cast<const uint16_t*>(at), dtype, f[0], hi);
   }
 }
 
@@ -256,20 +262,24 @@ struct BwdArgs {
   ssm_block_norm_bwd_args g;
   int rows, per, len, unit;  // rows in all, of a run, of a sequence, that share a gate
   int stages, has_r, has_d, d_dtype;  // rows in shared memory; the residual is one, and the gradient that came through it
+  int o_dy, o_r, o_d, o_g, stage;     // places in a row's part of shared memory, its size; parameters behind the rows
 };
 
-template <int V, int G, int MC, bool BIAS, bool GATE>
-__global__ void __launch_bounds__(G) block_norm_bwd_kernel(const __grid_constant__ BwdArgs args) {
+template <int V, int MC, bool BIAS, int GATE, int TYPES>  // GATE: 0 none, 1 per channel or sequence, 2 per token
+__global__ void __launch_bounds__(512) block_norm_bwd_kernel(const __grid_constant__ BwdArgs args) {
   const ssm_block_norm_bwd_args& g = args.g;
   const ssm_block_norm_args& a = g.fwd;
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float2 scratch[2][16];
-  constexpr int kT = RowRing<V, G, MC>::kBytes, kB = BIAS ? MC : 1, kG = GATE ? MC : 1;
+  constexpr int kB = BIAS ? MC : 1, kG = GATE == 1 ? MC : 1;
+  constexpr bool kCached = MC * V <= 8;  // the parameters of rows of up to 4096 columns have room in shared memory
+  const int io = io_type<TYPES>(a.io_dtype), rt = stream_type<TYPES>(a.res_dtype), dt = stream_type<TYPES>(args.d_dtype), pt = io_type<TYPES>(a.param_dtype), gt = io_type<TYPES>(a.gate_dtype);
+  const int ie = io == SSM_F32 ? 4 : 2, re = rt == SSM_F32 ? 4 : 2, de = dt == SSM_F32 ? 4 : 2, ge = gt == SSM_F32 ? 4 : 2;
+  const bool has_r = TYPES || args.has_r, has_d = TYPES || args.has_d, two = args.stages == 2;
   int turn = 0;
-  const int tid = threadIdx.x, dim = a.dim, n = dim / V;
+  const int tid = threadIdx.x, threads = blockDim.x, dim = a.dim, n = dim / V;
   const float inv = 1.f / (float)dim;
   const int first = blockIdx.x * args.per, last = min(args.rows, first + args.per);
-  const bool has_r = args.has_r, has_d = args.has_d, two = args.stages == 2;
   float dpw[MC][V], dw[MC][V], dpb[kB][V], db[kB][V], dg[kG][V];
 #pragma unroll
   for (int c = 0; c < MC; ++c) {
@@ -277,50 +287,115 @@ __global__ void __launch_bounds__(G) block_norm_bwd_kernel(const __grid_constant
     for (int k = 0; k < V; ++k) {
       dpw[c][k] = dw[c][k] = 0.f;
       if (BIAS) dpb[BIAS ? c : 0][k] = db[BIAS ? c : 0][k] = 0.f;
-      if (GATE) dg[GATE ? c : 0][k] = 0.f;
+      if (GATE == 1) dg[GATE == 1 ? c : 0][k] = 0.f;
     }
   }
   float* const part = g.partial + (int64_t)blockIdx.x * kSlots * dim;
   const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
-
-  int stage = 0;
-  for (int next = first; next <= last; ++next) {  // the row `next` sets out, the one before it is worked on
-    const int into = two ? (next - first) & 1 : 0;
-    if (next < last && (two || next == first)) {
-      const int64_t at = (int64_t)next * dim;
+  // post_weight, weight, post_bias, gate times scale: [which][dim], a thread's own pieces
+  float* const par = reinterpret_cast<float*>(ring + args.stages * args.stage);
+  const int dim4 = (dim + 3) / 4 * 4;
 #pragma unroll
-      for (int c = 0; c < MC; ++c) {
-        const int p = c * G + tid;
-        if (p < n) {
-          const uint32_t to = ring0 + into * 4 * kT + p * V * 4;
-          copy_piece<V>(to, a.x, at + p * V, a.io_dtype);
-          copy_piece<V>(to + kT, g.dy, at + p * V, a.io_dtype);
-          copy_piece<V>(to + 2 * kT, a.residual, at + p * V, a.res_dtype);
-          copy_piece<V>(to + 3 * kT, g.dresidual_out, at + p * V, args.d_dtype);
-        }
+  for (int c = 0; c < MC; ++c) {
+    const int p = c * threads + tid;
+    if (kCached && p < n) {
+      float w[V];
+      load_vec<V>(a.post_weight, p * V, pt, w);
+#pragma unroll
+      for (int k = 0; k < V; ++k) par[p * V + k] = w[k];
+      load_vec<V>(a.weight, p * V, pt, w);
+#pragma unroll
+      for (int k = 0; k < V; ++k) par[dim4 + p * V + k] = w[k];
+      if (BIAS) {
+        load_vec<V>(a.post_bias, p * V, pt, w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) par[2 * dim4 + p * V + k] = w[k];
       }
     }
-    asm volatile("cp.async.commit_group;\n" ::: "memory");
-    if (next == first) continue;
-    if (two) asm volatile("cp.async.wait_group 1;\n" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-    const int row = next - 1;
-    const int64_t at = (int64_t)row * dim, gate_at = a.gate_kind == kToken ? at : a.gate_kind == kSequence ? (int64_t)(row / args.len) * dim : 0;
-    const unsigned char* const mine = ring + stage * 4 * kT;
+  }
+  auto set_out = [&](int row, int into) {
+    const int64_t at = (int64_t)row * dim;
+    const uint32_t to = ring0 + into * args.stage;
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+      const int p = c * threads + tid;
+      if (p < n) {
+        copy_piece<V>(to + p * V * ie, a.x, at + p * V, io);
+        copy_piece<V>(to + args.o_dy + p * V * ie, g.dy, at + p * V, io);
+        copy_piece<V>(to + args.o_r + p * V * re, a.residual, at + p * V, rt);
+        copy_piece<V>(to + args.o_d + p * V * de, g.dresidual_out, at + p * V, dt);
+        if (GATE == 2) copy_piece<V>(to + args.o_g + p * V * ge, a.gate, at + p * V, gt);
+      }
+    }
+  };
+
+  int stage = 0, gate_of = -1;
+  if (two && first < last) set_out(first, 0);
+  asm volatile("cp.async.commit_group;\n" ::: "memory");
+  for (int row = first; row < last; ++row) {
+    if (two) {
+      if (row + 1 < last) set_out(row + 1, stage ^ 1);
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+      asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+    } else {
+      set_out(row, 0);
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+      asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    }
+    const int64_t at = (int64_t)row * dim;
+    const unsigned char* const mine = ring + stage * args.stage;
     const float4 stats = reinterpret_cast<const float4*>(a.stats)[row];
     const float m1 = stats.x, s1 = stats.y, m2 = stats.z, s2 = stats.w;
+    const int64_t gate_at = GATE == 1 ? (int64_t)(row / args.unit) * dim : 0;
+    if (GATE == 1 && kCached) {
+      const int seq = row / args.unit;
+      if (seq != gate_of) {  // a thread's own pieces: no barrier
+#pragma unroll
+        for (int c = 0; c < MC; ++c) {
+          const int p = c * threads + tid;
+          if (p < n) {
+            float w[V];
+            load_vec<V>(a.gate, (int64_t)seq * dim + p * V, gt, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) par[3 * dim4 + p * V + k] = a.scale * w[k];
+          }
+        }
+        gate_of = seq;
+      }
+    }
+    auto param = [&](int which, const void* from, int p, float (&w)[V]) {
+      if (kCached) read_piece<V>(reinterpret_cast<const unsigned char*>(par + which * dim4 + p * V), SSM_F32, w);
+      else load_vec<V>(from, p * V, pt, w);
+    };
+    // h, n and the factor of n in r, for a piece
+    auto branch = [&](int p, float (&h)[V], float (&nn)[V], float (&ga)[V], float (&w)[V]) {
+      float x[V], b[V];
+      read_piece<V>(mine + p * V * ie, io, x);
+      param(0, a.post_weight, p, w);
+      if (BIAS) param(2, a.post_bias, p, b);
+      if (GATE == 1) {
+        if (kCached) read_piece<V>(reinterpret_cast<const unsigned char*>(par + 3 * dim4 + p * V), SSM_F32, ga);
+        else load_vec<V>(a.gate, gate_at + p * V, gt, ga);
+      }
+      if (GATE == 2) read_piece<V>(mine + args.o_g + p * V * ge, gt, ga);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        h[k] = (x[k] - m1) * s1;
+        nn[k] = BIAS ? fmaf(h[k], w[k], b[k]) : h[k] * w[k];
+        ga[k] = GATE == 2 || (GATE == 1 && !kCached) ? a.scale * ga[k] : GATE == 1 ? ga[k] : a.scale;
+      }
+    };
     float h2[MC][V], d[MC][V];
     float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
-      const int p = c * G + tid;
+      const int p = c * threads + tid;
       if (p < n) {
-        float x[V], h[V], b[V], ga[V], w[V], r[V], dy[V];
-        read_piece<V>(mine + p * V * 4, a.io_dtype, x);
-        branch<V, BIAS, GATE>(a, p * V, gate_at, m1, s1, x, h, b, ga, w);
-        read_piece<V>(mine + kT + p * V * 4, a.io_dtype, dy);
-        read_piece<V>(mine + 2 * kT + p * V * 4, a.res_dtype, r);
-        load_vec<V>(a.weight, p * V, a.param_dtype, w);
+        float h[V], b[V], ga[V], w[V], r[V], dy[V];
+        branch(p, h, b, ga, w);
+        read_piece<V>(mine + args.o_dy + p * V * ie, io, dy);
+        read_piece<V>(mine + args.o_r + p * V * re, rt, r);
+        param(1, a.weight, p, w);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           const float v = has_r ? fmaf(ga[k], b[k], r[k]) : ga[k] * b[k];
@@ -332,85 +407,273 @@ __global__ void __launch_bounds__(G) block_norm_bwd_kernel(const __grid_constant
         }
       }
     }
-    allsum2<G>(sum0, sum1, scratch, turn);
+    allsum2(sum0, sum1, scratch, turn);
     const float c2 = a.is_rms ? 0.f : sum0 * inv, e2 = sum1 * inv;
     sum0 = sum1 = 0.f;
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
-      const int p = c * G + tid;
+      const int p = c * threads + tid;
       if (p < n) {
-        float x[V], h[V], b[V], ga[V], w[V], o[V], gg[V];
-        read_piece<V>(mine + p * V * 4, a.io_dtype, x);
-        branch<V, BIAS, GATE>(a, p * V, gate_at, m1, s1, x, h, b, ga, w);
-        read_piece<V>(mine + 3 * kT + p * V * 4, args.d_dtype, o);
+        float h[V], b[V], ga[V], w[V], o[V], gg[V];
+        branch(p, h, b, ga, w);
+        read_piece<V>(mine + args.o_d + p * V * de, dt, o);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           float t = s2 * (d[c][k] - c2 - h2[c][k] * e2);
           if (has_d) t += o[k];
           o[k] = t;
           gg[k] = a.scale * t * b[k];
-          if (GATE) dg[GATE ? c : 0][k] += gg[k];
+          if (GATE == 1) dg[GATE == 1 ? c : 0][k] += gg[k];
           const float dn = ga[k] * t;
           dpw[c][k] = fmaf(dn, h[k], dpw[c][k]);
           if (BIAS) dpb[BIAS ? c : 0][k] += dn;
           d[c][k] = w[k] * dn;
           sum0 += d[c][k], sum1 = fmaf(d[c][k], h[k], sum1);
         }
-        if (g.dresidual) store_vec<V>(g.dresidual, at + p * V, a.res_dtype, o);
-        if (a.gate_kind == kToken) store_vec<V>(g.dgate, at + p * V, a.gate_dtype, gg);
+        if (TYPES || g.dresidual) store_vec<V>(g.dresidual, at + p * V, rt, o);
+        if (GATE == 2) store_vec<V>(g.dgate, at + p * V, gt, gg);
       }
     }
-    allsum2<G>(sum0, sum1, scratch, turn);
+    allsum2(sum0, sum1, scratch, turn);
     const float c1 = a.is_rms ? 0.f : sum0 * inv, e1 = sum1 * inv;
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
-      const int p = c * G + tid;
+      const int p = c * threads + tid;
       if (p < n) {
         float x[V];
-        read_piece<V>(mine + p * V * 4, a.io_dtype, x);
+        read_piece<V>(mine + p * V * ie, io, x);
 #pragma unroll
         for (int k = 0; k < V; ++k) x[k] = s1 * (d[c][k] - c1 - (x[k] - m1) * s1 * e1);
-        store_vec<V>(g.dx, at + p * V, a.io_dtype, x);
+        store_vec<V>(g.dx, at + p * V, io, x);
       }
     }
-    if (GATE && a.gate_kind != kToken && (row + 1 == last || (row + 1) % args.unit == 0)) {  // the gate's rows end here, or the run does
+    if (GATE == 1 && (row + 1 == last || (row + 1) % args.unit == 0)) {  // the gate's rows end here, or the run does
       const int seq = row / args.unit, begin = seq * args.unit, end = begin + args.unit;
 #pragma unroll
       for (int c = 0; c < MC; ++c) {
-        const int p = c * G + tid;
+        const int p = c * threads + tid;
         if (p < n) {
-          if (begin >= first && end <= last) store_vec<V>(g.dgate, (int64_t)seq * dim + p * V, a.gate_dtype, dg[GATE ? c : 0]);
-          else if (begin < first) store_vec<V>(part, 4 * dim + p * V, SSM_F32, dg[GATE ? c : 0]);
-          else store_vec<V>(part, 5 * dim + p * V, SSM_F32, dg[GATE ? c : 0]);
+          if (begin >= first && end <= last) store_vec<V>(g.dgate, (int64_t)seq * dim + p * V, gt, dg[GATE == 1 ? c : 0]);
+          else if (begin < first) store_vec<V>(part, 4 * dim + p * V, SSM_F32, dg[GATE == 1 ? c : 0]);
+          else store_vec<V>(part, 5 * dim + p * V, SSM_F32, dg[GATE == 1 ? c : 0]);
 #pragma unroll
-          for (int k = 0; k < V; ++k) dg[GATE ? c : 0][k] = 0.f;
+          for (int k = 0; k < V; ++k) dg[GATE == 1 ? c : 0][k] = 0.f;
         }
       }
     }
     stage = two ? stage ^ 1 : 0;
-    if (!two && next < last) {  // one row's room: the next one sets out now
-      const int64_t to_row = (int64_t)next * dim;
-#pragma unroll
-      for (int c = 0; c < MC; ++c) {
-        const int p = c * G + tid;
-        if (p < n) {
-          const uint32_t to = ring0 + p * V * 4;
-          copy_piece<V>(to, a.x, to_row + p * V, a.io_dtype);
-          copy_piece<V>(to + kT, g.dy, to_row + p * V, a.io_dtype);
-          copy_piece<V>(to + 2 * kT, a.residual, to_row + p * V, a.res_dtype);
-          copy_piece<V>(to + 3 * kT, g.dresidual_out, to_row + p * V, args.d_dtype);
-        }
-      }
-    }
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 #pragma unroll
   for (int c = 0; c < MC; ++c) {
-    const int p = c * G + tid;
+    const int p = c * threads + tid;
     if (p < n) {
       store_vec<V>(part, p * V, SSM_F32, dpw[c]);
       store_vec<V>(part, dim + p * V, SSM_F32, dw[c]);
       if (BIAS) store_vec<V>(part, 2 * dim + p * V, SSM_F32, dpb[BIAS ? c : 0]), store_vec<V>(part, 3 * dim + p * V, SSM_F32, db[BIAS ? c : 0]);
+    }
+  }
+}
+
+// The same for pieces of four, in pairs of fp32 (one instruction for two).  THREADS: at most; rows of up to 2560 columns leave room for two blocks to an SM.
+// 16384 rows of 2560 bf16 columns: scalar arithmetic, 91 instructions an element, one block to an SM: 254 us.
+struct Quad {
+  float2 a, b;
+};
+__device__ __forceinline__ Quad quad(float x) { return {make_float2(x, x), make_float2(x, x)}; }
+__device__ __forceinline__ Quad fma4(const Quad& x, const Quad& y, const Quad& z) { return {__ffma2_rn(x.a, y.a, z.a), __ffma2_rn(x.b, y.b, z.b)}; }
+__device__ __forceinline__ Quad mul4(const Quad& x, const Quad& y) { return {__fmul2_rn(x.a, y.a), __fmul2_rn(x.b, y.b)}; }
+__device__ __forceinline__ Quad add4(const Quad& x, const Quad& y) { return {__fadd2_rn(x.a, y.a), __fadd2_rn(x.b, y.b)}; }
+__device__ __forceinline__ float sum4(const Quad& x) { return (x.a.x + x.a.y) + (x.b.x + x.b.y); }
+__device__ __forceinline__ Quad read_quad(const unsigned char* at, int dtype) {
+  Quad q;
+  if (dtype == SSM_F32) {
+    const float4 v = *reinterpret_cast<const float4*>(at);
+    q.a = make_float2(v.x, v.y), q.b = make_float2(v.z, v.w);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    halves(v.x, dtype, q.a.x, q.a.y), halves(v.y, dtype, q.b.x, q.b.y);
+  }
+  return q;
+}
+__device__ __forceinline__ Quad load_quad(const void* base, int64_t i, int dtype) {
+  float f[4];
+  load_param_vec<4>(base, i, dtype, f);
+  return {make_float2(f[0], f[1]), make_float2(f[2], f[3])};
+}
+__device__ __forceinline__ void store_quad(void* base, int64_t i, int dtype, const Quad& q) {
+  const float f[4] = {q.a.x, q.a.y, q.b.x, q.b.y};
+  store_vec<4>(base, i, dtype, f);
+}
+
+template <int THREADS, int MC, bool BIAS, int GATE, int TYPES>  // GATE: 0 none, 1 per channel or sequence, 2 per token
+__global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1) block_norm_bwd4_kernel(const __grid_constant__ BwdArgs args) {
+  const ssm_block_norm_bwd_args& g = args.g;
+  const ssm_block_norm_args& a = g.fwd;
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float2 scratch[2][16];
+  constexpr int kB = BIAS ? MC : 1, kG = GATE == 1 ? MC : 1;
+  constexpr bool kCached = MC <= 2;  // the parameters of rows of up to 4096 columns have room in shared memory
+  const int io = io_type<TYPES>(a.io_dtype), rt = stream_type<TYPES>(a.res_dtype), dt = stream_type<TYPES>(args.d_dtype), pt = io_type<TYPES>(a.param_dtype), gt = io_type<TYPES>(a.gate_dtype);
+  const int ie = io == SSM_F32 ? 16 : 8, re = rt == SSM_F32 ? 16 : 8, de = dt == SSM_F32 ? 16 : 8, ge = gt == SSM_F32 ? 16 : 8;
+  const bool has_r = TYPES || args.has_r, has_d = TYPES || args.has_d, two = args.stages == 2, rms = a.is_rms;
+  int turn = 0;
+  const int tid = threadIdx.x, threads = blockDim.x, dim = a.dim, n = dim / 4;
+  const float inv = 1.f / (float)dim;
+  const int first = blockIdx.x * args.per, last = min(args.rows, first + args.per);
+  Quad dpw[MC], dw[MC], dpb[kB], db[kB], dg[kG];
+#pragma unroll
+  for (int c = 0; c < MC; ++c) {
+    dpw[c] = dw[c] = quad(0.f);
+    if (BIAS) dpb[BIAS ? c : 0] = db[BIAS ? c : 0] = quad(0.f);
+    if (GATE == 1) dg[GATE == 1 ? c : 0] = quad(0.f);
+  }
+  float* const part = g.partial + (int64_t)blockIdx.x * kSlots * dim;
+  const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
+  unsigned char* const par = ring + args.stages * args.stage;  // post_weight, weight, post_bias, gate times scale: [which][dim] fp32, a thread's own pieces
+  const Quad scale4 = quad(a.scale);
+#pragma unroll
+  for (int c = 0; c < MC; ++c) {
+    const int p = c * threads + tid;
+    if (kCached && p < n) {
+      Quad w = load_quad(a.post_weight, p * 4, pt);
+      *reinterpret_cast<float4*>(par + p * 16) = make_float4(w.a.x, w.a.y, w.b.x, w.b.y);
+      w = load_quad(a.weight, p * 4, pt);
+      *reinterpret_cast<float4*>(par + (n + p) * 16) = make_float4(w.a.x, w.a.y, w.b.x, w.b.y);
+      if (BIAS) {
+        w = load_quad(a.post_bias, p * 4, pt);
+        *reinterpret_cast<float4*>(par + (2 * n + p) * 16) = make_float4(w.a.x, w.a.y, w.b.x, w.b.y);
+      }
+    }
+  }
+  auto set_out = [&](int row, int into) {
+    const int64_t at = (int64_t)row * dim;
+    const uint32_t to = ring0 + into * args.stage;
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+      const int p = c * threads + tid;
+      if (p < n) {
+        copy_piece<4>(to + p * ie, a.x, at + p * 4, io);
+        copy_piece<4>(to + args.o_dy + p * ie, g.dy, at + p * 4, io);
+        copy_piece<4>(to + args.o_r + p * re, a.residual, at + p * 4, rt);
+        copy_piece<4>(to + args.o_d + p * de, g.dresidual_out, at + p * 4, dt);
+        if (GATE == 2) copy_piece<4>(to + args.o_g + p * ge, a.gate, at + p * 4, gt);
+      }
+    }
+  };
+
+  int stage = 0, gate_of = -1;
+  if (two && first < last) set_out(first, 0);
+  asm volatile("cp.async.commit_group;\n" ::: "memory");
+  float4 stats = first < last ? __ldg(reinterpret_cast<const float4*>(a.stats) + first) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int row = first; row < last; ++row) {
+    const float4 now = stats;
+    if (row + 1 < last) stats = __ldg(reinterpret_cast<const float4*>(a.stats) + row + 1);
+    if (two) {
+      if (row + 1 < last) set_out(row + 1, stage ^ 1);
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+      asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+    } else {
+      set_out(row, 0);
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+      asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    }
+    const int64_t at = (int64_t)row * dim;
+    const unsigned char* const mine = ring + stage * args.stage;
+    const Quad s1 = quad(now.y), o1 = quad(-now.x * now.y), s2 = quad(now.w), o2 = quad(-now.z * now.w);  // h = x s1 + o1
+    const int64_t gate_at = GATE == 1 ? (int64_t)(row / args.unit) * dim : 0;
+    if (GATE == 1 && kCached) {
+      const int seq = row / args.unit;
+      if (seq != gate_of) {  // a thread's own pieces: no barrier
+#pragma unroll
+        for (int c = 0; c < MC; ++c) {
+          const int p = c * threads + tid;
+          if (p < n) {
+            const Quad w = mul4(load_quad(a.gate, gate_at + p * 4, gt), scale4);
+            *reinterpret_cast<float4*>(par + (3 * n + p) * 16) = make_float4(w.a.x, w.a.y, w.b.x, w.b.y);
+          }
+        }
+        gate_of = seq;
+      }
+    }
+    auto param = [&](int which, const void* from, int p) { return kCached ? read_quad(par + (which * n + p) * 16, SSM_F32) : load_quad(from, p * 4, pt); };
+    auto factor = [&](int p) {  // of n in r
+      if (GATE == 1) return kCached ? read_quad(par + (3 * n + p) * 16, SSM_F32) : mul4(load_quad(a.gate, gate_at + p * 4, gt), scale4);
+      if (GATE == 2) return mul4(read_quad(mine + args.o_g + p * ge, gt), scale4);
+      return scale4;
+    };
+    Quad h2[MC], d[MC];
+    Quad sum = quad(0.f), dot = quad(0.f);
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+      const int p = c * threads + tid;
+      if (p < n) {
+        const Quad h = fma4(read_quad(mine + p * ie, io), s1, o1), w1 = param(0, a.post_weight, p), y = BIAS ? fma4(h, w1, param(2, a.post_bias, p)) : mul4(h, w1);
+        const Quad v = has_r ? fma4(factor(p), y, read_quad(mine + args.o_r + p * re, rt)) : mul4(factor(p), y), dy = read_quad(mine + args.o_dy + p * ie, io);
+        h2[c] = fma4(v, s2, o2);
+        dw[c] = fma4(dy, h2[c], dw[c]);
+        if (BIAS) db[BIAS ? c : 0] = add4(db[BIAS ? c : 0], dy);
+        d[c] = mul4(param(1, a.weight, p), dy);
+        if (!rms) sum = add4(sum, d[c]);
+        dot = fma4(d[c], h2[c], dot);
+      }
+    }
+    float sum0 = sum4(sum), sum1 = sum4(dot);
+    allsum2(sum0, sum1, scratch, turn);
+    const Quad k2 = quad(-now.w * sum0 * inv), e2 = quad(-sum1 * inv);  // -s2 mean g, -mean(g h)
+    sum = dot = quad(0.f);
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+      const int p = c * threads + tid;
+      if (p < n) {
+        const Quad h = fma4(read_quad(mine + p * ie, io), s1, o1), w1 = param(0, a.post_weight, p), y = BIAS ? fma4(h, w1, param(2, a.post_bias, p)) : mul4(h, w1);
+        Quad t = fma4(h2[c], e2, d[c]);
+        t = has_d ? fma4(t, s2, read_quad(mine + args.o_d + p * de, dt)) : mul4(t, s2);
+        if (!rms) t = add4(t, k2);
+        if (TYPES || g.dresidual) store_quad(g.dresidual, at + p * 4, rt, t);
+        if (GATE == 1) dg[GATE == 1 ? c : 0] = fma4(t, y, dg[GATE == 1 ? c : 0]);
+        if (GATE == 2) store_quad(g.dgate, at + p * 4, gt, mul4(mul4(t, scale4), y));
+        const Quad dn = mul4(factor(p), t);
+        dpw[c] = fma4(dn, h, dpw[c]);
+        if (BIAS) dpb[BIAS ? c : 0] = add4(dpb[BIAS ? c : 0], dn);
+        d[c] = mul4(w1, dn);
+        h2[c] = h;
+        if (!rms) sum = add4(sum, d[c]);
+        dot = fma4(d[c], h, dot);
+      }
+    }
+    sum0 = sum4(sum), sum1 = sum4(dot);
+    allsum2(sum0, sum1, scratch, turn);
+    const Quad k1 = quad(-now.y * sum0 * inv), e1 = quad(-sum1 * inv);
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+      const int p = c * threads + tid;
+      if (p < n) store_quad(g.dx, at + p * 4, io, rms ? mul4(fma4(h2[c], e1, d[c]), s1) : fma4(fma4(h2[c], e1, d[c]), s1, k1));
+    }
+    if (GATE == 1 && (row + 1 == last || (row + 1) % args.unit == 0)) {  // the gate's rows end here, or the run does
+      const int seq = row / args.unit, begin = seq * args.unit, end = begin + args.unit;
+#pragma unroll
+      for (int c = 0; c < MC; ++c) {
+        const int p = c * threads + tid;
+        if (p < n) {
+          const Quad v = mul4(dg[GATE == 1 ? c : 0], scale4);
+          if (begin >= first && end <= last) store_quad(g.dgate, (int64_t)seq * dim + p * 4, gt, v);
+          else if (begin < first) store_quad(part, 4 * dim + p * 4, SSM_F32, v);
+          else store_quad(part, 5 * dim + p * 4, SSM_F32, v);
+          dg[GATE == 1 ? c : 0] = quad(0.f);
+        }
+      }
+    }
+    stage = two ? stage ^ 1 : 0;
+  }
+  asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < MC; ++c) {
+    const int p = c * threads + tid;
+    if (p < n) {
+      store_quad(part, p * 4, SSM_F32, dpw[c]);
+      store_quad(part, dim + p * 4, SSM_F32, dw[c]);
+      if (BIAS) store_quad(part, 2 * dim + p * 4, SSM_F32, dpb[BIAS ? c : 0]), store_quad(part, 3 * dim + p * 4, SSM_F32, db[BIAS ? c : 0]);
     }
   }
 }
@@ -422,8 +685,8 @@ struct FoldArgs {
   int per, runs, unit, units;  // rows of a run; runs; rows that share a gate, how often
   int dim, param_dtype, gate_dtype;
 };
-__global__ void __launch_bounds__(256) block_norm_fold_kernel(const __grid_constant__ FoldArgs f) {
-  __shared__ float sums[8][32];
+__global__ void __launch_bounds__(1024) block_norm_fold_kernel(const __grid_constant__ FoldArgs f) {
+  __shared__ float sums[32][32];
   const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
   const int col = blockIdx.x * 32 + lane;
   for (int what = blockIdx.y; what < 4 + f.units; what += gridDim.y) {
@@ -436,7 +699,8 @@ __global__ void __launch_bounds__(256) block_norm_fold_kernel(const __grid_const
     }
     float t = 0.f;
     if (here && col < f.dim) {
-      for (int r = from + slice; r < to; r += 8) {
+#pragma unroll 4
+      for (int r = from + slice; r < to; r += 32) {
         const int slot = what < 4 ? what : begin < r * f.per ? 4 : 5;
         t += f.partial[((int64_t)r * kSlots + slot) * f.dim + col];
       }
@@ -446,7 +710,7 @@ __global__ void __launch_bounds__(256) block_norm_fold_kernel(const __grid_const
     __syncthreads();
     if (here && slice == 0 && col < f.dim) {
 #pragma unroll
-      for (int w = 1; w < 8; ++w) t += sums[w][lane];
+      for (int w = 1; w < 32; ++w) t += sums[w][lane];
       if (what == 0) store_dyn(f.dpost_weight, col, f.param_dtype, t);
       else if (what == 1) store_dyn(f.dweight, col, f.param_dtype, t);
       else if (what == 2) store_dyn(f.dpost_bias, col, f.param_dtype, t);
@@ -456,88 +720,118 @@ __global__ void __launch_bounds__(256) block_norm_fold_kernel(const __grid_const
   }
 }
 
-// runs of neighbouring rows: as many as blocks run at once, at least one row each
-int64_t rows_per_run(int64_t rows, int threads) {
-  const int64_t runs = std::min<int64_t>(kMaxRuns, (int64_t)sm_count() * std::max(1, 1024 / threads / 2));
-  return std::max<int64_t>(1, (rows + runs - 1) / runs);
+int types_of(const ssm_block_norm_args& a) {  // see io_type
+  const bool same = a.param_dtype == a.io_dtype && (!a.gate_kind || a.gate_dtype == a.io_dtype), stream = a.residual && a.res_dtype == SSM_F32 && a.resout_dtype == SSM_F32;
+  return !same || !stream ? 0 : a.io_dtype == SSM_BF16 ? 1 : a.io_dtype == SSM_F16 ? 2 : 3;
 }
+// whole warps for `n` pieces, MC each
+int threads_for(int n, int mc) { return std::max(32, ((n + mc - 1) / mc + 31) / 32 * 32); }
 
-template <int V, int G, int MC>
+template <int V, int MC, int TYPES>
 int launch_fwd(const ssm_block_norm_args& a, cudaStream_t st) {
   FwdArgs f{a, (int)std::min<int64_t>(a.len, a.rows), a.residual != nullptr};
   if (!f.has_r) f.a.residual = a.x, f.a.res_dtype = a.io_dtype;
   const unsigned grid = (unsigned)a.rows;
+  const int threads = threads_for(a.dim / V, MC);
   if (a.bias) {
-    if (a.gate_kind) block_norm_kernel<V, G, MC, true, true><<<grid, G, 0, st>>>(f);
-    else block_norm_kernel<V, G, MC, true, false><<<grid, G, 0, st>>>(f);
+    if (a.gate_kind) block_norm_kernel<V, MC, true, true, TYPES><<<grid, threads, 0, st>>>(f);
+    else block_norm_kernel<V, MC, true, false, TYPES><<<grid, threads, 0, st>>>(f);
   } else {
-    if (a.gate_kind) block_norm_kernel<V, G, MC, false, true><<<grid, G, 0, st>>>(f);
-    else block_norm_kernel<V, G, MC, false, false><<<grid, G, 0, st>>>(f);
+    if (a.gate_kind) block_norm_kernel<V, MC, false, true, TYPES><<<grid, threads, 0, st>>>(f);
+    else block_norm_kernel<V, MC, false, false, TYPES><<<grid, threads, 0, st>>>(f);
   }
   return launch_status("block_norm_kernel");
 }
-template <int V, int G, int MC, bool BIAS, bool GATE>
+// One piece to a thread where a row is short, two up to 1024, so that all threads have work whatever the width, more only where 512 threads cannot hold the row
+template <int TYPES>
+int fwd_of(const ssm_block_norm_args& a, bool wide, cudaStream_t st) {
+  constexpr int kWide = TYPES == 3 ? 4 : 8;
+  if (TYPES && wide && a.dim % kWide == 0) {
+    const int n = a.dim / kWide;
+    if (n <= 64) return launch_fwd<kWide, 1, TYPES>(a, st);
+    if (n <= 1024) return launch_fwd<kWide, 2, TYPES>(a, st);
+    return launch_fwd<kWide, 4, TYPES>(a, st);
+  }
+  if (wide && a.dim % 4 == 0) return a.dim <= 4096 ? launch_fwd<4, 2, 0>(a, st) : launch_fwd<4, 4, 0>(a, st);
+  constexpr int kOdd = TYPES == 3 ? 3 : 0;
+  return a.dim <= 1024 ? launch_fwd<1, 2, kOdd>(a, st) : a.dim <= 4096 ? launch_fwd<1, 8, kOdd>(a, st) : launch_fwd<1, 16, kOdd>(a, st);
+}
+int dispatch_fwd(const ssm_block_norm_args& a, bool wide, cudaStream_t st) {
+  switch (types_of(a)) {
+    case 1: return fwd_of<1>(a, wide, st);
+    case 2: return fwd_of<2>(a, wide, st);
+    case 3: return fwd_of<3>(a, wide, st);
+    default: return fwd_of<0>(a, wide, st);
+  }
+}
+
+constexpr int kRing = 200 * 1024;
+template <int V, int THREADS, int MC, bool BIAS, int GATE, int TYPES>
 int launch_bwd2(const ssm_block_norm_bwd_args& g, cudaStream_t st) {
   const ssm_block_norm_args& a = g.fwd;
-  const int per = (int)rows_per_run(a.rows, G), runs = (int)((a.rows + per - 1) / per);
+  const int threads = threads_for(a.dim / V, MC);
   BwdArgs b{};
-  b.g = g, b.rows = (int)a.rows, b.per = per, b.len = (int)std::min<int64_t>(a.len, a.rows);
+  b.g = g, b.rows = (int)a.rows, b.len = (int)std::min<int64_t>(a.len, a.rows);
   b.unit = a.gate_kind == kSequence ? b.len : b.rows;
   b.has_r = a.residual != nullptr, b.has_d = g.dresidual_out != nullptr, b.d_dtype = b.has_d ? a.resout_dtype : a.io_dtype;
   if (!b.has_r) b.g.fwd.residual = a.x, b.g.fwd.res_dtype = a.io_dtype;
   if (!b.has_d) b.g.dresidual_out = g.dy;
-  constexpr int kRow = 4 * RowRing<V, G, MC>::kBytes;
-  static_assert(kRow <= 200 * 1024, "a row's pieces lie in shared memory");
-  b.stages = 2 * kRow <= 200 * 1024 ? 2 : 1;
-  const int smem = b.stages * kRow;
-  auto kern = block_norm_bwd_kernel<V, G, MC, BIAS, GATE>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  kern<<<runs, G, smem, st>>>(b);
+  auto room = [&](int dtype) { return (a.dim * dtype_size(dtype) + 15) / 16 * 16; };
+  b.o_dy = room(a.io_dtype), b.o_r = 2 * b.o_dy, b.o_d = b.o_r + room(b.g.fwd.res_dtype), b.o_g = b.o_d + room(b.d_dtype), b.stage = b.o_g + (GATE == 2 ? room(a.gate_dtype) : 0);
+  const int params = MC * V <= 8 ? (GATE == 1 ? 4 : BIAS ? 3 : 2) * ((a.dim + 3) / 4 * 16) : 0;
+  b.stages = 2 * b.stage + params <= kRing ? 2 : 1;
+  const int smem = b.stages * b.stage + params;
+  SSM_REQUIRE(smem <= 227 * 1024 - 512, SSM_ERR_TOO_LARGE, "fused_block_norm: a row does not fit");
+  void (*kern)(BwdArgs);
+  if constexpr (V == 4) kern = block_norm_bwd4_kernel<THREADS, MC, BIAS, GATE, TYPES>;
+  else kern = block_norm_bwd_kernel<V, MC, BIAS, GATE, TYPES>;
+  // what the device says of this kernel, asked once for a size (it takes longer than a launch)
+  struct Known {
+    int device = -1, threads = 0, smem = 0, fit = 0;
+  };
+  static thread_local Known known;
+  int device = 0;
+  cudaGetDevice(&device);
+  if (known.device != device || known.threads != threads || known.smem != smem) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    int fit = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, threads, smem) != cudaSuccess || fit < 1) cudaGetLastError(), fit = 1;
+    known = Known{device, threads, smem, fit * sm_count()};
+  }
+  // runs of neighbouring rows, as many as run at once
+  const int64_t most = std::min(kMaxRuns, known.fit);
+  b.per = (int)std::max<int64_t>(1, (a.rows + most - 1) / most);
+  const int runs = (int)((a.rows + b.per - 1) / b.per);
+  kern<<<runs, threads, smem, st>>>(b);
   if (const int rc = launch_status("block_norm_bwd_kernel")) return rc;
   FoldArgs f{};
   f.partial = g.partial, f.dpost_weight = g.dpost_weight, f.dweight = g.dweight, f.dpost_bias = g.dpost_bias, f.dbias = g.dbias, f.dgate = g.dgate;
-  f.per = per, f.runs = runs, f.dim = a.dim, f.param_dtype = a.param_dtype, f.gate_dtype = a.gate_dtype, f.unit = b.unit, f.units = a.gate_kind == kChannel || a.gate_kind == kSequence ? b.rows / b.unit : 0;
-  block_norm_fold_kernel<<<dim3((a.dim + 31) / 32, std::min(4 + f.units, 1024)), 256, 0, st>>>(f);
+  f.per = b.per, f.runs = runs, f.dim = a.dim, f.param_dtype = a.param_dtype, f.gate_dtype = a.gate_dtype, f.unit = b.unit, f.units = GATE == 1 ? b.rows / b.unit : 0;
+  block_norm_fold_kernel<<<dim3((a.dim + 31) / 32, std::min(4 + f.units, 1024)), 1024, 0, st>>>(f);
   return launch_status("block_norm_fold_kernel");
 }
-template <int V, int G, int MC>
+template <int V, int THREADS, int MC, int TYPES>
 int launch_bwd(const ssm_block_norm_bwd_args& g, cudaStream_t st) {
-  const bool bias = g.fwd.bias, gate = g.fwd.gate_kind;
-  if (bias) return gate ? launch_bwd2<V, G, MC, true, true>(g, st) : launch_bwd2<V, G, MC, true, false>(g, st);
-  return gate ? launch_bwd2<V, G, MC, false, true>(g, st) : launch_bwd2<V, G, MC, false, false>(g, st);
-}
-
-constexpr int kMaxDim = 8192;
-
-// threads and pieces of a row: n pieces of V elements
-#define SSM_ROW_CASES(WHAT, V, n, ...)                    \
-  if ((n) <= 32) return WHAT<V, 32, 1>(__VA_ARGS__);      \
-  if ((n) <= 64) return WHAT<V, 32, 2>(__VA_ARGS__);      \
-  if ((n) <= 128) return WHAT<V, 64, 2>(__VA_ARGS__);     \
-  if ((n) <= 256) return WHAT<V, 128, 2>(__VA_ARGS__);    \
-  if ((n) <= 384) return WHAT<V, 128, 3>(__VA_ARGS__);    \
-  if ((n) <= 512) return WHAT<V, 256, 2>(__VA_ARGS__);    \
-  if ((n) <= 768) return WHAT<V, 256, 3>(__VA_ARGS__);    \
-  if ((n) <= 1024) return WHAT<V, 512, 2>(__VA_ARGS__);   \
-  if ((n) <= 2048) return WHAT<V, 512, 4>(__VA_ARGS__);
-
-int dispatch_fwd(const ssm_block_norm_args& a, bool wide, cudaStream_t st) {
-  if (wide && a.io_dtype != SSM_F32 && a.dim % 8 == 0) {
-    SSM_ROW_CASES(launch_fwd, 8, a.dim / 8, a, st)
-  }
-  if (wide && a.dim % 4 == 0) {
-    SSM_ROW_CASES(launch_fwd, 4, a.dim / 4, a, st)
-  }
-  SSM_ROW_CASES(launch_fwd, 1, a.dim, a, st)
-  return launch_fwd<1, 512, kMaxDim / 512>(a, st);
+  const int gate = g.fwd.gate_kind == kNone ? 0 : g.fwd.gate_kind == kToken ? 2 : 1;
+  if (g.fwd.bias) return gate == 0 ? launch_bwd2<V, THREADS, MC, true, 0, TYPES>(g, st) : gate == 1 ? launch_bwd2<V, THREADS, MC, true, 1, TYPES>(g, st) : launch_bwd2<V, THREADS, MC, true, 2, TYPES>(g, st);
+  return gate == 0 ? launch_bwd2<V, THREADS, MC, false, 0, TYPES>(g, st) : gate == 1 ? launch_bwd2<V, THREADS, MC, false, 1, TYPES>(g, st) : launch_bwd2<V, THREADS, MC, false, 2, TYPES>(g, st);
 }
 // four elements to a piece also in 16 bits: the sums of a thread's columns stay in registers
+template <int TYPES>
+int bwd_of(const ssm_block_norm_bwd_args& g, bool wide, cudaStream_t st) {
+  const int dim = g.fwd.dim;
+  constexpr int kOdd = TYPES == 3 ? 3 : 0;
+  if (wide && dim % 4 == 0)
+    return dim <= 256 ? launch_bwd<4, 320, 1, TYPES>(g, st) : dim <= 2560 ? launch_bwd<4, 320, 2, TYPES>(g, st) : dim <= 4096 ? launch_bwd<4, 512, 2, TYPES>(g, st) : launch_bwd<4, 512, 4, TYPES>(g, st);
+  return dim <= 1024 ? launch_bwd<1, 512, 2, kOdd>(g, st) : dim <= 4096 ? launch_bwd<1, 512, 8, kOdd>(g, st) : launch_bwd<1, 512, 16, kOdd>(g, st);
+}
 int dispatch_bwd(const ssm_block_norm_bwd_args& g, bool wide, cudaStream_t st) {
-  if (wide && g.fwd.dim % 4 == 0) {
-    SSM_ROW_CASES(launch_bwd, 4, g.fwd.dim / 4, g, st)
+  switch (g.dresidual && g.dresidual_out ? types_of(g.fwd) : 0) {
+    case 1: return bwd_of<1>(g, wide, st);
+    case 2: return bwd_of<2>(g, wide, st);
+    case 3: return bwd_of<3>(g, wide, st);
+    default: return bwd_of<0>(g, wide, st);
   }
-  SSM_ROW_CASES(launch_bwd, 1, g.fwd.dim, g, st)
-  return launch_bwd<1, 512, kMaxDim / 512>(g, st);
 }
 
 int check(const ssm_block_norm_args& a) {
