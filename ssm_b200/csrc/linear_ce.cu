@@ -156,7 +156,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t ring = (tc::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t full = tc::smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16;
-  const int live = min(g.rows, max(0, *g.count - g.row0));
+  int live = min(g.rows, max(0, *g.count - g.row0));
+  if (EPI == kKeep && g.again != nullptr) {
+    bool any = false;
+    for (int i = 0; i < (live + kTile - 1) / kTile; ++i) any = any || g.again[i] != 0;
+    if (!any) live = 0;
+  }
   constexpr int kProducts = PLANES == 1 ? 1 : kPairs;
   constexpr bool kSegments = EPI != kOut || PLANES > 1;
 
@@ -569,18 +574,18 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
   }
 }
 
-// The tiles of a row joined: 32 rows of a call to a block, eight slices of the columns.
-__global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
+// The tiles of a row joined: 32 rows of a call to a block, 32 slices of the columns (7 rows, 394 tiles: 21 us with eight slices).
+__global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
                                                    const int* __restrict__ targets, const float* __restrict__ z_target, float4* __restrict__ stats, float* __restrict__ row_loss,
                                                    float* __restrict__ log_z) {
-  __shared__ float2 slices[8][32];
+  __shared__ float2 slices[32][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   const int live = min(rows, *count - row0);
   if ((int)blockIdx.x * 32 >= live) return;
   float M = -INFINITY, s = 0.f;
   if (row < live) {
 #pragma unroll 4
-    for (int p = slice; p < parts; p += 8) {
+    for (int p = slice; p < parts; p += 32) {
       const float2 v = part[(int64_t)p * ld + row];
       const float top = fmaxf(M, v.x);
       s = s * ex2_approx(M - top) + v.y * ex2_approx(v.x - top);
@@ -590,8 +595,8 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ pa
   slices[slice][lane] = make_float2(M, s);
   __syncthreads();
   if (slice == 0 && row < live) {
-#pragma unroll
-    for (int w = 1; w < 8; ++w) {
+#pragma unroll 8
+    for (int w = 1; w < 32; ++w) {
       const float2 v = slices[w][lane];
       if (v.x == -INFINITY) continue;
       const float top = fmaxf(M, v.x);
@@ -636,17 +641,17 @@ __global__ void __launch_bounds__(256) reference_kernel(const __nv_bfloat16* __r
   }
 }
 // Its tiles joined.  A row whose maximum is too far from M gets one from its maximum, and its tile of rows is formed again; the second call (`second`) then joins those.
-__global__ void __launch_bounds__(256) join_keep_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
+__global__ void __launch_bounds__(1024) join_keep_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
                                                         const float* __restrict__ z_target, float4* __restrict__ row, int* __restrict__ again, int second, float* __restrict__ row_loss,
                                                         float* __restrict__ log_z) {
-  __shared__ float2 slices[8][32];
+  __shared__ float2 slices[32][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   const int live = min(rows, *count - row0);
   if ((int)blockIdx.x * 32 >= live || (second && !again[blockIdx.x * 32 / kTile])) return;
   float m = -INFINITY, s = 0.f;
   if (i < live) {
 #pragma unroll 4
-    for (int p = slice; p < parts; p += 8) {
+    for (int p = slice; p < parts; p += 32) {
       const float2 v = part[(int64_t)p * ld + i];
       m = fmaxf(m, v.x), s += v.y;
     }
@@ -654,8 +659,8 @@ __global__ void __launch_bounds__(256) join_keep_kernel(const float2* __restrict
   slices[slice][lane] = make_float2(m, s);
   __syncthreads();
   if (slice == 0 && i < live) {
-#pragma unroll
-    for (int w = 1; w < 8; ++w) m = fmaxf(m, slices[w][lane].x), s += slices[w][lane].y;
+#pragma unroll 8
+    for (int w = 1; w < 32; ++w) m = fmaxf(m, slices[w][lane].x), s += slices[w][lane].y;
     const int r = row0 + i, out = idx[r];
     const float z = z_target[r], top = ceilf(m * kLog2e);
     float4 v = row[r];
@@ -770,51 +775,114 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ 
   }
 }
 
-// Packed rows [8192 b, ..) in the order of their targets: keys (target, packed row), all ones behind them.  A block each.
+// Packed rows [8192 b, ..) in the order of their targets: keys (target, packed row), all ones behind them.  A block each; eight keys to a thread, compared in registers, by shuffles
+// within a warp and through shared memory beyond (8192 keys all through shared memory: 97 us).  Key: uint32_t where target and place fit.
 constexpr int kSort = 8192;
+template <typename Key>
+__device__ __forceinline__ Key shuffled(Key v, int lanes) { return __shfl_xor_sync(0xffffffffu, v, lanes); }
+template <typename Key>
 __global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targets, const int* __restrict__ count, int size, uint64_t* __restrict__ keys) {
-  extern __shared__ uint64_t key[];
-  const int first = blockIdx.x * kSort, n = *count;
-  for (int i = threadIdx.x; i < size; i += 1024) {
-    const int r = first + i, t = r < n ? targets[r] : -1;
-    key[i] = t >= 0 ? (uint64_t)t << 32 | (uint32_t)r : ~0ull;
+  extern __shared__ __align__(8) unsigned char sort_raw[];
+  Key* const other = reinterpret_cast<Key*>(sort_raw);
+  const int first = blockIdx.x * kSort, n = *count, tid = threadIdx.x, threads = blockDim.x;
+  Key key[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int i = tid * 8 + e, r = first + i, t = i < size && r < n ? targets[r] : -1;
+    key[e] = t >= 0 ? (Key)t << 13 | (Key)i : ~(Key)0;
   }
+  auto ordered = [](Key& a, Key& b, bool up) {  // a <= b where up
+    const Key lo = a < b ? a : b, hi = a < b ? b : a;
+    a = up ? lo : hi, b = up ? hi : lo;
+  };
   for (int k = 2; k <= size; k *= 2) {
-    for (int j = k / 2; j > 0; j /= 2) {
+    int j = k / 2;
+    for (; j >= 256; j /= 2) {
       __syncthreads();
-      for (int i = threadIdx.x; i < size; i += 1024) {
-        const int o = i ^ j;
-        if (o > i) {
-          const uint64_t a = key[i], b = key[o];
-          if ((a > b) == ((i & k) == 0)) key[i] = b, key[o] = a;
-        }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) other[e * threads + tid] = key[e];
+      __syncthreads();
+      const bool up = ((tid * 8) & k) == 0, low = (tid & (j / 8)) == 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Key o = other[e * threads + (tid ^ (j / 8))];
+        key[e] = (key[e] < o) == (up == low) ? key[e] : o;
       }
     }
+    for (; j >= 8; j /= 2) {
+      const bool up = ((tid * 8) & k) == 0, low = (tid & (j / 8)) == 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Key o = shuffled(key[e], j / 8);
+        key[e] = (key[e] < o) == (up == low) ? key[e] : o;
+      }
+    }
+    if (k >= 8) {
+      const bool up = ((tid * 8) & k) == 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ordered(key[e], key[e + 4], up);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) ordered(key[e], key[e + 2], up), ordered(key[e + 1], key[e + 3], up);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) ordered(key[e], key[e + 1], up);
+    } else if (k == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) ordered(key[e], key[e + 2], (e & 4) == 0), ordered(key[e + 1], key[e + 3], (e & 4) == 0);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) ordered(key[e], key[e + 1], (e & 4) == 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) ordered(key[e], key[e + 1], (e & 2) == 0);
+    }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < size; i += 1024) keys[first + i] = key[i];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (tid * 8 + e < size) keys[first + tid * 8 + e] = key[e] == ~(Key)0 ? ~0ull : (uint64_t)(key[e] >> 13) << 32 | (uint32_t)(first + (int)(key[e] & (kSort - 1)));
 }
-// dweight's row of a target += the sum of q h over the rows that have it, in their order: one block (of 512 columns) for each run of equal targets
+// dweight's row of a target += the sum of q h over the rows that have it, in their order: one block (of 128 V columns) for each run of equal targets, eight rows on their way at
+// a time (a common token has hundreds).
+template <int V>
 __global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* __restrict__ keys, int size, const float4* __restrict__ row, const int* __restrict__ idx, const void* hidden, int64_t stride, int dtype,
                                                           int dim, const float* __restrict__ scales, float* __restrict__ out, int64_t ld) {
   const int p = blockIdx.x;
   const uint64_t key = keys[p];
   if (key == ~0ull || (p > 0 && keys[p - 1] >> 32 == key >> 32)) return;
-  const int c0 = blockIdx.y * 512 + threadIdx.x;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int q = p; q < size && keys[q] >> 32 == key >> 32; ++q) {
-    const int r = (int)(uint32_t)keys[q];
-    const float w = row[r].w;
-    const int64_t at = idx[r] * stride;
+  const int c = (blockIdx.y * 128 + threadIdx.x) * V;
+  if (c >= dim) return;
+  float v[V] = {};
+  for (int q = p; q < size; q += 8) {
+    float w[8], e[8][V];
+    int r[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (c0 + 128 * k < dim) v[k] = fmaf(w, load_dyn(hidden, at + c0 + 128 * k, dtype), v[k]);
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t k = keys[min(q + i, size - 1)];
+      r[i] = q + i < size && k >> 32 == key >> 32 ? (int)(uint32_t)k : -1;
+    }
+    const int none = (int)(uint32_t)key;  // a row to read where there are no more
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int from = r[i] >= 0 ? r[i] : none;
+      w[i] = row[from].w;
+      const int64_t at = idx[from] * stride + c;
+      if constexpr (V == 4) load_param_vec<4>(hidden, at, dtype, e[i]);
+      else e[i][0] = load_dyn(hidden, at, dtype);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = r[i] >= 0 ? fmaf(w[i], e[i][k], v[k]) : v[k];
+    }
+    if (r[7] < 0) break;
   }
   const float scale = scales[0];
-  float* to = out + (int64_t)(key >> 32) * ld;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (c0 + 128 * k < dim) to[c0 + 128 * k] += v[k] * scale;
+  float* to = out + (int64_t)(key >> 32) * ld + c;
+  if constexpr (V == 4) {
+    float4 o = *reinterpret_cast<const float4*>(to);
+    o.x = fmaf(v[0], scale, o.x), o.y = fmaf(v[1], scale, o.y), o.z = fmaf(v[2], scale, o.z), o.w = fmaf(v[3], scale, o.w);
+    *reinterpret_cast<float4*>(to) = o;
+  } else {
+    *to = fmaf(v[0], scale, *to);
+  }
 }
 
 // out = factor * src, the factor scales[1] (dloss NULL) or scales[1] dloss; zeros where no row counts.  V elements at a time.
@@ -1032,12 +1100,20 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
 int target_rows(const Run& r, float* dw) {
   const Plan& p = r.p;
   uint64_t* keys = r.at<uint64_t>(p.keys);
-  cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
-  sort_kernel<<<p.sorts, 1024, p.sort * 8, r.st>>>(r.packed(), r.count(), p.sort, keys);
+  const unsigned threads = (unsigned)std::max(32, p.sort / 8);
+  if (p.vocab < 1 << 19) {
+    sort_kernel<uint32_t><<<p.sorts, threads, threads * 32, r.st>>>(r.packed(), r.count(), p.sort, keys);
+  } else {
+    cudaFuncSetAttribute(sort_kernel<uint64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
+    sort_kernel<uint64_t><<<p.sorts, threads, threads * 64, r.st>>>(r.packed(), r.count(), p.sort, keys);
+  }
   if (const int rc = launch_status("linear_ce sort_kernel")) return rc;
+  const bool wide = p.dim % 4 == 0 && r.a.hidden_stride % 4 == 0 && aligned_to(r.a.hidden, 16);
+  auto kern = wide ? target_rows_kernel<4> : target_rows_kernel<1>;
+  const int per = wide ? 512 : 128;
   for (int i = 0; i < p.sorts; ++i) {
-    target_rows_kernel<<<dim3((unsigned)p.sort, (unsigned)((p.dim + 511) / 512)), 128, 0, r.st>>>(keys + (int64_t)i * kSort, p.sort, r.row(), r.idx(), r.a.hidden, r.a.hidden_stride, r.a.io_dtype, (int)p.dim,
-                                                                                                  r.at<float>(p.scales), dw, p.ldo);
+    kern<<<dim3((unsigned)p.sort, (unsigned)((p.dim + per - 1) / per)), 128, 0, r.st>>>(keys + (int64_t)i * kSort, p.sort, r.row(), r.idx(), r.a.hidden, r.a.hidden_stride, r.a.io_dtype, (int)p.dim,
+                                                                                      r.at<float>(p.scales), dw, p.ldo);
     if (const int rc = launch_status("linear_ce target_rows_kernel")) return rc;
   }
   return SSM_OK;
@@ -1094,7 +1170,7 @@ extern "C" int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t st
       const int64_t rows = std::min(p.piece, p.rows - row0);
       const GemmArgs g = logits_args(r, row0, rows);
       if (const int rc = gemm_of<kStats>(p, r.mh, r.mw, r.mw, g, r.st)) return rc;
-      join_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z);
+      join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z);
       if (const int rc = launch_status("linear_ce join_kernel")) return rc;
     }
   }
@@ -1153,7 +1229,7 @@ extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidde
     for (int second = 0; second < 2; ++second) {
       g.again = second ? again : nullptr;
       if (const int rc = gemm_of<kKeep>(p, r.mh, r.mw, r.mw, g, r.st)) return rc;
-      join_keep_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), g.z_target, r.row(), again, second, a.row_loss, a.log_z);
+      join_keep_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), g.z_target, r.row(), again, second, a.row_loss, a.log_z);
       if (const int rc = launch_status("linear_ce join_keep_kernel")) return rc;
     }
     if (dweight) {
