@@ -246,7 +246,8 @@ int ssm_block_norm_bwd(const ssm_block_norm_bwd_args* args, ssm_stream_t stream)
  *
  * Backward: from dloss (rows, or one float with a reduction) and dlog_z (rows, nullable) writes dhidden (rows, dim; io_dtype) and dweight (vocab, dim; dweight_dtype),
  * dense, each nullable, via pieces of at most SSM_LINEAR_CE_PIECE_BYTES of the logits' gradient in 16 bits.
- * scratch: ssm_linear_ce_scratch_bytes(args, pass) bytes, 256-byte aligned; pass 0 forward, 1 backward, 2 both at once.
+ * packs, 256-byte aligned, ssm_linear_ce_packs_bytes(args) bytes: the rows that count (and, in fp32, the weight) as the products read them, written by the forward pass and read by
+ * the backward pass.  scratch: ssm_linear_ce_scratch_bytes(args, pass) bytes, 256-byte aligned; pass 0 forward, 1 backward, 2 both at once.
  *
  * ssm_linear_ce_train, for bf16 with a reduction: the forward pass and, for a dloss that is known later, dhidden (rows, dim) and dweight (vocab, dim rounded up to a multiple of
  * 4) in fp32, 16-byte aligned, each nullable; kept: three words.  ssm_linear_ce_scale then multiplies either, (rows, dim) at the row stride ld, by dloss and what `kept` holds.
@@ -262,12 +263,13 @@ typedef struct {
   float* log_z;
   float* loss;  /* nullable without a reduction */
   float* stats; /* nullable */
+  void* packs;
   void* scratch;
   int32_t* status;
 } ssm_linear_ce_args;
 
 typedef struct {
-  ssm_linear_ce_args fwd; /* hidden, weight, targets and stats are read */
+  ssm_linear_ce_args fwd; /* hidden, weight, targets, stats and packs are read */
   const float* dloss;
   const float* dlog_z; /* nullable */
   void* dhidden;       /* nullable */
@@ -275,6 +277,7 @@ typedef struct {
   int32_t dweight_dtype, reserved0;
 } ssm_linear_ce_bwd_args;
 
+int64_t ssm_linear_ce_packs_bytes(const ssm_linear_ce_args* args);
 int64_t ssm_linear_ce_scratch_bytes(const ssm_linear_ce_args* args, int32_t pass);
 int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t stream);
 int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_t stream);

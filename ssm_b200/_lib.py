@@ -211,7 +211,8 @@ class BlockNormBwdArgs(C.Structure):
 class LinearCeArgs(C.Structure):
     _fields_ = [
         ("rows", i64), ("hidden_stride", i64), ("weight_stride", i64), ("ignore_index", i64), ("dim", i32), ("vocab", i32), ("io_dtype", i32), ("reduction", i32),
-        ("hidden", vp), ("weight", vp), ("targets", vp), ("row_loss", fp), ("log_z", fp), ("loss", fp), ("stats", fp), ("scratch", vp), ("status", vp),
+        ("hidden", vp), ("weight", vp), ("targets", vp), ("row_loss", fp), ("log_z", fp), ("loss", fp), ("stats", fp), ("packs", vp),
+        ("scratch", vp), ("status", vp),
     ]
 
 
@@ -284,6 +285,7 @@ ENTRY_POINTS = {
     "ssm_block_norm_fwd": (C.c_int, [C.POINTER(BlockNormArgs), vp]),
     "ssm_block_norm_bwd_scratch_floats": (C.c_int64, [i64, i32]),
     "ssm_block_norm_bwd": (C.c_int, [C.POINTER(BlockNormBwdArgs), vp]),
+    "ssm_linear_ce_packs_bytes": (C.c_int64, [C.POINTER(LinearCeArgs)]),
     "ssm_linear_ce_scratch_bytes": (C.c_int64, [C.POINTER(LinearCeArgs), i32]),
     "ssm_linear_ce_fwd": (C.c_int, [C.POINTER(LinearCeArgs), vp]),
     "ssm_linear_ce_bwd": (C.c_int, [C.POINTER(LinearCeBwdArgs), vp]),

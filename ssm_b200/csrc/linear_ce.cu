@@ -37,7 +37,8 @@ constexpr float kFar = 268435456.f;    // M of a tile is no less than minus this
 constexpr int kPairs = 6;
 __constant__ const signed char kPlaneA[kPairs] = {2, 0, 1, 1, 0, 0}, kPlaneB[kPairs] = {0, 2, 1, 0, 1, 0};
 
-enum Epilogue { kStats = 0, kGrad = 1, kOut = 2, kKeep = 3 };
+enum Epilogue { kStats = 0, kGrad = 1, kOut = 2, kKeep = 3, kFew = 4 };  // kFew: kStats with the weight's rows as M
+constexpr int kFewRows = 64;           // up to which rows it is taken
 constexpr int kSegment = 8;            // blocks of K between two readings of an accumulator, where its sums have to keep 32 bits
 constexpr float kReach = 60.f;         // how far a row's maximum may be from the M of the one-pass form
 
@@ -60,7 +61,7 @@ struct GemmArgs {
   // kStats, kGrad, kKeep
   int vocab;
   const int* targets;          // of packed rows; -1: outside of the vocabulary
-  float2* part;                // [128 columns][rows of this call]: M, sum 2^(c z - M); kKeep: the maximum, the sum
+  float2* part;                // [128 columns][rows of this call]: M, sum 2^(c z - M); kKeep: the maximum, the sum; kFew: [row][32 columns]
   int part_ld;
   float* z_target;
   const float4* row;           // of packed rows: M, 1 / s, w + wz, q; kKeep: M
@@ -168,7 +169,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // This pair's k-th tile.  The first job's tiles (long ones) go round the pairs; pairs that have one less of them take as many rounds of the second job's alone as fit into
   // its time, then all take turns: the tiles that run at one time stay neighbours, and share operands in the L2.
   const int m0 = (live + kTile - 1) / kTile, kb_rows = (live + kK - 1) / kK;
-  const int tiles0 = live > 0 ? (g.job[0].k_is_rows ? g.job[0].m_tiles : min(g.job[0].m_tiles, m0)) * g.job[0].n_tiles * g.job[0].splits : 0;
+  const int tiles0 = live > 0 ? (g.job[0].k_is_rows || EPI == kFew ? g.job[0].m_tiles : min(g.job[0].m_tiles, m0)) * g.job[0].n_tiles * g.job[0].splits : 0;
   const int tiles1 = EPI == kOut && live > 0 ? (g.job[1].k_is_rows ? g.job[1].m_tiles : min(g.job[1].m_tiles, m0)) * g.job[1].n_tiles * g.job[1].splits : 0;
   const int extra = tiles0 % pairs, mine0 = tiles0 / pairs + (pair < extra ? 1 : 0);
   const int alone = EPI == kOut && extra ? g.job[0].k_blocks / g.job[0].splits / max(1, g.job[1].k_is_rows ? kb_rows : g.job[1].k_blocks) : 0;
@@ -191,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (p.job < 0) return p;
     }
     const Job& j = g.job[p.job];
-    const int m_tiles = j.k_is_rows ? j.m_tiles : min(j.m_tiles, m0), k_blocks = j.k_is_rows ? kb_rows : j.k_blocks, per = m_tiles * j.n_tiles;
+    const int m_tiles = j.k_is_rows || EPI == kFew ? j.m_tiles : min(j.m_tiles, m0), k_blocks = j.k_is_rows ? kb_rows : j.k_blocks, per = m_tiles * j.n_tiles;
     p.split = t / per, t -= p.split * per;
     if (j.m_inner) p.m = t % m_tiles, p.n = t / m_tiles;
     else p.n = t % j.n_tiles, p.m = t / j.n_tiles;
@@ -248,7 +249,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               const int ka = j.a_k0 + kb * kK, kb_at = j.b_k0 + kb * kK;
 #pragma unroll
               for (int i = 0; i < 2; ++i) load_box(at + i * kBoxBytes, &ma, bar, j.a_mn ? am + 64 * i : ka, j.a_mn ? ka : am + 64 * i, pa);
-              for (int i = 0; i < half / 64; ++i) load_box(at + (2 + i) * kBoxBytes, map_b, bar, j.b_mn ? bn + 64 * i : kb_at, j.b_mn ? kb_at : bn + 64 * i, pb);
+              if (EPI == kFew) load_box(at + 2 * kBoxBytes, map_b, bar, kb_at, bn, pb);  // a box of half the rows
+              else
+                for (int i = 0; i < half / 64; ++i) load_box(at + (2 + i) * kBoxBytes, map_b, bar, j.b_mn ? bn + 64 * i : kb_at, j.b_mn ? kb_at : bn + 64 * i, pb);
             }
           }
         }
@@ -349,19 +352,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         release(b);
         ++n;
       } else {
-        uint32_t v[4][32];
+        constexpr int kChunks = EPI == kFew ? 1 : 4;
+        uint32_t v[kChunks][32];
         for (int seg = p.kb0; seg < p.kb1 && ok; seg += kSegment, ++n) {
           const int b = n & 1;
           if (!arrived(b)) break;
           const uint32_t from = tmem + lanes + b * 256 + half * width;
           if (seg == p.kb0) {
+            if (EPI == kFew && width == 16) {
+              float w[16];
+              tc::tmem_ld16(from, w);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (32 * c < width) tmem_ld32_issue(from + 32 * c, v[c]);
-            tmem_wait_ld();
+              for (int i = 0; i < 16; ++i) v[0][i] = __float_as_uint(w[i]), v[0][16 + i] = 0u;
+            } else {
+#pragma unroll
+              for (int c = 0; c < kChunks; ++c)
+                if (32 * c < width) tmem_ld32_issue(from + 32 * c, v[c]);
+              tmem_wait_ld();
+            }
           } else {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int c = 0; c < 2 * kChunks; ++c) {
               if (16 * c < width) {
                 float w[16];
                 tc::tmem_ld16(from + 16 * c, w);
@@ -373,7 +384,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           release(b);
         }
         if (!ok) break;
-        if constexpr (EPI == kOut) {
+        if constexpr (EPI == kFew) {  // a thread has a row of the weight, its registers packed rows
+          const int id = p.m * kTile + row_in, first = half * width;
+          const bool in = id < g.vocab;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i >= width || first + i >= live) break;
+            const float z = in ? __uint_as_float(v[0][i]) : -INFINITY;
+            if (in && g.targets[g.row0 + first + i] == id) g.z_target[g.row0 + first + i] = z;
+            float m = z;
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            const float M = fmaxf(ceilf(m * kLog2e), -kFar);
+            const float s = warp_sum(ex2_approx(fmaf(z, kLog2e, -M)));
+            if (lane == 0) g.part[(int64_t)(first + i) * g.part_ld + (p.m * 2 + rank) * 4 + (warp & 3)] = make_float2(M, s);
+          }
+        } else if constexpr (EPI == kOut) {
           float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
           const int cols = (int)min((int64_t)width, j.ld - out_col);
           if (row < j.out_rows) {
@@ -428,30 +454,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (in) r = g.row[g.row0 + row];
             uint16_t* to = g.g + row * g.ldg + col0;
             const int room = (int)min((int64_t)128, g.ldg - col0);
+            const float f = in ? r.y * r.z : 0.f;
             float m = -INFINITY, s = 0.f;
+            if (left < 128 || !in) {  // columns behind the vocabulary, rows behind the last one: zeros
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!in || 32 * c + i >= left) v[c][i] = 0xff800000u;
+              if (!in) r.x = 0.f;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 const float z = __uint_as_float(v[c][i]);
-                const bool is = in && 32 * c + i < left;
                 float e = ex2_approx(fmaf(z, kLog2e, -r.x));
-                if constexpr (EPI == kKeep) {
-                  if (is) m = fmaxf(m, z), s += e;
-                } else {
-                  e = e * r.y * r.z;
-                }
-                v[c][i] = is && 32 * c + i != at ? __float_as_uint(e) : 0u;
+                if constexpr (EPI == kKeep) m = fmaxf(m, z), s += e;
+                else e *= f;
+                v[c][i] = __float_as_uint(e);
               }
+              // whole sectors of 32 bytes: the rows of a warp's threads lie apart
+              if constexpr (PLANES == 1) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) {
-                if (32 * c + i < room) {
-                  if constexpr (PLANES == 1) {
-                    uint32_t w[4];
+                for (int i = 0; i < 32; i += 16) {
+                  if (32 * c + i < room) {
+                    uint32_t w[8];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) w[q] = pack2<T>(__uint_as_float(v[c][i + 2 * q]), __uint_as_float(v[c][i + 2 * q + 1]));
-                    *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(w[0], w[1], w[2], w[3]);
-                  } else {
+                    for (int q = 0; q < 8; ++q) w[q] = pack2<T>(__uint_as_float(v[c][i + 2 * q]), __uint_as_float(v[c][i + 2 * q + 1]));
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to + 32 * c + i), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                                 "r"(w[7])
+                                 : "memory");
+                  }
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                  if (32 * c + i < room) {
                     __nv_bfloat16 e[8][3];
 #pragma unroll
                     for (int q = 0; q < 8; ++q) split3(__uint_as_float(v[c][i + q]), e[q]);
@@ -465,6 +504,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                   }
                 }
               }
+            }
+            if (at >= 0 && at < 128) {  // the target's own part goes to the gradients apart
+#pragma unroll
+              for (int q = 0; q < PLANES; ++q) to[q * g.g_plane + at] = 0;
             }
             if (EPI == kKeep && in) g.part[(int64_t)(p.n * 2 + half) * g.part_ld + row] = make_float2(m, s);
           }
@@ -486,7 +529,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // Rows whose target counts, in their order, from the front of idx; the others from its end.  One block.
 __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ targets, int rows, int64_t ignore, int vocab, int* __restrict__ idx, int* __restrict__ packed, int* __restrict__ count,
-                                                    float* __restrict__ row_loss, float* __restrict__ log_z, const int write) {
+                                                    float* __restrict__ row_loss, float* __restrict__ log_z) {
   __shared__ int sums[32];
   __shared__ int base_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -528,7 +571,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ 
           ++pos;
         } else {
           idx[rows - 1 - (at + k - pos)] = at + k;
-          if (write) row_loss[at + k] = 0.f, log_z[at + k] = 0.f;
+          row_loss[at + k] = 0.f, log_z[at + k] = 0.f;
         }
       }
     }
@@ -574,6 +617,53 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
   }
 }
 
+// Both for up to 64 rows, in one launch
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* __restrict__ targets, int rows, int64_t ignore, int vocab, const void* src, int64_t stride, int dim, int* __restrict__ idx,
+                                                        int* __restrict__ packed, int* __restrict__ count, float* __restrict__ row_loss, float* __restrict__ log_z, uint16_t* dst, int64_t ld,
+                                                        int64_t plane) {
+  __shared__ int rows_of[kFewRows];
+  __shared__ int kept_s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == 0) {
+    int base = 0;
+    for (int first = 0; first < rows; first += 32) {
+      const int i = first + lane;
+      const int64_t t = i < rows ? targets[i] : ignore;
+      const bool counts = t != ignore;
+      const uint32_t votes = __ballot_sync(0xffffffffu, counts);
+      const int before = base + __popc(votes & ((1u << lane) - 1));
+      if (i < rows) {
+        if (counts) {
+          idx[before] = i, packed[before] = t >= 0 && t < vocab ? (int)t : -1, rows_of[before] = i;
+        } else {
+          idx[rows - 1 - (i - before)] = i;
+          row_loss[i] = 0.f, log_z[i] = 0.f;
+        }
+      }
+      base += __popc(votes);
+    }
+    if (lane == 0) *count = kept_s = base;
+  }
+  __syncthreads();
+  const int n = kept_s;
+  for (int r = warp; r < rows; r += 32) {  // zeros behind the last one that counts
+    const T* row = reinterpret_cast<const T*>(src) + (r < n ? rows_of[r] : 0) * stride;
+#pragma unroll 4
+    for (int c = lane; c < dim; c += 32) {
+      if constexpr (PLANES == 1) {
+        const uint16_t bits = reinterpret_cast<const uint16_t*>(row)[c];
+        dst[r * ld + c] = r < n ? bits : (uint16_t)0;
+      } else {
+        __nv_bfloat16 p[3];
+        split3(r < n ? to_f<T>(row[c]) : 0.f, p);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) dst[q * plane + r * ld + c] = __bfloat16_as_ushort(p[q]);
+      }
+    }
+  }
+}
+
 // The tiles of a row joined: 32 rows of a call to a block, 32 slices of the columns (7 rows, 394 tiles: 21 us with eight slices).
 __global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
                                                    const int* __restrict__ targets, const float* __restrict__ z_target, float4* __restrict__ stats, float* __restrict__ row_loss,
@@ -607,6 +697,43 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ p
     const float ln_s = logf(s), z = t < 0 ? NAN : z_target[r];
     stats[r] = make_float4(M, s, z, 0.f);
     row_loss[out] = ln_s - kLn2 * fmaf(z, kLog2e, -M);  // log Z - z_t as differences from M, which take no bits from a small loss
+    log_z[out] = fmaf(M, kLn2, ln_s);
+  }
+}
+
+// The tiles of up to 64 rows joined, a block to a row
+__global__ void __launch_bounds__(256) few_join_kernel(const float2* __restrict__ part, int parts, const int* __restrict__ count, const int* __restrict__ idx, const int* __restrict__ targets,
+                                                       const float* __restrict__ z_target, float4* __restrict__ stats, float* __restrict__ row_loss, float* __restrict__ log_z) {
+  __shared__ float2 warps[8];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  if (r >= *count) return;
+  float M = -INFINITY, s = 0.f;
+  auto add = [&](float2 v) {
+    const float top = fmaxf(M, v.x);
+    s = (M == top ? s : s * ex2_approx(M - top)) + (v.x == top ? v.y : v.y * ex2_approx(v.x - top));
+    M = top;
+  };
+#pragma unroll 4
+  for (int p = tid; p < parts; p += 256) add(part[(int64_t)r * parts + p]);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    const float2 o = make_float2(__shfl_xor_sync(0xffffffffu, M, off), __shfl_xor_sync(0xffffffffu, s, off));
+    if (tid & off) {  // the same order on both sides
+      const float2 mine = make_float2(M, s);
+      M = o.x, s = o.y;
+      add(mine);
+    } else {
+      add(o);
+    }
+  }
+  if (tid % 32 == 0) warps[tid / 32] = make_float2(M, s);
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < 8; ++w) add(warps[w]);
+    const int t = targets[r], out = idx[r];
+    const float ln_s = logf(s), z = t < 0 ? NAN : z_target[r];
+    stats[r] = make_float4(M, s, z, 0.f);
+    row_loss[out] = ln_s - kLn2 * fmaf(z, kLog2e, -M);
     log_z[out] = fmaf(M, kLn2, ln_s);
   }
 }
@@ -753,9 +880,38 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ 
   const int t = in ? max(targets[r], 0) : 0;
   const float4 w = in ? row[r] : make_float4(0.f, 0.f, 0.f, 0.f);
   const float f = by_row ? w.y : scales[1];
+  if (in && V == 4) {  // four pieces in flight
+    for (int c0 = lane * 4; c0 < dim; c0 += 512) {
+      float4 x[4];
+      float e[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = __ldcs(reinterpret_cast<const float4*>(part + i * ld + min(c0 + 128 * k, dim - 4)));
+      for (int s = 1; s < splits; ++s) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 o = __ldcs(reinterpret_cast<const float4*>(part + s * split + i * ld + min(c0 + 128 * k, dim - 4)));
+          x[k].x += o.x, x[k].y += o.y, x[k].z += o.z, x[k].w += o.w;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) load_param_vec<4>(weight, t * weight_stride + min(c0 + 128 * k, dim - 4), weight_dtype, e[k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + 128 * k;
+        if (c >= dim) break;
+        const float v[4] = {fmaf(w.w, e[k][0], x[k].x * f), fmaf(w.w, e[k][1], x[k].y * f), fmaf(w.w, e[k][2], x[k].z * f), fmaf(w.w, e[k][3], x[k].w * f)};
+        if (dtype == SSM_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + to + c) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+          *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + to + c) =
+              dtype == SSM_BF16 ? make_uint2(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3])) : make_uint2(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]));
+      }
+    }
+    return;
+  }
   for (int c = lane * V; c < dim; c += 32 * V) {
     float v[V] = {}, e[V];
     if (in) {
+#pragma unroll 4
       for (int s = 0; s < splits; ++s) {
         const float* from = part + s * split + i * ld + c;
         if constexpr (V == 4) {
@@ -850,7 +1006,17 @@ __global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* __rest
   const int c = (blockIdx.y * 128 + threadIdx.x) * V;
   if (c >= dim) return;
   float v[V] = {};
-  for (int q = p; q < size; q += 8) {
+  int q = p;
+  if (p + 1 >= size || keys[p + 1] >> 32 != key >> 32) {  // the only row
+    const int r = (int)(uint32_t)key;
+    const float w = row[r].w;
+    if constexpr (V == 4) load_param_vec<4>(hidden, idx[r] * stride + c, dtype, v);
+    else v[0] = load_dyn(hidden, idx[r] * stride + c, dtype);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] *= w;
+    q = size;
+  }
+  for (; q < size; q += 8) {
     float w[8], e[8][V];
     int r[8];
 #pragma unroll
@@ -922,12 +1088,12 @@ __global__ void __launch_bounds__(256) scaled_copy_kernel(const float* __restric
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// (outer, inner) matrices of 16-bit elements, `planes` of them; boxes of 64 x 64
-int encode(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int planes, int64_t ld, int64_t plane, int fmt) {
+// (outer, inner) matrices of 16-bit elements, `planes` of them; boxes of 64 x `high`
+int encode(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int planes, int64_t ld, int64_t plane, int fmt, int high = 64) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(SSM_ERR_DEVICE, "linear_cross_entropy: cuTensorMapEncodeTiled is not available from this driver");
   const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)planes}, strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
-  const cuuint32_t box[3] = {64, 64, 1}, estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)high, 1}, estr[3] = {1, 1, 1};
   const CUresult rc = fn(m, fmt ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS ? SSM_OK : fail(SSM_ERR_DEVICE, "linear_cross_entropy: cuTensorMapEncodeTiled rejected the matrix");
@@ -942,8 +1108,8 @@ struct Plan {
   int64_t piece;      // rows of a piece
   int splits, bn;     // of dh = G W
   int parts, sort, sorts;
-  // offsets into scratch
-  int64_t idx, packed, count, scales, h, w, part, z, row, g, dh, dw, keys, again, hs, bytes;
+  // offsets: what both passes use (kept between them), then scratch
+  int64_t idx, packed, count, h, w, kept, scales, part, z, row, g, dh, dw, keys, again, hs, bytes;
 };
 constexpr int64_t kForwardRows = 16384;
 
@@ -979,16 +1145,18 @@ Plan plan_of(const ssm_linear_ce_args& a, int pass) {
     at += up(bytes, 256);
     return here;
   };
-  p.idx = take(p.rows * 4), p.packed = take(p.rows * 4), p.count = take(4), p.scales = take(8), p.row = take(p.rows * 16);  // row: stats of a forward pass that keeps none
+  p.idx = take(p.rows * 4), p.packed = take(p.rows * 4), p.count = take(4);
   p.h = take(p.planes * up(p.rows, kTile) * p.ldh * 2);
   p.w = take(p.copy_w ? p.planes * p.vocab * p.ldh * 2 : 0);
+  p.kept = at;
+  p.scales = take(8), p.row = take(p.rows * 16);  // row: stats of a forward pass that keeps none
   if (pass != kBackward) p.part = take((int64_t)p.parts * p.piece * 8), p.z = take(p.rows * 4);
   if (pass != kForward) {
     p.g = take(p.planes * p.piece * p.ldg * 2), p.dh = take((int64_t)p.splits * p.piece * p.ldo * 4), p.keys = take((int64_t)p.sorts * kSort * 8);
     if (pass == kBackward) p.dw = take(p.vocab * p.ldo * 4);
     else p.again = take(p.piece / kTile * 4), p.hs = take(up(p.rows, kTile) * p.ldh * 2);
   }
-  p.bytes = at;
+  p.bytes = at - p.kept;
   return p;
 }
 
@@ -997,8 +1165,8 @@ int check(const ssm_linear_ce_args& a) {
   SSM_REQUIRE(a.rows <= (1 << 28) && a.vocab <= (1 << 28) && a.dim <= (1 << 20), SSM_ERR_TOO_LARGE, "linear_cross_entropy: more than 2^28 rows or columns, or 2^20 channels");
   SSM_REQUIRE(valid_dtype(a.io_dtype), SSM_ERR_DTYPE, "linear_cross_entropy: unknown dtype");
   SSM_REQUIRE(a.reduction >= 0 && a.reduction <= 2, SSM_ERR_SHAPE, "linear_cross_entropy: unknown reduction");
-  SSM_REQUIRE(a.weight && (a.rows == 0 || (a.hidden && a.targets)) && a.scratch && a.status, SSM_ERR_NULL, "linear_cross_entropy: NULL pointer");
-  SSM_REQUIRE(aligned_to({a.hidden, a.weight}, dtype_size(a.io_dtype)) && aligned_to(a.targets, 8) && aligned_to(a.stats, 16) && aligned_to({a.row_loss, a.log_z, a.loss, a.status}, 4) && aligned_to(a.scratch, 256),
+  SSM_REQUIRE(a.weight && (a.rows == 0 || (a.hidden && a.targets)) && a.scratch && a.packs && a.status, SSM_ERR_NULL, "linear_cross_entropy: NULL pointer");
+  SSM_REQUIRE(aligned_to({a.hidden, a.weight}, dtype_size(a.io_dtype)) && aligned_to(a.targets, 8) && aligned_to(a.stats, 16) && aligned_to({a.row_loss, a.log_z, a.loss, a.status}, 4) && aligned_to({a.scratch, a.packs}, 256),
               SSM_ERR_ALIGN, "linear_cross_entropy: misaligned pointer");
   return SSM_OK;
 }
@@ -1030,7 +1198,7 @@ struct Run {
   cudaStream_t st;
   CUtensorMap mh, mw, mg;
   template <typename U>
-  U* at(int64_t off) const { return reinterpret_cast<U*>(base + off); }
+  U* at(int64_t off) const { return reinterpret_cast<U*>(off < p.kept ? static_cast<char*>(a.packs) + off : base + (off - p.kept)); }
   int* idx() const { return at<int>(p.idx); }
   int* packed() const { return at<int>(p.packed); }
   int* count() const { return at<int>(p.count); }
@@ -1038,12 +1206,12 @@ struct Run {
   const void* w() const { return p.copy_w ? at<void>(p.w) : a.weight; }
   int64_t ldw() const { return p.copy_w ? p.ldh : a.weight_stride; }
 };
-// packs the rows (and the weight, where it cannot be copied from its place) and describes them to the copies
-int prepare(Run& r, bool write) {
+// packs the rows (and the weight, where it cannot be copied from its place), unless they are from the pass before, and describes them to the copies
+int prepare(Run& r, bool packs) {
   const ssm_linear_ce_args& a = r.a;
   const Plan& p = r.p;
-  rows_kernel<<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z, write);
-  if (const int rc = launch_status("linear_ce rows_kernel")) return rc;
+  int device = 0;  // a thread's first call into the runtime makes the context current, which the description of a matrix needs (a backward pass runs on a thread of its own)
+  if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return fail(SSM_ERR_DEVICE, "linear_cross_entropy: no device");
   const int64_t plane_h = up(p.rows, kTile) * p.ldh, plane_w = p.copy_w ? p.vocab * p.ldh : p.vocab * a.weight_stride;
   auto pack = [&](const void* src, int64_t stride, int64_t rows, const int* map, uint16_t* dst, int64_t plane) {
     const unsigned grid = (unsigned)((rows + 7) / 8);
@@ -1051,12 +1219,24 @@ int prepare(Run& r, bool write) {
     else pack_kernel<uint16_t, 1><<<grid, 256, 0, r.st>>>(src, stride, rows, (int)p.dim, map, r.count(), dst, p.ldh, plane);
     return launch_status("linear_ce pack_kernel");
   };
-  if (const int rc = pack(a.hidden, a.hidden_stride, p.rows, r.idx(), r.at<uint16_t>(p.h), plane_h)) return rc;
-  if (p.copy_w)
+  if (packs && p.rows <= kFewRows) {
+    if (p.planes == 3)
+      few_rows_kernel<float, 3><<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, a.hidden, a.hidden_stride, (int)p.dim, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z,
+                                                      r.at<uint16_t>(p.h), p.ldh, plane_h);
+    else
+      few_rows_kernel<uint16_t, 1><<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, a.hidden, a.hidden_stride, (int)p.dim, r.idx(), r.packed(), r.count(), a.row_loss,
+                                                         a.log_z, r.at<uint16_t>(p.h), p.ldh, plane_h);
+    if (const int rc = launch_status("linear_ce few_rows_kernel")) return rc;
+  } else if (packs) {
+    rows_kernel<<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z);
+    if (const int rc = launch_status("linear_ce rows_kernel")) return rc;
+    if (const int rc = pack(a.hidden, a.hidden_stride, p.rows, r.idx(), r.at<uint16_t>(p.h), plane_h)) return rc;
+  }
+  if (packs && p.copy_w)
     if (const int rc = pack(a.weight, a.weight_stride, p.vocab, nullptr, r.at<uint16_t>(p.w), plane_w)) return rc;
   if (const int rc = encode(&r.mh, r.at<void>(p.h), p.dim, p.rows, p.planes, p.ldh, plane_h, p.fmt)) return rc;
   if (const int rc = encode(&r.mw, r.w(), p.dim, p.vocab, p.planes, r.ldw(), plane_w, p.fmt)) return rc;
-  return p.g ? encode(&r.mg, r.at<void>(p.g), p.vocab, p.piece, p.planes, p.ldg, p.piece * p.ldg, p.fmt) : SSM_OK;
+  return p.g > 0 ? encode(&r.mg, r.at<void>(p.g), p.vocab, p.piece, p.planes, p.ldg, p.piece * p.ldg, p.fmt) : SSM_OK;
 }
 // z = h W^T for the packed rows [row0, row0 + rows)
 GemmArgs logits_args(const Run& r, int64_t row0, int64_t rows) {
@@ -1090,7 +1270,7 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
   if (const int rc = gemm_of<kOut>(p, r.mg, r.mw, h2, g, r.st)) return rc;
   if (!dh) return SSM_OK;
   const unsigned grid = (unsigned)((rows + 7) / 8);
-  const bool wide = p.dim % 4 == 0 && r.a.weight_stride % 4 == 0 && aligned_to(r.a.weight, 16);
+  const bool wide = p.dim % 4 == 0 && r.a.weight_stride % 4 == 0 && aligned_to({r.a.weight, dh}, 16);
   auto kern = wide ? dhidden_kernel<4> : dhidden_kernel<1>;
   kern<<<grid, 256, 0, r.st>>>(a.out, a.splits, a.out_split, p.ldo, (int)p.dim, r.idx(), r.packed(), r.count(), (int)row0, (int)rows, r.row(), by_row, r.at<float>(p.scales), r.a.weight, r.a.weight_stride,
                                r.a.io_dtype, dh, dh_dtype);
@@ -1151,6 +1331,11 @@ __global__ void share_kernel(const int* count, int mean, float* kept, float* sca
 
 using namespace ssmb;
 
+extern "C" int64_t ssm_linear_ce_packs_bytes(const ssm_linear_ce_args* args) {
+  if (!args || args->rows < 0 || args->dim < 1 || args->vocab < 1) return 0;
+  return plan_of(*args, kForward).kept;
+}
+
 extern "C" int64_t ssm_linear_ce_scratch_bytes(const ssm_linear_ce_args* args, int32_t pass) {
   if (!args || args->rows < 0 || args->dim < 1 || args->vocab < 1) return 0;
   return plan_of(*args, pass).bytes;
@@ -1168,7 +1353,21 @@ extern "C" int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t st
     float4* stats = a.stats ? reinterpret_cast<float4*>(a.stats) : r.row();
     for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
       const int64_t rows = std::min(p.piece, p.rows - row0);
-      const GemmArgs g = logits_args(r, row0, rows);
+      GemmArgs g = logits_args(r, row0, rows);
+      // Up to 64 rows the weight's rows are M and the packed rows N (32 or 64 columns of a tile instead of 256 rows): the products then take no longer than the weight's way from
+      // memory (7 rows, 50277 x 768: 31 us the other way round)
+      if (p.rows <= kFewRows) {
+        g.bn = p.rows <= 32 ? 32 : 64;
+        Job& j = g.job[0];
+        j.m_tiles = j.n_tiles, j.n_tiles = 1, j.a_m0 = 0;
+        g.part_ld = 8 * j.m_tiles;
+        CUtensorMap mf;
+        if (const int rc = encode(&mf, r.at<void>(p.h), p.dim, p.rows, p.planes, p.ldh, up(p.rows, kTile) * p.ldh, p.fmt, g.bn / 2)) return rc;
+        if (const int rc = gemm_of<kFew>(p, r.mw, mf, mf, g, r.st)) return rc;
+        few_join_kernel<<<(unsigned)p.rows, 256, 0, r.st>>>(g.part, g.part_ld, g.count, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z);
+        if (const int rc = launch_status("linear_ce few_join_kernel")) return rc;
+        continue;
+      }
       if (const int rc = gemm_of<kStats>(p, r.mh, r.mw, r.mw, g, r.st)) return rc;
       join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z);
       if (const int rc = launch_status("linear_ce join_kernel")) return rc;

@@ -130,7 +130,7 @@ Tensor rows_of(const Tensor& t) {
   return (d.size(1) <= 1 || d.stride(1) == 1) && (d.size(0) <= 1 || d.stride(0) >= d.size(1)) ? d : d.contiguous();
 }
 struct LinearCeCall final : Call {
-  Tensor h, w, targets, stats, dh32, dw32, kept;  // stats: for a second pass; the others: of a pass that formed the gradients too
+  Tensor h, w, targets, stats, packs, dh32, dw32, kept;  // stats, packs: for a second pass; the others: of a pass that formed the gradients too
   std::vector<int64_t> shape, lead_shape;
   at::ScalarType t_w;
   int64_t ignore;
@@ -178,6 +178,8 @@ struct LinearCeCall final : Call {
     if (train && !both) stats = at::empty({std::max<int64_t>(rows(), 1), 4}, f32());
     ssm_linear_ce_args a{};
     fill(a);
+    packs = at::empty({std::max<int64_t>(ssm_linear_ce_packs_bytes(&a), 256)}, h.options().dtype(at::kByte));
+    a.packs = packs.data_ptr();
     const Tensor s = scratch(a, both ? 2 : 0);
     a.row_loss = row_loss.data_ptr<float>(), a.log_z = log_z.data_ptr<float>();
     if (reduction) loss = at::empty({}, f32()), a.loss = loss.data_ptr<float>();
@@ -189,6 +191,7 @@ struct LinearCeCall final : Call {
     } else {
       run(ssm_linear_ce_fwd(&a, stream_of(h)));
     }
+    if (both || !train) packs.reset();
     variable_list res = {reduction ? loss : row_loss};
     if (want_z) res.push_back(log_z);
     return res;
@@ -209,6 +212,7 @@ struct LinearCeCall final : Call {
     }
     ssm_linear_ce_bwd_args b{};
     fill(b.fwd);
+    b.fwd.packs = packs.data_ptr();
     const Tensor s = scratch(b.fwd, 1);
     b.dloss = gl.data_ptr<float>(), b.dlog_z = gz.defined() ? gz.data_ptr<float>() : nullptr;
     if (grad_h) b.dhidden = dh.data_ptr();
