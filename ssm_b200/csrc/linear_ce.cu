@@ -51,6 +51,7 @@ struct Job {
   float* out;                  // kOut: [split][row][ld]
   int64_t ld, out_split;
   int out_rows, add;
+  int last;                    // the last piece of dW: 1 rounded into its place, with the targets' part; 2 added to the sums, with it
 };
 struct GemmArgs {
   Job job[2];                  // kOut takes two; no tiles: none
@@ -68,6 +69,14 @@ struct GemmArgs {
   uint16_t* g;                 // [plane][row][ldg]
   int64_t ldg, g_plane;
   const int* again;            // kKeep, nullable: the tiles of rows to be formed again
+  // kOut, the last piece of dW: dw = (sums + the target's row) scales[1]
+  void* dw;
+  int64_t dw_ld;
+  int dw_dtype, dw_wide, dim;
+  const float* scales;
+  const int* heads;            // [sort][vocab]: the target's row in target_sums, or -1
+  int sorts;
+  const float* target_sums;    // [row][ld of the job]
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -146,6 +155,59 @@ struct TileAt {
   int job, m, n, split, kb0, kb1;  // job -1: no more
 };
 
+// 32 columns of a row of dW from `col` on, of which `cols` are there: the targets' part
+__device__ __forceinline__ void add_columns(const float* from, int cols, uint32_t (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    if (i < cols) {  // the rows of these buffers have room for whole pieces
+      const float4 o = *reinterpret_cast<const float4*>(from + i);
+      v[i] = __float_as_uint(__uint_as_float(v[i]) + o.x), v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) + o.y);
+      v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) + o.z), v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) + o.w);
+    }
+  }
+}
+__device__ __forceinline__ void add_target(const GemmArgs& g, const Job& j, int row, int64_t col, uint32_t (&v)[32]) {
+  const int cols = (int)min((int64_t)32, g.dim - col);
+  if (cols <= 0) return;
+  for (int b = 0; b < g.sorts; ++b) {
+    const int at = g.heads[(int64_t)b * j.out_rows + row];
+    if (at >= 0) add_columns(g.target_sums + at * j.ld + col, cols, v);
+  }
+}
+// ... and their way into dW
+__device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bool add, int row, int64_t col, uint32_t (&v)[32]) {
+  const int cols = (int)min((int64_t)32, g.dim - col);
+  if (cols <= 0) return;
+  if (add) add_columns(j.out + row * j.ld + col, cols, v);
+  const float f = g.scales[1];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+  const int64_t to = row * g.dw_ld + col;
+  if (g.dw_wide && cols == 32) {
+    if (g.dw_dtype == SSM_F32) {
+      float* out = reinterpret_cast<float*>(g.dw) + to;
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(out + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+      uint16_t* out = reinterpret_cast<uint16_t*>(g.dw) + to;
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = __uint_as_float(v[i + 2 * k]), b = __uint_as_float(v[i + 2 * k + 1]);
+          w[k] = g.dw_dtype == SSM_BF16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
+        }
+        *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < cols) store_dyn(g.dw, to + i, g.dw_dtype, __uint_as_float(v[i]));
+  }
+}
+
 template <int EPI, typename T, int PLANES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mb1, const __grid_constant__ GemmArgs g) {
@@ -170,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // its time, then all take turns: the tiles that run at one time stay neighbours, and share operands in the L2.
   const int m0 = (live + kTile - 1) / kTile, kb_rows = (live + kK - 1) / kK;
   const int tiles0 = live > 0 ? (g.job[0].k_is_rows || EPI == kFew ? g.job[0].m_tiles : min(g.job[0].m_tiles, m0)) * g.job[0].n_tiles * g.job[0].splits : 0;
-  const int tiles1 = EPI == kOut && live > 0 ? (g.job[1].k_is_rows ? g.job[1].m_tiles : min(g.job[1].m_tiles, m0)) * g.job[1].n_tiles * g.job[1].splits : 0;
+  const int tiles1 = EPI == kOut && (live > 0 || g.job[1].last) ? (g.job[1].k_is_rows ? g.job[1].m_tiles : min(g.job[1].m_tiles, m0)) * g.job[1].n_tiles * g.job[1].splits : 0;
   const int extra = tiles0 % pairs, mine0 = tiles0 / pairs + (pair < extra ? 1 : 0);
   const int alone = EPI == kOut && extra ? g.job[0].k_blocks / g.job[0].splits / max(1, g.job[1].k_is_rows ? kb_rows : g.job[1].k_blocks) : 0;
   auto place = [&](int k) {
@@ -327,30 +389,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Job& j = g.job[p.job];
       const int row = p.m * kTile + row_in, width = g.bn / 2;
       const int64_t out_col = p.n * g.bn + half * width;
+      const bool none = p.kb0 == p.kb1;  // no rows in the last piece
+      const bool add = EPI == kOut && j.add && *g.count > 0;
       if constexpr (!kSegments) {
         const int b = n & 1;
-        if (!arrived(b)) break;
+        if (!none && !arrived(b)) break;
         const uint32_t from = tmem + lanes + b * 256 + half * width;
         float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
         const int cols = (int)min((int64_t)width, j.ld - out_col);
         for (int c = 0; c < width; c += 32) {
           uint32_t v[32];
-          tmem_ld32_issue(from + c, v);
-          tmem_wait_ld();
-          if (row < j.out_rows) {
+          if (none) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0u;
+          } else {
+            tmem_ld32_issue(from + c, v);
+            tmem_wait_ld();
+          }
+          if (j.last && row < j.out_rows) add_target(g, j, row, out_col + c, v);
+          if (j.last == 1 && row < j.out_rows) {
+            last_columns(g, j, add, row, out_col + c, v);
+          } else if (row < j.out_rows) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               if (c + i < cols) {
-                if (j.add) asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"l"(out + c + i), "f"(__uint_as_float(v[i])), "f"(__uint_as_float(v[i + 1])),
-                                        "f"(__uint_as_float(v[i + 2])), "f"(__uint_as_float(v[i + 3]))
-                                        : "memory");
+                if (add) asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"l"(out + c + i), "f"(__uint_as_float(v[i])), "f"(__uint_as_float(v[i + 1])),
+                                      "f"(__uint_as_float(v[i + 2])), "f"(__uint_as_float(v[i + 3]))
+                                      : "memory");
                 else *reinterpret_cast<uint4*>(out + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
               }
             }
           }
+          __syncwarp();  // the next columns are read by the whole warp
         }
-        release(b);
-        ++n;
+        if (!none) {
+          release(b);
+          ++n;
+        }
       } else {
         constexpr int kChunks = EPI == kFew ? 1 : 4;
         uint32_t v[kChunks][32];
@@ -384,6 +459,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           release(b);
         }
         if (!ok) break;
+        if (EPI == kOut && none) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[c][i] = 0u;
+        }
         if constexpr (EPI == kFew) {  // a thread has a row of the weight, its registers packed rows
           const int id = p.m * kTile + row_in, first = half * width;
           const bool in = id < g.vocab;
@@ -402,13 +483,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         } else if constexpr (EPI == kOut) {
           float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
           const int cols = (int)min((int64_t)width, j.ld - out_col);
-          if (row < j.out_rows) {
+          if (row < j.out_rows && j.last) {  // fp32 is not formed in one pass
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (32 * c < width) {
+                add_target(g, j, row, out_col + 32 * c, v[c]);
+                last_columns(g, j, add, row, out_col + 32 * c, v[c]);
+              }
+            }
+          } else if (row < j.out_rows) {
 #pragma unroll
             for (int i = 0; i < 128; i += 4) {
               if (i < cols) {
                 float4 w = make_float4(__uint_as_float(v[i / 32][i % 32]), __uint_as_float(v[i / 32][i % 32 + 1]), __uint_as_float(v[i / 32][i % 32 + 2]), __uint_as_float(v[i / 32][i % 32 + 3]));
                 float4* to = reinterpret_cast<float4*>(out + i);
-                if (j.add) {
+                if (add) {
                   const float4 o = *to;
                   w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
                 }
@@ -607,6 +696,19 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
     } else {
       for (int c = lane; c < dim; c += 32) to[c] = zero ? (uint16_t)0 : bits[c];
     }
+  } else if (dim % 4 == 0 && reinterpret_cast<uintptr_t>(row) % 16 == 0) {
+#pragma unroll 4
+    for (int c = lane * 4; c < dim; c += 128) {
+      const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + c);
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      __nv_bfloat16 p[4][3];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) split3(zero ? 0.f : f[k], p[k]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<uint2*>(to + q * plane + c) = make_uint2((uint32_t)__bfloat16_as_ushort(p[0][q]) | (uint32_t)__bfloat16_as_ushort(p[1][q]) << 16,
+                                                                   (uint32_t)__bfloat16_as_ushort(p[2][q]) | (uint32_t)__bfloat16_as_ushort(p[3][q]) << 16);
+    }
   } else {
     for (int c = lane; c < dim; c += 32) {
       __nv_bfloat16 p[3];
@@ -649,6 +751,14 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* __restric
   const int n = kept_s;
   for (int r = warp; r < rows; r += 32) {  // zeros behind the last one that counts
     const T* row = reinterpret_cast<const T*>(src) + (r < n ? rows_of[r] : 0) * stride;
+    if (PLANES == 1 && dim % 8 == 0 && reinterpret_cast<uintptr_t>(row) % 16 == 0) {
+#pragma unroll 4
+      for (int c = lane * 8; c < dim; c += 256) {
+        const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + c);
+        *reinterpret_cast<uint4*>(dst + r * ld + c) = r < n ? v : make_uint4(0, 0, 0, 0);
+      }
+      continue;
+    }
 #pragma unroll 4
     for (int c = lane; c < dim; c += 32) {
       if constexpr (PLANES == 1) {
@@ -995,14 +1105,15 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targ
   for (int e = 0; e < 8; ++e)
     if (tid * 8 + e < size) keys[first + tid * 8 + e] = key[e] == ~(Key)0 ? ~0ull : (uint64_t)(key[e] >> 13) << 32 | (uint32_t)(first + (int)(key[e] & (kSort - 1)));
 }
-// dweight's row of a target += the sum of q h over the rows that have it, in their order: one block (of 128 V columns) for each run of equal targets, eight rows on their way at
-// a time (a common token has hundreds).
+// The sum of q h over the rows that have a target, in their order, at the place of the first of them, and that place by target: one block (of 128 V columns) for each run of equal
+// targets, eight rows on their way at a time (a common token has hundreds).
 template <int V>
 __global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* __restrict__ keys, int size, const float4* __restrict__ row, const int* __restrict__ idx, const void* hidden, int64_t stride, int dtype,
-                                                          int dim, const float* __restrict__ scales, float* __restrict__ out, int64_t ld) {
+                                                          int dim, const float* __restrict__ scales, float* __restrict__ sums, int64_t ld, int* __restrict__ heads, int place) {
   const int p = blockIdx.x;
   const uint64_t key = keys[p];
   if (key == ~0ull || (p > 0 && keys[p - 1] >> 32 == key >> 32)) return;
+  if (blockIdx.y == 0 && threadIdx.x == 0) heads[key >> 32] = place + p;
   const int c = (blockIdx.y * 128 + threadIdx.x) * V;
   if (c >= dim) return;
   float v[V] = {};
@@ -1041,14 +1152,9 @@ __global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* __rest
     if (r[7] < 0) break;
   }
   const float scale = scales[0];
-  float* to = out + (int64_t)(key >> 32) * ld + c;
-  if constexpr (V == 4) {
-    float4 o = *reinterpret_cast<const float4*>(to);
-    o.x = fmaf(v[0], scale, o.x), o.y = fmaf(v[1], scale, o.y), o.z = fmaf(v[2], scale, o.z), o.w = fmaf(v[3], scale, o.w);
-    *reinterpret_cast<float4*>(to) = o;
-  } else {
-    *to = fmaf(v[0], scale, *to);
-  }
+  float* to = sums + (int64_t)(place + p) * ld + c;
+  if constexpr (V == 4) *reinterpret_cast<float4*>(to) = make_float4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
+  else *to = v[0] * scale;
 }
 
 // out = factor * src, the factor scales[1] (dloss NULL) or scales[1] dloss; zeros where no row counts.  V elements at a time.
@@ -1109,7 +1215,7 @@ struct Plan {
   int splits, bn;     // of dh = G W
   int parts, sort, sorts;
   // offsets: what both passes use (kept between them), then scratch
-  int64_t idx, packed, count, h, w, kept, scales, part, z, row, g, dh, dw, keys, again, hs, bytes;
+  int64_t idx, packed, count, h, w, kept, scales, part, z, row, g, dh, dw, keys, heads, sums, again, hs, bytes;
 };
 constexpr int64_t kForwardRows = 16384;
 
@@ -1153,7 +1259,8 @@ Plan plan_of(const ssm_linear_ce_args& a, int pass) {
   if (pass != kBackward) p.part = take((int64_t)p.parts * p.piece * 8), p.z = take(p.rows * 4);
   if (pass != kForward) {
     p.g = take(p.planes * p.piece * p.ldg * 2), p.dh = take((int64_t)p.splits * p.piece * p.ldo * 4), p.keys = take((int64_t)p.sorts * kSort * 8);
-    if (pass == kBackward) p.dw = take(p.vocab * p.ldo * 4);
+    p.heads = take((int64_t)p.sorts * p.vocab * 4), p.sums = take((int64_t)p.sorts * p.sort * p.ldo * 4);
+    if (pass == kBackward) p.dw = take(p.piece < p.rows ? p.vocab * p.ldo * 4 : 0);
     else p.again = take(p.piece / kTile * 4), p.hs = take(up(p.rows, kTile) * p.ldh * 2);
   }
   p.bytes = at - p.kept;
@@ -1251,8 +1358,44 @@ GemmArgs logits_args(const Run& r, int64_t row0, int64_t rows) {
   g.g = r.at<uint16_t>(p.g), g.ldg = p.ldg, g.g_plane = p.piece * p.ldg;
   return g;
 }
+int zero(void* p, size_t bytes, cudaStream_t st, int byte = 0) {
+  const cudaError_t e = cudaMemsetAsync(p, byte, bytes, st);
+  if (e == cudaSuccess) return SSM_OK;
+  set_error("linear_cross_entropy: %s", cudaGetErrorString(e));
+  return (int)e;
+}
+// the targets' part of dW, by target
+int target_rows(const Run& r) {
+  const Plan& p = r.p;
+  uint64_t* keys = r.at<uint64_t>(p.keys);
+  const unsigned threads = (unsigned)std::max(32, p.sort / 8);
+  if (p.vocab < 1 << 19) {
+    sort_kernel<uint32_t><<<p.sorts, threads, threads * 32, r.st>>>(r.packed(), r.count(), p.sort, keys);
+  } else {
+    cudaFuncSetAttribute(sort_kernel<uint64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
+    sort_kernel<uint64_t><<<p.sorts, threads, threads * 64, r.st>>>(r.packed(), r.count(), p.sort, keys);
+  }
+  if (const int rc = launch_status("linear_ce sort_kernel")) return rc;
+  if (const int rc = zero(r.at<void>(p.heads), (size_t)p.sorts * p.vocab * 4, r.st, 0xff)) return rc;
+  const bool wide = p.dim % 4 == 0 && r.a.hidden_stride % 4 == 0 && aligned_to(r.a.hidden, 16);
+  auto kern = wide ? target_rows_kernel<4> : target_rows_kernel<1>;
+  const int per = wide ? 512 : 128;
+  for (int i = 0; i < p.sorts; ++i) {
+    kern<<<dim3((unsigned)p.sort, (unsigned)((p.dim + per - 1) / per)), 128, 0, r.st>>>(keys + (int64_t)i * kSort, p.sort, r.row(), r.idx(), r.a.hidden, r.a.hidden_stride, r.a.io_dtype, (int)p.dim,
+                                                                                      r.at<float>(p.scales), r.at<float>(p.sums), p.ldo, r.at<int>(p.heads) + (int64_t)i * p.vocab, i * p.sort);
+    if (const int rc = launch_status("linear_ce target_rows_kernel")) return rc;
+  }
+  return SSM_OK;
+}
+// dW's place: fp32 sums of the pieces before the last, and where the last one leaves it
+struct WeightGrad {
+  float* sums;
+  void* out;
+  int64_t ld;
+  int dtype;
+};
 // dh = G W and dW += G^T h of a piece, `h2` for h, and dh's way to its rows; each nullable
-int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, bool by_row, void* dh, int dh_dtype, float* dw) {
+int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, bool by_row, void* dh, int dh_dtype, const WeightGrad* dw) {
   const Plan& p = r.p;
   GemmArgs g{};
   g.bn = p.bn, g.fmt = p.fmt, g.row0 = (int)row0, g.rows = (int)rows, g.count = r.count(), g.status = r.a.status;
@@ -1265,7 +1408,12 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
   }
   if (dw) {
     b.m_tiles = (int)((p.vocab + kTile - 1) / kTile), b.n_tiles = d_tiles, b.a_mn = b.b_mn = 1, b.k_is_rows = 1, b.b_k0 = (int)row0;
-    b.out = dw, b.ld = p.ldo, b.out_rows = (int)p.vocab, b.add = row0 > 0;
+    b.out = dw->sums, b.ld = p.ldo, b.out_rows = (int)p.vocab, b.add = row0 > 0, b.last = row0 + rows < p.rows ? 0 : dw->out == dw->sums ? 2 : 1;
+    if (b.last) {
+      if (const int rc = target_rows(r)) return rc;
+      g.dw = dw->out, g.dw_ld = dw->ld, g.dw_dtype = dw->dtype, g.dw_wide = dw->ld % (dw->dtype == SSM_F32 ? 4 : 8) == 0 && aligned_to(dw->out, 16), g.dim = (int)p.dim;
+      g.scales = r.at<float>(p.scales), g.heads = r.at<int>(p.heads), g.sorts = p.sorts, g.target_sums = r.at<float>(p.sums);
+    }
   }
   if (const int rc = gemm_of<kOut>(p, r.mg, r.mw, h2, g, r.st)) return rc;
   if (!dh) return SSM_OK;
@@ -1276,28 +1424,6 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
                                r.a.io_dtype, dh, dh_dtype);
   return launch_status("linear_ce dhidden_kernel");
 }
-// the targets' part of dW
-int target_rows(const Run& r, float* dw) {
-  const Plan& p = r.p;
-  uint64_t* keys = r.at<uint64_t>(p.keys);
-  const unsigned threads = (unsigned)std::max(32, p.sort / 8);
-  if (p.vocab < 1 << 19) {
-    sort_kernel<uint32_t><<<p.sorts, threads, threads * 32, r.st>>>(r.packed(), r.count(), p.sort, keys);
-  } else {
-    cudaFuncSetAttribute(sort_kernel<uint64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
-    sort_kernel<uint64_t><<<p.sorts, threads, threads * 64, r.st>>>(r.packed(), r.count(), p.sort, keys);
-  }
-  if (const int rc = launch_status("linear_ce sort_kernel")) return rc;
-  const bool wide = p.dim % 4 == 0 && r.a.hidden_stride % 4 == 0 && aligned_to(r.a.hidden, 16);
-  auto kern = wide ? target_rows_kernel<4> : target_rows_kernel<1>;
-  const int per = wide ? 512 : 128;
-  for (int i = 0; i < p.sorts; ++i) {
-    kern<<<dim3((unsigned)p.sort, (unsigned)((p.dim + per - 1) / per)), 128, 0, r.st>>>(keys + (int64_t)i * kSort, p.sort, r.row(), r.idx(), r.a.hidden, r.a.hidden_stride, r.a.io_dtype, (int)p.dim,
-                                                                                      r.at<float>(p.scales), dw, p.ldo);
-    if (const int rc = launch_status("linear_ce target_rows_kernel")) return rc;
-  }
-  return SSM_OK;
-}
 int scaled_copy(const float* src, int64_t ld, int64_t rows, int64_t dim, const int* count, const float* scales, const float* dloss, void* out, int dtype, cudaStream_t st) {
   const bool wide = dim % 4 == 0 && ld % 4 == 0 && aligned_to({src, out}, 16);
   const int64_t all = rows * (wide ? dim / 4 : dim);
@@ -1305,12 +1431,6 @@ int scaled_copy(const float* src, int64_t ld, int64_t rows, int64_t dim, const i
   auto kern = wide ? scaled_copy_kernel<4> : scaled_copy_kernel<1>;
   kern<<<grid, 256, 0, st>>>(src, ld, rows, (int)dim, count, scales, dloss ? dloss : scales, dloss != nullptr, out, dtype);
   return launch_status("linear_ce scaled_copy_kernel");
-}
-int zero(void* p, size_t bytes, cudaStream_t st) {
-  const cudaError_t e = cudaMemsetAsync(p, 0, bytes, st);
-  if (e == cudaSuccess) return SSM_OK;
-  set_error("linear_cross_entropy: %s", cudaGetErrorString(e));
-  return (int)e;
 }
 int reduce(const Run& r) {
   if (r.a.reduction == 0) return SSM_OK;
@@ -1388,18 +1508,17 @@ extern "C" int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_
   const Plan& p = r.p;
   if (a.rows == 0) return args->dweight ? zero(args->dweight, (size_t)a.vocab * a.dim * dtype_size(args->dweight_dtype), r.st) : SSM_OK;
   if (const int rc = prepare(r, false)) return rc;
-  float *scales = r.at<float>(p.scales), *dw = args->dweight ? r.at<float>(p.dw) : nullptr;
+  float* scales = r.at<float>(p.scales);
+  const WeightGrad dw{r.at<float>(p.dw), args->dweight, p.dim, args->dweight_dtype};
   weights_kernel<<<1, 1024, 0, r.st>>>(reinterpret_cast<const float4*>(a.stats), r.idx(), r.count(), args->dloss, a.reduction, args->dlog_z ? args->dlog_z : args->dloss, args->dlog_z != nullptr,
                                        a.io_dtype == SSM_F16, r.row(), scales);
   if (const int rc = launch_status("linear_ce weights_kernel")) return rc;
   for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
     const int64_t rows = std::min(p.piece, p.rows - row0);
     if (const int rc = gemm_of<kGrad>(p, r.mh, r.mw, r.mw, logits_args(r, row0, rows), r.st)) return rc;
-    if (const int rc = gradients(r, row0, rows, r.mh, false, args->dhidden, a.io_dtype, dw)) return rc;
+    if (const int rc = gradients(r, row0, rows, r.mh, false, args->dhidden, a.io_dtype, args->dweight ? &dw : nullptr)) return rc;
   }
-  if (!dw) return SSM_OK;
-  if (const int rc = target_rows(r, dw)) return rc;
-  return scaled_copy(dw, p.ldo, p.vocab, p.dim, r.count(), scales, nullptr, args->dweight, args->dweight_dtype, r.st);
+  return SSM_OK;
 }
 
 extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidden, float* dweight, float* kept, ssm_stream_t stream) {
@@ -1419,6 +1538,7 @@ extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidde
   CUtensorMap mhs;
   if (const int rc = encode(&mhs, hs, p.dim, p.rows, 1, p.ldh, up(p.rows, kTile) * p.ldh, p.fmt)) return rc;
   int* again = r.at<int>(p.again);
+  const WeightGrad dw{dweight, dweight, p.ldo, SSM_F32};
   for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
     const int64_t rows = std::min(p.piece, p.rows - row0);
     const unsigned warps = (unsigned)((rows + 7) / 8);
@@ -1435,10 +1555,8 @@ extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidde
       scaled_rows_kernel<<<warps, 256, 0, r.st>>>(h, p.ldh, (int)p.dim, r.row(), r.count(), row0, rows, hs);
       if (const int rc = launch_status("linear_ce scaled_rows_kernel")) return rc;
     }
-    if (const int rc = gradients(r, row0, rows, mhs, true, dhidden, SSM_F32, dweight)) return rc;
+    if (const int rc = gradients(r, row0, rows, mhs, true, dhidden, SSM_F32, dweight ? &dw : nullptr)) return rc;
   }
-  if (dweight)
-    if (const int rc = target_rows(r, dweight)) return rc;
   return reduce(r);
 }
 

@@ -375,3 +375,28 @@ def test_an_edit_between_the_passes_and_second_derivatives_are_errors():
     g = torch.autograd.grad(ops.linear_cross_entropy(h, w, t).sum(), h, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="differentiable once"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_last_piece_without_rows(dtype):
+    """Pieces of 512 MB: nothing, or nothing in the last of them, counts."""
+    h, w, t, wl, wz = make(2000 if dtype != torch.float32 else 600, 40, 151936, dtype)
+    t[300:] = -100
+    check(h, w, t, wl, wz)
+    if dtype == torch.bfloat16:
+        one_pass(h, w, t)
+    t[:] = -100
+    dh, dw = check(h, w, t, wl, wz)
+    assert not dh.any() and not dw.any()
+
+
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("d", [33, 36, 40, 64, 264])
+def test_odd_widths_of_every_type_of_weight(wt, d):
+    h, w, t, wl, wz = make(400, d, 700, torch.bfloat16)
+    t[:200] = 3  # a common one
+    w = w.to(wt).requires_grad_(True)
+    h = h.requires_grad_(True)
+    val, tol = bounds(h, w.to(torch.bfloat16), t, wl, 0 * wz)[3]
+    near(torch.autograd.grad(ops.linear_cross_entropy(h, w, t), w, wl)[0], val, tol + half(wt) * val.abs(), "dw")
+    one_pass(h.detach(), w.detach().to(torch.bfloat16), t)
