@@ -37,8 +37,8 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
     at = torch.where(kept, targets, torch.zeros_like(targets)).long()
     bad = (at < 0) | (at >= weight.shape[0])
     loss = log_z - torch.gather(z, -1, at.clamp(0, weight.shape[0] - 1)[..., None])[..., 0]
-    loss = torch.where(bad, loss * math.nan, loss)
     none = torch.zeros((), dtype=z.dtype, device=z.device)
+    loss = loss + torch.where(bad, none + math.nan, none)
     loss, log_z = torch.where(kept, loss, none), torch.where(kept, log_z, none)
     if reduction != "none":
         loss = loss.sum()
@@ -64,3 +64,13 @@ def clip_global_norm_(tensors, max_norm, norm_type=2.0):
         for t in tensors:
             t.detach().copy_(t.detach().double() * c)
     return norm
+
+
+def namespace():
+    """The oracle's operators under one roof, as ``ssm_b200.ops`` has them."""
+    from . import lm_oracle
+
+    ns = lm_oracle.namespace()
+    for fn in (fused_block_norm, linear_cross_entropy, global_norm, clip_global_norm_):
+        setattr(ns, fn.__name__, fn)
+    return ns

@@ -12,7 +12,9 @@ Attention layers and the gated MLP of upstream's hybrid configurations are outsi
 rejected.  Beyond upstream: ``forward(..., sharded=True, group=pg)`` runs a Mamba-2 stack on one contiguous shard of a
 sequence split over ranks (`ssm_b200.seqpar`), and ``step`` decodes one token against caches allocated by
 ``allocate_inference_cache``; ``MambaLMHeadModel.score`` gives the log probabilities of given tokens and ``distill_loss`` the divergence from a
-teacher's top logits, both differentiable.
+teacher's top logits, both differentiable; ``loss`` is the cross entropy of the next token without the logits, ``clip_grad_norm_`` clips all gradients by their
+norm; ``ssm_cfg["post_norm"]`` puts a norm after every mixer, with a learned gate (``"post_gate"``) and a factor (``"residual_scale"``), one call with the
+residual add and the next layer's norm.
 """
 
 from __future__ import annotations
@@ -73,6 +75,10 @@ class MixerModel(nn.Module):
         cfg = dict(ssm_cfg or {})
         kind = cfg.pop("layer", "Mamba1")
         cfg.pop("dt_init", None)
+        self.post_norm, post_gate = bool(cfg.pop("post_norm", False)), bool(cfg.pop("post_gate", False))
+        self.residual_scale = float(cfg.pop("residual_scale", 1.0))
+        if not self.post_norm and (post_gate or self.residual_scale != 1.0):
+            raise ValueError("ssm_cfg['post_gate'] and ['residual_scale'] belong to ['post_norm']")
         if kind in ("Mamba2", "GatedDelta"):
             cfg.pop("dt_rank", None)  # one step size per head, projected straight from the input
         if kind not in ("Mamba1", "Mamba2", "GatedDelta"):
@@ -92,6 +98,13 @@ class MixerModel(nn.Module):
         if not rms_norm:
             for layer in self.layers:
                 layer.norm_b = nn.Parameter(torch.zeros(d_model, **kw))
+        if self.post_norm:
+            for layer in self.layers:
+                layer.post_norm_w = nn.Parameter(torch.ones(d_model, **kw))
+                if not rms_norm:
+                    layer.post_norm_b = nn.Parameter(torch.zeros(d_model, **kw))
+                if post_gate:
+                    layer.post_gate = nn.Parameter(torch.ones(d_model, **kw))
         rescale = (initializer_cfg or {}).get("rescale_prenorm_residual", True)
         if rescale:  # upstream divides the output projections by sqrt(n_layer) (lm.py:80-98)
             with torch.no_grad():
@@ -108,6 +121,13 @@ class MixerModel(nn.Module):
     def _pre_norm(self, layer):
         return (layer.norm_w if self.kind == "Mamba1" else layer.pre_norm_w), getattr(layer, "norm_b", None)
 
+    def _norm(self, ops, before, hidden: Tensor, residual: Optional[Tensor], w: Tensor, b: Optional[Tensor]):
+        """The stream behind layer ``before`` (``None``: behind the embedding), and its norm for what comes next."""
+        if before is not None and self.post_norm:
+            return ops.fused_block_norm(hidden, residual, before.post_norm_w, w, post_bias=getattr(before, "post_norm_b", None), bias=b, gate=getattr(before, "post_gate", None),
+                                        residual_scale=self.residual_scale, is_rms=self.rms_norm, eps=self.eps, residual_in_fp32=self.residual_in_fp32)
+        return ops.fused_layer_norm(hidden, w, b, residual=residual, is_rms=self.rms_norm, eps=self.eps, prenorm=True, residual_in_fp32=self.residual_in_fp32, return_residual=True)
+
     def allocate_inference_cache(self, batch_size: int, max_seqlen: int = 0, dtype: Optional[torch.dtype] = None, **kwargs) -> InferenceCache:
         del max_seqlen, kwargs  # state-space layers keep a fixed-size state
         return InferenceCache({i: layer.allocate_inference_cache(batch_size, dtype) for i, layer in enumerate(self.layers)})
@@ -117,14 +137,14 @@ class MixerModel(nn.Module):
         ``L == 1`` the call advances the caches by one token (decode)."""
         ops = self._namespace()
         hidden = self.embedding(input_ids)
-        residual = None
+        residual = before = None
         decode = inference_params is not None and input_ids.shape[1] == 1
         if inference_params is not None and not decode:
             raise ValueError("prefill into a cache is not built: feed the prompt token by token, or run forward() without a cache")
         for i, layer in enumerate(self.layers):
             w, b = self._pre_norm(layer)
-            hidden, residual = ops.fused_layer_norm(hidden, w, b, residual=residual, is_rms=self.rms_norm, eps=self.eps, prenorm=True,
-                                                    residual_in_fp32=self.residual_in_fp32, return_residual=True)
+            hidden, residual = self._norm(ops, before, hidden, residual, w, b)
+            before = layer
             if decode:
                 hidden = layer.mixer_step(hidden[:, 0], inference_params.layer_states[i]).unsqueeze(1)
             elif self.kind == "Mamba2":
@@ -135,6 +155,8 @@ class MixerModel(nn.Module):
                 hidden = layer.mixer_forward(hidden)
         if inference_params is not None:
             inference_params.seqlen_offset += input_ids.shape[1]
+        if self.post_norm and before is not None:
+            return self._norm(ops, before, hidden, residual, self.norm_f_weight, self.norm_f_bias)[0]
         return ops.fused_layer_norm(hidden, self.norm_f_weight, self.norm_f_bias, residual=residual, is_rms=self.rms_norm, eps=self.eps,
                                     prenorm=True, residual_in_fp32=self.residual_in_fp32)
 
@@ -172,19 +194,44 @@ class MambaLMHeadModel(nn.Module):
             hidden = hidden[:, -num_last_tokens:, :]
         return CausalLMOutput(logits=self.lm_head(hidden))
 
+    @staticmethod
+    def _whole(what: str, mixer_kwargs: dict) -> None:
+        if mixer_kwargs.get("sharded"):
+            raise ValueError(f"{what}: a shard of a sequence has neither the distribution before its first token nor the token behind its last one")
+        if mixer_kwargs.get("inference_params") is not None or mixer_kwargs.get("num_last_tokens"):
+            raise ValueError(f"{what} runs over the whole sequence: inference_params and num_last_tokens are not taken")
+
+    @staticmethod
+    def _next(tokens: Tensor, ignore_index: int) -> Tensor:
+        """What each position predicts; the last one nothing."""
+        return torch.cat([tokens[:, 1:], torch.full_like(tokens[:, :1], ignore_index)], 1)
+
+    def loss(self, input_ids: Tensor, labels: Optional[Tensor] = None, ignore_index: int = -100, reduction: str = "mean", return_log_z: bool = False, **mixer_kwargs):
+        """Cross entropy of a sequence's own next tokens, without the logits (``ops.linear_cross_entropy`` of the hidden states and the head): the mean over the
+        positions that count, their sum, or with ``reduction="none"`` one per position ``(B, L - 1)``; ``labels (B, L)`` in the place of the tokens, those equal to ``ignore_index``
+        left out; with ``return_log_z`` the log of the partition sums ``(B, L - 1)`` behind it.  A whole sequence at once; over all of the head's columns, padded ones too."""
+        self._whole("loss", mixer_kwargs)
+        if input_ids.dim() != 2:
+            raise ValueError("input_ids must be a 2D tensor of shape (batch, seqlen)")
+        hidden = self.backbone(input_ids, **mixer_kwargs)
+        targets = self._next(input_ids if labels is None else labels, ignore_index)
+        got = self.backbone._namespace().linear_cross_entropy(hidden, self.lm_head.weight, targets, ignore_index, reduction, return_log_z)
+        loss, *log_z = got if return_log_z else (got,)
+        loss = loss[:, :-1] if reduction == "none" else loss
+        return (loss, log_z[0][:, :-1]) if return_log_z else loss
+
+    def clip_grad_norm_(self, max_norm: float, norm_type: float = 2.0) -> Tensor:
+        """Clips the gradients of all parameters by their common norm, which is returned (``ops.clip_global_norm_``); parameters without one are left out."""
+        return self.backbone._namespace().clip_global_norm_([p.grad for p in self.parameters() if p.grad is not None], max_norm, norm_type)
+
     def score(self, input_ids: Tensor, labels: Optional[Tensor] = None, temperature: float = 1.0, top_k: int = 0, return_entropy: bool = False,
               ignore_index: int = -100, **mixer_kwargs):
         """Log probabilities of a sequence's own tokens, each given those before it: ``input_ids (B, L)`` -> ``(B, L - 1)`` fp32, with the entropies and
         the ``top_k`` alternatives behind them as in ``ops.token_log_probs``.  ``labels (B, L)`` in the place of the tokens; those equal to
         ``ignore_index`` give 0.  A whole sequence at once: no shard of one, no cache; over all of the head's columns, padded ones too."""
-        if mixer_kwargs.get("sharded"):
-            raise ValueError("score: a shard of a sequence has neither the distribution before its first token nor the token behind its last one")
-        if mixer_kwargs.get("inference_params") is not None or mixer_kwargs.get("num_last_tokens"):
-            raise ValueError("score runs over the whole sequence: inference_params and num_last_tokens are not taken")
+        self._whole("score", mixer_kwargs)
         logits = self.forward(input_ids, **mixer_kwargs).logits
-        targets = input_ids if labels is None else labels
-        # the logits as they lie, their last row with nothing to predict
-        targets = torch.cat([targets[:, 1:], torch.full_like(targets[:, :1], ignore_index)], 1)
+        targets = self._next(input_ids if labels is None else labels, ignore_index)
         got = self.backbone._namespace().token_log_probs(logits, targets, temperature, top_k, return_entropy, ignore_index)
         return tuple(t[:, :-1] for t in got) if isinstance(got, tuple) else got[:, :-1]
 
