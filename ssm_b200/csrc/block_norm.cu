@@ -98,22 +98,30 @@ __device__ __forceinline__ void convert(const Raw<V>& r, int dtype, float (&f)[V
   }
 }
 
-// sums of two values over a block
-__device__ __forceinline__ void allsum2(float& a, float& b, float2 (*scratch)[16], int& turn) {
+// sums of two values over a block, or of the second alone.  A warp's sums meet in shared memory, where each warp adds them up by shuffles (every thread reading all of them: 25 of the
+// backward pass's 81 instructions an element); two rows of scratch in turn, so that a sum takes one barrier.
+template <bool BOTH>
+__device__ __forceinline__ void allsum(float& a, float& b, float2 (*scratch)[16], int& turn) {
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off), b += __shfl_xor_sync(0xffffffffu, b, off);
-  const int warps = blockDim.x / 32;
-  if (warps > 1) {  // two rows of scratch in turn: a barrier a sum
-    if (threadIdx.x % 32 == 0) scratch[turn][threadIdx.x / 32] = make_float2(a, b);
+  for (int off = 16; off >= 1; off >>= 1) {
+    if (BOTH) a += __shfl_xor_sync(0xffffffffu, a, off);
+    b += __shfl_xor_sync(0xffffffffu, b, off);
+  }
+  const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
+  if (warps > 1) {
+    if (lane == 0) scratch[turn][threadIdx.x / 32] = make_float2(a, b);
     __syncthreads();
-    a = b = 0.f;
-    for (int w = 0; w < warps; ++w) {
-      const float2 v = scratch[turn][w];
-      a += v.x, b += v.y;
+    const float2 v = scratch[turn][lane % 16];
+    a = lane % 16 < warps ? v.x : 0.f, b = lane % 16 < warps ? v.y : 0.f;
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) {
+      if (BOTH) a += __shfl_xor_sync(0xffffffffu, a, off);
+      b += __shfl_xor_sync(0xffffffffu, b, off);
     }
     turn ^= 1;
   }
 }
+__device__ __forceinline__ void allsum2(float& a, float& b, float2 (*scratch)[16], int& turn) { allsum<true>(a, b, scratch, turn); }
 
 enum Gate { kNone = 0, kChannel = 1, kSequence = 2, kToken = 3 };
 
@@ -141,7 +149,7 @@ __device__ __forceinline__ void row_stats(const float (&f)[MC][V], int n, float 
 #pragma unroll
       for (int k = 0; k < V; ++k) t += (int)(c * blockDim.x + threadIdx.x) < n ? f[c][k] : 0.f;
     }
-    allsum2(t, q, scratch, turn);
+    allsum<false>(q, t, scratch, turn);
     mean = t * inv, q = 0.f;
   }
 #pragma unroll
@@ -154,7 +162,7 @@ __device__ __forceinline__ void row_stats(const float (&f)[MC][V], int n, float 
     }
   }
   t = 0.f;
-  allsum2(q, t, scratch, turn);
+  allsum<false>(t, q, scratch, turn);
   rstd = rsqrtf(q * inv + eps);
 }
 
@@ -619,7 +627,8 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1) block_norm_bw
       }
     }
     float sum0 = sum4(sum), sum1 = sum4(dot);
-    allsum2(sum0, sum1, scratch, turn);
+    if (rms) allsum<false>(sum0, sum1, scratch, turn);
+    else allsum<true>(sum0, sum1, scratch, turn);
     const Quad k2 = quad(-now.w * sum0 * inv), e2 = quad(-sum1 * inv);  // -s2 mean g, -mean(g h)
     sum = dot = quad(0.f);
 #pragma unroll
@@ -643,7 +652,8 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1) block_norm_bw
       }
     }
     sum0 = sum4(sum), sum1 = sum4(dot);
-    allsum2(sum0, sum1, scratch, turn);
+    if (rms) allsum<false>(sum0, sum1, scratch, turn);
+    else allsum<true>(sum0, sum1, scratch, turn);
     const Quad k1 = quad(-now.y * sum0 * inv), e1 = quad(-sum1 * inv);
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
@@ -685,8 +695,8 @@ struct FoldArgs {
   int per, runs, unit, units;  // rows of a run; runs; rows that share a gate, how often
   int dim, param_dtype, gate_dtype;
 };
-__global__ void __launch_bounds__(1024) block_norm_fold_kernel(const __grid_constant__ FoldArgs f) {
-  __shared__ float sums[32][32];
+__global__ void __launch_bounds__(256) block_norm_fold_kernel(const __grid_constant__ FoldArgs f) {
+  __shared__ float sums[8][32];
   const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
   const int col = blockIdx.x * 32 + lane;
   for (int what = blockIdx.y; what < 4 + f.units; what += gridDim.y) {
@@ -699,8 +709,8 @@ __global__ void __launch_bounds__(1024) block_norm_fold_kernel(const __grid_cons
     }
     float t = 0.f;
     if (here && col < f.dim) {
-#pragma unroll 4
-      for (int r = from + slice; r < to; r += 32) {
+#pragma unroll 8
+      for (int r = from + slice; r < to; r += 8) {
         const int slot = what < 4 ? what : begin < r * f.per ? 4 : 5;
         t += f.partial[((int64_t)r * kSlots + slot) * f.dim + col];
       }
@@ -710,7 +720,7 @@ __global__ void __launch_bounds__(1024) block_norm_fold_kernel(const __grid_cons
     __syncthreads();
     if (here && slice == 0 && col < f.dim) {
 #pragma unroll
-      for (int w = 1; w < 32; ++w) t += sums[w][lane];
+      for (int w = 1; w < 8; ++w) t += sums[w][lane];
       if (what == 0) store_dyn(f.dpost_weight, col, f.param_dtype, t);
       else if (what == 1) store_dyn(f.dweight, col, f.param_dtype, t);
       else if (what == 2) store_dyn(f.dpost_bias, col, f.param_dtype, t);
@@ -807,7 +817,7 @@ int launch_bwd2(const ssm_block_norm_bwd_args& g, cudaStream_t st) {
   FoldArgs f{};
   f.partial = g.partial, f.dpost_weight = g.dpost_weight, f.dweight = g.dweight, f.dpost_bias = g.dpost_bias, f.dbias = g.dbias, f.dgate = g.dgate;
   f.per = b.per, f.runs = runs, f.dim = a.dim, f.param_dtype = a.param_dtype, f.gate_dtype = a.gate_dtype, f.unit = b.unit, f.units = GATE == 1 ? b.rows / b.unit : 0;
-  block_norm_fold_kernel<<<dim3((a.dim + 31) / 32, std::min(4 + f.units, 1024)), 1024, 0, st>>>(f);
+  block_norm_fold_kernel<<<dim3((a.dim + 31) / 32, std::min(4 + f.units, 1024)), 256, 0, st>>>(f);
   return launch_status("block_norm_fold_kernel");
 }
 template <int V, int THREADS, int MC, int TYPES>

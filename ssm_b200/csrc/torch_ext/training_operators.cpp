@@ -13,6 +13,13 @@ namespace {
 
 namespace py = pybind11;
 
+// the tensor itself where it hangs in no graph (a view takes longer than the look), dense
+Tensor dense(const Tensor& t) {
+  const Tensor d = torch::autograd::impl::get_autograd_meta(t) ? t.detach() : t;
+  return d.is_contiguous() ? d : d.contiguous();
+}
+OptTensor dense(const OptTensor& t) { return t.has_value() ? OptTensor(dense(*t)) : OptTensor(); }
+
 // ---------------------------------------------------------------------------------------------
 // the norms after and before a block
 // ---------------------------------------------------------------------------------------------
@@ -59,10 +66,9 @@ struct BlockNormCall final : Call {
     if (b_.has_value()) dtype_code(*b_, "fused_block_norm bias");
     if (gate_.has_value()) dtype_code(*gate_, "fused_block_norm gate");
     input(x_), input(res_), input(pw_), input(w_), input(pb_), input(b_), input(gate_);
-    auto dense = [](const OptTensor& t) { return t.has_value() ? OptTensor(t->detach().contiguous()) : OptTensor(); };
-    x = x_.detach().contiguous(), res = dense(res_), gate = dense(gate_);
+    x = dense(x_), res = dense(res_), gate = dense(gate_);
     // the parameters go in as they are where they share a type
-    if (t_pw == t_w && (!pb_.has_value() || t_pb == t_w) && (!b_.has_value() || t_b == t_w)) pw = pw_.detach().contiguous(), w = w_.detach().contiguous(), pb = dense(pb_), b = dense(b_);
+    if (t_pw == t_w && (!pb_.has_value() || t_pb == t_w) && (!b_.has_value() || t_b == t_w)) pw = dense(pw_), w = dense(w_), pb = dense(pb_), b = dense(b_);
     else pw = f32c(pw_), w = f32c(w_), pb = f32c(pb_), b = f32c(b_);
     has_pb = pb.has_value(), has_b = b.has_value();
     if (has_pb != has_b) (has_pb ? b : pb) = at::zeros(w.sizes(), w.options());  // the kernels take both or neither
