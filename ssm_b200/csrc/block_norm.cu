@@ -803,7 +803,7 @@ int launch_bwd2(const ssm_block_norm_bwd_args& g, cudaStream_t st) {
   int device = 0;
   cudaGetDevice(&device);
   if (known.device != device || known.threads != threads || known.smem != smem) {
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512);  // the same for all calls, whichever thread makes them
     int fit = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, threads, smem) != cudaSuccess || fit < 1) cudaGetLastError(), fit = 1;
     known = Known{device, threads, smem, fit * sm_count()};
@@ -847,7 +847,7 @@ int dispatch_bwd(const ssm_block_norm_bwd_args& g, bool wide, cudaStream_t st) {
 int check(const ssm_block_norm_args& a) {
   SSM_REQUIRE(a.rows >= 0 && a.dim >= 1 && a.len >= 1, SSM_ERR_SHAPE, "fused_block_norm: bad shape");
   SSM_REQUIRE(a.dim <= kMaxDim, SSM_ERR_TOO_LARGE, "fused_block_norm: more than 8192 columns");
-  SSM_REQUIRE(a.rows < ((int64_t)1 << 31), SSM_ERR_TOO_LARGE, "fused_block_norm: 2^31 rows or more");
+  SSM_REQUIRE(a.rows < ((int64_t)1 << 30), SSM_ERR_TOO_LARGE, "fused_block_norm: 2^30 rows or more");
   SSM_REQUIRE(valid_dtype(a.io_dtype) && valid_dtype(a.res_dtype) && valid_dtype(a.resout_dtype) && valid_dtype(a.param_dtype) && valid_dtype(a.gate_dtype), SSM_ERR_DTYPE,
               "fused_block_norm: unknown dtype");
   SSM_REQUIRE(a.gate_kind >= kNone && a.gate_kind <= kToken && (a.gate_kind != kSequence || a.rows % a.len == 0), SSM_ERR_SHAPE, "fused_block_norm: bad gate");

@@ -33,7 +33,7 @@ constexpr int kTile = 256, kK = 64, kStages = 6, kThreads = 384, kEpilogueWarps 
 constexpr int kBoxBytes = 64 * kK * 2, kStageBytes = 4 * kBoxBytes;
 constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
 constexpr int kStatus = 128;           // status of a wait that ran out
-constexpr float kFar = 268435456.f;    // M of a tile is no less than minus this
+constexpr float kFar = 268435456.f;    // 2^28: M of a tile is no less than minus this; rows whose M reaches twice that give NaN (their logits' steps are larger than any difference that matters)
 constexpr int kPairs = 6;
 __constant__ const signed char kPlaneA[kPairs] = {2, 0, 1, 1, 0, 0}, kPlaneB[kPairs] = {0, 2, 1, 0, 1, 0};
 
@@ -51,7 +51,7 @@ struct Job {
   float* out;                  // kOut: [split][row][ld]
   int64_t ld, out_split;
   int out_rows, add;
-  int last;                    // the last piece of dW: 1 rounded into its place, with the targets' part; 2 added to the sums, with it
+  int last;                    // the last piece of dW: rounded into its place
 };
 struct GemmArgs {
   Job job[2];                  // kOut takes two; no tiles: none
@@ -69,7 +69,7 @@ struct GemmArgs {
   uint16_t* g;                 // [plane][row][ldg]
   int64_t ldg, g_plane;
   const int* again;            // kKeep, nullable: the tiles of rows to be formed again
-  // kOut, the last piece of dW: dw = (sums + the target's row) scales[1]
+  // kOut, dW: the targets' rows, and for the last piece dw = sums scales[1]
   void* dw;
   int64_t dw_ld;
   int dw_dtype, dw_wide, dim;
@@ -406,8 +406,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tmem_ld32_issue(from + c, v);
             tmem_wait_ld();
           }
-          if (j.last && row < j.out_rows) add_target(g, j, row, out_col + c, v);
-          if (j.last == 1 && row < j.out_rows) {
+          if (p.job && row < j.out_rows) add_target(g, j, row, out_col + c, v);
+          if (j.last && row < j.out_rows) {
             last_columns(g, j, add, row, out_col + c, v);
           } else if (row < j.out_rows) {
 #pragma unroll
@@ -483,14 +483,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         } else if constexpr (EPI == kOut) {
           float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
           const int cols = (int)min((int64_t)width, j.ld - out_col);
-          if (row < j.out_rows && j.last) {  // fp32 is not formed in one pass
+          if (p.job && row < j.out_rows) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (32 * c < width) {
-                add_target(g, j, row, out_col + 32 * c, v[c]);
-                last_columns(g, j, add, row, out_col + 32 * c, v[c]);
-              }
-            }
+            for (int c = 0; c < 4; ++c)
+              if (32 * c < width) add_target(g, j, row, out_col + 32 * c, v[c]);
+          }
+          if (row < j.out_rows && j.last) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (32 * c < width) last_columns(g, j, add, row, out_col + 32 * c, v[c]);
           } else if (row < j.out_rows) {
 #pragma unroll
             for (int i = 0; i < 128; i += 4) {
@@ -774,6 +775,8 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* __restric
   }
 }
 
+__device__ __forceinline__ float within_reach(float M) { return fabsf(M) < 2.f * kFar ? 0.f : NAN; }
+
 // The tiles of a row joined: 32 rows of a call to a block, 32 slices of the columns (7 rows, 394 tiles: 21 us with eight slices).
 __global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
                                                    const int* __restrict__ targets, const float* __restrict__ z_target, float4* __restrict__ stats, float* __restrict__ row_loss,
@@ -804,7 +807,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ p
       M = top;
     }
     const int r = row0 + row, t = targets[r], out = idx[r];
-    const float ln_s = logf(s), z = t < 0 ? NAN : z_target[r];
+    const float ln_s = logf(s) + within_reach(M), z = (t < 0 ? NAN : z_target[r]) + within_reach(M);
     stats[r] = make_float4(M, s, z, 0.f);
     row_loss[out] = ln_s - kLn2 * fmaf(z, kLog2e, -M);  // log Z - z_t as differences from M, which take no bits from a small loss
     log_z[out] = fmaf(M, kLn2, ln_s);
@@ -841,7 +844,7 @@ __global__ void __launch_bounds__(256) few_join_kernel(const float2* __restrict_
   if (tid == 0) {
     for (int w = 1; w < 8; ++w) add(warps[w]);
     const int t = targets[r], out = idx[r];
-    const float ln_s = logf(s), z = t < 0 ? NAN : z_target[r];
+    const float ln_s = logf(s) + within_reach(M), z = (t < 0 ? NAN : z_target[r]) + within_reach(M);
     stats[r] = make_float4(M, s, z, 0.f);
     row_loss[out] = ln_s - kLn2 * fmaf(z, kLog2e, -M);
     log_z[out] = fmaf(M, kLn2, ln_s);
@@ -906,8 +909,8 @@ __global__ void __launch_bounds__(1024) join_keep_kernel(const float2* __restric
       row[r] = make_float4(top, 0.f, 0.f, 0.f);
       return;
     }
-    const float d = fmaf(z, kLog2e, -v.x), inv = s < INFINITY ? 1.f / s : NAN, ln_s = s < INFINITY ? logf(s) : NAN;
-    const float bad = z != z ? NAN : 0.f;  // a target outside of the vocabulary, or a NaN
+    const float d = fmaf(z, kLog2e, -v.x), inv = s < INFINITY ? 1.f / s : NAN, ln_s = (s < INFINITY ? logf(s) : NAN) + within_reach(v.x);
+    const float bad = (z != z ? NAN : 0.f) + within_reach(v.x);  // a target outside of the vocabulary, or a NaN
     v.y = inv + bad, v.z = 1.f, v.w = ex2_approx(d) * inv - 1.f;
     row[r] = v;
     row_loss[out] = ln_s - kLn2 * d;
@@ -1041,20 +1044,20 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ 
   }
 }
 
-// Packed rows [8192 b, ..) in the order of their targets: keys (target, packed row), all ones behind them.  A block each; eight keys to a thread, compared in registers, by shuffles
+// A call's packed rows [8192 b, ..) in the order of their targets: keys (target, packed row), all ones behind them.  A block each; eight keys to a thread, compared in registers, by shuffles
 // within a warp and through shared memory beyond (8192 keys all through shared memory: 97 us).  Key: uint32_t where target and place fit.
 constexpr int kSort = 8192;
 template <typename Key>
 __device__ __forceinline__ Key shuffled(Key v, int lanes) { return __shfl_xor_sync(0xffffffffu, v, lanes); }
 template <typename Key>
-__global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targets, const int* __restrict__ count, int size, uint64_t* __restrict__ keys) {
+__global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targets, const int* __restrict__ count, int row0, int rows, int size, uint64_t* __restrict__ keys) {
   extern __shared__ __align__(8) unsigned char sort_raw[];
   Key* const other = reinterpret_cast<Key*>(sort_raw);
-  const int first = blockIdx.x * kSort, n = *count, tid = threadIdx.x, threads = blockDim.x;
+  const int first = blockIdx.x * kSort, n = min(rows, *count - row0), tid = threadIdx.x, threads = blockDim.x;
   Key key[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int i = tid * 8 + e, r = first + i, t = i < size && r < n ? targets[r] : -1;
+    const int i = tid * 8 + e, r = first + i, t = i < size && r < n ? targets[row0 + r] : -1;
     key[e] = t >= 0 ? (Key)t << 13 | (Key)i : ~(Key)0;
   }
   auto ordered = [](Key& a, Key& b, bool up) {  // a <= b where up
@@ -1103,7 +1106,7 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targ
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    if (tid * 8 + e < size) keys[first + tid * 8 + e] = key[e] == ~(Key)0 ? ~0ull : (uint64_t)(key[e] >> 13) << 32 | (uint32_t)(first + (int)(key[e] & (kSort - 1)));
+    if (tid * 8 + e < size) keys[first + tid * 8 + e] = key[e] == ~(Key)0 ? ~0ull : (uint64_t)(key[e] >> 13) << 32 | (uint32_t)(row0 + first + (int)(key[e] & (kSort - 1)));
 }
 // The sum of q h over the rows that have a target, in their order, at the place of the first of them, and that place by target: one block (of 128 V columns) for each run of equal
 // targets, eight rows on their way at a time (a common token has hundreds).
@@ -1217,7 +1220,7 @@ struct Plan {
   // offsets: what both passes use (kept between them), then scratch
   int64_t idx, packed, count, h, w, kept, scales, part, z, row, g, dh, dw, keys, heads, sums, again, hs, bytes;
 };
-constexpr int64_t kForwardRows = 16384;
+constexpr int64_t kPieceRows = 16384;  // at most, so that what a piece needs beside the logits' gradient has a bound
 
 Plan plan_of(const ssm_linear_ce_args& a, int pass) {
   Plan p{};
@@ -1229,12 +1232,12 @@ Plan plan_of(const ssm_linear_ce_args& a, int pass) {
   p.pairs = std::max(1, sm_count() / 2);
   p.bn = p.dim <= 128 ? 128 : 256;
   p.splits = 1, p.sort = 1;
-  while (p.sort < kSort && p.sort < p.rows) p.sort *= 2;
-  p.sorts = (int)((p.rows + kSort - 1) / kSort);
-  p.piece = std::min<int64_t>(up(p.rows, kTile), kForwardRows);
+  p.piece = std::min<int64_t>(up(p.rows, kTile), kPieceRows);
   if (pass != kForward) {
-    const int64_t fit = std::max<int64_t>(1, SSM_LINEAR_CE_PIECE_BYTES / (p.ldg * 2 * p.planes) / kTile) * kTile, n = (p.rows + fit - 1) / fit;
+    const int64_t fit = std::min(kPieceRows, std::max<int64_t>(1, SSM_LINEAR_CE_PIECE_BYTES / (p.ldg * 2 * p.planes) / kTile) * kTile), n = (p.rows + fit - 1) / fit;
     p.piece = up((p.rows + n - 1) / n, kTile);  // pieces of one size
+    while (p.sort < kSort && p.sort < std::min(p.piece, p.rows)) p.sort *= 2;
+    p.sorts = (int)((p.piece + kSort - 1) / kSort);
     // Splits of the vocabulary for dh: the pairs share its tiles and those of dW, which fill up where dh's do not come out even, as long as none of dh's takes longer than all of
     // a pair's share.  A split costs its partial sums' way through memory, 0.3 blocks of K a tile.
     const double t0 = (double)(p.piece / kTile) * (double)((p.dim + p.bn - 1) / p.bn), kb0 = (double)((p.vocab + kK - 1) / kK);
@@ -1364,16 +1367,16 @@ int zero(void* p, size_t bytes, cudaStream_t st, int byte = 0) {
   set_error("linear_cross_entropy: %s", cudaGetErrorString(e));
   return (int)e;
 }
-// the targets' part of dW, by target
-int target_rows(const Run& r) {
+// the part of a piece's targets in dW, by target
+int target_rows(const Run& r, int64_t row0, int64_t rows) {
   const Plan& p = r.p;
   uint64_t* keys = r.at<uint64_t>(p.keys);
   const unsigned threads = (unsigned)std::max(32, p.sort / 8);
   if (p.vocab < 1 << 19) {
-    sort_kernel<uint32_t><<<p.sorts, threads, threads * 32, r.st>>>(r.packed(), r.count(), p.sort, keys);
+    sort_kernel<uint32_t><<<p.sorts, threads, threads * 32, r.st>>>(r.packed(), r.count(), (int)row0, (int)rows, p.sort, keys);
   } else {
     cudaFuncSetAttribute(sort_kernel<uint64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
-    sort_kernel<uint64_t><<<p.sorts, threads, threads * 64, r.st>>>(r.packed(), r.count(), p.sort, keys);
+    sort_kernel<uint64_t><<<p.sorts, threads, threads * 64, r.st>>>(r.packed(), r.count(), (int)row0, (int)rows, p.sort, keys);
   }
   if (const int rc = launch_status("linear_ce sort_kernel")) return rc;
   if (const int rc = zero(r.at<void>(p.heads), (size_t)p.sorts * p.vocab * 4, r.st, 0xff)) return rc;
@@ -1408,12 +1411,10 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
   }
   if (dw) {
     b.m_tiles = (int)((p.vocab + kTile - 1) / kTile), b.n_tiles = d_tiles, b.a_mn = b.b_mn = 1, b.k_is_rows = 1, b.b_k0 = (int)row0;
-    b.out = dw->sums, b.ld = p.ldo, b.out_rows = (int)p.vocab, b.add = row0 > 0, b.last = row0 + rows < p.rows ? 0 : dw->out == dw->sums ? 2 : 1;
-    if (b.last) {
-      if (const int rc = target_rows(r)) return rc;
-      g.dw = dw->out, g.dw_ld = dw->ld, g.dw_dtype = dw->dtype, g.dw_wide = dw->ld % (dw->dtype == SSM_F32 ? 4 : 8) == 0 && aligned_to(dw->out, 16), g.dim = (int)p.dim;
-      g.scales = r.at<float>(p.scales), g.heads = r.at<int>(p.heads), g.sorts = p.sorts, g.target_sums = r.at<float>(p.sums);
-    }
+    b.out = dw->sums, b.ld = p.ldo, b.out_rows = (int)p.vocab, b.add = row0 > 0, b.last = row0 + rows >= p.rows && dw->out != dw->sums;
+    if (const int rc = target_rows(r, row0, rows)) return rc;
+    g.dw = dw->out, g.dw_ld = dw->ld, g.dw_dtype = dw->dtype, g.dw_wide = dw->ld % (dw->dtype == SSM_F32 ? 4 : 8) == 0 && aligned_to(dw->out, 16), g.dim = (int)p.dim;
+    g.scales = r.at<float>(p.scales), g.heads = r.at<int>(p.heads), g.sorts = p.sorts, g.target_sums = r.at<float>(p.sums);
   }
   if (const int rc = gemm_of<kOut>(p, r.mg, r.mw, h2, g, r.st)) return rc;
   if (!dh) return SSM_OK;

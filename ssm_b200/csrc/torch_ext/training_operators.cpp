@@ -39,7 +39,7 @@ struct BlockNormCall final : Call {
     SSM_ARG(x_.dim() == 3, "x must have shape (B, L, D).");
     dim = x_.size(2), len = x_.size(1), rows = x_.size(0) * x_.size(1);
     SSM_ARG(dim >= 1 && dim <= 8192, "fused_block_norm: D lies between 1 and 8192.");
-    SSM_ARG(rows < ((int64_t)1 << 31), "fused_block_norm: too many rows.");
+    SSM_ARG(rows < ((int64_t)1 << 30), "fused_block_norm: too many rows.");
     auto param = [&](const Tensor& t, const char* name) { SSM_ARG(t.dim() == 1 && t.size(0) == dim, name, " must have shape (D,)."); };
     param(pw_, "post_weight"), param(w_, "weight");
     if (pb_.has_value()) param(*pb_, "post_bias"), t_pb = pb_->scalar_type();

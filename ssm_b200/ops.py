@@ -892,9 +892,9 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore
     have their types; ``weight`` is read in ``hidden``'s type.
 
     A position whose target is ``ignore_index`` gives 0 (``log_z`` too) and no gradient, is not computed, and may hold anything.  Any other target outside of the vocabulary
-    makes its loss and the gradients NaN, as a hidden state that is not finite does.
+    makes its loss and the gradients NaN, as a hidden state that is not finite does, and logits of ``2**28`` and more.
 
-    Neither pass holds the logits; in 16 bits at most 512 MB of their gradient at a time.  For a sum or mean in bf16 without ``return_log_z`` the gradients are formed along with the
+    Neither pass holds the logits; in 16 bits at most 512 MB of their gradient (and 16384 rows) at a time.  For a sum or mean in bf16 without ``return_log_z`` the gradients are formed along with the
     loss, and held in fp32 until the backward pass scales them (``torch.no_grad()`` forms the loss alone); otherwise the backward pass forms the logits again.
 
     16-bit operands are multiplied as they are; the gradient with respect to the logits is rounded to their type before its two products, but for the targets' own, which keep 32 bits.

@@ -400,3 +400,31 @@ def test_odd_widths_of_every_type_of_weight(wt, d):
     val, tol = bounds(h, w.to(torch.bfloat16), t, wl, 0 * wz)[3]
     near(torch.autograd.grad(ops.linear_cross_entropy(h, w, t), w, wl)[0], val, tol + half(wt) * val.abs(), "dw")
     one_pass(h.detach(), w.detach().to(torch.bfloat16), t)
+
+
+@pytest.mark.parametrize("scale", [1e5, 1e7, 1e9])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_very_large_logits(scale, dtype):
+    """The products' rounding is all that counts then: the loss is the largest logit's distance, to 2^-18 of the sums of the products' sizes; from 2^28 on NaN."""
+    h, w, t, wl, _ = make(100, 64, 300, dtype)
+    h = (h.float() * scale).to(dtype).requires_grad_(True)
+    w.requires_grad_(True)
+    z = h.detach().double() @ w.detach().double().t()
+    kept = t != -100
+    want = (torch.logsumexp(z, -1) - torch.gather(z, 1, t.clamp(min=0)[:, None])[:, 0]) * kept
+    far = z.abs().amax(-1) * 1.4427 > 2.0 ** 28
+    for reduction in ("none", "sum"):
+        loss = ops.linear_cross_entropy(h, w, t, reduction=reduction)
+        dh, dw = torch.autograd.grad(loss, [h, w], torch.ones_like(loss))
+        if reduction == "none":
+            tol = 2.0 ** -18 * (h.detach().double().abs() @ w.detach().double().abs().t()).amax(-1)
+            ok = kept & ~far
+            assert ((loss.detach().double() - want).abs()[ok] <= tol[ok]).all()
+            assert (loss.isnan() | (loss.detach().double() - want).abs().le(tol)).all() and not dh[~kept].any()
+        if not far.any():
+            assert dh.isfinite().all() and dw.isfinite().all() and loss.isfinite().all()
+
+
+def test_a_long_batch_in_many_pieces():
+    check(*make(40000, 24, 200, torch.bfloat16))
+    one_pass(*make(40000, 24, 200, torch.bfloat16)[:3])
