@@ -29,8 +29,9 @@
 namespace ssmb {
 namespace {
 
-constexpr int kTile = 256, kK = 64, kThreads = 384, kEpilogueWarps = 8;
-constexpr int kBoxBytes = 64 * kK * 2;
+constexpr int kTile = 256, kK = 64, kStages = 6, kThreads = 384, kEpilogueWarps = 8;
+constexpr int kBoxBytes = 64 * kK * 2, kStageBytes = 4 * kBoxBytes;
+constexpr int kSmem = kStages * kStageBytes + 1024;
 constexpr int kStatus = 128;           // status of a wait that ran out
 constexpr float kFar = 268435456.f;    // 2^28: M of a tile is no less than minus this; rows whose M reaches twice that give NaN (their logits' steps are larger than any difference that matters)
 constexpr int kPairs = 6;
@@ -38,9 +39,6 @@ __constant__ const signed char kPlaneA[kPairs] = {2, 0, 1, 1, 0, 0}, kPlaneB[kPa
 
 enum Epilogue { kStats = 0, kGrad = 1, kOut = 2, kKeep = 3, kFew = 4 };  // kFew: kStats with the weight's rows as M
 constexpr int kFewRows = 64;           // up to which rows it is taken
-__host__ __device__ constexpr int stages_of(int epi) { return epi == kFew ? 10 : 6; }
-__host__ __device__ constexpr int stage_bytes(int epi) { return 2 * kBoxBytes + (epi == kFew ? kFewRows / 2 * kK * 2 : 2 * kBoxBytes); }
-__host__ __device__ constexpr int smem_of(int epi) { return stages_of(epi) * stage_bytes(epi) + 1024; }
 constexpr float kReach = 60.f;         // how far a row's maximum may be from the M of the one-pass form
 
 // one product: M x N in tiles, K in blocks of 64, cut into `splits`
@@ -212,7 +210,6 @@ __device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bo
 template <int EPI, typename T, int PLANES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mb1, const __grid_constant__ GemmArgs g) {
-  constexpr int kStages = stages_of(EPI), kStageBytes = stage_bytes(EPI);
   // Blocks of K between two readings of an accumulator; the logits' gradient in 16 bits asks for no more than the tensor core's own sums (1999 rows of 1024: 180 us with segments)
   constexpr int kSegment = EPI == kGrad && PLANES == 1 ? 1 << 20 : 8;
   extern __shared__ unsigned char raw[];
@@ -1288,10 +1285,10 @@ int check(const ssm_linear_ce_args& a) {
 template <int EPI, typename T, int PLANES>
 int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb1, const GemmArgs& g, int pairs, cudaStream_t st) {
   auto kern = gemm_kernel<EPI, T, PLANES>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(EPI));
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   int64_t tiles = 0;
   for (const Job& j : g.job) tiles += (int64_t)j.m_tiles * j.n_tiles * j.splits;
-  kern<<<(unsigned)(2 * std::max<int64_t>(1, std::min<int64_t>(tiles, pairs))), kThreads, smem_of(EPI), st>>>(ma, mb, mb1, g);
+  kern<<<(unsigned)(2 * std::max<int64_t>(1, std::min<int64_t>(tiles, pairs))), kThreads, kSmem, st>>>(ma, mb, mb1, g);
   return launch_status("linear_ce gemm_kernel");
 }
 template <int EPI>

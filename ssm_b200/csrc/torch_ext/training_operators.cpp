@@ -162,6 +162,9 @@ struct LinearCeCall final : Call {
     targets = targets_.detach().to(at::kLong).contiguous();
   }
   int64_t rows() const { return targets.numel(); }
+  // A sum or mean is multiplied by one number, which may come later: in bf16 loss and gradients are formed in one pass, 6 N D V operations instead of 8
+  bool one_pass() const { return reduction && !want_z && h.scalar_type() == at::kBFloat16 && rows() > 0 && (grad_h || grad_w); }
+  bool reads(size_t i) const override { return i < 2 && !one_pass(); }  // the targets' part is packed in the first pass
   at::TensorOptions f32() const { return h.options().dtype(at::kFloat).requires_grad(false); }
   void fill(ssm_linear_ce_args& a) const {
     a.rows = rows(), a.hidden_stride = rows() > 1 ? h.stride(0) : h.size(1), a.weight_stride = w.size(0) > 1 ? w.stride(0) : w.size(1), a.ignore_index = ignore;
@@ -179,8 +182,7 @@ struct LinearCeCall final : Call {
     c10::cuda::CUDAGuard guard(h.device());
     ssd_poll(h.get_device());  // a wait that ran out in an earlier launch surfaces here, without a synchronisation
     Tensor row_loss = at::empty(lead_shape, f32()), log_z = at::empty(lead_shape, f32()), loss;
-    // A sum or mean is multiplied by one number, which may come later: in bf16 loss and gradients are formed in one pass, 6 N D V operations instead of 8
-    const bool both = train && reduction && !want_z && h.scalar_type() == at::kBFloat16 && rows() > 0 && (grad_h || grad_w);
+    const bool both = train && one_pass();
     if (train && !both) stats = at::empty({std::max<int64_t>(rows(), 1), 4}, f32());
     ssm_linear_ce_args a{};
     fill(a);

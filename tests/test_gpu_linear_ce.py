@@ -372,6 +372,15 @@ def test_an_edit_between_the_passes_and_second_derivatives_are_errors():
     w.mul_(2)
     with pytest.raises(RuntimeError, match="modified in place"):
         loss.sum().backward()
+    # what is not read again may be edited: targets, and everything where the gradients came with the loss
+    for reduction in ("none", "mean"):
+        want = torch.autograd.grad(ops.linear_cross_entropy(h, w, t, reduction=reduction).sum(), h)[0]
+        t2, w2 = t.clone(), w.clone()
+        loss = ops.linear_cross_entropy(h, w2, t2, reduction=reduction)
+        t2.fill_(3)
+        if reduction == "mean":
+            w2.zero_()
+        assert torch.equal(torch.autograd.grad(loss.sum(), h)[0], want)
     g = torch.autograd.grad(ops.linear_cross_entropy(h, w, t).sum(), h, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="differentiable once"):
         g.sum().backward()

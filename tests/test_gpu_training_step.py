@@ -100,3 +100,23 @@ def test_a_step_in_a_graph_repeats_the_eager_one():
         graph.replay()
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+def test_traced_calls_are_made_again():
+    from ssm_b200 import ops
+
+    def f(x, res, w, head, t):
+        y, r = ops.fused_block_norm(x, res, w, w, gate=w, residual_scale=0.5)
+        return ops.linear_cross_entropy(y, head, t, reduction="mean"), r
+
+    def inputs(seed):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        rn = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+        return rn(2, 9, 64).bfloat16(), rn(2, 9, 64), rn(64).bfloat16(), rn(100, 64).bfloat16(), torch.randint(0, 100, (2, 9), device="cuda", generator=gen)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(f, inputs(0), check_trace=False)
+        for a, b in zip(traced(*inputs(1)), f(*inputs(1))):
+            assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="not traced"):
+            torch.jit.trace(lambda x: ops.global_norm([x]), (inputs(0)[0],), check_trace=False)
