@@ -695,10 +695,12 @@ struct FoldArgs {
   int per, runs, unit, units;  // rows of a run; runs; rows that share a gate, how often
   int dim, param_dtype, gate_dtype;
 };
-__global__ void __launch_bounds__(256) block_norm_fold_kernel(const __grid_constant__ FoldArgs f) {
-  __shared__ float sums[8][32];
+// 32 pieces of V columns to a block, 32 slices of the runs (293 runs of 2560 columns, in the L2: 6.6 us; element by element 15, with eight slices 13)
+template <int V>
+__global__ void __launch_bounds__(1024) block_norm_fold_kernel(const __grid_constant__ FoldArgs f) {
+  __shared__ float sums[V][32][33];
   const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
-  const int col = blockIdx.x * 32 + lane;
+  const int col = (blockIdx.x * 32 + lane) * V;
   for (int what = blockIdx.y; what < 4 + f.units; what += gridDim.y) {
     int from = 0, to = f.runs, begin = 0;
     bool here = what < 2 || (what == 2 && f.dpost_bias) || (what == 3 && f.dbias);
@@ -707,25 +709,35 @@ __global__ void __launch_bounds__(256) block_norm_fold_kernel(const __grid_const
       from = begin / f.per, to = (begin + f.unit - 1) / f.per + 1;
       here = to - from > 1;  // else written by its run
     }
-    float t = 0.f;
-    if (here && col < f.dim) {
-#pragma unroll 8
-      for (int r = from + slice; r < to; r += 8) {
+    if (!here) continue;  // the whole block
+    float t[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) t[k] = 0.f;
+    if (col < f.dim) {
+#pragma unroll 4
+      for (int r = from + slice; r < to; r += 32) {
         const int slot = what < 4 ? what : begin < r * f.per ? 4 : 5;
-        t += f.partial[((int64_t)r * kSlots + slot) * f.dim + col];
+        float v[V];
+        load_vec<V>(f.partial, ((int64_t)r * kSlots + slot) * f.dim + col, SSM_F32, v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) t[k] += v[k];
       }
     }
     __syncthreads();
-    sums[slice][lane] = t;
-    __syncthreads();
-    if (here && slice == 0 && col < f.dim) {
 #pragma unroll
-      for (int w = 1; w < 8; ++w) t += sums[w][lane];
-      if (what == 0) store_dyn(f.dpost_weight, col, f.param_dtype, t);
-      else if (what == 1) store_dyn(f.dweight, col, f.param_dtype, t);
-      else if (what == 2) store_dyn(f.dpost_bias, col, f.param_dtype, t);
-      else if (what == 3) store_dyn(f.dbias, col, f.param_dtype, t);
-      else store_dyn(f.dgate, (int64_t)(what - 4) * f.dim + col, f.gate_dtype, t);
+    for (int k = 0; k < V; ++k) sums[k][slice][lane] = t[k];
+    __syncthreads();
+    const int c = (blockIdx.x * 32 + slice) * V;  // a warp has the slices of a piece
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float s = warp_sum(sums[k][lane][slice]);
+      if (lane == 0 && c < f.dim) {
+        if (what == 0) store_dyn(f.dpost_weight, c + k, f.param_dtype, s);
+        else if (what == 1) store_dyn(f.dweight, c + k, f.param_dtype, s);
+        else if (what == 2) store_dyn(f.dpost_bias, c + k, f.param_dtype, s);
+        else if (what == 3) store_dyn(f.dbias, c + k, f.param_dtype, s);
+        else store_dyn(f.dgate, (int64_t)(what - 4) * f.dim + c + k, f.gate_dtype, s);
+      }
     }
   }
 }
@@ -817,7 +829,8 @@ int launch_bwd2(const ssm_block_norm_bwd_args& g, cudaStream_t st) {
   FoldArgs f{};
   f.partial = g.partial, f.dpost_weight = g.dpost_weight, f.dweight = g.dweight, f.dpost_bias = g.dpost_bias, f.dbias = g.dbias, f.dgate = g.dgate;
   f.per = b.per, f.runs = runs, f.dim = a.dim, f.param_dtype = a.param_dtype, f.gate_dtype = a.gate_dtype, f.unit = b.unit, f.units = GATE == 1 ? b.rows / b.unit : 0;
-  block_norm_fold_kernel<<<dim3((a.dim + 31) / 32, std::min(4 + f.units, 1024)), 256, 0, st>>>(f);
+  constexpr int kFold = V == 1 ? 1 : 4;
+  block_norm_fold_kernel<kFold><<<dim3((a.dim + 32 * kFold - 1) / (32 * kFold), std::min(4 + f.units, 1024)), 1024, 0, st>>>(f);
   return launch_status("block_norm_fold_kernel");
 }
 template <int V, int THREADS, int MC, int TYPES>
