@@ -15,6 +15,9 @@
 // Rows that are left out are not computed: the others are packed first, behind one another (which also gives the copies their alignment), and how many
 // there are is known on the device alone, so that every kernel reads it there.
 //
+// Launches overlap: each kernel waits for the one before ahead of its first access (7 rows: 37 -> 29 us, 500 fp32 rows with gradients 257 -> 241), and what it reads is
+// not marked as constant, so that no read moves ahead of the wait.
+//
 // Products: pairs of CTAs (cta_group::2) on tiles of 256 x 256 (x 128 for narrow outputs), a CTA holding 128 rows of the accumulator; operands by TMA in the 128-byte swizzle, blocks of 64 x 64, two to
 // an operand, with K innermost (h, W, G as stored) or M / N innermost (G^T, W and h as the second factor).  One thread copies, one multiplies, eight
 // warps read an accumulator while the next one is formed.  Logits, and all results in fp32, leave the accumulator every 512 terms and are added up by the warps that read it: the tensor core
@@ -220,15 +223,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t ring = (tc::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t full = tc::smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16;
+  constexpr int kProducts = PLANES == 1 ? 1 : kPairs;
+  constexpr bool kSegments = EPI != kOut || PLANES > 1;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) tc::mbar_init(full + 8 * s, 1), tc::mbar_init(empty + 8 * s, 1);
+    for (int b = 0; b < 2; ++b) tc::mbar_init(tfull + 8 * b, 1), tc::mbar_init(tempty + 8 * b, 2 * kEpilogueWarps);
+    gave_up = 0;
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc::smem_u32(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  pdl_wait();  // all above overlaps with the kernel before
+  pdl_trigger();
   int live = min(g.rows, max(0, *g.count - g.row0));
   if (EPI == kKeep && g.again != nullptr) {
     bool any = false;
     for (int i = 0; i < (live + kTile - 1) / kTile; ++i) any = any || g.again[i] != 0;
     if (!any) live = 0;
   }
-  constexpr int kProducts = PLANES == 1 ? 1 : kPairs;
-  constexpr bool kSegments = EPI != kOut || PLANES > 1;
-
   // This pair's k-th tile.  The first job's tiles (long ones) go round the pairs; pairs that have one less of them take as many rounds of the second job's alone as fit into
   // its time, then all take turns: the tiles that run at one time stay neighbours, and share operands in the L2.
   const int m0 = (live + kTile - 1) / kTile, kb_rows = (live + kK - 1) / kK;
@@ -263,21 +283,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (EPI == kKeep && g.again != nullptr && !g.again[p.m]) p.kb1 = p.kb0;  // nothing to do
     return p;
   };
-
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) tc::mbar_init(full + 8 * s, 1), tc::mbar_init(empty + 8 * s, 1);
-    for (int b = 0; b < 2; ++b) tc::mbar_init(tfull + 8 * b, 1), tc::mbar_init(tempty + 8 * b, 2 * kEpilogueWarps);
-    gave_up = 0;
-  }
-  if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc::smem_u32(&tmem_slot)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
-  }
-  tc::fence_before_sync();
-  __syncthreads();
-  cluster_sync();
-  tc::fence_after_sync();
-  const uint32_t tmem = tmem_slot;
 
   auto ran_out = [&]() {
     gave_up = 1;
@@ -619,8 +624,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ---- around the products ------------------------------------------------------------------------------------------------------
 
 // Rows whose target counts, in their order, from the front of idx; the others from its end.  One block.
-__global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ targets, int rows, int64_t ignore, int vocab, int* __restrict__ idx, int* __restrict__ packed, int* __restrict__ count,
+__global__ void __launch_bounds__(1024) rows_kernel(const int64_t* targets, int rows, int64_t ignore, int vocab, int* __restrict__ idx, int* __restrict__ packed, int* __restrict__ count,
                                                     float* __restrict__ row_loss, float* __restrict__ log_z) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ int sums[32];
   __shared__ int base_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -675,6 +682,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ 
 // (rows, dim) at a stride -> planes of 16-bit elements with rows of `ld`; with idx the packed rows, and zeros behind them to the end of their tile.  A warp per row.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stride, int64_t rows, int dim, const int* idx, const int* count, uint16_t* dst, int64_t ld, int64_t plane) {
+  pdl_wait();
+  pdl_trigger();
   const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x & 31;
   if (r >= rows) return;
@@ -723,9 +732,11 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
 
 // Both for up to 64 rows, in one launch
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* __restrict__ targets, int rows, int64_t ignore, int vocab, const void* src, int64_t stride, int dim, int* __restrict__ idx,
+__global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* targets, int rows, int64_t ignore, int vocab, const void* src, int64_t stride, int dim, int* __restrict__ idx,
                                                         int* __restrict__ packed, int* __restrict__ count, float* __restrict__ row_loss, float* __restrict__ log_z, uint16_t* dst, int64_t ld,
                                                         int64_t plane) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ int rows_of[kFewRows];
   __shared__ int kept_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -779,9 +790,11 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* __restric
 __device__ __forceinline__ float within_reach(float M) { return fabsf(M) < 2.f * kFar ? 0.f : NAN; }
 
 // The tiles of a row joined: 32 rows of a call to a block, 32 slices of the columns (7 rows, 394 tiles: 21 us with eight slices).
-__global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
-                                                   const int* __restrict__ targets, const float* __restrict__ z_target, float4* __restrict__ stats, float* __restrict__ row_loss,
+__global__ void __launch_bounds__(1024) join_kernel(const float2* part, int ld, int parts, const int* count, int row0, int rows, const int* idx,
+                                                   const int* targets, const float* z_target, float4* __restrict__ stats, float* __restrict__ row_loss,
                                                    float* __restrict__ log_z) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ float2 slices[32][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   const int live = min(rows, *count - row0);
@@ -816,8 +829,10 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ p
 }
 
 // The tiles of up to 64 rows joined, a block to a row
-__global__ void __launch_bounds__(256) few_join_kernel(const float2* __restrict__ part, int parts, const int* __restrict__ count, const int* __restrict__ idx, const int* __restrict__ targets,
-                                                       const float* __restrict__ z_target, float4* __restrict__ stats, float* __restrict__ row_loss, float* __restrict__ log_z) {
+__global__ void __launch_bounds__(256) few_join_kernel(const float2* part, int parts, const int* count, const int* idx, const int* targets,
+                                                       const float* z_target, float4* __restrict__ stats, float* __restrict__ row_loss, float* __restrict__ log_z) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ float2 warps[8];
   const int r = blockIdx.x, tid = threadIdx.x;
   if (r >= *count) return;
@@ -853,8 +868,10 @@ __global__ void __launch_bounds__(256) few_join_kernel(const float2* __restrict_
 }
 
 // ---- loss and gradient in one pass: the target's logit of packed rows, which M comes from
-__global__ void __launch_bounds__(256) reference_kernel(const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w, int64_t ldh, int64_t ldw, int dim, const int* __restrict__ targets,
-                                                        const int* __restrict__ count, int row0, int rows, float* __restrict__ z_target, float4* __restrict__ row, int* __restrict__ again) {
+__global__ void __launch_bounds__(256) reference_kernel(const __nv_bfloat16* h, const __nv_bfloat16* w, int64_t ldh, int64_t ldw, int dim, const int* targets,
+                                                        const int* count, int row0, int rows, float* __restrict__ z_target, float4* __restrict__ row, int* __restrict__ again) {
+  pdl_wait();
+  pdl_trigger();
   const int i = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31, r = row0 + i;
   if (i >= rows) return;
   if (lane == 0 && i % kTile == 0) again[i / kTile] = 0;
@@ -882,9 +899,11 @@ __global__ void __launch_bounds__(256) reference_kernel(const __nv_bfloat16* __r
   }
 }
 // Its tiles joined.  A row whose maximum is too far from M gets one from its maximum, and its tile of rows is formed again; the second call (`second`) then joins those.
-__global__ void __launch_bounds__(1024) join_keep_kernel(const float2* __restrict__ part, int ld, int parts, const int* __restrict__ count, int row0, int rows, const int* __restrict__ idx,
-                                                        const float* __restrict__ z_target, float4* __restrict__ row, int* __restrict__ again, int second, float* __restrict__ row_loss,
+__global__ void __launch_bounds__(1024) join_keep_kernel(const float2* part, int ld, int parts, const int* count, int row0, int rows, const int* idx,
+                                                        const float* z_target, float4* __restrict__ row, int* __restrict__ again, int second, float* __restrict__ row_loss,
                                                         float* __restrict__ log_z) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ float2 slices[32][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   const int live = min(rows, *count - row0);
@@ -919,8 +938,10 @@ __global__ void __launch_bounds__(1024) join_keep_kernel(const float2* __restric
   }
 }
 // packed rows times their 1 / sum, zeros behind them to the end of their tile
-__global__ void __launch_bounds__(256) scaled_rows_kernel(const __nv_bfloat16* __restrict__ h, int64_t ld, int dim, const float4* __restrict__ row, const int* __restrict__ count, int64_t row0, int64_t rows,
+__global__ void __launch_bounds__(256) scaled_rows_kernel(const __nv_bfloat16* h, int64_t ld, int dim, const float4* row, const int* count, int64_t row0, int64_t rows,
                                                           __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
   const int64_t r = row0 + (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x & 31, n = *count;
   if (r >= row0 + rows || r >= (n + kTile - 1) / kTile * kTile) return;
@@ -939,7 +960,9 @@ __global__ void __launch_bounds__(256) scaled_rows_kernel(const __nv_bfloat16* _
 }
 
 // sum or mean of the rows' losses, in a fixed order and 64 bits
-__global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ row_loss, int rows, const int* __restrict__ count, int mean, float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) reduce_kernel(const float* row_loss, int rows, const int* count, int mean, float* __restrict__ loss) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ double sums[32];
   double s = 0;
   for (int i = threadIdx.x; i < rows; i += 1024) s += row_loss[i];
@@ -955,8 +978,10 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ 
 }
 
 // What the backward pass needs of a packed row, and the power of two that brings the largest weight to 2^13 .. 2^14 where the pieces are fp16 (products of small weights would vanish there).
-__global__ void __launch_bounds__(1024) weights_kernel(const float4* __restrict__ stats, const int* __restrict__ idx, const int* __restrict__ count, const float* __restrict__ dloss, int reduction,
-                                                       const float* __restrict__ dlog_z, int has_z, int half, float4* __restrict__ row, float* __restrict__ scales) {
+__global__ void __launch_bounds__(1024) weights_kernel(const float4* stats, const int* idx, const int* count, const float* dloss, int reduction,
+                                                       const float* dlog_z, int has_z, int half, float4* __restrict__ row, float* __restrict__ scales) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ float tops[32];
   const int n = *count, tid = threadIdx.x;
   const float all = reduction == 0 ? 0.f : reduction == 1 ? dloss[0] : dloss[0] / (float)max(1, n);
@@ -984,9 +1009,11 @@ __global__ void __launch_bounds__(1024) weights_kernel(const float4* __restrict_
 // dhidden: a packed row's partial sums joined, times its own factor (`by_row`) or all rows', and q W_t, into its place; zeros for rows that are left out.  Rows [row0, row0 + rows) of idx, a
 // warp each.  V columns at a time.
 template <int V>
-__global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ part, int splits, int64_t split, int64_t ld, int dim, const int* __restrict__ idx, const int* __restrict__ targets,
-                                                      const int* __restrict__ count, int row0, int rows, const float4* __restrict__ row, int by_row, const float* __restrict__ scales, const void* weight,
+__global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int splits, int64_t split, int64_t ld, int dim, const int* idx, const int* targets,
+                                                      const int* count, int row0, int rows, const float4* row, int by_row, const float* scales, const void* weight,
                                                       int64_t weight_stride, int weight_dtype, void* out, int dtype) {
+  pdl_wait();
+  pdl_trigger();
   const int i = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31, r = row0 + i;
   if (i >= rows) return;
   const bool in = r < *count;
@@ -1051,7 +1078,9 @@ constexpr int kSort = 8192;
 template <typename Key>
 __device__ __forceinline__ Key shuffled(Key v, int lanes) { return __shfl_xor_sync(0xffffffffu, v, lanes); }
 template <typename Key>
-__global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targets, const int* __restrict__ count, int row0, int rows, int size, uint64_t* __restrict__ keys) {
+__global__ void __launch_bounds__(1024) sort_kernel(const int* targets, const int* count, int row0, int rows, int size, uint64_t* __restrict__ keys) {
+  pdl_wait();
+  pdl_trigger();
   extern __shared__ __align__(8) unsigned char sort_raw[];
   Key* const other = reinterpret_cast<Key*>(sort_raw);
   const int first = blockIdx.x * kSort, n = min(rows, *count - row0), tid = threadIdx.x, threads = blockDim.x;
@@ -1112,8 +1141,10 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int* __restrict__ targ
 // The sum of q h over the rows that have a target, in their order, at the place of the first of them, and that place by target: one block (of 128 V columns) for each run of equal
 // targets, eight rows on their way at a time (a common token has hundreds).
 template <int V>
-__global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* __restrict__ keys, int size, const float4* __restrict__ row, const int* __restrict__ idx, const void* hidden, int64_t stride, int dtype,
-                                                          int dim, const float* __restrict__ scales, float* __restrict__ sums, int64_t ld, int* __restrict__ heads, int place) {
+__global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* keys, int size, const float4* row, const int* idx, const void* hidden, int64_t stride, int dtype,
+                                                          int dim, const float* scales, float* __restrict__ sums, int64_t ld, int* __restrict__ heads, int place) {
+  pdl_wait();
+  pdl_trigger();
   const int p = blockIdx.x;
   const uint64_t key = keys[p];
   if (key == ~0ull || (p > 0 && keys[p - 1] >> 32 == key >> 32)) return;
@@ -1163,8 +1194,10 @@ __global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* __rest
 
 // out = factor * src, the factor scales[1] (dloss NULL) or scales[1] dloss; zeros where no row counts.  V elements at a time.
 template <int V>
-__global__ void __launch_bounds__(256) scaled_copy_kernel(const float* __restrict__ src, int64_t ld, int64_t rows, int dim, const int* __restrict__ count, const float* __restrict__ scales,
-                                                          const float* __restrict__ dloss, int has_dloss, void* out, int dtype) {
+__global__ void __launch_bounds__(256) scaled_copy_kernel(const float* src, int64_t ld, int64_t rows, int dim, const int* count, const float* scales,
+                                                          const float* dloss, int has_dloss, void* out, int dtype) {
+  pdl_wait();
+  pdl_trigger();
   const bool none = *count == 0;
   const float f = has_dloss ? scales[1] * dloss[0] : scales[1];
   const int per = dim / V;
@@ -1288,8 +1321,7 @@ int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap&
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   int64_t tiles = 0;
   for (const Job& j : g.job) tiles += (int64_t)j.m_tiles * j.n_tiles * j.splits;
-  kern<<<(unsigned)(2 * std::max<int64_t>(1, std::min<int64_t>(tiles, pairs))), kThreads, kSmem, st>>>(ma, mb, mb1, g);
-  return launch_status("linear_ce gemm_kernel");
+  return launch_overlapped("linear_ce gemm_kernel", kern, (unsigned)(2 * std::max<int64_t>(1, std::min<int64_t>(tiles, pairs))), kThreads, kSmem, st, ma, mb, mb1, g);
 }
 template <int EPI>
 int gemm_of(const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb1, const GemmArgs& g, cudaStream_t st) {
@@ -1326,21 +1358,17 @@ int prepare(Run& r, bool packs) {
   const int64_t plane_h = up(p.rows, kTile) * p.ldh, plane_w = p.copy_w ? p.vocab * p.ldh : p.vocab * a.weight_stride;
   auto pack = [&](const void* src, int64_t stride, int64_t rows, const int* map, uint16_t* dst, int64_t plane) {
     const unsigned grid = (unsigned)((rows + 7) / 8);
-    if (p.planes == 3) pack_kernel<float, 3><<<grid, 256, 0, r.st>>>(src, stride, rows, (int)p.dim, map, r.count(), dst, p.ldh, plane);
-    else pack_kernel<uint16_t, 1><<<grid, 256, 0, r.st>>>(src, stride, rows, (int)p.dim, map, r.count(), dst, p.ldh, plane);
-    return launch_status("linear_ce pack_kernel");
+    auto kern = p.planes == 3 ? pack_kernel<float, 3> : pack_kernel<uint16_t, 1>;
+    return launch_overlapped("linear_ce pack_kernel", kern, grid, 256, 0, r.st, src, stride, rows, (int)p.dim, map, r.count(), dst, p.ldh, plane);
   };
   if (packs && p.rows <= kFewRows) {
-    if (p.planes == 3)
-      few_rows_kernel<float, 3><<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, a.hidden, a.hidden_stride, (int)p.dim, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z,
-                                                      r.at<uint16_t>(p.h), p.ldh, plane_h);
-    else
-      few_rows_kernel<uint16_t, 1><<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, a.hidden, a.hidden_stride, (int)p.dim, r.idx(), r.packed(), r.count(), a.row_loss,
-                                                         a.log_z, r.at<uint16_t>(p.h), p.ldh, plane_h);
-    if (const int rc = launch_status("linear_ce few_rows_kernel")) return rc;
+    auto kern = p.planes == 3 ? few_rows_kernel<float, 3> : few_rows_kernel<uint16_t, 1>;
+    if (const int rc = launch_overlapped("linear_ce few_rows_kernel", kern, 1, 1024, 0, r.st,
+                                         a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, a.hidden, a.hidden_stride, (int)p.dim, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z,
+                                         r.at<uint16_t>(p.h), p.ldh, plane_h)) return rc;
   } else if (packs) {
-    rows_kernel<<<1, 1024, 0, r.st>>>(a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z);
-    if (const int rc = launch_status("linear_ce rows_kernel")) return rc;
+    if (const int rc = launch_overlapped("linear_ce rows_kernel", rows_kernel, 1, 1024, 0, r.st,
+                                         a.targets, (int)p.rows, a.ignore_index, (int)p.vocab, r.idx(), r.packed(), r.count(), a.row_loss, a.log_z)) return rc;
     if (const int rc = pack(a.hidden, a.hidden_stride, p.rows, r.idx(), r.at<uint16_t>(p.h), plane_h)) return rc;
   }
   if (packs && p.copy_w)
@@ -1373,21 +1401,19 @@ int target_rows(const Run& r, int64_t row0, int64_t rows) {
   const Plan& p = r.p;
   uint64_t* keys = r.at<uint64_t>(p.keys);
   const unsigned threads = (unsigned)std::max(32, p.sort / 8);
-  if (p.vocab < 1 << 19) {
-    sort_kernel<uint32_t><<<p.sorts, threads, threads * 32, r.st>>>(r.packed(), r.count(), (int)row0, (int)rows, p.sort, keys);
-  } else {
-    cudaFuncSetAttribute(sort_kernel<uint64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
-    sort_kernel<uint64_t><<<p.sorts, threads, threads * 64, r.st>>>(r.packed(), r.count(), (int)row0, (int)rows, p.sort, keys);
-  }
-  if (const int rc = launch_status("linear_ce sort_kernel")) return rc;
+  const bool narrow = p.vocab < 1 << 19;  // a key's target and place in 32 bits
+  auto sort = narrow ? sort_kernel<uint32_t> : sort_kernel<uint64_t>;
+  if (!narrow) cudaFuncSetAttribute(sort_kernel<uint64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSort * 8);
+  if (const int rc = launch_overlapped("linear_ce sort_kernel", sort, p.sorts, threads, threads * (narrow ? 32 : 64), r.st,
+                                       r.packed(), r.count(), (int)row0, (int)rows, p.sort, keys)) return rc;
   if (const int rc = zero(r.at<void>(p.heads), (size_t)p.sorts * p.vocab * 4, r.st, 0xff)) return rc;
   const bool wide = p.dim % 4 == 0 && r.a.hidden_stride % 4 == 0 && aligned_to(r.a.hidden, 16);
   auto kern = wide ? target_rows_kernel<4> : target_rows_kernel<1>;
   const int per = wide ? 512 : 128;
   for (int i = 0; i < p.sorts; ++i) {
-    kern<<<dim3((unsigned)p.sort, (unsigned)((p.dim + per - 1) / per)), 128, 0, r.st>>>(keys + (int64_t)i * kSort, p.sort, r.row(), r.idx(), r.a.hidden, r.a.hidden_stride, r.a.io_dtype, (int)p.dim,
-                                                                                      r.at<float>(p.scales), r.at<float>(p.sums), p.ldo, r.at<int>(p.heads) + (int64_t)i * p.vocab, i * p.sort);
-    if (const int rc = launch_status("linear_ce target_rows_kernel")) return rc;
+    if (const int rc = launch_overlapped("linear_ce target_rows_kernel", kern, dim3((unsigned)p.sort, (unsigned)((p.dim + per - 1) / per)), 128, 0, r.st,
+                                         keys + (int64_t)i * kSort, p.sort, r.row(), r.idx(), r.a.hidden, r.a.hidden_stride, r.a.io_dtype, (int)p.dim, r.at<float>(p.scales), r.at<float>(p.sums),
+                                         p.ldo, r.at<int>(p.heads) + (int64_t)i * p.vocab, i * p.sort)) return rc;
   }
   return SSM_OK;
 }
@@ -1422,26 +1448,26 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
   const unsigned grid = (unsigned)((rows + 7) / 8);
   const bool wide = p.dim % 4 == 0 && r.a.weight_stride % 4 == 0 && aligned_to({r.a.weight, dh}, 16);
   auto kern = wide ? dhidden_kernel<4> : dhidden_kernel<1>;
-  kern<<<grid, 256, 0, r.st>>>(a.out, a.splits, a.out_split, p.ldo, (int)p.dim, r.idx(), r.packed(), r.count(), (int)row0, (int)rows, r.row(), by_row, r.at<float>(p.scales), r.a.weight, r.a.weight_stride,
-                               r.a.io_dtype, dh, dh_dtype);
-  return launch_status("linear_ce dhidden_kernel");
+  return launch_overlapped("linear_ce dhidden_kernel", kern, grid, 256, 0, r.st,
+                           a.out, a.splits, a.out_split, p.ldo, (int)p.dim, r.idx(), r.packed(), r.count(), (int)row0, (int)rows, r.row(), by_row, r.at<float>(p.scales), r.a.weight,
+                           r.a.weight_stride, r.a.io_dtype, dh, dh_dtype);
 }
 int scaled_copy(const float* src, int64_t ld, int64_t rows, int64_t dim, const int* count, const float* scales, const float* dloss, void* out, int dtype, cudaStream_t st) {
   const bool wide = dim % 4 == 0 && ld % 4 == 0 && aligned_to({src, out}, 16);
   const int64_t all = rows * (wide ? dim / 4 : dim);
   const unsigned grid = (unsigned)std::min<int64_t>((all + 255) / 256, 148 * 32);
   auto kern = wide ? scaled_copy_kernel<4> : scaled_copy_kernel<1>;
-  kern<<<grid, 256, 0, st>>>(src, ld, rows, (int)dim, count, scales, dloss ? dloss : scales, dloss != nullptr, out, dtype);
-  return launch_status("linear_ce scaled_copy_kernel");
+  return launch_overlapped("linear_ce scaled_copy_kernel", kern, grid, 256, 0, st, src, ld, rows, (int)dim, count, scales, dloss ? dloss : scales, dloss != nullptr, out, dtype);
 }
 int reduce(const Run& r) {
   if (r.a.reduction == 0) return SSM_OK;
   if (r.a.rows == 0) return zero(r.a.loss, 4, r.st);
-  reduce_kernel<<<1, 1024, 0, r.st>>>(r.a.row_loss, (int)r.a.rows, r.count(), r.a.reduction == 2, r.a.loss);
-  return launch_status("linear_ce reduce_kernel");
+  return launch_overlapped("linear_ce reduce_kernel", reduce_kernel, 1, 1024, 0, r.st, r.a.row_loss, (int)r.a.rows, r.count(), r.a.reduction == 2, r.a.loss);
 }
 // what the one-pass form's gradients are multiplied by: kept[0] 1 / rows that count for a mean, kept[1] how many count (as an integer); scales of this call
 __global__ void share_kernel(const int* count, int mean, float* kept, float* scales) {
+  pdl_wait();
+  pdl_trigger();
   kept[0] = scales[0] = 1.f;
   scales[1] = 1.f;
   kept[1] = mean ? 1.f / (float)max(1, *count) : 1.f;
@@ -1486,13 +1512,13 @@ extern "C" int ssm_linear_ce_fwd(const ssm_linear_ce_args* args, ssm_stream_t st
         CUtensorMap mf;
         if (const int rc = encode(&mf, r.at<void>(p.h), p.dim, p.rows, p.planes, p.ldh, up(p.rows, kTile) * p.ldh, p.fmt, g.bn / 2)) return rc;
         if (const int rc = gemm_of<kFew>(p, r.mw, mf, mf, g, r.st)) return rc;
-        few_join_kernel<<<(unsigned)p.rows, 256, 0, r.st>>>(g.part, g.part_ld, g.count, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z);
-        if (const int rc = launch_status("linear_ce few_join_kernel")) return rc;
+        if (const int rc = launch_overlapped("linear_ce few_join_kernel", few_join_kernel, (unsigned)p.rows, 256, 0, r.st,
+                                             g.part, g.part_ld, g.count, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z)) return rc;
         continue;
       }
       if (const int rc = gemm_of<kStats>(p, r.mh, r.mw, r.mw, g, r.st)) return rc;
-      join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z);
-      if (const int rc = launch_status("linear_ce join_kernel")) return rc;
+      if (const int rc = launch_overlapped("linear_ce join_kernel", join_kernel, (unsigned)((rows + 31) / 32), 1024, 0, r.st,
+                                           g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), r.packed(), g.z_target, stats, a.row_loss, a.log_z)) return rc;
     }
   }
   return reduce(r);
@@ -1512,9 +1538,9 @@ extern "C" int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_
   if (const int rc = prepare(r, false)) return rc;
   float* scales = r.at<float>(p.scales);
   const WeightGrad dw{r.at<float>(p.dw), args->dweight, p.dim, args->dweight_dtype};
-  weights_kernel<<<1, 1024, 0, r.st>>>(reinterpret_cast<const float4*>(a.stats), r.idx(), r.count(), args->dloss, a.reduction, args->dlog_z ? args->dlog_z : args->dloss, args->dlog_z != nullptr,
-                                       a.io_dtype == SSM_F16, r.row(), scales);
-  if (const int rc = launch_status("linear_ce weights_kernel")) return rc;
+  if (const int rc = launch_overlapped("linear_ce weights_kernel", weights_kernel, 1, 1024, 0, r.st,
+                                       reinterpret_cast<const float4*>(a.stats), r.idx(), r.count(), args->dloss, a.reduction, args->dlog_z ? args->dlog_z : args->dloss, args->dlog_z != nullptr,
+                                       a.io_dtype == SSM_F16, r.row(), scales)) return rc;
   for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
     const int64_t rows = std::min(p.piece, p.rows - row0);
     if (const int rc = gemm_of<kGrad>(p, r.mh, r.mw, r.mw, logits_args(r, row0, rows), r.st)) return rc;
@@ -1533,8 +1559,7 @@ extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidde
   Run r{a, plan_of(a, kBoth), static_cast<char*>(a.scratch), reinterpret_cast<cudaStream_t>(stream)};
   const Plan& p = r.p;
   if (const int rc = prepare(r, true)) return rc;
-  share_kernel<<<1, 1, 0, r.st>>>(r.count(), a.reduction == 2, kept, r.at<float>(p.scales));
-  if (const int rc = launch_status("linear_ce share_kernel")) return rc;
+  if (const int rc = launch_overlapped("linear_ce share_kernel", share_kernel, 1, 1, 0, r.st, r.count(), a.reduction == 2, kept, r.at<float>(p.scales))) return rc;
   const __nv_bfloat16* h = r.at<__nv_bfloat16>(p.h);
   __nv_bfloat16* hs = r.at<__nv_bfloat16>(p.hs);
   CUtensorMap mhs;
@@ -1545,17 +1570,17 @@ extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidde
     const int64_t rows = std::min(p.piece, p.rows - row0);
     const unsigned warps = (unsigned)((rows + 7) / 8);
     GemmArgs g = logits_args(r, row0, rows);
-    reference_kernel<<<warps, 256, 0, r.st>>>(h, static_cast<const __nv_bfloat16*>(r.w()), p.ldh, r.ldw(), (int)p.dim, r.packed(), r.count(), (int)row0, (int)rows, g.z_target, r.row(), again);
-    if (const int rc = launch_status("linear_ce reference_kernel")) return rc;
+    if (const int rc = launch_overlapped("linear_ce reference_kernel", reference_kernel, warps, 256, 0, r.st,
+                                         h, static_cast<const __nv_bfloat16*>(r.w()), p.ldh, r.ldw(), (int)p.dim, r.packed(), r.count(), (int)row0, (int)rows, g.z_target, r.row(),
+                                         again)) return rc;
     for (int second = 0; second < 2; ++second) {
       g.again = second ? again : nullptr;
       if (const int rc = gemm_of<kKeep>(p, r.mh, r.mw, r.mw, g, r.st)) return rc;
-      join_keep_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, r.st>>>(g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), g.z_target, r.row(), again, second, a.row_loss, a.log_z);
-      if (const int rc = launch_status("linear_ce join_keep_kernel")) return rc;
+      if (const int rc = launch_overlapped("linear_ce join_keep_kernel", join_keep_kernel, (unsigned)((rows + 31) / 32), 1024, 0, r.st,
+                                           g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), g.z_target, r.row(), again, second, a.row_loss, a.log_z)) return rc;
     }
     if (dweight) {
-      scaled_rows_kernel<<<warps, 256, 0, r.st>>>(h, p.ldh, (int)p.dim, r.row(), r.count(), row0, rows, hs);
-      if (const int rc = launch_status("linear_ce scaled_rows_kernel")) return rc;
+      if (const int rc = launch_overlapped("linear_ce scaled_rows_kernel", scaled_rows_kernel, warps, 256, 0, r.st, h, p.ldh, (int)p.dim, r.row(), r.count(), row0, rows, hs)) return rc;
     }
     if (const int rc = gradients(r, row0, rows, mhs, true, dhidden, SSM_F32, dweight ? &dw : nullptr)) return rc;
   }
