@@ -1006,7 +1006,8 @@ __global__ void __launch_bounds__(1024) weights_kernel(const float4* stats, cons
   }
 }
 
-// dhidden: a packed row's partial sums joined, times its own factor (`by_row`) or all rows', and q W_t, into its place; zeros for rows that are left out.  Rows [row0, row0 + rows) of idx, a
+// dhidden: a packed row's partial sums joined, times its own factor (`by_row`) or all rows', and q W_t, into its place; zeros for rows that are left out (-0 with `by_row`: a factor
+// still to come, infinite or NaN, leaves those as they are).  Rows [row0, row0 + rows) of idx, a
 // warp each.  V columns at a time.
 template <int V>
 __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int splits, int64_t split, int64_t ld, int dim, const int* idx, const int* targets,
@@ -1051,6 +1052,10 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int spl
   }
   for (int c = lane * V; c < dim; c += 32 * V) {
     float v[V] = {}, e[V];
+    if (!in && by_row) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = -0.f;
+    }
     if (in) {
 #pragma unroll 4
       for (int s = 0; s < splits; ++s) {
@@ -1192,7 +1197,7 @@ __global__ void __launch_bounds__(128) target_rows_kernel(const uint64_t* keys, 
   else *to = v[0] * scale;
 }
 
-// out = factor * src, the factor scales[1] (dloss NULL) or scales[1] dloss; zeros where no row counts.  V elements at a time.
+// out = factor * src, the factor scales[1] (dloss NULL) or scales[1] dloss; zeros where no row counts, and for -0.  V elements at a time.
 template <int V>
 __global__ void __launch_bounds__(256) scaled_copy_kernel(const float* src, int64_t ld, int64_t rows, int dim, const int* count, const float* scales,
                                                           const float* dloss, int has_dloss, void* out, int dtype) {
@@ -1213,7 +1218,7 @@ __global__ void __launch_bounds__(256) scaled_copy_kernel(const float* src, int6
       v[0] = src[r * ld + c];
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = none ? 0.f : v[k] * f;
+    for (int k = 0; k < V; ++k) v[k] = none || __float_as_uint(v[k]) == 0x80000000u ? 0.f : v[k] * f;
     if constexpr (V == 4) {
       if (dtype == SSM_F32) {
         __stcs(reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + r * dim + c), make_float4(v[0], v[1], v[2], v[3]));

@@ -184,6 +184,16 @@ def test_one_pass_with_values_that_are_not_finite():
         assert dh[torch.arange(600, device="cuda") != 5].isfinite().all()
 
 
+@pytest.mark.parametrize("d", [64, 33])
+@pytest.mark.parametrize("factor", [math.inf, math.nan])
+def test_one_pass_with_a_factor_that_is_not_finite_keeps_rows_left_out_at_zero(factor, d):
+    h, w, t, _, _ = make(300, d, 400, torch.bfloat16)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    dh, dw = torch.autograd.grad(ops.linear_cross_entropy(h, w, t, reduction="sum"), [h, w], torch.full((), factor, device="cuda"))
+    out = t == -100
+    assert out.any() and torch.equal(dh[out], torch.zeros_like(dh[out])) and not dh[~out].isfinite().any() and not dw.isfinite().any()
+
+
 def test_one_pass_may_be_walked_twice():
     h, w, t, _, _ = make(300, 64, 400, torch.bfloat16)
     h, w = h.requires_grad_(True), w.requires_grad_(True)
