@@ -585,17 +585,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
               } else {
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
+                for (int i = 0; i < 32; i += 16) {
                   if (32 * c + i < room) {
-                    __nv_bfloat16 e[8][3];
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) split3(__uint_as_float(v[c][i + q]), e[q]);
+                    for (int q = 0; q < PLANES; ++q) {
+                      uint32_t w[8];
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                      uint32_t w[4];
-#pragma unroll
-                      for (int h = 0; h < 4; ++h) w[h] = (uint32_t)__bfloat16_as_ushort(e[2 * h][q]) | (uint32_t)__bfloat16_as_ushort(e[2 * h + 1][q]) << 16;
-                      *reinterpret_cast<uint4*>(to + q * g.g_plane + 32 * c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                      for (int h = 0; h < 8; ++h) {
+                        float x[2] = {__uint_as_float(v[c][i + 2 * h]), __uint_as_float(v[c][i + 2 * h + 1])};
+                        w[h] = pack2<__nv_bfloat16>(x[0], x[1]);
+                        x[0] -= __uint_as_float(w[h] << 16), x[1] -= __uint_as_float(w[h] & 0xffff0000u);  // what is not finite stays in the first
+                        v[c][i + 2 * h] = fabsf(x[0]) < INFINITY ? __float_as_uint(x[0]) : 0u, v[c][i + 2 * h + 1] = fabsf(x[1]) < INFINITY ? __float_as_uint(x[1]) : 0u;
+                      }
+                      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to + q * g.g_plane + 32 * c + i), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                                   "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                   : "memory");
                     }
                   }
                 }
