@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads) norm_partial_kernel(const __grid_con
 #pragma unroll
         for (int e = 0; e < 8; ++e) q = fmaf(f[e], f[e], q);
         if (q >= 0x1p-100f && q <= 0x1p100f) all += q;
-        else r.sum += wide_squares(f);
+        else if ((v[k].x | v[k].y | v[k].z | v[k].w) != 0u) r.sum += wide_squares(f);  // rows of zeros are common
       }
     }
     if constexpr (!MAX) r.sum += (double)all;
