@@ -35,6 +35,7 @@ namespace {
 constexpr int kTile = 256, kK = 64, kStages = 6, kThreads = 384, kEpilogueWarps = 8;
 constexpr int kBoxBytes = 64 * kK * 2, kStageBytes = 4 * kBoxBytes;
 constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr int kStagePitch = 33, kStaging = kEpilogueWarps * 32 * kStagePitch * 4;  // kOut: a warp's rows on their way to places that are not aligned
 constexpr int kStatus = 128;           // status of a wait that ran out
 constexpr float kFar = 268435456.f;    // 2^28: M of a tile is no less than minus this; rows whose M reaches twice that give NaN (their logits' steps are larger than any difference that matters)
 constexpr int kPairs = 6;
@@ -153,6 +154,21 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// 32 columns, a value of each in every lane, joined over the lanes: lane l gets column l in v[0].  31 exchanges, half of the columns going on each time (a column after another
+// 5 each, one waiting for the last: 43 rows, 106299 x 128: 69 us)
+template <typename Join>
+__device__ __forceinline__ void to_lanes(float (&v)[32], int lane, Join join) {
+#pragma unroll
+  for (int h = 16; h >= 1; h /= 2) {
+    const bool upper = lane & h;
+#pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + h], h);
+      v[i] = join(upper ? v[i + h] : v[i], other);
+    }
+  }
+}
+
 struct TileAt {
   int job, m, n, split, kb0, kb1;  // job -1: no more
 };
@@ -168,24 +184,36 @@ __device__ __forceinline__ void add_columns(const float* from, int cols, uint32_
     }
   }
 }
-__device__ __forceinline__ void add_target(const GemmArgs& g, const Job& j, int row, int64_t col, uint32_t (&v)[32]) {
-  const int cols = (int)min((int64_t)32, g.dim - col);
-  if (cols <= 0) return;
-  for (int b = 0; b < g.sorts; ++b) {
-    const int at = g.heads[(int64_t)b * j.out_rows + row];
-    if (at >= 0) add_columns(g.target_sums + at * j.ld + col, cols, v);
+// where the targets' part of a row of dW is, in each sort of a piece (two at most); -1: nowhere
+struct Heads {
+  int at[2];
+};
+__device__ __forceinline__ Heads heads_of(const GemmArgs& g, const Job& j, int row) {
+  Heads h{{-1, -1}};
+  if (row < j.out_rows) {
+    h.at[0] = g.heads[row];
+    if (g.sorts > 1) h.at[1] = g.heads[(int64_t)j.out_rows + row];
   }
+  return h;
 }
-// ... and their way into dW
-__device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bool add, int row, int64_t col, uint32_t (&v)[32]) {
+__device__ __forceinline__ void add_target(const GemmArgs& g, const Job& j, const Heads& h, int64_t col, uint32_t (&v)[32]) {
   const int cols = (int)min((int64_t)32, g.dim - col);
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+    if (h.at[b] >= 0) add_columns(g.target_sums + h.at[b] * j.ld + col, cols, v);
+}
+// ... and their way into dW, a warp's 32 rows from `row0` on.  Rows that are not aligned go through shared memory, so that a warp writes neighbouring columns (20 rows, 30855 x 1219 bf16:
+// the product with a thread to a row 645 us)
+__device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bool add, int row0, int64_t col, uint32_t (&v)[32], float* staging) {
+  const int cols = (int)min((int64_t)32, g.dim - col), lane = threadIdx.x & 31, row = row0 + lane;
   if (cols <= 0) return;
-  if (add) add_columns(j.out + row * j.ld + col, cols, v);
+  if (add && row < j.out_rows) add_columns(j.out + row * j.ld + col, cols, v);
   const float f = g.scales[1];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-  const int64_t to = row * g.dw_ld + col;
   if (g.dw_wide && cols == 32) {
+    if (row >= j.out_rows) return;
+    const int64_t to = row * g.dw_ld + col;
     if (g.dw_dtype == SSM_F32) {
       float* out = reinterpret_cast<float*>(g.dw) + to;
 #pragma unroll
@@ -204,9 +232,15 @@ __device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bo
       }
     }
   } else {
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < cols) store_dyn(g.dw, to + i, g.dw_dtype, __uint_as_float(v[i]));
+    for (int i = 0; i < 32; ++i) staging[lane * kStagePitch + i] = __uint_as_float(v[i]);
+    __syncwarp();
+    const int rows = min(32, j.out_rows - row0);
+    if (lane < cols) {
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) store_dyn(g.dw, (row0 + r) * g.dw_ld + col + lane, g.dw_dtype, staging[r * kStagePitch + lane]);
+    }
   }
 }
 
@@ -374,6 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp >= 4) {  // accumulators
     const uint32_t tempty0 = leader_address(tempty);
     const int half = (warp - 4) >> 2, row_in = rank * 128 + (warp & 3) * 32 + lane;
+    float* const staging = reinterpret_cast<float*>(raw + (ring - tc::smem_u32(raw)) + kStages * kStageBytes) + (warp - 4) * 32 * kStagePitch;  // kOut alone has it
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     int n = 0;
     bool ok = true;
@@ -397,13 +432,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int64_t out_col = p.n * g.bn + half * width;
       const bool none = p.kb0 == p.kb1;  // no rows in the last piece
       const bool add = EPI == kOut && j.add && *g.count > 0;
+      Heads heads{{-1, -1}};
+      if (EPI == kOut && p.job) heads = heads_of(g, j, row);  // before the accumulator is there
+      // a warp whose rows nobody reads: of a piece of G those up to the next block of K are (zeros), of all else those that are live
+      const bool idle = EPI != kFew && !(EPI == kOut && p.job) && row - lane >= (EPI == kGrad || EPI == kKeep ? (live + kK - 1) / kK * kK : live);
       if constexpr (!kSegments) {
         const int b = n & 1;
         if (!none && !arrived(b)) break;
         const uint32_t from = tmem + lanes + b * 256 + half * width;
         float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
         const int cols = (int)min((int64_t)width, j.ld - out_col);
-        for (int c = 0; c < width; c += 32) {
+        for (int c = 0; c < width && !idle; c += 32) {
           uint32_t v[32];
           if (none) {
 #pragma unroll
@@ -412,9 +451,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tmem_ld32_issue(from + c, v);
             tmem_wait_ld();
           }
-          if (p.job && row < j.out_rows) add_target(g, j, row, out_col + c, v);
-          if (j.last && row < j.out_rows) {
-            last_columns(g, j, add, row, out_col + c, v);
+          if (p.job) add_target(g, j, heads, out_col + c, v);
+          if (j.last) {
+            last_columns(g, j, add, row - lane, out_col + c, v, staging);
           } else if (row < j.out_rows) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
@@ -439,7 +478,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int b = n & 1;
           if (!arrived(b)) break;
           const uint32_t from = tmem + lanes + b * 256 + half * width;
-          if (seg == p.kb0) {
+          if (idle) {
+          } else if (seg == p.kb0) {
             if (EPI == kFew && width == 16) {
               float w[16];
               tc::tmem_ld16(from, w);
@@ -465,6 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           release(b);
         }
         if (!ok) break;
+        if (idle) continue;
         if (EPI == kOut && none) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
@@ -472,32 +513,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 32; ++i) v[c][i] = 0u;
         }
         if constexpr (EPI == kFew) {  // a thread has a row of the weight, its registers packed rows
-          const int id = p.m * kTile + row_in, first = half * width;
-          const bool in = id < g.vocab;
+          const int id = p.m * kTile + row_in, first = half * width, cols = min(width, live - first);
+          if (cols > 0) {
+            const int target = lane < cols ? g.targets[g.row0 + first + lane] - (id - lane) : -1;  // lane l for column l: a row of this warp, or none
+            for (uint32_t hits = __ballot_sync(0xffffffffu, target >= 0 && target < 32); hits; hits &= hits - 1) {
+              const int i = __ffs(hits) - 1;
+              if (lane == __shfl_sync(0xffffffffu, target, i) && id < g.vocab) {
+                float z = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (i >= width || first + i >= live) break;
-            const float z = in ? __uint_as_float(v[0][i]) : -INFINITY;
-            if (in && g.targets[g.row0 + first + i] == id) g.z_target[g.row0 + first + i] = z;
-            float m = z;
+                for (int k = 0; k < 32; ++k) z = k == i ? __uint_as_float(v[0][k]) : z;
+                g.z_target[g.row0 + first + i] = z;
+              }
+            }
+            float z[32];
 #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-            const float M = fmaxf(ceilf(m * kLog2e), -kFar);
-            const float s = warp_sum(ex2_approx(fmaf(z, kLog2e, -M)));
-            if (lane == 0) g.part[(int64_t)(first + i) * g.part_ld + (p.m * 2 + rank) * 4 + (warp & 3)] = make_float2(M, s);
+            for (int i = 0; i < 32; ++i) z[i] = id < g.vocab ? __uint_as_float(v[0][i]) : -INFINITY;
+            float e[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) e[i] = z[i];
+            to_lanes(e, lane, [](float x, float y) { return fmaxf(x, y); });
+            const float M = fmaxf(ceilf(e[0] * kLog2e), -kFar);  // of column `lane`
+#pragma unroll
+            for (int i = 0; i < 32; ++i) e[i] = ex2_approx(fmaf(z[i], kLog2e, -__shfl_sync(0xffffffffu, M, i)));
+            to_lanes(e, lane, [](float x, float y) { return x + y; });
+            if (lane < cols) g.part[(int64_t)(first + lane) * g.part_ld + (p.m * 2 + rank) * 4 + (warp & 3)] = make_float2(M, e[0]);
           }
         } else if constexpr (EPI == kOut) {
           float* out = j.out + p.split * j.out_split + row * j.ld + out_col;
           const int cols = (int)min((int64_t)width, j.ld - out_col);
-          if (p.job && row < j.out_rows) {
+          if (p.job) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              if (32 * c < width) add_target(g, j, row, out_col + 32 * c, v[c]);
+              if (32 * c < width) add_target(g, j, heads, out_col + 32 * c, v[c]);
           }
-          if (row < j.out_rows && j.last) {
+          if (j.last) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              if (32 * c < width) last_columns(g, j, add, row, out_col + 32 * c, v[c]);
+              if (32 * c < width) last_columns(g, j, add, row - lane, out_col + 32 * c, v[c], staging);
           } else if (row < j.out_rows) {
 #pragma unroll
             for (int i = 0; i < 128; i += 4) {
@@ -709,6 +761,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
         *reinterpret_cast<uint4*>(to + c) = v;
       }
     } else {
+#pragma unroll 8
       for (int c = lane; c < dim; c += 32) to[c] = zero ? (uint16_t)0 : bits[c];
     }
   } else if (dim % 4 == 0 && reinterpret_cast<uintptr_t>(row) % 16 == 0) {
@@ -776,7 +829,7 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* targets, 
       }
       continue;
     }
-#pragma unroll 4
+#pragma unroll 8
     for (int c = lane; c < dim; c += 32) {
       if constexpr (PLANES == 1) {
         const uint16_t bits = reinterpret_cast<const uint16_t*>(row)[c];
@@ -1027,11 +1080,12 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int spl
   const float4 w = in ? row[r] : make_float4(0.f, 0.f, 0.f, 0.f);
   const float f = by_row ? w.y : scales[1];
   if (in && V == 4) {  // four pieces in flight
-    for (int c0 = lane * 4; c0 < dim; c0 += 512) {
+    for (int c0 = blockIdx.y * 512 + lane * 4; c0 < dim; c0 += 512 * gridDim.y) {
       float4 x[4];
       float e[4][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[k] = __ldcs(reinterpret_cast<const float4*>(part + i * ld + min(c0 + 128 * k, dim - 4)));
+#pragma unroll 2
       for (int s = 1; s < splits; ++s) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -1054,7 +1108,7 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int spl
     }
     return;
   }
-  for (int c = lane * V; c < dim; c += 32 * V) {
+  for (int c = (blockIdx.y * 32 + lane) * V; c < dim; c += 32 * V * gridDim.y) {
     float v[V] = {}, e[V];
     if (!in && by_row) {
 #pragma unroll
@@ -1327,10 +1381,11 @@ int check(const ssm_linear_ce_args& a) {
 template <int EPI, typename T, int PLANES>
 int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb1, const GemmArgs& g, int pairs, cudaStream_t st) {
   auto kern = gemm_kernel<EPI, T, PLANES>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  constexpr int smem = kSmem + (EPI == kOut ? kStaging : 0);
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   int64_t tiles = 0;
   for (const Job& j : g.job) tiles += (int64_t)j.m_tiles * j.n_tiles * j.splits;
-  return launch_overlapped("linear_ce gemm_kernel", kern, (unsigned)(2 * std::max<int64_t>(1, std::min<int64_t>(tiles, pairs))), kThreads, kSmem, st, ma, mb, mb1, g);
+  return launch_overlapped("linear_ce gemm_kernel", kern, (unsigned)(2 * std::max<int64_t>(1, std::min<int64_t>(tiles, pairs))), kThreads, smem, st, ma, mb, mb1, g);
 }
 template <int EPI>
 int gemm_of(const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb1, const GemmArgs& g, cudaStream_t st) {
@@ -1454,9 +1509,11 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
   }
   if (const int rc = gemm_of<kOut>(p, r.mg, r.mw, h2, g, r.st)) return rc;
   if (!dh) return SSM_OK;
-  const unsigned grid = (unsigned)((rows + 7) / 8);
   const bool wide = p.dim % 4 == 0 && r.a.weight_stride % 4 == 0 && aligned_to({r.a.weight, dh}, 16);
   auto kern = wide ? dhidden_kernel<4> : dhidden_kernel<1>;
+  // few rows: their columns shared out too (20 rows of 1219 columns, a warp to a row: 53 us)
+  const int64_t blocks = (rows + 7) / 8, shares = (p.dim + (wide ? 511 : 31)) / (wide ? 512 : 32);
+  const dim3 grid((unsigned)blocks, (unsigned)std::max<int64_t>(1, std::min(shares, 4 * 148 / blocks)));
   return launch_overlapped("linear_ce dhidden_kernel", kern, grid, 256, 0, r.st,
                            a.out, a.splits, a.out_split, p.ldo, (int)p.dim, r.idx(), r.packed(), r.count(), (int)row0, (int)rows, r.row(), by_row, r.at<float>(p.scales), r.a.weight,
                            r.a.weight_stride, r.a.io_dtype, dh, dh_dtype);
