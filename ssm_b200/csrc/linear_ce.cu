@@ -15,7 +15,7 @@
 // Rows that are left out are not computed: the others are packed first, behind one another (which also gives the copies their alignment), and how many
 // there are is known on the device alone, so that every kernel reads it there.
 //
-// Launches overlap: each kernel waits for the one before ahead of its first access (7 rows: 37 -> 29 us, 500 fp32 rows with gradients 257 -> 241), and what it reads is
+// Launches overlap: each kernel waits for the one before ahead of its first access (7 rows: 37 -> 29 us then, 500 fp32 rows with gradients 257 -> 241), and what it reads is
 // not marked as constant, so that no read moves ahead of the wait.
 //
 // Products: pairs of CTAs (cta_group::2) on tiles of 256 x 256 (x 128 for narrow outputs), a CTA holding 128 rows of the accumulator; operands by TMA in the 128-byte swizzle, blocks of 64 x 64, two to
@@ -202,8 +202,13 @@ __device__ __forceinline__ void add_target(const GemmArgs& g, const Job& j, cons
   for (int b = 0; b < 2; ++b)
     if (h.at[b] >= 0) add_columns(g.target_sums + h.at[b] * j.ld + col, cols, v);
 }
+template <typename O>
+__device__ __forceinline__ void put_column(O* to, int64_t ld, const float* from, int rows) {
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r, to += ld) *to = from_f<O>(from[r * kStagePitch]);
+}
 // ... and their way into dW, a warp's 32 rows from `row0` on.  Rows that are not aligned go through shared memory, so that a warp writes neighbouring columns (20 rows, 30855 x 1219 bf16:
-// the product with a thread to a row 645 us)
+// the product with a thread to a row 645 us, so 113)
 __device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bool add, int row0, int64_t col, uint32_t (&v)[32], float* staging) {
   const int cols = (int)min((int64_t)32, g.dim - col), lane = threadIdx.x & 31, row = row0 + lane;
   if (cols <= 0) return;
@@ -238,8 +243,11 @@ __device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bo
     __syncwarp();
     const int rows = min(32, j.out_rows - row0);
     if (lane < cols) {
-#pragma unroll 8
-      for (int r = 0; r < rows; ++r) store_dyn(g.dw, (row0 + r) * g.dw_ld + col + lane, g.dw_dtype, staging[r * kStagePitch + lane]);
+      const float* from = staging + lane;
+      const int64_t to = row0 * g.dw_ld + col + lane;
+      if (g.dw_dtype == SSM_F32) put_column(reinterpret_cast<float*>(g.dw) + to, g.dw_ld, from, rows);
+      else if (g.dw_dtype == SSM_BF16) put_column(reinterpret_cast<__nv_bfloat16*>(g.dw) + to, g.dw_ld, from, rows);
+      else put_column(reinterpret_cast<__half*>(g.dw) + to, g.dw_ld, from, rows);
     }
   }
 }
@@ -735,6 +743,17 @@ __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* targets, int 
   if (tid == 0) *count = base;
 }
 
+// a row that is not aligned, by a warp, eight loads ahead of their stores (left to the compiler, 30855 rows of 1219: 66 us)
+__device__ __forceinline__ void copy_bits(const uint16_t* from, int dim, int lane, bool zero, uint16_t* to) {
+  for (int c = lane; c < dim; c += 256) {
+    uint16_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + 32 * k < dim ? from[c + 32 * k] : (uint16_t)0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + 32 * k < dim) to[c + 32 * k] = zero ? (uint16_t)0 : v[k];
+  }
+}
 // (rows, dim) at a stride -> planes of 16-bit elements with rows of `ld`; with idx the packed rows, and zeros behind them to the end of their tile.  A warp per row.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stride, int64_t rows, int dim, const int* idx, const int* count, uint16_t* dst, int64_t ld, int64_t plane) {
@@ -761,8 +780,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
         *reinterpret_cast<uint4*>(to + c) = v;
       }
     } else {
-#pragma unroll 8
-      for (int c = lane; c < dim; c += 32) to[c] = zero ? (uint16_t)0 : bits[c];
+      copy_bits(bits, dim, lane, zero, to);
     }
   } else if (dim % 4 == 0 && reinterpret_cast<uintptr_t>(row) % 16 == 0) {
 #pragma unroll 4
@@ -829,12 +847,13 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* targets, 
       }
       continue;
     }
-#pragma unroll 8
+    if (PLANES == 1) {
+      copy_bits(reinterpret_cast<const uint16_t*>(row), dim, lane, r >= n, dst + r * ld);
+      continue;
+    }
+#pragma unroll 4
     for (int c = lane; c < dim; c += 32) {
-      if constexpr (PLANES == 1) {
-        const uint16_t bits = reinterpret_cast<const uint16_t*>(row)[c];
-        dst[r * ld + c] = r < n ? bits : (uint16_t)0;
-      } else {
+      if constexpr (PLANES > 1) {
         __nv_bfloat16 p[3];
         split3(r < n ? to_f<T>(row[c]) : 0.f, p);
 #pragma unroll
@@ -1085,7 +1104,7 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int spl
       float e[4][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[k] = __ldcs(reinterpret_cast<const float4*>(part + i * ld + min(c0 + 128 * k, dim - 4)));
-#pragma unroll 2
+#pragma unroll 4
       for (int s = 1; s < splits; ++s) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
