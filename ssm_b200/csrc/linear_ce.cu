@@ -75,7 +75,7 @@ struct GemmArgs {
   // kOut, dW: the targets' rows, and for the last piece dw = sums scales[1]
   void* dw;
   int64_t dw_ld;
-  int dw_dtype, dw_wide, dim;
+  int dw_dtype, dw_wide, dim;  // dw_wide: rows on boundaries of 16 bytes (1), of 32 (2)
   const float* scales;
   const int* heads;            // [sort][vocab]: the target's row in target_sums, or -1
   int sorts;
@@ -169,6 +169,16 @@ __device__ __forceinline__ void to_lanes(float (&v)[32], int lane, Join join) {
   }
 }
 
+// 32 bytes; `whole`: on a boundary of 32, else of 16.  The rows of a warp's threads lie apart, so that halves of a sector would be two writes
+__device__ __forceinline__ void put_sector(void* to, const uint32_t (&w)[8], bool whole) {
+  if (whole) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+  } else {
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    *(reinterpret_cast<uint4*>(to) + 1) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 struct TileAt {
   int job, m, n, split, kb0, kb1;  // job -1: no more
 };
@@ -222,18 +232,21 @@ __device__ __forceinline__ void last_columns(const GemmArgs& g, const Job& j, bo
     if (g.dw_dtype == SSM_F32) {
       float* out = reinterpret_cast<float*>(g.dw) + to;
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(out + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      for (int i = 0; i < 32; i += 8) {
+        const uint32_t w[8] = {v[i], v[i + 1], v[i + 2], v[i + 3], v[i + 4], v[i + 5], v[i + 6], v[i + 7]};
+        put_sector(out + i, w, g.dw_wide > 1);
+      }
     } else {
       uint16_t* out = reinterpret_cast<uint16_t*>(g.dw) + to;
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        uint32_t w[4];
+      for (int i = 0; i < 32; i += 16) {
+        uint32_t w[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 8; ++k) {
           const float a = __uint_as_float(v[i + 2 * k]), b = __uint_as_float(v[i + 2 * k + 1]);
           w[k] = g.dw_dtype == SSM_BF16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
         }
-        *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        put_sector(out + i, w, g.dw_wide > 1);
       }
     }
   } else {
@@ -463,13 +476,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (j.last) {
             last_columns(g, j, add, row - lane, out_col + c, v, staging);
           } else if (row < j.out_rows) {
+            const bool whole = j.ld % 8 == 0 && reinterpret_cast<uintptr_t>(j.out) % 32 == 0;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              if (c + i < cols) {
-                if (add) asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"l"(out + c + i), "f"(__uint_as_float(v[i])), "f"(__uint_as_float(v[i + 1])),
-                                      "f"(__uint_as_float(v[i + 2])), "f"(__uint_as_float(v[i + 3]))
-                                      : "memory");
-                else *reinterpret_cast<uint4*>(out + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            for (int i = 0; i < 32; i += 8) {
+              if (!add && c + i + 8 <= cols) {
+                const uint32_t w[8] = {v[i], v[i + 1], v[i + 2], v[i + 3], v[i + 4], v[i + 5], v[i + 6], v[i + 7]};
+                put_sector(out + c + i, w, whole);
+              } else {
+#pragma unroll
+                for (int k = i; k < i + 8; k += 4) {
+                  if (c + k < cols) {
+                    if (add) asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"l"(out + c + k), "f"(__uint_as_float(v[k])), "f"(__uint_as_float(v[k + 1])),
+                                          "f"(__uint_as_float(v[k + 2])), "f"(__uint_as_float(v[k + 3]))
+                                          : "memory");
+                    else *reinterpret_cast<uint4*>(out + c + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                  }
+                }
               }
             }
           }
@@ -796,11 +818,19 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* src, int64_t stri
                                                                    (uint32_t)__bfloat16_as_ushort(p[2][q]) | (uint32_t)__bfloat16_as_ushort(p[3][q]) << 16);
     }
   } else {
-    for (int c = lane; c < dim; c += 32) {
-      __nv_bfloat16 p[3];
-      split3(zero ? 0.f : to_f<T>(row[c]), p);
+    for (int c = lane; c < dim; c += 256) {  // loads ahead of the stores
+      float f[8];
 #pragma unroll
-      for (int q = 0; q < 3; ++q) to[q * plane + c] = __bfloat16_as_ushort(p[q]);
+      for (int k = 0; k < 8; ++k) f[k] = c + 32 * k < dim && !zero ? to_f<T>(row[c + 32 * k]) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (c + 32 * k < dim) {
+          __nv_bfloat16 p[3];
+          split3(f[k], p);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) to[q * plane + c + 32 * k] = __bfloat16_as_ushort(p[q]);
+        }
+      }
     }
   }
 }
@@ -1523,7 +1553,9 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
     b.m_tiles = (int)((p.vocab + kTile - 1) / kTile), b.n_tiles = d_tiles, b.a_mn = b.b_mn = 1, b.k_is_rows = 1, b.b_k0 = (int)row0;
     b.out = dw->sums, b.ld = p.ldo, b.out_rows = (int)p.vocab, b.add = row0 > 0, b.last = row0 + rows >= p.rows && dw->out != dw->sums;
     if (const int rc = target_rows(r, row0, rows)) return rc;
-    g.dw = dw->out, g.dw_ld = dw->ld, g.dw_dtype = dw->dtype, g.dw_wide = dw->ld % (dw->dtype == SSM_F32 ? 4 : 8) == 0 && aligned_to(dw->out, 16), g.dim = (int)p.dim;
+    const int64_t bytes = dw->ld * dtype_size(dw->dtype);
+    g.dw_wide = bytes % 32 == 0 && aligned_to(dw->out, 32) ? 2 : bytes % 16 == 0 && aligned_to(dw->out, 16) ? 1 : 0;
+    g.dw = dw->out, g.dw_ld = dw->ld, g.dw_dtype = dw->dtype, g.dim = (int)p.dim;
     g.scales = r.at<float>(p.scales), g.heads = r.at<int>(p.heads), g.sorts = p.sorts, g.target_sums = r.at<float>(p.sums);
   }
   if (const int rc = gemm_of<kOut>(p, r.mg, r.mw, h2, g, r.st)) return rc;
