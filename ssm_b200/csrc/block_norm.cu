@@ -7,7 +7,7 @@
 //   g2 = w2 dy;   dr' = dr + s2 (g2 - [mean g2] - h2 mean(g2 h2));   dn = scale gate dr';   dgate = scale dr' n
 //   g1 = w1 dn;   dx = s1 (g1 - [mean g1] - h1 mean(g1 h1));   dresidual = dr';   dw1 = sum dn h1, db1 = sum dn, dw2 = sum dy h2, db2 = sum dy
 //
-// Bound: HBM, 12 bytes an element forward and 20 back with 16-bit activations and a 32-bit stream.  A row is owned by 32 to 512 threads and lies in their
+// Bound: HBM, 12 bytes an element forward and 18 back with 16-bit activations and a 32-bit stream.  A row is owned by 32 to 512 threads and lies in their
 // registers, read once; everything is computed in 32 bits.  The forward pass leaves m1, s1, m2, s2 of each row for the backward pass, which forms r
 // again from x and the residual (it would have to read one of the two anyway).  Backward blocks take runs of neighbouring rows and keep the parameters' gradients of their
 // columns in registers; partial rows are added up by a second kernel in a fixed order, so that the bits repeat.  A gate given per sequence has its

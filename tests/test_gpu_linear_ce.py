@@ -94,6 +94,25 @@ def test_sizes(dtype, n, d, v):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 31, 32, 33, 63, 64, 65])
+def test_up_to_64_rows_with_targets_all_over_a_warps_rows(n, dtype):
+    """Up to 64 rows are columns of a product of the weight's rows: a target is a lane of one warp."""
+    h, w, t, wl, wz = make(n, 96, 1001, dtype, left_out=0.0)
+    for first, step in ((0, 1), (31, 32), (990, 0)):
+        t = (first + step * torch.arange(n, device="cuda")).clamp(max=1000)
+        t[n // 2] = 1000
+        if step == 32:
+            t[n // 3] = -100
+        check(h, w, t, wl, wz)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_odd_width_with_few_and_with_many_rows(dtype):
+    check(*make(20, 1219, 700, dtype))
+    check(*make(300, 517, 333, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_several_pieces_of_the_backward_pass(dtype):
     v = 151936  # 512 MB hold 1766 such rows in 16 bits
     check(*make(2000 if dtype != torch.float32 else 600, 64, v, dtype))
