@@ -139,8 +139,7 @@ def test_reductions(reduction, dtype):
 
 
 def one_pass(h, w, t, reduction="mean", scale=3.0):
-    """bf16 sums and means form the gradients with the loss: values against the definition.  There the rows' 1 / sum is rounded into h once more (2^-9) for dw, and z_t comes from a
-    sum of its own."""
+    """bf16 sums and means form the gradients with the loss: values against the definition.  There the rows' 1 / sum is rounded into h once more (2^-9) for dw."""
     n = h.shape[0]
     share = scale / (1 if reduction == "sum" else max(1, int((t != -100).sum())))
     want = bounds(h, w, t, torch.full((n,), share, device="cuda"), torch.zeros(n, device="cuda"))
@@ -169,6 +168,18 @@ def test_one_pass_with_targets_far_below_the_maximum(spread):
     one_pass(h, w, t)
     one_pass(h, w, (h @ w.t()).float().argmax(-1))
     one_pass(h, w, (h @ w.t()).float().argmin(-1))
+
+
+def test_one_pass_takes_the_targets_logit_from_the_product():
+    """A loss near zero is a difference of two numbers that share the product's errors; only the exponentials, their sum and its logarithm differ between the forms: 2^-18 a row, as in
+    `bounds` (a target's logit summed apart was off by 2^-20 of logits of 64 and more)."""
+    h, w, _, _, _ = make(200, 1024, 700, torch.bfloat16, left_out=0.0)
+    h = h * 16
+    t = (h.float() @ w.float().t()).argmax(-1)
+    loss = ops.linear_cross_entropy(h.requires_grad_(True), w, t, reduction="sum").detach()
+    with torch.no_grad():
+        want = ops.linear_cross_entropy(h, w, t, reduction="sum")
+    assert (loss - want).abs() <= 200 * 2.0 ** -18 + 2.0 ** -22 * want
 
 
 def test_one_pass_where_one_tile_of_rows_is_formed_again():
