@@ -165,6 +165,8 @@ struct LinearCeCall final : Call {
   // A sum or mean is multiplied by one number, which may come later: in bf16 loss and gradients are formed in one pass, 6 N D V operations instead of 8
   bool one_pass() const { return reduction && !want_z && h.scalar_type() == at::kBFloat16 && rows() > 0 && (grad_h || grad_w); }
   bool reads(size_t i) const override { return i < 2 && !one_pass(); }  // the targets' part is packed in the first pass
+  // fp32 gradients of the whole head, or the packed operands, go with the walk: the node lives as long as the loss does
+  bool survives_its_walk() const override { return false; }
   at::TensorOptions f32() const { return h.options().dtype(at::kFloat).requires_grad(false); }
   void fill(ssm_linear_ce_args& a) const {
     a.rows = rows(), a.hidden_stride = rows() > 1 ? h.stride(0) : h.size(1), a.weight_stride = w.size(0) > 1 ? w.stride(0) : w.size(1), a.ignore_index = ignore;

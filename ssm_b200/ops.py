@@ -896,6 +896,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore
 
     Neither pass holds the logits; in 16 bits at most 512 MB of their gradient (and 16384 rows) at a time.  For a sum or mean in bf16 without ``return_log_z`` the gradients are formed along with the
     loss, and held in fp32 until the backward pass scales them (``torch.no_grad()`` forms the loss alone); otherwise the backward pass forms the logits again.
+    What a call holds for its backward pass goes with the walk that ends the graph: a second one needs ``retain_graph=True`` in the first.
 
     16-bit operands are multiplied as they are; the gradient with respect to the logits is rounded to their type before its two products, but for the targets' own, which keep 32 bits.
     fp32 operands are taken as sums of three bf16 numbers each, products below ``2**-24`` left out."""

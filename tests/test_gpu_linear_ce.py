@@ -477,3 +477,24 @@ def test_very_large_logits(scale, dtype):
 def test_a_long_batch_in_many_pieces():
     check(*make(40000, 24, 200, torch.bfloat16))
     one_pass(*make(40000, 24, 200, torch.bfloat16)[:3])
+
+
+@pytest.mark.parametrize("kind", ["one pass", "two passes", "fp32"])
+def test_a_walk_gives_back_what_the_call_held(kind):
+    """The gradients that came with the loss, or the rows (and an fp32 weight) as the products read them, go with the walk, not with the loss."""
+    n, d, v = 512, 256, 20000
+    h, w, t, wl, _ = make(n, d, v, torch.float32 if kind == "fp32" else torch.bfloat16)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    one = torch.ones((), device="cuda")
+    kw, g = ({"reduction": "mean"}, one) if kind == "one pass" else ({}, wl)
+    least = (n + v) * d * 4 if kind == "one pass" else n * d * 2 if kind == "two passes" else 3 * (n + v) * d * 2
+    loss = ops.linear_cross_entropy(h, w, t, **kw)
+    want = torch.autograd.grad(loss, [h, w], g, retain_graph=True)
+    before = torch.cuda.memory_allocated()
+    got = torch.autograd.grad(loss, [h, w], g)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    del got, a, b
+    assert before - torch.cuda.memory_allocated() >= least
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(loss, [h, w], g)
