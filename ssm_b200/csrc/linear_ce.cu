@@ -4,7 +4,8 @@
 // kernel joins the tiles.  Backward, from w = dloss and wz = dlog_z of a row: G = p (w + wz), q = p_t (w + wz) - w; dh = G' W + q W_t, dW = G'^T h + sum q h at the targets' rows, with
 // G' = G but 0 at the target.  G' is formed again by the same product, a piece of the rows at a time, rounded to the operands' type, and read by the two others:
 // 2 + 6 N D V operations where 6 are the least.  q, as a rule the largest number of its row by far, keeps 32 bits and goes to the results apart (rounded into G it gave
-// most of the gradients' error: 0.31e-3 in fp16 where the result's own rounding is 0.21e-3).
+// most of the gradients' error: 0.31e-3 in fp16 where the result's own rounding is 0.21e-3).  In fp16 a row of G' is taken times a power of two of the row's own weight, which its row of dh is
+// divided by and, where the weights differ, its row of h for dW: with one power for all, rows of 2^-20 of the largest weight lost their softmax part in G'.
 //
 // Loss and gradient in one pass, for sums and means in bf16: what the loss is multiplied by is one number, known later, and 6 N D V do.  The first product leaves
 // 2^(c z - M) in bf16 with M from the target's logit: bf16 reaches as far as fp32, so that any M within 2^60 of the maximum will do, and it needs not be known before.  A row's factor
@@ -43,6 +44,7 @@ __constant__ const signed char kPlaneA[kPairs] = {2, 0, 1, 1, 0, 0}, kPlaneB[kPa
 
 enum Epilogue { kStats = 0, kGrad = 1, kOut = 2, kKeep = 3, kFew = 4 };  // kFew: kStats with the weight's rows as M
 constexpr int kFewRows = 64;           // up to which rows it is taken
+constexpr int kLeastTop = -90;         // tops_kernel: no less, so that 2^(26 - top) is a number
 constexpr float kReach = 60.f;         // how far a row's maximum may be from the M of the one-pass form
 
 // one product: M x N in tiles, K in blocks of 64, cut into `splits`
@@ -68,7 +70,7 @@ struct GemmArgs {
   float2* part;                // [128 columns][rows of this call]: M, sum 2^(c z - M); kKeep: the maximum, the sum; kFew: [row][32 columns]
   int part_ld;
   float* z_target;
-  const float4* row;           // of packed rows: M, 1 / s, w + wz, q; kKeep: M
+  const float4* row;           // of packed rows: M, dh's factor, G's, q; kKeep: M
   uint16_t* g;                 // [plane][row][ldg]
   int64_t ldg, g_plane;
   const int* again;            // kKeep, nullable: the tiles of rows to be formed again
@@ -632,7 +634,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (in) r = g.row[g.row0 + row];
             uint16_t* to = g.g + row * g.ldg + col0;
             const int room = (int)min((int64_t)128, g.ldg - col0);
-            const float f = in ? r.y * r.z : 0.f;
+            const float f = r.z;
             float m = -INFINITY, s = 0.f;
             if (EPI == kKeep && at >= 0 && at < 128) {  // with the sum's own errors, which a loss near zero takes the difference of
               float z = 0.f;
@@ -1052,18 +1054,22 @@ __global__ void __launch_bounds__(1024) join_keep_kernel(const float2* part, int
     log_z[out] = fmaf(v.x, kLn2, ln_s);
   }
 }
-// packed rows times their 1 / sum, zeros behind them to the end of their tile
-__global__ void __launch_bounds__(256) scaled_rows_kernel(const __nv_bfloat16* h, int64_t ld, int dim, const float4* row, const int* count, int64_t row0, int64_t rows,
-                                                          __nv_bfloat16* __restrict__ out) {
+// Packed rows times their factors, zeros behind them to the end of their tile: 1 / sum in the one-pass form.  With `top` the other part of the rows' weights in dW's scale 2^(26 - top):
+// at most 2^14 then, and exact but for elements that lie 2^28 and more below the largest product of an element and its row's weight.
+template <typename T>
+__global__ void __launch_bounds__(256) scaled_rows_kernel(const T* h, int64_t ld, int dim, const float4* row, const int* count, int64_t row0, int64_t rows, T* __restrict__ out,
+                                                          const int* top, float* __restrict__ scales) {
   pdl_wait();
   pdl_trigger();
   const int64_t r = row0 + (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x & 31, n = *count;
+  const float all = top != nullptr ? scalbnf(1.f, 26 - *top) : 1.f;
+  if (top != nullptr && blockIdx.x == 0 && threadIdx.x == 0) scales[0] = all, scales[1] = 1.f / all;
   if (r >= row0 + rows || r >= (n + kTile - 1) / kTile * kTile) return;
   const bool zero = r >= n;
-  const float f = zero ? 0.f : row[r].y;
+  const float f = zero ? 0.f : row[r].y * all;
   for (int c = lane * 8; c < dim; c += 256) {  // rows have room for whole pieces
-    Vec16<__nv_bfloat16> v;
+    Vec16<T> v;
     float e[8];
     v.load(h + r * ld + c);
     v.unpack(e);
@@ -1092,9 +1098,10 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* row_loss, int
   }
 }
 
-// What the backward pass needs of a packed row, and the power of two that brings the largest weight to 2^13 .. 2^14 where the pieces are fp16 (products of small weights would vanish there).
+// What the backward pass needs of a packed row.  Where the pieces are fp16, a power of two brings a row's weight to 2^13 .. 2^14 (products of small weights would vanish there): with
+// `each` the row's own, else that of the largest weight, which all share.
 __global__ void __launch_bounds__(1024) weights_kernel(const float4* stats, const int* idx, const int* count, const float* dloss, int reduction,
-                                                       const float* dlog_z, int has_z, int half, float4* __restrict__ row, float* __restrict__ scales) {
+                                                       const float* dlog_z, int has_z, int half, int each, float4* __restrict__ row, float* __restrict__ scales) {
   pdl_wait();
   pdl_trigger();
   __shared__ float tops[32];
@@ -1111,22 +1118,51 @@ __global__ void __launch_bounds__(1024) weights_kernel(const float4* stats, cons
   __syncthreads();
   for (int w = 0; w < 32; ++w) top = fmaxf(top, tops[w]);
   float scale = 1.f;
-  if (half && top > 1e-30f && top < 1e30f) scale = exp2f((float)(13 - ilogbf(top)));
-  if (tid == 0) scales[0] = scale, scales[1] = 1.f / scale;
+  if (half && !each && top > 1e-30f && top < 1e30f) scale = exp2f((float)(13 - ilogbf(top)));
+  if (tid == 0) scales[0] = scale, scales[1] = 1.f / scale, reinterpret_cast<int*>(scales)[2] = kLeastTop;
   for (int i = tid; i < n; i += 1024) {
     const float w = reduction ? all : dloss[idx[i]], z = has_z ? dlog_z[idx[i]] : 0.f;
     const float4 s = stats[i];
     const float inv = 1.f / s.y, d = fmaf(s.z, kLog2e, -s.x), bad = s.z != s.z ? NAN : 0.f;  // a target outside of the vocabulary, or a NaN
-    row[i] = make_float4(s.x, inv, (w + z) * scale + bad, ex2_approx(d) * inv * (w + z) - w);
+    float mine = scale, back = 1.f / scale;
+    if (each) {
+      const int e = max(-100, min(99, ilogbf(w + z)));  // of zero, and of what is not finite, one of the two ends
+      mine = scalbnf(1.f, 13 - e), back = scalbnf(1.f, e - 13);
+    }
+    row[i] = make_float4(s.x, back, inv * ((w + z) * mine + bad), ex2_approx(d) * inv * (w + z) - w);
+  }
+}
+// With `each`, the largest product of a row's weight (or q, which is more where dloss and dlog_z cancel) and its largest element, as an exponent of two (0 and what is not finite left
+// out): dW's scale.  A warp per packed row.
+__global__ void __launch_bounds__(256) tops_kernel(const __half* h, int64_t ld, int dim, const float4* row, const int* count, int* __restrict__ top) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+  if (r >= *count) return;
+  float m = 0.f;
+  for (int c = lane * 8; c < dim; c += 256) {  // rows have room for whole pieces
+    Vec16<__half> v;
+    float e[8];
+    v.load(h + r * ld + c);
+    v.unpack(e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, c + k < dim && fabsf(e[k]) < INFINITY ? fabsf(e[k]) : 0.f);
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  if (lane == 0 && m > 0.f) {
+    const float4 w = row[r];
+    atomicMax(top, max(13 + ilogbf(w.y), max(-100, min(99, ilogbf(w.w)))) + ilogbf(m));
   }
 }
 
-// dhidden: a packed row's partial sums joined, times its own factor (`by_row`) or all rows', and q W_t, into its place; zeros for rows that are left out (-0 with `by_row`: a factor
+// dhidden: a packed row's partial sums joined, times its factor, and q W_t, into its place; zeros for rows that are left out (-0 with `later`: a factor
 // still to come, infinite or NaN, leaves those as they are).  Rows [row0, row0 + rows) of idx, a
 // warp each.  V columns at a time.
 template <int V>
 __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int splits, int64_t split, int64_t ld, int dim, const int* idx, const int* targets,
-                                                      const int* count, int row0, int rows, const float4* row, int by_row, const float* scales, const void* weight,
+                                                      const int* count, int row0, int rows, const float4* row, int later, const void* weight,
                                                       int64_t weight_stride, int weight_dtype, void* out, int dtype) {
   pdl_wait();
   pdl_trigger();
@@ -1136,7 +1172,7 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int spl
   const int64_t to = (int64_t)idx[r] * dim;
   const int t = in ? max(targets[r], 0) : 0;
   const float4 w = in ? row[r] : make_float4(0.f, 0.f, 0.f, 0.f);
-  const float f = by_row ? w.y : scales[1];
+  const float f = w.y;
   if (in && V == 4) {  // four pieces in flight
     for (int c0 = blockIdx.y * 512 + lane * 4; c0 < dim; c0 += 512 * gridDim.y) {
       float4 x[4];
@@ -1168,7 +1204,7 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* part, int spl
   }
   for (int c = (blockIdx.y * 32 + lane) * V; c < dim; c += 32 * V * gridDim.y) {
     float v[V] = {}, e[V];
-    if (!in && by_row) {
+    if (!in && later) {
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = -0.f;
     }
@@ -1413,13 +1449,14 @@ Plan plan_of(const ssm_linear_ce_args& a, int pass) {
   p.h = take(p.planes * up(p.rows, kTile) * p.ldh * 2);
   p.w = take(p.copy_w ? p.planes * p.vocab * p.ldh * 2 : 0);
   p.kept = at;
-  p.scales = take(8), p.row = take(p.rows * 16);  // row: stats of a forward pass that keeps none
+  p.scales = take(12), p.row = take(p.rows * 16);  // row: stats of a forward pass that keeps none
   if (pass != kBackward) p.part = take((int64_t)p.parts * p.piece * 8), p.z = take(p.rows * 4);
   if (pass != kForward) {
     p.g = take(p.planes * p.piece * p.ldg * 2), p.dh = take((int64_t)p.splits * p.piece * p.ldo * 4), p.keys = take((int64_t)p.sorts * kSort * 8);
     p.heads = take((int64_t)p.sorts * p.vocab * 4), p.sums = take((int64_t)p.sorts * p.sort * p.ldo * 4);
     if (pass == kBackward) p.dw = take(p.piece < p.rows ? p.vocab * p.ldo * 4 : 0);
-    else p.again = take(p.piece / kTile * 4), p.hs = take(up(p.rows, kTile) * p.ldh * 2);
+    else p.again = take(p.piece / kTile * 4);
+    if (pass == kBoth || p.fmt == 0) p.hs = take(up(p.rows, kTile) * p.ldh * 2);
   }
   p.bytes = at - p.kept;
   return p;
@@ -1547,7 +1584,7 @@ struct WeightGrad {
   int dtype;
 };
 // dh = G W and dW += G^T h of a piece, `h2` for h, and dh's way to its rows; each nullable
-int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, bool by_row, void* dh, int dh_dtype, const WeightGrad* dw) {
+int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, bool later, void* dh, int dh_dtype, const WeightGrad* dw) {
   const Plan& p = r.p;
   GemmArgs g{};
   g.bn = p.bn, g.fmt = p.fmt, g.row0 = (int)row0, g.rows = (int)rows, g.count = r.count(), g.status = r.a.status;
@@ -1575,7 +1612,7 @@ int gradients(const Run& r, int64_t row0, int64_t rows, const CUtensorMap& h2, b
   const int64_t blocks = (rows + 7) / 8, shares = (p.dim + (wide ? 511 : 31)) / (wide ? 512 : 32);
   const dim3 grid((unsigned)blocks, (unsigned)std::max<int64_t>(1, std::min(shares, 4 * 148 / blocks)));
   return launch_overlapped("linear_ce dhidden_kernel", kern, grid, 256, 0, r.st,
-                           a.out, a.splits, a.out_split, p.ldo, (int)p.dim, r.idx(), r.packed(), r.count(), (int)row0, (int)rows, r.row(), by_row, r.at<float>(p.scales), r.a.weight,
+                           a.out, a.splits, a.out_split, p.ldo, (int)p.dim, r.idx(), r.packed(), r.count(), (int)row0, (int)rows, r.row(), later, r.a.weight,
                            r.a.weight_stride, r.a.io_dtype, dh, dh_dtype);
 }
 int scaled_copy(const float* src, int64_t ld, int64_t rows, int64_t dim, const int* count, const float* scales, const float* dloss, void* out, int dtype, cudaStream_t st) {
@@ -1663,14 +1700,26 @@ extern "C" int ssm_linear_ce_bwd(const ssm_linear_ce_bwd_args* args, ssm_stream_
   if (a.rows == 0) return args->dweight ? zero(args->dweight, (size_t)a.vocab * a.dim * dtype_size(args->dweight_dtype), r.st) : SSM_OK;
   if (const int rc = prepare(r, false)) return rc;
   float* scales = r.at<float>(p.scales);
+  const bool each = a.io_dtype == SSM_F16 && (a.reduction == 0 || args->dlog_z);  // weights that may differ
   const WeightGrad dw{r.at<float>(p.dw), args->dweight, p.dim, args->dweight_dtype};
   if (const int rc = launch_overlapped("linear_ce weights_kernel", weights_kernel, 1, 1024, 0, r.st,
                                        reinterpret_cast<const float4*>(a.stats), r.idx(), r.count(), args->dloss, a.reduction, args->dlog_z ? args->dlog_z : args->dloss, args->dlog_z != nullptr,
-                                       a.io_dtype == SSM_F16, r.row(), scales)) return rc;
+                                       a.io_dtype == SSM_F16, each, r.row(), scales)) return rc;
+  const __half* h = r.at<__half>(p.h);
+  CUtensorMap mhs = r.mh;
+  int* top = reinterpret_cast<int*>(scales) + 2;
+  if (each && args->dweight) {
+    if (const int rc = launch_overlapped("linear_ce tops_kernel", tops_kernel, (unsigned)((p.rows + 7) / 8), 256, 0, r.st, h, p.ldh, (int)p.dim, r.row(), r.count(), top)) return rc;
+    if (const int rc = encode(&mhs, r.at<void>(p.hs), p.dim, p.rows, 1, p.ldh, up(p.rows, kTile) * p.ldh, p.fmt)) return rc;
+  }
   for (int64_t row0 = 0; row0 < p.rows; row0 += p.piece) {
     const int64_t rows = std::min(p.piece, p.rows - row0);
     if (const int rc = gemm_of<kGrad>(p, r.mh, r.mw, r.mw, logits_args(r, row0, rows), r.st)) return rc;
-    if (const int rc = gradients(r, row0, rows, r.mh, false, args->dhidden, a.io_dtype, args->dweight ? &dw : nullptr)) return rc;
+    if (each && args->dweight) {
+      if (const int rc = launch_overlapped("linear_ce scaled_rows_kernel", scaled_rows_kernel<__half>, (unsigned)((rows + 7) / 8), 256, 0, r.st, h, p.ldh, (int)p.dim, r.row(), r.count(), row0,
+                                           rows, r.at<__half>(p.hs), top, scales)) return rc;
+    }
+    if (const int rc = gradients(r, row0, rows, mhs, false, args->dhidden, a.io_dtype, args->dweight ? &dw : nullptr)) return rc;
   }
   return SSM_OK;
 }
@@ -1706,7 +1755,8 @@ extern "C" int ssm_linear_ce_train(const ssm_linear_ce_args* args, float* dhidde
                                            g.part, g.part_ld, p.parts, g.count, (int)row0, (int)rows, r.idx(), g.z_target, r.row(), again, second, a.row_loss, a.log_z)) return rc;
     }
     if (dweight) {
-      if (const int rc = launch_overlapped("linear_ce scaled_rows_kernel", scaled_rows_kernel, warps, 256, 0, r.st, h, p.ldh, (int)p.dim, r.row(), r.count(), row0, rows, hs)) return rc;
+      if (const int rc = launch_overlapped("linear_ce scaled_rows_kernel", scaled_rows_kernel<__nv_bfloat16>, warps, 256, 0, r.st, h, p.ldh, (int)p.dim, r.row(), r.count(), row0, rows, hs,
+                                           static_cast<const int*>(nullptr), r.at<float>(p.scales))) return rc;
     }
     if (const int rc = gradients(r, row0, rows, mhs, true, dhidden, SSM_F32, dweight ? &dw : nullptr)) return rc;
   }

@@ -899,6 +899,8 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore
     What a call holds for its backward pass goes with the walk that ends the graph: a second one needs ``retain_graph=True`` in the first.
 
     16-bit operands are multiplied as they are; the gradient with respect to the logits is rounded to their type before its two products, but for the targets' own, which keep 32 bits.
+    In fp16 that happens at a power of two of each position's own weight, however far the weights lie apart; for ``weight``'s gradient the hidden states then carry the rest of it, exact but for
+    what lies ``2**28`` below the largest product of a position's weight and hidden state.
     fp32 operands are taken as sums of three bf16 numbers each, products below ``2**-24`` left out."""
     return _run("linear_cross_entropy", hidden, weight, targets, int(ignore_index), str(reduction), bool(return_log_z))
 

@@ -498,3 +498,47 @@ def test_a_walk_gives_back_what_the_call_held(kind):
     assert before - torch.cuda.memory_allocated() >= least
     with pytest.raises(RuntimeError, match="second time"):
         torch.autograd.grad(loss, [h, w], g)
+
+
+@pytest.mark.parametrize("n,v", [(50, 4000), (400, 4000)])
+@pytest.mark.parametrize("by", ["loss", "log_z"])
+def test_weights_of_rows_that_lie_far_apart_in_fp16(by, n, v):
+    """Each row's gradient is as exact as its own weight asks, 2^12 down to 2^-12; dW where light rows alone reach is too.  A row's weight moves nothing but a power of two (`bounds`
+    for weights of 1, times the row's own); for dW it goes to h, whose step is then 2^-25 of 2^13 of the largest product of a weight and a row's largest h at the worst, so
+    2^-37 of that largest product for each row, times p."""
+    h, w, t, _, _ = make(n, 64, v, torch.float16, left_out=0.1)
+    size = torch.exp2((12 - 24 * torch.arange(n, device="cuda") // (n - 1)).float())
+    light = torch.arange(n, device="cuda") >= n // 2  # these rows' distributions lie in the second half of the vocabulary
+    h[:, 0], h[:, 1] = torch.where(light, -4.0, 4.0), torch.where(light, 4.0, -4.0)
+    w[:, :2] = 0
+    w[: v // 2, 0], w[v // 2:, 1] = 5.0, 5.0
+    t = torch.where(t == -100, t, t % (v // 2) + (v // 2) * light)
+    zero, one = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    unit = (one, zero) if by == "loss" else (zero, one)
+    kept = t != -100
+    hl, wl = h.requires_grad_(True), w.requires_grad_(True)
+    dh, dw = torch.autograd.grad(list(ops.linear_cross_entropy(hl, wl, t, return_log_z=True)), [hl, wl], [size * u for u in unit])
+    (val, tol) = bounds(h, w, t, *unit)[2]
+    near(dh, val * size[:, None].double(), tol * size[:, None], "dh")
+    hd, wd, s = h.detach().double() * kept[:, None], w.detach().double(), size.double() * kept
+    z = hd @ wd.t()
+    p = torch.softmax(z, -1) * s[:, None]
+    far = ((64 / 4 + 8) * 2.0 ** -23 * (hd.abs() @ wd.abs().t())).amax(-1)
+    g = p.clone()
+    if by == "loss":
+        g.scatter_add_(1, t.clamp(min=0)[:, None], -s[:, None])
+    e = p * (2 * far + 2.0 ** -18)[:, None] + half(torch.float16) * g.abs() + 2.0 ** -38 * s[:, None]
+    val = g.t() @ hd
+    tol = (e.t() + (n / 4 + 8) * 2.0 ** -23 * g.abs().t()) @ hd.abs() + half(torch.float16) * val.abs()
+    tol = tol + 2.0 ** -37 * float((s * hd.abs().amax(-1)).max()) * (p / s.clamp(min=1e-30)[:, None]).sum(0)[:, None]
+    near(dw, val, tol, "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_that_cancel(dtype):
+    """dloss and dlog_z that add up to nothing, or to little, leave the target's part alone."""
+    h, w, t, wl, _ = make(300, 64, 500, dtype)
+    check(h, w, t, wl, -wl)
+    check(h, w, t, wl, -wl * (1 - 2.0 ** -20))
+    check(h, w, t, wl, torch.where(torch.arange(300, device="cuda") % 2 == 0, -wl, wl))
+    check(h, w, t, 0 * wl, 0 * wl)
