@@ -38,7 +38,7 @@ constexpr int kBoxBytes = 64 * kK * 2, kStageBytes = 4 * kBoxBytes;
 constexpr int kSmem = kStages * kStageBytes + 1024;
 constexpr int kStagePitch = 33, kStaging = kEpilogueWarps * 32 * kStagePitch * 4;  // kOut: a warp's rows on their way to places that are not aligned
 constexpr int kStatus = 128;           // status of a wait that ran out
-constexpr float kFar = 268435456.f;    // 2^28: M of a tile is no less than minus this; rows whose M reaches twice that give NaN (their logits' steps are larger than any difference that matters)
+constexpr float kFar = 536870912.f;    // 2^29: rows whose M reaches this, either way, give NaN (their logits' steps are larger than any difference that matters); M of a tile is no less than minus this
 constexpr int kPairs = 6;
 __constant__ const signed char kPlaneA[kPairs] = {2, 0, 1, 1, 0, 0}, kPlaneB[kPairs] = {0, 2, 1, 0, 1, 0};
 
@@ -903,7 +903,7 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const int64_t* targets, 
   }
 }
 
-__device__ __forceinline__ float within_reach(float M) { return fabsf(M) < 2.f * kFar ? 0.f : NAN; }
+__device__ __forceinline__ float within_reach(float M) { return fabsf(M) < kFar ? 0.f : NAN; }
 
 // The tiles of a row joined: 32 rows of a call to a block, 32 slices of the columns (7 rows, 394 tiles: 21 us with eight slices).
 __global__ void __launch_bounds__(1024) join_kernel(const float2* part, int ld, int parts, const int* count, int row0, int rows, const int* idx,

@@ -892,7 +892,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore
     have their types; ``weight`` is read in ``hidden``'s type.
 
     A position whose target is ``ignore_index`` gives 0 (``log_z`` too) and no gradient, is not computed, and may hold anything.  Any other target outside of the vocabulary
-    makes its loss and the gradients NaN, as a hidden state that is not finite does, and logits of ``2**28`` and more.
+    makes its loss and the gradients NaN, as a hidden state that is not finite does, and a largest logit of ``2**29 ln 2`` (3.7e8) and more, or as far below zero.
 
     Neither pass holds the logits; in 16 bits at most 512 MB of their gradient (and 16384 rows) at a time.  For a sum or mean in bf16 without ``return_log_z`` the gradients are formed along with the
     loss, and held in fp32 until the backward pass scales them (``torch.no_grad()`` forms the loss alone); otherwise the backward pass forms the logits again.

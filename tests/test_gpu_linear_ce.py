@@ -542,3 +542,28 @@ def test_weights_that_cancel(dtype):
     check(h, w, t, wl, -wl * (1 - 2.0 ** -20))
     check(h, w, t, wl, torch.where(torch.arange(300, device="cuda") % 2 == 0, -wl, wl))
     check(h, w, t, 0 * wl, 0 * wl)
+
+
+@pytest.mark.parametrize("n", [20, 100])
+@pytest.mark.parametrize("v", [1, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_whose_logits_are_all_far_below_zero(dtype, v, n):
+    """As in `test_very_large_logits`: logits of one sign, around -1e8 to -3.6e8, within 2^29 ln 2 = 3.72e8; beyond it NaN, not an infinite loss."""
+    h, w, t, _, _ = make(n, 64, v, dtype, left_out=0.0)
+    h = (1 + 0.2 * h.float().abs().clamp(max=2.0)) / 64
+    w = -(1 + 0.2 * w.float().abs().clamp(max=2.0))
+    for size, reach in ((1e8, True), (1.85e8, True), (4e8, False)):
+        hl, wl = (size * h).to(dtype).requires_grad_(True), w.to(dtype).requires_grad_(True)
+        z = hl.detach().double() @ wl.detach().double().t()
+        assert z.amax() * 1.4427 > -2.0 ** 29 if reach else z.amax() < -3.8e8
+        want = torch.logsumexp(z, -1) - torch.gather(z, 1, t[:, None])[:, 0]
+        tol = 2.0 ** -18 * z.abs().amax(-1)
+        loss, log_z = ops.linear_cross_entropy(hl, wl, t, return_log_z=True)
+        total = ops.linear_cross_entropy(hl, wl, t, reduction="sum")
+        for out, g in ((loss, torch.ones(n, device="cuda")), (total, torch.ones((), device="cuda"))):
+            assert all(x.isfinite().all() if reach else x.isnan().all() for x in (out, *torch.autograd.grad(out, [hl, wl], g)))
+        if reach:
+            assert ((loss.detach().double() - want).abs() <= tol).all() and ((log_z.detach().double() - torch.logsumexp(z, -1)).abs() <= tol).all()
+            assert (total.detach().double() - want.sum()).abs() <= tol.sum()
+        else:
+            assert log_z.isnan().all()
