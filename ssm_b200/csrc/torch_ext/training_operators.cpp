@@ -241,7 +241,35 @@ py::object linear_cross_entropy(const Tensor& hidden, const Tensor& weight, cons
 // ---------------------------------------------------------------------------------------------
 // the norm over many tensors, and clipping by it
 // ---------------------------------------------------------------------------------------------
+// Whether two tensors whose spans overlap share no byte all the same, as columns of one matrix do.  Modulo a stride S of either, axes whose strides are multiples of S move nothing, and the
+// others cover a run of bytes: runs that do not meet on the circle of S are proof.
+bool lie_apart(const Tensor& a, const Tensor& b) {
+  const auto run = [](const Tensor& t, int64_t period) {
+    int64_t bytes = t.element_size();
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      const int64_t stride = t.stride(i) * t.element_size();
+      if (stride % period != 0) bytes += (t.size(i) - 1) * stride;
+    }
+    return bytes;
+  };
+  for (const Tensor* t : {&a, &b}) {
+    for (int64_t i = 0; i < t->dim(); ++i) {
+      if (t->size(i) <= 1) continue;
+      const int64_t period = t->stride(i) * t->element_size(), runs[2] = {run(a, period), run(b, period)};
+      const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(a.data_ptr()) % period), to = (int64_t)(reinterpret_cast<uintptr_t>(b.data_ptr()) % period);
+      const int64_t ahead = (to - at + period) % period;  // from a's run to b's
+      if (ahead >= runs[0] && period - ahead >= runs[1]) return true;
+    }
+  }
+  return false;
+}
+
 struct TensorList {
+  struct Span {
+    uintptr_t from, to;
+    size_t index;
+    bool operator<(const Span& o) const { return from < o.from; }
+  };
   std::vector<ssm_tensor_ref> refs;
   std::vector<Tensor> held;                        // dense copies
   std::vector<std::pair<Tensor, Tensor>> strided;  // (given, copy) of those that do not fill their memory
@@ -254,7 +282,7 @@ struct TensorList {
       if (!THPVariable_Check(PyList_GET_ITEM(tensors.ptr(), i))) throw py::type_error(std::string(what) + " takes tensors");
     device = count == 0 ? c10::Device(c10::kCUDA, at::cuda::current_device()) : THPVariable_Unpack(PyList_GET_ITEM(tensors.ptr(), 0)).device();
     const bool recorded = at::GradMode::is_enabled();
-    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    std::vector<Span> spans;
     refs.reserve(count);
     if (in_place) spans.reserve(count);
     for (size_t k = 0; k < count; ++k) {
@@ -279,7 +307,7 @@ struct TensorList {
             reach += (t.size(i) - 1) * t.stride(i);
           }
         }
-        spans.emplace_back(at, at + (uintptr_t)(reach + 1) * t.element_size());
+        spans.push_back(Span{at, at + (uintptr_t)(reach + 1) * t.element_size(), k});
       }
       if (dense) {
         refs.push_back(ssm_tensor_ref{reinterpret_cast<const void*>(at), n, type, 0});
@@ -291,7 +319,14 @@ struct TensorList {
       }
     }
     if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); ++i) SSM_ARG(spans[i].first >= spans[i - 1].second, what, ": two of the tensors share memory (one given twice would be scaled twice).");
+    std::vector<Span> open;  // those that reach beyond where the next one begins
+    for (const Span& s : spans) {
+      open.erase(std::remove_if(open.begin(), open.end(), [&](const Span& o) { return o.to <= s.from; }), open.end());
+      for (const Span& o : open)
+        SSM_ARG(lie_apart(THPVariable_Unpack(PyList_GET_ITEM(tensors.ptr(), o.index)), THPVariable_Unpack(PyList_GET_ITEM(tensors.ptr(), s.index))), what,
+                ": two of the tensors share memory (one given twice would be scaled twice), or lie between one another in a way that is not told from it.");
+      open.push_back(s);
+    }
   }
 };
 int max_of(double norm_type) {

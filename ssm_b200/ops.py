@@ -920,8 +920,9 @@ def global_norm(tensors, norm_type: float = 2.0) -> Tensor:
 
 def clip_global_norm_(tensors, max_norm: float, norm_type: float = 2.0) -> Tensor:
     """Extension: multiplies all tensors in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being :func:`global_norm` of them, which is
-    returned (its value before).  No synchronisation; where nothing is to be clipped, nothing is written.  A norm of infinity leaves 0 (NaN in place of
-    infinities), a NaN makes all NaN; ``max_norm=inf`` clips nothing.  Tensors that share memory, and broadcast ones, are refused."""
+    returned (its value before).  No synchronisation; where nothing is to be clipped, nothing is written (tensors with gaps excepted: those are copied, and written back as they were).  A
+    norm of infinity leaves 0 (NaN in place of infinities), a NaN makes all NaN; ``max_norm=inf`` clips nothing.  Tensors that share memory, and broadcast ones, are refused; columns of one
+    matrix and other views that lie between one another are taken."""
     return _native().clip_global_norm_(_tensor_list(tensors, "clip_global_norm_"), float(max_norm), float(norm_type))
 
 

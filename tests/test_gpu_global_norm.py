@@ -173,3 +173,28 @@ def test_repeats_streams_and_graphs_give_the_same_bits():
     fresh[0].mul_(100)
     graph.replay()
     same(held, oracle.global_norm([t.cpu() for t in fresh]))
+
+
+def test_views_of_one_buffer_that_lie_between_one_another():
+    """Columns of one matrix, every second element, planes of the last axis: their spans overlap, their elements do not."""
+    def pieces(kind):
+        m = rn(64, 40, seed=3)
+        return m, {"columns": [m[:, :13], m[:, 13:20], m[:, 20:]], "every second": [m[:, 1::2], m[:, ::2]], "rows and columns": [m[:32, :8], m[32:], m[:32, 8:]],
+                   "planes": [m.view(64, 8, 5)[..., i] for i in range(5)], "blocks": [m.view(16, 4, 40)[:, :1, :7], m.view(16, 4, 40)[:, 1:, :7], m[:, 7:]],
+                   "turned": [m.t()[:13], m.t()[13:]], "one column": [m[:, 0], m[:, 1:]]}[kind]
+
+    for kind in ("columns", "every second", "rows and columns", "planes", "blocks", "turned", "one column"):
+        m, parts = pieces(kind)
+        kept = m.clone()
+        clip(parts, 1.0)
+        c = min(1.0, 1.0 / (float(torch.cat([p.reshape(-1) for p in pieces(kind)[1]]).double().norm()) + 1e-6))
+        assert torch.allclose(m, kept * c, rtol=2e-6, atol=0), kind
+
+
+def test_views_of_one_buffer_that_share_elements_are_refused():
+    m = rn(64, 40, seed=3)
+    kept = m.clone()
+    for bad in ([m[:, :20], m[:, 19:]], [m[:, ::2], m[:, ::4]], [m[:, 3:], m[5]], [m[5], m[9, 2:7], m[:, 3:]], [m.t()[:5], m[:, 4:]], [m[:, 0], m[:, 5], m[40:, :6]], [m[::2], m[2::4]]):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.clip_global_norm_(bad, 1.0)
+    assert torch.equal(m, kept)
