@@ -204,3 +204,10 @@ def test_second_derivatives_are_refused():
     g = torch.autograd.grad(call(ops, {**t, "x": x})[0].sum(), x, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="differentiable once"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("d", [97, 1001, 4101])
+@pytest.mark.parametrize("nb,nl", [(5, 421), (700, 3), (1, 1500)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_odd_widths_with_a_gate_per_sequence_whose_rows_several_blocks_share(dtype, nb, nl, d):
+    check(make(nb, nl, d, dtype, "sequence", True), is_rms=False)

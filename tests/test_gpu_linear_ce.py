@@ -567,3 +567,23 @@ def test_rows_whose_logits_are_all_far_below_zero(dtype, v, n):
             assert (total.detach().double() - want.sum()).abs() <= tol.sum()
         else:
             assert log_z.isnan().all()
+
+
+@pytest.mark.parametrize("v", [2 ** 19 - 1, 2 ** 19, 2 ** 19 + 1])
+def test_vocabularies_around_2_to_the_19(v):
+    """From 2^19 on a target and its row's place take 64 bits where the targets are sorted."""
+    h, w, t, wl, wz = make(70, 8, v, torch.bfloat16)
+    t[0], t[1], t[2], t[3:9], t[68] = v - 1, v - 2, 0, v // 2, v - 1
+    check(h, w, t, wl, wz)
+    one_pass(h, w, t)
+
+
+@pytest.mark.parametrize("wt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("n,d,v", [(20, 96, 1001), (500, 64, 700), (300, 33, 400)])
+def test_one_pass_with_a_weight_of_another_type(n, d, v, wt):
+    """A model's fp32 (or fp16) weight beside bf16 hidden states: read in bf16, its gradient leaves in its own type."""
+    h, w, t, _, _ = make(n, d, v, torch.bfloat16)
+    w = torch.where(w.abs() < 2.0 ** -10, torch.zeros_like(w), w).to(wt)  # numbers that both types hold
+    for reduction in ("mean", "sum"):
+        dh, dw = one_pass(h, w, t, reduction)
+        assert dh.dtype == torch.bfloat16 and dw.dtype == wt
