@@ -245,8 +245,9 @@ int ssm_block_norm_bwd(const ssm_block_norm_bwd_args* args, ssm_stream_t stream)
  * stats (rows, 4) fp32, 16-byte aligned, keeps what the backward pass needs (nullable).  status: a word in host memory that the device writes, set where a bounded wait ran out.
  *
  * Backward: from dloss (rows, or one float with a reduction) and dlog_z (rows, nullable) writes dhidden (rows, dim; io_dtype) and dweight (vocab, dim; dweight_dtype),
- * dense, each nullable, via pieces of at most SSM_LINEAR_CE_PIECE_BYTES of the logits' gradient in 16 bits.
- * packs, 256-byte aligned, ssm_linear_ce_packs_bytes(args) bytes: the rows that count (and, in fp32, the weight) as the products read them, written by the forward pass and read by
+ * dense, each nullable, via pieces of the logits' gradient in 16 bits (three times 16 for fp32): at most SSM_LINEAR_CE_PIECE_BYTES and 16384 rows, or 256 rows where those are larger.
+ * packs, 256-byte aligned, ssm_linear_ce_packs_bytes(args) bytes (which go by weight and weight_stride too: a weight that cannot be copied from its place is packed, so both are set before it
+ * is asked): the rows that count (and, in fp32, the weight) as the products read them, written by the forward pass and read by
  * the backward pass.  scratch: ssm_linear_ce_scratch_bytes(args, pass) bytes, 256-byte aligned; pass 0 forward, 1 backward, 2 both at once.
  *
  * ssm_linear_ce_train, for bf16 with a reduction: the forward pass and, for a dloss that is known later, dhidden (rows, dim) and dweight (vocab, dim rounded up to a multiple of

@@ -9,20 +9,23 @@
 //
 // Loss and gradient in one pass, for sums and means in bf16: what the loss is multiplied by is one number, known later, and 6 N D V do.  The first product leaves
 // 2^(c z - M) in bf16 with M from the target's logit: bf16 reaches as far as fp32, so that any M within 2^60 of the maximum will do, and it needs not be known before.  A row's factor
-// 1 / sum goes to h for dW, and to the result for dh.  Rows whose maximum is further away are noticed when their tiles are joined, and their tiles formed again.
+// 1 / sum goes to h for dW (rounded to bf16 there once more: rows of dW without a target are off by 2.8e-3, 2.3e-3 in two passes, the rounding of the result being 1.65e-3), and to the result
+// for dh.  Rows whose maximum is further away are noticed when their tiles are joined, and their tiles formed again.
 //
 // Bound: the tensor cores; for few rows, reading W.
 //
 // Rows that are left out are not computed: the others are packed first, behind one another (which also gives the copies their alignment), and how many
 // there are is known on the device alone, so that every kernel reads it there.
 //
-// Launches overlap: each kernel waits for the one before ahead of its first access (7 rows: 37 -> 29 us then, 500 fp32 rows with gradients 257 -> 241), and what it reads is
-// not marked as constant, so that no read moves ahead of the wait.
+// Launches overlap: each kernel waits for the one before ahead of its first access (7 rows: 37 -> 29 us then, 500 fp32 rows with gradients 257 -> 241), and what kernels of a call write for one
+// another is not marked as constant, so that no read of it moves ahead of the wait.  Operands and packed rows are read as constants where the address, or a branch around the read, depends on a
+// load behind the wait (a row's place or target, how many rows count).
 //
 // Products: pairs of CTAs (cta_group::2) on tiles of 256 x 256 (x 128 for narrow outputs), a CTA holding 128 rows of the accumulator; operands by TMA in the 128-byte swizzle, blocks of 64 x 64, two to
 // an operand, with K innermost (h, W, G as stored) or M / N innermost (G^T, W and h as the second factor).  One thread copies, one multiplies, eight
-// warps read an accumulator while the next one is formed.  Logits, and all results in fp32, leave the accumulator every 512 terms and are added up by the warps that read it: the tensor core
-// cuts its sums off (4096 rows of 2560: the losses were off by 1.0e-6, 2.4e-7 so).  fp32 operands are taken as sums of three bf16 numbers (24 bits of mantissa in all) and
+// warps read an accumulator while the next one is formed.  Logits, and products of fp32 operands, leave the accumulator every 512 terms and are added up by the warps that read it: the tensor core
+// cuts its sums off (4096 rows of 2560: the losses were off by 1.0e-6, 2.4e-7 so).  Gradients of 16-bit operands, also those that leave in fp32, are the tensor core's own sums: their terms were
+// rounded to 2^-9 or 2^-12 before, and so are the logits that two passes form again for them.  fp32 operands are taken as sums of three bf16 numbers (24 bits of mantissa in all) and
 // multiplied in six products, the smallest first; what is left out is below 2^-24.
 #include <algorithm>
 #include <cmath>
@@ -43,7 +46,9 @@ constexpr int kPairs = 6;
 __constant__ const signed char kPlaneA[kPairs] = {2, 0, 1, 1, 0, 0}, kPlaneB[kPairs] = {0, 2, 1, 0, 1, 0};
 
 enum Epilogue { kStats = 0, kGrad = 1, kOut = 2, kKeep = 3, kFew = 4 };  // kFew: kStats with the weight's rows as M
-constexpr int kFewRows = 64;           // up to which rows it is taken
+// Up to which rows it is taken; a tile has no room for more.  Both sides, 7 / 32 / 64 rows: 50277 x 768 bf16 19 / 20 / 22 us against 33 / 33 / 34, 50280 x 2560 57 / 58 / 66 against 78 / 65 / 67,
+// 16003 x 512 fp32 35 / 36 / 44 against 40 / 40 / 40 (launches replayed in a graph).
+constexpr int kFewRows = 64;
 constexpr int kLeastTop = -90;         // tops_kernel: no less, so that 2^(26 - top) is a number
 constexpr float kReach = 60.f;         // how far a row's maximum may be from the M of the one-pass form
 

@@ -894,11 +894,13 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore
     A position whose target is ``ignore_index`` gives 0 (``log_z`` too) and no gradient, is not computed, and may hold anything.  Any other target outside of the vocabulary
     makes its loss and the gradients NaN, as a hidden state that is not finite does, and a largest logit of ``2**29 ln 2`` (3.7e8) and more, or as far below zero.
 
-    Neither pass holds the logits; in 16 bits at most 512 MB of their gradient (and 16384 rows) at a time.  For a sum or mean in bf16 without ``return_log_z`` the gradients are formed along with the
+    Neither pass holds the logits; of their gradient, in 16 bits (fp32: three times 16), at most 512 MB and 16384 rows at a time, or 256 rows where those are more than 512 MB.  For a sum or mean in bf16 without ``return_log_z`` the gradients are formed along with the
     loss, and held in fp32 until the backward pass scales them (``torch.no_grad()`` forms the loss alone); otherwise the backward pass forms the logits again.
     What a call holds for its backward pass goes with the walk that ends the graph: a second one needs ``retain_graph=True`` in the first.
 
     16-bit operands are multiplied as they are; the gradient with respect to the logits is rounded to their type before its two products, but for the targets' own, which keep 32 bits.
+    Formed along with the loss, it is rounded before it is divided by a position's sum, and for ``weight``'s gradient the hidden state over that sum is rounded to bf16 too: rows of tokens that
+    are no target are off by 2.8e-3 then (relative norm), by 2.3e-3 in the other form, where their own rounding to bf16 is 1.65e-3; over all rows, 1.7e-3.
     In fp16 that happens at a power of two of each position's own weight, however far the weights lie apart; for ``weight``'s gradient the hidden states then carry the rest of it, exact but for
     what lies ``2**28`` below the largest product of a position's weight and hidden state.
     fp32 operands are taken as sums of three bf16 numbers each, products below ``2**-24`` left out."""
