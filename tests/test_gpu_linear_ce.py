@@ -587,3 +587,30 @@ def test_one_pass_with_a_weight_of_another_type(n, d, v, wt):
     for reduction in ("mean", "sum"):
         dh, dw = one_pass(h, w, t, reduction)
         assert dh.dtype == torch.bfloat16 and dw.dtype == wt
+
+
+def test_fp16_weights_of_rows_in_a_graph():
+    """The rows' powers of two and dW's scale are found on the device: a replay goes by the weights of that moment, and two runs give the same bits."""
+    h, w, t, wl, wz = make(700, 96, 1500, torch.float16)
+    h, w, wl = h.requires_grad_(True), w.requires_grad_(True), wl * torch.exp2(-(torch.arange(700, device="cuda") % 20).float())
+
+    def once():
+        loss, log_z = ops.linear_cross_entropy(h, w, t, return_log_z=True)
+        return torch.autograd.grad([loss, log_z], [h, w], [wl, wz])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for factor in (1.0, 2.0 ** -9, 3000.0):
+        wl.mul_(factor), wz.mul_(factor)
+        graph.replay()
+        got = [o.clone() for o in out]
+        for a, b in zip(got, once()):
+            assert torch.equal(a, b)
+        for a, (val, tol) in zip(got, bounds(h, w, t, wl, wz)[2:]):
+            near(a, val, tol, "gradient")
