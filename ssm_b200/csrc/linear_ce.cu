@@ -1138,7 +1138,7 @@ __global__ void __launch_bounds__(1024) weights_kernel(const float4* stats, cons
   }
 }
 // With `each`, the largest product of a row's weight (or q, which is more where dloss and dlog_z cancel) and its largest element, as an exponent of two (0 and what is not finite left
-// out): dW's scale.  A warp per packed row.
+// out): dW's scale.  A warp per packed row, bound by its start (1999 rows of 1024: 5 us, as scaled_rows_kernel behind it).
 __global__ void __launch_bounds__(256) tops_kernel(const __half* h, int64_t ld, int dim, const float4* row, const int* count, int* __restrict__ top) {
   pdl_wait();
   pdl_trigger();
